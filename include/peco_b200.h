@@ -237,6 +237,95 @@ int peco_exchange_put(const void* src, const long long* src_offsets, const int* 
                       int rank, int world, long long epoch, unsigned* done_counter, void* stream);
 int peco_exchange_wait(const long long* flags, int world, int flag_slot, long long epoch, void* stream);
 
+/* ---- transformer-block operators (no counterpart in the reference, whose
+ * blocks are the host framework's) ------------------------------------------ */
+
+/* out = residual + gate * act([x | x2] W^T + bias) over samples *
+ * rows_per_sample rows.  x [rows, k], x2 [rows, k2] (k2 = 0: absent), weight
+ * [n, k + k2], residual and out [rows, n]: rows ``*_stride`` elements apart,
+ * columns adjacent.  bias [n]; gate [samples, n] rows gate_stride apart (0:
+ * one for all); either and residual may be null.  preact, if given, [rows, n]
+ * contiguous, receives the pre-activation.  activation 0 none, 1 gelu (tanh
+ * form), 2 gelu (erf), 3 silu; dtype 0 fp16, 1 bf16.  Sums are fp32, each
+ * output is rounded once.  out may be residual.  Operands whose base or row
+ * stride is not a multiple of 16 bytes are copied into ``workspace`` first:
+ * peco_linear_forward_workspace says how many bytes (0 when all are aligned;
+ * -1: sizes out of range). */
+int peco_linear_forward(const void* x, long long x_stride, const void* x2, long long x2_stride, const void* weight,
+                        long long w_stride, const void* bias, const void* gate, long long gate_stride,
+                        const void* residual, long long res_stride, void* out, long long out_stride, void* preact,
+                        int samples, int rows_per_sample, int k, int k2, int n, int activation, int dtype,
+                        void* workspace, long long workspace_bytes, void* stream);
+long long peco_linear_forward_workspace(const void* x, long long x_stride, const void* x2, long long x2_stride,
+                                        const void* weight, long long w_stride, int samples, int rows_per_sample,
+                                        int k, int k2, int n);
+
+/* Gradients of peco_linear_forward for ``grad`` = d out (the residual's
+ * gradient is ``grad`` itself).  preact [rows, n] is needed when the
+ * activation is not 0 or dgate is asked for.  dx [rows, k], dx2 [rows, k2],
+ * dweight [n, k + k2], dbias [n], dgate [samples, n], contiguous; null: not
+ * computed.  grad * gate * act' is rounded to the operands' type for the two
+ * products; the sums for dbias and dgate are of the unrounded values and do
+ * not depend on the launch order.  Needs at least one row. */
+int peco_linear_backward(const void* grad, long long grad_stride, const void* preact, const void* x,
+                         long long x_stride, const void* x2, long long x2_stride, const void* weight,
+                         long long w_stride, const void* gate, long long gate_stride, void* dx, void* dx2,
+                         void* dweight, void* dbias, void* dgate, int samples, int rows_per_sample, int k, int k2,
+                         int n, int activation, int dtype, void* workspace, long long workspace_bytes, void* stream);
+long long peco_linear_backward_workspace(const void* grad, long long grad_stride, const void* x, long long x_stride,
+                                         const void* x2, long long x2_stride, const void* weight, long long w_stride,
+                                         int samples, int rows_per_sample, int k, int k2, int n, int activation,
+                                         int has_gate);
+
+/* Gated residual and norm: with b = post_norm(branch) * post_weight,
+ *   residual = residual_scale * x + gate * b
+ *   normed = norm(residual) * weight * (1 + scale) + shift
+ * for x and branch [samples, rows, width] (strides in elements, columns
+ * adjacent) and the sample's vectors gate / scale / shift [samples, width]
+ * (``*_batch`` elements apart, 0: shared).  norm 1 layer (mean and variance),
+ * 2 rms; post_norm 0 none, 1, 2.  Everything but x and normed may be null;
+ * gate, post_norm and residual need a branch.  residual and normed are
+ * contiguous and each rounded once.  width <= 16384; dtype 0 fp16, 1 bf16. */
+int peco_gated_norm(const void* x, long long x_batch, long long x_row, const void* branch, long long branch_batch,
+                    long long branch_row, const void* gate, long long gate_batch, const void* scale,
+                    long long scale_batch, const void* shift, long long shift_batch, const void* weight,
+                    const void* post_weight, void* residual, void* normed, int samples, int rows, int width, int norm,
+                    int post_norm, float eps, float post_eps, float residual_scale, int dtype, void* stream);
+
+/* Gradients of peco_gated_norm for grad_normed and grad_residual (null: 0).
+ * dx, dbranch [samples, rows, width] and the vector gradients, any of them
+ * null; a vector's gradient is [samples, width], or summed over the samples
+ * to [width] when its bit of ``shared`` is set (1 gate, 2 scale, 4 shift).
+ * The workspace is needed for vector gradients only; their sums run in a
+ * fixed order.  Needs at least one row. */
+int peco_gated_norm_backward(const void* grad_normed, long long gh_batch, long long gh_row, const void* grad_residual,
+                             long long gr_batch, long long gr_row, const void* x, long long x_batch, long long x_row,
+                             const void* branch, long long branch_batch, long long branch_row, const void* gate,
+                             long long gate_batch, const void* scale, long long scale_batch, const void* weight,
+                             const void* post_weight, void* dx, void* dbranch, void* dgate, void* dscale, void* dshift,
+                             int shared, void* dweight, void* dpost_weight, int samples, int rows, int width, int norm,
+                             int post_norm, float eps, float post_eps, float residual_scale, int dtype,
+                             void* workspace, long long workspace_bytes, void* stream);
+long long peco_gated_norm_backward_workspace(int samples, int rows, int width);
+
+/* Rotary embedding by positions on several axes, of q [batch, q_heads, rows,
+ * dims] and k (k_heads may be 0) in one launch.  ``*_strides`` (host memory):
+ * batch, head and token strides of the source, then of the destination, in
+ * elements; dims are adjacent.  A destination may be its source.  axes (host):
+ * dimensions of each of the n_axes <= 4 sections; pair j of axis a turns by
+ * position[a] * theta^(-2 j / axes[a]).  Rows [0, rotated_rows) turn, later
+ * rows and dimensions past the sections are copied.  Positions: grid (host, a
+ * row-major token grid whose product is rotated_rows), or ``positions``
+ * [batch, rotated_rows, n_axes] on the device (pos_type 0 int32, 1 int64, 2
+ * fp32; strides in elements).  interleaved: pairs (2i, 2i+1), else one from
+ * each half of the rotated dimensions.  inverse: the opposite turn.  dtype 0
+ * fp16, 1 bf16, 2 fp32; dims even, at most 256. */
+int peco_rotary(const void* q, void* q_out, int q_heads, const long long* q_strides, const void* k, void* k_out,
+                int k_heads, const long long* k_strides, int batch, int rows, int rotated_rows, int dims,
+                const int* axes, int n_axes, double theta, const int* grid, const void* positions,
+                long long pos_batch_stride, long long pos_row_stride, int pos_type, int interleaved, int inverse,
+                int dtype, void* stream);
+
 /* ---- diagnostics --------------------------------------------------------- */
 
 /* Copies the device status word of the current device to *out (synchronising

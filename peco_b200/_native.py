@@ -21,6 +21,7 @@ P = ctypes.c_void_p
 I = ctypes.c_int
 LL = ctypes.c_longlong
 F = ctypes.c_float
+D = ctypes.c_double
 
 _SIGNATURES = {
     "peco_assign_tokens_to_centers": [P] * 5 + [I] * 5 + [P],
@@ -41,6 +42,15 @@ _SIGNATURES = {
     "peco_prepare_qkv": [P, P, P, LL, I, P, P, P, LL, I, P, P, F, P, P, F, P, P, P, P, P, I, I, P],
     "peco_exchange_put": [P, P, P, P, LL, I, P, P, I, I, I, LL, P, P],
     "peco_exchange_wait": [P, I, I, LL, P],
+    "peco_linear_forward": [P, LL] * 3 + [P, P, LL, P, LL, P, LL, P] + [I] * 7 + [P, LL, P],
+    "peco_linear_forward_workspace": [P, LL] * 3 + [I] * 5,
+    "peco_linear_backward": [P, LL, P] + [P, LL] * 4 + [P] * 5 + [I] * 7 + [P, LL, P],
+    "peco_linear_backward_workspace": [P, LL] * 4 + [I] * 7,
+    "peco_gated_norm": [P, LL, LL] * 2 + [P, LL] * 3 + [P] * 4 + [I] * 5 + [F] * 3 + [I, P],
+    "peco_gated_norm_backward": [P, LL, LL] * 4 + [P, LL] * 2 + [P] * 7 + [I] + [P] * 2 + [I] * 5 + [F] * 3
+    + [I, P, LL, P],
+    "peco_gated_norm_backward_workspace": [I, I, I],
+    "peco_rotary": [P, P, I, P] * 2 + [I] * 4 + [P, I, D, P, P, LL, LL, I, I, I, I, P],
     "peco_attention_workspace_stride": [I, I, I, I],
     "peco_key_block_rows": [I, I],
     "peco_kmeans_work_floats": [I, I, I],
@@ -53,6 +63,9 @@ _SIGNATURES = {
 }
 _RESTYPES = {
     "peco_launch_count": ctypes.c_ulonglong,
+    "peco_linear_forward_workspace": LL,
+    "peco_linear_backward_workspace": LL,
+    "peco_gated_norm_backward_workspace": LL,
     "peco_attention_workspace_stride": LL,
     "peco_key_block_rows": LL,
     "peco_kmeans_work_floats": LL,

@@ -1,0 +1,702 @@
+// Linear layers of a transformer block with their epilogue, and their gradient.
+//
+//   out[m, n] = residual[m, n] + gate[sample(m), n] * act(sum_k x[m, k] W[n, k] + bias[n])
+//
+// x may be given as two inputs side by side (the attention rows and the MLP
+// hidden of a single-stream block), which replaces their concatenation.
+// Gradient, with z the pre-activation and g the gradient of out:
+//   dz = g * gate * act'(z);  dx = dz W;  dW = dz^T x;  dbias = sum_m dz;
+//   dgate[b, n] = sum over the sample's rows of g * act(z).
+//
+// All three products run through one tcgen05 kernel, D[M, N] = sum_k A[m, k]
+// B[n, k], whose operands are read in place by TMA whichever of their two
+// dimensions is contiguous (K-major, or MN-major for W in dx and for both
+// operands of dW).  Operands that TMA cannot address (a base or row stride
+// that is not a multiple of 16 bytes) are first copied to rows that it can.
+#include "common.cuh"
+#include "../../include/peco_b200.h"
+#include "internal.h"
+#include "rows.cuh"
+
+#include <type_traits>
+
+namespace peco {
+namespace {
+
+enum Activation : int { kActNone = 0, kActGeluTanh = 1, kActGelu = 2, kActSilu = 3 };
+
+constexpr int kTileM = 128;
+constexpr int kTileK = 64;   // one 128-byte swizzle panel of 16-bit elements
+constexpr int kGemmThreads = 192;  // TMA warp, MMA warp, four epilogue warps
+
+struct GemmArgs {
+  CUtensorMap a[2], b[2];    // K segments (x and x2; the second unused otherwise)
+  int kblocks[2];            // 64-wide K blocks of each segment
+  int m, n, tiles_m, tiles_n;
+  void* out;
+  long long out_stride;
+  // epilogue operands (null where absent)
+  const void* bias;          // [n]
+  const void* gate;          // [samples, n], rows gate_stride apart
+  long long gate_stride;
+  int rows_per_sample;
+  const void* residual;
+  long long res_stride;
+  void* preact;              // [m, n] rounded copy of the pre-activation
+  int act;
+  int vec;                   // every row of every [m, n] operand starts on 16 bytes and n % 8 == 0
+  unsigned* status;
+};
+
+// ---- activations -------------------------------------------------------------
+// Evaluated in fp32.  gelu_tanh is written as z * sigmoid(2u): the exponential
+// keeps full relative precision in the negative tail, where 1 + tanh(u) would
+// cancel.
+__device__ __forceinline__ float sigmoidf_(float x) { return __fdividef(1.0f, 1.0f + exp2_approx(-1.4426950408889634f * x)); }
+
+constexpr float kGeluC = 0.7978845608028654f;  // sqrt(2 / pi)
+
+__device__ __forceinline__ float activate(float z, int act) {
+  switch (act) {
+    case kActGeluTanh: return z * sigmoidf_(2.0f * kGeluC * fmaf(0.044715f * z * z, z, z));
+    case kActGelu: return 0.5f * z * (1.0f + erff(z * 0.7071067811865476f));
+    case kActSilu: return z * sigmoidf_(z);
+    default: return z;
+  }
+}
+
+// (act(z), act'(z))
+__device__ __forceinline__ float2 activate_slope(float z, int act) {
+  switch (act) {
+    case kActGeluTanh: {
+      const float s = sigmoidf_(2.0f * kGeluC * fmaf(0.044715f * z * z, z, z));
+      // d/dz [z s(2u)] = s + z s (1 - s) 2 u'
+      return make_float2(z * s, fmaf(z * s * (1.0f - s), 2.0f * kGeluC * fmaf(3.0f * 0.044715f * z, z, 1.0f), s));
+    }
+    case kActGelu: {
+      const float p = 0.5f * (1.0f + erff(z * 0.7071067811865476f));
+      return make_float2(z * p, fmaf(z * 0.3989422804014327f, __expf(-0.5f * z * z), p));
+    }
+    case kActSilu: {
+      const float s = sigmoidf_(z);
+      return make_float2(z * s, s * fmaf(z, 1.0f - s, 1.0f));
+    }
+    default: return make_float2(z, 1.0f);
+  }
+}
+
+// ---- the product -----------------------------------------------------------------
+// One CTA per SM walks output tiles of 128 x BN.  Warp 0 streams 64-wide K
+// blocks of A and B through a ring of shared-memory stages, warp 1 issues the
+// MMAs into one of two TMEM accumulators, warps 2-5 read the other one back,
+// apply the epilogue and store, so the epilogue of a tile runs under the MMAs
+// of the next.
+template <int BN>
+struct GemmLayout {
+  static constexpr int kABytes = kTileM * kTileK * 2;
+  static constexpr int kBBytes = BN * kTileK * 2;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = 6;
+  static constexpr int kSmem = kStages * kStageBytes + 1024;  // + alignment slack
+};
+
+template <int STAGES>
+struct GemmShared {
+  uint64_t full[STAGES], empty[STAGES];
+  uint64_t acc_full[2], acc_empty[2];
+  uint32_t tmem;
+  int abort_flag;
+};
+
+// (m tile, n tile) of a linear tile number: bands of kBand m tiles walked
+// down first, so that the CTAs running at one time share few rows of A and B
+constexpr int kBand = 8;
+__device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int& tm, int& tn) {
+  const int per_band = kBand * tiles_n;
+  const int band = t / per_band;
+  const int first = band * kBand;
+  const int height = min(kBand, tiles_m - first);
+  const int in = t - band * per_band;
+  tm = first + in % height;
+  tn = in / height;
+}
+
+// 128 (or BN) x 64 operand tile into shared memory: K-major rows of 128
+// bytes, or MN-major panels of 64 elements x 64 K rows
+template <bool MN, int ROWS>
+__device__ __forceinline__ void load_tile(unsigned char* dst, const CUtensorMap* map, int row0, int kb, uint64_t* bar) {
+  if (!MN) {
+    tma_load_2d(dst, map, kb * kTileK, row0, bar);
+  } else {
+#pragma unroll
+    for (int p = 0; p < ROWS / 64; ++p) tma_load_2d(dst + p * 8192, map, row0 + p * 64, kb * kTileK, bar);
+  }
+}
+
+// descriptor of the k-th 16-wide K step of a tile
+template <bool MN>
+__device__ __forceinline__ uint64_t step_desc(uint32_t base, int k) {
+  return MN ? smem_desc(base + k * 2048, 8192, 1024) : smem_desc(base + k * 32, 16, 1024);
+}
+
+template <typename T, int BN, bool AMN, bool BMN, bool EPI>
+__global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmArgs args) {
+  using L = GemmLayout<BN>;
+  constexpr int kStages = L::kStages;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ GemmShared<kStages> sh;
+  unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort_flag = &sh.abort_flag;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&sh.full[s], 1);
+      mbar_init(&sh.empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sh.acc_full[b], 1);
+      mbar_init(&sh.acc_empty[b], 4);
+    }
+    sh.abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&sh.tmem, 2 * BN);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  const int tiles = args.tiles_m * args.tiles_n;
+  const int kb0 = args.kblocks[0], kblocks = kb0 + args.kblocks[1];
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- TMA
+    if (lane == 0) {
+      bool ok = true;
+      uint32_t it = 0;
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        int tm, tn;
+        tile_coords(t, args.tiles_m, args.tiles_n, tm, tn);
+        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+          const int s = it % kStages;
+          ok = mbar_wait(&sh.empty[s], ((it / kStages) & 1) ^ 1, abort_flag, args.status);
+          if (!ok) break;
+          unsigned char* st = ring + s * L::kStageBytes;
+          mbar_arrive_expect_tx(&sh.full[s], L::kStageBytes);
+          const int seg = kb >= kb0 ? 1 : 0;
+          const int kx = kb - (seg ? kb0 : 0);
+          load_tile<AMN, kTileM>(st, &args.a[seg], tm * kTileM, kx, &sh.full[s]);
+          load_tile<BMN, BN>(st + L::kABytes, &args.b[seg], tn * BN, kx, &sh.full[s]);
+        }
+      }
+      // after an expired wait: let the copies still in flight land before the CTA ends
+      if (!ok) {
+        int drained = 0;
+        const uint32_t first = it > kStages ? it - kStages : 0;
+        for (uint32_t i = first; i < it; ++i)
+          mbar_wait(&sh.full[i % kStages], (i / kStages) & 1, &drained, args.status);
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA
+    if (lane == 0) {
+      constexpr int ab = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+      constexpr uint32_t idesc = instr_desc(kTileM, BN, ab, AMN, BMN);
+      bool ok = true;
+      uint32_t it = 0, local = 0;
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++local) {
+        const int b = local & 1;
+        ok = mbar_wait(&sh.acc_empty[b], ((local >> 1) & 1) ^ 1, abort_flag, args.status);
+        if (!ok) break;
+        tc_fence_after();
+        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+          const int s = it % kStages;
+          ok = mbar_wait(&sh.full[s], (it / kStages) & 1, abort_flag, args.status);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sa = smem_u32(ring + s * L::kStageBytes), sb = sa + L::kABytes;
+#pragma unroll
+          for (int k = 0; k < kTileK / 16; ++k)
+            umma_ss(tmem + b * BN, step_desc<AMN>(sa, k), step_desc<BMN>(sb, k), idesc, (kb | k) ? 1u : 0u);
+          umma_commit(&sh.empty[s]);
+        }
+        if (ok) umma_commit(&sh.acc_full[b]);
+      }
+    }
+  } else {
+    // ----------------------------------------------------------- epilogue
+    const int quarter = warp & 3;  // the TMEM lanes this warp may read
+    uint32_t local = 0;
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++local) {
+      int tm, tn;
+      tile_coords(t, args.tiles_m, args.tiles_n, tm, tn);
+      const int b = local & 1;
+      if (!mbar_wait_warp(&sh.acc_full[b], (local >> 1) & 1, abort_flag, args.status)) break;
+      tc_fence_after();
+      const long long row = static_cast<long long>(tm) * kTileM + quarter * 32 + lane;
+      const bool live = row < args.m;
+      const T* gate = nullptr;
+      if (EPI && args.gate && live)
+        gate = static_cast<const T*>(args.gate) + (row / args.rows_per_sample) * args.gate_stride;
+      for (int c = 0; c < BN; c += 32) {
+        uint32_t acc[32];
+        tmem_ld32_sync(tmem + b * BN + (static_cast<uint32_t>(quarter * 32) << 16) + c, acc);
+        if (live) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            const int col = tn * BN + c + j;
+            const int count = min(8, args.n - col);
+            if (count > 0) {
+              float v[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(acc[j + i]);
+              if (EPI) {
+                float e[8];
+                if (args.bias) {
+                  load_vec<8>(static_cast<const T*>(args.bias) + col, args.vec, count, e);
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) v[i] += e[i];
+                }
+                if (args.preact)
+                  store_vec<8>(static_cast<T*>(args.preact) + row * args.n + col, args.vec, count, v);
+                if (args.act != kActNone) {
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) v[i] = activate(v[i], args.act);
+                }
+                if (gate) {
+                  load_vec<8>(gate + col, args.vec, count, e);
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) v[i] *= e[i];
+                }
+                if (args.residual) {
+                  load_vec<8>(static_cast<const T*>(args.residual) + row * args.res_stride + col, args.vec, count, e);
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) v[i] += e[i];
+                }
+              }
+              store_vec<8>(static_cast<T*>(args.out) + row * args.out_stride + col, args.vec, count, v);
+            }
+          }
+        }
+        __syncwarp();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.acc_empty[b]);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 2 * BN);
+  }
+}
+
+// ---- unaligned operands ------------------------------------------------------------
+// rows [rows, cols] of 2-byte elements, any stride and alignment, to rows ld
+// elements apart (16-byte aligned); a block per row group, threads over columns
+__global__ void __launch_bounds__(256) pack_rows_kernel(const uint16_t* src, long long src_stride, uint16_t* dst,
+                                                        int ld, int rows, int cols) {
+  for (long long r = blockIdx.x; r < rows; r += gridDim.x)
+    for (int c = threadIdx.x; c < cols; c += blockDim.x) dst[r * ld + c] = src[r * src_stride + c];
+}
+
+// ---- gradient of the epilogue --------------------------------------------------------
+// One block per (256 columns, chunk of one sample's rows): lane l of every
+// warp owns 8 columns, the 8 warps take every eighth row.  Writes dz and the
+// chunk's column sums of dz and of g * act(z); a second kernel adds the
+// chunks in order, so the sums do not depend on the launch.
+struct ActBackwardArgs {
+  const void* grad;
+  long long grad_stride;
+  const void* preact;        // [rows, n] (null: act' = 1 and no gate gradient)
+  const void* gate;
+  long long gate_stride;
+  void* dz;                  // [rows, dz_stride] (null: not written)
+  int dz_stride;
+  float* part_bias;          // [samples * chunks, n] (null: no sums)
+  float* part_gate;
+  int samples, rows_per_sample, n, chunks, chunk_rows;
+  int act, vec;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) act_backward_kernel(const ActBackwardArgs a) {
+  __shared__ float red[2][8][256];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int sample = blockIdx.y / a.chunks, chunk = blockIdx.y - sample * a.chunks;
+  const int col = blockIdx.x * 256 + lane * 8;
+  const int count = min(8, a.n - col);
+  float gate[8], sum_dz[8], sum_ga[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    gate[i] = 1.0f;
+    sum_dz[i] = sum_ga[i] = 0.0f;
+  }
+  if (count > 0) {
+    if (a.gate) load_vec<8>(static_cast<const T*>(a.gate) + sample * a.gate_stride + col, a.vec, count, gate);
+    const int begin = chunk * a.chunk_rows, end = min(begin + a.chunk_rows, a.rows_per_sample);
+    for (int r = begin + warp; r < end; r += 8) {
+      const long long row = static_cast<long long>(sample) * a.rows_per_sample + r;
+      float g[8], z[8], dz[8];
+      load_vec<8>(static_cast<const T*>(a.grad) + row * a.grad_stride + col, a.vec, count, g);
+      if (a.preact) load_vec<8>(static_cast<const T*>(a.preact) + row * a.n + col, a.vec, count, z);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        dz[i] = g[i] * gate[i];
+        if (a.preact) {
+          const float2 f = activate_slope(z[i], a.act);
+          dz[i] *= f.y;
+          sum_ga[i] = fmaf(g[i], f.x, sum_ga[i]);
+        }
+        sum_dz[i] += dz[i];
+      }
+      // dz is rounded to the operands' type for the tensor core; its sums are not
+      if (a.dz) store_vec<8>(static_cast<T*>(a.dz) + row * a.dz_stride + col, a.vec, count, dz);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    red[0][warp][lane * 8 + i] = sum_dz[i];
+    red[1][warp][lane * 8 + i] = sum_ga[i];
+  }
+  __syncthreads();
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c < a.n) {
+    float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      s0 += red[0][w][threadIdx.x];
+      s1 += red[1][w][threadIdx.x];
+    }
+    const long long at = static_cast<long long>(blockIdx.y) * a.n + c;
+    if (a.part_bias) a.part_bias[at] = s0;
+    if (a.part_gate) a.part_gate[at] = s1;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) act_backward_sums_kernel(const float* part_bias, const float* part_gate,
+                                                                T* dbias, T* dgate, int samples, int chunks, int n) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= n) return;
+  float total = 0.0f;
+  for (int b = 0; b < samples; ++b) {
+    float gsum = 0.0f;
+    for (int i = 0; i < chunks; ++i) {
+      const long long at = (static_cast<long long>(b) * chunks + i) * n + c;
+      if (dbias) total += part_bias[at];
+      if (dgate) gsum += part_gate[at];
+    }
+    if (dgate) dgate[static_cast<long long>(b) * n + c] = from_f32<T>(gsum);
+  }
+  if (dbias) dbias[c] = from_f32<T>(total);
+}
+
+// ---- host side --------------------------------------------------------------------------
+constexpr long long kAlign = 256;
+long long align_up(long long v, long long a) { return (v + a - 1) / a * a; }
+
+// A matrix operand of a product in memory: ``rows`` rows of ``cols`` elements.
+struct Operand {
+  const void* ptr;
+  long long stride;  // elements between rows
+  int rows, cols;
+  bool aligned() const { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && (stride & 7) == 0; }
+  long long pack_bytes() const { return aligned() ? 0 : align_up(2LL * rows * align_up(cols, 8), kAlign); }
+};
+
+// Consecutive pieces of the caller's workspace.
+struct Carver {
+  unsigned char* base;
+  long long used;
+  void* take(long long bytes) {
+    void* p = base ? base + used : nullptr;
+    used += align_up(bytes, kAlign);
+    return p;
+  }
+};
+
+// The operand itself, or its copy in the workspace when TMA cannot read it.
+int prepare_operand(Operand& o, Carver& ws, cudaStream_t stream) {
+  if (o.aligned()) return kOk;
+  const int ld = static_cast<int>(align_up(o.cols, 8));
+  uint16_t* dst = static_cast<uint16_t*>(ws.take(o.pack_bytes()));
+  const int grid = o.rows < 8 * kNumSMs ? o.rows : 8 * kNumSMs;
+  pack_rows_kernel<<<grid, 256, 0, stream>>>(static_cast<const uint16_t*>(o.ptr), o.stride, dst, ld, o.rows, o.cols);
+  o.ptr = dst;
+  o.stride = ld;
+  return launch_status();
+}
+
+bool operand_map(CUtensorMap* map, const Operand& o, bool mn, int tile_rows, int dtype) {
+  const uint64_t dims[2] = {static_cast<uint64_t>(o.cols), static_cast<uint64_t>(o.rows)};
+  const uint64_t strides[1] = {static_cast<uint64_t>(o.stride) * 2};
+  // K-major: 64 K columns of tile_rows rows; MN-major: 64 columns of 64 K rows
+  const uint32_t box[2] = {64, static_cast<uint32_t>(mn ? 64 : tile_rows)};
+  return encode_tensor_map(map, dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                           o.ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <typename T, bool AMN, bool BMN, bool EPI>
+int launch_gemm(GemmArgs& g, const Operand* a, const Operand* b, int segments, int dtype, cudaStream_t stream) {
+  constexpr int BN = 128;
+  using L = GemmLayout<BN>;
+  g.tiles_m = (g.m + kTileM - 1) / kTileM;
+  g.tiles_n = (g.n + BN - 1) / BN;
+  if (static_cast<long long>(g.tiles_m) * g.tiles_n > 0x7fffffffLL) return kErrUnsupported;
+  for (int s = 0; s < 2; ++s) {
+    const int src = s < segments ? s : 0;
+    if (!operand_map(&g.a[s], a[src], AMN, kTileM, dtype) || !operand_map(&g.b[s], b[src], BMN, BN, dtype))
+      return kErrTensorMap;
+    g.kblocks[s] = s < segments ? ((AMN ? a[s].rows : a[s].cols) + kTileK - 1) / kTileK : 0;
+  }
+  g.status = device_status_ptr();
+  auto kernel = gemm_kernel<T, BN, AMN, BMN, EPI>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const int tiles = g.tiles_m * g.tiles_n;
+  kernel<<<tiles < kNumSMs ? tiles : kNumSMs, kGemmThreads, L::kSmem, stream>>>(g);
+  return launch_status();
+}
+
+bool aligned16(const void* p, long long stride) {
+  return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && (stride & 7) == 0);
+}
+
+struct LinearShape {
+  int samples, rows_per_sample, k, k2, n, act, dtype;
+  long long rows() const { return static_cast<long long>(samples) * rows_per_sample; }
+  bool valid() const {
+    return samples >= 0 && rows_per_sample >= 0 && k >= 1 && k2 >= 0 && n >= 1 && act >= kActNone && act <= kActSilu &&
+           (dtype == 0 || dtype == 1) && rows() <= 0x7fffff00LL &&
+           static_cast<long long>(k) + k2 <= 0x7fffff00LL && n <= 0x7fffff00;
+  }
+};
+
+const void* offset16(const void* p, long long elements) { return static_cast<const uint16_t*>(p) + elements; }
+
+template <typename T>
+int forward(const LinearShape& s, Operand (&a)[2], Operand (&b)[2], GemmArgs& g, Carver& ws, cudaStream_t stream) {
+  const int segments = s.k2 > 0 ? 2 : 1;
+  for (int i = 0; i < segments; ++i) {
+    if (int st = prepare_operand(a[i], ws, stream)) return st;
+    if (int st = prepare_operand(b[i], ws, stream)) return st;
+  }
+  return launch_gemm<T, false, false, true>(g, a, b, segments, s.dtype, stream);
+}
+
+// Row chunks per sample of the epilogue's gradient: enough blocks for four per SM
+int backward_chunks(const LinearShape& s) {
+  if (s.samples < 1) return 1;
+  const long long blocks = static_cast<long long>((s.n + 255) / 256) * s.samples;
+  long long chunks = (4LL * kNumSMs + blocks - 1) / blocks;
+  const long long most = (s.rows_per_sample + 15) / 16;
+  if (chunks > most) chunks = most;
+  const long long cap = 65535 / s.samples;
+  if (chunks > cap) chunks = cap;
+  return chunks < 1 ? 1 : static_cast<int>(chunks);
+}
+
+struct BackwardPlan {
+  bool elementwise;   // dz differs from grad, or grad cannot be read in place
+  bool sums;
+  int chunks;
+  long long dz_bytes, part_bytes;
+};
+
+BackwardPlan plan_backward(const LinearShape& s, const Operand& grad, bool has_gate, bool need_product, bool need_bias,
+                           bool need_gate) {
+  BackwardPlan p;
+  p.elementwise = need_product && (s.act != kActNone || has_gate || !grad.aligned());
+  p.sums = need_bias || need_gate;
+  p.chunks = backward_chunks(s);
+  p.dz_bytes = p.elementwise ? 2 * s.rows() * align_up(s.n, 8) : 0;
+  p.part_bytes = 4LL * s.samples * p.chunks * s.n;
+  return p;
+}
+
+template <typename T>
+int backward(const LinearShape& s, Operand grad, const void* preact, Operand (&x)[2], Operand (&w)[2],
+             const void* gate, long long gate_stride, void* (&dx)[2], void* dweight, void* dbias, void* dgate,
+             Carver& ws, cudaStream_t stream) {
+  const int segments = s.k2 > 0 ? 2 : 1;
+  const bool need_product = dx[0] || dx[1] || dweight;
+  const BackwardPlan p = plan_backward(s, grad, gate != nullptr, need_product, dbias != nullptr, dgate != nullptr);
+  Operand dz = grad;
+  if (p.elementwise || p.sums) {
+    ActBackwardArgs a{};
+    a.grad = grad.ptr;
+    a.grad_stride = grad.stride;
+    a.preact = (s.act != kActNone || dgate) ? preact : nullptr;
+    a.gate = gate;
+    a.gate_stride = gate_stride;
+    a.dz_stride = static_cast<int>(align_up(s.n, 8));
+    a.dz = p.elementwise ? ws.take(p.dz_bytes) : nullptr;
+    if (p.elementwise) dz = Operand{a.dz, a.dz_stride, static_cast<int>(s.rows()), s.n};
+    a.part_bias = dbias ? static_cast<float*>(ws.take(p.part_bytes)) : nullptr;
+    a.part_gate = dgate ? static_cast<float*>(ws.take(p.part_bytes)) : nullptr;
+    a.samples = s.samples;
+    a.rows_per_sample = s.rows_per_sample;
+    a.n = s.n;
+    a.chunks = p.chunks;
+    a.chunk_rows = (s.rows_per_sample + p.chunks - 1) / p.chunks;
+    a.act = s.act;
+    a.vec = s.n % 8 == 0 && aligned16(grad.ptr, grad.stride) && aligned16(a.preact, s.n) && aligned16(gate, gate_stride);
+    const dim3 grid((s.n + 255) / 256, s.samples * p.chunks);
+    act_backward_kernel<T><<<grid, 256, 0, stream>>>(a);
+    if (int st = launch_status()) return st;
+    if (p.sums) {
+      act_backward_sums_kernel<T><<<(s.n + 255) / 256, 256, 0, stream>>>(
+          a.part_bias, a.part_gate, static_cast<T*>(dbias), static_cast<T*>(dgate), s.samples, p.chunks, s.n);
+      if (int st = launch_status()) return st;
+    }
+  }
+  for (int i = 0; i < segments; ++i) {
+    const int cols = i ? s.k2 : s.k;
+    if (dx[i]) {
+      // dx[m, c] = sum_n dz[m, n] W[n, c]: W's rows run along the output's columns
+      if (int st = prepare_operand(w[i], ws, stream)) return st;
+      GemmArgs g{};
+      g.m = static_cast<int>(s.rows());
+      g.n = cols;
+      g.out = dx[i];
+      g.out_stride = cols;
+      g.vec = cols % 8 == 0 && aligned16(dx[i], cols);
+      if (int st = launch_gemm<T, false, true, false>(g, &dz, &w[i], 1, s.dtype, stream)) return st;
+    }
+    if (dweight) {
+      // dW[n, c] = sum_m dz[m, n] x[m, c]: both operands run along the outputs
+      if (int st = prepare_operand(x[i], ws, stream)) return st;
+      GemmArgs g{};
+      g.m = s.n;
+      g.n = cols;
+      g.out = static_cast<T*>(dweight) + (i ? s.k : 0);
+      g.out_stride = static_cast<long long>(s.k) + s.k2;
+      g.vec = cols % 8 == 0 && aligned16(g.out, g.out_stride);
+      if (int st = launch_gemm<T, true, true, false>(g, &dz, &x[i], 1, s.dtype, stream)) return st;
+    }
+  }
+  return kOk;
+}
+
+void make_operands(const LinearShape& s, const void* x, long long x_stride, const void* x2, long long x2_stride,
+                   const void* weight, long long w_stride, Operand (&a)[2], Operand (&b)[2]) {
+  const int rows = static_cast<int>(s.rows());
+  // the stride of a single row is never walked; TMA wants it aligned all the same
+  if (rows == 1) {
+    x_stride = align_up(s.k, 8);
+    x2_stride = align_up(s.k2, 8);
+  }
+  if (s.n == 1 && s.k2 == 0) w_stride = align_up(s.k, 8);
+  a[0] = Operand{x, x_stride, rows, s.k};
+  a[1] = Operand{x2, x2_stride, rows, s.k2};
+  b[0] = Operand{weight, w_stride, s.n, s.k};
+  b[1] = Operand{offset16(weight, s.k), w_stride, s.n, s.k2};
+}
+
+}  // namespace
+}  // namespace peco
+
+using namespace peco;
+
+extern "C" long long peco_linear_forward_workspace(const void* x, long long x_stride, const void* x2,
+                                                   long long x2_stride, const void* weight, long long w_stride,
+                                                   int samples, int rows_per_sample, int k, int k2, int n) {
+  const LinearShape s{samples, rows_per_sample, k, k2, n, 0, 0};
+  if (!s.valid()) return -1;
+  Operand a[2], b[2];
+  make_operands(s, x, x_stride, x2, x2_stride, weight, w_stride, a, b);
+  long long bytes = a[0].pack_bytes() + b[0].pack_bytes();
+  if (k2) bytes += a[1].pack_bytes() + b[1].pack_bytes();
+  return bytes;
+}
+
+extern "C" int peco_linear_forward(const void* x, long long x_stride, const void* x2, long long x2_stride,
+                                   const void* weight, long long w_stride, const void* bias, const void* gate,
+                                   long long gate_stride, const void* residual, long long res_stride, void* out,
+                                   long long out_stride, void* preact, int samples, int rows_per_sample, int k, int k2,
+                                   int n, int activation, int dtype, void* workspace, long long workspace_bytes,
+                                   void* stream_ptr) {
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  const LinearShape s{samples, rows_per_sample, k, k2, n, activation, dtype};
+  if (dtype != 0 && dtype != 1) return kErrUnsupported;
+  if (!s.valid()) return kErrInvalidValue;
+  if (s.rows() == 0) return kOk;
+  if (!x || !weight || !out || (k2 > 0 && !x2)) return kErrInvalidValue;
+  // gate_stride is free: a row shared by all samples has stride 0
+  if (x_stride < k || (k2 > 0 && x2_stride < k2) || w_stride < static_cast<long long>(k) + k2 || out_stride < n ||
+      (residual && res_stride < n) || gate_stride < 0)
+    return kErrInvalidValue;
+  const long long need =
+      peco_linear_forward_workspace(x, x_stride, x2, x2_stride, weight, w_stride, samples, rows_per_sample, k, k2, n);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return kErrWorkspace;
+  Operand a[2], b[2];
+  make_operands(s, x, x_stride, x2, x2_stride, weight, w_stride, a, b);
+  GemmArgs g{};
+  g.m = static_cast<int>(s.rows());
+  g.n = n;
+  g.out = out;
+  g.out_stride = out_stride;
+  g.bias = bias;
+  g.gate = gate;
+  g.gate_stride = gate_stride;
+  g.rows_per_sample = rows_per_sample;
+  g.residual = residual;
+  g.res_stride = res_stride;
+  g.preact = preact;
+  g.act = activation;
+  g.vec = n % 8 == 0 && aligned16(out, out_stride) && aligned16(bias, 8) && aligned16(gate, gate_stride) &&
+          aligned16(residual, res_stride) && aligned16(preact, n);
+  Carver ws{static_cast<unsigned char*>(workspace), 0};
+  return dtype == 1 ? forward<__nv_bfloat16>(s, a, b, g, ws, stream) : forward<__half>(s, a, b, g, ws, stream);
+}
+
+extern "C" long long peco_linear_backward_workspace(const void* grad, long long grad_stride, const void* x,
+                                                    long long x_stride, const void* x2, long long x2_stride,
+                                                    const void* weight, long long w_stride, int samples,
+                                                    int rows_per_sample, int k, int k2, int n, int activation,
+                                                    int has_gate) {
+  const LinearShape s{samples, rows_per_sample, k, k2, n, activation, 0};
+  if (!s.valid()) return -1;
+  Operand a[2], b[2];
+  make_operands(s, x, x_stride, x2, x2_stride, weight, w_stride, a, b);
+  const Operand g{grad, grad_stride, static_cast<int>(s.rows()), n};
+  const BackwardPlan p = plan_backward(s, g, has_gate != 0, true, true, true);
+  long long bytes = align_up(p.dz_bytes, kAlign) + 2 * align_up(p.part_bytes, kAlign) + a[0].pack_bytes() + b[0].pack_bytes();
+  if (k2) bytes += a[1].pack_bytes() + b[1].pack_bytes();
+  return bytes;
+}
+
+extern "C" int peco_linear_backward(const void* grad, long long grad_stride, const void* preact, const void* x,
+                                    long long x_stride, const void* x2, long long x2_stride, const void* weight,
+                                    long long w_stride, const void* gate, long long gate_stride, void* dx, void* dx2,
+                                    void* dweight, void* dbias, void* dgate, int samples, int rows_per_sample, int k,
+                                    int k2, int n, int activation, int dtype, void* workspace,
+                                    long long workspace_bytes, void* stream_ptr) {
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  const LinearShape s{samples, rows_per_sample, k, k2, n, activation, dtype};
+  if (dtype != 0 && dtype != 1) return kErrUnsupported;
+  if (!s.valid()) return kErrInvalidValue;
+  if (s.rows() == 0) return kErrInvalidValue;  // the sums over no rows are the caller's zeros
+  if (samples > 65535) return kErrUnsupported;
+  if (!grad || grad_stride < n || gate_stride < 0) return kErrInvalidValue;
+  if ((dx || dx2) && (!weight || w_stride < static_cast<long long>(k) + k2)) return kErrInvalidValue;
+  if (dweight && (!x || x_stride < k || (k2 > 0 && (!x2 || x2_stride < k2)))) return kErrInvalidValue;
+  if (dx2 && k2 == 0) return kErrInvalidValue;
+  if ((activation != kActNone || dgate) && !preact) return kErrInvalidValue;
+  const long long need = peco_linear_backward_workspace(grad, grad_stride, x, x_stride, x2, x2_stride, weight, w_stride,
+                                                        samples, rows_per_sample, k, k2, n, activation, gate != nullptr);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return kErrWorkspace;
+  Operand a[2], b[2];
+  make_operands(s, x, x_stride, x2, x2_stride, weight, w_stride, a, b);
+  const Operand g{grad, grad_stride, static_cast<int>(s.rows()), n};
+  void* dxs[2] = {dx, dx2};
+  Carver ws{static_cast<unsigned char*>(workspace), 0};
+  return dtype == 1 ? backward<__nv_bfloat16>(s, g, preact, a, b, gate, gate_stride, dxs, dweight, dbias, dgate, ws, stream)
+                    : backward<__half>(s, g, preact, a, b, gate, gate_stride, dxs, dweight, dbias, dgate, ws, stream);
+}

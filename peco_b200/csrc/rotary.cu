@@ -1,0 +1,259 @@
+// Rotary embedding by positions on several axes (time, height, width of a
+// video token), for Q and K of one attention call together.
+//
+// Head dimensions are cut into consecutive sections, one per axis, of d_a
+// dimensions each.  Pair j of axis a turns by
+//   angle = position[a] * theta^(-2 j / d_a),
+//   (a, b) -> (a cos - b sin, b cos + a sin),
+// where a pair is two neighbouring dimensions, or one from each half of the
+// rotated dimensions.  Dimensions past the sections, and rows past the rotated
+// ones (the text), are copied.  The inverse turn (the gradient) negates sin.
+//
+// No tables: the angle is formed in turns, position * (theta^(..) / 2 pi) in
+// 64 bits, reduced to [-1/2, 1/2] there and only then rounded to fp32, so its
+// error does not grow with the position.
+//
+// The operator moves bytes: each element is read once and written once, and
+// the floor is that traffic at the copy bandwidth.  A thread owns one 16-byte
+// run of dimensions (eight bytes of each half in the split pairing) of one
+// token and walks the heads with it, so the sine and cosine are computed once
+// per token and head group and the loads of several heads are in flight at
+// once.
+#include "common.cuh"
+#include "../../include/peco_b200.h"
+#include "internal.h"
+#include "rows.cuh"
+
+#include <math.h>
+
+namespace peco {
+namespace {
+
+constexpr int kMaxAxes = 4;
+constexpr int kMaxPairs = 128;  // head dimension up to 256
+constexpr int kThreads = 256;
+constexpr int kBatch = 4;       // heads whose loads are in flight together
+
+struct RotaryTensor {
+  const void* src;
+  void* dst;
+  long long sb, sh, sn;  // source strides (elements): batch, head, token
+  long long db, dh, dn;  // destination strides
+  int heads;
+};
+
+struct RotaryArgs {
+  RotaryTensor t[2];
+  int rows, rotated_rows, dims, pairs;
+  int units, tokens_per_block, token_blocks, heads_per_block;
+  int axes;
+  unsigned grid[kMaxAxes];      // token grid (positions == null)
+  const void* positions;        // [batch, rotated_rows, axes]
+  long long pos_sb, pos_sn;     // strides in elements; the axes are adjacent
+  int pos_type;                 // 0 int32, 1 int64, 2 fp32
+  int inverse;
+  double turns[kMaxPairs];      // turns per unit of position of each pair
+  unsigned char axis[kMaxPairs];
+};
+
+__device__ __forceinline__ double position_of(const RotaryArgs& a, int batch, int token, int axis) {
+  if (a.positions) {
+    const long long at = batch * a.pos_sb + token * a.pos_sn + axis;
+    if (a.pos_type == 0) return static_cast<const int*>(a.positions)[at];
+    if (a.pos_type == 1) return static_cast<double>(static_cast<const long long*>(a.positions)[at]);
+    return static_cast<const float*>(a.positions)[at];
+  }
+  unsigned rest = token;
+  for (int i = a.axes - 1; i > axis; --i) rest /= a.grid[i];
+  return axis ? rest % a.grid[axis] : rest;
+}
+
+// row of head h (Q's heads first, then K's) in the source or the destination
+template <typename T>
+__device__ __forceinline__ T* row_of(const RotaryArgs& a, int h, int batch, int token, bool destination) {
+  const int which = h >= a.t[0].heads ? 1 : 0;
+  const RotaryTensor& t = a.t[which];
+  const int head = h - (which ? a.t[0].heads : 0);
+  return destination ? static_cast<T*>(t.dst) + batch * t.db + head * t.dh + token * t.dn
+                     : static_cast<T*>(const_cast<void*>(t.src)) + batch * t.sb + head * t.sh + token * t.sn;
+}
+
+// V pairs per thread.  Interleaved: 2V neighbouring dimensions.  Split: V
+// dimensions in each half of the rotated ones; the copied tail is then cut
+// into runs of 2V like the interleaved form.
+template <typename T, int V, bool SPLIT>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryArgs a) {
+  const int slot = threadIdx.x / a.units, unit = threadIdx.x - slot * a.units;
+  const int batch = blockIdx.x / a.token_blocks;
+  const int token = (blockIdx.x - batch * a.token_blocks) * a.tokens_per_block + slot;
+  if (slot >= a.tokens_per_block || token >= a.rows) return;
+  const int pair0 = unit * V;
+  const bool rotated = token < a.rotated_rows && pair0 < a.pairs;
+  // the two runs of V elements this thread moves
+  const bool halves = SPLIT && pair0 < a.pairs;
+  const int lo = halves ? pair0 : 2 * pair0;
+  const int hi = halves ? pair0 + a.pairs : 2 * pair0 + V;
+  float c[V], s[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    c[i] = 1.0f;
+    s[i] = 0.0f;
+    if (rotated && pair0 + i < a.pairs) {
+      double t = position_of(a, batch, token, a.axis[pair0 + i]) * a.turns[pair0 + i];
+      t -= rint(t);
+      sincospif(2.0f * static_cast<float>(t), &s[i], &c[i]);
+      if (a.inverse) s[i] = -s[i];
+    }
+  }
+  const int all_heads = a.t[0].heads + a.t[1].heads;
+  const int first = blockIdx.y * a.heads_per_block;
+  const int last = min(first + a.heads_per_block, all_heads);
+  // The loads of kBatch heads are issued before the first store: source and
+  // destination may be the same tensor, so the compiler must not be left to
+  // order them.
+  for (int h0 = first; h0 < last; h0 += kBatch) {
+    float x[kBatch][2 * V];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if (h0 + j < last) {
+        const T* src = row_of<T>(a, h0 + j, batch, token, false);
+        if constexpr (V == 1) {
+          x[j][0] = to_f32<T>(src[lo]);
+          x[j][1] = to_f32<T>(src[hi]);
+        } else if constexpr (!SPLIT) {
+          load_aligned<2 * V>(src + lo, x[j]);
+        } else {
+          float p[V], q[V];
+          load_aligned<V>(src + lo, p);
+          load_aligned<V>(src + hi, q);
+#pragma unroll
+          for (int i = 0; i < V; ++i) x[j][i] = p[i], x[j][V + i] = q[i];
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if (h0 + j < last) {
+        if (rotated) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const int ia = SPLIT ? i : 2 * i, ib = SPLIT ? V + i : 2 * i + 1;
+            const float u = x[j][ia], w = x[j][ib];
+            x[j][ia] = u * c[i] - w * s[i];
+            x[j][ib] = w * c[i] + u * s[i];
+          }
+        }
+        T* dst = row_of<T>(a, h0 + j, batch, token, true);
+        if constexpr (V == 1) {
+          dst[lo] = from_f32<T>(x[j][0]);
+          dst[hi] = from_f32<T>(x[j][1]);
+        } else if constexpr (!SPLIT) {
+          store_aligned<2 * V>(dst + lo, x[j]);
+        } else {
+          float p[V], q[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) p[i] = x[j][i], q[i] = x[j][V + i];
+          store_aligned<V>(dst + lo, p);
+          store_aligned<V>(dst + hi, q);
+        }
+      }
+    }
+  }
+}
+
+template <typename T>
+int launch_rotary(RotaryArgs& a, int batch, bool split, cudaStream_t stream) {
+  constexpr int V = 4;
+  // one aligned access of 2V elements (interleaved) or V (split), fp32 in 16-byte pieces
+  const int align = sizeof(T) == 4 ? 4 : split ? V : 2 * V;
+  bool vec = (!split || a.pairs % V == 0) && a.dims % (2 * V) == 0;
+  for (const RotaryTensor& t : a.t) {
+    if (!t.heads) continue;
+    const long long step = t.sb | t.sh | t.sn | t.db | t.dh | t.dn;
+    const uintptr_t base = reinterpret_cast<uintptr_t>(t.src) | reinterpret_cast<uintptr_t>(t.dst);
+    vec = vec && step % align == 0 && base % (align * sizeof(T)) == 0;
+  }
+  a.units = a.dims / (vec ? 2 * V : 2);
+  a.tokens_per_block = kThreads / a.units;
+  a.token_blocks = (a.rows + a.tokens_per_block - 1) / a.tokens_per_block;
+  const long long blocks = static_cast<long long>(batch) * a.token_blocks;
+  if (blocks > 0x7fffffffLL) return kErrUnsupported;
+  // All heads in one block when the tokens alone fill the GPU (the sines are
+  // then computed once per token); otherwise heads are spread over blocks.
+  const int heads = a.t[0].heads + a.t[1].heads;
+  long long groups = (16LL * kNumSMs + blocks - 1) / blocks;
+  if (groups > heads) groups = heads;
+  a.heads_per_block = static_cast<int>((heads + groups - 1) / groups);
+  const dim3 grid(static_cast<unsigned>(blocks), (heads + a.heads_per_block - 1) / a.heads_per_block);
+  if (vec && split) rotary_kernel<T, V, true><<<grid, kThreads, 0, stream>>>(a);
+  else if (vec) rotary_kernel<T, V, false><<<grid, kThreads, 0, stream>>>(a);
+  else if (split) rotary_kernel<T, 1, true><<<grid, kThreads, 0, stream>>>(a);
+  else rotary_kernel<T, 1, false><<<grid, kThreads, 0, stream>>>(a);
+  return launch_status();
+}
+
+}  // namespace
+}  // namespace peco
+
+using namespace peco;
+
+extern "C" int peco_rotary(const void* q, void* q_out, int q_heads, const long long* q_strides, const void* k,
+                           void* k_out, int k_heads, const long long* k_strides, int batch, int rows,
+                           int rotated_rows, int dims, const int* axes, int n_axes, double theta, const int* grid,
+                           const void* positions, long long pos_batch_stride, long long pos_row_stride, int pos_type,
+                           int interleaved, int inverse, int dtype, void* stream_ptr) {
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  if (dtype < 0 || dtype > 2 || n_axes < 1 || n_axes > kMaxAxes || dims < 2 || dims > 2 * kMaxPairs || dims % 2)
+    return kErrUnsupported;
+  if (batch < 0 || rows < 0 || rotated_rows < 0 || rotated_rows > rows || q_heads < 0 || k_heads < 0 || !axes ||
+      !(theta > 0.0) || pos_type < 0 || pos_type > 2 || (!grid && !positions))
+    return kErrInvalidValue;
+  if ((q_heads && !q_strides) || (k_heads && !k_strides) || q_heads > 32767 || k_heads > 32767) return kErrInvalidValue;
+  RotaryArgs a{};
+  for (int i = 0; i < n_axes; ++i) {
+    if (axes[i] < 0 || axes[i] % 2 || 2 * a.pairs + axes[i] > dims) return kErrInvalidValue;
+    // theta^(-2 j / d) by repeated multiplication in 64 bits
+    const double step = axes[i] ? pow(theta, -2.0 / axes[i]) : 1.0;
+    double f = 0.15915494309189533577;  // 1 / (2 pi)
+    for (int j = 0; j < axes[i] / 2; ++j, f *= step) {
+      a.turns[a.pairs] = f;
+      a.axis[a.pairs++] = static_cast<unsigned char>(i);
+    }
+  }
+  if (!positions) {
+    long long tokens = 1;
+    for (int i = 0; i < n_axes; ++i) {
+      if (grid[i] < 0) return kErrInvalidValue;
+      a.grid[i] = grid[i] > 0 ? grid[i] : 1;
+      tokens *= grid[i];
+      if (tokens > rows) return kErrInvalidValue;
+    }
+    if (tokens != rotated_rows) return kErrInvalidValue;
+  }
+  if (batch == 0 || rows == 0 || q_heads + k_heads == 0) return kOk;
+  if ((q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out))) return kErrInvalidValue;
+  const void* src[2] = {q, k};
+  void* dst[2] = {q_out, k_out};
+  const int heads[2] = {q_heads, k_heads};
+  const long long* strides[2] = {q_strides, k_strides};
+  for (int i = 0; i < 2; ++i) {
+    if (!heads[i]) continue;
+    const long long* s = strides[i];
+    a.t[i] = RotaryTensor{src[i], dst[i], s[0], s[1], s[2], s[3], s[4], s[5], heads[i]};
+  }
+  a.rows = rows;
+  a.rotated_rows = rotated_rows;
+  a.dims = dims;
+  a.axes = n_axes;
+  a.positions = positions;
+  a.pos_sb = pos_batch_stride;
+  a.pos_sn = pos_row_stride;
+  a.pos_type = pos_type;
+  a.inverse = inverse;
+  const bool split = !interleaved;
+  switch (dtype) {
+    case 0: return launch_rotary<__half>(a, batch, split, stream);
+    case 1: return launch_rotary<__nv_bfloat16>(a, batch, split, stream);
+    default: return launch_rotary<float>(a, batch, split, stream);
+  }
+}

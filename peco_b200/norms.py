@@ -1,0 +1,216 @@
+"""Gated residual and norm between the parts of a transformer block, over libpeco_b200.so.
+
+``modulated_norm``: one pass over the rows for what a block otherwise runs as
+the branch's own norm, a product with the adaLN gate, the residual sum, a layer
+or RMS norm and the shift / scale modulation:
+
+    b = post_norm(branch) * post_weight
+    r = residual_scale * x + gate * b
+    h = norm(r) * weight * (1 + scale) + shift
+
+Statistics and products are fp32; r and h are each rounded once.  float16 and
+bfloat16, up to 16384 features.  Differentiable; nothing beyond the inputs is
+saved.  CUDA tensors only; work is enqueued on the current stream.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _native
+
+NORMS = {None: 0, "none": 0, "layer": 1, "rms": 2}
+
+
+class NormGrads(NamedTuple):
+    """Gradients of ``modulated_norm``; None where the input is absent."""
+
+    x: Optional[torch.Tensor]
+    branch: Optional[torch.Tensor]
+    gate: Optional[torch.Tensor]
+    scale: Optional[torch.Tensor]
+    shift: Optional[torch.Tensor]
+    weight: Optional[torch.Tensor]
+    post_weight: Optional[torch.Tensor]
+
+
+def _opt(t):
+    return _native.ptr(t) if t is not None else _native.P(0)
+
+
+def _rows(t, width):
+    """(tensor, batch stride, row stride) of [B, T, C] rows with adjacent columns."""
+    if t is None:
+        return None, 0, 0
+    t = t.reshape(-1, *t.shape[-2:]) if t.dim() != 3 else t
+    if t.stride(2) != 1 and width > 1:
+        t = t.contiguous()
+    return t, t.stride(0), t.stride(1)
+
+
+def _vec(t, width):
+    """(tensor, sample stride) of a vector [C] (stride 0) or [B, C] / [B, 1, C]."""
+    if t is None:
+        return None, 0
+    t = t.reshape(-1, width) if t.dim() == 3 else t
+    if t.stride(-1) != 1 and width > 1:
+        t = t.contiguous()
+    return t, t.stride(0) if t.dim() == 2 else 0
+
+
+def _as3(t):
+    """[T, C] or [C] rows as one sample; [B, ..., T, C] keeps its leading axis only."""
+    if t is None:
+        return None
+    if t.dim() <= 2:
+        return t.reshape(1, -1, t.shape[-1])
+    return t if t.dim() == 3 else t.reshape(t.shape[0], -1, t.shape[-1])
+
+
+def _check(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, eps, residual_scale):
+    if norm not in ("layer", "rms"):
+        raise ValueError(f'norm must be "layer" or "rms", got {norm!r}')
+    if post_norm not in NORMS:
+        raise ValueError(f'post_norm must be None, "layer" or "rms", got {post_norm!r}')
+    if not isinstance(x, torch.Tensor) or x.dim() < 1:
+        raise TypeError("x must be a torch tensor [..., C]")
+    there = [t for t in (x, branch, gate, scale, shift, weight, post_weight) if t is not None]
+    if x.dtype not in (torch.float16, torch.bfloat16) or any(t.dtype != x.dtype for t in there):
+        raise TypeError("modulated_norm takes float16 or bfloat16 tensors of one dtype")
+    c = x.shape[-1]
+    if not 1 <= c <= 16384:
+        raise ValueError("modulated_norm takes 1 to 16384 features")
+    if branch is not None and branch.shape != x.shape:
+        raise ValueError("branch must have the shape of x")
+    if branch is None and (gate is not None or NORMS[post_norm] or post_weight is not None):
+        raise ValueError("gate, post_norm and post_weight need a branch")
+    if post_weight is not None and not NORMS[post_norm]:
+        raise ValueError("post_weight needs a post_norm")
+    samples = x.shape[0] if x.dim() >= 3 else 1
+    for name, t in (("gate", gate), ("scale", scale), ("shift", shift)):
+        if t is not None and tuple(t.shape) not in ((c,), (samples, c), (samples, 1, c)):
+            raise ValueError(f"{name} must be [{c}] or one row for each of the {samples} samples, got {list(t.shape)}")
+    for name, t in (("weight", weight), ("post_weight", post_weight)):
+        if t is not None and tuple(t.shape) != (c,):
+            raise ValueError(f"{name} must be [{c}]")
+    if not eps >= 0 or not abs(residual_scale) < float("inf"):
+        raise ValueError("eps must be nonnegative and residual_scale finite")
+    _native.require_cuda(*there)
+
+
+def _forward(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, eps, post_eps, residual_scale):
+    _check(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, eps, residual_scale)
+    c = x.shape[-1]
+    normed = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    residual = torch.empty(x.shape, dtype=x.dtype, device=x.device) if branch is not None else None
+    if x.numel() == 0:
+        return residual, normed
+    x3, xb, xr = _rows(_as3(x), c)
+    b3, bb, br = _rows(_as3(branch), c)
+    (gate, gb), (scale, sb), (shift, tb) = (_vec(t, c) for t in (gate, scale, shift))
+    weight, post_weight = (None if t is None else t.contiguous() for t in (weight, post_weight))
+    lib = _native.load()
+    dev = x.device
+    with torch.cuda.device(dev):
+        stream = _native.stream_of(dev, x3, b3, gate, scale, shift, weight, post_weight, residual, normed)
+        status = lib.peco_gated_norm(_native.ptr(x3), xb, xr, _opt(b3), bb, br, _opt(gate), gb, _opt(scale), sb,
+                                     _opt(shift), tb, _opt(weight), _opt(post_weight), _opt(residual),
+                                     _native.ptr(normed), x3.shape[0], x3.shape[1], c, NORMS[norm], NORMS[post_norm],
+                                     float(eps), float(eps if post_eps is None else post_eps), float(residual_scale),
+                                     _native.DTYPE_CODE[x.dtype], stream)
+    _native.check(status, "peco_gated_norm")
+    return residual, normed
+
+
+class _ModulatedNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, branch, gate, scale, shift, weight, post_weight, options):
+        residual, normed = _forward(x, branch, gate, scale, shift, weight, post_weight, **options)
+        ctx.options = options
+        ctx.save_for_backward(x, branch, gate, scale, shift, weight, post_weight)
+        ctx.set_materialize_grads(False)
+        return normed if residual is None else (residual, normed)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        x = ctx.saved_tensors[0]
+        dr, dh = grads if len(grads) == 2 else (None, grads[0])
+        if dr is None and dh is None:
+            return (None,) * 8
+        if dh is None:
+            dh = torch.zeros_like(x)
+        names = [n for n, need in zip(NormGrads._fields, ctx.needs_input_grad) if need]
+        g = modulated_norm_backward(dh, dr, *ctx.saved_tensors[:2],
+                                    **dict(zip(NormGrads._fields[2:], ctx.saved_tensors[2:])), **ctx.options, needs=names)
+        return (*g, None)
+
+
+def modulated_norm(x, branch=None, *, gate=None, scale=None, shift=None, weight=None, post_weight=None, norm="layer",
+                   post_norm=None, eps=1e-6, post_eps=None, residual_scale=1.0):
+    """(r, h) of the module's formulas when there is a branch, h alone without one.
+
+    x, branch [B, T, C] (or [T, C], one sample; any row and batch strides);
+    gate, scale, shift [C] (one vector for all rows) or [B, C] / [B, 1, C];
+    weight, post_weight [C].  ``norm`` / ``post_norm``: "layer" (mean and
+    variance) or "rms"; ``post_eps`` defaults to ``eps``.  Absent parts drop out
+    of the formulas.
+    """
+    options = dict(norm=norm, post_norm=post_norm, eps=eps, post_eps=post_eps, residual_scale=residual_scale)
+    inputs = (x, branch, gate, scale, shift, weight, post_weight)
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in inputs):
+        return _ModulatedNorm.apply(*inputs, options)
+    residual, normed = _forward(*inputs, **options)
+    return normed if residual is None else (residual, normed)
+
+
+def modulated_norm_backward(grad_normed, grad_residual, x, branch=None, *, gate=None, scale=None, shift=None,
+                            weight=None, post_weight=None, norm="layer", post_norm=None, eps=1e-6, post_eps=None,
+                            residual_scale=1.0, needs=None):
+    """Gradients of ``modulated_norm`` for ``grad_normed`` = d h and
+    ``grad_residual`` = d r (None: zero).  ``needs``: names of the gradients to
+    compute (default: those of all inputs that are there)."""
+    inputs = dict(zip(NormGrads._fields, (x, branch, gate, scale, shift, weight, post_weight)))
+    _check(*inputs.values(), norm, post_norm, eps, residual_scale)
+    for name, t in (("grad_normed", grad_normed), ("grad_residual", grad_residual)):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise ValueError(f"{name} must have the shape and dtype of x")
+    if grad_normed is None:
+        raise ValueError("grad_normed is required")
+    if grad_residual is not None and branch is None:
+        raise ValueError("grad_residual needs a branch")
+    _native.require_cuda(*[t for t in (x, grad_normed, grad_residual) if t is not None])
+    needs = [n for n, t in inputs.items() if t is not None] if needs is None else list(needs)
+    if any(inputs.get(n) is None for n in needs):
+        raise ValueError("needs names a gradient whose input is absent")
+    if x.numel() == 0:
+        return NormGrads(**{n: torch.zeros(t.shape, dtype=x.dtype, device=x.device) if n in needs else None
+                            for n, t in inputs.items()})
+    grads = {n: torch.empty(inputs[n].shape, dtype=x.dtype, device=x.device) if n in needs else None for n in inputs}
+    c = x.shape[-1]
+    gh, ghb, ghr = _rows(_as3(grad_normed), c)
+    gr, grb, grr = _rows(_as3(grad_residual), c)
+    x3, xb, xr = _rows(_as3(x), c)
+    b3, bb, br = _rows(_as3(branch), c)
+    # a vector without a sample axis sums its gradient over the samples
+    shared = sum(bit for bit, t in ((1, gate), (2, scale), (4, shift)) if t is not None and t.dim() == 1)
+    (gv, gb), (sv, sb) = _vec(gate, c), _vec(scale, c)
+    weight, post_weight = (None if t is None else t.contiguous() for t in (weight, post_weight))
+    lib = _native.load()
+    dev = x.device
+    need, ws = 0, None
+    if any(n in needs for n in NormGrads._fields[2:]):
+        need = int(lib.peco_gated_norm_backward_workspace(x3.shape[0], x3.shape[1], c))
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        stream = _native.stream_of(dev, gh, gr, x3, b3, gv, sv, weight, post_weight, ws, *grads.values())
+        status = lib.peco_gated_norm_backward(
+            _native.ptr(gh), ghb, ghr, _opt(gr), grb, grr, _native.ptr(x3), xb, xr, _opt(b3), bb, br, _opt(gv), gb,
+            _opt(sv), sb, _opt(weight), _opt(post_weight), _opt(grads["x"]), _opt(grads["branch"]),
+            _opt(grads["gate"]), _opt(grads["scale"]), _opt(grads["shift"]), shared, _opt(grads["weight"]),
+            _opt(grads["post_weight"]), x3.shape[0], x3.shape[1], c, NORMS[norm], NORMS[post_norm], float(eps),
+            float(eps if post_eps is None else post_eps), float(residual_scale), _native.DTYPE_CODE[x.dtype],
+            _opt(ws), need, stream)
+    _native.check(status, "peco_gated_norm_backward")
+    return NormGrads(**grads)

@@ -1,0 +1,142 @@
+"""Rotary embedding by positions on several axes, over libpeco_b200.so.
+
+A video token has a position on each of several axes (time, height, width);
+the head dimension is cut into one section per axis and each section's pairs
+turn by its axis's position.  ``rotate`` turns Q and K of an attention call in
+one launch, without tables: the angles come from the token grid, or from
+explicit positions, in 64 bits.  float16, bfloat16 and float32, any strides.
+Differentiable (the gradient is the inverse turn).  CUDA tensors only; work is
+enqueued on the current stream.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _native
+
+_POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+
+def _check(q, k, axes, theta, grid, positions):
+    if not isinstance(q, torch.Tensor) or q.dim() != 4:
+        raise ValueError("Expected q [B, H, N, D]")
+    b, _, n, d = q.shape
+    if q.dtype not in _native.DTYPE_CODE:
+        raise TypeError("rotate takes float16, bfloat16 or float32 tensors")
+    if k is not None:
+        if k.dim() != 4 or (k.shape[0], k.shape[2], k.shape[3]) != (b, n, d):
+            raise ValueError("q and k must agree in batch, tokens and head dimension")
+        if k.dtype != q.dtype:
+            raise TypeError("q and k must have one dtype")
+    if d % 2 or not 2 <= d <= 256:
+        raise ValueError("the head dimension must be even and at most 256")
+    axes = tuple(int(a) for a in axes)
+    if not 1 <= len(axes) <= 4 or any(a < 0 or a % 2 for a in axes) or sum(axes) > d:
+        raise ValueError("axes must be one to four even section sizes that fit the head dimension")
+    if not (theta > 0 and math.isfinite(theta)):
+        raise ValueError("theta must be positive")
+    if (grid is None) == (positions is None):
+        raise ValueError("give either grid or positions")
+    if grid is not None:
+        grid = tuple(int(s) for s in grid)
+        if len(grid) != len(axes) or any(s < 0 for s in grid):
+            raise ValueError("grid must have one size per axis")
+        turned = math.prod(grid)
+    else:
+        if positions.dtype not in _POSITION_TYPES:
+            raise TypeError("positions must be int32, int64 or float32")
+        if positions.dim() not in (2, 3) or positions.shape[-1] != len(axes) or \
+                positions.dim() == 3 and positions.shape[0] not in (1, b):
+            raise ValueError("positions must be [tokens, axes] or [B, tokens, axes]")
+        turned = positions.shape[-2]
+    if turned > n:
+        raise ValueError(f"{turned} positions for {n} tokens")
+    _native.require_cuda(*[t for t in (q, k, positions) if t is not None])
+    return axes, grid, turned
+
+
+def _run(q, k, axes, theta, grid, positions, interleaved, inverse, inplace):
+    axes, grid, turned = _check(q, k, axes, theta, grid, positions)
+    b, _, n, d = q.shape
+    sources, outs, strides = [], [], []
+    for t in (q, k):
+        if t is None:
+            sources.append(None), outs.append(None), strides.append(None)
+            continue
+        if inplace and (t.stride(3) != 1 or any(s == 0 for s, m in zip(t.stride(), t.shape) if m > 1)):
+            raise ValueError("inplace needs adjacent head dimensions and no expanded axes")
+        src = t if t.stride(3) == 1 else t.contiguous()
+        out = t if inplace else torch.empty_like(src)  # keeps a dense layout (token-major views stay so)
+        if out.stride(3) != 1 and d > 1:
+            out = torch.empty(src.shape, dtype=src.dtype, device=src.device)
+        sources.append(src), outs.append(out)
+        strides.append((ctypes.c_longlong * 6)(*src.stride()[:3], *out.stride()[:3]))
+    pos_sb = pos_sn = pos_type = 0
+    if positions is not None:
+        if positions.stride(-1) != 1 and len(axes) > 1:
+            positions = positions.contiguous()
+        pos_type, pos_sn = _POSITION_TYPES[positions.dtype], positions.stride(-2)
+        pos_sb = positions.stride(0) if positions.dim() == 3 and positions.shape[0] > 1 else 0
+        if turned == 0:
+            positions, grid = None, (0,) * len(axes)
+    lib = _native.load()
+    dev = q.device
+    null = _native.P(0)
+    with torch.cuda.device(dev):
+        stream = _native.stream_of(dev, *sources, *outs, positions)
+        args = []
+        for src, out, st in zip(sources, outs, strides):
+            args += [null, null, 0, null] if src is None else [_native.ptr(src), _native.ptr(out), src.shape[1], st]
+        status = lib.peco_rotary(*args, b, n, turned, d, (ctypes.c_int * len(axes))(*axes), len(axes), float(theta),
+                                 (ctypes.c_int * len(axes))(*grid) if grid is not None else null,
+                                 _native.ptr(positions), pos_sb, pos_sn, pos_type, int(bool(interleaved)),
+                                 int(bool(inverse)), _native.DTYPE_CODE[q.dtype], stream)
+    _native.check(status, "peco_rotary")
+    return outs
+
+
+class _Rotate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, options):
+        ctx.options = options
+        ctx.set_materialize_grads(False)
+        q, k = _run(q, k, **options, inplace=False)
+        return q if k is None else (q, k)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        back = dict(ctx.options, inverse=not ctx.options["inverse"])
+        gq, gk = (*grads, None)[:2]
+        if gq is None and gk is None:
+            return None, None, None
+        if gq is None:
+            gk, _ = _run(gk, None, **back, inplace=False)
+        else:
+            gq, gk = _run(gq, gk, **back, inplace=False)
+        return gq, gk, None
+
+
+def rotate(q, k=None, *, axes, theta=256.0, grid=None, positions=None, interleaved=True, inverse=False,
+           inplace=False):
+    """q [B, H, N, D] (and k [B, Hk, N, D], H and Hk free) turned by their tokens' positions.
+
+    ``axes``: dimensions of each axis's section, in order, e.g. (16, 56, 56);
+    dimensions after them are copied.  ``grid``: sizes of a row-major token
+    grid that the first prod(grid) rows walk; or ``positions`` [N', axes] /
+    [B, N', axes] (int32, int64 or float32) of the first N' rows.  Later rows
+    (the text) are copied.  ``interleaved``: pairs (2i, 2i+1), else one from
+    each half of the rotated dimensions.  Angles are position * theta^(-2j/d).
+    ``inverse``: the opposite turn.  ``inplace`` (not under autograd)
+    overwrites q and k.  Returns q, or (q, k).
+    """
+    options = dict(axes=axes, theta=theta, grid=grid, positions=positions, interleaved=interleaved, inverse=inverse)
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k)):
+        if inplace:
+            raise RuntimeError("rotate(inplace=True) does not record gradients; use torch.no_grad()")
+        return _Rotate.apply(q, k, options)
+    q, k = _run(q, k, **options, inplace=inplace)
+    return q if k is None else (q, k)
