@@ -27,7 +27,8 @@ enum Activation : int { kActNone = 0, kActGeluTanh = 1, kActGelu = 2, kActSilu =
 
 constexpr int kTileM = 128;
 constexpr int kTileK = 64;   // one 128-byte swizzle panel of 16-bit elements
-constexpr int kGemmThreads = 192;  // TMA warp, MMA warp, four epilogue warps
+constexpr int kEpilogueWarps = 8;
+constexpr int kGemmThreads = 64 + 32 * kEpilogueWarps;  // TMA warp, MMA warp, epilogue warps
 
 struct GemmArgs {
   CUtensorMap a[2], b[2];    // K segments (x and x2; the second unused otherwise)
@@ -85,19 +86,105 @@ __device__ __forceinline__ float2 activate_slope(float z, int act) {
   }
 }
 
+// ---- CTA pairs -------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// address of the same shared-memory location in CTA ``rank`` of the cluster
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void tile_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  if constexpr (CG == 1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+  } else {  // the barrier may be the pair's first CTA's
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+  }
+}
+
+template <int CG>
+__device__ __forceinline__ void product_step(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CG == 1) {
+    umma_ss(d, a, b, idesc, accumulate);
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+
+// Arrive on ``bar`` (of both CTAs of a pair) once the products issued so far are done.
+template <int CG>
+__device__ __forceinline__ void product_commit(uint64_t* bar) {
+  if constexpr (CG == 1) {
+    umma_commit(bar);
+  } else {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+  }
+}
+
+template <int CG>
+__device__ __forceinline__ void tmem_take(uint32_t* slot, uint32_t cols) {
+  if constexpr (CG == 1) {
+    tmem_alloc(slot, cols);
+    tmem_relinquish();
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
+  if constexpr (CG == 1) tmem_dealloc(addr, cols);
+  else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+}
+
 // ---- the product -----------------------------------------------------------------
-// One CTA per SM walks output tiles of 128 x BN.  Warp 0 streams 64-wide K
-// blocks of A and B through a ring of shared-memory stages, warp 1 issues the
-// MMAs into one of two TMEM accumulators, warps 2-5 read the other one back,
-// apply the epilogue and store, so the epilogue of a tile runs under the MMAs
-// of the next.
-template <int BN>
+// Output tiles of (128 CG) x BN, walked by persistent groups of CG CTAs.  Warp
+// 0 of every CTA streams its 64-wide K blocks of A (128 rows) and B (BN / CG
+// rows) through a ring of shared-memory stages; warp 1 of the group's first
+// CTA issues the MMAs into one of two TMEM accumulators; warps 2-9 read the
+// other one back, apply the epilogue and store, so the epilogue of a tile runs
+// under the MMAs of the next.
+//
+// CG = 2 pairs two SMs on one 256 x 256 tile: each CTA stages half of A's rows
+// and half of B's, so a K block costs 32 KB of shared memory and of TMA traffic
+// per SM for twice the products of a 128 x 128 tile.
+template <int CG, int BN>
 struct GemmLayout {
+  static constexpr int kBRows = BN / CG;
   static constexpr int kABytes = kTileM * kTileK * 2;
-  static constexpr int kBBytes = BN * kTileK * 2;
+  static constexpr int kBBytes = kBRows * kTileK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = 6;
+  static constexpr int kStages = 192 * 1024 / kStageBytes;
   static constexpr int kSmem = kStages * kStageBytes + 1024;  // + alignment slack
+  static constexpr int kTmemCols = 2 * BN;
 };
 
 template <int STAGES>
@@ -121,15 +208,15 @@ __device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int
   tn = in / height;
 }
 
-// 128 (or BN) x 64 operand tile into shared memory: K-major rows of 128
-// bytes, or MN-major panels of 64 elements x 64 K rows
-template <bool MN, int ROWS>
-__device__ __forceinline__ void load_tile(unsigned char* dst, const CUtensorMap* map, int row0, int kb, uint64_t* bar) {
-  if (!MN) {
-    tma_load_2d(dst, map, kb * kTileK, row0, bar);
+// ROWS x 64 operand tile into shared memory: K-major rows of 128 bytes, or
+// MN-major panels of 64 elements x 64 K rows
+template <int CG, bool MN, int ROWS>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int row0, int kb, uint32_t bar) {
+  if constexpr (!MN) {
+    tile_load_2d<CG>(dst, map, kb * kTileK, row0, bar);
   } else {
 #pragma unroll
-    for (int p = 0; p < ROWS / 64; ++p) tma_load_2d(dst + p * 8192, map, row0 + p * 64, kb * kTileK, bar);
+    for (int p = 0; p < ROWS / 64; ++p) tile_load_2d<CG>(dst + p * 8192, map, row0 + p * 64, kb * kTileK, bar);
   }
 }
 
@@ -139,14 +226,78 @@ __device__ __forceinline__ uint64_t step_desc(uint32_t base, int k) {
   return MN ? smem_desc(base + k * 2048, 8192, 1024) : smem_desc(base + k * 32, 16, 1024);
 }
 
-template <typename T, int BN, bool AMN, bool BMN, bool EPI>
+// Epilogue of 32 columns of one row; ``count`` of them exist.
+template <typename T, bool EPI>
+__device__ __forceinline__ void finish_row(const GemmArgs& args, const uint32_t (&acc)[32], long long row, int col0,
+                                           const T* gate) {
+#pragma unroll
+  for (int j = 0; j < 32; j += 8) {
+    const int col = col0 + j;
+    const int count = min(8, args.n - col);
+    if (count <= 0) break;
+    float v[8], res[8], e[8];
+    if (EPI && args.residual)
+      load_vec<8>(static_cast<const T*>(args.residual) + row * args.res_stride + col, args.vec, count, res);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(acc[j + i]);
+    if (EPI) {
+      if (args.bias) {
+        load_vec<8>(static_cast<const T*>(args.bias) + col, args.vec, count, e);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += e[i];
+      }
+      if (args.preact) store_vec<8>(static_cast<T*>(args.preact) + row * args.n + col, args.vec, count, v);
+      switch (args.act) {
+        case kActGeluTanh:
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = activate(v[i], kActGeluTanh);
+          break;
+        case kActGelu:
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = activate(v[i], kActGelu);
+          break;
+        case kActSilu:
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = activate(v[i], kActSilu);
+          break;
+        default: break;
+      }
+      if (gate) {
+        load_vec<8>(gate + col, args.vec, count, e);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= e[i];
+      }
+      if (args.residual) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += res[i];
+      }
+    }
+    store_vec<8>(static_cast<T*>(args.out) + row * args.out_stride + col, args.vec, count, v);
+  }
+}
+
+// 32 TMEM columns per lane; the values may be read after tmem_ld_wait_for
+__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
+// Waits for the loads in flight and ties ``r`` to the wait, so that no use of
+// it is scheduled earlier.
+__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])::"memory");
+}
+
+template <typename T, int CG, int BN, bool AMN, bool BMN, bool EPI>
 __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmArgs args) {
-  using L = GemmLayout<BN>;
+  using L = GemmLayout<CG, BN>;
   constexpr int kStages = L::kStages;
   extern __shared__ unsigned char smem_raw[];
   __shared__ GemmShared<kStages> sh;
-  unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 1 ? 0 : cluster_rank();
   volatile int* abort_flag = &sh.abort_flag;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -155,58 +306,60 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sh.acc_full[b], 1);
-      mbar_init(&sh.acc_empty[b], 4);
+      mbar_init(&sh.acc_empty[b], CG * kEpilogueWarps);
     }
     sh.abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 1) {
-    tmem_alloc(&sh.tmem, 2 * BN);
-    tmem_relinquish();
-  }
+  if (warp == 1) tmem_take<CG>(&sh.tmem, L::kTmemCols);
   tc_fence_before();
   __syncthreads();
+  if (CG > 1) cluster_sync();  // the pair's barriers are ready before either CTA signals the other
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
   const int tiles = args.tiles_m * args.tiles_n;
   const int kb0 = args.kblocks[0], kblocks = kb0 + args.kblocks[1];
+  const int group = blockIdx.x / CG, groups = gridDim.x / CG;
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA
     if (lane == 0) {
       bool ok = true;
       uint32_t it = 0;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      for (int t = group; t < tiles && ok; t += groups) {
         int tm, tn;
         tile_coords(t, args.tiles_m, args.tiles_n, tm, tn);
+        const int row_a = (tm * CG + rank) * kTileM, row_b = tn * BN + rank * L::kBRows;
         for (int kb = 0; kb < kblocks; ++kb, ++it) {
           const int s = it % kStages;
           ok = mbar_wait(&sh.empty[s], ((it / kStages) & 1) ^ 1, abort_flag, args.status);
           if (!ok) break;
-          unsigned char* st = ring + s * L::kStageBytes;
-          mbar_arrive_expect_tx(&sh.full[s], L::kStageBytes);
+          const uint32_t st = ring + s * L::kStageBytes;
+          // the pair's stages fill one barrier, the first CTA's, which expects both CTAs' bytes
+          uint32_t bar = smem_u32(&sh.full[s]);
+          if (CG > 1) bar = map_rank(bar, 0);
+          if (rank == 0) mbar_arrive_expect_tx(&sh.full[s], CG * L::kStageBytes);
           const int seg = kb >= kb0 ? 1 : 0;
           const int kx = kb - (seg ? kb0 : 0);
-          load_tile<AMN, kTileM>(st, &args.a[seg], tm * kTileM, kx, &sh.full[s]);
-          load_tile<BMN, BN>(st + L::kABytes, &args.b[seg], tn * BN, kx, &sh.full[s]);
+          load_tile<CG, AMN, kTileM>(st, &args.a[seg], row_a, kx, bar);
+          load_tile<CG, BMN, L::kBRows>(st + L::kABytes, &args.b[seg], row_b, kx, bar);
         }
       }
-      // after an expired wait: let the copies still in flight land before the CTA ends
+      // after an expired wait: time for the copies still in flight to land before the CTA ends
       if (!ok) {
-        int drained = 0;
-        const uint32_t first = it > kStages ? it - kStages : 0;
-        for (uint32_t i = first; i < it; ++i)
-          mbar_wait(&sh.full[i % kStages], (i / kStages) & 1, &drained, args.status);
+        const unsigned long long t0 = globaltimer();
+        while (globaltimer() - t0 < 2000000ull) {
+        }
       }
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       constexpr int ab = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
-      constexpr uint32_t idesc = instr_desc(kTileM, BN, ab, AMN, BMN);
+      constexpr uint32_t idesc = instr_desc(kTileM * CG, BN, ab, AMN, BMN);
       bool ok = true;
       uint32_t it = 0, local = 0;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++local) {
+      for (int t = group; t < tiles && ok; t += groups, ++local) {
         const int b = local & 1;
         ok = mbar_wait(&sh.acc_empty[b], ((local >> 1) & 1) ^ 1, abort_flag, args.status);
         if (!ok) break;
@@ -216,83 +369,59 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
           ok = mbar_wait(&sh.full[s], (it / kStages) & 1, abort_flag, args.status);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t sa = smem_u32(ring + s * L::kStageBytes), sb = sa + L::kABytes;
+          const uint32_t sa = ring + s * L::kStageBytes, sb = sa + L::kABytes;
 #pragma unroll
           for (int k = 0; k < kTileK / 16; ++k)
-            umma_ss(tmem + b * BN, step_desc<AMN>(sa, k), step_desc<BMN>(sb, k), idesc, (kb | k) ? 1u : 0u);
-          umma_commit(&sh.empty[s]);
+            product_step<CG>(tmem + b * BN, step_desc<AMN>(sa, k), step_desc<BMN>(sb, k), idesc, (kb | k) ? 1u : 0u);
+          product_commit<CG>(&sh.empty[s]);
         }
-        if (ok) umma_commit(&sh.acc_full[b]);
+        if (ok) product_commit<CG>(&sh.acc_full[b]);
       }
     }
   } else {
     // ----------------------------------------------------------- epilogue
-    const int quarter = warp & 3;  // the TMEM lanes this warp may read
+    // two warps per quarter of the TMEM lanes, each half of the columns
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    constexpr int kCols = BN / 2;
     uint32_t local = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++local) {
+    for (int t = group; t < tiles; t += groups, ++local) {
       int tm, tn;
       tile_coords(t, args.tiles_m, args.tiles_n, tm, tn);
       const int b = local & 1;
       if (!mbar_wait_warp(&sh.acc_full[b], (local >> 1) & 1, abort_flag, args.status)) break;
       tc_fence_after();
-      const long long row = static_cast<long long>(tm) * kTileM + quarter * 32 + lane;
+      const long long row = static_cast<long long>(tm * CG + rank) * kTileM + quarter * 32 + lane;
       const bool live = row < args.m;
       const T* gate = nullptr;
       if (EPI && args.gate && live)
         gate = static_cast<const T*>(args.gate) + (row / args.rows_per_sample) * args.gate_stride;
-      for (int c = 0; c < BN; c += 32) {
-        uint32_t acc[32];
-        tmem_ld32_sync(tmem + b * BN + (static_cast<uint32_t>(quarter * 32) << 16) + c, acc);
-        if (live) {
+      const uint32_t src = tmem + b * BN + half * kCols + (static_cast<uint32_t>(quarter * 32) << 16);
+      const int col0 = tn * BN + half * kCols;
+      // the next 32 columns are on their way while these are finished
+      uint32_t acc[2][32];
+      tmem_ld32_start(src, acc[0]);
 #pragma unroll
-          for (int j = 0; j < 32; j += 8) {
-            const int col = tn * BN + c + j;
-            const int count = min(8, args.n - col);
-            if (count > 0) {
-              float v[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(acc[j + i]);
-              if (EPI) {
-                float e[8];
-                if (args.bias) {
-                  load_vec<8>(static_cast<const T*>(args.bias) + col, args.vec, count, e);
-#pragma unroll
-                  for (int i = 0; i < 8; ++i) v[i] += e[i];
-                }
-                if (args.preact)
-                  store_vec<8>(static_cast<T*>(args.preact) + row * args.n + col, args.vec, count, v);
-                if (args.act != kActNone) {
-#pragma unroll
-                  for (int i = 0; i < 8; ++i) v[i] = activate(v[i], args.act);
-                }
-                if (gate) {
-                  load_vec<8>(gate + col, args.vec, count, e);
-#pragma unroll
-                  for (int i = 0; i < 8; ++i) v[i] *= e[i];
-                }
-                if (args.residual) {
-                  load_vec<8>(static_cast<const T*>(args.residual) + row * args.res_stride + col, args.vec, count, e);
-#pragma unroll
-                  for (int i = 0; i < 8; ++i) v[i] += e[i];
-                }
-              }
-              store_vec<8>(static_cast<T*>(args.out) + row * args.out_stride + col, args.vec, count, v);
-            }
-          }
-        }
+      for (int c = 0; c < kCols / 32; ++c) {
+        tmem_ld_wait_for(acc[c & 1]);
+        if (c + 1 < kCols / 32) tmem_ld32_start(src + (c + 1) * 32, acc[(c + 1) & 1]);
+        if (live) finish_row<T, EPI>(args, acc[c & 1], row, col0 + c * 32, gate);
         __syncwarp();
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.acc_empty[b]);
+      if (lane == 0) {
+        if (CG == 1) mbar_arrive(&sh.acc_empty[b]);
+        else arrive_cluster(map_rank(smem_u32(&sh.acc_empty[b]), 0));
+      }
     }
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  if (CG > 1) cluster_sync();  // neither CTA leaves while the other may still signal it
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 2 * BN);
+    tmem_free<CG>(tmem, L::kTmemCols);
   }
 }
 
@@ -442,26 +571,44 @@ bool operand_map(CUtensorMap* map, const Operand& o, bool mn, int tile_rows, int
                            o.ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <typename T, bool AMN, bool BMN, bool EPI>
-int launch_gemm(GemmArgs& g, const Operand* a, const Operand* b, int segments, int dtype, cudaStream_t stream) {
-  constexpr int BN = 128;
-  using L = GemmLayout<BN>;
-  g.tiles_m = (g.m + kTileM - 1) / kTileM;
+template <typename T, int CG, int BN, bool AMN, bool BMN, bool EPI>
+int launch_tiles(GemmArgs& g, const Operand* a, const Operand* b, int segments, int dtype, cudaStream_t stream) {
+  using L = GemmLayout<CG, BN>;
+  g.tiles_m = (g.m + CG * kTileM - 1) / (CG * kTileM);
   g.tiles_n = (g.n + BN - 1) / BN;
   if (static_cast<long long>(g.tiles_m) * g.tiles_n > 0x7fffffffLL) return kErrUnsupported;
   for (int s = 0; s < 2; ++s) {
     const int src = s < segments ? s : 0;
-    if (!operand_map(&g.a[s], a[src], AMN, kTileM, dtype) || !operand_map(&g.b[s], b[src], BMN, BN, dtype))
+    if (!operand_map(&g.a[s], a[src], AMN, kTileM, dtype) || !operand_map(&g.b[s], b[src], BMN, L::kBRows, dtype))
       return kErrTensorMap;
     g.kblocks[s] = s < segments ? ((AMN ? a[s].rows : a[s].cols) + kTileK - 1) / kTileK : 0;
   }
   g.status = device_status_ptr();
-  auto kernel = gemm_kernel<T, BN, AMN, BMN, EPI>;
+  auto kernel = gemm_kernel<T, CG, BN, AMN, BMN, EPI>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
   if (e != cudaSuccess) return static_cast<int>(e);
-  const int tiles = g.tiles_m * g.tiles_n;
-  kernel<<<tiles < kNumSMs ? tiles : kNumSMs, kGemmThreads, L::kSmem, stream>>>(g);
-  return launch_status();
+  const int tiles = g.tiles_m * g.tiles_n, most = kNumSMs / CG;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((tiles < most ? tiles : most) * CG);
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = L::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kernel, g);
+  const int st = launch_status();
+  return e != cudaSuccess ? static_cast<int>(e) : st;
+}
+
+template <typename T, bool AMN, bool BMN, bool EPI>
+int launch_gemm(GemmArgs& g, const Operand* a, const Operand* b, int segments, int dtype, cudaStream_t stream) {
+  const long long big = static_cast<long long>((g.m + 255) / 256) * ((g.n + 255) / 256);
+  if (big >= 37) return launch_tiles<T, 2, 256, AMN, BMN, EPI>(g, a, b, segments, dtype, stream);
+  return launch_tiles<T, 1, 128, AMN, BMN, EPI>(g, a, b, segments, dtype, stream);
 }
 
 bool aligned16(const void* p, long long stride) {
