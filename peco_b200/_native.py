@@ -128,6 +128,35 @@ def stream_of(device: torch.device, *tensors: torch.Tensor) -> P:
     return P(s.cuda_stream)
 
 
+_STREAMS = {}  # (device index, raw stream) -> torch stream object
+
+
+def enqueue(device: torch.device, what: str, fn, args, inputs) -> None:
+    """Call ``fn(*args, stream)`` on the current stream of ``device`` and raise on
+    a non-zero status.  Pointers in ``args`` are plain integers.  ``inputs`` are
+    the caller's tensors (None skipped): their memory stays theirs until the
+    stream has consumed it.  Buffers that were allocated for this call belong to
+    the stream already."""
+    raw = torch._C._cuda_getCurrentRawStream(device.index)
+    stream = _STREAMS.get((device.index, raw))
+    if stream is None:  # building the stream object costs more than the look-up
+        stream = _STREAMS[device.index, raw] = torch.cuda.current_stream(device)
+    for t in inputs:
+        if t is not None:
+            t.record_stream(stream)
+    if device.index == torch._C._cuda_getDevice():
+        status = fn(*args, raw)
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, raw)
+    if status:
+        check(status, what)
+
+
+def address(t: torch.Tensor | None) -> int:
+    return t.data_ptr() if t is not None else 0
+
+
 def ptr(t: torch.Tensor | None) -> P:
     return P(t.data_ptr() if t is not None else 0)
 

@@ -18,6 +18,7 @@
 #include "internal.h"
 #include "rows.cuh"
 
+#include <atomic>
 #include <type_traits>
 
 namespace peco {
@@ -453,7 +454,7 @@ struct ActBackwardArgs {
   int act, vec;
 };
 
-template <typename T>
+template <typename T, int ACT>
 __global__ void __launch_bounds__(256) act_backward_kernel(const ActBackwardArgs a) {
   __shared__ float red[2][8][256];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -469,25 +470,39 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const ActBackwardArgs
   if (count > 0) {
     if (a.gate) load_vec<8>(static_cast<const T*>(a.gate) + sample * a.gate_stride + col, a.vec, count, gate);
     const int begin = chunk * a.chunk_rows, end = min(begin + a.chunk_rows, a.rows_per_sample);
-    for (int r = begin + warp; r < end; r += 8) {
-      const long long row = static_cast<long long>(sample) * a.rows_per_sample + r;
-      float g[8], z[8], dz[8];
-      load_vec<8>(static_cast<const T*>(a.grad) + row * a.grad_stride + col, a.vec, count, g);
-      if (a.preact) load_vec<8>(static_cast<const T*>(a.preact) + row * a.n + col, a.vec, count, z);
+    const long long row0 = static_cast<long long>(sample) * a.rows_per_sample;
+    // two of the warp's rows in flight
+    for (int r = begin + warp; r < end; r += 16) {
+      float g[2][8], z[2][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        dz[i] = g[i] * gate[i];
-        if (a.preact) {
-          const float2 f = activate_slope(z[i], a.act);
-          dz[i] *= f.y;
-          sum_ga[i] = fmaf(g[i], f.x, sum_ga[i]);
+      for (int j = 0; j < 2; ++j) {
+        if (r + 8 * j < end) {
+          const long long row = row0 + r + 8 * j;
+          load_vec<8>(static_cast<const T*>(a.grad) + row * a.grad_stride + col, a.vec, count, g[j]);
+          if (a.preact) load_vec<8>(static_cast<const T*>(a.preact) + row * a.n + col, a.vec, count, z[j]);
         }
-        sum_dz[i] += dz[i];
       }
-      // dz is rounded to the operands' type for the tensor core; its sums are not
-      if (a.dz) store_vec<8>(static_cast<T*>(a.dz) + row * a.dz_stride + col, a.vec, count, dz);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (r + 8 * j < end) {
+          float dz[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            dz[i] = g[j][i] * gate[i];
+            if (a.preact) {
+              const float2 f = activate_slope(z[j][i], ACT);
+              dz[i] *= f.y;
+              sum_ga[i] = fmaf(g[j][i], f.x, sum_ga[i]);
+            }
+            sum_dz[i] += dz[i];
+          }
+          // dz is rounded to the operands' type for the tensor core; its sums are not
+          if (a.dz) store_vec<8>(static_cast<T*>(a.dz) + (row0 + r + 8 * j) * a.dz_stride + col, a.vec, count, dz);
+        }
+      }
     }
   }
+  if (!a.part_bias && !a.part_gate) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     red[0][warp][lane * 8 + i] = sum_dz[i];
@@ -508,22 +523,39 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const ActBackwardArgs
   }
 }
 
+// Sums of the chunks: 32 columns x 8 lanes of chunks per block, the lanes'
+// sums added in order, sample after sample.
 template <typename T>
 __global__ void __launch_bounds__(256) act_backward_sums_kernel(const float* part_bias, const float* part_gate,
                                                                 T* dbias, T* dgate, int samples, int chunks, int n) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= n) return;
+  __shared__ float red[2][8][33];
+  const int cx = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + cx;
   float total = 0.0f;
   for (int b = 0; b < samples; ++b) {
-    float gsum = 0.0f;
-    for (int i = 0; i < chunks; ++i) {
-      const long long at = (static_cast<long long>(b) * chunks + i) * n + c;
-      if (dbias) total += part_bias[at];
-      if (dgate) gsum += part_gate[at];
+    float s[2] = {0.0f, 0.0f};
+    if (c < n) {
+#pragma unroll 4
+      for (int i = y; i < chunks; i += 8) {
+        const long long at = (static_cast<long long>(b) * chunks + i) * n + c;
+        if (part_bias) s[0] += part_bias[at];
+        if (part_gate) s[1] += part_gate[at];
+      }
     }
-    if (dgate) dgate[static_cast<long long>(b) * n + c] = from_f32<T>(gsum);
+    red[0][y][cx] = s[0];
+    red[1][y][cx] = s[1];
+    __syncthreads();
+    if (y == 0 && c < n) {
+      float g = 0.0f;
+      for (int i = 0; i < 8; ++i) {
+        total += red[0][i][cx];
+        g += red[1][i][cx];
+      }
+      if (dgate) dgate[static_cast<long long>(b) * n + c] = from_f32<T>(g);
+    }
+    __syncthreads();
   }
-  if (dbias) dbias[c] = from_f32<T>(total);
+  if (dbias && y == 0 && c < n) dbias[c] = from_f32<T>(total);
 }
 
 // ---- host side --------------------------------------------------------------------------
@@ -571,21 +603,33 @@ bool operand_map(CUtensorMap* map, const Operand& o, bool mn, int tile_rows, int
                            o.ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// Dynamic shared memory of a kernel, granted once per device.
+cudaError_t grant_smem(const void* kernel, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
 template <typename T, int CG, int BN, bool AMN, bool BMN, bool EPI>
 int launch_tiles(GemmArgs& g, const Operand* a, const Operand* b, int segments, int dtype, cudaStream_t stream) {
   using L = GemmLayout<CG, BN>;
   g.tiles_m = (g.m + CG * kTileM - 1) / (CG * kTileM);
   g.tiles_n = (g.n + BN - 1) / BN;
   if (static_cast<long long>(g.tiles_m) * g.tiles_n > 0x7fffffffLL) return kErrUnsupported;
-  for (int s = 0; s < 2; ++s) {
-    const int src = s < segments ? s : 0;
-    if (!operand_map(&g.a[s], a[src], AMN, kTileM, dtype) || !operand_map(&g.b[s], b[src], BMN, L::kBRows, dtype))
+  for (int s = 0; s < segments; ++s) {
+    if (!operand_map(&g.a[s], a[s], AMN, kTileM, dtype) || !operand_map(&g.b[s], b[s], BMN, L::kBRows, dtype))
       return kErrTensorMap;
-    g.kblocks[s] = s < segments ? ((AMN ? a[s].rows : a[s].cols) + kTileK - 1) / kTileK : 0;
+    g.kblocks[s] = ((AMN ? a[s].rows : a[s].cols) + kTileK - 1) / kTileK;
   }
   g.status = device_status_ptr();
   auto kernel = gemm_kernel<T, CG, BN, AMN, BMN, EPI>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+  static std::atomic<unsigned long long> opened{0};  // devices whose kernel has its shared memory granted
+  cudaError_t e = grant_smem(reinterpret_cast<const void*>(kernel), L::kSmem, opened);
   if (e != cudaSuccess) return static_cast<int>(e);
   const int tiles = g.tiles_m * g.tiles_n, most = kNumSMs / CG;
   cudaLaunchConfig_t cfg{};
@@ -637,13 +681,16 @@ int forward(const LinearShape& s, Operand (&a)[2], Operand (&b)[2], GemmArgs& g,
   return launch_gemm<T, false, false, true>(g, a, b, segments, s.dtype, stream);
 }
 
-// Row chunks per sample of the epilogue's gradient: enough blocks for four per SM
+// Row chunks per sample of the epilogue's gradient: 64 rows each (short enough
+// that the last blocks of the launch cost little, long enough that the sums
+// written per chunk stay under 2% of the rows' traffic), shorter when that
+// leaves SMs without a block
 int backward_chunks(const LinearShape& s) {
   if (s.samples < 1) return 1;
   const long long blocks = static_cast<long long>((s.n + 255) / 256) * s.samples;
-  long long chunks = (4LL * kNumSMs + blocks - 1) / blocks;
-  const long long most = (s.rows_per_sample + 15) / 16;
-  if (chunks > most) chunks = most;
+  long long chunks = (s.rows_per_sample + 63) / 64;
+  const long long fill = (4LL * kNumSMs + blocks - 1) / blocks, most = (s.rows_per_sample + 15) / 16;
+  if (chunks < fill) chunks = fill < most ? fill : most;
   const long long cap = 65535 / s.samples;
   if (chunks > cap) chunks = cap;
   return chunks < 1 ? 1 : static_cast<int>(chunks);
@@ -695,10 +742,15 @@ int backward(const LinearShape& s, Operand grad, const void* preact, Operand (&x
     a.act = s.act;
     a.vec = s.n % 8 == 0 && aligned16(grad.ptr, grad.stride) && aligned16(a.preact, s.n) && aligned16(gate, gate_stride);
     const dim3 grid((s.n + 255) / 256, s.samples * p.chunks);
-    act_backward_kernel<T><<<grid, 256, 0, stream>>>(a);
+    switch (s.act) {
+      case kActGeluTanh: act_backward_kernel<T, kActGeluTanh><<<grid, 256, 0, stream>>>(a); break;
+      case kActGelu: act_backward_kernel<T, kActGelu><<<grid, 256, 0, stream>>>(a); break;
+      case kActSilu: act_backward_kernel<T, kActSilu><<<grid, 256, 0, stream>>>(a); break;
+      default: act_backward_kernel<T, kActNone><<<grid, 256, 0, stream>>>(a);
+    }
     if (int st = launch_status()) return st;
     if (p.sums) {
-      act_backward_sums_kernel<T><<<(s.n + 255) / 256, 256, 0, stream>>>(
+      act_backward_sums_kernel<T><<<(s.n + 31) / 32, 256, 0, stream>>>(
           a.part_bias, a.part_gate, static_cast<T*>(dbias), static_cast<T*>(dgate), s.samples, p.chunks, s.n);
       if (int st = launch_status()) return st;
     }

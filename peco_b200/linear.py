@@ -47,43 +47,44 @@ def _stride(t: Optional[torch.Tensor]) -> int:
     return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
 
 
-def _opt(t: Optional[torch.Tensor]):
-    return _native.ptr(t) if t is not None else _native.P(0)
-
-
 def _check(x, weight, bias, gate, residual, x2, activation):
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
     if not isinstance(x, torch.Tensor) or not isinstance(weight, torch.Tensor):
         raise TypeError("x and weight must be torch tensors")
-    there = [t for t in (x, weight, bias, gate, residual, x2) if t is not None]
-    if x.dtype not in (torch.float16, torch.bfloat16) or any(t.dtype != x.dtype for t in there):
+    dtype, device = x.dtype, x.device
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise TypeError("linear_act takes float16 or bfloat16 tensors of one dtype")
+    for t in (weight, bias, gate, residual, x2):
+        if t is not None and t.dtype is not dtype:
+            raise TypeError("linear_act takes float16 or bfloat16 tensors of one dtype")
     if x.dim() < 1 or weight.dim() != 2:
         raise ValueError("Expected x [..., K] and weight [N, K + K2]")
-    k, k2 = x.shape[-1], 0 if x2 is None else x2.shape[-1]
-    if x2 is not None and x2.shape[:-1] != x.shape[:-1]:
-        raise ValueError("x and x2 must have the same leading shape")
-    if x2 is not None and k2 < 1:
-        raise ValueError("x2 must have at least one feature")
-    if k < 1 or weight.shape[0] < 1 or weight.shape[1] != k + k2:
+    shape = x.shape
+    n, wide = weight.shape
+    k, k2 = shape[-1], 0
+    if x2 is not None:
+        k2 = x2.shape[-1]
+        if x2.shape[:-1] != shape[:-1]:
+            raise ValueError("x and x2 must have the same leading shape")
+        if k2 < 1:
+            raise ValueError("x2 must have at least one feature")
+    if k < 1 or n < 1 or wide != k + k2:
         raise ValueError(f"weight must be [N, {k + k2}] for these inputs, got {list(weight.shape)}")
-    n = weight.shape[0]
     if bias is not None and bias.shape != (n,):
         raise ValueError(f"bias must be [{n}]")
     samples = 1
-    if gate is not None:
-        shape = tuple(gate.shape)
-        lead = x.shape[0] if x.dim() >= 3 else 1
-        if shape == (n,):
-            samples = 1
-        elif shape in ((lead, n), (lead, 1, n)):
-            samples = lead
-        else:
-            raise ValueError(f"gate must be [{n}] or one row for each of the {lead} samples, got {list(shape)}")
-    if residual is not None and residual.shape != (*x.shape[:-1], n):
-        raise ValueError(f"residual must have the output's shape {[*x.shape[:-1], n]}")
-    _native.require_cuda(*there)
+    if gate is not None and gate.shape != (n,):
+        samples = shape[0] if len(shape) >= 3 else 1
+        if tuple(gate.shape) not in ((samples, n), (samples, 1, n)):
+            raise ValueError(f"gate must be [{n}] or one row for each of the {samples} samples, got {list(gate.shape)}")
+    if residual is not None and residual.shape != (*shape[:-1], n):
+        raise ValueError(f"residual must have the output's shape {[*shape[:-1], n]}")
+    if device.type != "cuda":
+        _native.require_cuda(x)
+    for t in (weight, bias, gate, residual, x2):
+        if t is not None and t.device != device:
+            _native.require_cuda(x, t)
     return k, k2, n, samples
 
 
@@ -117,18 +118,18 @@ def _forward(x, weight, bias, gate, residual, x2, activation, out, want_preact):
     gates = _gate_rows(gate, n)
     bias = None if bias is None else bias.contiguous()
     lib = _native.load()
-    dev = x.device
-    operands = (_native.ptr(xf), _stride(xf), _opt(x2f), _stride(x2f), _native.ptr(w), _stride(w))
+    dev, addr = x.device, _native.address
+    operands = (addr(xf), _stride(xf), addr(x2f), _stride(x2f), addr(w), _stride(w))
     sizes = (samples, rows // samples, k, k2, n)
-    need = int(lib.peco_linear_forward_workspace(*operands, *sizes))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-    with torch.cuda.device(dev):
-        stream = _native.stream_of(dev, xf, x2f, w, bias, gates, res, out, preact, ws)
-        status = lib.peco_linear_forward(*operands, _opt(bias), _opt(gates), gates.stride(0) if samples > 1 else 0,
-                                         _opt(res), _stride(res), _native.ptr(out_rows), _stride(out_rows),
-                                         _opt(preact), *sizes, ACTIVATIONS[activation], _native.DTYPE_CODE[x.dtype],
-                                         _opt(ws), max(need, 0), stream)
-    _native.check(status, "peco_linear_forward")
+    need, ws = 0, None
+    if (operands[0] | operands[2] | operands[4]) & 15 or (operands[1] | operands[3] | operands[5] | (k if k2 else 0)) & 7:
+        # some operand may not start every row on 16 bytes
+        need = int(lib.peco_linear_forward_workspace(*operands, *sizes))
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    _native.enqueue(dev, "peco_linear_forward", lib.peco_linear_forward,
+                    (*operands, addr(bias), addr(gates), gates.stride(0) if samples > 1 else 0, addr(res), _stride(res),
+                     out_rows.data_ptr(), _stride(out_rows), addr(preact), *sizes, ACTIVATIONS[activation],
+                     _native.DTYPE_CODE[x.dtype], addr(ws), max(need, 0)), (xf, x2f, w, bias, gates, res, out))
     return out, preact
 
 
@@ -210,16 +211,13 @@ def linear_act_backward(grad, x, weight, *, preact=None, activation=None, gate=N
     g, xf, x2f, gates = _flat(grad), _flat(x), None if x2 is None else _flat(x2), _gate_rows(gate, n)
     w = weight if weight.stride(1) == 1 and weight.stride(0) >= weight.shape[1] else weight.contiguous()
     lib = _native.load()
-    dev = x.device
-    operands = (_native.ptr(xf), _stride(xf), _opt(x2f), _stride(x2f), _native.ptr(w), _stride(w))
+    dev, addr = x.device, _native.address
+    operands = (addr(xf), _stride(xf), addr(x2f), _stride(x2f), addr(w), _stride(w))
     sizes = (samples, rows // samples, k, k2, n, act)
-    need = int(lib.peco_linear_backward_workspace(_native.ptr(g), _stride(g), *operands, *sizes, int(gate is not None)))
+    need = int(lib.peco_linear_backward_workspace(addr(g), _stride(g), *operands, *sizes, int(gate is not None)))
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-    with torch.cuda.device(dev):
-        stream = _native.stream_of(dev, g, preact, xf, x2f, w, gates, ws, *outs.values())
-        status = lib.peco_linear_backward(_native.ptr(g), _stride(g), _opt(preact), *operands, _opt(gates),
-                                          gates.stride(0) if samples > 1 else 0, _opt(outs["x"]), _opt(outs["x2"]),
-                                          _opt(outs["weight"]), _opt(outs["bias"]), _opt(outs["gate"]), *sizes,
-                                          _native.DTYPE_CODE[x.dtype], _opt(ws), max(need, 0), stream)
-    _native.check(status, "peco_linear_backward")
+    _native.enqueue(dev, "peco_linear_backward", lib.peco_linear_backward,
+                    (addr(g), _stride(g), addr(preact), *operands, addr(gates), gates.stride(0) if samples > 1 else 0,
+                     *(addr(outs[f]) for f in ("x", "x2", "weight", "bias", "gate")), *sizes,
+                     _native.DTYPE_CODE[x.dtype], addr(ws), max(need, 0)), (g, preact, xf, x2f, w, gates))
     return LinearGrads(**outs)

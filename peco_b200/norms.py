@@ -36,10 +36,6 @@ class NormGrads(NamedTuple):
     post_weight: Optional[torch.Tensor]
 
 
-def _opt(t):
-    return _native.ptr(t) if t is not None else _native.P(0)
-
-
 def _rows(t, width):
     """(tensor, batch stride, row stride) of [B, T, C] rows with adjacent columns."""
     if t is None:
@@ -76,9 +72,17 @@ def _check(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, 
         raise ValueError(f'post_norm must be None, "layer" or "rms", got {post_norm!r}')
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         raise TypeError("x must be a torch tensor [..., C]")
-    there = [t for t in (x, branch, gate, scale, shift, weight, post_weight) if t is not None]
-    if x.dtype not in (torch.float16, torch.bfloat16) or any(t.dtype != x.dtype for t in there):
+    dtype, device = x.dtype, x.device
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise TypeError("modulated_norm takes float16 or bfloat16 tensors of one dtype")
+    if device.type != "cuda":
+        _native.require_cuda(x)
+    for t in (branch, gate, scale, shift, weight, post_weight):
+        if t is not None:
+            if t.dtype is not dtype:
+                raise TypeError("modulated_norm takes float16 or bfloat16 tensors of one dtype")
+            if t.device != device:
+                _native.require_cuda(x, t)
     c = x.shape[-1]
     if not 1 <= c <= 16384:
         raise ValueError("modulated_norm takes 1 to 16384 features")
@@ -97,7 +101,6 @@ def _check(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, 
             raise ValueError(f"{name} must be [{c}]")
     if not eps >= 0 or not abs(residual_scale) < float("inf"):
         raise ValueError("eps must be nonnegative and residual_scale finite")
-    _native.require_cuda(*there)
 
 
 def _forward(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, eps, post_eps, residual_scale):
@@ -111,16 +114,12 @@ def _forward(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm
     b3, bb, br = _rows(_as3(branch), c)
     (gate, gb), (scale, sb), (shift, tb) = (_vec(t, c) for t in (gate, scale, shift))
     weight, post_weight = (None if t is None else t.contiguous() for t in (weight, post_weight))
-    lib = _native.load()
-    dev = x.device
-    with torch.cuda.device(dev):
-        stream = _native.stream_of(dev, x3, b3, gate, scale, shift, weight, post_weight, residual, normed)
-        status = lib.peco_gated_norm(_native.ptr(x3), xb, xr, _opt(b3), bb, br, _opt(gate), gb, _opt(scale), sb,
-                                     _opt(shift), tb, _opt(weight), _opt(post_weight), _opt(residual),
-                                     _native.ptr(normed), x3.shape[0], x3.shape[1], c, NORMS[norm], NORMS[post_norm],
-                                     float(eps), float(eps if post_eps is None else post_eps), float(residual_scale),
-                                     _native.DTYPE_CODE[x.dtype], stream)
-    _native.check(status, "peco_gated_norm")
+    addr = _native.address
+    _native.enqueue(x.device, "peco_gated_norm", _native.load().peco_gated_norm,
+                    (x3.data_ptr(), xb, xr, addr(b3), bb, br, addr(gate), gb, addr(scale), sb, addr(shift), tb,
+                     addr(weight), addr(post_weight), addr(residual), normed.data_ptr(), x3.shape[0], x3.shape[1], c,
+                     NORMS[norm], NORMS[post_norm], eps, eps if post_eps is None else post_eps, residual_scale,
+                     _native.DTYPE_CODE[x.dtype]), (x3, b3, gate, scale, shift, weight, post_weight))
     return residual, normed
 
 
@@ -198,19 +197,16 @@ def modulated_norm_backward(grad_normed, grad_residual, x, branch=None, *, gate=
     (gv, gb), (sv, sb) = _vec(gate, c), _vec(scale, c)
     weight, post_weight = (None if t is None else t.contiguous() for t in (weight, post_weight))
     lib = _native.load()
-    dev = x.device
+    dev, addr = x.device, _native.address
     need, ws = 0, None
     if any(n in needs for n in NormGrads._fields[2:]):
         need = int(lib.peco_gated_norm_backward_workspace(x3.shape[0], x3.shape[1], c))
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        stream = _native.stream_of(dev, gh, gr, x3, b3, gv, sv, weight, post_weight, ws, *grads.values())
-        status = lib.peco_gated_norm_backward(
-            _native.ptr(gh), ghb, ghr, _opt(gr), grb, grr, _native.ptr(x3), xb, xr, _opt(b3), bb, br, _opt(gv), gb,
-            _opt(sv), sb, _opt(weight), _opt(post_weight), _opt(grads["x"]), _opt(grads["branch"]),
-            _opt(grads["gate"]), _opt(grads["scale"]), _opt(grads["shift"]), shared, _opt(grads["weight"]),
-            _opt(grads["post_weight"]), x3.shape[0], x3.shape[1], c, NORMS[norm], NORMS[post_norm], float(eps),
-            float(eps if post_eps is None else post_eps), float(residual_scale), _native.DTYPE_CODE[x.dtype],
-            _opt(ws), need, stream)
-    _native.check(status, "peco_gated_norm_backward")
+    _native.enqueue(dev, "peco_gated_norm_backward", lib.peco_gated_norm_backward,
+                    (addr(gh), ghb, ghr, addr(gr), grb, grr, addr(x3), xb, xr, addr(b3), bb, br, addr(gv), gb, addr(sv),
+                     sb, addr(weight), addr(post_weight),
+                     *(addr(grads[n]) for n in ("x", "branch", "gate", "scale", "shift")), shared,
+                     addr(grads["weight"]), addr(grads["post_weight"]), x3.shape[0], x3.shape[1], c, NORMS[norm],
+                     NORMS[post_norm], eps, eps if post_eps is None else post_eps, residual_scale,
+                     _native.DTYPE_CODE[x.dtype], addr(ws), need), (gh, gr, x3, b3, gv, sv, weight, post_weight))
     return NormGrads(**grads)

@@ -55,7 +55,11 @@ def _check(q, k, axes, theta, grid, positions):
         turned = positions.shape[-2]
     if turned > n:
         raise ValueError(f"{turned} positions for {n} tokens")
-    _native.require_cuda(*[t for t in (q, k, positions) if t is not None])
+    if q.device.type != "cuda":
+        _native.require_cuda(q)
+    for t in (k, positions):
+        if t is not None and t.device != q.device:
+            _native.require_cuda(q, t)
     return axes, grid, turned
 
 
@@ -83,19 +87,15 @@ def _run(q, k, axes, theta, grid, positions, interleaved, inverse, inplace):
         pos_sb = positions.stride(0) if positions.dim() == 3 and positions.shape[0] > 1 else 0
         if turned == 0:
             positions, grid = None, (0,) * len(axes)
-    lib = _native.load()
-    dev = q.device
-    null = _native.P(0)
-    with torch.cuda.device(dev):
-        stream = _native.stream_of(dev, *sources, *outs, positions)
-        args = []
-        for src, out, st in zip(sources, outs, strides):
-            args += [null, null, 0, null] if src is None else [_native.ptr(src), _native.ptr(out), src.shape[1], st]
-        status = lib.peco_rotary(*args, b, n, turned, d, (ctypes.c_int * len(axes))(*axes), len(axes), float(theta),
-                                 (ctypes.c_int * len(axes))(*grid) if grid is not None else null,
-                                 _native.ptr(positions), pos_sb, pos_sn, pos_type, int(bool(interleaved)),
-                                 int(bool(inverse)), _native.DTYPE_CODE[q.dtype], stream)
-    _native.check(status, "peco_rotary")
+    args = []
+    for src, out, st in zip(sources, outs, strides):
+        args += [0, 0, 0, None] if src is None else [src.data_ptr(), out.data_ptr(), src.shape[1], st]
+    a = len(axes)
+    _native.enqueue(q.device, "peco_rotary", _native.load().peco_rotary,
+                    (*args, b, n, turned, d, (_native.I * a)(*axes), a, theta,
+                     (_native.I * a)(*grid) if grid is not None else None, _native.address(positions), pos_sb, pos_sn,
+                     pos_type, int(bool(interleaved)), int(bool(inverse)), _native.DTYPE_CODE[q.dtype]),
+                    (*sources, positions))
     return outs
 
 
