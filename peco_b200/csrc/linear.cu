@@ -35,6 +35,9 @@ struct GemmArgs {
   CUtensorMap a[2], b[2];    // K segments (x and x2; the second unused otherwise)
   int kblocks[2];            // 64-wide K blocks of each segment
   int m, n, tiles_m, tiles_n;
+  int bn;                    // columns of a tile, a multiple of 32
+  int a_panels, b_panels;    // 64-wide panels of an MN-major operand per CTA
+  uint32_t stage_tx;         // bytes one CTA loads per K block
   void* out;
   long long out_stride;
   // epilogue operands (null where absent)
@@ -51,39 +54,48 @@ struct GemmArgs {
 };
 
 // ---- activations -------------------------------------------------------------
-// Evaluated in fp32.  gelu_tanh is written as z * sigmoid(2u): the exponential
-// keeps full relative precision in the negative tail, where 1 + tanh(u) would
-// cancel.
-__device__ __forceinline__ float sigmoidf_(float x) { return __fdividef(1.0f, 1.0f + exp2_approx(-1.4426950408889634f * x)); }
+// Evaluated in fp32.  gelu_tanh is written as z * sigmoid(2u), u = sqrt(2/pi)
+// (z + 0.044715 z^3): the exponential keeps full relative precision in the
+// negative tail, where 1 + tanh(u) would cancel.
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kGelu1 = 2.0f * 0.7978845608028654f;  // 2u = z (kGelu1 + kGelu3 z^2)
+constexpr float kGelu3 = kGelu1 * 0.044715f;
 
-constexpr float kGeluC = 0.7978845608028654f;  // sqrt(2 / pi)
+__device__ __forceinline__ float recip_approx(float x) { return __fdividef(1.0f, x); }
 
-__device__ __forceinline__ float activate(float z, int act) {
-  switch (act) {
-    case kActGeluTanh: return z * sigmoidf_(2.0f * kGeluC * fmaf(0.044715f * z * z, z, z));
-    case kActGelu: return 0.5f * z * (1.0f + erff(z * 0.7071067811865476f));
-    case kActSilu: return z * sigmoidf_(z);
-    default: return z;
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
+  if constexpr (ACT == kActGeluTanh) {
+    const float w = z * fmaf(-kLog2e * kGelu3, z * z, -kLog2e * kGelu1);
+    return z * recip_approx(1.0f + exp2_approx(w));
+  } else if constexpr (ACT == kActGelu) {
+    return 0.5f * z * (1.0f + erff(z * 0.7071067811865476f));
+  } else if constexpr (ACT == kActSilu) {
+    return z * recip_approx(1.0f + exp2_approx(-kLog2e * z));
+  } else {
+    return z;
   }
 }
 
 // (act(z), act'(z))
-__device__ __forceinline__ float2 activate_slope(float z, int act) {
-  switch (act) {
-    case kActGeluTanh: {
-      const float s = sigmoidf_(2.0f * kGeluC * fmaf(0.044715f * z * z, z, z));
-      // d/dz [z s(2u)] = s + z s (1 - s) 2 u'
-      return make_float2(z * s, fmaf(z * s * (1.0f - s), 2.0f * kGeluC * fmaf(3.0f * 0.044715f * z, z, 1.0f), s));
-    }
-    case kActGelu: {
-      const float p = 0.5f * (1.0f + erff(z * 0.7071067811865476f));
-      return make_float2(z * p, fmaf(z * 0.3989422804014327f, __expf(-0.5f * z * z), p));
-    }
-    case kActSilu: {
-      const float s = sigmoidf_(z);
-      return make_float2(z * s, s * fmaf(z, 1.0f - s, 1.0f));
-    }
-    default: return make_float2(z, 1.0f);
+template <int ACT>
+__device__ __forceinline__ float2 activate_slope(float z) {
+  if constexpr (ACT == kActGeluTanh) {
+    const float z2 = z * z;
+    const float s = recip_approx(1.0f + exp2_approx(z * fmaf(-kLog2e * kGelu3, z2, -kLog2e * kGelu1)));
+    // d/dz [z s(2u)] = s + z s (1 - s) d(2u)/dz
+    const float d = z * fmaf(3.0f * kGelu3, z2, kGelu1);
+    const float slope = fmaf(s, fmaf(-s, d, d), s);
+    // far out the product of a vanishing and an overflowing factor is replaced by its limit
+    return make_float2(z * s, fabsf(z) > 32.0f ? (z > 0.0f ? 1.0f : 0.0f) : slope);
+  } else if constexpr (ACT == kActGelu) {
+    const float p = 0.5f * (1.0f + erff(z * 0.7071067811865476f));
+    return make_float2(z * p, fmaf(z * 0.3989422804014327f, exp2_approx(-0.5f * kLog2e * z * z), p));
+  } else if constexpr (ACT == kActSilu) {
+    const float s = recip_approx(1.0f + exp2_approx(-kLog2e * z));
+    return make_float2(z * s, s * fmaf(z, 1.0f - s, 1.0f));
+  } else {
+    return make_float2(z, 1.0f);
   }
 }
 
@@ -135,16 +147,17 @@ __device__ __forceinline__ void product_step(uint32_t d, uint64_t a, uint64_t b,
   }
 }
 
-// Arrive on ``bar`` (of both CTAs of a pair) once the products issued so far are done.
+// Arrive on ``bar`` (of both CTAs of a pair, whose first has rank ``lead``) once
+// the products issued so far are done.
 template <int CG>
-__device__ __forceinline__ void product_commit(uint64_t* bar) {
+__device__ __forceinline__ void product_commit(uint64_t* bar, uint32_t lead) {
   if constexpr (CG == 1) {
     umma_commit(bar);
   } else {
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
             smem_u32(bar)),
-        "h"(static_cast<uint16_t>(3))
+        "h"(static_cast<uint16_t>(3u << lead))
         : "memory");
   }
 }
@@ -167,30 +180,32 @@ __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
 }
 
 // ---- the product -----------------------------------------------------------------
-// Output tiles of (128 CG) x BN, walked by persistent groups of CG CTAs.  Warp
-// 0 of every CTA streams its 64-wide K blocks of A (128 rows) and B (BN / CG
+// Output tiles of (128 CG) x bn, walked by persistent groups of CG CTAs.  Warp
+// 0 of every CTA streams its 64-wide K blocks of A (128 rows) and B (bn / CG
 // rows) through a ring of shared-memory stages; warp 1 of the group's first
 // CTA issues the MMAs into one of two TMEM accumulators; warps 2-9 read the
 // other one back, apply the epilogue and store, so the epilogue of a tile runs
 // under the MMAs of the next.
 //
-// CG = 2 pairs two SMs on one 256 x 256 tile: each CTA stages half of A's rows
-// and half of B's, so a K block costs 32 KB of shared memory and of TMA traffic
-// per SM for twice the products of a 128 x 128 tile.
-template <int CG, int BN>
-struct GemmLayout {
-  static constexpr int kBRows = BN / CG;
-  static constexpr int kABytes = kTileM * kTileK * 2;
-  static constexpr int kBBytes = kBRows * kTileK * 2;
-  static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = 192 * 1024 / kStageBytes;
-  static constexpr int kSmem = kStages * kStageBytes + 1024;  // + alignment slack
-  static constexpr int kTmemCols = 2 * BN;
-};
+// CG = 2 pairs two SMs on one tile: each CTA stages half of A's rows and half
+// of B's, so a 256 x 256 tile costs 32 KB of shared memory and of TMA traffic
+// per SM and K block, for twice the products of a 128 x 128 tile.
+//
+// SPLIT: one tile per cluster of S groups, each taking a range of the K
+// blocks.  The groups' fp32 partial tiles meet in shared memory: every CTA
+// adds 128 / S rows over the S partials, in the groups' order, and finishes
+// them.
+constexpr int kStages = 6;
+constexpr int kABytes = kTileM * kTileK * 2;
+constexpr int kStageBytes = 2 * kABytes;        // A's 128 rows and up to 128 of B
+constexpr int kRingBytes = kStages * kStageBytes;
+constexpr int kStageRow = 32;                    // columns an epilogue warp finishes at a time
+constexpr int kStagingBytes = kEpilogueWarps * 32 * kStageRow * 4;
+constexpr int kGemmSmem = kRingBytes + kStagingBytes + 1024;  // + alignment slack
+constexpr int kMaxSplitColumns = 128;            // a split tile's fp32 partial (64 KB) fits the ring
 
-template <int STAGES>
 struct GemmShared {
-  uint64_t full[STAGES], empty[STAGES];
+  uint64_t full[kStages], empty[kStages];
   uint64_t acc_full[2], acc_empty[2];
   uint32_t tmem;
   int abort_flag;
@@ -209,15 +224,14 @@ __device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int
   tn = in / height;
 }
 
-// ROWS x 64 operand tile into shared memory: K-major rows of 128 bytes, or
+// Operand rows x 64 into shared memory: K-major rows of 128 bytes (one box), or
 // MN-major panels of 64 elements x 64 K rows
-template <int CG, bool MN, int ROWS>
-__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int row0, int kb, uint32_t bar) {
+template <int CG, bool MN>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int row0, int panels, int kb, uint32_t bar) {
   if constexpr (!MN) {
     tile_load_2d<CG>(dst, map, kb * kTileK, row0, bar);
   } else {
-#pragma unroll
-    for (int p = 0; p < ROWS / 64; ++p) tile_load_2d<CG>(dst + p * 8192, map, row0 + p * 64, kb * kTileK, bar);
+    for (int p = 0; p < panels; ++p) tile_load_2d<CG>(dst + p * 8192, map, row0 + p * 64, kb * kTileK, bar);
   }
 }
 
@@ -227,60 +241,60 @@ __device__ __forceinline__ uint64_t step_desc(uint32_t base, int k) {
   return MN ? smem_desc(base + k * 2048, 8192, 1024) : smem_desc(base + k * 32, 16, 1024);
 }
 
-// Epilogue of 32 columns of one row; ``count`` of them exist.
-template <typename T, bool EPI>
-__device__ __forceinline__ void finish_row(const GemmArgs& args, const uint32_t (&acc)[32], long long row, int col0,
-                                           const T* gate) {
+template <int ACT>
+__device__ __forceinline__ void activate_all(float (&v)[8]) {
 #pragma unroll
-  for (int j = 0; j < 32; j += 8) {
-    const int col = col0 + j;
-    const int count = min(8, args.n - col);
-    if (count <= 0) break;
-    float v[8], res[8], e[8];
-    if (EPI && args.residual)
-      load_vec<8>(static_cast<const T*>(args.residual) + row * args.res_stride + col, args.vec, count, res);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(acc[j + i]);
-    if (EPI) {
-      if (args.bias) {
-        load_vec<8>(static_cast<const T*>(args.bias) + col, args.vec, count, e);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += e[i];
-      }
-      if (args.preact) store_vec<8>(static_cast<T*>(args.preact) + row * args.n + col, args.vec, count, v);
-      switch (args.act) {
-        case kActGeluTanh:
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = activate(v[i], kActGeluTanh);
-          break;
-        case kActGelu:
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = activate(v[i], kActGelu);
-          break;
-        case kActSilu:
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = activate(v[i], kActSilu);
-          break;
-        default: break;
-      }
-      if (gate) {
-        load_vec<8>(gate + col, args.vec, count, e);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= e[i];
-      }
-      if (args.residual) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += res[i];
-      }
-    }
-    store_vec<8>(static_cast<T*>(args.out) + row * args.out_stride + col, args.vec, count, v);
-  }
+  for (int i = 0; i < 8; ++i) v[i] = activate<ACT>(v[i]);
 }
 
-// 32 TMEM columns per lane; the values may be read after tmem_ld_wait_for
-__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
-// Waits for the loads in flight and ties ``r`` to the wait, so that no use of
-// it is scheduled earlier.
+// Epilogue and store of 8 neighbouring columns of one row; ``count`` of them
+// exist.  ``bias`` and ``res`` are the bias and the residual there.
+template <typename T, bool EPI>
+__device__ __forceinline__ void finish8(const GemmArgs& args, float (&v)[8], long long row, int col, int count,
+                                        const float (&bias)[8], const T* gate, const float (&res)[8]) {
+  if (EPI) {
+    float e[8];
+    if (gate) load_vec<8>(gate + col, args.vec, count, e);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += bias[i];
+    if (args.preact) store_vec<8>(static_cast<T*>(args.preact) + row * args.n + col, args.vec, count, v);
+    switch (args.act) {
+      case kActGeluTanh: activate_all<kActGeluTanh>(v); break;
+      case kActGelu: activate_all<kActGelu>(v); break;
+      case kActSilu: activate_all<kActSilu>(v); break;
+      default: break;
+    }
+    if (gate) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= e[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += res[i];
+  }
+  store_vec<8>(static_cast<T*>(args.out) + row * args.out_stride + col, args.vec, count, v);
+}
+
+template <typename T, bool EPI>
+__device__ __forceinline__ void load_bias(const GemmArgs& args, int col, int count, float (&bias)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) bias[i] = 0.0f;
+  if (EPI && args.bias && count > 0) load_vec<8>(static_cast<const T*>(args.bias) + col, args.vec, count, bias);
+}
+template <typename T, bool EPI>
+__device__ __forceinline__ void load_residual(const GemmArgs& args, long long row, int col, int count, float (&res)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) res[i] = 0.0f;
+  if (EPI && args.residual && row < args.m && count > 0)
+    load_vec<8>(static_cast<const T*>(args.residual) + row * args.res_stride + col, args.vec, count, res);
+}
+template <typename T, bool EPI>
+__device__ __forceinline__ const T* gate_row(const GemmArgs& args, long long row) {
+  if (!EPI || !args.gate || row >= args.m) return nullptr;
+  return static_cast<const T*>(args.gate) + (args.gate_stride ? (row / args.rows_per_sample) * args.gate_stride : 0);
+}
+
+// Waits for the TMEM loads in flight and ties ``r`` to the wait, so that no use
+// of it is scheduled earlier.
 __device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
@@ -290,16 +304,82 @@ __device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
                  "+r"(r[30]), "+r"(r[31])::"memory");
 }
 
-template <typename T, int CG, int BN, bool AMN, bool BMN, bool EPI>
-__global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmArgs args) {
-  using L = GemmLayout<CG, BN>;
-  constexpr int kStages = L::kStages;
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ float4 ld_shared_v4(uint32_t addr) {
+  float4 f;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(addr) : "memory");
+  return f;
+}
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
+  float4 f;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w)
+               : "r"(addr)
+               : "memory");
+  return f;
+}
+
+// The epilogue of one tile by one of its 8 warps: TMEM lanes ``quarter``, every
+// other chunk of 32 columns.  A chunk leaves TMEM one row per lane and crosses
+// the warp's staging block (16-byte pieces XORed with the row, free of bank
+// conflicts both ways) to 4 lanes per row with 8 columns each, so that stores
+// and residual reads cover whole 32-byte sectors of eight rows at a time.  The
+// next chunk's TMEM load is in flight meanwhile.
+template <typename T, bool EPI>
+__device__ __forceinline__ void finish_tile(const GemmArgs& args, uint32_t tmem, uint32_t staging, long long row0,
+                                            int col0, int lane, int half) {
+  const int col_end = min(args.n, col0 + args.bn);
+  const int chunks = (args.bn + kStageRow - 1) / kStageRow;
+  const int rr = lane >> 2, cc = (lane & 3) * 8;
+  const T* gate[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) gate[i] = gate_row<T, EPI>(args, row0 + i * 8 + rr);
+  uint32_t acc[32];
+  if (half < chunks) tmem_ld32(tmem + half * kStageRow, acc);
+  for (int c = half; c < chunks; c += 2) {
+    const int col = col0 + c * kStageRow + cc;
+    const int count = min(8, col_end - col);
+    float res[4][8], bias[8];
+    load_bias<T, EPI>(args, col, count, bias);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) load_residual<T, EPI>(args, row0 + i * 8 + rr, col, count, res[i]);
+    tmem_ld_wait_for(acc);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      st_shared_v4(staging + lane * 128 + ((j ^ (lane & 7)) << 4), acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+    if (c + 2 < chunks) tmem_ld32(tmem + (c + 2) * kStageRow, acc);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + rr;
+      const float4 lo = ld_shared_v4(staging + r * 128 + (((cc >> 2) ^ (r & 7)) << 4));
+      const float4 hi = ld_shared_v4(staging + r * 128 + ((((cc >> 2) + 1) ^ (r & 7)) << 4));
+      if (row0 + r < args.m && count > 0) {
+        float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        finish8<T, EPI>(args, v, row0 + r, col, count, bias, gate[i], res[i]);
+      }
+    }
+    __syncwarp();
+  }
+}
+
+// byte offset of the 16-byte piece ``c`` of row ``row`` in a split tile's partial
+__device__ __forceinline__ uint32_t partial_offset(int row, int c, int bn) {
+  return static_cast<uint32_t>(row * bn * 4 + (((c & ~7) | ((c ^ row) & 7)) << 4));
+}
+
+template <typename T, int CG, bool SPLIT, bool AMN, bool BMN, bool EPI>
+__global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmArgs args, int splits) {
   extern __shared__ unsigned char smem_raw[];
-  __shared__ GemmShared<kStages> sh;
+  __shared__ GemmShared sh;
   const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = CG == 1 ? 0 : cluster_rank();
+  const uint32_t cta = CG == 1 && !SPLIT ? 0 : cluster_rank();
+  const uint32_t rank = CG == 1 ? 0 : cta & 1, lead = cta - rank;  // within the pair; the pair's first CTA
   volatile int* abort_flag = &sh.abort_flag;
+  constexpr uint32_t kAccumulator = CG == 1 ? 128 : 256;  // columns between the two accumulators
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&sh.full[s], 1);
@@ -312,7 +392,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     sh.abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 1) tmem_take<CG>(&sh.tmem, L::kTmemCols);
+  if (warp == 1) tmem_take<CG>(&sh.tmem, 2 * kAccumulator);
   tc_fence_before();
   __syncthreads();
   if (CG > 1) cluster_sync();  // the pair's barriers are ready before either CTA signals the other
@@ -320,7 +400,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
   const uint32_t tmem = sh.tmem;
   const int tiles = args.tiles_m * args.tiles_n;
   const int kb0 = args.kblocks[0], kblocks = kb0 + args.kblocks[1];
-  const int group = blockIdx.x / CG, groups = gridDim.x / CG;
+  // persistent: tiles group, group + groups, ...; split: this cluster's one tile
+  const int group = SPLIT ? blockIdx.x / (CG * splits) : blockIdx.x / CG;
+  const int groups = SPLIT ? tiles : gridDim.x / CG;
+  const int part = SPLIT ? static_cast<int>(cta) / CG : 0;
+  const int kb_begin = SPLIT ? static_cast<int>(static_cast<long long>(kblocks) * part / splits) : 0;
+  const int kb_end = SPLIT ? static_cast<int>(static_cast<long long>(kblocks) * (part + 1) / splits) : kblocks;
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA
@@ -330,20 +415,20 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
       for (int t = group; t < tiles && ok; t += groups) {
         int tm, tn;
         tile_coords(t, args.tiles_m, args.tiles_n, tm, tn);
-        const int row_a = (tm * CG + rank) * kTileM, row_b = tn * BN + rank * L::kBRows;
-        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+        const int row_a = (tm * CG + rank) * kTileM, row_b = tn * args.bn + rank * (args.bn / CG);
+        for (int kb = kb_begin; kb < kb_end; ++kb, ++it) {
           const int s = it % kStages;
           ok = mbar_wait(&sh.empty[s], ((it / kStages) & 1) ^ 1, abort_flag, args.status);
           if (!ok) break;
-          const uint32_t st = ring + s * L::kStageBytes;
+          const uint32_t st = ring + s * kStageBytes;
           // the pair's stages fill one barrier, the first CTA's, which expects both CTAs' bytes
           uint32_t bar = smem_u32(&sh.full[s]);
-          if (CG > 1) bar = map_rank(bar, 0);
-          if (rank == 0) mbar_arrive_expect_tx(&sh.full[s], CG * L::kStageBytes);
+          if (CG > 1) bar = map_rank(bar, lead);
+          if (rank == 0) mbar_arrive_expect_tx(&sh.full[s], CG * args.stage_tx);
           const int seg = kb >= kb0 ? 1 : 0;
           const int kx = kb - (seg ? kb0 : 0);
-          load_tile<CG, AMN, kTileM>(st, &args.a[seg], row_a, kx, bar);
-          load_tile<CG, BMN, L::kBRows>(st + L::kABytes, &args.b[seg], row_b, kx, bar);
+          load_tile<CG, AMN>(st, &args.a[seg], row_a, args.a_panels, kx, bar);
+          load_tile<CG, BMN>(st + kABytes, &args.b[seg], row_b, args.b_panels, kx, bar);
         }
       }
       // after an expired wait: time for the copies still in flight to land before the CTA ends
@@ -357,7 +442,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     // ---------------------------------------------------------------- MMA
     if (lane == 0 && rank == 0) {
       constexpr int ab = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
-      constexpr uint32_t idesc = instr_desc(kTileM * CG, BN, ab, AMN, BMN);
+      const uint32_t idesc = instr_desc(kTileM * CG, args.bn, ab, AMN, BMN);
       bool ok = true;
       uint32_t it = 0, local = 0;
       for (int t = group; t < tiles && ok; t += groups, ++local) {
@@ -365,25 +450,25 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         ok = mbar_wait(&sh.acc_empty[b], ((local >> 1) & 1) ^ 1, abort_flag, args.status);
         if (!ok) break;
         tc_fence_after();
-        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+        for (int kb = kb_begin; kb < kb_end; ++kb, ++it) {
           const int s = it % kStages;
           ok = mbar_wait(&sh.full[s], (it / kStages) & 1, abort_flag, args.status);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t sa = ring + s * L::kStageBytes, sb = sa + L::kABytes;
+          const uint32_t sa = ring + s * kStageBytes, sb = sa + kABytes;
 #pragma unroll
           for (int k = 0; k < kTileK / 16; ++k)
-            product_step<CG>(tmem + b * BN, step_desc<AMN>(sa, k), step_desc<BMN>(sb, k), idesc, (kb | k) ? 1u : 0u);
-          product_commit<CG>(&sh.empty[s]);
+            product_step<CG>(tmem + b * kAccumulator, step_desc<AMN>(sa, k), step_desc<BMN>(sb, k), idesc,
+                             (kb > kb_begin || k) ? 1u : 0u);
+          product_commit<CG>(&sh.empty[s], lead);
         }
-        if (ok) product_commit<CG>(&sh.acc_full[b]);
+        if (ok) product_commit<CG>(&sh.acc_full[b], lead);
       }
     }
   } else {
     // ----------------------------------------------------------- epilogue
-    // two warps per quarter of the TMEM lanes, each half of the columns
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
-    constexpr int kCols = BN / 2;
+    const int quarter = warp & 3, half = (warp - 2) >> 2;  // the TMEM lanes this warp may read; its column chunks
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     uint32_t local = 0;
     for (int t = group; t < tiles; t += groups, ++local) {
       int tm, tn;
@@ -391,38 +476,67 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
       const int b = local & 1;
       if (!mbar_wait_warp(&sh.acc_full[b], (local >> 1) & 1, abort_flag, args.status)) break;
       tc_fence_after();
-      const long long row = static_cast<long long>(tm * CG + rank) * kTileM + quarter * 32 + lane;
-      const bool live = row < args.m;
-      const T* gate = nullptr;
-      if (EPI && args.gate && live)
-        gate = static_cast<const T*>(args.gate) + (row / args.rows_per_sample) * args.gate_stride;
-      const uint32_t src = tmem + b * BN + half * kCols + (static_cast<uint32_t>(quarter * 32) << 16);
-      const int col0 = tn * BN + half * kCols;
-      // the next 32 columns are on their way while these are finished
-      uint32_t acc[2][32];
-      tmem_ld32_start(src, acc[0]);
+      if constexpr (SPLIT) {
+        // the partial tile, one row per lane, into the drained ring
+        const int row = quarter * 32 + lane;
+        for (int c = half * 32; c < args.bn; c += 64) {
+          uint32_t acc[32];
+          tmem_ld32_sync(tmem + lanes + c, acc);
 #pragma unroll
-      for (int c = 0; c < kCols / 32; ++c) {
-        tmem_ld_wait_for(acc[c & 1]);
-        if (c + 1 < kCols / 32) tmem_ld32_start(src + (c + 1) * 32, acc[(c + 1) & 1]);
-        if (live) finish_row<T, EPI>(args, acc[c & 1], row, col0 + c * 32, gate);
+          for (int j = 0; j < 8; ++j)
+            st_shared_v4(ring + partial_offset(row, (c >> 2) + j, args.bn), acc[4 * j], acc[4 * j + 1], acc[4 * j + 2],
+                         acc[4 * j + 3]);
+        }
+      } else {
+        const long long row0 = static_cast<long long>(tm * CG + static_cast<int>(rank)) * kTileM + quarter * 32;
+        finish_tile<T, EPI>(args, tmem + b * kAccumulator + lanes, ring + kRingBytes + (warp - 2) * 4096, row0,
+                            tn * args.bn, lane, half);
+        tc_fence_before();
         __syncwarp();
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (CG == 1) mbar_arrive(&sh.acc_empty[b]);
-        else arrive_cluster(map_rank(smem_u32(&sh.acc_empty[b]), 0));
+        if (lane == 0) {
+          if (CG == 1) mbar_arrive(&sh.acc_empty[b]);
+          else arrive_cluster(map_rank(smem_u32(&sh.acc_empty[b]), lead));
+        }
       }
     }
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (CG > 1) cluster_sync();  // neither CTA leaves while the other may still signal it
+  // split: every partial is written; otherwise neither CTA of a pair leaves while the other may still signal it
+  if (CG > 1 || SPLIT) cluster_sync();
   if (warp == 1) {
     tc_fence_after();
-    tmem_free<CG>(tmem, L::kTmemCols);
+    tmem_free<CG>(tmem, 2 * kAccumulator);
+  }
+  if constexpr (SPLIT) {
+    int tm, tn;
+    tile_coords(group, args.tiles_m, args.tiles_n, tm, tn);
+    const int first = kTileM * part / splits, rows = kTileM * (part + 1) / splits - first;
+    const int pieces = args.bn / 8;  // 8 columns each
+    const int col0 = tn * args.bn;
+    const long long row0 = static_cast<long long>(tm * CG + static_cast<int>(rank)) * kTileM;
+    for (int i = threadIdx.x; i < rows * pieces && !sh.abort_flag; i += kGemmThreads) {
+      const int r = first + i / pieces, c = i % pieces;
+      const long long row = row0 + r;
+      const int col = col0 + c * 8, count = min(8, args.n - col);
+      if (row >= args.m || count <= 0) continue;
+      float v[8], bias[8], res[8];
+      load_bias<T, EPI>(args, col, count, bias);
+      load_residual<T, EPI>(args, row, col, count, res);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+      for (int p = 0; p < splits; ++p) {
+        const uint32_t base = map_rank(ring, p * CG + rank);
+        const float4 lo = ld_cluster_v4(base + partial_offset(r, 2 * c, args.bn));
+        const float4 hi = ld_cluster_v4(base + partial_offset(r, 2 * c + 1, args.bn));
+        v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
+        v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
+      }
+      finish8<T, EPI>(args, v, row, col, count, bias, gate_row<T, EPI>(args, row), res);
+    }
+    __syncthreads();
+    cluster_sync();  // no CTA's partial goes away while another reads it
   }
 }
 
@@ -490,7 +604,7 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const ActBackwardArgs
           for (int i = 0; i < 8; ++i) {
             dz[i] = g[j][i] * gate[i];
             if (a.preact) {
-              const float2 f = activate_slope(z[j][i], ACT);
+              const float2 f = activate_slope<ACT>(z[j][i]);
               dz[i] *= f.y;
               sum_ga[i] = fmaf(g[j][i], f.x, sum_ga[i]);
             }
@@ -615,44 +729,90 @@ cudaError_t grant_smem(const void* kernel, int bytes, std::atomic<unsigned long 
   return e;
 }
 
-template <typename T, int CG, int BN, bool AMN, bool BMN, bool EPI>
-int launch_tiles(GemmArgs& g, const Operand* a, const Operand* b, int segments, int dtype, cudaStream_t stream) {
-  using L = GemmLayout<CG, BN>;
-  g.tiles_m = (g.m + CG * kTileM - 1) / (CG * kTileM);
-  g.tiles_n = (g.n + BN - 1) / BN;
-  if (static_cast<long long>(g.tiles_m) * g.tiles_n > 0x7fffffffLL) return kErrUnsupported;
-  for (int s = 0; s < segments; ++s) {
-    if (!operand_map(&g.a[s], a[s], AMN, kTileM, dtype) || !operand_map(&g.b[s], b[s], BMN, L::kBRows, dtype))
-      return kErrTensorMap;
-    g.kblocks[s] = ((AMN ? a[s].rows : a[s].cols) + kTileK - 1) / kTileK;
+// How a product is cut: CTAs per group, columns per tile, K splits.
+struct TileChoice {
+  int cg, bn, splits;
+};
+
+// Estimated clocks of a choice, from what one SM does per 64-wide K block: 2 bn
+// clocks of MMA (128 bn CG x 16 products take bn / 2 clocks per CTA), or the
+// operand bytes at about 64 a clock, whichever is longer; plus a start and a
+// finish per tile and the meeting of a split's partials.
+TileChoice choose_tiles(int m, int n, int kblocks, bool amn) {
+  TileChoice best{1, 128, 1};
+  double least = 1e300;
+  const int cg = m > kTileM ? 2 : 1;
+  const int a_rows = amn ? (m > 64 ? 128 : 64) : (m < kTileM ? (m + 7) / 8 * 8 : kTileM);
+  const long long tiles_m = (m + kTileM * cg - 1) / (kTileM * cg);
+  for (int splits = 1; splits * cg <= 8; splits *= 2) {
+    if (splits > 1 && kblocks < 4 * splits) break;
+    const int most = splits > 1 || cg == 1 ? kMaxSplitColumns : 256;
+    for (int bn = 32 * cg; bn <= most; bn += 32) {
+      const long long tiles = tiles_m * ((n + bn - 1) / bn);
+      const long long waves = (tiles * splits * cg + kNumSMs - 1) / kNumSMs;
+      if (splits > 1 && waves > 1) continue;
+      const double mma = 2.0 * bn, load = 2.0 * (a_rows + bn / cg);
+      const double cost = waves * (static_cast<double>(kblocks) / splits * (mma > load ? mma : load) + 200.0) +
+                          (splits > 1 ? 2500.0 : 6.0 * bn);
+      if (cost < least) {
+        least = cost;
+        best = TileChoice{cg, bn, splits};
+      }
+    }
   }
-  g.status = device_status_ptr();
-  auto kernel = gemm_kernel<T, CG, BN, AMN, BMN, EPI>;
+  return best;
+}
+
+template <typename T, int CG, bool SPLIT, bool AMN, bool BMN, bool EPI>
+int launch_tiles(const GemmArgs& g, int splits, cudaStream_t stream) {
+  auto kernel = gemm_kernel<T, CG, SPLIT, AMN, BMN, EPI>;
   static std::atomic<unsigned long long> opened{0};  // devices whose kernel has its shared memory granted
-  cudaError_t e = grant_smem(reinterpret_cast<const void*>(kernel), L::kSmem, opened);
+  cudaError_t e = grant_smem(reinterpret_cast<const void*>(kernel), kGemmSmem, opened);
   if (e != cudaSuccess) return static_cast<int>(e);
   const int tiles = g.tiles_m * g.tiles_n, most = kNumSMs / CG;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((tiles < most ? tiles : most) * CG);
+  cfg.gridDim = dim3(SPLIT ? tiles * CG * splits : (tiles < most ? tiles : most) * CG);
   cfg.blockDim = dim3(kGemmThreads);
-  cfg.dynamicSmemBytes = L::kSmem;
+  cfg.dynamicSmemBytes = kGemmSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.x = CG * splits;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kernel, g);
+  e = cudaLaunchKernelEx(&cfg, kernel, g, splits);
   const int st = launch_status();
   return e != cudaSuccess ? static_cast<int>(e) : st;
 }
 
 template <typename T, bool AMN, bool BMN, bool EPI>
 int launch_gemm(GemmArgs& g, const Operand* a, const Operand* b, int segments, int dtype, cudaStream_t stream) {
-  const long long big = static_cast<long long>((g.m + 255) / 256) * ((g.n + 255) / 256);
-  if (big >= 37) return launch_tiles<T, 2, 256, AMN, BMN, EPI>(g, a, b, segments, dtype, stream);
-  return launch_tiles<T, 1, 128, AMN, BMN, EPI>(g, a, b, segments, dtype, stream);
+  int kblocks = 0;
+  for (int s = 0; s < segments; ++s) {
+    g.kblocks[s] = ((AMN ? a[s].rows : a[s].cols) + kTileK - 1) / kTileK;
+    kblocks += g.kblocks[s];
+  }
+  const TileChoice c = choose_tiles(g.m, g.n, kblocks, AMN);
+  g.bn = c.bn;
+  g.tiles_m = (g.m + c.cg * kTileM - 1) / (c.cg * kTileM);
+  g.tiles_n = (g.n + c.bn - 1) / c.bn;
+  if (static_cast<long long>(g.tiles_m) * g.tiles_n > 0x0fffffffLL) return kErrUnsupported;
+  // rows (or panels) of the operands one CTA stages per K block; a single tile
+  // of few rows loads only those, the others' results are never stored
+  const int a_rows = g.m < kTileM ? (g.m + 7) / 8 * 8 : kTileM, b_rows = c.bn / c.cg;
+  g.a_panels = g.m > 64 ? 2 : 1;
+  g.b_panels = (b_rows + 63) / 64;
+  g.stage_tx = (AMN ? g.a_panels * 8192 : a_rows * 128) + (BMN ? g.b_panels * 8192 : b_rows * 128);
+  for (int s = 0; s < segments; ++s)
+    if (!operand_map(&g.a[s], a[s], AMN, a_rows, dtype) || !operand_map(&g.b[s], b[s], BMN, b_rows, dtype))
+      return kErrTensorMap;
+  g.status = device_status_ptr();
+  if (c.splits > 1)
+    return c.cg == 2 ? launch_tiles<T, 2, true, AMN, BMN, EPI>(g, c.splits, stream)
+                     : launch_tiles<T, 1, true, AMN, BMN, EPI>(g, c.splits, stream);
+  return c.cg == 2 ? launch_tiles<T, 2, false, AMN, BMN, EPI>(g, 1, stream)
+                   : launch_tiles<T, 1, false, AMN, BMN, EPI>(g, 1, stream);
 }
 
 bool aligned16(const void* p, long long stride) {
