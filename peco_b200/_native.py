@@ -153,6 +153,13 @@ def enqueue(device: torch.device, what: str, fn, args, inputs) -> None:
         check(status, what)
 
 
+def wants_grad(*inputs) -> bool:
+    for t in inputs:
+        if t is not None and t.requires_grad:
+            return True
+    return False
+
+
 def address(t: torch.Tensor | None) -> int:
     return t.data_ptr() if t is not None else 0
 

@@ -32,19 +32,16 @@ class LinearGrads(NamedTuple):
     gate: Optional[torch.Tensor]
 
 
-def _flat(t: torch.Tensor) -> torch.Tensor:
-    """[rows, features] view with adjacent features and one stride between rows
-    (a copy where the layout has no such view)."""
-    t = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
-    if t.stride(1) != 1 and t.shape[1] > 1 or t.stride(0) < t.shape[1] and t.shape[0] > 1:
-        t = t.contiguous()
-    return t
-
-
-def _stride(t: Optional[torch.Tensor]) -> int:
-    if t is None:
-        return 0
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+def _rows(t: torch.Tensor, width: int):
+    """(tensor, elements between rows) of [..., width] rows with adjacent columns
+    and one stride between rows; a copy where the layout has no such view."""
+    if t.is_contiguous():
+        return t, width
+    f = t.reshape(-1, width) if t.dim() != 2 else t
+    rows, step = f.shape[0], f.stride(0)
+    if f.stride(1) != 1 and width > 1 or step < width and rows > 1:
+        return f.contiguous(), width
+    return f, max(step, width)
 
 
 def _check(x, weight, bias, gate, residual, x2, activation):
@@ -88,48 +85,77 @@ def _check(x, weight, bias, gate, residual, x2, activation):
     return k, k2, n, samples
 
 
-def _gate_rows(gate, n):
-    """The gate as [samples, N] with adjacent columns."""
-    if gate is None:
-        return None
-    gate = gate.reshape(-1, n) if gate.dim() != 2 else gate
-    return gate if gate.stride(1) == 1 or n == 1 else gate.contiguous()
+def _gate_rows(gate, n, samples):
+    """(gate as rows of adjacent columns, elements between samples)."""
+    if gate.is_contiguous():
+        return gate, n if samples > 1 else 0
+    gate = gate.reshape(-1, n)
+    if gate.stride(1) != 1 and n > 1:
+        gate = gate.contiguous()
+    return gate, gate.stride(0) if samples > 1 else 0
+
+
+def _weight_rows(weight):
+    """(weight, elements between rows); rows may be padded."""
+    step, inner = weight.stride()
+    k = weight.shape[1]
+    if (inner == 1 or k == 1) and step >= k:
+        return weight, step
+    return weight.contiguous(), k
+
+
+def _misaligned(ptrs: int, strides: int) -> bool:
+    """Whether some operand may not start every row on 16 bytes."""
+    return bool(ptrs & 15 or strides & 7)
 
 
 def _forward(x, weight, bias, gate, residual, x2, activation, out, want_preact):
     k, k2, n, samples = _check(x, weight, bias, gate, residual, x2, activation)
     shape = (*x.shape[:-1], n)
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
-    elif out.shape != shape or out.dtype != x.dtype or out.device != x.device:
-        raise ValueError(f"out must be a {x.dtype} tensor of shape {list(shape)} on {x.device}")
+        out = out_rows = x.new_empty(shape)
+        out_step = n
+    else:
+        if out.shape != shape or out.dtype != x.dtype or out.device != x.device:
+            raise ValueError(f"out must be a {x.dtype} tensor of shape {list(shape)} on {x.device}")
+        try:
+            out_rows, out_step = out.view(-1, n) if out.numel() else out, n
+        except RuntimeError:
+            raise ValueError("out must have one stride between rows") from None
+        if out.numel():
+            if out_rows.stride(1) != 1 and n > 1 or out_rows.stride(0) < n and out_rows.shape[0] > 1:
+                raise ValueError("out must have adjacent columns and rows apart")
+            out_step = max(out_rows.stride(0), n)
     rows = out.numel() // n
-    preact = torch.empty((rows, n), dtype=x.dtype, device=x.device) if want_preact else None
+    preact = x.new_empty((rows, n)) if want_preact else None
     if rows == 0:
         return out, preact
-    try:
-        out_rows = out.view(-1, n) if out.dim() != 2 else out
-    except RuntimeError:
-        out_rows = None
-    if out_rows is None or out_rows.stride(1) != 1 and n > 1 or out_rows.stride(0) < n and rows > 1:
-        raise ValueError("out must have adjacent columns and one stride between rows")
-    xf, x2f, res = _flat(x), None if x2 is None else _flat(x2), None if residual is None else _flat(residual)
-    w = weight if weight.stride(1) == 1 and weight.stride(0) >= weight.shape[1] else weight.contiguous()
-    gates = _gate_rows(gate, n)
-    bias = None if bias is None else bias.contiguous()
+    x, x_step = _rows(x, k)
+    weight, w_step = _weight_rows(weight)
+    xp, wp, x2p, bp, gp, rp = x.data_ptr(), weight.data_ptr(), 0, 0, 0, 0
+    x2_step = g_step = r_step = 0
+    if x2 is not None:
+        x2, x2_step = _rows(x2, k2)
+        x2p = x2.data_ptr()
+    if bias is not None:
+        bias = bias.contiguous()
+        bp = bias.data_ptr()
+    if gate is not None:
+        gate, g_step = _gate_rows(gate, n, samples)
+        gp = gate.data_ptr()
+    if residual is not None:
+        residual, r_step = _rows(residual, n)
+        rp = residual.data_ptr()
     lib = _native.load()
-    dev, addr = x.device, _native.address
-    operands = (addr(xf), _stride(xf), addr(x2f), _stride(x2f), addr(w), _stride(w))
-    sizes = (samples, rows // samples, k, k2, n)
-    need, ws = 0, None
-    if (operands[0] | operands[2] | operands[4]) & 15 or (operands[1] | operands[3] | operands[5] | (k if k2 else 0)) & 7:
-        # some operand may not start every row on 16 bytes
-        need = int(lib.peco_linear_forward_workspace(*operands, *sizes))
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-    _native.enqueue(dev, "peco_linear_forward", lib.peco_linear_forward,
-                    (*operands, addr(bias), addr(gates), gates.stride(0) if samples > 1 else 0, addr(res), _stride(res),
-                     out_rows.data_ptr(), _stride(out_rows), addr(preact), *sizes, ACTIVATIONS[activation],
-                     _native.DTYPE_CODE[x.dtype], addr(ws), max(need, 0)), (xf, x2f, w, bias, gates, res, out))
+    per, need, ws = rows // samples, 0, None
+    if _misaligned(xp | wp | x2p, x_step | w_step | x2_step | (k if k2 else 0)):
+        need = int(lib.peco_linear_forward_workspace(xp, x_step, x2p, x2_step, wp, w_step, samples, per, k, k2, n))
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need > 0 else None
+    _native.enqueue(x.device, "peco_linear_forward", lib.peco_linear_forward,
+                    (xp, x_step, x2p, x2_step, wp, w_step, bp, gp, g_step, rp, r_step, out_rows.data_ptr(), out_step,
+                     _native.address(preact), samples, per, k, k2, n, ACTIVATIONS[activation],
+                     _native.DTYPE_CODE[x.dtype], _native.address(ws), max(need, 0)),
+                    (x, weight, bias, gate, residual, x2, out))
     return out, preact
 
 
@@ -167,12 +193,11 @@ def linear_act(x, weight, bias=None, *, activation=None, gate=None, residual=Non
     (keep odd-width weights in padded rows to avoid that).  ``out`` (not under
     autograd) receives the result and may be ``residual``.
     """
-    inputs = (x, weight, bias, gate, residual, x2)
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in inputs):
+    if torch.is_grad_enabled() and _native.wants_grad(x, weight, bias, gate, residual, x2):
         if out is not None:
             raise RuntimeError("linear_act(out=...) does not record gradients; use torch.no_grad()")
         return _LinearAct.apply(x, weight, bias, gate, residual, x2, activation)
-    return _forward(*inputs, activation, out, False)[0]
+    return _forward(x, weight, bias, gate, residual, x2, activation, out, False)[0]
 
 
 def linear_act_backward(grad, x, weight, *, preact=None, activation=None, gate=None, x2=None, bias=False, needs=None):
@@ -206,18 +231,20 @@ def linear_act_backward(grad, x, weight, *, preact=None, activation=None, gate=N
         preact = preact.reshape(rows, n).contiguous()
     else:
         preact = None
-    outs = {f: torch.empty(shapes[f], dtype=x.dtype, device=x.device) if f in needs else None
-            for f in LinearGrads._fields}
-    g, xf, x2f, gates = _flat(grad), _flat(x), None if x2 is None else _flat(x2), _gate_rows(gate, n)
-    w = weight if weight.stride(1) == 1 and weight.stride(0) >= weight.shape[1] else weight.contiguous()
+    outs = {f: x.new_empty(shapes[f]) if f in needs else None for f in LinearGrads._fields}
+    grad, grad_step = _rows(grad, n)
+    x, x_step = _rows(x, k)
+    x2, x2_step = (None, 0) if x2 is None else _rows(x2, k2)
+    gate, g_step = (None, 0) if gate is None else _gate_rows(gate, n, samples)
+    weight, w_step = _weight_rows(weight)
     lib = _native.load()
-    dev, addr = x.device, _native.address
-    operands = (addr(xf), _stride(xf), addr(x2f), _stride(x2f), addr(w), _stride(w))
+    addr = _native.address
+    operands = (x.data_ptr(), x_step, addr(x2), x2_step, weight.data_ptr(), w_step)
     sizes = (samples, rows // samples, k, k2, n, act)
-    need = int(lib.peco_linear_backward_workspace(addr(g), _stride(g), *operands, *sizes, int(gate is not None)))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-    _native.enqueue(dev, "peco_linear_backward", lib.peco_linear_backward,
-                    (addr(g), _stride(g), addr(preact), *operands, addr(gates), gates.stride(0) if samples > 1 else 0,
+    need = int(lib.peco_linear_backward_workspace(grad.data_ptr(), grad_step, *operands, *sizes, int(gate is not None)))
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need > 0 else None
+    _native.enqueue(x.device, "peco_linear_backward", lib.peco_linear_backward,
+                    (grad.data_ptr(), grad_step, addr(preact), *operands, addr(gate), g_step,
                      *(addr(outs[f]) for f in ("x", "x2", "weight", "bias", "gate")), *sizes,
-                     _native.DTYPE_CODE[x.dtype], addr(ws), max(need, 0)), (g, preact, xf, x2f, w, gates))
+                     _native.DTYPE_CODE[x.dtype], addr(ws), max(need, 0)), (grad, preact, x, x2, weight, gate))
     return LinearGrads(**outs)

@@ -36,13 +36,15 @@ class NormGrads(NamedTuple):
     post_weight: Optional[torch.Tensor]
 
 
-def _rows(t, width):
-    """(tensor, batch stride, row stride) of [B, T, C] rows with adjacent columns."""
+def _rows(t, samples, rows, width):
+    """(tensor, batch stride, row stride) of rows [samples, rows, width] with adjacent columns."""
     if t is None:
         return None, 0, 0
-    t = t.reshape(-1, *t.shape[-2:]) if t.dim() != 3 else t
+    if t.is_contiguous():
+        return t, rows * width, width
+    t = t.reshape(samples, rows, width) if t.dim() != 3 else t
     if t.stride(2) != 1 and width > 1:
-        t = t.contiguous()
+        return t.contiguous(), rows * width, width
     return t, t.stride(0), t.stride(1)
 
 
@@ -50,19 +52,18 @@ def _vec(t, width):
     """(tensor, sample stride) of a vector [C] (stride 0) or [B, C] / [B, 1, C]."""
     if t is None:
         return None, 0
-    t = t.reshape(-1, width) if t.dim() == 3 else t
+    if t.is_contiguous():
+        return t, width if t.dim() > 1 else 0
     if t.stride(-1) != 1 and width > 1:
         t = t.contiguous()
-    return t, t.stride(0) if t.dim() == 2 else 0
+    return t, t.stride(0) if t.dim() > 1 else 0
 
 
-def _as3(t):
-    """[T, C] or [C] rows as one sample; [B, ..., T, C] keeps its leading axis only."""
-    if t is None:
-        return None
-    if t.dim() <= 2:
-        return t.reshape(1, -1, t.shape[-1])
-    return t if t.dim() == 3 else t.reshape(t.shape[0], -1, t.shape[-1])
+def _extent(x):
+    """(samples, rows) of x: the leading axis of [B, ..., T, C] counts samples, [T, C] and [C] are one."""
+    c = x.shape[-1]
+    samples = x.shape[0] if x.dim() >= 3 else 1
+    return samples, x.numel() // (c * samples) if samples else 0
 
 
 def _check(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, eps, residual_scale):
@@ -106,18 +107,22 @@ def _check(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, 
 def _forward(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, eps, post_eps, residual_scale):
     _check(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, eps, residual_scale)
     c = x.shape[-1]
-    normed = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    residual = torch.empty(x.shape, dtype=x.dtype, device=x.device) if branch is not None else None
-    if x.numel() == 0:
+    normed = x.new_empty(x.shape)
+    residual = x.new_empty(x.shape) if branch is not None else None
+    samples, rows = _extent(x)
+    if samples * rows == 0:
         return residual, normed
-    x3, xb, xr = _rows(_as3(x), c)
-    b3, bb, br = _rows(_as3(branch), c)
-    (gate, gb), (scale, sb), (shift, tb) = (_vec(t, c) for t in (gate, scale, shift))
-    weight, post_weight = (None if t is None else t.contiguous() for t in (weight, post_weight))
+    x3, xb, xr = _rows(x, samples, rows, c)
+    b3, bb, br = _rows(branch, samples, rows, c)
+    gate, gb = _vec(gate, c)
+    scale, sb = _vec(scale, c)
+    shift, tb = _vec(shift, c)
+    weight = None if weight is None else weight.contiguous()
+    post_weight = None if post_weight is None else post_weight.contiguous()
     addr = _native.address
     _native.enqueue(x.device, "peco_gated_norm", _native.load().peco_gated_norm,
                     (x3.data_ptr(), xb, xr, addr(b3), bb, br, addr(gate), gb, addr(scale), sb, addr(shift), tb,
-                     addr(weight), addr(post_weight), addr(residual), normed.data_ptr(), x3.shape[0], x3.shape[1], c,
+                     addr(weight), addr(post_weight), addr(residual), normed.data_ptr(), samples, rows, c,
                      NORMS[norm], NORMS[post_norm], eps, eps if post_eps is None else post_eps, residual_scale,
                      _native.DTYPE_CODE[x.dtype]), (x3, b3, gate, scale, shift, weight, post_weight))
     return residual, normed
@@ -158,7 +163,7 @@ def modulated_norm(x, branch=None, *, gate=None, scale=None, shift=None, weight=
     """
     options = dict(norm=norm, post_norm=post_norm, eps=eps, post_eps=post_eps, residual_scale=residual_scale)
     inputs = (x, branch, gate, scale, shift, weight, post_weight)
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in inputs):
+    if torch.is_grad_enabled() and _native.wants_grad(*inputs):
         return _ModulatedNorm.apply(*inputs, options)
     residual, normed = _forward(*inputs, **options)
     return normed if residual is None else (residual, normed)
@@ -186,12 +191,13 @@ def modulated_norm_backward(grad_normed, grad_residual, x, branch=None, *, gate=
     if x.numel() == 0:
         return NormGrads(**{n: torch.zeros(t.shape, dtype=x.dtype, device=x.device) if n in needs else None
                             for n, t in inputs.items()})
-    grads = {n: torch.empty(inputs[n].shape, dtype=x.dtype, device=x.device) if n in needs else None for n in inputs}
+    grads = {n: x.new_empty(t.shape) if n in needs else None for n, t in inputs.items()}
     c = x.shape[-1]
-    gh, ghb, ghr = _rows(_as3(grad_normed), c)
-    gr, grb, grr = _rows(_as3(grad_residual), c)
-    x3, xb, xr = _rows(_as3(x), c)
-    b3, bb, br = _rows(_as3(branch), c)
+    samples, rows = _extent(x)
+    gh, ghb, ghr = _rows(grad_normed, samples, rows, c)
+    gr, grb, grr = _rows(grad_residual, samples, rows, c)
+    x3, xb, xr = _rows(x, samples, rows, c)
+    b3, bb, br = _rows(branch, samples, rows, c)
     # a vector without a sample axis sums its gradient over the samples
     shared = sum(bit for bit, t in ((1, gate), (2, scale), (4, shift)) if t is not None and t.dim() == 1)
     (gv, gb), (sv, sb) = _vec(gate, c), _vec(scale, c)
@@ -200,13 +206,13 @@ def modulated_norm_backward(grad_normed, grad_residual, x, branch=None, *, gate=
     dev, addr = x.device, _native.address
     need, ws = 0, None
     if any(n in needs for n in NormGrads._fields[2:]):
-        need = int(lib.peco_gated_norm_backward_workspace(x3.shape[0], x3.shape[1], c))
+        need = int(lib.peco_gated_norm_backward_workspace(samples, rows, c))
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
     _native.enqueue(dev, "peco_gated_norm_backward", lib.peco_gated_norm_backward,
                     (addr(gh), ghb, ghr, addr(gr), grb, grr, addr(x3), xb, xr, addr(b3), bb, br, addr(gv), gb, addr(sv),
                      sb, addr(weight), addr(post_weight),
                      *(addr(grads[n]) for n in ("x", "branch", "gate", "scale", "shift")), shared,
-                     addr(grads["weight"]), addr(grads["post_weight"]), x3.shape[0], x3.shape[1], c, NORMS[norm],
+                     addr(grads["weight"]), addr(grads["post_weight"]), samples, rows, c, NORMS[norm],
                      NORMS[post_norm], eps, eps if post_eps is None else post_eps, residual_scale,
                      _native.DTYPE_CODE[x.dtype], addr(ws), need), (gh, gr, x3, b3, gv, sv, weight, post_weight))
     return NormGrads(**grads)

@@ -18,6 +18,8 @@ import torch
 
 from . import _native
 
+_Strides = ctypes.c_longlong * 6
+_Ints = [ctypes.c_int * i for i in range(5)]
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 
 
@@ -78,7 +80,7 @@ def _run(q, k, axes, theta, grid, positions, interleaved, inverse, inplace):
         if out.stride(3) != 1 and d > 1:
             out = torch.empty(src.shape, dtype=src.dtype, device=src.device)
         sources.append(src), outs.append(out)
-        strides.append((ctypes.c_longlong * 6)(*src.stride()[:3], *out.stride()[:3]))
+        strides.append(_Strides(*src.stride()[:3], *out.stride()[:3]))
     pos_sb = pos_sn = pos_type = 0
     if positions is not None:
         if positions.stride(-1) != 1 and len(axes) > 1:
@@ -92,8 +94,8 @@ def _run(q, k, axes, theta, grid, positions, interleaved, inverse, inplace):
         args += [0, 0, 0, None] if src is None else [src.data_ptr(), out.data_ptr(), src.shape[1], st]
     a = len(axes)
     _native.enqueue(q.device, "peco_rotary", _native.load().peco_rotary,
-                    (*args, b, n, turned, d, (_native.I * a)(*axes), a, theta,
-                     (_native.I * a)(*grid) if grid is not None else None, _native.address(positions), pos_sb, pos_sn,
+                    (*args, b, n, turned, d, _Ints[a](*axes), a, theta,
+                     _Ints[a](*grid) if grid is not None else None, _native.address(positions), pos_sb, pos_sn,
                      pos_type, int(bool(interleaved)), int(bool(inverse)), _native.DTYPE_CODE[q.dtype]),
                     (*sources, positions))
     return outs
@@ -134,7 +136,7 @@ def rotate(q, k=None, *, axes, theta=256.0, grid=None, positions=None, interleav
     overwrites q and k.  Returns q, or (q, k).
     """
     options = dict(axes=axes, theta=theta, grid=grid, positions=positions, interleaved=interleaved, inverse=inverse)
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k)):
+    if torch.is_grad_enabled() and _native.wants_grad(q, k):
         if inplace:
             raise RuntimeError("rotate(inplace=True) does not record gradients; use torch.no_grad()")
         return _Rotate.apply(q, k, options)
