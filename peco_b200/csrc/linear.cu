@@ -568,8 +568,8 @@ struct ActBackwardArgs {
   int act, vec;
 };
 
-template <typename T, int ACT>
-__global__ void __launch_bounds__(256) act_backward_kernel(const ActBackwardArgs a) {
+template <typename T, int ACT, bool GATE>
+__global__ void __launch_bounds__(256, GATE ? 3 : 4) act_backward_kernel(const ActBackwardArgs a) {
   __shared__ float red[2][8][256];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sample = blockIdx.y / a.chunks, chunk = blockIdx.y - sample * a.chunks;
@@ -582,7 +582,7 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const ActBackwardArgs
     sum_dz[i] = sum_ga[i] = 0.0f;
   }
   if (count > 0) {
-    if (a.gate) load_vec<8>(static_cast<const T*>(a.gate) + sample * a.gate_stride + col, a.vec, count, gate);
+    if (GATE) load_vec<8>(static_cast<const T*>(a.gate) + sample * a.gate_stride + col, a.vec, count, gate);
     const int begin = chunk * a.chunk_rows, end = min(begin + a.chunk_rows, a.rows_per_sample);
     const long long row0 = static_cast<long long>(sample) * a.rows_per_sample;
     // two of the warp's rows in flight
@@ -602,11 +602,11 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const ActBackwardArgs
           float dz[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            dz[i] = g[j][i] * gate[i];
+            dz[i] = GATE ? g[j][i] * gate[i] : g[j][i];
             if (a.preact) {
               const float2 f = activate_slope<ACT>(z[j][i]);
               dz[i] *= f.y;
-              sum_ga[i] = fmaf(g[j][i], f.x, sum_ga[i]);
+              if (GATE) sum_ga[i] = fmaf(g[j][i], f.x, sum_ga[i]);
             }
             sum_dz[i] += dz[i];
           }
@@ -874,6 +874,12 @@ BackwardPlan plan_backward(const LinearShape& s, const Operand& grad, bool has_g
   return p;
 }
 
+template <typename T, int ACT>
+void launch_act_backward(const ActBackwardArgs& a, dim3 grid, cudaStream_t stream) {
+  if (a.gate) act_backward_kernel<T, ACT, true><<<grid, 256, 0, stream>>>(a);
+  else act_backward_kernel<T, ACT, false><<<grid, 256, 0, stream>>>(a);
+}
+
 template <typename T>
 int backward(const LinearShape& s, Operand grad, const void* preact, Operand (&x)[2], Operand (&w)[2],
              const void* gate, long long gate_stride, void* (&dx)[2], void* dweight, void* dbias, void* dgate,
@@ -903,10 +909,10 @@ int backward(const LinearShape& s, Operand grad, const void* preact, Operand (&x
     a.vec = s.n % 8 == 0 && aligned16(grad.ptr, grad.stride) && aligned16(a.preact, s.n) && aligned16(gate, gate_stride);
     const dim3 grid((s.n + 255) / 256, s.samples * p.chunks);
     switch (s.act) {
-      case kActGeluTanh: act_backward_kernel<T, kActGeluTanh><<<grid, 256, 0, stream>>>(a); break;
-      case kActGelu: act_backward_kernel<T, kActGelu><<<grid, 256, 0, stream>>>(a); break;
-      case kActSilu: act_backward_kernel<T, kActSilu><<<grid, 256, 0, stream>>>(a); break;
-      default: act_backward_kernel<T, kActNone><<<grid, 256, 0, stream>>>(a);
+      case kActGeluTanh: launch_act_backward<T, kActGeluTanh>(a, grid, stream); break;
+      case kActGelu: launch_act_backward<T, kActGelu>(a, grid, stream); break;
+      case kActSilu: launch_act_backward<T, kActSilu>(a, grid, stream); break;
+      default: launch_act_backward<T, kActNone>(a, grid, stream);
     }
     if (int st = launch_status()) return st;
     if (p.sums) {

@@ -22,12 +22,14 @@
 // Both directions move bytes: the floor is each input read once and each
 // output written once at the copy bandwidth.  A row is read once into
 // registers of the threads that share it, and every statistic is taken from
-// there in fp32, the variance around the mean already known.  The backward
-// kernel recomputes r from x and the branch, so nothing has to be saved.
+// there in fp32, squares around the mean.  The backward kernel recomputes r
+// from x and the branch, so nothing has to be saved.
 #include "common.cuh"
 #include "../../include/peco_b200.h"
 #include "internal.h"
 #include "rows.cuh"
+
+#include <atomic>
 
 namespace peco {
 namespace {
@@ -59,287 +61,460 @@ struct NormArgs {
   int chunks;       // backward: row chunks per sample
 };
 
-// ---- sums over the threads of one row ---------------------------------------
-template <int WARPS>
-struct RowGroup {
-  static constexpr int kThreads = 32 * WARPS;
-};
+// ---- a row in registers ----------------------------------------------------------
+// A row is shared by 32 * WARPS threads, each with NCH chunks of 8 columns held
+// as four fp32 pairs (the pairs' arithmetic takes one instruction for two).
+// Aligned rows: chunk i of a thread is 8 neighbouring columns, one 16-byte
+// access.  Other rows: its 8 columns lie a row of threads apart, so that single
+// elements are still read side by side.  Columns past the width hold 0.
+constexpr int kChunk = 8;
 
-// Sum of K values over the row's threads, on every thread; ``buf`` is K *
-// WARPS floats that no other reduction in flight uses.
-template <int WARPS, int K>
-__device__ __forceinline__ void row_sum(float (&v)[K], float* buf) {
-#pragma unroll
-  for (int k = 0; k < K; ++k) v[k] = warp_sum(v[k]);
-  if constexpr (WARPS > 1) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (lane == 0) {
-#pragma unroll
-      for (int k = 0; k < K; ++k) buf[k * WARPS + warp] = v[k];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      float s = 0.0f;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) s += buf[k * WARPS + w];
-      v[k] = s;
-    }
-  }
-}
-
-// One thread's part of a row: chunk i holds VEC neighbouring elements at
-// column (i * threads + thread) * VEC; elements past the width read as 0.
-template <int VEC, int NCH, int THREADS>
+template <int WARPS, int NCH, bool ALIGNED>
 struct Span {
+  static constexpr int kThreads = 32 * WARPS;
   int thread, width;
-  __device__ __forceinline__ int column(int i) const { return (i * THREADS + thread) * VEC; }
-  __device__ __forceinline__ bool inside(int i) const { return column(i) < width; }
+  __device__ __forceinline__ int column(int i, int e) const {
+    return ALIGNED ? (i * kThreads + thread) * kChunk + e : (i * kChunk + e) * kThreads + thread;
+  }
+  __device__ __forceinline__ bool inside(int i, int e) const { return column(i, ALIGNED ? 0 : e) < width; }
+  // columns that warp w of the row's threads holds
+  __device__ __forceinline__ float held_by(int w) const {
+    int n = 0;
+    if (ALIGNED) {
+      for (int i = 0; i < NCH; ++i) n += max(0, min(32 * kChunk, width - (i * kThreads + w * 32) * kChunk));
+    } else {
+      for (int i = 0; i < NCH * kChunk; ++i) n += max(0, min(32, width - i * kThreads - w * 32));
+    }
+    return static_cast<float>(n);
+  }
 };
 
-template <typename T, int VEC, int NCH, int THREADS>
-__device__ __forceinline__ void load_row(const Span<VEC, NCH, THREADS>& sp, const T* p, float (&v)[NCH][VEC]) {
-#pragma unroll
-  for (int i = 0; i < NCH; ++i) {
-    if (sp.inside(i)) {
-      if constexpr (VEC == 1) v[i][0] = to_f32<T>(p[sp.column(i)]);
-      else load_aligned<VEC>(p + sp.column(i), v[i]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[i][e] = 0.0f;
+// The 8 elements of a chunk as they lie in memory, two to a register.
+struct RawChunk {
+  uint32_t w[4];
+};
+
+template <typename T, int WARPS, int NCH, bool ALIGNED>
+__device__ __forceinline__ void fetch(const Span<WARPS, NCH, ALIGNED>& sp, const T* row, int i, RawChunk& r) {
+  r.w[0] = r.w[1] = r.w[2] = r.w[3] = 0;
+  if constexpr (ALIGNED) {
+    if (sp.inside(i, 0)) {
+      const uint4 u = *reinterpret_cast<const uint4*>(row + sp.column(i, 0));
+      r.w[0] = u.x, r.w[1] = u.y, r.w[2] = u.z, r.w[3] = u.w;
     }
+  } else {
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+    for (int e = 0; e < kChunk; ++e)
+      if (sp.inside(i, e)) r.w[e >> 1] |= static_cast<uint32_t>(p[sp.column(i, e)]) << (16 * (e & 1));
   }
 }
 
-template <typename T, int VEC>
-__device__ __forceinline__ void load_chunk(const void* p, long long at, float (&v)[VEC]) {
-  if constexpr (VEC == 1) v[0] = to_f32<T>(static_cast<const T*>(p)[at]);
-  else load_aligned<VEC>(static_cast<const T*>(p) + at, v);
-}
-template <typename T, int VEC>
-__device__ __forceinline__ void store_chunk(void* p, long long at, const float (&v)[VEC]) {
-  if constexpr (VEC == 1) static_cast<T*>(p)[at] = from_f32<T>(v[0]);
-  else store_aligned<VEC>(static_cast<T*>(p) + at, v);
+template <typename T>
+__device__ __forceinline__ void widen(const RawChunk& r, float2 (&v)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = unpack2<T>(r.w[j]);
 }
 
-// (mean, rstd) of a row held in registers
-template <int WARPS, int VEC, int NCH, int THREADS>
-__device__ __forceinline__ void row_stats(const Span<VEC, NCH, THREADS>& sp, const float (&v)[NCH][VEC], int kind,
-                                          float eps, float& mean, float& rstd, float* buf) {
-  const float inv = 1.0f / static_cast<float>(sp.width);
-  mean = 0.0f;
-  if (kind == kNormLayer) {
-    float s[1] = {0.0f};
+// a vector's (gate, scale, ...) part of chunk i
+template <typename T, typename SP>
+__device__ __forceinline__ void load_part(const SP& sp, const void* p, long long at, int i, float2 (&v)[4]) {
+  RawChunk r;
+  fetch<T>(sp, static_cast<const T*>(p) + at, i, r);
+  widen<T>(r, v);
+}
+
+template <typename T, int WARPS, int NCH, bool ALIGNED>
+__device__ __forceinline__ void store(const Span<WARPS, NCH, ALIGNED>& sp, void* p, long long at, int i, const float2 (&v)[4]) {
+  T* row = static_cast<T*>(p) + at;
+  if constexpr (ALIGNED) {
+    if (sp.inside(i, 0))
+      *reinterpret_cast<uint4*>(row + sp.column(i, 0)) =
+          make_uint4(pack2<T>(v[0].x, v[0].y), pack2<T>(v[1].x, v[1].y), pack2<T>(v[2].x, v[2].y), pack2<T>(v[3].x, v[3].y));
+  } else {
+#pragma unroll
+    for (int e = 0; e < kChunk; ++e)
+      if (sp.inside(i, e)) row[sp.column(i, e)] = from_f32<T>(e & 1 ? v[e >> 1].y : v[e >> 1].x);
+  }
+}
+
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// v with the columns past the width set to 0
+template <typename SP>
+__device__ __forceinline__ float2 only_inside(const SP& sp, int i, int j, float2 v) {
+  if (!sp.inside(i, 2 * j)) v.x = 0.0f;
+  if (!sp.inside(i, 2 * j + 1)) v.y = 0.0f;
+  return v;
+}
+
+// ---- moments of a row ---------------------------------------------------------
+// mean and sum of squared deviations of the row's values, and the sums of a
+// second row d and of d times the deviations, on every thread of the row.  Each
+// warp takes its own mean first and all its sums around that mean; the warps'
+// results (one float4 each in ``buf``) are then moved to the common mean, so one
+// barrier per row is enough and nothing cancels where the mean is far from zero.
+struct Moments {
+  float mean, squares, sum_d, sum_dv;
+};
+
+// What a thread has to know of the row's division among warps.
+struct Shares {
+  float own_inv;  // 1 / columns of this warp (0: none)
+  float lane_n;   // columns of the warp that this lane reads in the second step
+};
+
+constexpr int warp_levels(int warps) { return warps <= 4 ? 2 : warps <= 8 ? 3 : warps <= 16 ? 4 : 5; }
+
+template <int WARPS, int NCH, bool ALIGNED>
+__device__ __forceinline__ Shares shares_of(const Span<WARPS, NCH, ALIGNED>& sp) {
+  const float own = sp.held_by(sp.thread >> 5);
+  const int w = sp.thread & ((1 << warp_levels(WARPS)) - 1);
+  return Shares{own > 0.0f ? 1.0f / own : 0.0f, WARPS > 1 && w < WARPS ? sp.held_by(w) : 0.0f};
+}
+
+template <int LEVELS>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = 1 << (LEVELS - 1); o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <bool WITH_D, int WARPS, int NCH, bool ALIGNED>
+__device__ __forceinline__ Moments row_moments(const Span<WARPS, NCH, ALIGNED>& sp, const Shares& share,
+                                               const float2 (&v)[NCH][4], const float2 (&d)[NCH][4], bool centred,
+                                               float inv_width, float4* buf) {
+  Moments m{0.0f, 0.0f, 0.0f, 0.0f};
+  if (centred) {
+    float2 s = both(0.0f);
 #pragma unroll
     for (int i = 0; i < NCH; ++i)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) s[0] += v[i][e];
-    row_sum<WARPS>(s, buf);
-    mean = s[0] * inv;
+      for (int j = 0; j < 4; ++j) s = fadd2(s, v[i][j]);
+    m.mean = warp_sum(s.x + s.y) * share.own_inv;
   }
-  float q[1] = {0.0f};
+  float2 q = both(0.0f), sd = both(0.0f), sv = both(0.0f);
+  const float2 minus = both(-m.mean);
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    if (sp.inside(i)) {
+    if (ALIGNED && !sp.inside(i, 0)) continue;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) q[0] = fmaf(v[i][e] - mean, v[i][e] - mean, q[0]);
+    for (int j = 0; j < 4; ++j) {
+      float2 dev = fadd2(v[i][j], minus);
+      if (!ALIGNED) dev = only_inside(sp, i, j, dev);
+      q = ffma2(dev, dev, q);
+      if (WITH_D) {
+        sd = fadd2(sd, d[i][j]);
+        sv = ffma2(d[i][j], dev, sv);
+      }
     }
   }
-  row_sum<WARPS>(q, buf + WARPS);
-  rstd = rsqrtf(q[0] * inv + eps);
+  m.squares = warp_sum(q.x + q.y);
+  if (WITH_D) {
+    m.sum_d = warp_sum(sd.x + sd.y);
+    m.sum_dv = warp_sum(sv.x + sv.y);
+  }
+  if constexpr (WARPS > 1) {
+    constexpr int kLevels = warp_levels(WARPS);
+    const int warp = sp.thread >> 5, lane = sp.thread & 31;
+    if (lane == 0) buf[warp] = make_float4(m.mean, m.squares, m.sum_d, m.sum_dv);
+    __syncthreads();
+    const int w = lane & ((1 << kLevels) - 1);
+    const float4 f = w < WARPS ? buf[w] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    m.mean = centred ? group_sum<kLevels>(share.lane_n * f.x) * inv_width : 0.0f;
+    const float shift = f.x - m.mean;  // unused warps: no columns and sums of 0
+    m.squares = group_sum<kLevels>(fmaf(share.lane_n * shift, shift, f.y));
+    if (WITH_D) {
+      m.sum_d = group_sum<kLevels>(f.z);
+      m.sum_dv = group_sum<kLevels>(fmaf(shift, f.z, f.w));
+    }
+  }
+  return m;
 }
 
 // ---- forward --------------------------------------------------------------------
-// WARPS warps per row; a block of at least four warps holds 4 / WARPS rows
-// when a row needs fewer.
-template <typename T, int VEC, int WARPS, int NCH, bool POST>
+// Blocks stay and walk the rows: WARPS warps per row (a block of four warps
+// holds four rows when one warp is enough).  The next row's loads are issued as
+// soon as the current row is in fp32 registers, before its reduction.
+template <typename T, int WARPS, int NCH, bool ALIGNED, bool POST>
 __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS) norm_forward_kernel(const __grid_constant__ NormArgs a) {
   static_assert(WARPS == 1 || WARPS >= 4, "rows of two warps would share block barriers");
   constexpr int kThreads = 32 * WARPS;
-  constexpr int kRows = WARPS < 4 ? 4 / WARPS : 1;
-  __shared__ float buf[4 * (WARPS < 4 ? 1 : WARPS)];
+  constexpr unsigned kRows = WARPS < 4 ? 4 / WARPS : 1;
+  __shared__ float4 buf[2][2][WARPS];  // alternates between rows: a row's last read may meet the next one's write
   const int slot = threadIdx.x / kThreads;
-  const long long row = static_cast<long long>(blockIdx.x) * kRows + slot;
-  if (row >= static_cast<long long>(a.samples) * a.rows) return;  // whole warps only: kRows > 1 means one warp per row
-  const int sample = static_cast<int>(row / a.rows);
-  const long long at = row - static_cast<long long>(sample) * a.rows;
-  const Span<VEC, NCH, kThreads> sp{static_cast<int>(threadIdx.x) - slot * kThreads, a.width};
-  float r[NCH][VEC];
-  load_row(sp, static_cast<const T*>(a.x.p) + sample * a.x.sb + at * a.x.sn, r);
-  if (a.branch.p) {
-    float b[NCH][VEC];
-    load_row(sp, static_cast<const T*>(a.branch.p) + sample * a.branch.sb + at * a.branch.sn, b);
+  const Span<WARPS, NCH, ALIGNED> sp{static_cast<int>(threadIdx.x) - slot * kThreads, a.width};
+  const Shares share = shares_of(sp);
+  const float inv = 1.0f / static_cast<float>(a.width);
+  const unsigned total = static_cast<unsigned>(a.samples) * a.rows, step = gridDim.x * kRows;  // below 2^31
+  unsigned row = blockIdx.x * kRows + slot;
+  if (row >= total) return;  // whole warps only: kRows > 1 means one warp per row
+  unsigned sample = row / a.rows, at = row - sample * a.rows;
+  auto row_of = [&](const RowTensor& t) { return static_cast<const T*>(t.p) + sample * t.sb + at * t.sn; };
+  RawChunk raw_x[NCH], raw_b[NCH];
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    fetch(sp, row_of(a.x), i, raw_x[i]);
+    if (a.branch.p) fetch(sp, row_of(a.branch), i, raw_b[i]);
+  }
+  const float2 rs = both(a.residual_scale);
+  int turn = 0;
+  while (row < total) {
+    float2 r[NCH][4];
+    const long long out = static_cast<long long>(row) * a.width;
+    const long long gate_at = sample * a.gate.sb, scale_at = sample * a.scale.sb, shift_at = sample * a.shift.sb;
+    float2 pscale = both(1.0f), pshift = both(0.0f);  // post norm: b * rstd - mean * rstd
     if constexpr (POST) {
-      float mean, rstd;
-      row_stats<WARPS>(sp, b, a.post, a.post_eps, mean, rstd, buf + 2 * WARPS);
+      float2 b[NCH][4];
 #pragma unroll
-      for (int i = 0; i < NCH; ++i) {
-        if (!sp.inside(i)) continue;
-        float w[VEC];
-        if (a.post_weight) load_chunk<T>(a.post_weight, sp.column(i), w);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          b[i][e] = (b[i][e] - mean) * rstd;
-          if (a.post_weight) b[i][e] *= w[e];
-        }
-      }
+      for (int i = 0; i < NCH; ++i) widen<T>(raw_b[i], b[i]);
+      const Moments m = row_moments<false>(sp, share, b, b, a.post == kNormLayer, inv, buf[turn][1]);
+      const float rstd = rsqrtf(m.squares * inv + a.post_eps);
+      pscale = both(rstd);
+      pshift = both(-m.mean * rstd);
     }
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      if (!sp.inside(i)) continue;
-      float g[VEC];
-      if (a.gate.p) load_chunk<T>(a.gate.p, sample * a.gate.sb + sp.column(i), g);
+      widen<T>(raw_x[i], r[i]);
+      if (a.branch.p) {
+        float2 b[4], g[4];
+        widen<T>(raw_b[i], b);
+        if constexpr (POST) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float gb = a.gate.p ? g[e] * b[i][e] : b[i][e];
-        r[i][e] = fmaf(a.residual_scale, r[i][e], gb);
+          for (int j = 0; j < 4; ++j) b[j] = ffma2(b[j], pscale, pshift);
+          if (a.post_weight) {
+            load_part<T>(sp, a.post_weight, 0, i, g);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j] = fmul2(b[j], g[j]);
+          }
+          if (!ALIGNED || !sp.inside(i, 0)) {  // the shift of columns past the width
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j] = only_inside(sp, i, j, b[j]);
+          }
+        }
+        if (a.gate.p) {
+          load_part<T>(sp, a.gate.p, gate_at, i, g);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) b[j] = fmul2(b[j], g[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[i][j] = ffma2(rs, r[i][j], b[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[i][j] = fmul2(rs, r[i][j]);
       }
     }
-  } else {
+    row += step;
+    if (row < total) {
+      sample = row / a.rows;
+      at = row - sample * a.rows;
 #pragma unroll
-    for (int i = 0; i < NCH; ++i)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) r[i][e] *= a.residual_scale;
-  }
-  const long long out = row * a.width;
-  if (a.out_r) {
-#pragma unroll
-    for (int i = 0; i < NCH; ++i)
-      if (sp.inside(i)) store_chunk<T>(a.out_r, out + sp.column(i), r[i]);
-  }
-  float mean, rstd;
-  row_stats<WARPS>(sp, r, a.norm, a.eps, mean, rstd, buf);
-#pragma unroll
-  for (int i = 0; i < NCH; ++i) {
-    if (!sp.inside(i)) continue;
-    float w[VEC], s[VEC], t[VEC];
-    if (a.weight) load_chunk<T>(a.weight, sp.column(i), w);
-    if (a.scale.p) load_chunk<T>(a.scale.p, sample * a.scale.sb + sp.column(i), s);
-    if (a.shift.p) load_chunk<T>(a.shift.p, sample * a.shift.sb + sp.column(i), t);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      float y = (r[i][e] - mean) * rstd;
-      if (a.weight) y *= w[e];
-      if (a.scale.p) y *= 1.0f + s[e];
-      if (a.shift.p) y += t[e];
-      r[i][e] = y;
+      for (int i = 0; i < NCH; ++i) {
+        fetch(sp, row_of(a.x), i, raw_x[i]);
+        if (a.branch.p) fetch(sp, row_of(a.branch), i, raw_b[i]);
+      }
     }
-    store_chunk<T>(a.out_h, out + sp.column(i), r[i]);
+    if (a.out_r) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) store<T>(sp, a.out_r, out, i, r[i]);
+    }
+    const Moments m = row_moments<false>(sp, share, r, r, a.norm == kNormLayer, inv, buf[turn][0]);
+    turn ^= 1;
+    const float rstd = rsqrtf(m.squares * inv + a.eps);
+    const float2 minus = both(-m.mean), times = both(rstd);
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      float2 f[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[i][j] = fmul2(fadd2(r[i][j], minus), times);
+      if (a.weight) {
+        load_part<T>(sp, a.weight, 0, i, f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[i][j] = fmul2(r[i][j], f[j]);
+      }
+      if (a.scale.p) {
+        load_part<T>(sp, a.scale.p, scale_at, i, f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[i][j] = fmul2(r[i][j], fadd2(f[j], both(1.0f)));
+      }
+      if (a.shift.p) {
+        load_part<T>(sp, a.shift.p, shift_at, i, f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[i][j] = fadd2(r[i][j], f[j]);
+      }
+      store<T>(sp, a.out_h, out, i, r[i]);
+    }
   }
 }
 
 // ---- backward ---------------------------------------------------------------------
-// A block takes every chunks-th row of one sample and keeps its threads'
-// column sums in registers; a second kernel adds the blocks' sums in order.
-template <typename T, int VEC, int WARPS, int NCH, bool POST>
+// A block takes every chunks-th row of one sample and keeps its column sums,
+// each with the thread that owns the column, in registers or (more than three
+// chunks a thread) in shared memory; a second kernel adds the blocks' sums in
+// order.  A register that held a piece of the row takes the next row's piece as
+// soon as it is free.
+template <typename T, int WARPS, int NCH, bool ALIGNED, bool POST>
 __global__ void __launch_bounds__(32 * WARPS) norm_backward_kernel(const __grid_constant__ NormArgs a) {
   constexpr int kThreads = 32 * WARPS;
-  __shared__ float buf[2][8 * WARPS];  // double-buffered between rows: one row's last read may meet the next one's write
-  const int sample = blockIdx.x / a.chunks, chunk = blockIdx.x - sample * a.chunks;
-  const Span<VEC, NCH, kThreads> sp{static_cast<int>(threadIdx.x), a.width};
+  __shared__ float4 buf[2][3][WARPS];  // alternates between rows: a row's last read may meet the next one's write
+  const unsigned sample = blockIdx.x / a.chunks, chunk = blockIdx.x - sample * a.chunks;
+  const Span<WARPS, NCH, ALIGNED> sp{static_cast<int>(threadIdx.x), a.width};
+  const Shares share = shares_of(sp);
   const float inv = 1.0f / static_cast<float>(a.width);
-  float a0[NCH][VEC], a1[NCH][VEC], g0[NCH][VEC];
+  constexpr bool kShared = NCH > 3;
+  extern __shared__ float shared_sums[];  // [3][NCH * 8][threads]: a thread's own entries, bank by bank
+  constexpr int kR = kShared ? 1 : NCH;
+  float2 a0[kR][4], a1[kR][4], g0[kR][4];
 #pragma unroll
-  for (int i = 0; i < NCH; ++i)
+  for (int i = 0; i < kR; ++i)
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) a0[i][e] = a1[i][e] = g0[i][e] = 0.0f;
+    for (int j = 0; j < 4; ++j) a0[i][j] = a1[i][j] = g0[i][j] = both(0.0f);
+  auto shared_at = [&](int k, int i, int j) {
+    return reinterpret_cast<float2*>(shared_sums) + ((k * NCH + i) * 4 + j) * kThreads + threadIdx.x;
+  };
+  if (kShared) {
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+      for (int j = 0; j < 4; ++j)
+        for (int k = 0; k < 3; ++k) *shared_at(k, i, j) = both(0.0f);
+  }
+  const long long gate_at = sample * a.gate.sb, scale_at = sample * a.scale.sb;
+  auto row_of = [&](const RowTensor& t, unsigned at) { return static_cast<const T*>(t.p) + sample * t.sb + at * t.sn; };
+  RawChunk raw_x[NCH], raw_d[NCH], raw_b[NCH], raw_e[NCH];
+  const unsigned rows = a.rows, stride = a.chunks;
+  if (chunk < rows) {
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      fetch(sp, row_of(a.x, chunk), i, raw_x[i]);
+      fetch(sp, row_of(a.grad_h, chunk), i, raw_d[i]);
+      if (a.branch.p) fetch(sp, row_of(a.branch, chunk), i, raw_b[i]);
+      if (a.grad_r.p) fetch(sp, row_of(a.grad_r, chunk), i, raw_e[i]);
+    }
+  }
+  const float2 rs = both(a.residual_scale);
   int turn = 0;
-  for (int at = chunk; at < a.rows; at += a.chunks, turn ^= 1) {
-    float* bf = buf[turn];
-    const long long out = (static_cast<long long>(sample) * a.rows + at) * a.width;
-    float r[NCH][VEC], d[NCH][VEC], b[NCH][VEC];
-    load_row(sp, static_cast<const T*>(a.x.p) + sample * a.x.sb + at * a.x.sn, r);
-    load_row(sp, static_cast<const T*>(a.grad_h.p) + sample * a.grad_h.sb + at * a.grad_h.sn, d);
-    float pmean = 0.0f, prstd = 1.0f;
-    if (a.branch.p) {
-      load_row(sp, static_cast<const T*>(a.branch.p) + sample * a.branch.sb + at * a.branch.sn, b);
-      if constexpr (POST) {
-        row_stats<WARPS>(sp, b, a.post, a.post_eps, pmean, prstd, bf);
+  for (unsigned at = chunk; at < rows; at += stride, turn ^= 1) {
+    const long long out = (static_cast<long long>(sample) * rows + at) * a.width;
+    const unsigned next = at + stride;
+    float2 r[NCH][4], dn[NCH][4];
+    float2 pscale = both(1.0f), pshift = both(0.0f);  // post norm: b * rstd - mean * rstd
+    float prstd = 1.0f;
+    if constexpr (POST) {
+      float2 b[NCH][4];
 #pragma unroll
-        for (int i = 0; i < NCH; ++i)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) b[i][e] = sp.inside(i) ? (b[i][e] - pmean) * prstd : 0.0f;
-      }
+      for (int i = 0; i < NCH; ++i) widen<T>(raw_b[i], b[i]);
+      const Moments m = row_moments<false>(sp, share, b, b, a.post == kNormLayer, inv, buf[turn][1]);
+      prstd = rsqrtf(m.squares * inv + a.post_eps);
+      pscale = both(prstd);
+      pshift = both(-m.mean * prstd);
     }
+    // r and dn = dh (1 + scale) weight
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      if (!sp.inside(i)) continue;
-      float g[VEC], w[VEC];
-      if (a.gate.p) load_chunk<T>(a.gate.p, sample * a.gate.sb + sp.column(i), g);
-      if (POST && a.post_weight) load_chunk<T>(a.post_weight, sp.column(i), w);
+      float2 f[4];
+      widen<T>(raw_x[i], r[i]);
+      if (next < rows) fetch(sp, row_of(a.x, next), i, raw_x[i]);
+      if (a.branch.p) {
+        float2 b[4];
+        widen<T>(raw_b[i], b);
+        if constexpr (POST) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        float gb = 0.0f;
-        if (a.branch.p) {
-          gb = b[i][e];
-          if (POST && a.post_weight) gb *= w[e];
-          if (a.gate.p) gb *= g[e];
-        }
-        r[i][e] = fmaf(a.residual_scale, r[i][e], gb);
-      }
-    }
-    float mean, rstd;
-    row_stats<WARPS>(sp, r, a.norm, a.eps, mean, rstd, bf + 2 * WARPS);
-    // r -> n, d -> dn, and the two means of the norm's gradient
-    float m[2] = {0.0f, 0.0f};
+          for (int j = 0; j < 4; ++j) b[j] = ffma2(b[j], pscale, pshift);
+          if (a.post_weight) {
+            load_part<T>(sp, a.post_weight, 0, i, f);
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      if (!sp.inside(i)) continue;
-      float w[VEC], s[VEC];
-      if (a.weight) load_chunk<T>(a.weight, sp.column(i), w);
-      if (a.scale.p) load_chunk<T>(a.scale.p, sample * a.scale.sb + sp.column(i), s);
+            for (int j = 0; j < 4; ++j) b[j] = fmul2(b[j], f[j]);
+          }
+          if (!ALIGNED || !sp.inside(i, 0)) {  // the shift of columns past the width
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float n = (r[i][e] - mean) * rstd;
-        float dn = d[i][e];
-        a0[i][e] += dn;
-        a1[i][e] = fmaf(dn, n, a1[i][e]);
-        if (a.scale.p) dn *= 1.0f + s[e];
-        if (a.weight) dn *= w[e];
-        m[0] += dn;
-        m[1] = fmaf(dn, n, m[1]);
-        r[i][e] = n;
-        d[i][e] = dn;
-      }
-    }
-    row_sum<WARPS>(m, bf + 4 * WARPS);
-    const float mean_dn = a.norm == kNormLayer ? m[0] * inv : 0.0f, mean_dnn = m[1] * inv;
-    float pm[2] = {0.0f, 0.0f};
-#pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      if (!sp.inside(i)) continue;
-      float e4[VEC], g[VEC], w[VEC];
-      if (a.grad_r.p) load_chunk<T>(a.grad_r.p, sample * a.grad_r.sb + at * a.grad_r.sn + sp.column(i), e4);
-      if (a.gate.p) load_chunk<T>(a.gate.p, sample * a.gate.sb + sp.column(i), g);
-      if (POST && a.post_weight) load_chunk<T>(a.post_weight, sp.column(i), w);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        float dr = rstd * (d[i][e] - mean_dn - r[i][e] * mean_dnn);
-        if (a.grad_r.p) dr += e4[e];
-        r[i][e] = a.residual_scale * dr;
-        if (a.branch.p) {
-          g0[i][e] = fmaf(dr, b[i][e], g0[i][e]);
-          float db = a.gate.p ? dr * g[e] : dr;
-          if (POST && a.post_weight) db *= w[e];
-          d[i][e] = db;
-          if (POST) {
-            pm[0] += db;
-            pm[1] = fmaf(db, b[i][e], pm[1]);
+            for (int j = 0; j < 4; ++j) b[j] = only_inside(sp, i, j, b[j]);
           }
         }
+        if (a.gate.p) {
+          load_part<T>(sp, a.gate.p, gate_at, i, f);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) b[j] = fmul2(b[j], f[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[i][j] = ffma2(rs, r[i][j], b[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[i][j] = fmul2(rs, r[i][j]);
       }
-      if (a.out_h) store_chunk<T>(a.out_h, out + sp.column(i), r[i]);
-      if (!POST && a.out_r) store_chunk<T>(a.out_r, out + sp.column(i), d[i]);
+      widen<T>(raw_d[i], dn[i]);
+      if (a.scale.p) {
+        load_part<T>(sp, a.scale.p, scale_at, i, f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dn[i][j] = ffma2(dn[i][j], f[j], dn[i][j]);
+      }
+      if (a.weight) {
+        load_part<T>(sp, a.weight, 0, i, f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dn[i][j] = fmul2(dn[i][j], f[j]);
+      }
+    }
+    const Moments m = row_moments<true>(sp, share, r, dn, a.norm == kNormLayer, inv, buf[turn][0]);
+    const float rstd = rsqrtf(m.squares * inv + a.eps);
+    const float mean_dn = a.norm == kNormLayer ? m.sum_d * inv : 0.0f, mean_dnn = m.sum_dv * rstd * inv;
+    const float2 minus = both(-m.mean), times = both(rstd);
+    const float2 c_dn = both(-mean_dn * rstd), c_n = both(-mean_dnn * rstd);  // dr = rstd dn + c_dn + c_n n
+    float2 v[POST ? NCH : 1][4];  // post norm: the branch's row once more
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      float2 d[4], b[4], e4[4], g[4], pw[4];
+      widen<T>(raw_d[i], d);
+      if (a.branch.p) widen<T>(raw_b[i], b);
+      if (a.grad_r.p) widen<T>(raw_e[i], e4);
+      if (next < rows) {
+        fetch(sp, row_of(a.grad_h, next), i, raw_d[i]);
+        if (a.branch.p) fetch(sp, row_of(a.branch, next), i, raw_b[i]);
+        if (a.grad_r.p) fetch(sp, row_of(a.grad_r, next), i, raw_e[i]);
+      }
+      if (a.gate.p) load_part<T>(sp, a.gate.p, gate_at, i, g);
+      if (POST && a.post_weight) load_part<T>(sp, a.post_weight, 0, i, pw);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 n = fmul2(fadd2(r[i][j], minus), times);
+        float2 dr = ffma2(dn[i][j], times, ffma2(n, c_n, c_dn));
+        if (a.grad_r.p) dr = fadd2(dr, e4[j]);
+        float2 pn = both(0.0f);
+        if (a.branch.p) {
+          pn = b[j];
+          if constexpr (POST) {
+            v[i][j] = b[j];
+            pn = ffma2(b[j], pscale, pshift);
+          }
+          float2 db = a.gate.p ? fmul2(dr, g[j]) : dr;
+          if (POST && a.post_weight) db = fmul2(db, pw[j]);
+          if (POST) db = only_inside(sp, i, j, db);
+          dn[i][j] = db;
+        }
+        if constexpr (kShared) {
+          *shared_at(0, i, j) = fadd2(*shared_at(0, i, j), d[j]);
+          *shared_at(1, i, j) = ffma2(d[j], n, *shared_at(1, i, j));
+          *shared_at(2, i, j) = ffma2(dr, pn, *shared_at(2, i, j));
+        } else {
+          a0[i][j] = fadd2(a0[i][j], d[j]);
+          a1[i][j] = ffma2(d[j], n, a1[i][j]);
+          g0[i][j] = ffma2(dr, pn, g0[i][j]);
+        }
+        r[i][j] = fmul2(rs, dr);
+      }
+      if (a.out_h) store<T>(sp, a.out_h, out, i, r[i]);
+      if (!POST && a.out_r) store<T>(sp, a.out_r, out, i, dn[i]);
     }
     if constexpr (POST) {
-      row_sum<WARPS>(pm, bf + 6 * WARPS);
-      const float pmean_d = a.post == kNormLayer ? pm[0] * inv : 0.0f, pmean_dn = pm[1] * inv;
+      // through the post norm: dn holds the gradient of its output, whose sums
+      // with the branch's deviations are taken here (their squares are known)
+      const Moments q = row_moments<true>(sp, share, v, dn, a.post == kNormLayer, inv, buf[turn][2]);
+      const float pmean_d = a.post == kNormLayer ? q.sum_d * inv : 0.0f, pmean_dn = q.sum_dv * prstd * inv;
+      const float2 c_d = both(-pmean_d * prstd), c_pn = both(-pmean_dn * prstd);
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
-        if (!sp.inside(i)) continue;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) d[i][e] = prstd * (d[i][e] - pmean_d - b[i][e] * pmean_dn);
-        if (a.out_r) store_chunk<T>(a.out_r, out + sp.column(i), d[i]);
+        for (int j = 0; j < 4; ++j)
+          dn[i][j] = ffma2(dn[i][j], pscale, ffma2(ffma2(v[i][j], pscale, pshift), c_pn, c_d));
+        if (a.out_r) store<T>(sp, a.out_r, out, i, dn[i]);
       }
     }
   }
@@ -347,13 +522,17 @@ __global__ void __launch_bounds__(32 * WARPS) norm_backward_kernel(const __grid_
     float* part = a.partial + static_cast<long long>(blockIdx.x) * 3 * a.width;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      if (!sp.inside(i)) continue;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const int c = sp.column(i) + e;
-        part[c] = a0[i][e];
-        part[a.width + c] = a1[i][e];
-        part[2LL * a.width + c] = g0[i][e];
+      for (int e = 0; e < kChunk; ++e) {
+        if (!sp.inside(i, e)) continue;
+        const int c = sp.column(i, e);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          float2 s;
+          if constexpr (kShared) s = *shared_at(k, i, e >> 1);
+          else s = k == 0 ? a0[i][e >> 1] : k == 1 ? a1[i][e >> 1] : g0[i][e >> 1];
+          part[static_cast<long long>(k) * a.width + c] = e & 1 ? s.y : s.x;
+        }
       }
     }
   }
@@ -369,99 +548,127 @@ struct NormSumsArgs {
   int samples, chunks, width;
 };
 
-// Column sums of the blocks' partials: 32 columns x 16 lanes of chunks per
-// block, lanes added in order, samples one after the other.
+// Column sums of the blocks' partials: 32 columns x 32 lanes of chunks per
+// block, lanes added in order, samples one after the other.  blockIdx.y picks
+// A0 (dshift), A1 (dscale, dweight) or G (dgate, dpost).
 template <typename T>
-__global__ void __launch_bounds__(512) norm_sums_kernel(const __grid_constant__ NormSumsArgs a) {
-  __shared__ float red[3][16][33];
-  const int cx = threadIdx.x & 31, y = threadIdx.x >> 5;
+__global__ void __launch_bounds__(1024) norm_sums_kernel(const __grid_constant__ NormSumsArgs a) {
+  __shared__ float red[32][33];
+  const int cx = threadIdx.x & 31, y = threadIdx.x >> 5, k = blockIdx.y;
   const int c = blockIdx.x * 32 + cx;
-  float dweight = 0.0f, dpost = 0.0f, dgate = 0.0f, dscale = 0.0f, dshift = 0.0f;
+  void* each = k == 0 ? a.dshift : k == 1 ? a.dscale : a.dgate;      // one vector per sample, or their sum
+  void* all = k == 0 ? nullptr : k == 1 ? a.dweight : a.dpost;       // summed over the samples
+  const int shared = k == 0 ? a.shift_shared : k == 1 ? a.scale_shared : a.gate_shared;
+  if (!each && !all) return;
+  float sum_each = 0.0f, sum_all = 0.0f;
   for (int b = 0; b < a.samples; ++b) {
-    float s[3] = {0.0f, 0.0f, 0.0f};
+    float s = 0.0f;
     if (c < a.width) {
+      const float* p = a.partial + static_cast<long long>(b) * a.chunks * 3 * a.width + static_cast<long long>(k) * a.width + c;
 #pragma unroll 4
-      for (int i = y; i < a.chunks; i += 16) {
-        const float* p = a.partial + (static_cast<long long>(b) * a.chunks + i) * 3 * a.width + c;
-        s[0] += p[0];
-        s[1] += p[a.width];
-        s[2] += p[2LL * a.width];
-      }
+      for (int i = y; i < a.chunks; i += 32) s += p[static_cast<long long>(i) * 3 * a.width];
     }
-#pragma unroll
-    for (int k = 0; k < 3; ++k) red[k][y][cx] = s[k];
+    red[y][cx] = s;
     __syncthreads();
     if (y == 0 && c < a.width) {
-      float t[3] = {0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int k = 0; k < 3; ++k)
-        for (int i = 0; i < 16; ++i) t[k] += red[k][i][cx];
-      const float gate = a.gate.p ? to_f32<T>(static_cast<const T*>(a.gate.p)[b * a.gate.sb + c]) : 1.0f;
-      const float scale = a.scale.p ? to_f32<T>(static_cast<const T*>(a.scale.p)[b * a.scale.sb + c]) : 0.0f;
-      const float w = a.weight ? to_f32<T>(static_cast<const T*>(a.weight)[c]) : 1.0f;
-      const float pw = a.post_weight ? to_f32<T>(static_cast<const T*>(a.post_weight)[c]) : 1.0f;
-      const long long at = static_cast<long long>(b) * a.width + c;
-      dweight = fmaf(1.0f + scale, t[1], dweight);
-      dpost = fmaf(gate, t[2], dpost);
-      dshift = a.shift_shared ? dshift + t[0] : t[0];
-      dscale = a.scale_shared ? fmaf(w, t[1], dscale) : w * t[1];
-      dgate = a.gate_shared ? fmaf(pw, t[2], dgate) : pw * t[2];
-      if (a.dshift && !a.shift_shared) static_cast<T*>(a.dshift)[at] = from_f32<T>(dshift);
-      if (a.dscale && !a.scale_shared) static_cast<T*>(a.dscale)[at] = from_f32<T>(dscale);
-      if (a.dgate && !a.gate_shared) static_cast<T*>(a.dgate)[at] = from_f32<T>(dgate);
+      float t = 0.0f;
+      for (int i = 0; i < 32; ++i) t += red[i][cx];
+      float factor = 1.0f, other = 1.0f;
+      if (k == 1) {
+        if (a.weight) factor = to_f32<T>(static_cast<const T*>(a.weight)[c]);
+        if (a.scale.p) other = 1.0f + to_f32<T>(static_cast<const T*>(a.scale.p)[b * a.scale.sb + c]);
+      } else if (k == 2) {
+        if (a.post_weight) factor = to_f32<T>(static_cast<const T*>(a.post_weight)[c]);
+        if (a.gate.p) other = to_f32<T>(static_cast<const T*>(a.gate.p)[b * a.gate.sb + c]);
+      }
+      sum_all = fmaf(other, t, sum_all);
+      sum_each = shared ? fmaf(factor, t, sum_each) : factor * t;
+      if (each && !shared) static_cast<T*>(each)[static_cast<long long>(b) * a.width + c] = from_f32<T>(sum_each);
     }
     __syncthreads();
   }
   if (y == 0 && c < a.width) {
-    if (a.dshift && a.shift_shared) static_cast<T*>(a.dshift)[c] = from_f32<T>(dshift);
-    if (a.dscale && a.scale_shared) static_cast<T*>(a.dscale)[c] = from_f32<T>(dscale);
-    if (a.dgate && a.gate_shared) static_cast<T*>(a.dgate)[c] = from_f32<T>(dgate);
-    if (a.dweight) static_cast<T*>(a.dweight)[c] = from_f32<T>(dweight);
-    if (a.dpost) static_cast<T*>(a.dpost)[c] = from_f32<T>(dpost);
+    if (each && shared) static_cast<T*>(each)[c] = from_f32<T>(sum_each);
+    if (all) static_cast<T*>(all)[c] = from_f32<T>(sum_all);
   }
 }
 
 // ---- host side -----------------------------------------------------------------------
 constexpr int kMaxWidth = 16384;
 
-template <typename T, int VEC, int WARPS, int NCH>
+// Resident blocks of a kernel per SM, asked once.
+int blocks_per_sm(const void* kernel, int threads, std::atomic<int>& known) {
+  int n = known.load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != cudaSuccess || n < 1) return 1;
+  known.store(n, std::memory_order_relaxed);
+  return n;
+}
+
+template <typename T, int WARPS, int NCH, bool ALIGNED, bool POST>
 int launch_one(const NormArgs& a, bool backward, cudaStream_t stream) {
-  const bool post = a.post != kNormNone;
   if (backward) {
-    const int grid = a.samples * a.chunks;
-    if (post) norm_backward_kernel<T, VEC, WARPS, NCH, true><<<grid, 32 * WARPS, 0, stream>>>(a);
-    else norm_backward_kernel<T, VEC, WARPS, NCH, false><<<grid, 32 * WARPS, 0, stream>>>(a);
+    auto kernel = norm_backward_kernel<T, WARPS, NCH, ALIGNED, POST>;
+    constexpr int kSmem = NCH > 3 ? 3 * NCH * kChunk * 32 * WARPS * 4 : 0;  // the column sums
+    if (kSmem > 0) {  // granted once per device
+      static std::atomic<unsigned long long> opened;
+      int dev = 0;
+      cudaError_t e = cudaGetDevice(&dev);
+      if (e != cudaSuccess) return static_cast<int>(e);
+      const unsigned long long bit = 1ull << (dev & 63);
+      if (dev >= 64 || !(opened.load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        if (e != cudaSuccess) return static_cast<int>(e);
+        opened.fetch_or(bit, std::memory_order_relaxed);
+      }
+    }
+    kernel<<<a.samples * a.chunks, 32 * WARPS, kSmem, stream>>>(a);
   } else {
-    constexpr int kRows = WARPS < 4 ? 4 / WARPS : 1;
-    const long long rows = static_cast<long long>(a.samples) * a.rows;
-    const unsigned grid = static_cast<unsigned>((rows + kRows - 1) / kRows);
-    if (post) norm_forward_kernel<T, VEC, WARPS, NCH, true><<<grid, WARPS < 4 ? 128 : 32 * WARPS, 0, stream>>>(a);
-    else norm_forward_kernel<T, VEC, WARPS, NCH, false><<<grid, WARPS < 4 ? 128 : 32 * WARPS, 0, stream>>>(a);
+    constexpr int kRows = WARPS < 4 ? 4 / WARPS : 1, kBlock = WARPS < 4 ? 128 : 32 * WARPS;
+    auto kernel = norm_forward_kernel<T, WARPS, NCH, ALIGNED, POST>;
+    static std::atomic<int> resident;
+    const long long want = (static_cast<long long>(a.samples) * a.rows + kRows - 1) / kRows;
+    const long long most = static_cast<long long>(kNumSMs) * blocks_per_sm(reinterpret_cast<const void*>(kernel), kBlock, resident);
+    kernel<<<static_cast<unsigned>(want < most ? want : most), kBlock, 0, stream>>>(a);
   }
   return launch_status();
 }
 
-template <typename T>
-int launch_norm(const NormArgs& a, bool backward, cudaStream_t stream) {
+// Warps per row: the fewest whose threads hold the row in three chunks each
+// (few warps make the row's reduction cheap), more chunks only past 8192 columns.
+template <typename T, bool ALIGNED, bool POST>
+int launch_width(const NormArgs& a, bool backward, cudaStream_t stream) {
   const int w = a.width;
-  if (a.vec) {
-    if (w <= 512) return launch_one<T, 8, 1, 2>(a, backward, stream);
-    if (w <= 1024) return launch_one<T, 8, 4, 1>(a, backward, stream);
-    if (w <= 2048) return launch_one<T, 8, 4, 2>(a, backward, stream);
-    if (w <= 3072) return launch_one<T, 8, 4, 3>(a, backward, stream);
-    if (w <= 6144) return launch_one<T, 8, 8, 3>(a, backward, stream);
-    return launch_one<T, 8, 16, 4>(a, backward, stream);
-  }
-  if (w <= 1024) return launch_one<T, 1, 4, 8>(a, backward, stream);
-  if (w <= 4096) return launch_one<T, 1, 8, 16>(a, backward, stream);
-  return launch_one<T, 1, 16, 32>(a, backward, stream);
+  if (w <= 256) return launch_one<T, 1, 1, ALIGNED, POST>(a, backward, stream);
+  if (w <= 768) return launch_one<T, 1, 3, ALIGNED, POST>(a, backward, stream);
+  if (w <= 1024) return launch_one<T, 4, 1, ALIGNED, POST>(a, backward, stream);
+  if (w <= 2048) return launch_one<T, 4, 2, ALIGNED, POST>(a, backward, stream);
+  if (w <= 3072) return launch_one<T, 4, 3, ALIGNED, POST>(a, backward, stream);
+  if (w <= 4096) return launch_one<T, 8, 2, ALIGNED, POST>(a, backward, stream);
+  if (w <= 6144) return launch_one<T, 8, 3, ALIGNED, POST>(a, backward, stream);
+  if (w <= 8192) return launch_one<T, 16, 2, ALIGNED, POST>(a, backward, stream);
+  return launch_one<T, 16, 4, ALIGNED, POST>(a, backward, stream);
 }
 
-// Row chunks per sample of the backward kernel: about two blocks per SM
-// (their partial sums are a small part of the traffic), fewer for short samples.
-int norm_chunks(int samples, int rows) {
+template <typename T>
+int launch_norm(const NormArgs& a, bool backward, cudaStream_t stream) {
+  if (a.vec)
+    return a.post ? launch_width<T, true, true>(a, backward, stream) : launch_width<T, true, false>(a, backward, stream);
+  return a.post ? launch_width<T, false, true>(a, backward, stream) : launch_width<T, false, false>(a, backward, stream);
+}
+
+// Row chunks per sample of the backward kernel, one block each: as many as are
+// resident at about 8 warps per SM, but 8 rows each at least, so that the
+// partial sums stay a small part of the traffic.
+int norm_chunks(int samples, int rows, int width) {
   if (samples < 1) return 1;
-  long long chunks = (2LL * kNumSMs + samples - 1) / samples;
+  const int warps = width <= 768 ? 1 : width <= 3072 ? 4 : width <= 6144 ? 8 : 16;
+  const long long per_sm = warps > 8 ? 1 : 8 / warps;
+  long long chunks = (per_sm * kNumSMs + samples - 1) / samples;
+  const long long fewest = kNumSMs / samples + 1;  // short inputs still spread over the SMs
+  long long most = (rows + 7) / 8;
+  if (most < fewest) most = fewest;
+  if (chunks > most) chunks = most;
   if (chunks > rows) chunks = rows;
   return chunks < 1 ? 1 : static_cast<int>(chunks);
 }
@@ -520,7 +727,7 @@ extern "C" int peco_gated_norm(const void* x, long long x_batch, long long x_row
 
 extern "C" long long peco_gated_norm_backward_workspace(int samples, int rows, int width) {
   if (samples < 0 || rows < 0 || width < 1) return -1;
-  return 12LL * samples * norm_chunks(samples, rows) * width;
+  return 12LL * samples * norm_chunks(samples, rows, width) * width;
 }
 
 extern "C" int peco_gated_norm_backward(
@@ -568,7 +775,7 @@ extern "C" int peco_gated_norm_backward(
   a.eps = eps;
   a.post_eps = post_eps;
   a.residual_scale = residual_scale;
-  a.chunks = norm_chunks(samples, rows);
+  a.chunks = norm_chunks(samples, rows, width);
   int st = dtype == 1 ? launch_norm<__nv_bfloat16>(a, true, stream) : launch_norm<__half>(a, true, stream);
   if (st || !sums) return st;
   NormSumsArgs s{};
@@ -588,8 +795,8 @@ extern "C" int peco_gated_norm_backward(
   s.samples = samples;
   s.chunks = a.chunks;
   s.width = width;
-  const int grid = (width + 31) / 32;
-  if (dtype == 1) norm_sums_kernel<__nv_bfloat16><<<grid, 512, 0, stream>>>(s);
-  else norm_sums_kernel<__half><<<grid, 512, 0, stream>>>(s);
+  const dim3 grid((width + 31) / 32, 3);
+  if (dtype == 1) norm_sums_kernel<__nv_bfloat16><<<grid, 1024, 0, stream>>>(s);
+  else norm_sums_kernel<__half><<<grid, 1024, 0, stream>>>(s);
   return launch_status();
 }

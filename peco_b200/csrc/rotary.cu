@@ -32,7 +32,6 @@ namespace {
 constexpr int kMaxAxes = 4;
 constexpr int kMaxPairs = 128;  // head dimension up to 256
 constexpr int kThreads = 256;
-constexpr int kBatch = 4;       // heads whose loads are in flight together
 
 struct RotaryTensor {
   const void* src;
@@ -56,16 +55,42 @@ struct RotaryArgs {
   unsigned char axis[kMaxPairs];
 };
 
-__device__ __forceinline__ double position_of(const RotaryArgs& a, int batch, int token, int axis) {
+// Position of a token on every axis.
+__device__ __forceinline__ void positions_of(const RotaryArgs& a, int batch, int token, double (&p)[kMaxAxes]) {
   if (a.positions) {
-    const long long at = batch * a.pos_sb + token * a.pos_sn + axis;
-    if (a.pos_type == 0) return static_cast<const int*>(a.positions)[at];
-    if (a.pos_type == 1) return static_cast<double>(static_cast<const long long*>(a.positions)[at]);
-    return static_cast<const float*>(a.positions)[at];
+    const long long at = batch * a.pos_sb + token * a.pos_sn;
+#pragma unroll
+    for (int i = 0; i < kMaxAxes; ++i) {
+      p[i] = 0.0;
+      if (i >= a.axes) continue;
+      if (a.pos_type == 0) p[i] = static_cast<const int*>(a.positions)[at + i];
+      else if (a.pos_type == 1) p[i] = static_cast<double>(static_cast<const long long*>(a.positions)[at + i]);
+      else p[i] = static_cast<const float*>(a.positions)[at + i];
+    }
+  } else {
+    unsigned rest = token;
+#pragma unroll
+    for (int i = kMaxAxes - 1; i >= 0; --i) {
+      p[i] = 0.0;
+      if (i >= a.axes) continue;
+      const unsigned up = i ? rest / a.grid[i] : 0;
+      p[i] = static_cast<double>(rest - up * a.grid[i]);
+      rest = up;
+    }
   }
-  unsigned rest = token;
-  for (int i = a.axes - 1; i > axis; --i) rest /= a.grid[i];
-  return axis ? rest % a.grid[axis] : rest;
+}
+
+// (cos, sin) of ``turns`` full turns, |turns| <= 1/2.  16-bit results hide the
+// special-function unit's absolute error of 2^-20; fp32 ones take the library's.
+template <typename T>
+__device__ __forceinline__ void turn_to(float turns, float& c, float& s) {
+  if constexpr (sizeof(T) == 2) {
+    const float angle = 6.2831853071795865f * turns;
+    c = __cosf(angle);
+    s = __sinf(angle);
+  } else {
+    sincospif(2.0f * turns, &s, &c);
+  }
 }
 
 // row of head h (Q's heads first, then K's) in the source or the destination
@@ -78,102 +103,121 @@ __device__ __forceinline__ T* row_of(const RotaryArgs& a, int h, int batch, int 
                      : static_cast<T*>(const_cast<void*>(t.src)) + batch * t.sb + head * t.sh + token * t.sn;
 }
 
+// BYTES (2 to 32) between memory and registers in accesses of up to 16 bytes;
+// the address is aligned to min(BYTES, 16).
+template <int BYTES>
+__device__ __forceinline__ void move_bytes(void* to, const void* from) {
+  if constexpr (BYTES == 32) {
+    reinterpret_cast<uint4*>(to)[0] = reinterpret_cast<const uint4*>(from)[0];
+    reinterpret_cast<uint4*>(to)[1] = reinterpret_cast<const uint4*>(from)[1];
+  } else if constexpr (BYTES == 16) {
+    *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
+  } else if constexpr (BYTES == 8) {
+    *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(from);
+  } else if constexpr (BYTES == 4) {
+    *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
+  } else {
+    *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
+  }
+}
+
+// The 2V elements a thread moves of one row, as they lie in memory.
+template <typename T, int V>
+struct alignas(16) Run {
+  T e[2 * V];
+};
+
 // V pairs per thread.  Interleaved: 2V neighbouring dimensions.  Split: V
 // dimensions in each half of the rotated ones; the copied tail is then cut
-// into runs of 2V like the interleaved form.
-template <typename T, int V, bool SPLIT>
+// into runs of 2V like the interleaved form.  A thread walks its heads HEADS
+// at a time with the next ones' loads in flight: source and destination may be
+// the same tensor, so the order of loads and stores is written out here (heads
+// never share memory).
+template <typename T, int V, bool SPLIT, int HEADS>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryArgs a) {
   const int slot = threadIdx.x / a.units, unit = threadIdx.x - slot * a.units;
   const int batch = blockIdx.x / a.token_blocks;
   const int token = (blockIdx.x - batch * a.token_blocks) * a.tokens_per_block + slot;
   if (slot >= a.tokens_per_block || token >= a.rows) return;
   const int pair0 = unit * V;
-  const bool rotated = token < a.rotated_rows && pair0 < a.pairs;
   // the two runs of V elements this thread moves
   const bool halves = SPLIT && pair0 < a.pairs;
   const int lo = halves ? pair0 : 2 * pair0;
   const int hi = halves ? pair0 + a.pairs : 2 * pair0 + V;
-  float c[V], s[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    c[i] = 1.0f;
-    s[i] = 0.0f;
-    if (rotated && pair0 + i < a.pairs) {
-      double t = position_of(a, batch, token, a.axis[pair0 + i]) * a.turns[pair0 + i];
-      t -= rint(t);
-      sincospif(2.0f * static_cast<float>(t), &s[i], &c[i]);
-      if (a.inverse) s[i] = -s[i];
-    }
-  }
   const int all_heads = a.t[0].heads + a.t[1].heads;
   const int first = blockIdx.y * a.heads_per_block;
   const int last = min(first + a.heads_per_block, all_heads);
-  // The loads of kBatch heads are issued before the first store: source and
-  // destination may be the same tensor, so the compiler must not be left to
-  // order them.
-  for (int h0 = first; h0 < last; h0 += kBatch) {
-    float x[kBatch][2 * V];
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      if (h0 + j < last) {
-        const T* src = row_of<T>(a, h0 + j, batch, token, false);
-        if constexpr (V == 1) {
-          x[j][0] = to_f32<T>(src[lo]);
-          x[j][1] = to_f32<T>(src[hi]);
-        } else if constexpr (!SPLIT) {
-          load_aligned<2 * V>(src + lo, x[j]);
-        } else {
-          float p[V], q[V];
-          load_aligned<V>(src + lo, p);
-          load_aligned<V>(src + hi, q);
-#pragma unroll
-          for (int i = 0; i < V; ++i) x[j][i] = p[i], x[j][V + i] = q[i];
-        }
-      }
+  constexpr int kRun = V * sizeof(T);
+  // interleaved runs are adjacent: one access (V == 1: element by element, as the rows are not aligned)
+  constexpr bool kJoined = !SPLIT && V > 1;
+
+  auto load = [&](int h, Run<T, V>& r) {
+    const T* src = row_of<T>(a, h, batch, token, false);
+    if constexpr (kJoined) {
+      move_bytes<2 * kRun>(r.e, src + lo);
+    } else {
+      move_bytes<kRun>(r.e, src + lo);
+      move_bytes<kRun>(r.e + V, src + hi);
     }
+  };
+  Run<T, V> next[HEADS];
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      if (h0 + j < last) {
-        if (rotated) {
+  for (int h = 0; h < HEADS; ++h)
+    if (first + h < last) load(first + h, next[h]);
+
+  const int live = token < a.rotated_rows ? min(V, a.pairs - pair0) : 0;  // pairs that turn; the rest is copied
+  float c[V], s[V];
+  if (live > 0) {
+    double p[kMaxAxes];
+    positions_of(a, batch, token, p);
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const int ia = SPLIT ? i : 2 * i, ib = SPLIT ? V + i : 2 * i + 1;
-            const float u = x[j][ia], w = x[j][ib];
-            x[j][ia] = u * c[i] - w * s[i];
-            x[j][ib] = w * c[i] + u * s[i];
+    for (int i = 0; i < V; ++i) {
+      if (i >= live) continue;
+      const int axis = a.axis[pair0 + i];
+      double t = (axis == 0 ? p[0] : axis == 1 ? p[1] : axis == 2 ? p[2] : p[3]) * a.turns[pair0 + i];
+      t -= rint(t);
+      turn_to<T>(static_cast<float>(t), c[i], s[i]);
+      if (a.inverse) s[i] = -s[i];
+    }
+  }
+
+  for (int h0 = first; h0 < last; h0 += HEADS) {
+    Run<T, V> now[HEADS];
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) now[h] = next[h];
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h)
+      if (h0 + HEADS + h < last) load(h0 + HEADS + h, next[h]);
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
+      if (h0 + h >= last) continue;
+      Run<T, V>& r = now[h];
+      if (live > 0) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const int ia = SPLIT ? i : 2 * i, ib = SPLIT ? V + i : 2 * i + 1;
+          const float u = to_f32<T>(r.e[ia]), w = to_f32<T>(r.e[ib]);
+          const T x = from_f32<T>(u * c[i] - w * s[i]), y = from_f32<T>(w * c[i] + u * s[i]);
+          if (i < live) {
+            r.e[ia] = x;
+            r.e[ib] = y;
           }
         }
-        T* dst = row_of<T>(a, h0 + j, batch, token, true);
-        if constexpr (V == 1) {
-          dst[lo] = from_f32<T>(x[j][0]);
-          dst[hi] = from_f32<T>(x[j][1]);
-        } else if constexpr (!SPLIT) {
-          store_aligned<2 * V>(dst + lo, x[j]);
-        } else {
-          float p[V], q[V];
-#pragma unroll
-          for (int i = 0; i < V; ++i) p[i] = x[j][i], q[i] = x[j][V + i];
-          store_aligned<V>(dst + lo, p);
-          store_aligned<V>(dst + hi, q);
-        }
+      }
+      T* dst = row_of<T>(a, h0 + h, batch, token, true);
+      if constexpr (kJoined) {
+        move_bytes<2 * kRun>(dst + lo, r.e);
+      } else {
+        move_bytes<kRun>(dst + lo, r.e);
+        move_bytes<kRun>(dst + hi, r.e + V);
       }
     }
   }
 }
 
-template <typename T>
-int launch_rotary(RotaryArgs& a, int batch, bool split, cudaStream_t stream) {
-  constexpr int V = 4;
-  // one aligned access of 2V elements (interleaved) or V (split), fp32 in 16-byte pieces
-  const int align = sizeof(T) == 4 ? 4 : split ? V : 2 * V;
-  bool vec = (!split || a.pairs % V == 0) && a.dims % (2 * V) == 0;
-  for (const RotaryTensor& t : a.t) {
-    if (!t.heads) continue;
-    const long long step = t.sb | t.sh | t.sn | t.db | t.dh | t.dn;
-    const uintptr_t base = reinterpret_cast<uintptr_t>(t.src) | reinterpret_cast<uintptr_t>(t.dst);
-    vec = vec && step % align == 0 && base % (align * sizeof(T)) == 0;
-  }
-  a.units = a.dims / (vec ? 2 * V : 2);
+template <typename T, int V, bool SPLIT, int HEADS>
+int launch_form(RotaryArgs& a, int batch, cudaStream_t stream) {
+  a.units = a.dims / (2 * V);
   a.tokens_per_block = kThreads / a.units;
   a.token_blocks = (a.rows + a.tokens_per_block - 1) / a.tokens_per_block;
   const long long blocks = static_cast<long long>(batch) * a.token_blocks;
@@ -181,15 +225,36 @@ int launch_rotary(RotaryArgs& a, int batch, bool split, cudaStream_t stream) {
   // All heads in one block when the tokens alone fill the GPU (the sines are
   // then computed once per token); otherwise heads are spread over blocks.
   const int heads = a.t[0].heads + a.t[1].heads;
-  long long groups = (16LL * kNumSMs + blocks - 1) / blocks;
+  long long groups = (8LL * kNumSMs + blocks - 1) / blocks;
   if (groups > heads) groups = heads;
   a.heads_per_block = static_cast<int>((heads + groups - 1) / groups);
   const dim3 grid(static_cast<unsigned>(blocks), (heads + a.heads_per_block - 1) / a.heads_per_block);
-  if (vec && split) rotary_kernel<T, V, true><<<grid, kThreads, 0, stream>>>(a);
-  else if (vec) rotary_kernel<T, V, false><<<grid, kThreads, 0, stream>>>(a);
-  else if (split) rotary_kernel<T, 1, true><<<grid, kThreads, 0, stream>>>(a);
-  else rotary_kernel<T, 1, false><<<grid, kThreads, 0, stream>>>(a);
+  rotary_kernel<T, V, SPLIT, HEADS><<<grid, kThreads, 0, stream>>>(a);
   return launch_status();
+}
+
+// Whether every row's runs of V pairs start on the boundaries that V needs.
+template <typename T>
+bool runs_aligned(const RotaryArgs& a, int v, bool split) {
+  if (a.dims % (2 * v) || (split && a.pairs % v)) return false;
+  const long long bytes = (split ? v : 2 * v) * sizeof(T), align = bytes < 16 ? bytes : 16;
+  for (const RotaryTensor& t : a.t) {
+    if (!t.heads) continue;
+    const long long step = (t.sb | t.sh | t.sn | t.db | t.dh | t.dn) * static_cast<long long>(sizeof(T));
+    if ((step | static_cast<long long>(reinterpret_cast<uintptr_t>(t.src) | reinterpret_cast<uintptr_t>(t.dst))) & (align - 1))
+      return false;
+  }
+  return true;
+}
+
+template <typename T>
+int launch_rotary(RotaryArgs& a, int batch, bool split, cudaStream_t stream) {
+  if constexpr (sizeof(T) == 2) {  // eight pairs: 16 bytes of each half
+    if (split && runs_aligned<T>(a, 8, true)) return launch_form<T, 8, true, 2>(a, batch, stream);
+  }
+  if (runs_aligned<T>(a, 4, split))
+    return split ? launch_form<T, 4, true, 4>(a, batch, stream) : launch_form<T, 4, false, 4>(a, batch, stream);
+  return split ? launch_form<T, 1, true, 4>(a, batch, stream) : launch_form<T, 1, false, 4>(a, batch, stream);
 }
 
 }  // namespace
