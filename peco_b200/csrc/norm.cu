@@ -140,6 +140,36 @@ __device__ __forceinline__ void store(const Span<WARPS, NCH, ALIGNED>& sp, void*
 
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
+// A sample's vectors, in registers while its rows pass: a load between a row's
+// prefetch and its use would make the warp wait for the prefetch as well (loads
+// share few scoreboards).
+// gate * post_weight of chunk i
+template <typename T, typename SP>
+__device__ __forceinline__ void load_gate(const NormArgs& a, const SP& sp, unsigned sample, int i, float2 (&g)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) g[j] = both(1.0f);
+  if (a.gate.p) load_part<T>(sp, a.gate.p, sample * a.gate.sb, i, g);
+  if (a.post_weight) {
+    float2 w[4];
+    load_part<T>(sp, a.post_weight, 0, i, w);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] = fmul2(g[j], w[j]);
+  }
+}
+// (1 + scale) * weight of chunk i
+template <typename T, typename SP>
+__device__ __forceinline__ void load_factor(const NormArgs& a, const SP& sp, unsigned sample, int i, float2 (&f)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f[j] = both(1.0f);
+  if (a.weight) load_part<T>(sp, a.weight, 0, i, f);
+  if (a.scale.p) {
+    float2 s[4];
+    load_part<T>(sp, a.scale.p, sample * a.scale.sb, i, s);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = ffma2(f[j], s[j], f[j]);
+  }
+}
+
 // v with the columns past the width set to 0
 template <typename SP>
 __device__ __forceinline__ float2 only_inside(const SP& sp, int i, int j, float2 v) {
@@ -249,7 +279,7 @@ __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS) norm_forward_ker
   const unsigned total = static_cast<unsigned>(a.samples) * a.rows, step = gridDim.x * kRows;  // below 2^31
   unsigned row = blockIdx.x * kRows + slot;
   if (row >= total) return;  // whole warps only: kRows > 1 means one warp per row
-  unsigned sample = row / a.rows, at = row - sample * a.rows;
+  unsigned sample = row / a.rows, at = row - sample * a.rows, loaded = 0xffffffffu;
   auto row_of = [&](const RowTensor& t) { return static_cast<const T*>(t.p) + sample * t.sb + at * t.sn; };
   RawChunk raw_x[NCH], raw_b[NCH];
 #pragma unroll
@@ -258,11 +288,22 @@ __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS) norm_forward_ker
     if (a.branch.p) fetch(sp, row_of(a.branch), i, raw_b[i]);
   }
   const float2 rs = both(a.residual_scale);
+  float2 gate[NCH][4], factor[NCH][4], shift[NCH][4];
   int turn = 0;
   while (row < total) {
+    if (sample != loaded) {
+      loaded = sample;
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        load_gate<T>(a, sp, sample, i, gate[i]);
+        load_factor<T>(a, sp, sample, i, factor[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) shift[i][j] = both(0.0f);
+        if (a.shift.p) load_part<T>(sp, a.shift.p, sample * a.shift.sb, i, shift[i]);
+      }
+    }
     float2 r[NCH][4];
     const long long out = static_cast<long long>(row) * a.width;
-    const long long gate_at = sample * a.gate.sb, scale_at = sample * a.scale.sb, shift_at = sample * a.shift.sb;
     float2 pscale = both(1.0f), pshift = both(0.0f);  // post norm: b * rstd - mean * rstd
     if constexpr (POST) {
       float2 b[NCH][4];
@@ -277,28 +318,13 @@ __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS) norm_forward_ker
     for (int i = 0; i < NCH; ++i) {
       widen<T>(raw_x[i], r[i]);
       if (a.branch.p) {
-        float2 b[4], g[4];
+        float2 b[4];
         widen<T>(raw_b[i], b);
-        if constexpr (POST) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) b[j] = ffma2(b[j], pscale, pshift);
-          if (a.post_weight) {
-            load_part<T>(sp, a.post_weight, 0, i, g);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) b[j] = fmul2(b[j], g[j]);
-          }
-          if (!ALIGNED || !sp.inside(i, 0)) {  // the shift of columns past the width
-#pragma unroll
-            for (int j = 0; j < 4; ++j) b[j] = only_inside(sp, i, j, b[j]);
-          }
+        for (int j = 0; j < 4; ++j) {
+          if (POST) b[j] = only_inside(sp, i, j, ffma2(b[j], pscale, pshift));  // the shift of columns past the width
+          r[i][j] = ffma2(rs, r[i][j], fmul2(gate[i][j], b[j]));
         }
-        if (a.gate.p) {
-          load_part<T>(sp, a.gate.p, gate_at, i, g);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) b[j] = fmul2(b[j], g[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) r[i][j] = ffma2(rs, r[i][j], b[j]);
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) r[i][j] = fmul2(rs, r[i][j]);
@@ -320,28 +346,12 @@ __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS) norm_forward_ker
     }
     const Moments m = row_moments<false>(sp, share, r, r, a.norm == kNormLayer, inv, buf[turn][0]);
     turn ^= 1;
-    const float rstd = rsqrtf(m.squares * inv + a.eps);
-    const float2 minus = both(-m.mean), times = both(rstd);
+    const float2 minus = both(-m.mean), times = both(rsqrtf(m.squares * inv + a.eps));
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      float2 f[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r[i][j] = fmul2(fadd2(r[i][j], minus), times);
-      if (a.weight) {
-        load_part<T>(sp, a.weight, 0, i, f);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) r[i][j] = fmul2(r[i][j], f[j]);
-      }
-      if (a.scale.p) {
-        load_part<T>(sp, a.scale.p, scale_at, i, f);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) r[i][j] = fmul2(r[i][j], fadd2(f[j], both(1.0f)));
-      }
-      if (a.shift.p) {
-        load_part<T>(sp, a.shift.p, shift_at, i, f);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) r[i][j] = fadd2(r[i][j], f[j]);
-      }
+      for (int j = 0; j < 4; ++j)
+        r[i][j] = ffma2(fmul2(fadd2(r[i][j], minus), times), factor[i][j], shift[i][j]);
       store<T>(sp, a.out_h, out, i, r[i]);
     }
   }
@@ -353,8 +363,8 @@ __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS) norm_forward_ker
 // chunks a thread) in shared memory; a second kernel adds the blocks' sums in
 // order.  A register that held a piece of the row takes the next row's piece as
 // soon as it is free.
-template <typename T, int WARPS, int NCH, bool ALIGNED, bool POST>
-__global__ void __launch_bounds__(32 * WARPS) norm_backward_kernel(const __grid_constant__ NormArgs a) {
+template <typename T, int WARPS, int NCH, int BLOCKS, bool ALIGNED, bool POST>
+__global__ void __launch_bounds__(32 * WARPS, BLOCKS) norm_backward_kernel(const __grid_constant__ NormArgs a) {
   constexpr int kThreads = 32 * WARPS;
   __shared__ float4 buf[2][3][WARPS];  // alternates between rows: a row's last read may meet the next one's write
   const unsigned sample = blockIdx.x / a.chunks, chunk = blockIdx.x - sample * a.chunks;
@@ -378,7 +388,12 @@ __global__ void __launch_bounds__(32 * WARPS) norm_backward_kernel(const __grid_
       for (int j = 0; j < 4; ++j)
         for (int k = 0; k < 3; ++k) *shared_at(k, i, j) = both(0.0f);
   }
-  const long long gate_at = sample * a.gate.sb, scale_at = sample * a.scale.sb;
+  float2 gate[NCH][4], factor[NCH][4];
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    load_gate<T>(a, sp, sample, i, gate[i]);
+    load_factor<T>(a, sp, sample, i, factor[i]);
+  }
   auto row_of = [&](const RowTensor& t, unsigned at) { return static_cast<const T*>(t.p) + sample * t.sb + at * t.sn; };
   RawChunk raw_x[NCH], raw_d[NCH], raw_b[NCH], raw_e[NCH];
   const unsigned rows = a.rows, stride = a.chunks;
@@ -411,46 +426,23 @@ __global__ void __launch_bounds__(32 * WARPS) norm_backward_kernel(const __grid_
     // r and dn = dh (1 + scale) weight
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      float2 f[4];
       widen<T>(raw_x[i], r[i]);
       if (next < rows) fetch(sp, row_of(a.x, next), i, raw_x[i]);
+      float2 d[4];
+      widen<T>(raw_d[i], d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) dn[i][j] = fmul2(d[j], factor[i][j]);
       if (a.branch.p) {
         float2 b[4];
         widen<T>(raw_b[i], b);
-        if constexpr (POST) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) b[j] = ffma2(b[j], pscale, pshift);
-          if (a.post_weight) {
-            load_part<T>(sp, a.post_weight, 0, i, f);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) b[j] = fmul2(b[j], f[j]);
-          }
-          if (!ALIGNED || !sp.inside(i, 0)) {  // the shift of columns past the width
-#pragma unroll
-            for (int j = 0; j < 4; ++j) b[j] = only_inside(sp, i, j, b[j]);
-          }
+        for (int j = 0; j < 4; ++j) {
+          if (POST) b[j] = only_inside(sp, i, j, ffma2(b[j], pscale, pshift));  // the shift of columns past the width
+          r[i][j] = ffma2(rs, r[i][j], fmul2(gate[i][j], b[j]));
         }
-        if (a.gate.p) {
-          load_part<T>(sp, a.gate.p, gate_at, i, f);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) b[j] = fmul2(b[j], f[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) r[i][j] = ffma2(rs, r[i][j], b[j]);
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) r[i][j] = fmul2(rs, r[i][j]);
-      }
-      widen<T>(raw_d[i], dn[i]);
-      if (a.scale.p) {
-        load_part<T>(sp, a.scale.p, scale_at, i, f);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) dn[i][j] = ffma2(dn[i][j], f[j], dn[i][j]);
-      }
-      if (a.weight) {
-        load_part<T>(sp, a.weight, 0, i, f);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) dn[i][j] = fmul2(dn[i][j], f[j]);
       }
     }
     const Moments m = row_moments<true>(sp, share, r, dn, a.norm == kNormLayer, inv, buf[turn][0]);
@@ -461,7 +453,7 @@ __global__ void __launch_bounds__(32 * WARPS) norm_backward_kernel(const __grid_
     float2 v[POST ? NCH : 1][4];  // post norm: the branch's row once more
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      float2 d[4], b[4], e4[4], g[4], pw[4];
+      float2 d[4], b[4], e4[4];
       widen<T>(raw_d[i], d);
       if (a.branch.p) widen<T>(raw_b[i], b);
       if (a.grad_r.p) widen<T>(raw_e[i], e4);
@@ -470,8 +462,6 @@ __global__ void __launch_bounds__(32 * WARPS) norm_backward_kernel(const __grid_
         if (a.branch.p) fetch(sp, row_of(a.branch, next), i, raw_b[i]);
         if (a.grad_r.p) fetch(sp, row_of(a.grad_r, next), i, raw_e[i]);
       }
-      if (a.gate.p) load_part<T>(sp, a.gate.p, gate_at, i, g);
-      if (POST && a.post_weight) load_part<T>(sp, a.post_weight, 0, i, pw);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float2 n = fmul2(fadd2(r[i][j], minus), times);
@@ -484,8 +474,7 @@ __global__ void __launch_bounds__(32 * WARPS) norm_backward_kernel(const __grid_
             v[i][j] = b[j];
             pn = ffma2(b[j], pscale, pshift);
           }
-          float2 db = a.gate.p ? fmul2(dr, g[j]) : dr;
-          if (POST && a.post_weight) db = fmul2(db, pw[j]);
+          float2 db = fmul2(dr, gate[i][j]);
           if (POST) db = only_inside(sp, i, j, db);
           dn[i][j] = db;
         }
@@ -605,49 +594,65 @@ int blocks_per_sm(const void* kernel, int threads, std::atomic<int>& known) {
   return n;
 }
 
-template <typename T, int WARPS, int NCH, bool ALIGNED, bool POST>
-int launch_one(const NormArgs& a, bool backward, cudaStream_t stream) {
-  if (backward) {
-    auto kernel = norm_backward_kernel<T, WARPS, NCH, ALIGNED, POST>;
-    constexpr int kSmem = NCH > 3 ? 3 * NCH * kChunk * 32 * WARPS * 4 : 0;  // the column sums
-    if (kSmem > 0) {  // granted once per device
-      static std::atomic<unsigned long long> opened;
-      int dev = 0;
-      cudaError_t e = cudaGetDevice(&dev);
+template <typename T, int WARPS, int NCH, int BLOCKS, bool ALIGNED, bool POST>
+int launch_backward(const NormArgs& a, cudaStream_t stream) {
+  auto kernel = norm_backward_kernel<T, WARPS, NCH, BLOCKS, ALIGNED, POST>;
+  constexpr int kSmem = NCH > 3 ? 3 * NCH * kChunk * 32 * WARPS * 4 : 0;  // the column sums
+  if (kSmem > 0) {  // granted once per device
+    static std::atomic<unsigned long long> opened;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (dev >= 64 || !(opened.load(std::memory_order_relaxed) & bit)) {
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
       if (e != cudaSuccess) return static_cast<int>(e);
-      const unsigned long long bit = 1ull << (dev & 63);
-      if (dev >= 64 || !(opened.load(std::memory_order_relaxed) & bit)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-        if (e != cudaSuccess) return static_cast<int>(e);
-        opened.fetch_or(bit, std::memory_order_relaxed);
-      }
+      opened.fetch_or(bit, std::memory_order_relaxed);
     }
-    kernel<<<a.samples * a.chunks, 32 * WARPS, kSmem, stream>>>(a);
-  } else {
-    constexpr int kRows = WARPS < 4 ? 4 / WARPS : 1, kBlock = WARPS < 4 ? 128 : 32 * WARPS;
-    auto kernel = norm_forward_kernel<T, WARPS, NCH, ALIGNED, POST>;
-    static std::atomic<int> resident;
-    const long long want = (static_cast<long long>(a.samples) * a.rows + kRows - 1) / kRows;
-    const long long most = static_cast<long long>(kNumSMs) * blocks_per_sm(reinterpret_cast<const void*>(kernel), kBlock, resident);
-    kernel<<<static_cast<unsigned>(want < most ? want : most), kBlock, 0, stream>>>(a);
   }
+  kernel<<<a.samples * a.chunks, 32 * WARPS, kSmem, stream>>>(a);
   return launch_status();
 }
 
+template <typename T, int WARPS, int NCH, bool ALIGNED, bool POST>
+int launch_forward(const NormArgs& a, cudaStream_t stream) {
+  constexpr int kRows = WARPS < 4 ? 4 / WARPS : 1, kBlock = WARPS < 4 ? 128 : 32 * WARPS;
+  auto kernel = norm_forward_kernel<T, WARPS, NCH, ALIGNED, POST>;
+  static std::atomic<int> resident;
+  const long long want = (static_cast<long long>(a.samples) * a.rows + kRows - 1) / kRows;
+  const long long most = static_cast<long long>(kNumSMs) * blocks_per_sm(reinterpret_cast<const void*>(kernel), kBlock, resident);
+  kernel<<<static_cast<unsigned>(want < most ? want : most), kBlock, 0, stream>>>(a);
+  return launch_status();
+}
+
+#ifndef BW_W
+#define BW_W 12
+#define BW_N 1
+#define BW_B 1
+#endif
 // Warps per row: the fewest whose threads hold the row in three chunks each
 // (few warps make the row's reduction cheap), more chunks only past 8192 columns.
 template <typename T, bool ALIGNED, bool POST>
 int launch_width(const NormArgs& a, bool backward, cudaStream_t stream) {
   const int w = a.width;
-  if (w <= 256) return launch_one<T, 1, 1, ALIGNED, POST>(a, backward, stream);
-  if (w <= 768) return launch_one<T, 1, 3, ALIGNED, POST>(a, backward, stream);
-  if (w <= 1024) return launch_one<T, 4, 1, ALIGNED, POST>(a, backward, stream);
-  if (w <= 2048) return launch_one<T, 4, 2, ALIGNED, POST>(a, backward, stream);
-  if (w <= 3072) return launch_one<T, 4, 3, ALIGNED, POST>(a, backward, stream);
-  if (w <= 4096) return launch_one<T, 8, 2, ALIGNED, POST>(a, backward, stream);
-  if (w <= 6144) return launch_one<T, 8, 3, ALIGNED, POST>(a, backward, stream);
-  if (w <= 8192) return launch_one<T, 16, 2, ALIGNED, POST>(a, backward, stream);
-  return launch_one<T, 16, 4, ALIGNED, POST>(a, backward, stream);
+  if (backward) {
+    if (w <= 256) return launch_backward<T, 1, 1, 16, ALIGNED, POST>(a, stream);
+    if (w <= 1024) return launch_backward<T, 4, 1, 4, ALIGNED, POST>(a, stream);
+    if (w <= 2048) return launch_backward<T, 8, 1, 2, ALIGNED, POST>(a, stream);
+    if (w <= 3072) return launch_backward<T, BW_W, BW_N, BW_B, ALIGNED, POST>(a, stream);
+    if (w <= 4096) return launch_backward<T, 16, 1, 1, ALIGNED, POST>(a, stream);
+    if (w <= 8192) return launch_backward<T, 16, 2, 1, ALIGNED, POST>(a, stream);
+    return launch_backward<T, 16, 4, 1, ALIGNED, POST>(a, stream);
+  }
+  if (w <= 256) return launch_forward<T, 1, 1, ALIGNED, POST>(a, stream);
+  if (w <= 768) return launch_forward<T, 1, 3, ALIGNED, POST>(a, stream);
+  if (w <= 1024) return launch_forward<T, 4, 1, ALIGNED, POST>(a, stream);
+  if (w <= 2048) return launch_forward<T, 4, 2, ALIGNED, POST>(a, stream);
+  if (w <= 3072) return launch_forward<T, 4, 3, ALIGNED, POST>(a, stream);
+  if (w <= 4096) return launch_forward<T, 8, 2, ALIGNED, POST>(a, stream);
+  if (w <= 6144) return launch_forward<T, 8, 3, ALIGNED, POST>(a, stream);
+  if (w <= 8192) return launch_forward<T, 16, 2, ALIGNED, POST>(a, stream);
+  return launch_forward<T, 16, 4, ALIGNED, POST>(a, stream);
 }
 
 template <typename T>
@@ -662,8 +667,7 @@ int launch_norm(const NormArgs& a, bool backward, cudaStream_t stream) {
 // partial sums stay a small part of the traffic.
 int norm_chunks(int samples, int rows, int width) {
   if (samples < 1) return 1;
-  const int warps = width <= 768 ? 1 : width <= 3072 ? 4 : width <= 6144 ? 8 : 16;
-  const long long per_sm = warps > 8 ? 1 : 8 / warps;
+  const long long per_sm = width <= 256 ? 16 : width <= 1024 ? 4 : width <= 2048 ? 2 : width <= 3072 ? BW_B : 1;
   long long chunks = (per_sm * kNumSMs + samples - 1) / samples;
   const long long fewest = kNumSMs / samples + 1;  // short inputs still spread over the SMs
   long long most = (rows + 7) / 8;
