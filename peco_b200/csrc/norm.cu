@@ -59,6 +59,8 @@ struct NormArgs {
   int norm, post;
   float eps, post_eps, residual_scale;
   int chunks;       // backward: row chunks per sample
+  int stages, stage_bytes;  // ring of rows in shared memory
+  unsigned* status;
 };
 
 // ---- a row in registers ----------------------------------------------------------
@@ -69,18 +71,25 @@ struct NormArgs {
 // elements are still read side by side.  Columns past the width hold 0.
 constexpr int kChunk = 8;
 
-template <int WARPS, int NCH, bool ALIGNED>
+// Full rows are aligned rows that fill every thread's chunks.
+enum RowMode : int { kUnaligned = 0, kAligned = 1, kFull = 2 };
+
+template <int WARPS, int NCH, int MODE>
 struct Span {
   static constexpr int kThreads = 32 * WARPS;
+  static constexpr bool kIsAligned = MODE != kUnaligned;
   int thread, width;
   __device__ __forceinline__ int column(int i, int e) const {
-    return ALIGNED ? (i * kThreads + thread) * kChunk + e : (i * kChunk + e) * kThreads + thread;
+    return kIsAligned ? (i * kThreads + thread) * kChunk + e : (i * kChunk + e) * kThreads + thread;
   }
-  __device__ __forceinline__ bool inside(int i, int e) const { return column(i, ALIGNED ? 0 : e) < width; }
+  __device__ __forceinline__ bool inside(int i, int e) const {
+    return MODE == kFull || column(i, kIsAligned ? 0 : e) < width;
+  }
   // columns that warp w of the row's threads holds
   __device__ __forceinline__ float held_by(int w) const {
+    if (MODE == kFull) return static_cast<float>(32 * kChunk * NCH);
     int n = 0;
-    if (ALIGNED) {
+    if (kIsAligned) {
       for (int i = 0; i < NCH; ++i) n += max(0, min(32 * kChunk, width - (i * kThreads + w * 32) * kChunk));
     } else {
       for (int i = 0; i < NCH * kChunk; ++i) n += max(0, min(32, width - i * kThreads - w * 32));
@@ -94,10 +103,10 @@ struct RawChunk {
   uint32_t w[4];
 };
 
-template <typename T, int WARPS, int NCH, bool ALIGNED>
-__device__ __forceinline__ void fetch(const Span<WARPS, NCH, ALIGNED>& sp, const T* row, int i, RawChunk& r) {
+template <typename T, int WARPS, int NCH, int MODE>
+__device__ __forceinline__ void fetch(const Span<WARPS, NCH, MODE>& sp, const T* row, int i, RawChunk& r) {
   r.w[0] = r.w[1] = r.w[2] = r.w[3] = 0;
-  if constexpr (ALIGNED) {
+  if constexpr (MODE != kUnaligned) {
     if (sp.inside(i, 0)) {
       const uint4 u = *reinterpret_cast<const uint4*>(row + sp.column(i, 0));
       r.w[0] = u.x, r.w[1] = u.y, r.w[2] = u.z, r.w[3] = u.w;
@@ -124,10 +133,10 @@ __device__ __forceinline__ void load_part(const SP& sp, const void* p, long long
   widen<T>(r, v);
 }
 
-template <typename T, int WARPS, int NCH, bool ALIGNED>
-__device__ __forceinline__ void store(const Span<WARPS, NCH, ALIGNED>& sp, void* p, long long at, int i, const float2 (&v)[4]) {
+template <typename T, int WARPS, int NCH, int MODE>
+__device__ __forceinline__ void store(const Span<WARPS, NCH, MODE>& sp, void* p, long long at, int i, const float2 (&v)[4]) {
   T* row = static_cast<T*>(p) + at;
-  if constexpr (ALIGNED) {
+  if constexpr (MODE != kUnaligned) {
     if (sp.inside(i, 0))
       *reinterpret_cast<uint4*>(row + sp.column(i, 0)) =
           make_uint4(pack2<T>(v[0].x, v[0].y), pack2<T>(v[1].x, v[1].y), pack2<T>(v[2].x, v[2].y), pack2<T>(v[3].x, v[3].y));
@@ -171,11 +180,84 @@ __device__ __forceinline__ void load_factor(const NormArgs& a, const SP& sp, uns
 }
 
 // v with the columns past the width set to 0
-template <typename SP>
-__device__ __forceinline__ float2 only_inside(const SP& sp, int i, int j, float2 v) {
+template <int WARPS, int NCH, int MODE>
+__device__ __forceinline__ float2 only_inside(const Span<WARPS, NCH, MODE>& sp, int i, int j, float2 v) {
+  if (MODE == kFull) return v;
   if (!sp.inside(i, 2 * j)) v.x = 0.0f;
   if (!sp.inside(i, 2 * j + 1)) v.y = 0.0f;
   return v;
+}
+
+// ---- rows through shared memory ---------------------------------------------------
+// Aligned rows shared by several warps arrive by bulk copies into a ring of
+// stages, a row of every input each, a few rows ahead of the one in work: the
+// copies hold no registers, so enough of them are in flight to cover HBM's
+// latency (as loads into registers, a row's prefetch and its vectors' loads
+// waited for one another).  Thread 0 refills the stage of the row before once
+// the block has passed the current row's barrier, where nobody reads that stage
+// any more.
+constexpr int kMaxStages = 6;
+
+struct RowRing {
+  unsigned char* base;
+  uint64_t* full;
+  volatile int* abort_flag;
+  unsigned* status;
+  int stages, stage_bytes, row_bytes;
+  int take_s, take_p;    // stage and phase of the next row to take
+  int start_s;           // stage of the next row to start
+
+  __device__ __forceinline__ void open() {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < stages; ++i) mbar_init(&full[i], 1);
+      *abort_flag = 0;
+      fence_barrier_init();
+    }
+    __syncthreads();
+    take_s = take_p = start_s = 0;
+  }
+  // thread 0: start the block's next row, whose inputs are ``src``
+  __device__ __forceinline__ void start(const void* const (&src)[4]) {
+    if (*abort_flag) return;
+    int present = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) present += src[k] != nullptr;
+    mbar_arrive_expect_tx(&full[start_s], present * row_bytes);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (src[k]) bulk_load(base + start_s * stage_bytes + k * row_bytes, src[k], row_bytes, &full[start_s]);
+    start_s = start_s + 1 == stages ? 0 : start_s + 1;
+  }
+  // wait for the next row; its stage
+  __device__ __forceinline__ const unsigned char* next() {
+    const unsigned char* stage = base + take_s * stage_bytes;
+    if (!mbar_try_wait(&full[take_s], take_p) && !*abort_flag) mbar_wait(&full[take_s], take_p, abort_flag, status);
+    if (++take_s == stages) {
+      take_s = 0;
+      take_p ^= 1;
+    }
+    return stage;
+  }
+  // after an expired wait: time for the copies still in flight to land before the block ends
+  __device__ __forceinline__ void close() {
+    if (*abort_flag && threadIdx.x == 0) {
+      const unsigned long long t0 = globaltimer();
+      while (globaltimer() - t0 < 2000000ull) {
+      }
+    }
+  }
+};
+
+// chunk i of input k in a stage
+template <typename SP>
+__device__ __forceinline__ RawChunk staged(const SP& sp, const unsigned char* stage, int k, int row_bytes, int i) {
+  RawChunk r;
+  r.w[0] = r.w[1] = r.w[2] = r.w[3] = 0;
+  if (sp.inside(i, 0)) {
+    const uint4 u = *reinterpret_cast<const uint4*>(stage + k * row_bytes + sp.column(i, 0) * 2);
+    r.w[0] = u.x, r.w[1] = u.y, r.w[2] = u.z, r.w[3] = u.w;
+  }
+  return r;
 }
 
 // ---- moments of a row ---------------------------------------------------------
@@ -196,8 +278,8 @@ struct Shares {
 
 constexpr int warp_levels(int warps) { return warps <= 4 ? 2 : warps <= 8 ? 3 : warps <= 16 ? 4 : 5; }
 
-template <int WARPS, int NCH, bool ALIGNED>
-__device__ __forceinline__ Shares shares_of(const Span<WARPS, NCH, ALIGNED>& sp) {
+template <int WARPS, int NCH, int MODE>
+__device__ __forceinline__ Shares shares_of(const Span<WARPS, NCH, MODE>& sp) {
   const float own = sp.held_by(sp.thread >> 5);
   const int w = sp.thread & ((1 << warp_levels(WARPS)) - 1);
   return Shares{own > 0.0f ? 1.0f / own : 0.0f, WARPS > 1 && w < WARPS ? sp.held_by(w) : 0.0f};
@@ -210,8 +292,8 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
-template <bool WITH_D, int WARPS, int NCH, bool ALIGNED>
-__device__ __forceinline__ Moments row_moments(const Span<WARPS, NCH, ALIGNED>& sp, const Shares& share,
+template <bool WITH_D, int WARPS, int NCH, int MODE>
+__device__ __forceinline__ Moments row_moments(const Span<WARPS, NCH, MODE>& sp, const Shares& share,
                                                const float2 (&v)[NCH][4], const float2 (&d)[NCH][4], bool centred,
                                                float inv_width, float4* buf) {
   Moments m{0.0f, 0.0f, 0.0f, 0.0f};
@@ -227,11 +309,11 @@ __device__ __forceinline__ Moments row_moments(const Span<WARPS, NCH, ALIGNED>& 
   const float2 minus = both(-m.mean);
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    if (ALIGNED && !sp.inside(i, 0)) continue;
+    if (MODE == kAligned && !sp.inside(i, 0)) continue;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       float2 dev = fadd2(v[i][j], minus);
-      if (!ALIGNED) dev = only_inside(sp, i, j, dev);
+      if (MODE == kUnaligned) dev = only_inside(sp, i, j, dev);
       q = ffma2(dev, dev, q);
       if (WITH_D) {
         sd = fadd2(sd, d[i][j]);
@@ -266,14 +348,14 @@ __device__ __forceinline__ Moments row_moments(const Span<WARPS, NCH, ALIGNED>& 
 // Blocks stay and walk the rows: WARPS warps per row (a block of four warps
 // holds four rows when one warp is enough).  The next row's loads are issued as
 // soon as the current row is in fp32 registers, before its reduction.
-template <typename T, int WARPS, int NCH, bool ALIGNED, bool POST>
+template <typename T, int WARPS, int NCH, int MODE, bool POST>
 __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS) norm_forward_kernel(const __grid_constant__ NormArgs a) {
   static_assert(WARPS == 1 || WARPS >= 4, "rows of two warps would share block barriers");
   constexpr int kThreads = 32 * WARPS;
   constexpr unsigned kRows = WARPS < 4 ? 4 / WARPS : 1;
   __shared__ float4 buf[2][2][WARPS];  // alternates between rows: a row's last read may meet the next one's write
   const int slot = threadIdx.x / kThreads;
-  const Span<WARPS, NCH, ALIGNED> sp{static_cast<int>(threadIdx.x) - slot * kThreads, a.width};
+  const Span<WARPS, NCH, MODE> sp{static_cast<int>(threadIdx.x) - slot * kThreads, a.width};
   const Shares share = shares_of(sp);
   const float inv = 1.0f / static_cast<float>(a.width);
   const unsigned total = static_cast<unsigned>(a.samples) * a.rows, step = gridDim.x * kRows;  // below 2^31
@@ -281,11 +363,31 @@ __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS) norm_forward_ker
   if (row >= total) return;  // whole warps only: kRows > 1 means one warp per row
   unsigned sample = row / a.rows, at = row - sample * a.rows, loaded = 0xffffffffu;
   auto row_of = [&](const RowTensor& t) { return static_cast<const T*>(t.p) + sample * t.sb + at * t.sn; };
+  constexpr bool kRing = MODE != kUnaligned && WARPS > 1;
+  extern __shared__ __align__(128) unsigned char ring_bytes[];
+  __shared__ uint64_t ring_full[kMaxStages];
+  __shared__ int ring_abort;
+  RowRing ring{ring_bytes, ring_full, &ring_abort, a.status, a.stages, a.stage_bytes, a.width * 2, 0, 0, 0};
+  unsigned ahead = row;  // thread 0: the next row to start
+  auto start = [&]() {
+    const unsigned sm = ahead / a.rows, t = ahead - sm * a.rows;
+    const void* src[4] = {static_cast<const T*>(a.x.p) + sm * a.x.sb + t * a.x.sn,
+                          a.branch.p ? static_cast<const T*>(a.branch.p) + sm * a.branch.sb + t * a.branch.sn : nullptr,
+                          nullptr, nullptr};
+    ring.start(src);
+    ahead = ahead + step < ahead ? 0xffffffffu : ahead + step;
+  };
   RawChunk raw_x[NCH], raw_b[NCH];
+  if constexpr (kRing) {
+    ring.open();
+    if (threadIdx.x == 0)
+      for (int n = 0; n + 1 < a.stages && ahead < total; ++n) start();
+  } else {
 #pragma unroll
-  for (int i = 0; i < NCH; ++i) {
-    fetch(sp, row_of(a.x), i, raw_x[i]);
-    if (a.branch.p) fetch(sp, row_of(a.branch), i, raw_b[i]);
+    for (int i = 0; i < NCH; ++i) {
+      fetch(sp, row_of(a.x), i, raw_x[i]);
+      if (a.branch.p) fetch(sp, row_of(a.branch), i, raw_b[i]);
+    }
   }
   const float2 rs = both(a.residual_scale);
   float2 gate[NCH][4], factor[NCH][4], shift[NCH][4];
@@ -304,6 +406,14 @@ __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS) norm_forward_ker
     }
     float2 r[NCH][4];
     const long long out = static_cast<long long>(row) * a.width;
+    if constexpr (kRing) {
+      const unsigned char* stage = ring.next();
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        raw_x[i] = staged(sp, stage, 0, a.width * 2, i);
+        if (a.branch.p) raw_b[i] = staged(sp, stage, 1, a.width * 2, i);
+      }
+    }
     float2 pscale = both(1.0f), pshift = both(0.0f);  // post norm: b * rstd - mean * rstd
     if constexpr (POST) {
       float2 b[NCH][4];
@@ -333,11 +443,13 @@ __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS) norm_forward_ker
     row += step;
     if (row < total) {
       sample = row / a.rows;
-      at = row - sample * a.rows;
+      if constexpr (!kRing) {
+        at = row - sample * a.rows;
 #pragma unroll
-      for (int i = 0; i < NCH; ++i) {
-        fetch(sp, row_of(a.x), i, raw_x[i]);
-        if (a.branch.p) fetch(sp, row_of(a.branch), i, raw_b[i]);
+        for (int i = 0; i < NCH; ++i) {
+          fetch(sp, row_of(a.x), i, raw_x[i]);
+          if (a.branch.p) fetch(sp, row_of(a.branch), i, raw_b[i]);
+        }
       }
     }
     if (a.out_r) {
@@ -345,6 +457,7 @@ __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS) norm_forward_ker
       for (int i = 0; i < NCH; ++i) store<T>(sp, a.out_r, out, i, r[i]);
     }
     const Moments m = row_moments<false>(sp, share, r, r, a.norm == kNormLayer, inv, buf[turn][0]);
+    if (kRing && threadIdx.x == 0 && ahead < total) start();  // every thread is done with the rows before this one
     turn ^= 1;
     const float2 minus = both(-m.mean), times = both(rsqrtf(m.squares * inv + a.eps));
 #pragma unroll
@@ -355,6 +468,7 @@ __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS) norm_forward_ker
       store<T>(sp, a.out_h, out, i, r[i]);
     }
   }
+  if constexpr (kRing) ring.close();
 }
 
 // ---- backward ---------------------------------------------------------------------
@@ -363,16 +477,17 @@ __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS) norm_forward_ker
 // chunks a thread) in shared memory; a second kernel adds the blocks' sums in
 // order.  A register that held a piece of the row takes the next row's piece as
 // soon as it is free.
-template <typename T, int WARPS, int NCH, int BLOCKS, bool ALIGNED, bool POST>
+template <typename T, int WARPS, int NCH, int BLOCKS, int MODE, bool POST>
 __global__ void __launch_bounds__(32 * WARPS, BLOCKS) norm_backward_kernel(const __grid_constant__ NormArgs a) {
   constexpr int kThreads = 32 * WARPS;
   __shared__ float4 buf[2][3][WARPS];  // alternates between rows: a row's last read may meet the next one's write
   const unsigned sample = blockIdx.x / a.chunks, chunk = blockIdx.x - sample * a.chunks;
-  const Span<WARPS, NCH, ALIGNED> sp{static_cast<int>(threadIdx.x), a.width};
+  const Span<WARPS, NCH, MODE> sp{static_cast<int>(threadIdx.x), a.width};
   const Shares share = shares_of(sp);
   const float inv = 1.0f / static_cast<float>(a.width);
   constexpr bool kShared = NCH > 3;
-  extern __shared__ float shared_sums[];  // [3][NCH * 8][threads]: a thread's own entries, bank by bank
+  // column sums [3][NCH * 8][threads], a thread's own entries bank by bank; or the ring of rows
+  extern __shared__ __align__(128) float shared_sums[];
   constexpr int kR = kShared ? 1 : NCH;
   float2 a0[kR][4], a1[kR][4], g0[kR][4];
 #pragma unroll
@@ -395,9 +510,25 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS) norm_backward_kernel(const
     load_factor<T>(a, sp, sample, i, factor[i]);
   }
   auto row_of = [&](const RowTensor& t, unsigned at) { return static_cast<const T*>(t.p) + sample * t.sb + at * t.sn; };
-  RawChunk raw_x[NCH], raw_d[NCH], raw_b[NCH], raw_e[NCH];
+  constexpr bool kRing = MODE != kUnaligned && WARPS > 1 && !kShared;
+  __shared__ uint64_t ring_full[kMaxStages];
+  __shared__ int ring_abort;
+  RowRing ring{reinterpret_cast<unsigned char*>(shared_sums), ring_full, &ring_abort, a.status, a.stages, a.stage_bytes,
+               a.width * 2, 0, 0, 0};
   const unsigned rows = a.rows, stride = a.chunks;
-  if (chunk < rows) {
+  unsigned ahead = chunk;  // thread 0: the next row to start
+  auto start = [&]() {
+    const void* src[4] = {row_of(a.x, ahead), row_of(a.grad_h, ahead), a.branch.p ? row_of(a.branch, ahead) : nullptr,
+                          a.grad_r.p ? row_of(a.grad_r, ahead) : nullptr};
+    ring.start(src);
+    ahead = ahead + stride < ahead ? 0xffffffffu : ahead + stride;
+  };
+  RawChunk raw_x[NCH], raw_d[NCH], raw_b[NCH], raw_e[NCH];
+  if constexpr (kRing) {
+    ring.open();
+    if (threadIdx.x == 0)
+      for (int n = 0; n + 1 < a.stages && ahead < rows; ++n) start();
+  } else if (chunk < rows) {
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       fetch(sp, row_of(a.x, chunk), i, raw_x[i]);
@@ -412,12 +543,16 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS) norm_backward_kernel(const
     const long long out = (static_cast<long long>(sample) * rows + at) * a.width;
     const unsigned next = at + stride;
     float2 r[NCH][4], dn[NCH][4];
+    const unsigned char* stage = nullptr;
+    if constexpr (kRing) stage = ring.next();
+    // a piece of an input: from the stage, as often as it is needed, or from its register
+    auto piece = [&](int k, int i, const RawChunk& held) { return kRing ? staged(sp, stage, k, a.width * 2, i) : held; };
     float2 pscale = both(1.0f), pshift = both(0.0f);  // post norm: b * rstd - mean * rstd
     float prstd = 1.0f;
     if constexpr (POST) {
       float2 b[NCH][4];
 #pragma unroll
-      for (int i = 0; i < NCH; ++i) widen<T>(raw_b[i], b[i]);
+      for (int i = 0; i < NCH; ++i) widen<T>(piece(2, i, raw_b[i]), b[i]);
       const Moments m = row_moments<false>(sp, share, b, b, a.post == kNormLayer, inv, buf[turn][1]);
       prstd = rsqrtf(m.squares * inv + a.post_eps);
       pscale = both(prstd);
@@ -426,15 +561,15 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS) norm_backward_kernel(const
     // r and dn = dh (1 + scale) weight
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      widen<T>(raw_x[i], r[i]);
-      if (next < rows) fetch(sp, row_of(a.x, next), i, raw_x[i]);
+      widen<T>(piece(0, i, raw_x[i]), r[i]);
+      if (!kRing && next < rows) fetch(sp, row_of(a.x, next), i, raw_x[i]);
       float2 d[4];
-      widen<T>(raw_d[i], d);
+      widen<T>(piece(1, i, raw_d[i]), d);
 #pragma unroll
       for (int j = 0; j < 4; ++j) dn[i][j] = fmul2(d[j], factor[i][j]);
       if (a.branch.p) {
         float2 b[4];
-        widen<T>(raw_b[i], b);
+        widen<T>(piece(2, i, raw_b[i]), b);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (POST) b[j] = only_inside(sp, i, j, ffma2(b[j], pscale, pshift));  // the shift of columns past the width
@@ -446,6 +581,7 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS) norm_backward_kernel(const
       }
     }
     const Moments m = row_moments<true>(sp, share, r, dn, a.norm == kNormLayer, inv, buf[turn][0]);
+    if (kRing && threadIdx.x == 0 && ahead < rows) start();  // every thread is done with the rows before this one
     const float rstd = rsqrtf(m.squares * inv + a.eps);
     const float mean_dn = a.norm == kNormLayer ? m.sum_d * inv : 0.0f, mean_dnn = m.sum_dv * rstd * inv;
     const float2 minus = both(-m.mean), times = both(rstd);
@@ -454,10 +590,10 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS) norm_backward_kernel(const
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       float2 d[4], b[4], e4[4];
-      widen<T>(raw_d[i], d);
-      if (a.branch.p) widen<T>(raw_b[i], b);
-      if (a.grad_r.p) widen<T>(raw_e[i], e4);
-      if (next < rows) {
+      widen<T>(piece(1, i, raw_d[i]), d);
+      if (a.branch.p) widen<T>(piece(2, i, raw_b[i]), b);
+      if (a.grad_r.p) widen<T>(piece(3, i, raw_e[i]), e4);
+      if (!kRing && next < rows) {
         fetch(sp, row_of(a.grad_h, next), i, raw_d[i]);
         if (a.branch.p) fetch(sp, row_of(a.branch, next), i, raw_b[i]);
         if (a.grad_r.p) fetch(sp, row_of(a.grad_r, next), i, raw_e[i]);
@@ -507,20 +643,30 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS) norm_backward_kernel(const
       }
     }
   }
+  if constexpr (kRing) ring.close();
   if (a.partial) {
     float* part = a.partial + static_cast<long long>(blockIdx.x) * 3 * a.width;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
 #pragma unroll
-      for (int e = 0; e < kChunk; ++e) {
-        if (!sp.inside(i, e)) continue;
-        const int c = sp.column(i, e);
+      for (int k = 0; k < 3; ++k) {
+        float* to = part + static_cast<long long>(k) * a.width;
+        float2 s[4];
 #pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          float2 s;
-          if constexpr (kShared) s = *shared_at(k, i, e >> 1);
-          else s = k == 0 ? a0[i][e >> 1] : k == 1 ? a1[i][e >> 1] : g0[i][e >> 1];
-          part[static_cast<long long>(k) * a.width + c] = e & 1 ? s.y : s.x;
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (kShared) s[j] = *shared_at(k, i, j);
+          else s[j] = k == 0 ? a0[i][j] : k == 1 ? a1[i][j] : g0[i][j];
+        }
+        if constexpr (MODE != kUnaligned) {
+          if (sp.inside(i, 0)) {
+            float4* p = reinterpret_cast<float4*>(to + sp.column(i, 0));
+            p[0] = make_float4(s[0].x, s[0].y, s[1].x, s[1].y);
+            p[1] = make_float4(s[2].x, s[2].y, s[3].x, s[3].y);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < kChunk; ++e)
+            if (sp.inside(i, e)) to[sp.column(i, e)] = e & 1 ? s[e >> 1].y : s[e >> 1].x;
         }
       }
     }
@@ -554,7 +700,7 @@ __global__ void __launch_bounds__(1024) norm_sums_kernel(const __grid_constant__
     float s = 0.0f;
     if (c < a.width) {
       const float* p = a.partial + static_cast<long long>(b) * a.chunks * 3 * a.width + static_cast<long long>(k) * a.width + c;
-#pragma unroll 4
+#pragma unroll 8
       for (int i = y; i < a.chunks; i += 32) s += p[static_cast<long long>(i) * 3 * a.width];
     }
     red[y][cx] = s;
@@ -594,85 +740,126 @@ int blocks_per_sm(const void* kernel, int threads, std::atomic<int>& known) {
   return n;
 }
 
-template <typename T, int WARPS, int NCH, int BLOCKS, bool ALIGNED, bool POST>
-int launch_backward(const NormArgs& a, cudaStream_t stream) {
-  auto kernel = norm_backward_kernel<T, WARPS, NCH, BLOCKS, ALIGNED, POST>;
-  constexpr int kSmem = NCH > 3 ? 3 * NCH * kChunk * 32 * WARPS * 4 : 0;  // the column sums
-  if (kSmem > 0) {  // granted once per device
-    static std::atomic<unsigned long long> opened;
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return static_cast<int>(e);
-    const unsigned long long bit = 1ull << (dev & 63);
-    if (dev >= 64 || !(opened.load(std::memory_order_relaxed) & bit)) {
-      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-      if (e != cudaSuccess) return static_cast<int>(e);
-      opened.fetch_or(bit, std::memory_order_relaxed);
-    }
+// Lets a kernel take ``bytes`` of dynamic shared memory, once per device.
+cudaError_t grant_smem(const void* kernel, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
+// Stages of a ring with ``blocks`` blocks per SM: as many as fit beside each
+// block's static arrays and the system's part, two at least.
+constexpr int kRingBudget = 220 * 1024;  // of one block alone
+int ring_bytes_of(int blocks) { return (kRingBudget + 4096) / blocks - 4096; }
+int ring_stages(int stage_bytes, int blocks) {
+  const int n = ring_bytes_of(blocks) / stage_bytes;
+  return n < 2 ? 2 : n > kMaxStages ? kMaxStages : n;
+}
+
+template <typename T, int WARPS, int NCH, int BLOCKS, int MODE, bool POST>
+int launch_backward_mode(NormArgs a, cudaStream_t stream) {
+  auto kernel = norm_backward_kernel<T, WARPS, NCH, BLOCKS, MODE, POST>;
+  int smem = NCH > 3 ? 3 * NCH * kChunk * 32 * WARPS * 4 : 0;  // the column sums
+  if (MODE != kUnaligned && WARPS > 1 && NCH <= 3) {
+    a.stage_bytes = a.width * 2 * (a.grad_r.p ? 4 : a.branch.p ? 3 : 2);
+    a.stages = ring_stages(a.stage_bytes, BLOCKS);
+    smem = a.stages * a.stage_bytes;
   }
-  kernel<<<a.samples * a.chunks, 32 * WARPS, kSmem, stream>>>(a);
+  if (smem > 0) {
+    static std::atomic<unsigned long long> opened;
+    const cudaError_t e = grant_smem(reinterpret_cast<const void*>(kernel), kRingBudget, opened);
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  kernel<<<a.samples * a.chunks, 32 * WARPS, smem, stream>>>(a);
   return launch_status();
 }
 
-template <typename T, int WARPS, int NCH, bool ALIGNED, bool POST>
-int launch_forward(const NormArgs& a, cudaStream_t stream) {
+template <typename T, int WARPS, int NCH, int BLOCKS, bool POST>
+int launch_backward(const NormArgs& a, cudaStream_t stream) {
+  if (!a.vec) return launch_backward_mode<T, WARPS, NCH, BLOCKS, kUnaligned, POST>(a, stream);
+  if (a.width == 32 * kChunk * WARPS * NCH) return launch_backward_mode<T, WARPS, NCH, BLOCKS, kFull, POST>(a, stream);
+  return launch_backward_mode<T, WARPS, NCH, BLOCKS, kAligned, POST>(a, stream);
+}
+
+template <typename T, int WARPS, int NCH, int MODE, bool POST>
+int launch_forward_mode(NormArgs a, cudaStream_t stream) {
   constexpr int kRows = WARPS < 4 ? 4 / WARPS : 1, kBlock = WARPS < 4 ? 128 : 32 * WARPS;
-  auto kernel = norm_forward_kernel<T, WARPS, NCH, ALIGNED, POST>;
+  auto kernel = norm_forward_kernel<T, WARPS, NCH, MODE, POST>;
   static std::atomic<int> resident;
+  int blocks = blocks_per_sm(reinterpret_cast<const void*>(kernel), kBlock, resident), smem = 0;
+  if (MODE != kUnaligned && WARPS > 1) {
+    a.stage_bytes = a.width * 2 * (a.branch.p ? 2 : 1);
+    while (blocks > 1 && ring_bytes_of(blocks) < 2 * a.stage_bytes) --blocks;
+    a.stages = ring_stages(a.stage_bytes, blocks);
+    smem = a.stages * a.stage_bytes;
+    static std::atomic<unsigned long long> opened;
+    const cudaError_t e = grant_smem(reinterpret_cast<const void*>(kernel), kRingBudget, opened);
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
   const long long want = (static_cast<long long>(a.samples) * a.rows + kRows - 1) / kRows;
-  const long long most = static_cast<long long>(kNumSMs) * blocks_per_sm(reinterpret_cast<const void*>(kernel), kBlock, resident);
-  kernel<<<static_cast<unsigned>(want < most ? want : most), kBlock, 0, stream>>>(a);
+  const long long most = static_cast<long long>(kNumSMs) * blocks;
+  kernel<<<static_cast<unsigned>(want < most ? want : most), kBlock, smem, stream>>>(a);
   return launch_status();
+}
+
+template <typename T, int WARPS, int NCH, bool POST>
+int launch_forward(const NormArgs& a, cudaStream_t stream) {
+  if (!a.vec) return launch_forward_mode<T, WARPS, NCH, kUnaligned, POST>(a, stream);
+  if (a.width == 32 * kChunk * WARPS * NCH) return launch_forward_mode<T, WARPS, NCH, kFull, POST>(a, stream);
+  return launch_forward_mode<T, WARPS, NCH, kAligned, POST>(a, stream);
 }
 
 #ifndef BW_W
-#define BW_W 12
-#define BW_N 1
-#define BW_B 1
+#define BW_W 6
+#define BW_N 2
+#define BW_B 2
 #endif
-// Warps per row: the fewest whose threads hold the row in three chunks each
-// (few warps make the row's reduction cheap), more chunks only past 8192 columns.
-template <typename T, bool ALIGNED, bool POST>
-int launch_width(const NormArgs& a, bool backward, cudaStream_t stream) {
+#ifndef FW_W
+#define FW_W 4
+#define FW_N 3
+#endif
+template <typename T, bool POST>
+int launch_norm(const NormArgs& a, bool backward, cudaStream_t stream) {
   const int w = a.width;
   if (backward) {
-    if (w <= 256) return launch_backward<T, 1, 1, 16, ALIGNED, POST>(a, stream);
-    if (w <= 1024) return launch_backward<T, 4, 1, 4, ALIGNED, POST>(a, stream);
-    if (w <= 2048) return launch_backward<T, 8, 1, 2, ALIGNED, POST>(a, stream);
-    if (w <= 3072) return launch_backward<T, BW_W, BW_N, BW_B, ALIGNED, POST>(a, stream);
-    if (w <= 4096) return launch_backward<T, 16, 1, 1, ALIGNED, POST>(a, stream);
-    if (w <= 8192) return launch_backward<T, 16, 2, 1, ALIGNED, POST>(a, stream);
-    return launch_backward<T, 16, 4, 1, ALIGNED, POST>(a, stream);
+    if (w <= 256) return launch_backward<T, 1, 1, 12, POST>(a, stream);
+    if (w <= 512) return launch_backward<T, 1, 2, 12, POST>(a, stream);
+    if (w <= 1024) return launch_backward<T, 4, 1, 4, POST>(a, stream);
+    if (w <= 2048) return launch_backward<T, 4, 2, 3, POST>(a, stream);
+    if (w <= 3072) return launch_backward<T, BW_W, BW_N, BW_B, POST>(a, stream);
+    if (w <= 4096) return launch_backward<T, 8, 2, 1, POST>(a, stream);
+    if (w <= 6144) return launch_backward<T, 12, 2, 1, POST>(a, stream);
+    if (w <= 8192) return launch_backward<T, 16, 2, 1, POST>(a, stream);
+    return launch_backward<T, 16, 4, 1, POST>(a, stream);
   }
-  if (w <= 256) return launch_forward<T, 1, 1, ALIGNED, POST>(a, stream);
-  if (w <= 768) return launch_forward<T, 1, 3, ALIGNED, POST>(a, stream);
-  if (w <= 1024) return launch_forward<T, 4, 1, ALIGNED, POST>(a, stream);
-  if (w <= 2048) return launch_forward<T, 4, 2, ALIGNED, POST>(a, stream);
-  if (w <= 3072) return launch_forward<T, 4, 3, ALIGNED, POST>(a, stream);
-  if (w <= 4096) return launch_forward<T, 8, 2, ALIGNED, POST>(a, stream);
-  if (w <= 6144) return launch_forward<T, 8, 3, ALIGNED, POST>(a, stream);
-  if (w <= 8192) return launch_forward<T, 16, 2, ALIGNED, POST>(a, stream);
-  return launch_forward<T, 16, 4, ALIGNED, POST>(a, stream);
+  if (w <= 256) return launch_forward<T, 1, 1, POST>(a, stream);
+  if (w <= 768) return launch_forward<T, 1, 3, POST>(a, stream);
+  if (w <= 1024) return launch_forward<T, 4, 1, POST>(a, stream);
+  if (w <= 2048) return launch_forward<T, 4, 2, POST>(a, stream);
+  if (w <= 3072) return launch_forward<T, FW_W, FW_N, POST>(a, stream);
+  if (w <= 4096) return launch_forward<T, 8, 2, POST>(a, stream);
+  if (w <= 6144) return launch_forward<T, 8, 3, POST>(a, stream);
+  if (w <= 8192) return launch_forward<T, 16, 2, POST>(a, stream);
+  return launch_forward<T, 16, 4, POST>(a, stream);
 }
 
-template <typename T>
-int launch_norm(const NormArgs& a, bool backward, cudaStream_t stream) {
-  if (a.vec)
-    return a.post ? launch_width<T, true, true>(a, backward, stream) : launch_width<T, true, false>(a, backward, stream);
-  return a.post ? launch_width<T, false, true>(a, backward, stream) : launch_width<T, false, false>(a, backward, stream);
+int launch_any(const NormArgs& a, int dtype, bool backward, cudaStream_t stream) {
+  if (a.post)
+    return dtype == 1 ? launch_norm<__nv_bfloat16, true>(a, backward, stream) : launch_norm<__half, true>(a, backward, stream);
+  return dtype == 1 ? launch_norm<__nv_bfloat16, false>(a, backward, stream) : launch_norm<__half, false>(a, backward, stream);
 }
 
-// Row chunks per sample of the backward kernel, one block each: as many as are
-// resident at about 8 warps per SM, but 8 rows each at least, so that the
-// partial sums stay a small part of the traffic.
+// Row chunks per sample of the backward kernel, one block each: the resident
+// blocks of launch_backward, but no more than there are rows.
 int norm_chunks(int samples, int rows, int width) {
   if (samples < 1) return 1;
-  const long long per_sm = width <= 256 ? 16 : width <= 1024 ? 4 : width <= 2048 ? 2 : width <= 3072 ? BW_B : 1;
+  const long long per_sm = width <= 512 ? 12 : width <= 1024 ? 4 : width <= 2048 ? 3 : width <= 3072 ? BW_B : 1;
   long long chunks = (per_sm * kNumSMs + samples - 1) / samples;
-  const long long fewest = kNumSMs / samples + 1;  // short inputs still spread over the SMs
-  long long most = (rows + 7) / 8;
-  if (most < fewest) most = fewest;
-  if (chunks > most) chunks = most;
   if (chunks > rows) chunks = rows;
   return chunks < 1 ? 1 : static_cast<int>(chunks);
 }
@@ -726,7 +913,8 @@ extern "C" int peco_gated_norm(const void* x, long long x_batch, long long x_row
   a.eps = eps;
   a.post_eps = post_eps;
   a.residual_scale = residual_scale;
-  return dtype == 1 ? launch_norm<__nv_bfloat16>(a, false, stream) : launch_norm<__half>(a, false, stream);
+  a.status = device_status_ptr();
+  return launch_any(a, dtype, false, stream);
 }
 
 extern "C" long long peco_gated_norm_backward_workspace(int samples, int rows, int width) {
@@ -779,8 +967,9 @@ extern "C" int peco_gated_norm_backward(
   a.eps = eps;
   a.post_eps = post_eps;
   a.residual_scale = residual_scale;
+  a.status = device_status_ptr();
   a.chunks = norm_chunks(samples, rows, width);
-  int st = dtype == 1 ? launch_norm<__nv_bfloat16>(a, true, stream) : launch_norm<__half>(a, true, stream);
+  int st = launch_any(a, dtype, true, stream);
   if (st || !sums) return st;
   NormSumsArgs s{};
   s.partial = a.partial;
