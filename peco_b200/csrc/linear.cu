@@ -77,18 +77,10 @@ __device__ __forceinline__ float activate(float z) {
   }
 }
 
-// (act(z), act'(z))
+// (act(z), act'(z)) of the forms that take no pairs
 template <int ACT>
 __device__ __forceinline__ float2 activate_slope(float z) {
-  if constexpr (ACT == kActGeluTanh) {
-    const float z2 = z * z;
-    const float s = recip_approx(1.0f + exp2_approx(z * fmaf(-kLog2e * kGelu3, z2, -kLog2e * kGelu1)));
-    // d/dz [z s(2u)] = s + z s (1 - s) d(2u)/dz
-    const float d = z * fmaf(3.0f * kGelu3, z2, kGelu1);
-    const float slope = fmaf(s, fmaf(-s, d, d), s);
-    // far out the product of a vanishing and an overflowing factor is replaced by its limit
-    return make_float2(z * s, fabsf(z) > 32.0f ? (z > 0.0f ? 1.0f : 0.0f) : slope);
-  } else if constexpr (ACT == kActGelu) {
+  if constexpr (ACT == kActGelu) {
     const float p = 0.5f * (1.0f + erff(z * 0.7071067811865476f));
     return make_float2(z * p, fmaf(z * 0.3989422804014327f, exp2_approx(-0.5f * kLog2e * z * z), p));
   } else if constexpr (ACT == kActSilu) {
@@ -96,6 +88,30 @@ __device__ __forceinline__ float2 activate_slope(float z) {
     return make_float2(z * s, s * fmaf(z, 1.0f - s, 1.0f));
   } else {
     return make_float2(z, 1.0f);
+  }
+}
+
+// (act(z), act'(z)) of a pair; the value only where ``value`` is set
+template <int ACT, bool VALUE>
+__device__ __forceinline__ void activate_slope2(float2 z, float2& value, float2& slope) {
+  auto both = [](float x) { return make_float2(x, x); };
+  if constexpr (ACT == kActGeluTanh) {
+    const float2 z2 = fmul2(z, z);
+    const float2 w = fmul2(z, ffma2(z2, both(-kLog2e * kGelu3), both(-kLog2e * kGelu1)));
+    const float2 e = fadd2(make_float2(exp2_approx(w.x), exp2_approx(w.y)), both(1.0f));
+    const float2 s = make_float2(recip_approx(e.x), recip_approx(e.y));
+    // s + z s (1 - s) d(2u)/dz; far out a vanishing factor meets one that
+    // overflows, which is held finite (a NaN comes back through s)
+    float2 d = fmul2(z, ffma2(z2, both(3.0f * kGelu3), both(kGelu1)));
+    d.x = fminf(fmaxf(d.x, -1e30f), 1e30f);
+    d.y = fminf(fmaxf(d.y, -1e30f), 1e30f);
+    const float2 rest = ffma2(make_float2(-s.x, -s.y), d, d);
+    slope = ffma2(s, rest, s);
+    if (VALUE) value = fmul2(z, s);
+  } else {
+    const float2 a = activate_slope<ACT>(z.x), b = activate_slope<ACT>(z.y);
+    value = make_float2(a.x, b.x);
+    slope = make_float2(a.y, b.y);
   }
 }
 
@@ -568,59 +584,94 @@ struct ActBackwardArgs {
   int act, vec;
 };
 
-template <typename T, int ACT, bool GATE>
-__global__ void __launch_bounds__(256, GATE ? 3 : 4) act_backward_kernel(const ActBackwardArgs a) {
-  __shared__ float red[2][8][256];
+// 8 neighbouring elements as four pairs
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_pairs(const T* p, int count, float2 (&v)[4]) {
+  if constexpr (VEC) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    v[0] = unpack2<T>(u.x), v[1] = unpack2<T>(u.y), v[2] = unpack2<T>(u.z), v[3] = unpack2<T>(u.w);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = make_float2(2 * i < count ? to_f32<T>(p[2 * i]) : 0.0f, 2 * i + 1 < count ? to_f32<T>(p[2 * i + 1]) : 0.0f);
+  }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_pairs(T* p, int count, const float2 (&v)[4]) {
+  if constexpr (VEC) {
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(pack2<T>(v[0].x, v[0].y), pack2<T>(v[1].x, v[1].y), pack2<T>(v[2].x, v[2].y), pack2<T>(v[3].x, v[3].y));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (2 * i < count) p[2 * i] = from_f32<T>(v[i].x);
+      if (2 * i + 1 < count) p[2 * i + 1] = from_f32<T>(v[i].y);
+    }
+  }
+}
+
+template <typename T, int ACT, bool GATE, bool VEC>
+__global__ void __launch_bounds__(256, GATE ? 3 : 4) act_backward_kernel(const __grid_constant__ ActBackwardArgs a) {
+  __shared__ float red[GATE ? 2 : 1][8][256];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sample = blockIdx.y / a.chunks, chunk = blockIdx.y - sample * a.chunks;
   const int col = blockIdx.x * 256 + lane * 8;
   const int count = min(8, a.n - col);
-  float gate[8], sum_dz[8], sum_ga[8];
+  constexpr bool kValue = ACT != kActNone || GATE;  // the pre-activation is read
+  float2 gate[4], sum_dz[4], sum_ga[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    gate[i] = 1.0f;
-    sum_dz[i] = sum_ga[i] = 0.0f;
-  }
+  for (int i = 0; i < 4; ++i) sum_dz[i] = sum_ga[i] = gate[i] = make_float2(0.0f, 0.0f);
   if (count > 0) {
-    if (GATE) load_vec<8>(static_cast<const T*>(a.gate) + sample * a.gate_stride + col, a.vec, count, gate);
-    const int begin = chunk * a.chunk_rows, end = min(begin + a.chunk_rows, a.rows_per_sample);
-    const long long row0 = static_cast<long long>(sample) * a.rows_per_sample;
+    if (GATE) load_pairs<T, VEC>(static_cast<const T*>(a.gate) + sample * a.gate_stride + col, count, gate);
+    const int begin = chunk * a.chunk_rows + warp, end = min((chunk + 1) * a.chunk_rows, a.rows_per_sample);
+    const long long row0 = static_cast<long long>(sample) * a.rows_per_sample + begin;
+    const T* gp = static_cast<const T*>(a.grad) + row0 * a.grad_stride + col;
+    const T* zp = static_cast<const T*>(a.preact) + row0 * a.n + col;
+    T* dp = static_cast<T*>(a.dz) + row0 * a.dz_stride + col;
+    const long long g_step = 8 * a.grad_stride, z_step = 8LL * a.n, d_step = 8LL * a.dz_stride;
+    const bool read_z = kValue && a.preact, write = a.dz != nullptr;
     // two of the warp's rows in flight
-    for (int r = begin + warp; r < end; r += 16) {
-      float g[2][8], z[2][8];
+    for (int r = begin; r < end; r += 16) {
+      float2 g[2][4], z[2][4];
+      const int rows = r + 8 < end ? 2 : 1;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if (r + 8 * j < end) {
-          const long long row = row0 + r + 8 * j;
-          load_vec<8>(static_cast<const T*>(a.grad) + row * a.grad_stride + col, a.vec, count, g[j]);
-          if (a.preact) load_vec<8>(static_cast<const T*>(a.preact) + row * a.n + col, a.vec, count, z[j]);
+        if (j < rows) {
+          load_pairs<T, VEC>(gp + j * g_step, count, g[j]);
+          if (read_z) load_pairs<T, VEC>(zp + j * z_step, count, z[j]);
         }
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if (r + 8 * j < end) {
-          float dz[8];
+        if (j < rows) {
+          float2 dz[4];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            dz[i] = GATE ? g[j][i] * gate[i] : g[j][i];
-            if (a.preact) {
-              const float2 f = activate_slope<ACT>(z[j][i]);
-              dz[i] *= f.y;
-              if (GATE) sum_ga[i] = fmaf(g[j][i], f.x, sum_ga[i]);
+          for (int i = 0; i < 4; ++i) {
+            dz[i] = GATE ? fmul2(g[j][i], gate[i]) : g[j][i];
+            if (read_z) {
+              float2 value = z[j][i], slope;
+              if constexpr (ACT != kActNone) {
+                activate_slope2<ACT, GATE>(z[j][i], value, slope);
+                dz[i] = fmul2(dz[i], slope);
+              }
+              if (GATE) sum_ga[i] = ffma2(g[j][i], value, sum_ga[i]);
             }
-            sum_dz[i] += dz[i];
+            sum_dz[i] = fadd2(sum_dz[i], dz[i]);
           }
           // dz is rounded to the operands' type for the tensor core; its sums are not
-          if (a.dz) store_vec<8>(static_cast<T*>(a.dz) + (row0 + r + 8 * j) * a.dz_stride + col, a.vec, count, dz);
+          if (write) store_pairs<T, VEC>(dp + j * d_step, count, dz);
         }
       }
+      gp += 2 * g_step;
+      zp += 2 * z_step;
+      dp += 2 * d_step;
     }
   }
   if (!a.part_bias && !a.part_gate) return;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    red[0][warp][lane * 8 + i] = sum_dz[i];
-    red[1][warp][lane * 8 + i] = sum_ga[i];
+  for (int i = 0; i < 4; ++i) {
+    *reinterpret_cast<float2*>(&red[0][warp][lane * 8 + 2 * i]) = sum_dz[i];
+    if (GATE) *reinterpret_cast<float2*>(&red[GATE ? 1 : 0][warp][lane * 8 + 2 * i]) = sum_ga[i];
   }
   __syncthreads();
   const int c = blockIdx.x * 256 + threadIdx.x;
@@ -629,11 +680,11 @@ __global__ void __launch_bounds__(256, GATE ? 3 : 4) act_backward_kernel(const A
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
       s0 += red[0][w][threadIdx.x];
-      s1 += red[1][w][threadIdx.x];
+      if (GATE) s1 += red[GATE ? 1 : 0][w][threadIdx.x];
     }
     const long long at = static_cast<long long>(blockIdx.y) * a.n + c;
     if (a.part_bias) a.part_bias[at] = s0;
-    if (a.part_gate) a.part_gate[at] = s1;
+    if (GATE && a.part_gate) a.part_gate[at] = s1;
   }
 }
 
@@ -876,8 +927,10 @@ BackwardPlan plan_backward(const LinearShape& s, const Operand& grad, bool has_g
 
 template <typename T, int ACT>
 void launch_act_backward(const ActBackwardArgs& a, dim3 grid, cudaStream_t stream) {
-  if (a.gate) act_backward_kernel<T, ACT, true><<<grid, 256, 0, stream>>>(a);
-  else act_backward_kernel<T, ACT, false><<<grid, 256, 0, stream>>>(a);
+  if (a.gate && a.vec) act_backward_kernel<T, ACT, true, true><<<grid, 256, 0, stream>>>(a);
+  else if (a.gate) act_backward_kernel<T, ACT, true, false><<<grid, 256, 0, stream>>>(a);
+  else if (a.vec) act_backward_kernel<T, ACT, false, true><<<grid, 256, 0, stream>>>(a);
+  else act_backward_kernel<T, ACT, false, false><<<grid, 256, 0, stream>>>(a);
 }
 
 template <typename T>

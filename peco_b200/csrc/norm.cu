@@ -795,7 +795,9 @@ int launch_forward_mode(NormArgs a, cudaStream_t stream) {
   if (MODE != kUnaligned && WARPS > 1) {
     a.stage_bytes = a.width * 2 * (a.branch.p ? 2 : 1);
     while (blocks > 1 && ring_bytes_of(blocks) < 2 * a.stage_bytes) --blocks;
-    a.stages = ring_stages(a.stage_bytes, blocks);
+    // three stages: deeper rings read further ahead of the writes and measured
+    // slower (gated rows of 3072: 145 us with three, 161 with four and more)
+    a.stages = ring_stages(a.stage_bytes, blocks) < 3 ? 2 : 3;
     smem = a.stages * a.stage_bytes;
     static std::atomic<unsigned long long> opened;
     const cudaError_t e = grant_smem(reinterpret_cast<const void*>(kernel), kRingBudget, opened);
@@ -814,15 +816,10 @@ int launch_forward(const NormArgs& a, cudaStream_t stream) {
   return launch_forward_mode<T, WARPS, NCH, kAligned, POST>(a, stream);
 }
 
-#ifndef BW_W
-#define BW_W 6
-#define BW_N 2
-#define BW_B 2
-#endif
-#ifndef FW_W
-#define FW_W 4
-#define FW_N 3
-#endif
+// Threads per row.  Few warps keep a row's reduction cheap, few columns per
+// thread its registers; measured at 3072 columns (34680 rows): backward 238 us
+// with 6 warps x 2 chunks, 412 with 12 x 1, 234 with 4 x 3 (equal at 7006 rows);
+// forward 145 us with 4 x 3, 161 with 12 x 1, 179 with 8 x 2.
 template <typename T, bool POST>
 int launch_norm(const NormArgs& a, bool backward, cudaStream_t stream) {
   const int w = a.width;
@@ -831,7 +828,7 @@ int launch_norm(const NormArgs& a, bool backward, cudaStream_t stream) {
     if (w <= 512) return launch_backward<T, 1, 2, 12, POST>(a, stream);
     if (w <= 1024) return launch_backward<T, 4, 1, 4, POST>(a, stream);
     if (w <= 2048) return launch_backward<T, 4, 2, 3, POST>(a, stream);
-    if (w <= 3072) return launch_backward<T, BW_W, BW_N, BW_B, POST>(a, stream);
+    if (w <= 3072) return launch_backward<T, 6, 2, 2, POST>(a, stream);
     if (w <= 4096) return launch_backward<T, 8, 2, 1, POST>(a, stream);
     if (w <= 6144) return launch_backward<T, 12, 2, 1, POST>(a, stream);
     if (w <= 8192) return launch_backward<T, 16, 2, 1, POST>(a, stream);
@@ -841,7 +838,7 @@ int launch_norm(const NormArgs& a, bool backward, cudaStream_t stream) {
   if (w <= 768) return launch_forward<T, 1, 3, POST>(a, stream);
   if (w <= 1024) return launch_forward<T, 4, 1, POST>(a, stream);
   if (w <= 2048) return launch_forward<T, 4, 2, POST>(a, stream);
-  if (w <= 3072) return launch_forward<T, FW_W, FW_N, POST>(a, stream);
+  if (w <= 3072) return launch_forward<T, 4, 3, POST>(a, stream);
   if (w <= 4096) return launch_forward<T, 8, 2, POST>(a, stream);
   if (w <= 6144) return launch_forward<T, 8, 3, POST>(a, stream);
   if (w <= 8192) return launch_forward<T, 16, 2, POST>(a, stream);
@@ -858,7 +855,7 @@ int launch_any(const NormArgs& a, int dtype, bool backward, cudaStream_t stream)
 // blocks of launch_backward, but no more than there are rows.
 int norm_chunks(int samples, int rows, int width) {
   if (samples < 1) return 1;
-  const long long per_sm = width <= 512 ? 12 : width <= 1024 ? 4 : width <= 2048 ? 3 : width <= 3072 ? BW_B : 1;
+  const long long per_sm = width <= 512 ? 12 : width <= 1024 ? 4 : width <= 2048 ? 3 : width <= 3072 ? 2 : 1;
   long long chunks = (per_sm * kNumSMs + samples - 1) / samples;
   if (chunks > rows) chunks = rows;
   return chunks < 1 ? 1 : static_cast<int>(chunks);
