@@ -29,7 +29,7 @@ enum Activation : int { kActNone = 0, kActGeluTanh = 1, kActGelu = 2, kActSilu =
 constexpr int kTileM = 128;
 constexpr int kTileK = 64;   // one 128-byte swizzle panel of 16-bit elements
 constexpr int kEpilogueWarps = 8;
-constexpr int kGemmThreads = 64 + 32 * kEpilogueWarps;  // TMA warp, MMA warp, epilogue warps
+constexpr int kGemmThreads = 96 + 32 * kEpilogueWarps;  // TMA warp for A, MMA warp, epilogue warps, TMA warp for B
 
 struct GemmArgs {
   CUtensorMap a[2], b[2];    // K segments (x and x2; the second unused otherwise)
@@ -37,6 +37,7 @@ struct GemmArgs {
   int m, n, tiles_m, tiles_n;
   int bn;                    // columns of a tile, a multiple of 32
   int a_panels, b_panels;    // 64-wide panels of an MN-major operand per CTA
+  int a_joined, b_joined;    // ... all of them in one copy (the operand's width is a multiple of 64)
   uint32_t stage_tx;         // bytes one CTA loads per K block
   void* out;
   long long out_stride;
@@ -151,6 +152,22 @@ __device__ __forceinline__ void tile_load_2d(uint32_t dst, const CUtensorMap* ma
 }
 
 template <int CG>
+__device__ __forceinline__ void tile_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  if constexpr (CG == 1) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+            "r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  }
+}
+
+template <int CG>
 __device__ __forceinline__ void product_step(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   if constexpr (CG == 1) {
     umma_ss(d, a, b, idesc, accumulate);
@@ -211,7 +228,10 @@ __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
 // blocks.  The groups' fp32 partial tiles meet in shared memory: every CTA
 // adds 128 / S rows over the S partials, in the groups' order, and finishes
 // them.
-constexpr int kStages = 6;
+#ifndef KST
+#define KST 6
+#endif
+constexpr int kStages = KST;
 constexpr int kABytes = kTileM * kTileK * 2;
 constexpr int kStageBytes = 2 * kABytes;        // A's 128 rows and up to 128 of B
 constexpr int kRingBytes = kStages * kStageBytes;
@@ -229,7 +249,10 @@ struct GemmShared {
 
 // (m tile, n tile) of a linear tile number: bands of kBand m tiles walked
 // down first, so that the CTAs running at one time share few rows of A and B
-constexpr int kBand = 8;
+#ifndef KBAND
+#define KBAND 8
+#endif
+constexpr int kBand = KBAND;
 __device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int& tm, int& tn) {
   const int per_band = kBand * tiles_n;
   const int band = t / per_band;
@@ -241,21 +264,39 @@ __device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int
 }
 
 // Operand rows x 64 into shared memory: K-major rows of 128 bytes (one box), or
-// MN-major panels of 64 elements x 64 K rows
+// MN-major panels of 64 elements x 64 K rows, in one copy of a [panel][K][64]
+// view where the operand's width allows it
 template <int CG, bool MN>
-__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int row0, int panels, int kb, uint32_t bar) {
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int row0, int panels, int joined, int k0,
+                                          uint32_t bar) {
   if constexpr (!MN) {
-    tile_load_2d<CG>(dst, map, kb * kTileK, row0, bar);
+    tile_load_2d<CG>(dst, map, k0, row0, bar);
+  } else if (joined) {
+    tile_load_3d<CG>(dst, map, 0, k0, row0 >> 6, bar);
   } else {
-    for (int p = 0; p < panels; ++p) tile_load_2d<CG>(dst + p * 8192, map, row0 + p * 64, kb * kTileK, bar);
+    for (int p = 0; p < panels; ++p) tile_load_2d<CG>(dst + p * 8192, map, row0 + p * 64, k0, bar);
   }
 }
 
-// descriptor of the k-th 16-wide K step of a tile
+// what the k-th 16-wide K step of a tile adds to its descriptor's address (16-byte units)
 template <bool MN>
-__device__ __forceinline__ uint64_t step_desc(uint32_t base, int k) {
-  return MN ? smem_desc(base + k * 2048, 8192, 1024) : smem_desc(base + k * 32, 16, 1024);
+__device__ __forceinline__ constexpr uint32_t step_offset(int k) { return MN ? k * 128 : k * 2; }
+template <bool MN>
+__device__ __forceinline__ uint64_t tile_desc(uint32_t base) {
+  return MN ? smem_desc(base, 8192, 1024) : smem_desc(base, 16, 1024);
 }
+
+// Position in the ring: stage and the phase of its barriers.
+struct RingPos {
+  int s = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void step() {
+    if (++s == kStages) {
+      s = 0;
+      phase ^= 1;
+    }
+  }
+};
 
 template <int ACT>
 __device__ __forceinline__ void activate_all(float (&v)[8]) {
@@ -423,28 +464,31 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
   const int kb_begin = SPLIT ? static_cast<int>(static_cast<long long>(kblocks) * part / splits) : 0;
   const int kb_end = SPLIT ? static_cast<int>(static_cast<long long>(kblocks) * (part + 1) / splits) : kblocks;
 
-  if (warp == 0) {
-    // ---------------------------------------------------------------- TMA
+  if (warp == 0 || warp == kEpilogueWarps + 2) {
+    // ------------------------------------------- TMA: one warp for A, one for B
     if (lane == 0) {
+      const bool is_a = warp == 0;
       bool ok = true;
-      uint32_t it = 0;
+      RingPos pos;
+      // the pair's stages fill one barrier, the first CTA's, which expects both CTAs' bytes
+      const uint32_t bar0 = CG > 1 ? map_rank(smem_u32(&sh.full[0]), lead) : smem_u32(&sh.full[0]);
       for (int t = group; t < tiles && ok; t += groups) {
         int tm, tn;
         tile_coords(t, args.tiles_m, args.tiles_n, tm, tn);
-        const int row_a = (tm * CG + rank) * kTileM, row_b = tn * args.bn + rank * (args.bn / CG);
-        for (int kb = kb_begin; kb < kb_end; ++kb, ++it) {
-          const int s = it % kStages;
-          ok = mbar_wait(&sh.empty[s], ((it / kStages) & 1) ^ 1, abort_flag, args.status);
+        const int row0 = is_a ? (tm * CG + rank) * kTileM : tn * args.bn + rank * (args.bn / CG);
+        for (int kb = kb_begin; kb < kb_end; ++kb) {
+          ok = mbar_wait(&sh.empty[pos.s], pos.phase ^ 1, abort_flag, args.status);
           if (!ok) break;
-          const uint32_t st = ring + s * kStageBytes;
-          // the pair's stages fill one barrier, the first CTA's, which expects both CTAs' bytes
-          uint32_t bar = smem_u32(&sh.full[s]);
-          if (CG > 1) bar = map_rank(bar, lead);
-          if (rank == 0) mbar_arrive_expect_tx(&sh.full[s], CG * args.stage_tx);
+          const uint32_t st = ring + pos.s * kStageBytes, bar = bar0 + pos.s * 8;
           const int seg = kb >= kb0 ? 1 : 0;
-          const int kx = kb - (seg ? kb0 : 0);
-          load_tile<CG, AMN>(st, &args.a[seg], row_a, args.a_panels, kx, bar);
-          load_tile<CG, BMN>(st + kABytes, &args.b[seg], row_b, args.b_panels, kx, bar);
+          const int k0 = (kb - (seg ? kb0 : 0)) * kTileK;
+          if (is_a) {
+            if (rank == 0) mbar_arrive_expect_tx(&sh.full[pos.s], CG * args.stage_tx);
+            load_tile<CG, AMN>(st, &args.a[seg], row0, args.a_panels, args.a_joined, k0, bar);
+          } else {
+            load_tile<CG, BMN>(st + kABytes, &args.b[seg], row0, args.b_panels, args.b_joined, k0, bar);
+          }
+          pos.step();
         }
       }
       // after an expired wait: time for the copies still in flight to land before the CTA ends
@@ -459,24 +503,29 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     if (lane == 0 && rank == 0) {
       constexpr int ab = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
       const uint32_t idesc = instr_desc(kTileM * CG, args.bn, ab, AMN, BMN);
+      const uint64_t desc_a = tile_desc<AMN>(ring), desc_b = tile_desc<BMN>(ring + kABytes);
       bool ok = true;
-      uint32_t it = 0, local = 0;
+      RingPos pos;
+      uint32_t local = 0;
       for (int t = group; t < tiles && ok; t += groups, ++local) {
         const int b = local & 1;
         ok = mbar_wait(&sh.acc_empty[b], ((local >> 1) & 1) ^ 1, abort_flag, args.status);
         if (!ok) break;
         tc_fence_after();
-        for (int kb = kb_begin; kb < kb_end; ++kb, ++it) {
-          const int s = it % kStages;
-          ok = mbar_wait(&sh.full[s], (it / kStages) & 1, abort_flag, args.status);
+        const uint32_t acc = tmem + b * kAccumulator;
+        uint32_t accumulate = 0;
+        for (int kb = kb_begin; kb < kb_end; ++kb) {
+          ok = mbar_wait(&sh.full[pos.s], pos.phase, abort_flag, args.status);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t sa = ring + s * kStageBytes, sb = sa + kABytes;
+          const uint32_t at = pos.s * (kStageBytes >> 4);
 #pragma unroll
-          for (int k = 0; k < kTileK / 16; ++k)
-            product_step<CG>(tmem + b * kAccumulator, step_desc<AMN>(sa, k), step_desc<BMN>(sb, k), idesc,
-                             (kb > kb_begin || k) ? 1u : 0u);
-          product_commit<CG>(&sh.empty[s], lead);
+          for (int k = 0; k < kTileK / 16; ++k) {
+            product_step<CG>(acc, desc_a + (at + step_offset<AMN>(k)), desc_b + (at + step_offset<BMN>(k)), idesc, accumulate);
+            accumulate = 1;
+          }
+          product_commit<CG>(&sh.empty[pos.s], lead);
+          pos.step();
         }
         if (ok) product_commit<CG>(&sh.acc_full[b], lead);
       }
@@ -759,13 +808,19 @@ int prepare_operand(Operand& o, Carver& ws, cudaStream_t stream) {
   return launch_status();
 }
 
-bool operand_map(CUtensorMap* map, const Operand& o, bool mn, int tile_rows, int dtype) {
+bool operand_map(CUtensorMap* map, const Operand& o, bool mn, int tile_rows, int joined_panels, int dtype) {
+  const CUtensorMapDataType type = dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  if (joined_panels) {  // [width / 64][K][64]
+    const uint64_t dims[3] = {64, static_cast<uint64_t>(o.rows), static_cast<uint64_t>(o.cols / 64)};
+    const uint64_t strides[2] = {static_cast<uint64_t>(o.stride) * 2, 128};
+    const uint32_t box[3] = {64, 64, static_cast<uint32_t>(joined_panels)};
+    return encode_tensor_map(map, type, 3, o.ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  }
   const uint64_t dims[2] = {static_cast<uint64_t>(o.cols), static_cast<uint64_t>(o.rows)};
   const uint64_t strides[1] = {static_cast<uint64_t>(o.stride) * 2};
   // K-major: 64 K columns of tile_rows rows; MN-major: 64 columns of 64 K rows
   const uint32_t box[2] = {64, static_cast<uint32_t>(mn ? 64 : tile_rows)};
-  return encode_tensor_map(map, dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-                           o.ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  return encode_tensor_map(map, type, 2, o.ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // Dynamic shared memory of a kernel, granted once per device.
@@ -855,8 +910,12 @@ int launch_gemm(GemmArgs& g, const Operand* a, const Operand* b, int segments, i
   g.a_panels = g.m > 64 ? 2 : 1;
   g.b_panels = (b_rows + 63) / 64;
   g.stage_tx = (AMN ? g.a_panels * 8192 : a_rows * 128) + (BMN ? g.b_panels * 8192 : b_rows * 128);
+  // a joined copy starts on a whole panel
+  g.a_joined = AMN && g.m % 64 == 0;
+  g.b_joined = BMN && g.n % 64 == 0 && b_rows % 64 == 0;
   for (int s = 0; s < segments; ++s)
-    if (!operand_map(&g.a[s], a[s], AMN, a_rows, dtype) || !operand_map(&g.b[s], b[s], BMN, b_rows, dtype))
+    if (!operand_map(&g.a[s], a[s], AMN, a_rows, g.a_joined ? g.a_panels : 0, dtype) ||
+        !operand_map(&g.b[s], b[s], BMN, b_rows, g.b_joined ? g.b_panels : 0, dtype))
       return kErrTensorMap;
   g.status = device_status_ptr();
   if (c.splits > 1)
