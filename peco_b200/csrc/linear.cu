@@ -213,8 +213,8 @@ __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
 }
 
 // ---- the product -----------------------------------------------------------------
-// Output tiles of (128 CG) x bn, walked by persistent groups of CG CTAs.  Warp
-// 0 of every CTA streams its 64-wide K blocks of A (128 rows) and B (bn / CG
+// Output tiles of (128 CG) x bn, walked by persistent groups of CG CTAs.  Two
+// warps of every CTA stream its 64-wide K blocks of A (128 rows) and B (bn / CG
 // rows) through a ring of shared-memory stages; warp 1 of the group's first
 // CTA issues the MMAs into one of two TMEM accumulators; warps 2-9 read the
 // other one back, apply the epilogue and store, so the epilogue of a tile runs
@@ -224,24 +224,33 @@ __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
 // of B's, so a 256 x 256 tile costs 32 KB of shared memory and of TMA traffic
 // per SM and K block, for twice the products of a 128 x 128 tile.
 //
+// WIDE (with CG = 2): the tile is 256 x 2 bn, both accumulators hold one half of
+// it and share A's stage.  L2 delivers about 45 bytes per clock and SM here, and
+// a 256 x 256 tile wants 64 to keep the tensor core busy; 256 x 512 wants 48.
+// The price is that a tile's epilogue no longer hides entirely: the first K
+// blocks' products go to the half that is drained first, the last ones' finish
+// that half first.
+//
 // SPLIT: one tile per cluster of S groups, each taking a range of the K
 // blocks.  The groups' fp32 partial tiles meet in shared memory: every CTA
 // adds 128 / S rows over the S partials, in the groups' order, and finishes
 // them.
-#ifndef KST
-#define KST 6
-#endif
-constexpr int kStages = KST;
-constexpr int kABytes = kTileM * kTileK * 2;
-constexpr int kStageBytes = 2 * kABytes;        // A's 128 rows and up to 128 of B
-constexpr int kRingBytes = kStages * kStageBytes;
+constexpr int kABytes = kTileM * kTileK * 2;    // also the room of 128 rows of B
+template <bool WIDE>
+struct RingShape {
+  static constexpr int kStageBytes = (WIDE ? 3 : 2) * kABytes;
+  static constexpr int kStages = WIDE ? 4 : 6;
+};
+constexpr int kRingBytes = 192 * 1024;
+constexpr int kMaxStages = 6;
 constexpr int kStageRow = 32;                    // columns an epilogue warp finishes at a time
-constexpr int kStagingBytes = kEpilogueWarps * 32 * kStageRow * 4;
-constexpr int kGemmSmem = kRingBytes + kStagingBytes + 1024;  // + alignment slack
+constexpr int kStagingBytes = kEpilogueWarps * 32 * kStageRow * 2;
+constexpr int kVectorBytes = 2 * 2 * 256 * 4;    // bias and gate of two accumulators' columns, fp32
+constexpr int kGemmSmem = kRingBytes + kStagingBytes + kVectorBytes + 1024;  // + alignment slack
 constexpr int kMaxSplitColumns = 128;            // a split tile's fp32 partial (64 KB) fits the ring
 
 struct GemmShared {
-  uint64_t full[kStages], empty[kStages];
+  uint64_t full[kMaxStages], empty[kMaxStages];
   uint64_t acc_full[2], acc_empty[2];
   uint32_t tmem;
   int abort_flag;
@@ -249,10 +258,7 @@ struct GemmShared {
 
 // (m tile, n tile) of a linear tile number: bands of kBand m tiles walked
 // down first, so that the CTAs running at one time share few rows of A and B
-#ifndef KBAND
-#define KBAND 8
-#endif
-constexpr int kBand = KBAND;
+constexpr int kBand = 8;
 __device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int& tm, int& tn) {
   const int per_band = kBand * tiles_n;
   const int band = t / per_band;
@@ -287,11 +293,12 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t base) {
 }
 
 // Position in the ring: stage and the phase of its barriers.
+template <int STAGES>
 struct RingPos {
   int s = 0;
   uint32_t phase = 0;
   __device__ __forceinline__ void step() {
-    if (++s == kStages) {
+    if (++s == STAGES) {
       s = 0;
       phase ^= 1;
     }
@@ -378,47 +385,183 @@ __device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
   return f;
 }
 
-// The epilogue of one tile by one of its 8 warps: TMEM lanes ``quarter``, every
-// other chunk of 32 columns.  A chunk leaves TMEM one row per lane and crosses
-// the warp's staging block (16-byte pieces XORed with the row, free of bank
-// conflicts both ways) to 4 lanes per row with 8 columns each, so that stores
-// and residual reads cover whole 32-byte sectors of eight rows at a time.  The
-// next chunk's TMEM load is in flight meanwhile.
-template <typename T, bool EPI>
-__device__ __forceinline__ void finish_tile(const GemmArgs& args, uint32_t tmem, uint32_t staging, long long row0,
-                                            int col0, int lane, int half) {
-  const int col_end = min(args.n, col0 + args.bn);
-  const int chunks = (args.bn + kStageRow - 1) / kStageRow;
-  const int rr = lane >> 2, cc = (lane & 3) * 8;
-  const T* gate[4];
+// act of 16 pairs
+template <int ACT>
+__device__ __forceinline__ void activate_pairs(float2 (&v)[16]) {
+  auto both = [](float x) { return make_float2(x, x); };
 #pragma unroll
-  for (int i = 0; i < 4; ++i) gate[i] = gate_row<T, EPI>(args, row0 + i * 8 + rr);
-  uint32_t acc[32];
-  if (half < chunks) tmem_ld32(tmem + half * kStageRow, acc);
-  for (int c = half; c < chunks; c += 2) {
-    const int col = col0 + c * kStageRow + cc;
-    const int count = min(8, col_end - col);
-    float res[4][8], bias[8];
-    load_bias<T, EPI>(args, col, count, bias);
+  for (int j = 0; j < 16; ++j) {
+    if constexpr (ACT == kActGelu) {
+      v[j] = make_float2(activate<ACT>(v[j].x), activate<ACT>(v[j].y));
+    } else {
+      // z / (1 + 2^w), each element by itself: a NaN stays in its column
+      float2 w;
+      if constexpr (ACT == kActGeluTanh) w = fmul2(v[j], ffma2(fmul2(v[j], v[j]), both(-kLog2e * kGelu3), both(-kLog2e * kGelu1)));
+      else w = fmul2(v[j], both(-kLog2e));
+      const float2 e = fadd2(make_float2(exp2_approx(w.x), exp2_approx(w.y)), both(1.0f));
+      v[j] = fmul2(v[j], make_float2(recip_approx(e.x), recip_approx(e.y)));
+    }
+  }
+}
+
+__device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 2, %0;" ::"n"(32 * kEpilogueWarps) : "memory"); }
+
+// One chunk of 32 x 32 results (``lane`` holds row ``lane``) to ``out`` through
+// the warp's staging block: 64-byte rows whose 16-byte pieces are XORed with the
+// row, free of bank conflicts both ways, so that stores cover whole sectors.
+__device__ __forceinline__ uint32_t staging_offset(int row, int piece) { return row * 64 + ((piece ^ ((row >> 1) & 3)) << 4); }
+
+template <typename T>
+__device__ __forceinline__ void store_chunk(const GemmArgs& args, uint32_t staging, const float2 (&v)[16], T* out,
+                                            long long stride, long long row0, int col, int col_end, int lane) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load_residual<T, EPI>(args, row0 + i * 8 + rr, col, count, res[i]);
-    tmem_ld_wait_for(acc);
+  for (int p = 0; p < 4; ++p)
+    st_shared_v4(staging + staging_offset(lane, p), pack2<T>(v[4 * p].x, v[4 * p].y), pack2<T>(v[4 * p + 1].x, v[4 * p + 1].y),
+                 pack2<T>(v[4 * p + 2].x, v[4 * p + 2].y), pack2<T>(v[4 * p + 3].x, v[4 * p + 3].y));
+  __syncwarp();
+  if (args.vec) {
+    const int piece = lane & 3;
+    if (col + piece * 8 < col_end) {
+      T* p = out + (row0 + (lane >> 2)) * stride + col + piece * 8;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      st_shared_v4(staging + lane * 128 + ((j ^ (lane & 7)) << 4), acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
-    if (c + 2 < chunks) tmem_ld32(tmem + (c + 2) * kStageRow, acc);
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = i * 8 + rr;
-      const float4 lo = ld_shared_v4(staging + r * 128 + (((cc >> 2) ^ (r & 7)) << 4));
-      const float4 hi = ld_shared_v4(staging + r * 128 + ((((cc >> 2) + 1) ^ (r & 7)) << 4));
-      if (row0 + r < args.m && count > 0) {
-        float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-        finish8<T, EPI>(args, v, row0 + r, col, count, bias, gate[i], res[i]);
+      for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 2);
+        const float4 f = ld_shared_v4(staging + staging_offset(r, piece));
+        if (row0 + r < args.m) *reinterpret_cast<float4*>(p + i * 8 * stride) = f;
       }
     }
-    __syncwarp();
+  } else if (col + lane < col_end) {
+    const int rows = static_cast<int>(min(32LL, args.m - row0));
+    for (int r = 0; r < rows; ++r) {
+      uint16_t u;
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(staging + staging_offset(r, lane >> 3) + (lane & 7) * 2) : "memory");
+      reinterpret_cast<uint16_t*>(out)[(row0 + r) * stride + col + lane] = u;
+    }
+  }
+  __syncwarp();
+}
+
+// The residual's chunk, in the layout of the results, added to them.
+template <typename T>
+__device__ __forceinline__ void fetch_residual(const GemmArgs& args, uint4 (&held)[4], long long row0, int col, int col_end,
+                                               int lane) {
+  const int piece = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const long long row = row0 + i * 8 + (lane >> 2);
+    held[i] = make_uint4(0, 0, 0, 0);
+    if (row < args.m && col + piece * 8 < col_end)
+      held[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(args.residual) + row * args.res_stride + col + piece * 8);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void add_residual(const GemmArgs& args, uint32_t staging, const uint4 (&held)[4], float2 (&v)[16],
+                                             long long row0, int col, int col_end, int lane) {
+  if (args.vec) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      st_shared_v4(staging + staging_offset(i * 8 + (lane >> 2), lane & 3), held[i].x, held[i].y, held[i].z, held[i].w);
+  } else {
+    for (int r = 0; r < 32; ++r) {
+      uint16_t u = 0;
+      if (row0 + r < args.m && col + lane < col_end)
+        u = static_cast<const uint16_t*>(args.residual)[(row0 + r) * args.res_stride + col + lane];
+      asm volatile("st.shared.u16 [%0], %1;" ::"r"(staging + staging_offset(r, lane >> 3) + (lane & 7) * 2), "h"(u) : "memory");
+    }
+  }
+  __syncwarp();
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const float4 f = ld_shared_v4(staging + staging_offset(lane, p));
+    const uint32_t w[4] = {__float_as_uint(f.x), __float_as_uint(f.y), __float_as_uint(f.z), __float_as_uint(f.w)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[4 * p + i] = fadd2(v[4 * p + i], unpack2<T>(w[i]));
+  }
+  __syncwarp();
+}
+
+// bias (0: none) and gate of an accumulator's columns into ``vectors``, where
+// the whole tile has one gate row; every epilogue thread takes one column
+template <typename T>
+__device__ __forceinline__ void stage_vectors(const GemmArgs& args, float* vectors, const T* gate, int col0, int thread) {
+  const int col = col0 + thread;
+  const bool inside = thread < args.bn && col < args.n;
+  vectors[thread] = inside && args.bias ? to_f32<T>(static_cast<const T*>(args.bias)[col]) : 0.0f;
+  vectors[256 + thread] = inside && gate ? to_f32<T>(gate[col]) : 1.0f;
+}
+
+// The epilogue of one accumulator by one of its 8 warps: TMEM lanes of its
+// quarter (a row per lane), every other chunk of 32 columns.  A chunk's results
+// are computed in pairs where they lie, rounded, and leave through the staging
+// block; the next chunk's TMEM load is in flight meanwhile.
+template <typename T, bool EPI>
+__device__ __forceinline__ void finish_chunk(const GemmArgs& args, const uint32_t (&acc)[32], uint32_t staging,
+                                             const float* vectors, const T* own_gate, long long row0, int col0, int c,
+                                             int col_end, int lane) {
+  const int col = col0 + c * kStageRow;
+  if (col >= col_end) return;  // uniform over the warp
+  float2 v[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j] = make_float2(__uint_as_float(acc[2 * j]), __uint_as_float(acc[2 * j + 1]));
+  if constexpr (EPI) {
+    uint4 held[4];
+    if (args.residual && args.vec) fetch_residual<T>(args, held, row0, col, col_end, lane);
+    if (args.bias) {
+      const float4* b = reinterpret_cast<const float4*>(vectors + c * kStageRow);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float4 f = b[j];
+        v[2 * j] = fadd2(v[2 * j], make_float2(f.x, f.y));
+        v[2 * j + 1] = fadd2(v[2 * j + 1], make_float2(f.z, f.w));
+      }
+    }
+    if (args.preact) store_chunk<T>(args, staging, v, static_cast<T*>(args.preact), args.n, row0, col, col_end, lane);
+    switch (args.act) {
+      case kActGeluTanh: activate_pairs<kActGeluTanh>(v); break;
+      case kActGelu: activate_pairs<kActGelu>(v); break;
+      case kActSilu: activate_pairs<kActSilu>(v); break;
+      default: break;
+    }
+    if (own_gate) {  // rows of several samples: each lane reads its own row's gate
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        float g[8];
+        const int count = min(8, col_end - col - 8 * p);
+        if (count <= 0) continue;
+        load_vec<8>(own_gate + col + 8 * p, args.vec, count, g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[4 * p + i] = fmul2(v[4 * p + i], make_float2(g[2 * i], g[2 * i + 1]));
+      }
+    } else if (args.gate) {
+      const float4* g = reinterpret_cast<const float4*>(vectors + 256 + c * kStageRow);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float4 f = g[j];
+        v[2 * j] = fmul2(v[2 * j], make_float2(f.x, f.y));
+        v[2 * j + 1] = fmul2(v[2 * j + 1], make_float2(f.z, f.w));
+      }
+    }
+    if (args.residual) add_residual<T>(args, staging, held, v, row0, col, col_end, lane);
+  }
+  store_chunk<T>(args, staging, v, static_cast<T*>(args.out), args.out_stride, row0, col, col_end, lane);
+}
+
+template <typename T, bool EPI>
+__device__ __forceinline__ void finish_tile(const GemmArgs& args, uint32_t tmem, uint32_t staging, const float* vectors,
+                                            const T* own_gate, long long row0, int col0, int lane, int half) {
+  const int col_end = min(args.n, col0 + args.bn);
+  const int chunks = args.bn / kStageRow;
+  uint32_t acc0[32], acc1[32];
+  if (half < chunks) tmem_ld32(tmem + half * kStageRow, acc0);
+  for (int c = half; c < chunks; c += 4) {
+    tmem_ld_wait_for(acc0);
+    if (c + 2 < chunks) tmem_ld32(tmem + (c + 2) * kStageRow, acc1);
+    finish_chunk<T, EPI>(args, acc0, staging, vectors, own_gate, row0, col0, c, col_end, lane);
+    if (c + 2 < chunks) {
+      tmem_ld_wait_for(acc1);
+      if (c + 4 < chunks) tmem_ld32(tmem + (c + 4) * kStageRow, acc0);
+      finish_chunk<T, EPI>(args, acc1, staging, vectors, own_gate, row0, col0, c + 2, col_end, lane);
+    }
   }
 }
 
@@ -427,7 +570,7 @@ __device__ __forceinline__ uint32_t partial_offset(int row, int c, int bn) {
   return static_cast<uint32_t>(row * bn * 4 + (((c & ~7) | ((c ^ row) & 7)) << 4));
 }
 
-template <typename T, int CG, bool SPLIT, bool AMN, bool BMN, bool EPI>
+template <typename T, int CG, bool SPLIT, bool WIDE, bool AMN, bool BMN, bool EPI>
 __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmArgs args, int splits) {
   extern __shared__ unsigned char smem_raw[];
   __shared__ GemmShared sh;
@@ -437,6 +580,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
   const uint32_t rank = CG == 1 ? 0 : cta & 1, lead = cta - rank;  // within the pair; the pair's first CTA
   volatile int* abort_flag = &sh.abort_flag;
   constexpr uint32_t kAccumulator = CG == 1 ? 128 : 256;  // columns between the two accumulators
+  constexpr int kStages = RingShape<WIDE>::kStages, kStageBytes = RingShape<WIDE>::kStageBytes;
+  constexpr int kHalves = WIDE ? 2 : 1;  // accumulators per tile
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&sh.full[s], 1);
@@ -469,13 +614,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     if (lane == 0) {
       const bool is_a = warp == 0;
       bool ok = true;
-      RingPos pos;
+      RingPos<kStages> pos;
       // the pair's stages fill one barrier, the first CTA's, which expects both CTAs' bytes
       const uint32_t bar0 = CG > 1 ? map_rank(smem_u32(&sh.full[0]), lead) : smem_u32(&sh.full[0]);
       for (int t = group; t < tiles && ok; t += groups) {
         int tm, tn;
         tile_coords(t, args.tiles_m, args.tiles_n, tm, tn);
-        const int row0 = is_a ? (tm * CG + rank) * kTileM : tn * args.bn + rank * (args.bn / CG);
+        const int row0 = is_a ? (tm * CG + rank) * kTileM : tn * kHalves * args.bn + rank * (args.bn / CG);
         for (int kb = kb_begin; kb < kb_end; ++kb) {
           ok = mbar_wait(&sh.empty[pos.s], pos.phase ^ 1, abort_flag, args.status);
           if (!ok) break;
@@ -486,7 +631,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             if (rank == 0) mbar_arrive_expect_tx(&sh.full[pos.s], CG * args.stage_tx);
             load_tile<CG, AMN>(st, &args.a[seg], row0, args.a_panels, args.a_joined, k0, bar);
           } else {
-            load_tile<CG, BMN>(st + kABytes, &args.b[seg], row0, args.b_panels, args.b_joined, k0, bar);
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h)
+              load_tile<CG, BMN>(st + (1 + h) * kABytes, &args.b[seg], row0 + h * args.bn, args.b_panels, args.b_joined, k0, bar);
           }
           pos.step();
         }
@@ -505,62 +652,125 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
       const uint32_t idesc = instr_desc(kTileM * CG, args.bn, ab, AMN, BMN);
       const uint64_t desc_a = tile_desc<AMN>(ring), desc_b = tile_desc<BMN>(ring + kABytes);
       bool ok = true;
-      RingPos pos;
+      RingPos<kStages> pos;
       uint32_t local = 0;
+      // one K block's products for one accumulator; the first of a tile overwrite it
+      auto products = [&](int s, int half, uint32_t acc, bool first) {
+        const uint32_t at = s * (kStageBytes >> 4), at_b = at + half * (kABytes >> 4);
+        uint32_t accumulate = first ? 0 : 1;
+#pragma unroll
+        for (int k = 0; k < kTileK / 16; ++k) {
+          product_step<CG>(acc, desc_a + (at + step_offset<AMN>(k)), desc_b + (at_b + step_offset<BMN>(k)), idesc, accumulate);
+          accumulate = 1;
+        }
+      };
       for (int t = group; t < tiles && ok; t += groups, ++local) {
-        const int b = local & 1;
-        ok = mbar_wait(&sh.acc_empty[b], ((local >> 1) & 1) ^ 1, abort_flag, args.status);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t acc = tmem + b * kAccumulator;
-        uint32_t accumulate = 0;
-        for (int kb = kb_begin; kb < kb_end; ++kb) {
-          ok = mbar_wait(&sh.full[pos.s], pos.phase, abort_flag, args.status);
+        if constexpr (!WIDE) {
+          const int b = local & 1;
+          ok = mbar_wait(&sh.acc_empty[b], ((local >> 1) & 1) ^ 1, abort_flag, args.status);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t at = pos.s * (kStageBytes >> 4);
-#pragma unroll
-          for (int k = 0; k < kTileK / 16; ++k) {
-            product_step<CG>(acc, desc_a + (at + step_offset<AMN>(k)), desc_b + (at + step_offset<BMN>(k)), idesc, accumulate);
-            accumulate = 1;
+          for (int kb = kb_begin; kb < kb_end; ++kb) {
+            ok = mbar_wait(&sh.full[pos.s], pos.phase, abort_flag, args.status);
+            if (!ok) break;
+            tc_fence_after();
+            products(pos.s, 0, tmem + b * kAccumulator, kb == kb_begin);
+            product_commit<CG>(&sh.empty[pos.s], lead);
+            pos.step();
           }
-          product_commit<CG>(&sh.empty[pos.s], lead);
-          pos.step();
+          if (ok) product_commit<CG>(&sh.acc_full[b], lead);
+        } else {
+          // K blocks in order for each half; the second half trails the first by
+          // up to a ring of stages at the tile's start and at its end
+          const uint32_t free_phase = (local & 1) ^ 1;
+          const int skew = min(kStages, kblocks), last = max(skew, kblocks - kStages);
+          ok = mbar_wait(&sh.acc_empty[0], free_phase, abort_flag, args.status);
+          if (!ok) break;
+          tc_fence_after();
+          RingPos<kStages> ahead = pos;
+          auto first_half = [&](int kb) {
+            ok = mbar_wait(&sh.full[ahead.s], ahead.phase, abort_flag, args.status);
+            if (!ok) return;
+            tc_fence_after();
+            products(ahead.s, 0, tmem, kb == 0);
+            ahead.step();
+          };
+          auto second_half = [&](int kb) {
+            products(pos.s, 1, tmem + kAccumulator, kb == 0);
+            product_commit<CG>(&sh.empty[pos.s], lead);
+            pos.step();
+          };
+          for (int kb = 0; kb < skew && ok; ++kb) first_half(kb);
+          if (!ok) break;
+          if (skew == kblocks) product_commit<CG>(&sh.acc_full[0], lead);
+          ok = mbar_wait(&sh.acc_empty[1], free_phase, abort_flag, args.status);
+          if (!ok) break;
+          tc_fence_after();
+          for (int kb = 0; kb < skew; ++kb) second_half(kb);
+          for (int kb = skew; kb < last && ok; ++kb) {
+            first_half(kb);
+            if (ok) second_half(kb);
+          }
+          if (!ok) break;
+          if (last < kblocks) {
+            for (int kb = last; kb < kblocks && ok; ++kb) first_half(kb);
+            if (!ok) break;
+            product_commit<CG>(&sh.acc_full[0], lead);
+            for (int kb = last; kb < kblocks; ++kb) second_half(kb);
+          }
+          product_commit<CG>(&sh.acc_full[1], lead);
         }
-        if (ok) product_commit<CG>(&sh.acc_full[b], lead);
       }
     }
   } else {
     // ----------------------------------------------------------- epilogue
     const int quarter = warp & 3, half = (warp - 2) >> 2;  // the TMEM lanes this warp may read; its column chunks
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    uint32_t local = 0;
-    for (int t = group; t < tiles; t += groups, ++local) {
+    const int thread = threadIdx.x - 64;
+    float* vectors = reinterpret_cast<float*>(smem_raw + (ring - smem_u32(smem_raw)) + kRingBytes + kStagingBytes);
+    uint32_t turn = 0;  // accumulators finished
+    for (int t = group; t < tiles; t += groups) {
       int tm, tn;
       tile_coords(t, args.tiles_m, args.tiles_n, tm, tn);
-      const int b = local & 1;
-      if (!mbar_wait_warp(&sh.acc_full[b], (local >> 1) & 1, abort_flag, args.status)) break;
-      tc_fence_after();
-      if constexpr (SPLIT) {
-        // the partial tile, one row per lane, into the drained ring
-        const int row = quarter * 32 + lane;
-        for (int c = half * 32; c < args.bn; c += 64) {
-          uint32_t acc[32];
-          tmem_ld32_sync(tmem + lanes + c, acc);
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            st_shared_v4(ring + partial_offset(row, (c >> 2) + j, args.bn), acc[4 * j], acc[4 * j + 1], acc[4 * j + 2],
-                         acc[4 * j + 3]);
+      const long long tile_row = static_cast<long long>(tm * CG + static_cast<int>(rank)) * kTileM;
+      const long long row0 = tile_row + quarter * 32;
+      // one gate row for all of the CTA's rows, or each row's own
+      const T* gate = gate_row<T, EPI>(args, tile_row);
+      const T* own_gate = nullptr;
+      if (gate && gate != gate_row<T, EPI>(args, min(tile_row + kTileM, static_cast<long long>(args.m)) - 1))
+        own_gate = gate_row<T, EPI>(args, min(row0 + lane, static_cast<long long>(args.m) - 1));
+#pragma unroll 1
+      for (int h = 0; h < kHalves; ++h, ++turn) {
+        const int b = turn & 1;
+        const int col0 = (tn * kHalves + h) * args.bn;
+        float* vec = vectors + b * 512;
+        if (EPI && !SPLIT && (args.bias || gate)) {
+          stage_vectors<T>(args, vec, gate, col0, thread);
+          epilogue_barrier();
         }
-      } else {
-        const long long row0 = static_cast<long long>(tm * CG + static_cast<int>(rank)) * kTileM + quarter * 32;
-        finish_tile<T, EPI>(args, tmem + b * kAccumulator + lanes, ring + kRingBytes + (warp - 2) * 4096, row0,
-                            tn * args.bn, lane, half);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if (CG == 1) mbar_arrive(&sh.acc_empty[b]);
-          else arrive_cluster(map_rank(smem_u32(&sh.acc_empty[b]), lead));
+        // after an expired wait the warp still meets the others at the barriers above
+        if (!mbar_wait_warp(&sh.acc_full[b], (turn >> 1) & 1, abort_flag, args.status)) continue;
+        tc_fence_after();
+        if constexpr (SPLIT) {
+          // the partial tile, one row per lane, into the drained ring
+          const int row = quarter * 32 + lane;
+          for (int c = half * 32; c < args.bn; c += 64) {
+            uint32_t acc[32];
+            tmem_ld32_sync(tmem + lanes + c, acc);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              st_shared_v4(ring + partial_offset(row, (c >> 2) + j, args.bn), acc[4 * j], acc[4 * j + 1], acc[4 * j + 2],
+                           acc[4 * j + 3]);
+          }
+        } else {
+          finish_tile<T, EPI>(args, tmem + b * kAccumulator + lanes, ring + kRingBytes + (warp - 2) * 2048, vec, own_gate,
+                              row0, col0, lane, half);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (CG == 1) mbar_arrive(&sh.acc_empty[b]);
+            else arrive_cluster(map_rank(smem_u32(&sh.acc_empty[b]), lead));
+          }
         }
       }
     }
@@ -835,43 +1045,51 @@ cudaError_t grant_smem(const void* kernel, int bytes, std::atomic<unsigned long 
   return e;
 }
 
-// How a product is cut: CTAs per group, columns per tile, K splits.
+// How a product is cut: CTAs per group, columns per accumulator, accumulators
+// per tile, K splits.
 struct TileChoice {
-  int cg, bn, splits;
+  int cg, bn, halves, splits;
 };
 
-// Estimated clocks of a choice, from what one SM does per 64-wide K block: 2 bn
-// clocks of MMA (128 bn CG x 16 products take bn / 2 clocks per CTA), or the
-// operand bytes at about 64 a clock, whichever is longer; plus a start and a
-// finish per tile and the meeting of a split's partials.
+// Estimated clocks of a choice, from what one SM does per 64-wide K block: 2
+// clocks of MMA per column of its tile (128 rows x 16 take half a clock a
+// column), or its operand rows' 128 bytes at the 45 bytes a clock that L2 was
+// measured to deliver, whichever is longer; plus what a tile adds: little where
+// the epilogue hides under the next tile, about 4000 clocks where it does not
+// (wide), a meeting of partials (split).
 TileChoice choose_tiles(int m, int n, int kblocks, bool amn) {
-  TileChoice best{1, 128, 1};
+  TileChoice best{1, 128, 1, 1};
   double least = 1e300;
   const int cg = m > kTileM ? 2 : 1;
   const int a_rows = amn ? (m > 64 ? 128 : 64) : (m < kTileM ? (m + 7) / 8 * 8 : kTileM);
   const long long tiles_m = (m + kTileM * cg - 1) / (kTileM * cg);
+  auto consider = [&](int bn, int halves, int splits) {
+    const int cols = bn * halves;
+    const long long tiles = tiles_m * ((n + cols - 1) / cols);
+    const long long waves = (tiles * splits * cg + kNumSMs - 1) / kNumSMs;
+    if (splits > 1 && waves > 1) return;
+    const double mma = 2.0 * cols, load = 128.0 / 45.0 * (a_rows + cols / cg);
+    const double cost = waves * (static_cast<double>(kblocks) / splits * (mma > load ? mma : load) +
+                                 (halves > 1 ? 16.0 * bn : 200.0)) +
+                        (splits > 1 ? 2500.0 : 6.0 * cols);
+    if (cost < least) {
+      least = cost;
+      best = TileChoice{cg, bn, halves, splits};
+    }
+  };
   for (int splits = 1; splits * cg <= 8; splits *= 2) {
     if (splits > 1 && kblocks < 4 * splits) break;
     const int most = splits > 1 || cg == 1 ? kMaxSplitColumns : 256;
-    for (int bn = 32 * cg; bn <= most; bn += 32) {
-      const long long tiles = tiles_m * ((n + bn - 1) / bn);
-      const long long waves = (tiles * splits * cg + kNumSMs - 1) / kNumSMs;
-      if (splits > 1 && waves > 1) continue;
-      const double mma = 2.0 * bn, load = 2.0 * (a_rows + bn / cg);
-      const double cost = waves * (static_cast<double>(kblocks) / splits * (mma > load ? mma : load) + 200.0) +
-                          (splits > 1 ? 2500.0 : 6.0 * bn);
-      if (cost < least) {
-        least = cost;
-        best = TileChoice{cg, bn, splits};
-      }
-    }
+    for (int bn = 32 * cg; bn <= most; bn += 32) consider(bn, 1, splits);
   }
+  if (cg == 2)
+    for (int bn = 160; bn <= 256; bn += 32) consider(bn, 2, 1);
   return best;
 }
 
-template <typename T, int CG, bool SPLIT, bool AMN, bool BMN, bool EPI>
+template <typename T, int CG, bool SPLIT, bool WIDE, bool AMN, bool BMN, bool EPI>
 int launch_tiles(const GemmArgs& g, int splits, cudaStream_t stream) {
-  auto kernel = gemm_kernel<T, CG, SPLIT, AMN, BMN, EPI>;
+  auto kernel = gemm_kernel<T, CG, SPLIT, WIDE, AMN, BMN, EPI>;
   static std::atomic<unsigned long long> opened{0};  // devices whose kernel has its shared memory granted
   cudaError_t e = grant_smem(reinterpret_cast<const void*>(kernel), kGemmSmem, opened);
   if (e != cudaSuccess) return static_cast<int>(e);
@@ -902,14 +1120,14 @@ int launch_gemm(GemmArgs& g, const Operand* a, const Operand* b, int segments, i
   const TileChoice c = choose_tiles(g.m, g.n, kblocks, AMN);
   g.bn = c.bn;
   g.tiles_m = (g.m + c.cg * kTileM - 1) / (c.cg * kTileM);
-  g.tiles_n = (g.n + c.bn - 1) / c.bn;
+  g.tiles_n = (g.n + c.bn * c.halves - 1) / (c.bn * c.halves);
   if (static_cast<long long>(g.tiles_m) * g.tiles_n > 0x0fffffffLL) return kErrUnsupported;
   // rows (or panels) of the operands one CTA stages per K block; a single tile
   // of few rows loads only those, the others' results are never stored
   const int a_rows = g.m < kTileM ? (g.m + 7) / 8 * 8 : kTileM, b_rows = c.bn / c.cg;
   g.a_panels = g.m > 64 ? 2 : 1;
   g.b_panels = (b_rows + 63) / 64;
-  g.stage_tx = (AMN ? g.a_panels * 8192 : a_rows * 128) + (BMN ? g.b_panels * 8192 : b_rows * 128);
+  g.stage_tx = (AMN ? g.a_panels * 8192 : a_rows * 128) + c.halves * (BMN ? g.b_panels * 8192 : b_rows * 128);
   // a joined copy starts on a whole panel
   g.a_joined = AMN && g.m % 64 == 0;
   g.b_joined = BMN && g.n % 64 == 0 && b_rows % 64 == 0;
@@ -919,10 +1137,11 @@ int launch_gemm(GemmArgs& g, const Operand* a, const Operand* b, int segments, i
       return kErrTensorMap;
   g.status = device_status_ptr();
   if (c.splits > 1)
-    return c.cg == 2 ? launch_tiles<T, 2, true, AMN, BMN, EPI>(g, c.splits, stream)
-                     : launch_tiles<T, 1, true, AMN, BMN, EPI>(g, c.splits, stream);
-  return c.cg == 2 ? launch_tiles<T, 2, false, AMN, BMN, EPI>(g, 1, stream)
-                   : launch_tiles<T, 1, false, AMN, BMN, EPI>(g, 1, stream);
+    return c.cg == 2 ? launch_tiles<T, 2, true, false, AMN, BMN, EPI>(g, c.splits, stream)
+                     : launch_tiles<T, 1, true, false, AMN, BMN, EPI>(g, c.splits, stream);
+  if (c.halves > 1) return launch_tiles<T, 2, false, true, AMN, BMN, EPI>(g, 1, stream);
+  return c.cg == 2 ? launch_tiles<T, 2, false, false, AMN, BMN, EPI>(g, 1, stream)
+                   : launch_tiles<T, 1, false, false, AMN, BMN, EPI>(g, 1, stream);
 }
 
 bool aligned16(const void* p, long long stride) {
