@@ -64,13 +64,33 @@ constexpr float kGelu3 = kGelu1 * 0.044715f;
 
 __device__ __forceinline__ float recip_approx(float x) { return __fdividef(1.0f, x); }
 
+// z Phi(z) of a pair.  With x = |z| / sqrt 2 and t = 1 / (1 + p x), erfc(x) is a
+// polynomial in t times exp(-x^2) (Abramowitz and Stegun, Handbook of
+// Mathematical Functions, 7.1.26, within 1.5e-7); it keeps its relative
+// precision in the negative tail, where 1 + erf would cancel.
+__device__ __forceinline__ float2 gelu_pair(float2 z) {
+  auto both = [](float x) { return make_float2(x, x); };
+  const float2 x = make_float2(fabsf(z.x) * 0.7071067811865476f, fabsf(z.y) * 0.7071067811865476f);
+  const float2 d = ffma2(x, both(0.3275911f), both(1.0f));
+  const float2 t = make_float2(recip_approx(d.x), recip_approx(d.y));
+  float2 poly = ffma2(t, both(1.061405429f), both(-1.453152027f));
+  poly = ffma2(t, poly, both(1.421413741f));
+  poly = ffma2(t, poly, both(-0.284496736f));
+  poly = ffma2(t, poly, both(0.254829592f));
+  const float2 w = fmul2(fmul2(x, x), both(-kLog2e));
+  // half of erfc(|z| / sqrt 2), and its complement for positive z
+  const float2 half = fmul2(fmul2(poly, t), make_float2(0.5f * exp2_approx(w.x), 0.5f * exp2_approx(w.y)));
+  const float2 p = make_float2(z.x > 0.0f ? 1.0f - half.x : half.x, z.y > 0.0f ? 1.0f - half.y : half.y);
+  return fmul2(z, p);
+}
+
 template <int ACT>
 __device__ __forceinline__ float activate(float z) {
   if constexpr (ACT == kActGeluTanh) {
     const float w = z * fmaf(-kLog2e * kGelu3, z * z, -kLog2e * kGelu1);
     return z * recip_approx(1.0f + exp2_approx(w));
   } else if constexpr (ACT == kActGelu) {
-    return 0.5f * z * (1.0f + erff(z * 0.7071067811865476f));
+    return gelu_pair(make_float2(z, z)).x;
   } else if constexpr (ACT == kActSilu) {
     return z * recip_approx(1.0f + exp2_approx(-kLog2e * z));
   } else {
@@ -131,8 +151,11 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
+// Arrive on a barrier of another CTA of the cluster.  What it orders is the TMEM
+// reads before it (waited for, with the tcgen05 fence); a release at cluster
+// scope would also wait for all the warp's global stores.
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 template <int CG>
@@ -392,7 +415,7 @@ __device__ __forceinline__ void activate_pairs(float2 (&v)[16]) {
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     if constexpr (ACT == kActGelu) {
-      v[j] = make_float2(activate<ACT>(v[j].x), activate<ACT>(v[j].y));
+      v[j] = gelu_pair(v[j]);
     } else {
       // z / (1 + 2^w), each element by itself: a NaN stays in its column
       float2 w;
@@ -432,6 +455,7 @@ __device__ __forceinline__ void store_chunk(const GemmArgs& args, uint32_t stagi
     }
   } else if (col + lane < col_end) {
     const int rows = static_cast<int>(min(32LL, args.m - row0));
+#pragma unroll 1
     for (int r = 0; r < rows; ++r) {
       uint16_t u;
       asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(staging + staging_offset(r, lane >> 3) + (lane & 7) * 2) : "memory");
@@ -462,6 +486,7 @@ __device__ __forceinline__ void add_residual(const GemmArgs& args, uint32_t stag
     for (int i = 0; i < 4; ++i)
       st_shared_v4(staging + staging_offset(i * 8 + (lane >> 2), lane & 3), held[i].x, held[i].y, held[i].z, held[i].w);
   } else {
+#pragma unroll 1
     for (int r = 0; r < 32; ++r) {
       uint16_t u = 0;
       if (row0 + r < args.m && col + lane < col_end)
@@ -495,14 +520,11 @@ __device__ __forceinline__ void stage_vectors(const GemmArgs& args, float* vecto
 // are computed in pairs where they lie, rounded, and leave through the staging
 // block; the next chunk's TMEM load is in flight meanwhile.
 template <typename T, bool EPI>
-__device__ __forceinline__ void finish_chunk(const GemmArgs& args, const uint32_t (&acc)[32], uint32_t staging,
+__device__ __forceinline__ void finish_chunk(const GemmArgs& args, float2 (&v)[16], uint32_t staging,
                                              const float* vectors, const T* own_gate, long long row0, int col0, int c,
                                              int col_end, int lane) {
   const int col = col0 + c * kStageRow;
   if (col >= col_end) return;  // uniform over the warp
-  float2 v[16];
-#pragma unroll
-  for (int j = 0; j < 16; ++j) v[j] = make_float2(__uint_as_float(acc[2 * j]), __uint_as_float(acc[2 * j + 1]));
   if constexpr (EPI) {
     uint4 held[4];
     if (args.residual && args.vec) fetch_residual<T>(args, held, row0, col, col_end, lane);
@@ -551,17 +573,16 @@ __device__ __forceinline__ void finish_tile(const GemmArgs& args, uint32_t tmem,
                                             const T* own_gate, long long row0, int col0, int lane, int half) {
   const int col_end = min(args.n, col0 + args.bn);
   const int chunks = args.bn / kStageRow;
-  uint32_t acc0[32], acc1[32];
-  if (half < chunks) tmem_ld32(tmem + half * kStageRow, acc0);
-  for (int c = half; c < chunks; c += 4) {
-    tmem_ld_wait_for(acc0);
-    if (c + 2 < chunks) tmem_ld32(tmem + (c + 2) * kStageRow, acc1);
-    finish_chunk<T, EPI>(args, acc0, staging, vectors, own_gate, row0, col0, c, col_end, lane);
-    if (c + 2 < chunks) {
-      tmem_ld_wait_for(acc1);
-      if (c + 4 < chunks) tmem_ld32(tmem + (c + 4) * kStageRow, acc0);
-      finish_chunk<T, EPI>(args, acc1, staging, vectors, own_gate, row0, col0, c + 2, col_end, lane);
-    }
+  uint32_t acc[32];
+  if (half < chunks) tmem_ld32(tmem + half * kStageRow, acc);
+#pragma unroll 1
+  for (int c = half; c < chunks; c += 2) {
+    tmem_ld_wait_for(acc);
+    float2 v[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = make_float2(__uint_as_float(acc[2 * j]), __uint_as_float(acc[2 * j + 1]));
+    if (c + 2 < chunks) tmem_ld32(tmem + (c + 2) * kStageRow, acc);
+    finish_chunk<T, EPI>(args, v, staging, vectors, own_gate, row0, col0, c, col_end, lane);
   }
 }
 
