@@ -203,6 +203,18 @@ __device__ __forceinline__ void product_step(uint32_t d, uint64_t a, uint64_t b,
   }
 }
 
+// Two products of a pair with one A operand, into two accumulators: the second
+// takes A from the collector that the first filled, not from shared memory again.
+__device__ __forceinline__ void product_step_twice(uint32_t d0, uint32_t d1, uint64_t a, uint64_t b0, uint64_t b1,
+                                                   uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16.collector::a::fill [%0], %2, %3, %5, p;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16.collector::a::lastuse [%1], %2, %4, %5, p;\n\t}" ::"r"(d0),
+      "r"(d1), "l"(a), "l"(b0), "l"(b1), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // Arrive on ``bar`` (of both CTAs of a pair, whose first has rank ``lead``) once
 // the products issued so far are done.
 template <int CG>
@@ -728,10 +740,20 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
           if (!ok) break;
           tc_fence_after();
           for (int kb = 0; kb < skew; ++kb) second_half(kb);
-          for (int kb = skew; kb < last && ok; ++kb) {
-            first_half(kb);
-            if (ok) second_half(kb);
+          for (int kb = skew; kb < last; ++kb) {
+            ok = mbar_wait(&sh.full[pos.s], pos.phase, abort_flag, args.status);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t at = pos.s * (kStageBytes >> 4);
+#pragma unroll
+            for (int k = 0; k < kTileK / 16; ++k) {
+              const uint64_t b0 = desc_b + (at + step_offset<BMN>(k));
+              product_step_twice(tmem, tmem + kAccumulator, desc_a + (at + step_offset<AMN>(k)), b0, b0 + (kABytes >> 4), idesc, 1);
+            }
+            product_commit<CG>(&sh.empty[pos.s], lead);
+            pos.step();
           }
+          ahead = pos;
           if (!ok) break;
           if (last < kblocks) {
             for (int kb = last; kb < kblocks && ok; ++kb) first_half(kb);
