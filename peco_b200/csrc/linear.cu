@@ -38,7 +38,9 @@ struct GemmArgs {
   int bn;                    // columns of a tile, a multiple of 32
   int a_panels, b_panels;    // 64-wide panels of an MN-major operand per CTA
   int a_joined, b_joined;    // ... all of them in one copy (the operand's width is a multiple of 64)
-  uint32_t stage_tx;         // bytes one CTA loads per K block
+  int stages;                // of the ring in shared memory
+  uint32_t a_bytes, b_bytes; // one operand tile in a stage; B's once per accumulator
+  uint32_t stage_bytes;      // what one CTA loads per K block, and a stage's size
   void* out;
   long long out_stride;
   // epilogue operands (null where absent)
@@ -270,14 +272,8 @@ __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
 // blocks.  The groups' fp32 partial tiles meet in shared memory: every CTA
 // adds 128 / S rows over the S partials, in the groups' order, and finishes
 // them.
-constexpr int kABytes = kTileM * kTileK * 2;    // also the room of 128 rows of B
-template <bool WIDE>
-struct RingShape {
-  static constexpr int kStageBytes = (WIDE ? 3 : 2) * kABytes;
-  static constexpr int kStages = WIDE ? 4 : 6;
-};
 constexpr int kRingBytes = 192 * 1024;
-constexpr int kMaxStages = 6;
+constexpr int kMaxStages = 24;                  // stages hold what a tile needs: small ones have many in flight
 constexpr int kStageRow = 32;                    // columns an epilogue warp finishes at a time
 constexpr int kStagingBytes = kEpilogueWarps * 32 * kStageRow * 2;
 constexpr int kVectorBytes = 2 * 2 * 256 * 4;    // bias and gate of two accumulators' columns, fp32
@@ -328,12 +324,11 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t base) {
 }
 
 // Position in the ring: stage and the phase of its barriers.
-template <int STAGES>
 struct RingPos {
-  int s = 0;
-  uint32_t phase = 0;
-  __device__ __forceinline__ void step() {
-    if (++s == STAGES) {
+  int s;
+  uint32_t phase;
+  __device__ __forceinline__ void step(int stages) {
+    if (++s == stages) {
       s = 0;
       phase ^= 1;
     }
@@ -613,10 +608,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
   const uint32_t rank = CG == 1 ? 0 : cta & 1, lead = cta - rank;  // within the pair; the pair's first CTA
   volatile int* abort_flag = &sh.abort_flag;
   constexpr uint32_t kAccumulator = CG == 1 ? 128 : 256;  // columns between the two accumulators
-  constexpr int kStages = RingShape<WIDE>::kStages, kStageBytes = RingShape<WIDE>::kStageBytes;
+  const int stages = args.stages;
   constexpr int kHalves = WIDE ? 2 : 1;  // accumulators per tile
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+  if (lane == 0 && (warp == 0 || warp == kEpilogueWarps + 2)) {
+    prefetch_tensormap(warp == 0 ? &args.a[0] : &args.b[0]);
+    if (args.kblocks[1]) prefetch_tensormap(warp == 0 ? &args.a[1] : &args.b[1]);
+  }
+  if (threadIdx.x == 64) {
+    for (int s = 0; s < stages; ++s) {
       mbar_init(&sh.full[s], 1);
       mbar_init(&sh.empty[s], 1);
     }
@@ -647,7 +646,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     if (lane == 0) {
       const bool is_a = warp == 0;
       bool ok = true;
-      RingPos<kStages> pos;
+      RingPos pos{0, 0};
       // the pair's stages fill one barrier, the first CTA's, which expects both CTAs' bytes
       const uint32_t bar0 = CG > 1 ? map_rank(smem_u32(&sh.full[0]), lead) : smem_u32(&sh.full[0]);
       for (int t = group; t < tiles && ok; t += groups) {
@@ -657,18 +656,18 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         for (int kb = kb_begin; kb < kb_end; ++kb) {
           ok = mbar_wait(&sh.empty[pos.s], pos.phase ^ 1, abort_flag, args.status);
           if (!ok) break;
-          const uint32_t st = ring + pos.s * kStageBytes, bar = bar0 + pos.s * 8;
+          const uint32_t st = ring + pos.s * args.stage_bytes, bar = bar0 + pos.s * 8;
           const int seg = kb >= kb0 ? 1 : 0;
           const int k0 = (kb - (seg ? kb0 : 0)) * kTileK;
           if (is_a) {
-            if (rank == 0) mbar_arrive_expect_tx(&sh.full[pos.s], CG * args.stage_tx);
+            if (rank == 0) mbar_arrive_expect_tx(&sh.full[pos.s], CG * args.stage_bytes);
             load_tile<CG, AMN>(st, &args.a[seg], row0, args.a_panels, args.a_joined, k0, bar);
           } else {
 #pragma unroll
             for (int h = 0; h < kHalves; ++h)
-              load_tile<CG, BMN>(st + (1 + h) * kABytes, &args.b[seg], row0 + h * args.bn, args.b_panels, args.b_joined, k0, bar);
+              load_tile<CG, BMN>(st + args.a_bytes + h * args.b_bytes, &args.b[seg], row0 + h * args.bn, args.b_panels, args.b_joined, k0, bar);
           }
-          pos.step();
+          pos.step(stages);
         }
       }
       // after an expired wait: time for the copies still in flight to land before the CTA ends
@@ -683,13 +682,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     if (lane == 0 && rank == 0) {
       constexpr int ab = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
       const uint32_t idesc = instr_desc(kTileM * CG, args.bn, ab, AMN, BMN);
-      const uint64_t desc_a = tile_desc<AMN>(ring), desc_b = tile_desc<BMN>(ring + kABytes);
+      const uint64_t desc_a = tile_desc<AMN>(ring), desc_b = tile_desc<BMN>(ring + args.a_bytes);
+      const uint32_t stage_step = args.stage_bytes >> 4, half_step = args.b_bytes >> 4;
       bool ok = true;
-      RingPos<kStages> pos;
+      RingPos pos{0, 0};
       uint32_t local = 0;
       // one K block's products for one accumulator; the first of a tile overwrite it
       auto products = [&](int s, int half, uint32_t acc, bool first) {
-        const uint32_t at = s * (kStageBytes >> 4), at_b = at + half * (kABytes >> 4);
+        const uint32_t at = s * stage_step, at_b = at + half * half_step;
         uint32_t accumulate = first ? 0 : 1;
 #pragma unroll
         for (int k = 0; k < kTileK / 16; ++k) {
@@ -709,29 +709,29 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             tc_fence_after();
             products(pos.s, 0, tmem + b * kAccumulator, kb == kb_begin);
             product_commit<CG>(&sh.empty[pos.s], lead);
-            pos.step();
+            pos.step(stages);
           }
           if (ok) product_commit<CG>(&sh.acc_full[b], lead);
         } else {
           // K blocks in order for each half; the second half trails the first by
           // up to a ring of stages at the tile's start and at its end
           const uint32_t free_phase = (local & 1) ^ 1;
-          const int skew = min(kStages, kblocks), last = max(skew, kblocks - kStages);
+          const int skew = min(stages, kblocks), last = max(skew, kblocks - stages);
           ok = mbar_wait(&sh.acc_empty[0], free_phase, abort_flag, args.status);
           if (!ok) break;
           tc_fence_after();
-          RingPos<kStages> ahead = pos;
+          RingPos ahead = pos;
           auto first_half = [&](int kb) {
             ok = mbar_wait(&sh.full[ahead.s], ahead.phase, abort_flag, args.status);
             if (!ok) return;
             tc_fence_after();
             products(ahead.s, 0, tmem, kb == 0);
-            ahead.step();
+            ahead.step(stages);
           };
           auto second_half = [&](int kb) {
             products(pos.s, 1, tmem + kAccumulator, kb == 0);
             product_commit<CG>(&sh.empty[pos.s], lead);
-            pos.step();
+            pos.step(stages);
           };
           for (int kb = 0; kb < skew && ok; ++kb) first_half(kb);
           if (!ok) break;
@@ -744,14 +744,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             ok = mbar_wait(&sh.full[pos.s], pos.phase, abort_flag, args.status);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t at = pos.s * (kStageBytes >> 4);
+            const uint32_t at = pos.s * stage_step;
 #pragma unroll
             for (int k = 0; k < kTileK / 16; ++k) {
               const uint64_t b0 = desc_b + (at + step_offset<BMN>(k));
-              product_step_twice(tmem, tmem + kAccumulator, desc_a + (at + step_offset<AMN>(k)), b0, b0 + (kABytes >> 4), idesc, 1);
+              product_step_twice(tmem, tmem + kAccumulator, desc_a + (at + step_offset<AMN>(k)), b0, b0 + half_step, idesc, 1);
             }
             product_commit<CG>(&sh.empty[pos.s], lead);
-            pos.step();
+            pos.step(stages);
           }
           ahead = pos;
           if (!ok) break;
@@ -1098,9 +1098,9 @@ struct TileChoice {
 // clocks of MMA per column of its tile (128 rows x 16 take half a clock a
 // column), or its operand rows' 128 bytes at the 45 bytes a clock that L2 was
 // measured to deliver, whichever is longer; plus what a tile adds: little where
-// the epilogue hides under the next tile, about 4000 clocks where it does not
-// (wide), a meeting of partials (split).
-TileChoice choose_tiles(int m, int n, int kblocks, bool amn) {
+// the epilogue hides under the next tile, ``exposed`` clocks a column where it
+// does not (wide), a meeting of partials (split).
+TileChoice choose_tiles(int m, int n, int kblocks, bool amn, double exposed) {
   TileChoice best{1, 128, 1, 1};
   double least = 1e300;
   const int cg = m > kTileM ? 2 : 1;
@@ -1113,7 +1113,7 @@ TileChoice choose_tiles(int m, int n, int kblocks, bool amn) {
     if (splits > 1 && waves > 1) return;
     const double mma = 2.0 * cols, load = 128.0 / 45.0 * (a_rows + cols / cg);
     const double cost = waves * (static_cast<double>(kblocks) / splits * (mma > load ? mma : load) +
-                                 (halves > 1 ? 16.0 * bn : 200.0)) +
+                                 (halves > 1 ? exposed * bn : 200.0)) +
                         (splits > 1 ? 2500.0 : 6.0 * cols);
     if (cost < least) {
       least = cost;
@@ -1160,7 +1160,7 @@ int launch_gemm(GemmArgs& g, const Operand* a, const Operand* b, int segments, i
     g.kblocks[s] = ((AMN ? a[s].rows : a[s].cols) + kTileK - 1) / kTileK;
     kblocks += g.kblocks[s];
   }
-  const TileChoice c = choose_tiles(g.m, g.n, kblocks, AMN);
+  const TileChoice c = choose_tiles(g.m, g.n, kblocks, AMN, !EPI ? 24.0 : g.act == kActNone ? 48.0 : 88.0);
   g.bn = c.bn;
   g.tiles_m = (g.m + c.cg * kTileM - 1) / (c.cg * kTileM);
   g.tiles_n = (g.n + c.bn * c.halves - 1) / (c.bn * c.halves);
@@ -1170,7 +1170,11 @@ int launch_gemm(GemmArgs& g, const Operand* a, const Operand* b, int segments, i
   const int a_rows = g.m < kTileM ? (g.m + 7) / 8 * 8 : kTileM, b_rows = c.bn / c.cg;
   g.a_panels = g.m > 64 ? 2 : 1;
   g.b_panels = (b_rows + 63) / 64;
-  g.stage_tx = (AMN ? g.a_panels * 8192 : a_rows * 128) + c.halves * (BMN ? g.b_panels * 8192 : b_rows * 128);
+  g.a_bytes = AMN ? g.a_panels * 8192 : a_rows * 128;
+  g.b_bytes = BMN ? g.b_panels * 8192 : b_rows * 128;
+  g.stage_bytes = g.a_bytes + c.halves * g.b_bytes;
+  g.stages = kRingBytes / static_cast<int>(g.stage_bytes);
+  if (g.stages > kMaxStages) g.stages = kMaxStages;
   // a joined copy starts on a whole panel
   g.a_joined = AMN && g.m % 64 == 0;
   g.b_joined = BMN && g.n % 64 == 0 && b_rows % 64 == 0;
