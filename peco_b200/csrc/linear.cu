@@ -138,6 +138,19 @@ __device__ __forceinline__ void activate_slope2(float2 z, float2& value, float2&
   }
 }
 
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// Bounded wait of a whole warp: one try by every lane, then as mbar_wait_warp.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t phase, volatile int* abort_flag, unsigned* status) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, phase))) return true;
+  return mbar_wait_warp(bar, phase, abort_flag, status);
+}
+
 // ---- CTA pairs -------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -208,12 +221,12 @@ __device__ __forceinline__ void product_step(uint32_t d, uint64_t a, uint64_t b,
 // Two products of a pair with one A operand, into two accumulators: the second
 // takes A from the collector that the first filled, not from shared memory again.
 __device__ __forceinline__ void product_step_twice(uint32_t d0, uint32_t d1, uint64_t a, uint64_t b0, uint64_t b1,
-                                                   uint32_t idesc, uint32_t accumulate) {
+                                                   uint32_t idesc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+      "{\n\t.reg .pred p;\n\tsetp.eq.b32 p, 0, 0;\n\t"
       "tcgen05.mma.cta_group::2.kind::f16.collector::a::fill [%0], %2, %3, %5, p;\n\t"
       "tcgen05.mma.cta_group::2.kind::f16.collector::a::lastuse [%1], %2, %4, %5, p;\n\t}" ::"r"(d0),
-      "r"(d1), "l"(a), "l"(b0), "l"(b1), "r"(idesc), "r"(accumulate)
+      "r"(d1), "l"(a), "l"(b0), "l"(b1), "r"(idesc)
       : "memory");
 }
 
@@ -641,127 +654,143 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
   const int kb_begin = SPLIT ? static_cast<int>(static_cast<long long>(kblocks) * part / splits) : 0;
   const int kb_end = SPLIT ? static_cast<int>(static_cast<long long>(kblocks) * (part + 1) / splits) : kblocks;
 
+  // The feeding and issuing warps run their loops whole, so that addresses and
+  // descriptors stay in uniform registers, and one elected lane issues.
   if (warp == 0 || warp == kEpilogueWarps + 2) {
     // ------------------------------------------- TMA: one warp for A, one for B
-    if (lane == 0) {
-      const bool is_a = warp == 0;
-      bool ok = true;
-      RingPos pos{0, 0};
-      // the pair's stages fill one barrier, the first CTA's, which expects both CTAs' bytes
-      const uint32_t bar0 = CG > 1 ? map_rank(smem_u32(&sh.full[0]), lead) : smem_u32(&sh.full[0]);
-      for (int t = group; t < tiles && ok; t += groups) {
-        int tm, tn;
-        tile_coords(t, args.tiles_m, args.tiles_n, tm, tn);
-        const int row0 = is_a ? (tm * CG + rank) * kTileM : tn * kHalves * args.bn + rank * (args.bn / CG);
-        for (int kb = kb_begin; kb < kb_end; ++kb) {
-          ok = mbar_wait(&sh.empty[pos.s], pos.phase ^ 1, abort_flag, args.status);
-          if (!ok) break;
-          const uint32_t st = ring + pos.s * args.stage_bytes, bar = bar0 + pos.s * 8;
-          const int seg = kb >= kb0 ? 1 : 0;
-          const int k0 = (kb - (seg ? kb0 : 0)) * kTileK;
+    const bool is_a = warp == 0, issuer = elect_one();
+    bool ok = true;
+    RingPos pos{0, 0};
+    // the pair's stages fill one barrier, the first CTA's, which expects both CTAs' bytes
+    const uint32_t bar0 = CG > 1 ? map_rank(smem_u32(&sh.full[0]), lead) : smem_u32(&sh.full[0]);
+    for (int t = group; t < tiles && ok; t += groups) {
+      int tm, tn;
+      tile_coords(t, args.tiles_m, args.tiles_n, tm, tn);
+      const int row0 = is_a ? (tm * CG + rank) * kTileM : tn * kHalves * args.bn + rank * (args.bn / CG);
+      for (int kb = kb_begin; kb < kb_end; ++kb) {
+        ok = warp_wait(&sh.empty[pos.s], pos.phase ^ 1, abort_flag, args.status);
+        if (!ok) break;
+        const uint32_t st = ring + pos.s * args.stage_bytes, bar = bar0 + pos.s * 8;
+        const int seg = kb >= kb0 ? 1 : 0;
+        const int k0 = (kb - (seg ? kb0 : 0)) * kTileK;
+        if (issuer) {
           if (is_a) {
             if (rank == 0) mbar_arrive_expect_tx(&sh.full[pos.s], CG * args.stage_bytes);
             load_tile<CG, AMN>(st, &args.a[seg], row0, args.a_panels, args.a_joined, k0, bar);
           } else {
 #pragma unroll
             for (int h = 0; h < kHalves; ++h)
-              load_tile<CG, BMN>(st + args.a_bytes + h * args.b_bytes, &args.b[seg], row0 + h * args.bn, args.b_panels, args.b_joined, k0, bar);
+              load_tile<CG, BMN>(st + args.a_bytes + h * args.b_bytes, &args.b[seg], row0 + h * args.bn, args.b_panels,
+                                 args.b_joined, k0, bar);
           }
-          pos.step(stages);
         }
+        __syncwarp();
+        pos.step(stages);
       }
-      // after an expired wait: time for the copies still in flight to land before the CTA ends
-      if (!ok) {
-        const unsigned long long t0 = globaltimer();
-        while (globaltimer() - t0 < 2000000ull) {
-        }
+    }
+    // after an expired wait: time for the copies still in flight to land before the CTA ends
+    if (!ok) {
+      const unsigned long long t0 = globaltimer();
+      while (globaltimer() - t0 < 2000000ull) {
       }
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       constexpr int ab = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+      const bool issuer = elect_one();
       const uint32_t idesc = instr_desc(kTileM * CG, args.bn, ab, AMN, BMN);
       const uint64_t desc_a = tile_desc<AMN>(ring), desc_b = tile_desc<BMN>(ring + args.a_bytes);
       const uint32_t stage_step = args.stage_bytes >> 4, half_step = args.b_bytes >> 4;
       bool ok = true;
       RingPos pos{0, 0};
       uint32_t local = 0;
-      // one K block's products for one accumulator; the first of a tile overwrite it
-      auto products = [&](int s, int half, uint32_t acc, bool first) {
+      // one K block's products for one accumulator (``accumulate`` 0: overwriting it)
+      auto products = [&](int s, int half, uint32_t acc, uint32_t accumulate) {
         const uint32_t at = s * stage_step, at_b = at + half * half_step;
-        uint32_t accumulate = first ? 0 : 1;
+        product_step<CG>(acc, desc_a + at, desc_b + at_b, idesc, accumulate);
 #pragma unroll
-        for (int k = 0; k < kTileK / 16; ++k) {
-          product_step<CG>(acc, desc_a + (at + step_offset<AMN>(k)), desc_b + (at_b + step_offset<BMN>(k)), idesc, accumulate);
-          accumulate = 1;
-        }
+        for (int k = 1; k < kTileK / 16; ++k)
+          product_step<CG>(acc, desc_a + (at + step_offset<AMN>(k)), desc_b + (at_b + step_offset<BMN>(k)), idesc, 1);
+      };
+      auto wait_full = [&](const RingPos& p) {
+        ok = warp_wait(&sh.full[p.s], p.phase, abort_flag, args.status);
+        if (ok) tc_fence_after();
+        return ok;
       };
       for (int t = group; t < tiles && ok; t += groups, ++local) {
         if constexpr (!WIDE) {
           const int b = local & 1;
-          ok = mbar_wait(&sh.acc_empty[b], ((local >> 1) & 1) ^ 1, abort_flag, args.status);
+          ok = warp_wait(&sh.acc_empty[b], ((local >> 1) & 1) ^ 1, abort_flag, args.status);
           if (!ok) break;
           tc_fence_after();
           for (int kb = kb_begin; kb < kb_end; ++kb) {
-            ok = mbar_wait(&sh.full[pos.s], pos.phase, abort_flag, args.status);
-            if (!ok) break;
-            tc_fence_after();
-            products(pos.s, 0, tmem + b * kAccumulator, kb == kb_begin);
-            product_commit<CG>(&sh.empty[pos.s], lead);
+            if (!wait_full(pos)) break;
+            if (issuer) {
+              products(pos.s, 0, tmem + b * kAccumulator, kb > kb_begin);
+              product_commit<CG>(&sh.empty[pos.s], lead);
+            }
+            __syncwarp();
             pos.step(stages);
           }
-          if (ok) product_commit<CG>(&sh.acc_full[b], lead);
+          if (ok && issuer) product_commit<CG>(&sh.acc_full[b], lead);
+          __syncwarp();
         } else {
           // K blocks in order for each half; the second half trails the first by
           // up to a ring of stages at the tile's start and at its end
           const uint32_t free_phase = (local & 1) ^ 1;
           const int skew = min(stages, kblocks), last = max(skew, kblocks - stages);
-          ok = mbar_wait(&sh.acc_empty[0], free_phase, abort_flag, args.status);
+          ok = warp_wait(&sh.acc_empty[0], free_phase, abort_flag, args.status);
           if (!ok) break;
           tc_fence_after();
           RingPos ahead = pos;
           auto first_half = [&](int kb) {
-            ok = mbar_wait(&sh.full[ahead.s], ahead.phase, abort_flag, args.status);
-            if (!ok) return;
-            tc_fence_after();
-            products(ahead.s, 0, tmem, kb == 0);
+            if (!wait_full(ahead)) return;
+            if (issuer) products(ahead.s, 0, tmem, kb > 0);
+            __syncwarp();
             ahead.step(stages);
           };
           auto second_half = [&](int kb) {
-            products(pos.s, 1, tmem + kAccumulator, kb == 0);
-            product_commit<CG>(&sh.empty[pos.s], lead);
+            if (issuer) {
+              products(pos.s, 1, tmem + kAccumulator, kb > 0);
+              product_commit<CG>(&sh.empty[pos.s], lead);
+            }
+            __syncwarp();
             pos.step(stages);
           };
           for (int kb = 0; kb < skew && ok; ++kb) first_half(kb);
           if (!ok) break;
-          if (skew == kblocks) product_commit<CG>(&sh.acc_full[0], lead);
-          ok = mbar_wait(&sh.acc_empty[1], free_phase, abort_flag, args.status);
+          if (skew == kblocks && issuer) product_commit<CG>(&sh.acc_full[0], lead);
+          __syncwarp();
+          ok = warp_wait(&sh.acc_empty[1], free_phase, abort_flag, args.status);
           if (!ok) break;
           tc_fence_after();
           for (int kb = 0; kb < skew; ++kb) second_half(kb);
           for (int kb = skew; kb < last; ++kb) {
-            ok = mbar_wait(&sh.full[pos.s], pos.phase, abort_flag, args.status);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t at = pos.s * stage_step;
+            if (!wait_full(pos)) break;
+            if (issuer) {
+              const uint32_t at = pos.s * stage_step;
 #pragma unroll
-            for (int k = 0; k < kTileK / 16; ++k) {
-              const uint64_t b0 = desc_b + (at + step_offset<BMN>(k));
-              product_step_twice(tmem, tmem + kAccumulator, desc_a + (at + step_offset<AMN>(k)), b0, b0 + half_step, idesc, 1);
+              for (int k = 0; k < kTileK / 16; ++k) {
+                const uint64_t b0 = desc_b + (at + step_offset<BMN>(k));
+                product_step_twice(tmem, tmem + kAccumulator, desc_a + (at + step_offset<AMN>(k)), b0, b0 + half_step, idesc);
+              }
+              product_commit<CG>(&sh.empty[pos.s], lead);
             }
-            product_commit<CG>(&sh.empty[pos.s], lead);
+            __syncwarp();
             pos.step(stages);
           }
-          ahead = pos;
           if (!ok) break;
+          ahead = pos;
           if (last < kblocks) {
             for (int kb = last; kb < kblocks && ok; ++kb) first_half(kb);
             if (!ok) break;
-            product_commit<CG>(&sh.acc_full[0], lead);
+            if (issuer) product_commit<CG>(&sh.acc_full[0], lead);
+            __syncwarp();
             for (int kb = last; kb < kblocks; ++kb) second_half(kb);
           }
-          product_commit<CG>(&sh.acc_full[1], lead);
+          if (issuer) product_commit<CG>(&sh.acc_full[1], lead);
+          __syncwarp();
         }
       }
     }
