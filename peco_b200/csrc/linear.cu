@@ -35,7 +35,8 @@ struct GemmArgs {
   CUtensorMap a[2], b[2];    // K segments (x and x2; the second unused otherwise)
   int kblocks[2];            // 64-wide K blocks of each segment
   int m, n, tiles_m, tiles_n;
-  int bn;                    // columns of a tile, a multiple of 32
+  int bn;                    // columns of an accumulator, a multiple of 32
+  int band;                  // m tiles walked together
   int a_panels, b_panels;    // 64-wide panels of an MN-major operand per CTA
   int a_joined, b_joined;    // ... all of them in one copy (the operand's width is a multiple of 64)
   int stages;                // of the ring in shared memory
@@ -300,17 +301,16 @@ struct GemmShared {
   int abort_flag;
 };
 
-// (m tile, n tile) of a linear tile number: bands of kBand m tiles walked
-// down first, so that the CTAs running at one time share few rows of A and B
-constexpr int kBand = 8;
-__device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int& tm, int& tn) {
-  const int per_band = kBand * tiles_n;
+// (m tile, n tile) of a linear tile number: bands of ``band`` m tiles, walked
+// down first.
+__device__ __forceinline__ void tile_coords(const GemmArgs& args, int t, int& tm, int& tn) {
+  const int per_band = args.band * args.tiles_n;
   const int band = t / per_band;
-  const int first = band * kBand;
-  const int height = min(kBand, tiles_m - first);
+  const int first = band * args.band;
+  const int height = min(args.band, args.tiles_m - first);
   const int in = t - band * per_band;
-  tm = first + in % height;
   tn = in / height;
+  tm = first + in - tn * height;
 }
 
 // Operand rows x 64 into shared memory: K-major rows of 128 bytes (one box), or
@@ -665,7 +665,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     const uint32_t bar0 = CG > 1 ? map_rank(smem_u32(&sh.full[0]), lead) : smem_u32(&sh.full[0]);
     for (int t = group; t < tiles && ok; t += groups) {
       int tm, tn;
-      tile_coords(t, args.tiles_m, args.tiles_n, tm, tn);
+      tile_coords(args, t, tm, tn);
       const int row0 = is_a ? (tm * CG + rank) * kTileM : tn * kHalves * args.bn + rank * (args.bn / CG);
       for (int kb = kb_begin; kb < kb_end; ++kb) {
         ok = warp_wait(&sh.empty[pos.s], pos.phase ^ 1, abort_flag, args.status);
@@ -803,7 +803,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     uint32_t turn = 0;  // accumulators finished
     for (int t = group; t < tiles; t += groups) {
       int tm, tn;
-      tile_coords(t, args.tiles_m, args.tiles_n, tm, tn);
+      tile_coords(args, t, tm, tn);
       const long long tile_row = static_cast<long long>(tm * CG + static_cast<int>(rank)) * kTileM;
       const long long row0 = tile_row + quarter * 32;
       // one gate row for all of the CTA's rows, or each row's own
@@ -858,7 +858,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
   }
   if constexpr (SPLIT) {
     int tm, tn;
-    tile_coords(group, args.tiles_m, args.tiles_n, tm, tn);
+    tile_coords(args, group, tm, tn);
     const int first = kTileM * part / splits, rows = kTileM * (part + 1) / splits - first;
     const int pieces = args.bn / 8;  // 8 columns each
     const int col0 = tn * args.bn;
@@ -1125,8 +1125,7 @@ struct TileChoice {
 
 // Estimated clocks of a choice, from what one SM does per 64-wide K block: 2
 // clocks of MMA per column of its tile (128 rows x 16 take half a clock a
-// column), or its operand rows' 128 bytes at the 45 bytes a clock that L2 was
-// measured to deliver, whichever is longer; plus what a tile adds: little where
+// column), or its operand rows' 128 bytes at 50 bytes a clock, whichever is longer; plus what a tile adds: little where
 // the epilogue hides under the next tile, ``exposed`` clocks a column where it
 // does not (wide), a meeting of partials (split).
 TileChoice choose_tiles(int m, int n, int kblocks, bool amn, double exposed) {
@@ -1140,7 +1139,7 @@ TileChoice choose_tiles(int m, int n, int kblocks, bool amn, double exposed) {
     const long long tiles = tiles_m * ((n + cols - 1) / cols);
     const long long waves = (tiles * splits * cg + kNumSMs - 1) / kNumSMs;
     if (splits > 1 && waves > 1) return;
-    const double mma = 2.0 * cols, load = 128.0 / 45.0 * (a_rows + cols / cg);
+    const double mma = 2.0 * cols, load = 128.0 / 50.0 * (a_rows + cols / cg);
     const double cost = waves * (static_cast<double>(kblocks) / splits * (mma > load ? mma : load) +
                                  (halves > 1 ? exposed * bn : 200.0)) +
                         (splits > 1 ? 2500.0 : 6.0 * cols);
@@ -1189,11 +1188,19 @@ int launch_gemm(GemmArgs& g, const Operand* a, const Operand* b, int segments, i
     g.kblocks[s] = ((AMN ? a[s].rows : a[s].cols) + kTileK - 1) / kTileK;
     kblocks += g.kblocks[s];
   }
-  const TileChoice c = choose_tiles(g.m, g.n, kblocks, AMN, !EPI ? 24.0 : g.act == kActNone ? 48.0 : 88.0);
+  const TileChoice c = choose_tiles(g.m, g.n, kblocks, AMN, !EPI ? 24.0 : g.act == kActNone ? 72.0 : 88.0);
   g.bn = c.bn;
   g.tiles_m = (g.m + c.cg * kTileM - 1) / (c.cg * kTileM);
   g.tiles_n = (g.n + c.bn * c.halves - 1) / (c.bn * c.halves);
   if (static_cast<long long>(g.tiles_m) * g.tiles_n > 0x0fffffffLL) return kErrUnsupported;
+  // The smaller operand stays in L2 while the larger passes once: A smaller, all
+  // m tiles under every column of tiles; B smaller, two m tiles across all
+  // columns.  The SMs are at their power limit in long products, so DRAM traffic
+  // costs time (6750 x 3072 x 12288: 374 us with all m tiles, 400 with bands of
+  // eight; 6750 x 12288 x 3072: 378 us with four, 394 with all).
+  const double a_all = 128.0 * g.m * kblocks, b_all = 128.0 * g.n * kblocks;
+  g.band = (a_all < b_all ? a_all : b_all) > 96e6 ? 8 : a_all <= b_all ? g.tiles_m : 2;
+  if (g.band > g.tiles_m) g.band = g.tiles_m;
   // rows (or panels) of the operands one CTA stages per K block; a single tile
   // of few rows loads only those, the others' results are never stored
   const int a_rows = g.m < kTileM ? (g.m + 7) / 8 * 8 : kTileM, b_rows = c.bn / c.cg;
