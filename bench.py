@@ -60,6 +60,8 @@ def parse_args():
                          "(strong scaling, the long-video config)")
     ap.add_argument("--long-steps", type=int, default=10,
                     help="timed steps of the long-video sub-record, at least about a second's worth (0 skips it)")
+    ap.add_argument("--block-operators", action="store_true",
+                    help="hv-step: run the blocks around the attention through linear_act and modulated_norm")
     ap.add_argument("--e2e-steps", type=int, default=100)
     ap.add_argument("--cpu-sample-heads", type=int, default=2)
     ap.add_argument("--baselines", choices=("all", "none"), default="all",
@@ -354,6 +356,9 @@ def run_step(args, world, rank, local):
     pcfg = PecoConfig(num_q_centroids=256, num_k_centroids=ck, top_p=1e-9, min_kc_ratio=top_k / ck, kmeans_iter_init=5,
                       kmeans_iter_step=5, warmup_steps=0, base_offset_bits=4)
     install_attention(pipe, pcfg)
+    if args.block_operators:
+        from peco_b200.hunyuan import use_block_operators
+        use_block_operators(model)
     g = torch.Generator(device="cpu").manual_seed(1000)  # every rank holds the same step's inputs
     latent_h = torch.randn(1, 16, 17, 68, 120, generator=g).to(torch.bfloat16).pin_memory()
     text_h = torch.randn(1, 256, hcfg.text_dim, generator=g).to(torch.bfloat16).pin_memory()
@@ -431,7 +436,8 @@ def run_step(args, world, rank, local):
         "config": {
             "workload": f"hv-step: HunyuanVideo architecture (20 dual + 40 single blocks, hidden 3072, 24 heads x 128, "
                         f"MLP x4, RMSNorm Q/K, 3D RoPE), latent 16x17x68x120 -> {tokens} video + 256 text tokens; "
-                        "PECO CQ=256, CK=512, 5 Lloyd iterations, top-32, 4-bit Base-Offset in every block",
+                        "PECO CQ=256, CK=512, 5 Lloyd iterations, top-32, 4-bit Base-Offset in every block"
+                        + ("; blocks through linear_act / modulated_norm" if args.block_operators else ""),
             "parallelism": f"head-parallel over {world} rank(s): {hcfg.heads // world} attention heads and 1/{world} of "
                            "every MLP hidden layer per rank, one all-reduce after each row-parallel projection",
             "l2": "inputs and weights far larger than L2",

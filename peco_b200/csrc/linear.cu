@@ -888,12 +888,22 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
 }
 
 // ---- unaligned operands ------------------------------------------------------------
-// rows [rows, cols] of 2-byte elements, any stride and alignment, to rows ld
-// elements apart (16-byte aligned); a block per row group, threads over columns
-__global__ void __launch_bounds__(256) pack_rows_kernel(const uint16_t* src, long long src_stride, uint16_t* dst,
-                                                        int ld, int rows, int cols) {
-  for (long long r = blockIdx.x; r < rows; r += gridDim.x)
-    for (int c = threadIdx.x; c < cols; c += blockDim.x) dst[r * ld + c] = src[r * src_stride + c];
+// Rows [rows, cols] of 2-byte elements, any stride and alignment, to rows ld
+// elements apart (16-byte aligned), up to four operands in one launch: blocks
+// stride over an operand's rows, threads over columns.
+struct PackArgs {
+  const uint16_t* src[4];
+  uint16_t* dst[4];
+  long long stride[4];
+  int ld[4], rows[4], cols[4];
+};
+__global__ void __launch_bounds__(256) pack_rows_kernel(const __grid_constant__ PackArgs a) {
+  const int k = blockIdx.y, cols = a.cols[k];
+  for (long long r = blockIdx.x; r < a.rows[k]; r += gridDim.x) {
+    const uint16_t* src = a.src[k] + r * a.stride[k];
+    uint16_t* dst = a.dst[k] + r * a.ld[k];
+    for (int c = threadIdx.x; c < cols; c += 256) dst[c] = src[c];
+  }
 }
 
 // ---- gradient of the epilogue --------------------------------------------------------
@@ -1078,15 +1088,26 @@ struct Carver {
   }
 };
 
-// The operand itself, or its copy in the workspace when TMA cannot read it.
-int prepare_operand(Operand& o, Carver& ws, cudaStream_t stream) {
-  if (o.aligned()) return kOk;
-  const int ld = static_cast<int>(align_up(o.cols, 8));
-  uint16_t* dst = static_cast<uint16_t*>(ws.take(o.pack_bytes()));
-  const int grid = o.rows < 8 * kNumSMs ? o.rows : 8 * kNumSMs;
-  pack_rows_kernel<<<grid, 256, 0, stream>>>(static_cast<const uint16_t*>(o.ptr), o.stride, dst, ld, o.rows, o.cols);
-  o.ptr = dst;
-  o.stride = ld;
+// Operands that TMA cannot read become copies in the workspace, in one launch.
+int prepare_operands(Operand* const* list, int n, Carver& ws, cudaStream_t stream) {
+  PackArgs p{};
+  int jobs = 0, most = 0;
+  for (int i = 0; i < n; ++i) {
+    Operand& o = *list[i];
+    if (o.aligned()) continue;
+    p.src[jobs] = static_cast<const uint16_t*>(o.ptr);
+    p.stride[jobs] = o.stride;
+    p.dst[jobs] = static_cast<uint16_t*>(ws.take(o.pack_bytes()));
+    p.ld[jobs] = static_cast<int>(align_up(o.cols, 8));
+    p.rows[jobs] = o.rows;
+    p.cols[jobs] = o.cols;
+    if (o.rows > most) most = o.rows;
+    o.ptr = p.dst[jobs];
+    o.stride = p.ld[jobs];
+    ++jobs;
+  }
+  if (!jobs) return kOk;
+  pack_rows_kernel<<<dim3(most < 8 * kNumSMs ? most : 8 * kNumSMs, jobs), 256, 0, stream>>>(p);
   return launch_status();
 }
 
@@ -1246,10 +1267,8 @@ const void* offset16(const void* p, long long elements) { return static_cast<con
 template <typename T>
 int forward(const LinearShape& s, Operand (&a)[2], Operand (&b)[2], GemmArgs& g, Carver& ws, cudaStream_t stream) {
   const int segments = s.k2 > 0 ? 2 : 1;
-  for (int i = 0; i < segments; ++i) {
-    if (int st = prepare_operand(a[i], ws, stream)) return st;
-    if (int st = prepare_operand(b[i], ws, stream)) return st;
-  }
+  Operand* list[4] = {&a[0], &b[0], &a[1], &b[1]};
+  if (int st = prepare_operands(list, 2 * segments, ws, stream)) return st;
   return launch_gemm<T, false, false, true>(g, a, b, segments, s.dtype, stream);
 }
 
@@ -1335,11 +1354,17 @@ int backward(const LinearShape& s, Operand grad, const void* preact, Operand (&x
       if (int st = launch_status()) return st;
     }
   }
+  Operand* list[4];
+  int wanted = 0;
+  for (int i = 0; i < segments; ++i) {
+    if (dx[i]) list[wanted++] = &w[i];
+    if (dweight) list[wanted++] = &x[i];
+  }
+  if (int st = prepare_operands(list, wanted, ws, stream)) return st;
   for (int i = 0; i < segments; ++i) {
     const int cols = i ? s.k2 : s.k;
     if (dx[i]) {
       // dx[m, c] = sum_n dz[m, n] W[n, c]: W's rows run along the output's columns
-      if (int st = prepare_operand(w[i], ws, stream)) return st;
       GemmArgs g{};
       g.m = static_cast<int>(s.rows());
       g.n = cols;
@@ -1350,7 +1375,6 @@ int backward(const LinearShape& s, Operand grad, const void* preact, Operand (&x
     }
     if (dweight) {
       // dW[n, c] = sum_m dz[m, n] x[m, c]: both operands run along the outputs
-      if (int st = prepare_operand(x[i], ws, stream)) return st;
       GemmArgs g{};
       g.m = s.n;
       g.n = cols;

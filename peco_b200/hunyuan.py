@@ -47,7 +47,10 @@ import torch.distributed as dist
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .linear import linear_act
+from .norms import modulated_norm
 from .processor import InferenceContext, PecoAttention, PecoConfig
+from .rotary import AxialPositions
 
 
 @dataclass(frozen=True)
@@ -234,6 +237,29 @@ class Attention(nn.Module):
         return self.processor(self, hidden_states, encoder_hidden_states, attention_mask, image_rotary_emb)
 
 
+# Block operators (``use_block_operators``): the same block math through
+# linear_act, modulated_norm and table-free rotary positions.
+
+def _modulation(layer, e, parts):
+    """The modulation vectors [B, D] of a block, as views of one projection."""
+    return linear_act(e, layer.weight, layer.bias).unflatten(-1, (parts, -1)).unbind(1)
+
+
+def _row_operator(layer, x, gate, residual, x2=None):
+    """residual + gate * (layer([x | x2])) of a row-parallel layer; over several
+    ranks the partial products are summed first."""
+    if layer.tp.world == 1:
+        return linear_act(x, layer.weight, layer.bias, gate=gate, residual=residual, x2=x2)
+    y = linear_act(x, layer.weight, x2=x2)
+    dist.all_reduce(y, group=layer.tp.group)
+    return torch.addcmul(residual, gate[:, None], y + layer.bias)
+
+
+def _mlp_operator(ff, h, gate, residual):
+    hidden = linear_act(h, ff[0].weight, ff[0].bias, activation="gelu_tanh")
+    return _row_operator(ff[2], hidden, gate, residual)
+
+
 def _mlp(dim, ratio, tp: TensorParallel = SINGLE):
     hidden = dim * ratio
     return nn.Sequential(column_linear(dim, hidden, tp), nn.GELU(approximate="tanh"),
@@ -249,8 +275,11 @@ class DualStreamBlock(nn.Module):
         self.attn = Attention(d, cfg.heads, cfg.head_dim, joint_text=True, pre_only=False, tp=tp)
         self.ff = _mlp(d, cfg.mlp_ratio, tp)
         self.ff_context = _mlp(d, cfg.mlp_ratio, tp)
+        self.block_operators = False
 
     def forward(self, img, txt, temb, rope):
+        if self.block_operators:
+            return self._forward_operators(img, txt, temb, rope)
         e = F.silu(temb)
         i_shift, i_scale, i_gate, i_shift2, i_scale2, i_gate2 = self.img_mod(e)[:, None].chunk(6, dim=-1)
         t_shift, t_scale, t_gate, t_shift2, t_scale2, t_gate2 = self.txt_mod(e)[:, None].chunk(6, dim=-1)
@@ -260,6 +289,16 @@ class DualStreamBlock(nn.Module):
         img = img + i_gate2 * self.ff(_ln(img) * (1 + i_scale2) + i_shift2)
         txt = txt + t_gate2 * self.ff_context(_ln(txt) * (1 + t_scale2) + t_shift2)
         return img, txt
+
+    def _forward_operators(self, img, txt, temb, rope):
+        e = F.silu(temb)
+        i_shift, i_scale, i_gate, i_shift2, i_scale2, i_gate2 = _modulation(self.img_mod, e, 6)
+        t_shift, t_scale, t_gate, t_shift2, t_scale2, t_gate2 = _modulation(self.txt_mod, e, 6)
+        a_img, a_txt = self.attn(modulated_norm(img, scale=i_scale, shift=i_shift),
+                                 modulated_norm(txt, scale=t_scale, shift=t_shift), None, rope)
+        img, h_img = modulated_norm(img, a_img, gate=i_gate, scale=i_scale2, shift=i_shift2)
+        txt, h_txt = modulated_norm(txt, a_txt, gate=t_gate, scale=t_scale2, shift=t_shift2)
+        return _mlp_operator(self.ff, h_img, i_gate2, img), _mlp_operator(self.ff_context, h_txt, t_gate2, txt)
 
 
 class SingleStreamBlock(nn.Module):
@@ -274,8 +313,11 @@ class SingleStreamBlock(nn.Module):
         a, b = tp.span(inner)
         c, e = tp.span(hidden)
         self.proj_out = RowParallelLinear(d, inner + hidden, [(a, b), (inner + c, inner + e)], tp)
+        self.block_operators = False
 
     def forward(self, img, txt, temb, rope):
+        if self.block_operators:
+            return self._forward_operators(img, txt, temb, rope)
         n_txt = txt.shape[1]
         x = torch.cat((img, txt), 1)
         shift, scale, gate = self.mod(F.silu(temb))[:, None].chunk(3, dim=-1)
@@ -284,6 +326,16 @@ class SingleStreamBlock(nn.Module):
         a_img, a_txt = self.attn(h[:, :-n_txt], h[:, -n_txt:], None, rope)
         x = x + gate * self.proj_out(torch.cat((torch.cat((a_img, a_txt), 1), mlp), -1))
         return x[:, :-n_txt], x[:, -n_txt:]
+
+    def _forward_operators(self, img, txt, temb, rope):
+        n_img = img.shape[1]
+        x = torch.cat((img, txt), 1)
+        shift, scale, gate = _modulation(self.mod, F.silu(temb), 3)
+        h = modulated_norm(x, scale=scale, shift=shift)
+        mlp = linear_act(h, self.proj_mlp.weight, self.proj_mlp.bias, activation="gelu_tanh")
+        a_img, a_txt = self.attn(h[:, :n_img], h[:, n_img:], None, rope)
+        x = _row_operator(self.proj_out, torch.cat((a_img, a_txt), 1), gate, x, x2=mlp)
+        return x[:, :n_img], x[:, n_img:]
 
 
 def _timestep_embedding(t, dim=256, max_period=10000.0):
@@ -311,6 +363,7 @@ class HunyuanVideoTransformer(nn.Module):
         super().__init__()
         self.cfg = cfg
         self.tp = tp
+        self.block_operators = False
         d = cfg.hidden
         self.x_embedder = nn.Conv3d(cfg.in_channels, d, kernel_size=cfg.patch, stride=cfg.patch)
         self.context_embedder = nn.Linear(cfg.text_dim, d)
@@ -354,7 +407,9 @@ class HunyuanVideoTransformer(nn.Module):
         temb = self.time_in(_timestep_embedding(timestep).to(img.dtype)) + self.vector_in(pooled_projections)
         key = (grid, img.device)
         rope = self._rope.get(key) if hasattr(self, "_rope") else None
-        if rope is None:  # built once per grid (host tables copied to the device)
+        if self.block_operators:  # positions instead of tables
+            rope = AxialPositions(self.cfg.rope_axes, self.cfg.rope_theta, grid=grid)
+        elif rope is None:  # built once per grid (host tables copied to the device)
             rope = rope_3d(grid, self.cfg.rope_axes, self.cfg.rope_theta, img.device)
             self._rope = {key: rope}
         for block in self.transformer_blocks:
@@ -390,6 +445,17 @@ class Pipe:
 
     def __init__(self, transformer):
         self.transformer = transformer
+
+
+def use_block_operators(transformer, enabled=True):
+    """Run every block's norms, modulation, projections, MLPs, gates and
+    residuals through ``modulated_norm`` and ``linear_act``, and rotate Q and K by
+    grid positions instead of tables.  For CUDA float16 / bfloat16 inference; the
+    attention processors stay as installed (their bfloat16 rule included)."""
+    transformer.block_operators = enabled
+    for block in [*transformer.transformer_blocks, *transformer.single_transformer_blocks]:
+        block.block_operators = enabled
+        block.attn.block_operators = enabled
 
 
 def use_dense_attention(transformer, context: InferenceContext):

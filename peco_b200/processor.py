@@ -30,6 +30,8 @@ import torch
 
 from . import _native
 from .clustering import kmeans_fit_pair, fit_token_clusters
+from .linear import linear_act
+from .rotary import AxialPositions
 
 
 @dataclass(frozen=True)
@@ -308,15 +310,21 @@ class PecoAttention:
         embedding of the video rows and the text rows appended after them.
         The attention output goes back through ``to_out`` (video) and
         ``to_add_out`` (text) where the module has them.
+
+        ``image_rotary_emb``: the (cos, sin) tables, or a
+        ``rotary.AxialPositions`` of the video rows, which are then rotated
+        without tables.  A module with a true ``block_operators`` attribute has
+        its projections run by ``linear.linear_act``.
         """
         _native.require_cuda(hidden_states)
         n_text = 0 if encoder_hidden_states is None else encoder_hidden_states.shape[1]
         separate_text = attn.add_q_proj is not None  # dual-stream: text has its own weights
         heads = attn.heads
-        video_proj = [layer(hidden_states) for layer in (attn.to_q, attn.to_k, attn.to_v)]
+        project = _project if getattr(attn, "block_operators", False) else (lambda layer, x: layer(x))
+        video_proj = [project(layer, hidden_states) for layer in (attn.to_q, attn.to_k, attn.to_v)]
         text_layers = (attn.add_q_proj, attn.add_k_proj, attn.add_v_proj) if separate_text else \
             (attn.to_q, attn.to_k, attn.to_v)
-        text_proj = [layer(encoder_hidden_states) for layer in text_layers] if n_text else [None] * 3
+        text_proj = [project(layer, encoder_hidden_states) for layer in text_layers] if n_text else [None] * 3
         b, n_video, inner = video_proj[0].shape
         if b != 1:
             raise ValueError("This minimal HunyuanVideo entry supports one prompt per call")
@@ -329,7 +337,11 @@ class PecoAttention:
         text_norms = (_rms_gain(attn.norm_added_q, dims), _rms_gain(attn.norm_added_k, dims)) if separate_text \
             else video_norms
         cos = sin = None
-        if image_rotary_emb is not None:
+        positions = image_rotary_emb if isinstance(image_rotary_emb, AxialPositions) else None
+        if positions is not None:
+            if positions.rows != n_video:
+                raise ValueError(f"rotary positions of {positions.rows} rows for {n_video} video rows")
+        elif image_rotary_emb is not None:
             cos, sin = (t.to(device=hidden_states.device, dtype=torch.float32).reshape(n_video, dims).contiguous()
                         for t in image_rotary_emb)
         seq = n_video + n_text
@@ -348,6 +360,8 @@ class PecoAttention:
                 opt(text_norms[1][0]), text_norms[0][1], opt(cos), opt(sin), _native.ptr(q), _native.ptr(k),
                 _native.ptr(v), heads, dims, _native.stream_of(dev, *keep))
         _native.check(st, "peco_prepare_qkv")
+        if positions is not None:
+            positions.rotate(q, k, inplace=True)  # the text rows behind the video's stay as they are
         out = self.attention(q, k, v)
         rows = out.transpose(1, 2).reshape(1, seq, inner)  # token-major, heads side by side
         video_out, text_out = rows[:, :n_video], rows[:, n_video:]
@@ -355,10 +369,19 @@ class PecoAttention:
             return video_out, encoder_hidden_states
         if getattr(attn, "to_out", None) is not None:
             for layer in attn.to_out:
-                video_out = layer(video_out)
+                video_out = project(layer, video_out)
         if getattr(attn, "to_add_out", None) is not None:
-            text_out = attn.to_add_out(text_out)
+            text_out = project(attn.to_add_out, text_out)
         return video_out, text_out
+
+
+def _project(layer, x):
+    """``layer(x)`` through linear_act where the layer is a linear map of this rank alone."""
+    weight = getattr(layer, "weight", None)
+    sharded = getattr(getattr(layer, "tp", None), "world", 1) > 1
+    if weight is None or weight.dim() != 2 or sharded:
+        return layer(x)
+    return linear_act(x, weight, layer.bias)
 
 
 def _rms_gain(norm, dims):

@@ -13,6 +13,8 @@ from __future__ import annotations
 
 import ctypes
 import math
+from dataclasses import dataclass
+from typing import Optional
 
 import torch
 
@@ -142,3 +144,25 @@ def rotate(q, k=None, *, axes, theta=256.0, grid=None, positions=None, interleav
         return _Rotate.apply(q, k, options)
     q, k = _run(q, k, **options, inplace=inplace)
     return q if k is None else (q, k)
+
+
+@dataclass(frozen=True)
+class AxialPositions:
+    """Rotary positions of a call's video rows, in place of (cos, sin) tables:
+    the arguments of ``rotate`` that describe them.  The attention processor
+    takes one as ``image_rotary_emb``."""
+
+    axes: tuple
+    theta: float = 256.0
+    grid: Optional[tuple] = None
+    positions: Optional[torch.Tensor] = None
+    interleaved: bool = True
+
+    @property
+    def rows(self) -> int:
+        """How many rows have positions."""
+        return math.prod(self.grid) if self.grid is not None else self.positions.shape[-2]
+
+    def rotate(self, q, k=None, **options):
+        return rotate(q, k, axes=self.axes, theta=self.theta, grid=self.grid, positions=self.positions,
+                      interleaved=self.interleaved, **options)
