@@ -474,12 +474,14 @@ __device__ __forceinline__ void store_chunk(const GemmArgs& args, uint32_t stagi
       }
     }
   } else if (col + lane < col_end) {
+    // a column per lane, one row at a time
     const int rows = static_cast<int>(min(32LL, args.m - row0));
-#pragma unroll 1
-    for (int r = 0; r < rows; ++r) {
+    uint16_t* p = reinterpret_cast<uint16_t*>(out) + row0 * stride + col + lane;
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r, p += stride) {
       uint16_t u;
-      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(staging + staging_offset(r, lane >> 3) + (lane & 7) * 2) : "memory");
-      reinterpret_cast<uint16_t*>(out)[(row0 + r) * stride + col + lane] = u;
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(staging + staging_offset(r, lane >> 3) + (lane & 7) * 2));
+      *p = u;
     }
   }
   __syncwarp();
@@ -506,12 +508,16 @@ __device__ __forceinline__ void add_residual(const GemmArgs& args, uint32_t stag
     for (int i = 0; i < 4; ++i)
       st_shared_v4(staging + staging_offset(i * 8 + (lane >> 2), lane & 3), held[i].x, held[i].y, held[i].z, held[i].w);
   } else {
+    const uint16_t* p = static_cast<const uint16_t*>(args.residual) + row0 * args.res_stride + col + lane;
+    const int rows = col + lane < col_end ? static_cast<int>(min(32LL, args.m - row0)) : 0;
 #pragma unroll 1
-    for (int r = 0; r < 32; ++r) {
-      uint16_t u = 0;
-      if (row0 + r < args.m && col + lane < col_end)
-        u = static_cast<const uint16_t*>(args.residual)[(row0 + r) * args.res_stride + col + lane];
-      asm volatile("st.shared.u16 [%0], %1;" ::"r"(staging + staging_offset(r, lane >> 3) + (lane & 7) * 2), "h"(u) : "memory");
+    for (int r0 = 0; r0 < 32; r0 += 16) {  // sixteen loads in flight
+      uint16_t u[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) u[r] = r0 + r < rows ? p[(r0 + r) * args.res_stride] : static_cast<uint16_t>(0);
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        asm volatile("st.shared.u16 [%0], %1;" ::"r"(staging + staging_offset(r0 + r, lane >> 3) + (lane & 7) * 2), "h"(u[r]) : "memory");
     }
   }
   __syncwarp();
@@ -900,8 +906,9 @@ struct PackArgs {
 __global__ void __launch_bounds__(256) pack_rows_kernel(const __grid_constant__ PackArgs a) {
   const int k = blockIdx.y, cols = a.cols[k];
   for (long long r = blockIdx.x; r < a.rows[k]; r += gridDim.x) {
-    const uint16_t* src = a.src[k] + r * a.stride[k];
-    uint16_t* dst = a.dst[k] + r * a.ld[k];
+    const uint16_t* __restrict__ src = a.src[k] + r * a.stride[k];
+    uint16_t* __restrict__ dst = a.dst[k] + r * a.ld[k];
+#pragma unroll 4
     for (int c = threadIdx.x; c < cols; c += 256) dst[c] = src[c];
   }
 }

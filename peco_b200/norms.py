@@ -15,6 +15,7 @@ saved.  CUDA tensors only; work is enqueued on the current stream.
 
 from __future__ import annotations
 
+import math
 from typing import NamedTuple, Optional
 
 import torch
@@ -67,40 +68,45 @@ def _extent(x):
 
 
 def _check(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, eps, residual_scale):
-    if norm not in ("layer", "rms"):
+    if norm != "layer" and norm != "rms":
         raise ValueError(f'norm must be "layer" or "rms", got {norm!r}')
-    if post_norm not in NORMS:
+    post = NORMS.get(post_norm)
+    if post is None:
         raise ValueError(f'post_norm must be None, "layer" or "rms", got {post_norm!r}')
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         raise TypeError("x must be a torch tensor [..., C]")
-    dtype, device = x.dtype, x.device
+    dtype, device, shape = x.dtype, x.device, x.shape
     if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise TypeError("modulated_norm takes float16 or bfloat16 tensors of one dtype")
     if device.type != "cuda":
         _native.require_cuda(x)
+    c = shape[-1]
+    samples = shape[0] if len(shape) >= 3 else 1
     for t in (branch, gate, scale, shift, weight, post_weight):
         if t is not None:
             if t.dtype is not dtype:
                 raise TypeError("modulated_norm takes float16 or bfloat16 tensors of one dtype")
             if t.device != device:
                 _native.require_cuda(x, t)
-    c = x.shape[-1]
     if not 1 <= c <= 16384:
         raise ValueError("modulated_norm takes 1 to 16384 features")
-    if branch is not None and branch.shape != x.shape:
+    if branch is None:
+        if gate is not None or post or post_weight is not None:
+            raise ValueError("gate, post_norm and post_weight need a branch")
+    elif branch.shape != shape:
         raise ValueError("branch must have the shape of x")
-    if branch is None and (gate is not None or NORMS[post_norm] or post_weight is not None):
-        raise ValueError("gate, post_norm and post_weight need a branch")
-    if post_weight is not None and not NORMS[post_norm]:
+    if post_weight is not None and not post:
         raise ValueError("post_weight needs a post_norm")
-    samples = x.shape[0] if x.dim() >= 3 else 1
-    for name, t in (("gate", gate), ("scale", scale), ("shift", shift)):
-        if t is not None and tuple(t.shape) not in ((c,), (samples, c), (samples, 1, c)):
-            raise ValueError(f"{name} must be [{c}] or one row for each of the {samples} samples, got {list(t.shape)}")
-    for name, t in (("weight", weight), ("post_weight", post_weight)):
-        if t is not None and tuple(t.shape) != (c,):
-            raise ValueError(f"{name} must be [{c}]")
-    if not eps >= 0 or not abs(residual_scale) < float("inf"):
+    for t in (gate, scale, shift):
+        if t is not None:
+            v = t.shape
+            if v != (samples, c) and v != (c,) and v != (samples, 1, c):
+                raise ValueError(f"gate, scale and shift must be [{c}] or one row for each of the {samples} samples, "
+                                 f"got {list(v)}")
+    for t in (weight, post_weight):
+        if t is not None and t.shape != (c,):
+            raise ValueError(f"weight and post_weight must be [{c}]")
+    if not eps >= 0 or not abs(residual_scale) < math.inf:
         raise ValueError("eps must be nonnegative and residual_scale finite")
 
 

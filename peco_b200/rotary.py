@@ -12,6 +12,7 @@ enqueued on the current stream.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 from typing import Optional
@@ -25,82 +26,100 @@ _Ints = [ctypes.c_int * i for i in range(5)]
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 
 
-def _check(q, k, axes, theta, grid, positions):
+@functools.lru_cache(maxsize=256)
+def _sections(axes, d):
+    """The checked section sizes as a C array."""
+    sizes = tuple(int(a) for a in axes)
+    if not 1 <= len(sizes) <= 4 or any(a < 0 or a % 2 for a in sizes) or sum(sizes) > d:
+        raise ValueError("axes must be one to four even section sizes that fit the head dimension")
+    return _Ints[len(sizes)](*sizes)
+
+
+@functools.lru_cache(maxsize=256)
+def _grid(grid, n_axes):
+    """(the token grid as a C array, its number of tokens)."""
+    sizes = tuple(int(s) for s in grid)
+    if len(sizes) != n_axes or any(s < 0 for s in sizes):
+        raise ValueError("grid must have one size per axis")
+    return _Ints[n_axes](*sizes), math.prod(sizes)
+
+
+def _run(q, k, axes, theta, grid, positions, interleaved, inverse, inplace):
     if not isinstance(q, torch.Tensor) or q.dim() != 4:
         raise ValueError("Expected q [B, H, N, D]")
     b, _, n, d = q.shape
-    if q.dtype not in _native.DTYPE_CODE:
+    dtype, device = q.dtype, q.device
+    code = _native.DTYPE_CODE.get(dtype)
+    if code is None:
         raise TypeError("rotate takes float16, bfloat16 or float32 tensors")
     if k is not None:
         if k.dim() != 4 or (k.shape[0], k.shape[2], k.shape[3]) != (b, n, d):
             raise ValueError("q and k must agree in batch, tokens and head dimension")
-        if k.dtype != q.dtype:
+        if k.dtype is not dtype:
             raise TypeError("q and k must have one dtype")
     if d % 2 or not 2 <= d <= 256:
         raise ValueError("the head dimension must be even and at most 256")
-    axes = tuple(int(a) for a in axes)
-    if not 1 <= len(axes) <= 4 or any(a < 0 or a % 2 for a in axes) or sum(axes) > d:
-        raise ValueError("axes must be one to four even section sizes that fit the head dimension")
+    sections = _sections(tuple(axes), d)
+    a = len(sections)
     if not (theta > 0 and math.isfinite(theta)):
         raise ValueError("theta must be positive")
     if (grid is None) == (positions is None):
         raise ValueError("give either grid or positions")
+    pos_p = pos_sb = pos_sn = pos_type = 0
+    grid_c = None
     if grid is not None:
-        grid = tuple(int(s) for s in grid)
-        if len(grid) != len(axes) or any(s < 0 for s in grid):
-            raise ValueError("grid must have one size per axis")
-        turned = math.prod(grid)
+        grid_c, turned = _grid(tuple(grid), a)
     else:
         if positions.dtype not in _POSITION_TYPES:
             raise TypeError("positions must be int32, int64 or float32")
-        if positions.dim() not in (2, 3) or positions.shape[-1] != len(axes) or \
+        if positions.dim() not in (2, 3) or positions.shape[-1] != a or \
                 positions.dim() == 3 and positions.shape[0] not in (1, b):
             raise ValueError("positions must be [tokens, axes] or [B, tokens, axes]")
         turned = positions.shape[-2]
     if turned > n:
         raise ValueError(f"{turned} positions for {n} tokens")
-    if q.device.type != "cuda":
+    if device.type != "cuda":
         _native.require_cuda(q)
     for t in (k, positions):
-        if t is not None and t.device != q.device:
+        if t is not None and t.device != device:
             _native.require_cuda(q, t)
-    return axes, grid, turned
-
-
-def _run(q, k, axes, theta, grid, positions, interleaved, inverse, inplace):
-    axes, grid, turned = _check(q, k, axes, theta, grid, positions)
-    b, _, n, d = q.shape
-    sources, outs, strides = [], [], []
-    for t in (q, k):
-        if t is None:
-            sources.append(None), outs.append(None), strides.append(None)
-            continue
-        if inplace and (t.stride(3) != 1 or any(s == 0 for s, m in zip(t.stride(), t.shape) if m > 1)):
-            raise ValueError("inplace needs adjacent head dimensions and no expanded axes")
-        src = t if t.stride(3) == 1 else t.contiguous()
-        out = t if inplace else torch.empty_like(src)  # keeps a dense layout (token-major views stay so)
-        if out.stride(3) != 1 and d > 1:
-            out = torch.empty(src.shape, dtype=src.dtype, device=src.device)
-        sources.append(src), outs.append(out)
-        strides.append(_Strides(*src.stride()[:3], *out.stride()[:3]))
-    pos_sb = pos_sn = pos_type = 0
     if positions is not None:
-        if positions.stride(-1) != 1 and len(axes) > 1:
+        if positions.stride(-1) != 1 and a > 1:
             positions = positions.contiguous()
         pos_type, pos_sn = _POSITION_TYPES[positions.dtype], positions.stride(-2)
         pos_sb = positions.stride(0) if positions.dim() == 3 and positions.shape[0] > 1 else 0
+        pos_p = positions.data_ptr()
         if turned == 0:
-            positions, grid = None, (0,) * len(axes)
-    args = []
-    for src, out, st in zip(sources, outs, strides):
-        args += [0, 0, 0, None] if src is None else [src.data_ptr(), out.data_ptr(), src.shape[1], st]
-    a = len(axes)
-    _native.enqueue(q.device, "peco_rotary", _native.load().peco_rotary,
-                    (*args, b, n, turned, d, _Ints[a](*axes), a, theta,
-                     _Ints[a](*grid) if grid is not None else None, _native.address(positions), pos_sb, pos_sn,
-                     pos_type, int(bool(interleaved)), int(bool(inverse)), _native.DTYPE_CODE[q.dtype]),
-                    (*sources, positions))
-    return outs
+            pos_p, grid_c = 0, _grid((0,) * a, a)[0]
+    q, q_out, q_args = _source(q, d, inplace)
+    k_out, k_args = None, (0, 0, 0, None)
+    if k is not None:
+        k, k_out, k_args = _source(k, d, inplace)
+    _native.enqueue(device, "peco_rotary", _native.load().peco_rotary,
+                    (*q_args, *k_args, b, n, turned, d, sections, a, theta, grid_c, pos_p, pos_sb, pos_sn, pos_type,
+                     1 if interleaved else 0, 1 if inverse else 0, code), (q, k, positions))
+    return q_out, k_out
+
+
+def _source(t, d, inplace):
+    """(readable tensor, its output, the call's arguments for the two)."""
+    st = t.stride()
+    if st[3] != 1 and d > 1:
+        if inplace:
+            raise ValueError("inplace needs adjacent head dimensions and no expanded axes")
+        t = t.contiguous()
+        st = t.stride()
+    if inplace:
+        if any(s == 0 for s, m in zip(st, t.shape) if m > 1):
+            raise ValueError("inplace needs adjacent head dimensions and no expanded axes")
+        out, so = t, st
+    else:
+        out = torch.empty_like(t)  # keeps a dense layout (token-major views stay so)
+        so = out.stride()
+        if so[3] != 1:
+            out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+            so = out.stride()
+    return t, out, (t.data_ptr(), out.data_ptr(), t.shape[1], _Strides(st[0], st[1], st[2], so[0], so[1], so[2]))
 
 
 class _Rotate(torch.autograd.Function):
@@ -138,7 +157,7 @@ def rotate(q, k=None, *, axes, theta=256.0, grid=None, positions=None, interleav
     overwrites q and k.  Returns q, or (q, k).
     """
     options = dict(axes=axes, theta=theta, grid=grid, positions=positions, interleaved=interleaved, inverse=inverse)
-    if torch.is_grad_enabled() and _native.wants_grad(q, k):
+    if torch.is_grad_enabled() and isinstance(q, torch.Tensor) and _native.wants_grad(q, k):
         if inplace:
             raise RuntimeError("rotate(inplace=True) does not record gradients; use torch.no_grad()")
         return _Rotate.apply(q, k, options)
