@@ -276,16 +276,26 @@ __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
 // per SM and K block, for twice the products of a 128 x 128 tile.
 //
 // WIDE (with CG = 2): the tile is 256 x 2 bn, both accumulators hold one half of
-// it and share A's stage.  L2 delivers about 45 bytes per clock and SM here, and
-// a 256 x 256 tile wants 64 to keep the tensor core busy; 256 x 512 wants 48.
-// The price is that a tile's epilogue no longer hides entirely: the first K
-// blocks' products go to the half that is drained first, the last ones' finish
-// that half first.
+// it and share A's stage (and A's trip from shared memory).  At the tensor
+// core's full rate a 256 x 256 tile draws 64 bytes per clock and SM from L2, a
+// 256 x 512 one 48, and long products run at the board's power limit, where
+// traffic costs time.  The price is that a tile's epilogue no longer hides
+// entirely: the first K blocks' products go to the half that is drained first,
+// the last ones' finish that half first.  Back to back for half a second each:
+// 6750 x 12288 x 3072 387 us wide and 426 not, the weight gradient of 6750 x
+// 3072 x 12288 372 and 400; but 6750 x 3072 x 12288, with four times as many
+// epilogues per product, 414 and 397.
 //
 // SPLIT: one tile per cluster of S groups, each taking a range of the K
 // blocks.  The groups' fp32 partial tiles meet in shared memory: every CTA
 // adds 128 / S rows over the S partials, in the groups' order, and finishes
 // them.
+//
+// What it measured (B200, cold weights): 1 x 3072 x 18432 25 us (4.5 TB/s of
+// weights; bound by HBM and the start of the kernel), 256 x 3072 x 12288 with
+// gelu 27 us, 6750 x 3072 x 12288 with gelu 391 us (1.30 PFLOP/s at the power
+// limit, 335 us and 1.52 PFLOP/s in short runs), 7006 x 15360 x 3072 with gate
+// and residual 546 us; bound by the tensor core and the power limit.
 constexpr int kRingBytes = 192 * 1024;
 constexpr int kMaxStages = 24;                  // stages hold what a tile needs: small ones have many in flight
 constexpr int kStageRow = 32;                    // columns an epilogue warp finishes at a time
@@ -914,6 +924,8 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const __grid_constant__ 
 }
 
 // ---- gradient of the epilogue --------------------------------------------------------
+// Bound by HBM with the arithmetic close behind: 6750 x 12288 with gelu reads g
+// and z, writes dz: 498 MB in 99 us (5.0 TB/s).
 // One block per (256 columns, chunk of one sample's rows): lane l of every
 // warp owns 8 columns, the 8 warps take every eighth row.  Writes dz and the
 // chunk's column sums of dz and of g * act(z); a second kernel adds the
@@ -1153,7 +1165,8 @@ struct TileChoice {
 
 // Estimated clocks of a choice, from what one SM does per 64-wide K block: 2
 // clocks of MMA per column of its tile (128 rows x 16 take half a clock a
-// column), or its operand rows' 128 bytes at 50 bytes a clock, whichever is longer; plus what a tile adds: little where
+// column), or its operand rows' 128 bytes at 50 bytes a clock (the traffic that
+// measured equal to it), whichever is longer; plus what a tile adds: little where
 // the epilogue hides under the next tile, ``exposed`` clocks a column where it
 // does not (wide), a meeting of partials (split).
 TileChoice choose_tiles(int m, int n, int kblocks, bool amn, double exposed) {

@@ -14,11 +14,13 @@
 // error does not grow with the position.
 //
 // The operator moves bytes: each element is read once and written once, and
-// the floor is that traffic at the copy bandwidth.  A thread owns one 16-byte
-// run of dimensions (eight bytes of each half in the split pairing) of one
-// token and walks the heads with it, so the sine and cosine are computed once
-// per token and head group and the loads of several heads are in flight at
-// once.
+// the floor is that traffic at the copy bandwidth.  A thread owns 16 bytes of
+// one token's row (of each half in the split pairing of 16-bit types) and walks
+// the heads with it, so the sine and cosine are computed once per token and
+// head group; the next four heads' loads are in flight while the current four
+// are turned and stored.  24 + 24 heads x 119056 tokens x 128 bf16: 452 us, 6.47
+// TB/s, the rate of a plain copy (643 us without the loads ahead, 473 / 461 /
+// 522 / 489 us with 2 / 3 / 6 / 8 heads at a time).
 #include "common.cuh"
 #include "../../include/peco_b200.h"
 #include "internal.h"

@@ -16,6 +16,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native
 
@@ -171,6 +172,7 @@ class _LinearAct(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         x, weight, gate, x2, preact = ctx.saved_tensors
         need = ctx.needs_input_grad

@@ -19,6 +19,7 @@ import math
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native
 
@@ -144,6 +145,7 @@ class _ModulatedNorm(torch.autograd.Function):
         return normed if residual is None else (residual, normed)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, *grads):
         x = ctx.saved_tensors[0]
         dr, dh = grads if len(grads) == 2 else (None, grads[0])

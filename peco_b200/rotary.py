@@ -18,6 +18,7 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native
 
@@ -131,6 +132,7 @@ class _Rotate(torch.autograd.Function):
         return q if k is None else (q, k)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, *grads):
         back = dict(ctx.options, inverse=not ctx.options["inverse"])
         gq, gk = (*grads, None)[:2]
