@@ -7,4 +7,5 @@ Python signatures over a C-ABI shared library, ``libpeco_b200.so``, built from
 importing the package never needs a GPU.
 """
 
-__all__ = ["processor", "clustering", "quantization", "clustering_cuda", "attention_cuda", "synthetic"]
+__all__ = ["processor", "clustering", "quantization", "clustering_cuda", "attention_cuda", "synthetic",
+           "linear", "norms", "rotary"]
