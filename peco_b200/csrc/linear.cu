@@ -65,7 +65,12 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGelu1 = 2.0f * 0.7978845608028654f;  // 2u = z (kGelu1 + kGelu3 z^2)
 constexpr float kGelu3 = kGelu1 * 0.044715f;
 
-__device__ __forceinline__ float recip_approx(float x) { return __fdividef(1.0f, x); }
+// 1 / x from the hardware's approximate reciprocal (within an ulp; infinity gives 0)
+__device__ __forceinline__ float recip_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 // z Phi(z) of a pair.  With x = |z| / sqrt 2 and t = 1 / (1 + p x), erfc(x) is a
 // polynomial in t times exp(-x^2) (Abramowitz and Stegun, Handbook of
@@ -660,6 +665,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
   __syncthreads();
   if (CG > 1) cluster_sync();  // the pair's barriers are ready before either CTA signals the other
   tc_fence_after();
+  // The launch may overlap the end of the kernel before it in the stream (its
+  // memory is not touched up to here); a kernel after it may do the same.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = sh.tmem;
   const int tiles = args.tiles_m * args.tiles_n;
   const int kb0 = args.kblocks[0], kblocks = kb0 + args.kblocks[1];
@@ -1211,12 +1220,14 @@ int launch_tiles(const GemmArgs& g, int splits, cudaStream_t stream) {
   cfg.blockDim = dim3(kGemmThreads);
   cfg.dynamicSmemBytes = kGemmSmem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = CG * splits;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   e = cudaLaunchKernelEx(&cfg, kernel, g, splits);
   const int st = launch_status();
   return e != cudaSuccess ? static_cast<int>(e) : st;
