@@ -128,6 +128,10 @@ def stream_of(device: torch.device, *tensors: torch.Tensor) -> P:
     return P(s.cuda_stream)
 
 
+# torch.cuda.current_stream / current_device without their argument handling
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _STREAMS = {}  # (device index, raw stream) -> torch stream object
 
 
@@ -137,14 +141,15 @@ def enqueue(device: torch.device, what: str, fn, args, inputs) -> None:
     the caller's tensors (None skipped): their memory stays theirs until the
     stream has consumed it.  Buffers that were allocated for this call belong to
     the stream already."""
-    raw = torch._C._cuda_getCurrentRawStream(device.index)
-    stream = _STREAMS.get((device.index, raw))
+    index = device.index
+    raw = _raw_stream(index)
+    stream = _STREAMS.get((index, raw))
     if stream is None:  # building the stream object costs more than the look-up
-        stream = _STREAMS[device.index, raw] = torch.cuda.current_stream(device)
+        stream = _STREAMS[index, raw] = torch.cuda.current_stream(device)
     for t in inputs:
         if t is not None:
             t.record_stream(stream)
-    if device.index == torch._C._cuda_getDevice():
+    if index == _current_device():
         status = fn(*args, raw)
     else:
         with torch.cuda.device(device):

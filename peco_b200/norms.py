@@ -113,25 +113,48 @@ def _check(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, 
 
 def _forward(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, eps, post_eps, residual_scale):
     _check(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, eps, residual_scale)
-    c = x.shape[-1]
-    normed = x.new_empty(x.shape)
-    residual = x.new_empty(x.shape) if branch is not None else None
-    samples, rows = _extent(x)
-    if samples * rows == 0:
-        return residual, normed
-    x3, xb, xr = _rows(x, samples, rows, c)
-    b3, bb, br = _rows(branch, samples, rows, c)
-    gate, gb = _vec(gate, c)
-    scale, sb = _vec(scale, c)
-    shift, tb = _vec(shift, c)
-    weight = None if weight is None else weight.contiguous()
-    post_weight = None if post_weight is None else post_weight.contiguous()
-    addr = _native.address
+    shape = x.shape
+    c = shape[-1]
+    normed = torch.empty_like(x, memory_format=torch.contiguous_format)
+    residual = None
+    samples = shape[0] if len(shape) >= 3 else 1
+    size = x.numel()
+    if size == 0:
+        return (None if branch is None else torch.empty_like(normed)), normed
+    rows = size // (c * samples)
+    xp = xb = xr = bp = bb = br = gp = gb = sp = sb = tp = tb = wp = pp = rp = 0
+    if x.is_contiguous():
+        xb, xr = rows * c, c
+    else:
+        x, xb, xr = _rows(x, samples, rows, c)
+    xp = x.data_ptr()
+    if branch is not None:
+        if branch.is_contiguous():
+            bb, br = rows * c, c
+        else:
+            branch, bb, br = _rows(branch, samples, rows, c)
+        bp = branch.data_ptr()
+        residual = torch.empty_like(normed)
+        rp = residual.data_ptr()
+    if gate is not None:
+        gate, gb = _vec(gate, c)
+        gp = gate.data_ptr()
+    if scale is not None:
+        scale, sb = _vec(scale, c)
+        sp = scale.data_ptr()
+    if shift is not None:
+        shift, tb = _vec(shift, c)
+        tp = shift.data_ptr()
+    if weight is not None:
+        weight = weight.contiguous()
+        wp = weight.data_ptr()
+    if post_weight is not None:
+        post_weight = post_weight.contiguous()
+        pp = post_weight.data_ptr()
     _native.enqueue(x.device, "peco_gated_norm", _native.load().peco_gated_norm,
-                    (x3.data_ptr(), xb, xr, addr(b3), bb, br, addr(gate), gb, addr(scale), sb, addr(shift), tb,
-                     addr(weight), addr(post_weight), addr(residual), normed.data_ptr(), samples, rows, c,
+                    (xp, xb, xr, bp, bb, br, gp, gb, sp, sb, tp, tb, wp, pp, rp, normed.data_ptr(), samples, rows, c,
                      NORMS[norm], NORMS[post_norm], eps, eps if post_eps is None else post_eps, residual_scale,
-                     _native.DTYPE_CODE[x.dtype]), (x3, b3, gate, scale, shift, weight, post_weight))
+                     _native.DTYPE_CODE[x.dtype]), (x, branch, gate, scale, shift, weight, post_weight))
     return residual, normed
 
 
@@ -169,11 +192,11 @@ def modulated_norm(x, branch=None, *, gate=None, scale=None, shift=None, weight=
     variance) or "rms"; ``post_eps`` defaults to ``eps``.  Absent parts drop out
     of the formulas.
     """
-    options = dict(norm=norm, post_norm=post_norm, eps=eps, post_eps=post_eps, residual_scale=residual_scale)
-    inputs = (x, branch, gate, scale, shift, weight, post_weight)
-    if torch.is_grad_enabled() and _native.wants_grad(*inputs):
-        return _ModulatedNorm.apply(*inputs, options)
-    residual, normed = _forward(*inputs, **options)
+    if torch.is_grad_enabled() and _native.wants_grad(x, branch, gate, scale, shift, weight, post_weight):
+        options = dict(norm=norm, post_norm=post_norm, eps=eps, post_eps=post_eps, residual_scale=residual_scale)
+        return _ModulatedNorm.apply(x, branch, gate, scale, shift, weight, post_weight, options)
+    residual, normed = _forward(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, eps, post_eps,
+                                residual_scale)
     return normed if residual is None else (residual, normed)
 
 
