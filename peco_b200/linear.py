@@ -212,41 +212,53 @@ def linear_act_backward(grad, x, weight, *, preact=None, activation=None, gate=N
     of x, x2, weight, bias, gate that are there).
     """
     k, k2, n, samples = _check(x, weight, None, gate, grad, x2, activation)
-    there = [name for name, t in (("x", x), ("x2", x2), ("weight", weight), ("bias", bias or None), ("gate", gate))
-             if t is not None]
-    needs = there if needs is None else list(needs)
-    if any(name not in there for name in needs):
-        raise ValueError(f"needs must name gradients among {there}, got {needs}")
-    shapes = {"x": x.shape, "x2": None if x2 is None else x2.shape, "weight": weight.shape, "bias": (n,),
-              "gate": None if gate is None else gate.shape}
+    if needs is None:
+        want_x, want_x2, want_w, want_b, want_g = True, x2 is not None, True, bool(bias), gate is not None
+    else:
+        want_x, want_x2, want_w, want_b, want_g = (name in needs for name in LinearGrads._fields)
+        if len(set(needs) - set(LinearGrads._fields)) or want_x2 and x2 is None or want_b and not bias or \
+                want_g and gate is None:
+            raise ValueError(f"needs must name gradients of inputs that are there, got {list(needs)}")
+    dx = x.new_empty(x.shape) if want_x else None
+    dx2 = x.new_empty(x2.shape) if want_x2 else None
+    dw = x.new_empty((n, k + k2)) if want_w else None
+    db = x.new_empty((n,)) if want_b else None
+    dg = x.new_empty(gate.shape) if want_g else None
     rows = grad.numel() // n
     if rows == 0:
-        return LinearGrads(**{f: torch.zeros(shapes[f], dtype=x.dtype, device=x.device) if f in needs else None
-                              for f in LinearGrads._fields})
+        return LinearGrads(*(None if t is None else t.zero_() for t in (dx, dx2, dw, db, dg)))
     act = ACTIVATIONS[activation]
-    if act or "gate" in needs:
+    preact_p = 0
+    if act or want_g:
         if preact is None:
             raise ValueError("this gradient needs the saved pre-activation (preact)")
         if preact.numel() != rows * n or preact.shape[-1] != n or preact.dtype != x.dtype:
             raise ValueError("preact must be the output-shaped pre-activation of the same dtype")
-        _native.require_cuda(x, preact)
-        preact = preact.reshape(rows, n).contiguous()
+        if preact.device != x.device:
+            _native.require_cuda(x, preact)
+        preact = preact.contiguous()
+        preact_p = preact.data_ptr()
     else:
         preact = None
-    outs = {f: x.new_empty(shapes[f]) if f in needs else None for f in LinearGrads._fields}
     grad, grad_step = _rows(grad, n)
     x, x_step = _rows(x, k)
-    x2, x2_step = (None, 0) if x2 is None else _rows(x2, k2)
-    gate, g_step = (None, 0) if gate is None else _gate_rows(gate, n, samples)
+    x2p = x2_step = gp = g_step = 0
+    if x2 is not None:
+        x2, x2_step = _rows(x2, k2)
+        x2p = x2.data_ptr()
+    if gate is not None:
+        gate, g_step = _gate_rows(gate, n, samples)
+        gp = gate.data_ptr()
     weight, w_step = _weight_rows(weight)
     lib = _native.load()
     addr = _native.address
-    operands = (x.data_ptr(), x_step, addr(x2), x2_step, weight.data_ptr(), w_step)
+    grad_p = grad.data_ptr()
+    operands = (x.data_ptr(), x_step, x2p, x2_step, weight.data_ptr(), w_step)
     sizes = (samples, rows // samples, k, k2, n, act)
-    need = int(lib.peco_linear_backward_workspace(grad.data_ptr(), grad_step, *operands, *sizes, int(gate is not None)))
+    need = int(lib.peco_linear_backward_workspace(grad_p, grad_step, *operands, *sizes, 1 if gp else 0))
     ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need > 0 else None
     _native.enqueue(x.device, "peco_linear_backward", lib.peco_linear_backward,
-                    (grad.data_ptr(), grad_step, addr(preact), *operands, addr(gate), g_step,
-                     *(addr(outs[f]) for f in ("x", "x2", "weight", "bias", "gate")), *sizes,
-                     _native.DTYPE_CODE[x.dtype], addr(ws), max(need, 0)), (grad, preact, x, x2, weight, gate))
-    return LinearGrads(**outs)
+                    (grad_p, grad_step, preact_p, *operands, gp, g_step, addr(dx), addr(dx2), addr(dw), addr(db),
+                     addr(dg), *sizes, _native.DTYPE_CODE[x.dtype], addr(ws), max(need, 0)),
+                    (grad, preact, x, x2, weight, gate))
+    return LinearGrads(dx, dx2, dw, db, dg)

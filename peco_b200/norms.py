@@ -206,44 +206,53 @@ def modulated_norm_backward(grad_normed, grad_residual, x, branch=None, *, gate=
     """Gradients of ``modulated_norm`` for ``grad_normed`` = d h and
     ``grad_residual`` = d r (None: zero).  ``needs``: names of the gradients to
     compute (default: those of all inputs that are there)."""
-    inputs = dict(zip(NormGrads._fields, (x, branch, gate, scale, shift, weight, post_weight)))
-    _check(*inputs.values(), norm, post_norm, eps, residual_scale)
-    for name, t in (("grad_normed", grad_normed), ("grad_residual", grad_residual)):
-        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
-            raise ValueError(f"{name} must have the shape and dtype of x")
+    _check(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, eps, residual_scale)
     if grad_normed is None:
         raise ValueError("grad_normed is required")
+    shape, dtype, device = x.shape, x.dtype, x.device
+    for t in (grad_normed, grad_residual):
+        if t is not None:
+            if t.shape != shape or t.dtype is not dtype:
+                raise ValueError("grad_normed and grad_residual must have the shape and dtype of x")
+            if t.device != device:
+                _native.require_cuda(x, t)
     if grad_residual is not None and branch is None:
         raise ValueError("grad_residual needs a branch")
-    _native.require_cuda(*[t for t in (x, grad_normed, grad_residual) if t is not None])
-    needs = [n for n, t in inputs.items() if t is not None] if needs is None else list(needs)
-    if any(inputs.get(n) is None for n in needs):
-        raise ValueError("needs names a gradient whose input is absent")
-    if x.numel() == 0:
-        return NormGrads(**{n: torch.zeros(t.shape, dtype=x.dtype, device=x.device) if n in needs else None
-                            for n, t in inputs.items()})
-    grads = {n: x.new_empty(t.shape) if n in needs else None for n, t in inputs.items()}
-    c = x.shape[-1]
+    inputs = (x, branch, gate, scale, shift, weight, post_weight)
+    if needs is None:
+        grads = [None if t is None else x.new_empty(t.shape) for t in inputs]
+    else:
+        if any(n not in NormGrads._fields or inputs[NormGrads._fields.index(n)] is None for n in needs):
+            raise ValueError("needs names a gradient whose input is absent")
+        grads = [x.new_empty(t.shape) if n in needs else None for n, t in zip(NormGrads._fields, inputs)]
     samples, rows = _extent(x)
+    if samples * rows == 0:
+        return NormGrads(*(None if g is None else g.zero_() for g in grads))
+    c = shape[-1]
     gh, ghb, ghr = _rows(grad_normed, samples, rows, c)
     gr, grb, grr = _rows(grad_residual, samples, rows, c)
-    x3, xb, xr = _rows(x, samples, rows, c)
-    b3, bb, br = _rows(branch, samples, rows, c)
+    x, xb, xr = _rows(x, samples, rows, c)
+    branch, bb, br = _rows(branch, samples, rows, c)
     # a vector without a sample axis sums its gradient over the samples
-    shared = sum(bit for bit, t in ((1, gate), (2, scale), (4, shift)) if t is not None and t.dim() == 1)
-    (gv, gb), (sv, sb) = _vec(gate, c), _vec(scale, c)
-    weight, post_weight = (None if t is None else t.contiguous() for t in (weight, post_weight))
+    shared = (1 if gate is not None and gate.dim() == 1 else 0) | (2 if scale is not None and scale.dim() == 1 else 0) | \
+        (4 if shift is not None and shift.dim() == 1 else 0)
+    gate, gb = _vec(gate, c)
+    scale, sb = _vec(scale, c)
+    if weight is not None:
+        weight = weight.contiguous()
+    if post_weight is not None:
+        post_weight = post_weight.contiguous()
     lib = _native.load()
-    dev, addr = x.device, _native.address
     need, ws = 0, None
-    if any(n in needs for n in NormGrads._fields[2:]):
+    if any(g is not None for g in grads[2:]):
         need = int(lib.peco_gated_norm_backward_workspace(samples, rows, c))
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    _native.enqueue(dev, "peco_gated_norm_backward", lib.peco_gated_norm_backward,
-                    (addr(gh), ghb, ghr, addr(gr), grb, grr, addr(x3), xb, xr, addr(b3), bb, br, addr(gv), gb, addr(sv),
-                     sb, addr(weight), addr(post_weight),
-                     *(addr(grads[n]) for n in ("x", "branch", "gate", "scale", "shift")), shared,
-                     addr(grads["weight"]), addr(grads["post_weight"]), samples, rows, c, NORMS[norm],
-                     NORMS[post_norm], eps, eps if post_eps is None else post_eps, residual_scale,
-                     _native.DTYPE_CODE[x.dtype], addr(ws), need), (gh, gr, x3, b3, gv, sv, weight, post_weight))
-    return NormGrads(**grads)
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+    addr = _native.address
+    _native.enqueue(device, "peco_gated_norm_backward", lib.peco_gated_norm_backward,
+                    (gh.data_ptr(), ghb, ghr, addr(gr), grb, grr, x.data_ptr(), xb, xr, addr(branch), bb, br, addr(gate),
+                     gb, addr(scale), sb, addr(weight), addr(post_weight), addr(grads[0]), addr(grads[1]),
+                     addr(grads[2]), addr(grads[3]), addr(grads[4]), shared, addr(grads[5]), addr(grads[6]), samples,
+                     rows, c, NORMS[norm], NORMS[post_norm], eps, eps if post_eps is None else post_eps, residual_scale,
+                     _native.DTYPE_CODE[dtype], addr(ws), need),
+                    (gh, gr, x, branch, gate, scale, weight, post_weight))
+    return NormGrads(*grads)
