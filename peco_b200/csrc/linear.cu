@@ -665,10 +665,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
   __syncthreads();
   if (CG > 1) cluster_sync();  // the pair's barriers are ready before either CTA signals the other
   tc_fence_after();
-  // The launch may overlap the end of the kernel before it in the stream (its
-  // memory is not touched up to here); a kernel after it may do the same.
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  wait_for_prior();
+  let_next_start();
   const uint32_t tmem = sh.tmem;
   const int tiles = args.tiles_m * args.tiles_n;
   const int kb0 = args.kblocks[0], kblocks = kb0 + args.kblocks[1];
@@ -982,6 +980,8 @@ __device__ __forceinline__ void store_pairs(T* p, int count, const float2 (&v)[4
 template <typename T, int ACT, bool GATE, bool VEC>
 __global__ void __launch_bounds__(256, GATE ? 3 : 4) act_backward_kernel(const __grid_constant__ ActBackwardArgs a) {
   __shared__ float red[GATE ? 2 : 1][8][256];
+  wait_for_prior();
+  let_next_start();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sample = blockIdx.y / a.chunks, chunk = blockIdx.y - sample * a.chunks;
   const int col = blockIdx.x * 256 + lane * 8;
@@ -1063,6 +1063,8 @@ template <typename T>
 __global__ void __launch_bounds__(256) act_backward_sums_kernel(const float* part_bias, const float* part_gate,
                                                                 T* dbias, T* dgate, int samples, int chunks, int n) {
   __shared__ float red[2][8][33];
+  wait_for_prior();
+  let_next_start();
   const int cx = threadIdx.x & 31, y = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + cx;
   float total = 0.0f;
@@ -1215,22 +1217,8 @@ int launch_tiles(const GemmArgs& g, int splits, cudaStream_t stream) {
   cudaError_t e = grant_smem(reinterpret_cast<const void*>(kernel), kGemmSmem, opened);
   if (e != cudaSuccess) return static_cast<int>(e);
   const int tiles = g.tiles_m * g.tiles_n, most = kNumSMs / CG;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(SPLIT ? tiles * CG * splits : (tiles < most ? tiles : most) * CG);
-  cfg.blockDim = dim3(kGemmThreads);
-  cfg.dynamicSmemBytes = kGemmSmem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG * splits;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  e = cudaLaunchKernelEx(&cfg, kernel, g, splits);
-  const int st = launch_status();
-  return e != cudaSuccess ? static_cast<int>(e) : st;
+  const unsigned grid = SPLIT ? tiles * CG * splits : (tiles < most ? tiles : most) * CG;
+  return launch_overlapped(kernel, dim3(grid), dim3(kGemmThreads), kGemmSmem, CG * splits, stream, g, splits);
 }
 
 template <typename T, bool AMN, bool BMN, bool EPI>
@@ -1337,11 +1325,11 @@ BackwardPlan plan_backward(const LinearShape& s, const Operand& grad, bool has_g
 }
 
 template <typename T, int ACT>
-void launch_act_backward(const ActBackwardArgs& a, dim3 grid, cudaStream_t stream) {
-  if (a.gate && a.vec) act_backward_kernel<T, ACT, true, true><<<grid, 256, 0, stream>>>(a);
-  else if (a.gate) act_backward_kernel<T, ACT, true, false><<<grid, 256, 0, stream>>>(a);
-  else if (a.vec) act_backward_kernel<T, ACT, false, true><<<grid, 256, 0, stream>>>(a);
-  else act_backward_kernel<T, ACT, false, false><<<grid, 256, 0, stream>>>(a);
+int launch_act_backward(const ActBackwardArgs& a, dim3 grid, cudaStream_t stream) {
+  if (a.gate && a.vec) return launch_overlapped(act_backward_kernel<T, ACT, true, true>, grid, dim3(256), 0, 0, stream, a);
+  if (a.gate) return launch_overlapped(act_backward_kernel<T, ACT, true, false>, grid, dim3(256), 0, 0, stream, a);
+  if (a.vec) return launch_overlapped(act_backward_kernel<T, ACT, false, true>, grid, dim3(256), 0, 0, stream, a);
+  return launch_overlapped(act_backward_kernel<T, ACT, false, false>, grid, dim3(256), 0, 0, stream, a);
 }
 
 template <typename T>
@@ -1372,17 +1360,16 @@ int backward(const LinearShape& s, Operand grad, const void* preact, Operand (&x
     a.act = s.act;
     a.vec = s.n % 8 == 0 && aligned16(grad.ptr, grad.stride) && aligned16(a.preact, s.n) && aligned16(gate, gate_stride);
     const dim3 grid((s.n + 255) / 256, s.samples * p.chunks);
-    switch (s.act) {
-      case kActGeluTanh: launch_act_backward<T, kActGeluTanh>(a, grid, stream); break;
-      case kActGelu: launch_act_backward<T, kActGelu>(a, grid, stream); break;
-      case kActSilu: launch_act_backward<T, kActSilu>(a, grid, stream); break;
-      default: launch_act_backward<T, kActNone>(a, grid, stream);
-    }
-    if (int st = launch_status()) return st;
+    const int st = s.act == kActGeluTanh ? launch_act_backward<T, kActGeluTanh>(a, grid, stream)
+                   : s.act == kActGelu   ? launch_act_backward<T, kActGelu>(a, grid, stream)
+                   : s.act == kActSilu   ? launch_act_backward<T, kActSilu>(a, grid, stream)
+                                         : launch_act_backward<T, kActNone>(a, grid, stream);
+    if (st) return st;
     if (p.sums) {
-      act_backward_sums_kernel<T><<<(s.n + 31) / 32, 256, 0, stream>>>(
-          a.part_bias, a.part_gate, static_cast<T*>(dbias), static_cast<T*>(dgate), s.samples, p.chunks, s.n);
-      if (int st = launch_status()) return st;
+      const int sums = launch_overlapped(act_backward_sums_kernel<T>, dim3((s.n + 31) / 32), dim3(256), 0, 0, stream,
+                                         a.part_bias, a.part_gate, static_cast<T*>(dbias), static_cast<T*>(dgate),
+                                         s.samples, p.chunks, s.n);
+      if (sums) return sums;
     }
   }
   Operand* list[4];

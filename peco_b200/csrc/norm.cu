@@ -357,6 +357,8 @@ __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS) norm_forward_ker
   static_assert(WARPS == 1 || WARPS >= 4, "rows of two warps would share block barriers");
   constexpr int kThreads = 32 * WARPS;
   constexpr unsigned kRows = WARPS < 4 ? 4 / WARPS : 1;
+  wait_for_prior();
+  let_next_start();
   __shared__ float4 buf[2][2][WARPS];  // alternates between rows: a row's last read may meet the next one's write
   const int slot = threadIdx.x / kThreads;
   const Span<WARPS, NCH, MODE> sp{static_cast<int>(threadIdx.x) - slot * kThreads, a.width};
@@ -484,6 +486,8 @@ __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS) norm_forward_ker
 template <typename T, int WARPS, int NCH, int BLOCKS, int MODE, bool POST>
 __global__ void __launch_bounds__(32 * WARPS, BLOCKS) norm_backward_kernel(const __grid_constant__ NormArgs a) {
   constexpr int kThreads = 32 * WARPS;
+  wait_for_prior();
+  let_next_start();
   __shared__ float4 buf[2][3][WARPS];  // alternates between rows: a row's last read may meet the next one's write
   const unsigned sample = blockIdx.x / a.chunks, chunk = blockIdx.x - sample * a.chunks;
   const Span<WARPS, NCH, MODE> sp{static_cast<int>(threadIdx.x), a.width};
@@ -693,6 +697,8 @@ struct NormSumsArgs {
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_sums_kernel(const __grid_constant__ NormSumsArgs a) {
   __shared__ float red[32][33];
+  wait_for_prior();
+  let_next_start();
   const int cx = threadIdx.x & 31, y = threadIdx.x >> 5, k = blockIdx.y;
   const int c = blockIdx.x * 32 + cx;
   void* each = k == 0 ? a.dshift : k == 1 ? a.dscale : a.dgate;      // one vector per sample, or their sum
@@ -779,8 +785,7 @@ int launch_backward_mode(NormArgs a, cudaStream_t stream) {
     const cudaError_t e = grant_smem(reinterpret_cast<const void*>(kernel), kRingBudget, opened);
     if (e != cudaSuccess) return static_cast<int>(e);
   }
-  kernel<<<a.samples * a.chunks, 32 * WARPS, smem, stream>>>(a);
-  return launch_status();
+  return launch_overlapped(kernel, dim3(a.samples * a.chunks), dim3(32 * WARPS), smem, 0, stream, a);
 }
 
 template <typename T, int WARPS, int NCH, int BLOCKS, bool POST>
@@ -809,8 +814,7 @@ int launch_forward_mode(NormArgs a, cudaStream_t stream) {
   }
   const long long want = (static_cast<long long>(a.samples) * a.rows + kRows - 1) / kRows;
   const long long most = static_cast<long long>(kNumSMs) * blocks;
-  kernel<<<static_cast<unsigned>(want < most ? want : most), kBlock, smem, stream>>>(a);
-  return launch_status();
+  return launch_overlapped(kernel, dim3(static_cast<unsigned>(want < most ? want : most)), dim3(kBlock), smem, 0, stream, a);
 }
 
 template <typename T, int WARPS, int NCH, bool POST>
@@ -990,7 +994,6 @@ extern "C" int peco_gated_norm_backward(
   s.chunks = a.chunks;
   s.width = width;
   const dim3 grid((width + 31) / 32, 3);
-  if (dtype == 1) norm_sums_kernel<__nv_bfloat16><<<grid, 1024, 0, stream>>>(s);
-  else norm_sums_kernel<__half><<<grid, 1024, 0, stream>>>(s);
-  return launch_status();
+  return dtype == 1 ? launch_overlapped(norm_sums_kernel<__nv_bfloat16>, grid, dim3(1024), 0, 0, stream, s)
+                    : launch_overlapped(norm_sums_kernel<__half>, grid, dim3(1024), 0, 0, stream, s);
 }

@@ -137,6 +137,8 @@ struct alignas(16) Run {
 // never share memory).
 template <typename T, int V, bool SPLIT, int HEADS>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryArgs a) {
+  wait_for_prior();
+  let_next_start();
   const int slot = threadIdx.x / a.units, unit = threadIdx.x - slot * a.units;
   const int batch = blockIdx.x / a.token_blocks;
   const int token = (blockIdx.x - batch * a.token_blocks) * a.tokens_per_block + slot;
@@ -231,8 +233,7 @@ int launch_form(RotaryArgs& a, int batch, cudaStream_t stream) {
   if (groups > heads) groups = heads;
   a.heads_per_block = static_cast<int>((heads + groups - 1) / groups);
   const dim3 grid(static_cast<unsigned>(blocks), (heads + a.heads_per_block - 1) / a.heads_per_block);
-  rotary_kernel<T, V, SPLIT, HEADS><<<grid, kThreads, 0, stream>>>(a);
-  return launch_status();
+  return launch_overlapped(rotary_kernel<T, V, SPLIT, HEADS>, grid, dim3(kThreads), 0, 0, stream, a);
 }
 
 // Whether every row's runs of V pairs start on the boundaries that V needs.

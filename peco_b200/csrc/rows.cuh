@@ -91,4 +91,32 @@ __device__ __forceinline__ void store_vec(T* p, int vec, int count, const float 
   }
 }
 
+// A kernel that may be launched while the one before it in the stream is still
+// ending touches no memory before wait_for_prior(); one that lets the next such
+// kernel come early says so with let_next_start() (the next one still waits for
+// all of it).
+__device__ __forceinline__ void wait_for_prior() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Launch of a kernel that begins with wait_for_prior().
+template <typename... P, typename... A>
+int launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 0 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+  const int st = launch_status();
+  return e != cudaSuccess ? static_cast<int>(e) : st;
+}
+
 }  // namespace peco
