@@ -92,20 +92,6 @@ __device__ __forceinline__ float2 gelu_pair(float2 z) {
   return fmul2(z, p);
 }
 
-template <int ACT>
-__device__ __forceinline__ float activate(float z) {
-  if constexpr (ACT == kActGeluTanh) {
-    const float w = z * fmaf(-kLog2e * kGelu3, z * z, -kLog2e * kGelu1);
-    return z * recip_approx(1.0f + exp2_approx(w));
-  } else if constexpr (ACT == kActGelu) {
-    return gelu_pair(make_float2(z, z)).x;
-  } else if constexpr (ACT == kActSilu) {
-    return z * recip_approx(1.0f + exp2_approx(-kLog2e * z));
-  } else {
-    return z;
-  }
-}
-
 // (act(z), act'(z)) of the forms that take no pairs
 template <int ACT>
 __device__ __forceinline__ float2 activate_slope(float z) {
@@ -292,22 +278,22 @@ __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
 // epilogues per product, 414 and 397.
 //
 // SPLIT: one tile per cluster of S groups, each taking a range of the K
-// blocks.  The groups' fp32 partial tiles meet in shared memory: every CTA
-// adds 128 / S rows over the S partials, in the groups' order, and finishes
-// them.
+// blocks and finishing a share of the tile's columns: the groups store their
+// fp32 partials of a share into its group's drained ring, which adds them in a
+// fixed order to its own.
 //
-// What it measured (B200, cold weights): 1 x 3072 x 18432 25 us (4.5 TB/s of
+// What it measured (B200, cold weights): 1 x 3072 x 18432 23 us (4.9 TB/s of
 // weights; bound by HBM and the start of the kernel), 256 x 3072 x 12288 with
-// gelu 27 us, 6750 x 3072 x 12288 with gelu 391 us (1.30 PFLOP/s at the power
-// limit, 335 us and 1.52 PFLOP/s in short runs), 7006 x 15360 x 3072 with gate
-// and residual 546 us; bound by the tensor core and the power limit.
+// gelu 23 us, 256 x 12288 x 3072 26 us (split), 6750 x 3072 x 12288 with gelu 378
+// us (1.35 PFLOP/s at the power limit, 335 us and 1.52 PFLOP/s in short runs),
+// 7006 x 15360 x 3072 with gate and residual 543 us; the large ones are bound by
+// the tensor core and the power limit.
 constexpr int kRingBytes = 192 * 1024;
 constexpr int kMaxStages = 24;                  // stages hold what a tile needs: small ones have many in flight
 constexpr int kStageRow = 32;                    // columns an epilogue warp finishes at a time
 constexpr int kStagingBytes = kEpilogueWarps * 32 * kStageRow * 2;
 constexpr int kVectorBytes = 2 * 2 * 256 * 4;    // bias and gate of two accumulators' columns, fp32
 constexpr int kGemmSmem = kRingBytes + kStagingBytes + kVectorBytes + 1024;  // + alignment slack
-constexpr int kMaxSplitColumns = 128;            // a split tile's fp32 partial (64 KB) fits the ring
 
 struct GemmShared {
   uint64_t full[kMaxStages], empty[kMaxStages];
@@ -363,52 +349,6 @@ struct RingPos {
   }
 };
 
-template <int ACT>
-__device__ __forceinline__ void activate_all(float (&v)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = activate<ACT>(v[i]);
-}
-
-// Epilogue and store of 8 neighbouring columns of one row; ``count`` of them
-// exist.  ``bias`` and ``res`` are the bias and the residual there.
-template <typename T, bool EPI>
-__device__ __forceinline__ void finish8(const GemmArgs& args, float (&v)[8], long long row, int col, int count,
-                                        const float (&bias)[8], const T* gate, const float (&res)[8]) {
-  if (EPI) {
-    float e[8];
-    if (gate) load_vec<8>(gate + col, args.vec, count, e);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += bias[i];
-    if (args.preact) store_vec<8>(static_cast<T*>(args.preact) + row * args.n + col, args.vec, count, v);
-    switch (args.act) {
-      case kActGeluTanh: activate_all<kActGeluTanh>(v); break;
-      case kActGelu: activate_all<kActGelu>(v); break;
-      case kActSilu: activate_all<kActSilu>(v); break;
-      default: break;
-    }
-    if (gate) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= e[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += res[i];
-  }
-  store_vec<8>(static_cast<T*>(args.out) + row * args.out_stride + col, args.vec, count, v);
-}
-
-template <typename T, bool EPI>
-__device__ __forceinline__ void load_bias(const GemmArgs& args, int col, int count, float (&bias)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) bias[i] = 0.0f;
-  if (EPI && args.bias && count > 0) load_vec<8>(static_cast<const T*>(args.bias) + col, args.vec, count, bias);
-}
-template <typename T, bool EPI>
-__device__ __forceinline__ void load_residual(const GemmArgs& args, long long row, int col, int count, float (&res)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) res[i] = 0.0f;
-  if (EPI && args.residual && row < args.m && count > 0)
-    load_vec<8>(static_cast<const T*>(args.residual) + row * args.res_stride + col, args.vec, count, res);
-}
 template <typename T, bool EPI>
 __device__ __forceinline__ const T* gate_row(const GemmArgs& args, long long row) {
   if (!EPI || !args.gate || row >= args.m) return nullptr;
@@ -434,13 +374,10 @@ __device__ __forceinline__ float4 ld_shared_v4(uint32_t addr) {
   asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(addr) : "memory");
   return f;
 }
-__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
-  float4 f;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w)
-               : "r"(addr)
+// to another CTA's shared memory (``addr`` from map_rank)
+__device__ __forceinline__ void st_cluster_v4(uint32_t addr, const uint32_t* v) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
                : "memory");
-  return f;
 }
 
 // act of 16 pairs
@@ -546,12 +483,13 @@ __device__ __forceinline__ void add_residual(const GemmArgs& args, uint32_t stag
   __syncwarp();
 }
 
-// bias (0: none) and gate of an accumulator's columns into ``vectors``, where
-// the whole tile has one gate row; every epilogue thread takes one column
+// bias (0: none) and gate of ``cols`` columns into ``vectors``, where the whole
+// tile has one gate row; every epilogue thread takes one column
 template <typename T>
-__device__ __forceinline__ void stage_vectors(const GemmArgs& args, float* vectors, const T* gate, int col0, int thread) {
+__device__ __forceinline__ void stage_vectors(const GemmArgs& args, float* vectors, const T* gate, int col0, int cols,
+                                              int thread) {
   const int col = col0 + thread;
-  const bool inside = thread < args.bn && col < args.n;
+  const bool inside = thread < cols && col < args.n;
   vectors[thread] = inside && args.bias ? to_f32<T>(static_cast<const T*>(args.bias)[col]) : 0.0f;
   vectors[256 + thread] = inside && gate ? to_f32<T>(gate[col]) : 1.0f;
 }
@@ -591,7 +529,7 @@ __device__ __forceinline__ void finish_chunk(const GemmArgs& args, float2 (&v)[1
         float g[8];
         const int count = min(8, col_end - col - 8 * p);
         if (count <= 0) continue;
-        load_vec<8>(own_gate + col + 8 * p, args.vec, count, g);
+        load8(own_gate + col + 8 * p, args.vec, count, g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[4 * p + i] = fmul2(v[4 * p + i], make_float2(g[2 * i], g[2 * i + 1]));
       }
@@ -627,10 +565,14 @@ __device__ __forceinline__ void finish_tile(const GemmArgs& args, uint32_t tmem,
   }
 }
 
-// byte offset of the 16-byte piece ``c`` of row ``row`` in a split tile's partial
-__device__ __forceinline__ uint32_t partial_offset(int row, int c, int bn) {
-  return static_cast<uint32_t>(row * bn * 4 + (((c & ~7) | ((c ^ row) & 7)) << 4));
+// The column chunks of a split tile that one of its groups finishes.
+struct OwnChunks {
+  int begin, end;
+};
+__device__ __forceinline__ OwnChunks own_chunks(int chunks, int part, int splits) {
+  return OwnChunks{chunks * part / splits, chunks * (part + 1) / splits};
 }
+constexpr int kChunkBytes = kTileM * kStageRow * 4;  // fp32 partial of a chunk: [4 columns][128 rows][16 bytes]
 
 template <typename T, int CG, bool SPLIT, bool WIDE, bool AMN, bool BMN, bool EPI>
 __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmArgs args, int splits) {
@@ -839,25 +781,19 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         const int b = turn & 1;
         const int col0 = (tn * kHalves + h) * args.bn;
         float* vec = vectors + b * 512;
-        if (EPI && !SPLIT && (args.bias || gate)) {
-          stage_vectors<T>(args, vec, gate, col0, thread);
-          epilogue_barrier();
+        if (EPI && (args.bias || gate)) {
+          if constexpr (SPLIT) {  // the columns that this group finishes; read after the barriers below
+            const OwnChunks own = own_chunks(args.bn / kStageRow, part, splits);
+            stage_vectors<T>(args, vec, gate, col0 + own.begin * kStageRow, (own.end - own.begin) * kStageRow, thread);
+          } else {
+            stage_vectors<T>(args, vec, gate, col0, args.bn, thread);
+            epilogue_barrier();
+          }
         }
         // after an expired wait the warp still meets the others at the barriers above
         if (!mbar_wait_warp(&sh.acc_full[b], (turn >> 1) & 1, abort_flag, args.status)) continue;
         tc_fence_after();
-        if constexpr (SPLIT) {
-          // the partial tile, one row per lane, into the drained ring
-          const int row = quarter * 32 + lane;
-          for (int c = half * 32; c < args.bn; c += 64) {
-            uint32_t acc[32];
-            tmem_ld32_sync(tmem + lanes + c, acc);
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              st_shared_v4(ring + partial_offset(row, (c >> 2) + j, args.bn), acc[4 * j], acc[4 * j + 1], acc[4 * j + 2],
-                           acc[4 * j + 3]);
-          }
-        } else {
+        if constexpr (!SPLIT) {
           finish_tile<T, EPI>(args, tmem + b * kAccumulator + lanes, ring + kRingBytes + (warp - 2) * 2048, vec, own_gate,
                               row0, col0, lane, half);
           tc_fence_before();
@@ -873,40 +809,70 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  // split: every partial is written; otherwise neither CTA of a pair leaves while the other may still signal it
+  // split: every group's ring is drained; otherwise neither CTA of a pair leaves while the other may still signal it
   if (CG > 1 || SPLIT) cluster_sync();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_free<CG>(tmem, 2 * kAccumulator);
-  }
   if constexpr (SPLIT) {
     int tm, tn;
     tile_coords(args, group, tm, tn);
-    const int first = kTileM * part / splits, rows = kTileM * (part + 1) / splits - first;
-    const int pieces = args.bn / 8;  // 8 columns each
-    const int col0 = tn * args.bn;
-    const long long row0 = static_cast<long long>(tm * CG + static_cast<int>(rank)) * kTileM;
-    for (int i = threadIdx.x; i < rows * pieces && !sh.abort_flag; i += kGemmThreads) {
-      const int r = first + i / pieces, c = i % pieces;
-      const long long row = row0 + r;
-      const int col = col0 + c * 8, count = min(8, args.n - col);
-      if (row >= args.m || count <= 0) continue;
-      float v[8], bias[8], res[8];
-      load_bias<T, EPI>(args, col, count, bias);
-      load_residual<T, EPI>(args, row, col, count, res);
+    const bool works = warp >= 2 && warp < 2 + kEpilogueWarps && !sh.abort_flag;
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const long long tile_row = static_cast<long long>(tm * CG + static_cast<int>(rank)) * kTileM, row0 = tile_row + quarter * 32;
+    const int chunks = args.bn / kStageRow;
+    const uint32_t at_lane = (quarter * 32 + lane) * 16;
+    tc_fence_after();
+    if (works) {  // the other groups' columns, each to its group; groups in turn from the next one on
+      for (int d = 1; d < splits; ++d) {
+        const int to = (part + d) % splits, slot = splits - 1 - d;  // this group is number ``slot`` after ``to``
+        const OwnChunks theirs = own_chunks(chunks, to, splits);
+        const uint32_t base = map_rank(ring, to * CG + rank) + slot * (theirs.end - theirs.begin) * kChunkBytes + at_lane;
+        for (int c = theirs.begin + half; c < theirs.end; c += 2) {
+          uint32_t acc[32];
+          tmem_ld32_sync(tmem + lanes + c * kStageRow, acc);
+          if (row0 + lane >= args.m) continue;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-      for (int p = 0; p < splits; ++p) {
-        const uint32_t base = map_rank(ring, p * CG + rank);
-        const float4 lo = ld_cluster_v4(base + partial_offset(r, 2 * c, args.bn));
-        const float4 hi = ld_cluster_v4(base + partial_offset(r, 2 * c + 1, args.bn));
-        v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
-        v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
+          for (int j = 0; j < 8; ++j)
+            st_cluster_v4(base + (c - theirs.begin) * kChunkBytes + j * kTileM * 16, acc + 4 * j);
+        }
       }
-      finish8<T, EPI>(args, v, row, col, count, bias, gate_row<T, EPI>(args, row), res);
     }
-    __syncthreads();
-    cluster_sync();  // no CTA's partial goes away while another reads it
+    __syncwarp();
+    cluster_sync();  // every partial has arrived
+    if (works) {
+      const OwnChunks own = own_chunks(chunks, part, splits);
+      const int col0 = tn * args.bn + own.begin * kStageRow, count = own.end - own.begin;
+      const int col_end = min(args.n, col0 + count * kStageRow);
+      const float* vectors = reinterpret_cast<const float*>(smem_raw + (ring - smem_u32(smem_raw)) + kRingBytes + kStagingBytes);
+      const T* gate = gate_row<T, EPI>(args, tile_row);
+      const T* own_gate = nullptr;
+      if (gate && gate != gate_row<T, EPI>(args, min(tile_row + kTileM, static_cast<long long>(args.m)) - 1))
+        own_gate = gate_row<T, EPI>(args, min(row0 + lane, static_cast<long long>(args.m) - 1));
+      for (int c = half; c < count; c += 2) {
+        uint32_t acc[32];
+        tmem_ld32_sync(tmem + lanes + (own.begin + c) * kStageRow, acc);
+        float2 v[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = make_float2(__uint_as_float(acc[2 * j]), __uint_as_float(acc[2 * j + 1]));
+        for (int p = 0; p < splits - 1; ++p) {
+          const uint32_t from = ring + (p * count + c) * kChunkBytes + at_lane;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float4 f = ld_shared_v4(from + j * kTileM * 16);
+            v[2 * j] = fadd2(v[2 * j], make_float2(f.x, f.y));
+            v[2 * j + 1] = fadd2(v[2 * j + 1], make_float2(f.z, f.w));
+          }
+        }
+        finish_chunk<T, EPI>(args, v, ring + kRingBytes + (warp - 2) * 2048, vectors, own_gate, row0, col0, c, col_end, lane);
+      }
+    }
+    __syncwarp();
+    tc_fence_before();
+    if (CG > 1) cluster_sync();  // the pair frees its TMEM together
+    else __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_free<CG>(tmem, 2 * kAccumulator);
   }
 }
 
@@ -1179,22 +1145,29 @@ struct TileChoice {
 // column), or its operand rows' 128 bytes at 50 bytes a clock (the traffic that
 // measured equal to it), whichever is longer; plus what a tile adds: little where
 // the epilogue hides under the next tile, ``exposed`` clocks a column where it
-// does not (wide), a meeting of partials (split).
+// does not (wide), the partials at 8 bytes a clock between SMs and the meeting
+// (split).  Of all the choices for a shape this takes the fastest or one within
+// 3% of it: 256 x 12288 x 3072 25.7 us (224 columns, 4 splits; 128 and 2: 28.1),
+// 128 x 12288 x 3072 21.3 us (96 and 4; 64 and 2: 27.6), 256 x 3072 x 12288 22.9
+// us (192, no split; 256: 25.5).
 TileChoice choose_tiles(int m, int n, int kblocks, bool amn, double exposed) {
   TileChoice best{1, 128, 1, 1};
   double least = 1e300;
   const int cg = m > kTileM ? 2 : 1;
-  const int a_rows = amn ? (m > 64 ? 128 : 64) : (m < kTileM ? (m + 7) / 8 * 8 : kTileM);
+  const int valid = m < kTileM ? m : kTileM;
+  const int a_rows = amn ? (m > 64 ? 128 : 64) : (valid + 7) / 8 * 8;
   const long long tiles_m = (m + kTileM * cg - 1) / (kTileM * cg);
   auto consider = [&](int bn, int halves, int splits) {
-    const int cols = bn * halves;
+    const int cols = bn * halves, size = splits * cg;
     const long long tiles = tiles_m * ((n + cols - 1) / cols);
-    const long long waves = (tiles * splits * cg + kNumSMs - 1) / kNumSMs;
+    // clusters of one CTA per SM that the GPU holds at a time
+    const int fit = size == 1 ? kNumSMs : size == 2 ? kNumSMs / 2 : size == 4 ? 33 : 15;
+    const long long waves = (tiles + fit - 1) / fit;
     if (splits > 1 && waves > 1) return;
     const double mma = 2.0 * cols, load = 128.0 / 50.0 * (a_rows + cols / cg);
     const double cost = waves * (static_cast<double>(kblocks) / splits * (mma > load ? mma : load) +
                                  (halves > 1 ? exposed * bn : 200.0)) +
-                        (splits > 1 ? 2500.0 : 6.0 * cols);
+                        (splits > 1 ? 3500.0 + 0.5 * valid * cols * (splits - 1) / splits : 6.0 * cols);
     if (cost < least) {
       least = cost;
       best = TileChoice{cg, bn, halves, splits};
@@ -1202,7 +1175,7 @@ TileChoice choose_tiles(int m, int n, int kblocks, bool amn, double exposed) {
   };
   for (int splits = 1; splits * cg <= 8; splits *= 2) {
     if (splits > 1 && kblocks < 4 * splits) break;
-    const int most = splits > 1 || cg == 1 ? kMaxSplitColumns : 256;
+    const int most = splits == 1 && cg == 1 ? 128 : 256;  // a CTA's accumulators are 128 columns apart, a pair's 256
     for (int bn = 32 * cg; bn <= most; bn += 32) consider(bn, 1, splits);
   }
   if (cg == 2)

@@ -293,3 +293,15 @@ def test_refusals():
     assert lib.peco_linear_forward(p, 16, z, 0, p, 16, z, z, 0, z, 0, p, 8, z, 1, 2, 8, 8, 8, 0, 1, z, 0, s) == 1
     assert lib.peco_linear_forward(p, 15, z, 0, p, 16, z, z, 0, z, 0, p, 8, z, 1, 2, 15, 0, 8, 0, 1, z, 0, s) == 20005
     assert lib.peco_launch_count() == launches
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(1, 256, 1536, 12288), (1, 200, 1000, 6000), (2, 80, 3000, 999), (1, 256, 4096, 2688),
+                                   (1, 129, 2048, 5000), (3, 170, 2048, 2050), (1, 100, 2048, 9000), (1, 7, 4096, 700),
+                                   (1, 256, 8192, 2048)])
+def test_few_rows_over_long_sums(shape, dtype):
+    # the sum over K is shared out among CTAs, on tiles of one and of two accumulators
+    for i, act in enumerate(("gelu_tanh", None)):
+        c = _case(7 + i, *shape, dtype=dtype, gate="sample" if i else "shared", residual=i == 0)
+        _check(linear_act(**c, activation=act), *_forward64(c, act), U[dtype])
+    assert _native.device_status(clear=True) == 0
