@@ -887,12 +887,20 @@ struct PackArgs {
   int ld[4], rows[4], cols[4];
 };
 __global__ void __launch_bounds__(256) pack_rows_kernel(const __grid_constant__ PackArgs a) {
+  wait_for_prior();
+  let_next_start();
   const int k = blockIdx.y, cols = a.cols[k];
   for (long long r = blockIdx.x; r < a.rows[k]; r += gridDim.x) {
-    const uint16_t* __restrict__ src = a.src[k] + r * a.stride[k];
-    uint16_t* __restrict__ dst = a.dst[k] + r * a.ld[k];
-#pragma unroll 4
-    for (int c = threadIdx.x; c < cols; c += 256) dst[c] = src[c];
+    const uint16_t* src = a.src[k] + r * a.stride[k];
+    uint16_t* dst = a.dst[k] + r * a.ld[k];
+    for (int c0 = threadIdx.x; c0 < cols; c0 += 8 * 256) {
+      uint16_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = c0 + i * 256 < cols ? src[c0 + i * 256] : static_cast<uint16_t>(0);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c0 + i * 256 < cols) dst[c0 + i * 256] = v[i];
+    }
   }
 }
 
@@ -1103,8 +1111,7 @@ int prepare_operands(Operand* const* list, int n, Carver& ws, cudaStream_t strea
     ++jobs;
   }
   if (!jobs) return kOk;
-  pack_rows_kernel<<<dim3(most < 8 * kNumSMs ? most : 8 * kNumSMs, jobs), 256, 0, stream>>>(p);
-  return launch_status();
+  return launch_overlapped(pack_rows_kernel, dim3(most < 8 * kNumSMs ? most : 8 * kNumSMs, jobs), dim3(256), 0, 0, stream, p);
 }
 
 bool operand_map(CUtensorMap* map, const Operand& o, bool mn, int tile_rows, int joined_panels, int dtype) {
