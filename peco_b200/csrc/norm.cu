@@ -24,10 +24,10 @@
 // registers of the threads that share it, and every statistic is taken from
 // there in fp32, squares around the mean.  The backward kernel recomputes r
 // from x and the branch, so nothing has to be saved.  Measured at 3072 bf16
-// columns: forward with branch, gate and modulation 34680 rows 135-143 us (6.0
-// to 6.3 TB/s), backward 7006 rows 60 us (4.3 TB/s, of it 6.5 us for the second
-// kernel), 34680 rows 238 us (5.4 TB/s); the backward is bound by the latency
-// of a row's reduction at the 12 warps per SM that its registers allow.
+// columns: forward with branch, gate and modulation 34680 rows 133 us (6.4
+// TB/s), backward 7006 rows 57 us (4.5 TB/s, of it 6 us for the second kernel),
+// 34680 rows 238 us (5.4 TB/s); the backward is bound by the latency of a row's
+// reduction at the 12 warps per SM that its registers allow.
 #include "common.cuh"
 #include "../../include/peco_b200.h"
 #include "internal.h"

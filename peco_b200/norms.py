@@ -68,7 +68,7 @@ def _extent(x):
     return samples, x.numel() // (c * samples) if samples else 0
 
 
-def _check(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, eps, residual_scale):
+def _check(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, eps, post_eps, residual_scale):
     if norm != "layer" and norm != "rms":
         raise ValueError(f'norm must be "layer" or "rms", got {norm!r}')
     post = NORMS.get(post_norm)
@@ -107,12 +107,12 @@ def _check(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, 
     for t in (weight, post_weight):
         if t is not None and t.shape != (c,):
             raise ValueError(f"weight and post_weight must be [{c}]")
-    if not eps >= 0 or not abs(residual_scale) < math.inf:
-        raise ValueError("eps must be nonnegative and residual_scale finite")
+    if not eps >= 0 or post_eps is not None and not post_eps >= 0 or not abs(residual_scale) < math.inf:
+        raise ValueError("eps and post_eps must be nonnegative and residual_scale finite")
 
 
 def _forward(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, eps, post_eps, residual_scale):
-    _check(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, eps, residual_scale)
+    _check(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, eps, post_eps, residual_scale)
     shape = x.shape
     c = shape[-1]
     normed = torch.empty_like(x, memory_format=torch.contiguous_format)
@@ -206,7 +206,7 @@ def modulated_norm_backward(grad_normed, grad_residual, x, branch=None, *, gate=
     """Gradients of ``modulated_norm`` for ``grad_normed`` = d h and
     ``grad_residual`` = d r (None: zero).  ``needs``: names of the gradients to
     compute (default: those of all inputs that are there)."""
-    _check(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, eps, residual_scale)
+    _check(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, eps, post_eps, residual_scale)
     if grad_normed is None:
         raise ValueError("grad_normed is required")
     shape, dtype, device = x.shape, x.dtype, x.device

@@ -58,6 +58,8 @@ def _run(q, k, axes, theta, grid, positions, interleaved, inverse, inplace):
             raise ValueError("q and k must agree in batch, tokens and head dimension")
         if k.dtype is not dtype:
             raise TypeError("q and k must have one dtype")
+        if inplace and k.data_ptr() == q.data_ptr() and q.numel():
+            raise ValueError("inplace would turn q and k twice: they are one tensor")
     if d % 2 or not 2 <= d <= 256:
         raise ValueError("the head dimension must be even and at most 256")
     sections = _sections(tuple(axes), d)

@@ -362,3 +362,14 @@ def test_rotary_refusals():
         rotate(q.cpu(), axes=(64,), grid=(12,))
     with pytest.raises(RuntimeError):
         rotate(q.clone().requires_grad_(), **ok, inplace=True)
+
+
+def test_second_epsilon_and_shared_operand_are_refused():
+    x = torch.randn(1, 4, 16, device=DEV).to(torch.bfloat16)
+    with pytest.raises(ValueError):
+        modulated_norm(x, x, post_norm="rms", post_eps=-1.0)
+    with pytest.raises(ValueError):
+        modulated_norm_backward(x, None, x, x, post_norm="rms", post_eps=float("nan"))
+    q = torch.randn(1, 2, 4, 16, device=DEV).to(torch.bfloat16)
+    with pytest.raises(ValueError):
+        rotate(q, q, axes=(16,), grid=(4,), inplace=True)

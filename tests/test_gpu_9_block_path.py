@@ -13,9 +13,11 @@ import torch
 
 from peco_b200 import _native
 from peco_b200.hunyuan import HunyuanConfig, Pipe, build_transformer, use_block_operators, use_dense_attention
+from peco_b200.linear import linear_act, linear_act_backward
 from peco_b200.model import install_attention
+from peco_b200.norms import modulated_norm, modulated_norm_backward
 from peco_b200.processor import InferenceContext, PecoConfig
-from peco_b200.rotary import AxialPositions
+from peco_b200.rotary import AxialPositions, rotate
 
 pytestmark = pytest.mark.gpu
 
@@ -97,3 +99,42 @@ def test_processor_takes_positions():
             assert _cosine(a, b) >= 0.9999
         with pytest.raises(ValueError, match="rotary positions"):
             attn(x, txt, None, AxialPositions(CFG.rope_axes, CFG.rope_theta, grid=(2, 8, 7)))
+
+
+@pytest.mark.parametrize("width", [64, 1001])
+def test_launches_in_a_row_are_ordered(width):
+    # every kernel may start before the one in front of it has ended and has to wait for its results
+    g = torch.Generator(device="cuda").manual_seed(3)
+
+    def normal(*shape, std=1.0):
+        return (torch.randn(shape, generator=g, device="cuda") * std).to(torch.bfloat16)
+
+    rows, heads = 150, 2
+    w1, w2 = normal(heads * 64, width, std=width ** -0.5), normal(width, heads * 64, std=0.1)
+    gate, scale, b = normal(2, width), normal(2, width), normal(width)
+
+    def chain(x, wait):
+        kept = []
+        for _ in range(6):
+            h = modulated_norm(x, scale=scale, shift=gate)
+            wait()
+            q = linear_act(h, w1, activation="silu")
+            wait()
+            q = rotate(q.view(2, rows, heads, 64).transpose(1, 2), axes=(16, 24, 24), grid=(1, 10, 15))
+            wait()
+            y = linear_act(q.transpose(1, 2).reshape(2, rows, heads * 64), w2, b, gate=gate, residual=x)
+            wait()
+            d = linear_act_backward(q.transpose(1, 2).reshape(2, rows, heads * 64), h, w1, bias=True)
+            wait()
+            n = modulated_norm_backward(d.x, y, x, y, gate=gate, scale=scale)
+            wait()
+            x = modulated_norm(y, n.x, gate=n.gate)[1]
+            wait()
+            kept += [y, d.weight, d.bias, n.scale, x]
+        torch.cuda.synchronize()
+        return kept
+
+    x = normal(2, rows, width)
+    for a, c in zip(chain(x, torch.cuda.synchronize), chain(x, lambda: None)):
+        assert torch.equal(a, c)
+    assert _native.device_status(clear=True) == 0
