@@ -34,6 +34,7 @@
 #include "rows.cuh"
 
 #include <atomic>
+#include <type_traits>
 
 namespace peco {
 namespace {
@@ -127,6 +128,24 @@ template <typename T>
 __device__ __forceinline__ void widen(const RawChunk& r, float2 (&v)[4]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) v[j] = unpack2<T>(r.w[j]);
+}
+
+// The same with a register for each element of an unaligned row: joining two
+// loads in one would wait for them where they are issued.  The forward kernel
+// has the registers for its prefetch.
+struct RawElements {
+  uint32_t w[kChunk];
+};
+template <typename T, int WARPS, int NCH>
+__device__ __forceinline__ void fetch(const Span<WARPS, NCH, kUnaligned>& sp, const T* row, int i, RawElements& r) {
+  const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+  for (int e = 0; e < kChunk; ++e) r.w[e] = sp.inside(i, e) ? p[sp.column(i, e)] : 0u;
+}
+template <typename T>
+__device__ __forceinline__ void widen(const RawElements& r, float2 (&v)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = unpack2<T>(r.w[2 * j] | r.w[2 * j + 1] << 16);
 }
 
 // a vector's (gate, scale, ...) part of chunk i
@@ -383,7 +402,7 @@ __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS) norm_forward_ker
     ring.start(src);
     ahead = ahead + step < ahead ? 0xffffffffu : ahead + step;
   };
-  RawChunk raw_x[NCH], raw_b[NCH];
+  std::conditional_t<MODE == kUnaligned, RawElements, RawChunk> raw_x[NCH], raw_b[NCH];
   if constexpr (kRing) {
     ring.open();
     if (threadIdx.x == 0)
