@@ -131,8 +131,7 @@ __device__ __forceinline__ void widen(const RawChunk& r, float2 (&v)[4]) {
 }
 
 // The same with a register for each element of an unaligned row: joining two
-// loads in one would wait for them where they are issued.  The forward kernel
-// has the registers for its prefetch.
+// loads in one would wait for them where they are issued.
 struct RawElements {
   uint32_t w[kChunk];
 };
@@ -550,7 +549,8 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS) norm_backward_kernel(const
     ring.start(src);
     ahead = ahead + stride < ahead ? 0xffffffffu : ahead + stride;
   };
-  RawChunk raw_x[NCH], raw_d[NCH], raw_b[NCH], raw_e[NCH];
+  using Raw = std::conditional_t<MODE == kUnaligned && NCH == 1, RawElements, RawChunk>;  // two chunks' would spill
+  Raw raw_x[NCH], raw_d[NCH], raw_b[NCH], raw_e[NCH];
   if constexpr (kRing) {
     ring.open();
     if (threadIdx.x == 0)
@@ -573,7 +573,10 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS) norm_backward_kernel(const
     const unsigned char* stage = nullptr;
     if constexpr (kRing) stage = ring.next();
     // a piece of an input: from the stage, as often as it is needed, or from its register
-    auto piece = [&](int k, int i, const RawChunk& held) { return kRing ? staged(sp, stage, k, a.width * 2, i) : held; };
+    auto piece = [&](int k, int i, const Raw& held) {
+      if constexpr (kRing) return staged(sp, stage, k, a.width * 2, i);
+      else return held;
+    };
     float2 pscale = both(1.0f), pshift = both(0.0f);  // post norm: b * rstd - mean * rstd
     float prstd = 1.0f;
     if constexpr (POST) {
@@ -808,10 +811,14 @@ int launch_backward_mode(NormArgs a, cudaStream_t stream) {
 }
 
 template <typename T, int WARPS, int NCH, int BLOCKS, bool POST>
-int launch_backward(const NormArgs& a, cudaStream_t stream) {
-  if (!a.vec) return launch_backward_mode<T, WARPS, NCH, BLOCKS, kUnaligned, POST>(a, stream);
+int launch_backward_aligned(const NormArgs& a, cudaStream_t stream) {
   if (a.width == 32 * kChunk * WARPS * NCH) return launch_backward_mode<T, WARPS, NCH, BLOCKS, kFull, POST>(a, stream);
   return launch_backward_mode<T, WARPS, NCH, BLOCKS, kAligned, POST>(a, stream);
+}
+template <typename T, int WARPS, int NCH, int BLOCKS, bool POST>
+int launch_backward(const NormArgs& a, cudaStream_t stream) {
+  if (!a.vec) return launch_backward_mode<T, WARPS, NCH, BLOCKS, kUnaligned, POST>(a, stream);
+  return launch_backward_aligned<T, WARPS, NCH, BLOCKS, POST>(a, stream);
 }
 
 template <typename T, int WARPS, int NCH, int MODE, bool POST>
@@ -854,9 +861,14 @@ int launch_norm(const NormArgs& a, bool backward, cudaStream_t stream) {
     if (w <= 256) return launch_backward<T, 1, 1, 12, POST>(a, stream);
     if (w <= 512) return launch_backward<T, 1, 2, 12, POST>(a, stream);
     if (w <= 1024) return launch_backward<T, 4, 1, 4, POST>(a, stream);
-    if (w <= 2048) return launch_backward<T, 4, 2, 3, POST>(a, stream);
-    if (w <= 3072) return launch_backward<T, 6, 2, 2, POST>(a, stream);
-    if (w <= 4096) return launch_backward<T, 8, 2, 1, POST>(a, stream);
+    if (!a.vec && w <= 4096) {
+      if (w <= 2048) return launch_backward_mode<T, 8, 1, 2, kUnaligned, POST>(a, stream);
+      if (w <= 3072) return launch_backward_mode<T, 12, 1, 1, kUnaligned, POST>(a, stream);
+      return launch_backward_mode<T, 16, 1, 1, kUnaligned, POST>(a, stream);
+    }
+    if (w <= 2048) return launch_backward_aligned<T, 4, 2, 3, POST>(a, stream);
+    if (w <= 3072) return launch_backward_aligned<T, 6, 2, 2, POST>(a, stream);
+    if (w <= 4096) return launch_backward_aligned<T, 8, 2, 1, POST>(a, stream);
     if (w <= 6144) return launch_backward<T, 12, 2, 1, POST>(a, stream);
     if (w <= 8192) return launch_backward<T, 16, 2, 1, POST>(a, stream);
     return launch_backward<T, 16, 4, 1, POST>(a, stream);
