@@ -844,16 +844,23 @@ int launch_forward_mode(NormArgs a, cudaStream_t stream) {
 }
 
 template <typename T, int WARPS, int NCH, bool POST>
-int launch_forward(const NormArgs& a, cudaStream_t stream) {
-  if (!a.vec) return launch_forward_mode<T, WARPS, NCH, kUnaligned, POST>(a, stream);
+int launch_forward_aligned(const NormArgs& a, cudaStream_t stream) {
   if (a.width == 32 * kChunk * WARPS * NCH) return launch_forward_mode<T, WARPS, NCH, kFull, POST>(a, stream);
   return launch_forward_mode<T, WARPS, NCH, kAligned, POST>(a, stream);
+}
+template <typename T, int WARPS, int NCH, bool POST>
+int launch_forward(const NormArgs& a, cudaStream_t stream) {
+  if (!a.vec) return launch_forward_mode<T, WARPS, NCH, kUnaligned, POST>(a, stream);
+  return launch_forward_aligned<T, WARPS, NCH, POST>(a, stream);
 }
 
 // Threads per row.  Few warps keep a row's reduction cheap, few columns per
 // thread its registers; measured at 3072 columns (34680 rows): backward 238 us
 // with 6 warps x 2 chunks, 412 with 12 x 1, 234 with 4 x 3 (equal at 7006 rows);
-// forward 145 us with 4 x 3, 161 with 12 x 1, 179 with 8 x 2.
+// forward 145 us with 4 x 3, 161 with 12 x 1, 179 with 8 x 2.  Unaligned rows
+// hold a register per element ahead and take fewer of them: 14769 x 2241 backward
+// 168 us with 12 x 1 (348 with 6 x 2, two elements to a register), forward 68 us
+// with 4 x 3, 90 with 8 x 2; 8000 x 6001 forward 104 us with 16 x 2, 151 with 8 x 3.
 template <typename T, bool POST>
 int launch_norm(const NormArgs& a, bool backward, cudaStream_t stream) {
   const int w = a.width;
@@ -879,7 +886,7 @@ int launch_norm(const NormArgs& a, bool backward, cudaStream_t stream) {
   if (w <= 2048) return launch_forward<T, 4, 2, POST>(a, stream);
   if (w <= 3072) return launch_forward<T, 4, 3, POST>(a, stream);
   if (w <= 4096) return launch_forward<T, 8, 2, POST>(a, stream);
-  if (w <= 6144) return launch_forward<T, 8, 3, POST>(a, stream);
+  if (a.vec && w <= 6144) return launch_forward_aligned<T, 8, 3, POST>(a, stream);
   if (w <= 8192) return launch_forward<T, 16, 2, POST>(a, stream);
   return launch_forward<T, 16, 4, POST>(a, stream);
 }
