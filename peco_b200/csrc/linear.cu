@@ -781,7 +781,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         const int b = turn & 1;
         const int col0 = (tn * kHalves + h) * args.bn;
         float* vec = vectors + b * 512;
-        if (EPI && (args.bias || gate)) {
+        // the same for every tile, also where this CTA's rows lie past the matrix and it has no gate row: the
+        // barrier is what keeps a tile's vectors from being overwritten while a slower warp still reads them
+        if (EPI && (args.bias || args.gate)) {
           if constexpr (SPLIT) {  // the columns that this group finishes; read after the barriers below
             const OwnChunks own = own_chunks(args.bn / kStageRow, part, splits);
             stage_vectors<T>(args, vec, gate, col0 + own.begin * kStageRow, (own.end - own.begin) * kStageRow, thread);
