@@ -831,10 +831,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         for (int c = theirs.begin + half; c < theirs.end; c += 2) {
           uint32_t acc[32];
           tmem_ld32_sync(tmem + lanes + c * kStageRow, acc);
-          if (row0 + lane >= args.m) continue;
+          if (row0 + lane < args.m) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            st_cluster_v4(base + (c - theirs.begin) * kChunkBytes + j * kTileM * 16, acc + 4 * j);
+            for (int j = 0; j < 8; ++j)
+              st_cluster_v4(base + (c - theirs.begin) * kChunkBytes + j * kTileM * 16, acc + 4 * j);
+          }
+          __syncwarp();  // the next TMEM load wants the whole warp
         }
       }
     }

@@ -46,3 +46,18 @@ def test_gate_without_bias_past_the_last_rows(rows, k, n, residual):
     for _ in range(50):
         assert torch.equal(linear_act(x, w, gate=gate, residual=r), got)
     assert _native.device_status(clear=True) == 0
+
+
+@pytest.mark.parametrize("rows", [1, 31, 33, 97, 127, 130, 161, 255])
+@pytest.mark.parametrize("k,n", [(4096, 700), (2048, 5000)])
+def test_sums_shared_out_over_ragged_rows(rows, k, n):
+    # K over the groups of a cluster, with warps some of whose lanes have no row
+    normal = _normal(rows + k)
+    x, w, b = normal(rows, k), normal(n, k, std=k ** -0.5), normal(n)
+    got = linear_act(x, w, b)
+    y = x.double() @ w.double().t() + b.double()
+    slack = (k + 2) * 2.0 ** -24 * (x.double().abs() @ w.double().abs().t() + b.double().abs())
+    _within(got, y, slack + 2.0 ** -23 * y.abs(), U[torch.bfloat16])
+    for _ in range(10):
+        assert torch.equal(linear_act(x, w, b), got)
+    assert _native.device_status(clear=True) == 0
