@@ -72,33 +72,33 @@ __device__ __forceinline__ float recip_approx(float x) {
   return y;
 }
 
-// z Phi(z) of a pair.  With x = |z| / sqrt 2 and t = 1 / (1 + p x), erfc(x) is a
-// polynomial in t times exp(-x^2) (Abramowitz and Stegun, Handbook of
-// Mathematical Functions, 7.1.26, within 1.5e-7); it keeps its relative
-// precision in the negative tail, where 1 + erf would cancel.
-__device__ __forceinline__ float2 gelu_pair(float2 z) {
+// Phi(z) of a pair, the normal distribution's integral, and exp(-z^2 / 2).  With
+// t = 1 / (1 + 0.36 |z|), Phi(-|z|) exp(z^2 / 2) / t is smooth in t down to its
+// limit at t = 0, so a polynomial (fitted for the least relative error over
+// 0 <= |z| <= 13.2: 2^-20.4) times the exponential keeps its relative precision
+// in the negative tail, where 1 + erf would cancel.  In fp32 the exponential's
+// argument rounds too: about 2^-18 of the value down to z = -8, 2^-17 down to -12.8,
+// where the exponential nears the smallest normal number.
+__device__ __forceinline__ float2 normal_integral_pair(float2 z, float2& bell) {
   auto both = [](float x) { return make_float2(x, x); };
-  const float2 x = make_float2(fabsf(z.x) * 0.7071067811865476f, fabsf(z.y) * 0.7071067811865476f);
-  const float2 d = ffma2(x, both(0.3275911f), both(1.0f));
+  const float2 d = ffma2(make_float2(fabsf(z.x), fabsf(z.y)), both(0.36f), both(1.0f));
   const float2 t = make_float2(recip_approx(d.x), recip_approx(d.y));
-  float2 poly = ffma2(t, both(1.061405429f), both(-1.453152027f));
-  poly = ffma2(t, poly, both(1.421413741f));
-  poly = ffma2(t, poly, both(-0.284496736f));
-  poly = ffma2(t, poly, both(0.254829592f));
-  const float2 w = fmul2(fmul2(x, x), both(-kLog2e));
-  // half of erfc(|z| / sqrt 2), and its complement for positive z
-  const float2 half = fmul2(fmul2(poly, t), make_float2(0.5f * exp2_approx(w.x), 0.5f * exp2_approx(w.y)));
-  const float2 p = make_float2(z.x > 0.0f ? 1.0f - half.x : half.x, z.y > 0.0f ? 1.0f - half.y : half.y);
-  return fmul2(z, p);
+  float2 poly = ffma2(t, both(0.04752533882856369f), both(-0.18137013912200928f));
+  poly = ffma2(t, poly, both(0.1831398457288742f));
+  poly = ffma2(t, poly, both(0.025042641907930374f));
+  poly = ffma2(t, poly, both(0.14027050137519836f));
+  poly = ffma2(t, poly, both(0.1416715383529663f));
+  poly = ffma2(t, poly, both(0.14372023940086365f));
+  const float2 w = fmul2(fmul2(z, z), both(-0.5f * kLog2e));
+  bell = make_float2(exp2_approx(w.x), exp2_approx(w.y));
+  const float2 tail = fmul2(fmul2(poly, t), bell);
+  return make_float2(z.x > 0.0f ? 1.0f - tail.x : tail.x, z.y > 0.0f ? 1.0f - tail.y : tail.y);
 }
 
 // (act(z), act'(z)) of the forms that take no pairs
 template <int ACT>
 __device__ __forceinline__ float2 activate_slope(float z) {
-  if constexpr (ACT == kActGelu) {
-    const float p = 0.5f * (1.0f + erff(z * 0.7071067811865476f));
-    return make_float2(z * p, fmaf(z * 0.3989422804014327f, exp2_approx(-0.5f * kLog2e * z * z), p));
-  } else if constexpr (ACT == kActSilu) {
+  if constexpr (ACT == kActSilu) {
     const float s = recip_approx(1.0f + exp2_approx(-kLog2e * z));
     return make_float2(z * s, s * fmaf(z, 1.0f - s, 1.0f));
   } else {
@@ -123,6 +123,11 @@ __device__ __forceinline__ void activate_slope2(float2 z, float2& value, float2&
     const float2 rest = ffma2(make_float2(-s.x, -s.y), d, d);
     slope = ffma2(s, rest, s);
     if (VALUE) value = fmul2(z, s);
+  } else if constexpr (ACT == kActGelu) {
+    float2 bell;
+    const float2 p = normal_integral_pair(z, bell);
+    slope = ffma2(fmul2(z, both(0.3989422804014327f)), bell, p);
+    if (VALUE) value = fmul2(z, p);
   } else {
     const float2 a = activate_slope<ACT>(z.x), b = activate_slope<ACT>(z.y);
     value = make_float2(a.x, b.x);
@@ -387,7 +392,8 @@ __device__ __forceinline__ void activate_pairs(float2 (&v)[16]) {
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     if constexpr (ACT == kActGelu) {
-      v[j] = gelu_pair(v[j]);
+      float2 bell;
+      v[j] = fmul2(v[j], normal_integral_pair(v[j], bell));
     } else {
       // z / (1 + 2^w), each element by itself: a NaN stays in its column
       float2 w;
