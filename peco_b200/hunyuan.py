@@ -47,7 +47,7 @@ import torch.distributed as dist
 import torch.nn as nn
 import torch.nn.functional as F
 
-from .linear import linear_act
+from .linear import is_plain_linear, linear_act, without_hooks
 from .norms import modulated_norm
 from .processor import InferenceContext, PecoAttention, PecoConfig
 from .rotary import AxialPositions
@@ -110,6 +110,8 @@ class RowParallelLinear(nn.Module):
     """y = sum over ranks of x_r W_r^T, plus the bias: each rank holds the
     weight columns of its input features (``cols``, ranges of the full input)
     and one all-reduce adds the partial products."""
+
+    plain_linear = True  # (on one rank) the product and the bias alone
 
     def __init__(self, dim_out, full_in, cols, tp: TensorParallel):
         super().__init__()
@@ -238,26 +240,40 @@ class Attention(nn.Module):
 
 
 # Block operators (``use_block_operators``): the same block math through
-# linear_act, modulated_norm and table-free rotary positions.
+# linear_act, modulated_norm and table-free rotary positions.  A layer that is
+# more than a plain linear (a wrapper, an adapter, hooks) is called instead.
+
+def _linear(layer, x, activation=None):
+    """activation(layer(x)); ``activation`` None or "gelu_tanh"."""
+    if is_plain_linear(layer):
+        return linear_act(x, layer.weight, layer.bias, activation=activation)
+    y = layer(x)
+    return y if activation is None else F.gelu(y, approximate="tanh")
+
 
 def _modulation(layer, e, parts):
     """The modulation vectors [B, D] of a block, as views of one projection."""
-    return linear_act(e, layer.weight, layer.bias).unflatten(-1, (parts, -1)).unbind(1)
+    return _linear(layer, e).unflatten(-1, (parts, -1)).unbind(1)
 
 
 def _row_operator(layer, x, gate, residual, x2=None):
     """residual + gate * (layer([x | x2])) of a row-parallel layer; over several
     ranks the partial products are summed first."""
-    if layer.tp.world == 1:
+    if not is_plain_linear(layer):
+        return residual + gate[:, None] * layer(x if x2 is None else torch.cat((x, x2), -1))
+    tp = getattr(layer, "tp", SINGLE)
+    if tp.world == 1:
         return linear_act(x, layer.weight, layer.bias, gate=gate, residual=residual, x2=x2)
     y = linear_act(x, layer.weight, x2=x2)
-    dist.all_reduce(y, group=layer.tp.group)
+    dist.all_reduce(y, group=tp.group)
     return torch.addcmul(residual, gate[:, None], y + layer.bias)
 
 
 def _mlp_operator(ff, h, gate, residual):
-    hidden = linear_act(h, ff[0].weight, ff[0].bias, activation="gelu_tanh")
-    return _row_operator(ff[2], hidden, gate, residual)
+    as_built = type(ff) is nn.Sequential and len(ff) == 3 and type(ff[1]) is nn.GELU and ff[1].approximate == "tanh"
+    if not as_built or not without_hooks(ff) or not without_hooks(ff[1]):
+        return residual + gate[:, None] * ff(h)
+    return _row_operator(ff[2], _linear(ff[0], h, "gelu_tanh"), gate, residual)
 
 
 def _mlp(dim, ratio, tp: TensorParallel = SINGLE):
@@ -332,7 +348,7 @@ class SingleStreamBlock(nn.Module):
         x = torch.cat((img, txt), 1)
         shift, scale, gate = _modulation(self.mod, F.silu(temb), 3)
         h = modulated_norm(x, scale=scale, shift=shift)
-        mlp = linear_act(h, self.proj_mlp.weight, self.proj_mlp.bias, activation="gelu_tanh")
+        mlp = _linear(self.proj_mlp, h, "gelu_tanh")
         a_img, a_txt = self.attn(h[:, :n_img], h[:, n_img:], None, rope)
         x = _row_operator(self.proj_out, torch.cat((a_img, a_txt), 1), gate, x, x2=mlp)
         return x[:, :n_img], x[:, n_img:]

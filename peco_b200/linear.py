@@ -20,6 +20,8 @@ from torch.autograd.function import once_differentiable
 
 from . import _native
 
+_module = torch.nn.modules.module  # holds the hooks of all modules
+
 ACTIVATIONS = {None: 0, "none": 0, "gelu_tanh": 1, "gelu": 2, "silu": 3}
 
 
@@ -262,3 +264,21 @@ def linear_act_backward(grad, x, weight, *, preact=None, activation=None, gate=N
                      addr(dg), *sizes, _native.DTYPE_CODE[x.dtype], addr(ws), max(need, 0)),
                     (grad, preact, x, x2, weight, gate))
     return LinearGrads(dx, dx2, dw, db, dg)
+
+
+def without_hooks(module) -> bool:
+    """Whether calling ``module`` runs its class's ``forward`` and nothing else."""
+    return "forward" not in vars(module) and not (
+        module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks
+        or _module._global_forward_hooks or _module._global_forward_pre_hooks or _module._global_backward_hooks
+        or _module._global_backward_pre_hooks)
+
+
+def is_plain_linear(layer) -> bool:
+    """Whether ``linear_act(x, layer.weight, layer.bias)`` stands for ``layer(x)``:
+    an ``nn.Linear`` itself, or a class that says ``plain_linear`` of itself (not of
+    its subclasses), with an ordinary weight and no hooks.  Wrapped, adapted,
+    quantised and observed layers are to be called."""
+    kind = type(layer)
+    return (kind is torch.nn.Linear or vars(kind).get("plain_linear") is True) and \
+        type(layer.weight) in (torch.nn.Parameter, torch.Tensor) and without_hooks(layer)

@@ -30,7 +30,7 @@ import torch
 
 from . import _native
 from .clustering import kmeans_fit_pair, fit_token_clusters
-from .linear import linear_act
+from .linear import is_plain_linear, linear_act
 from .rotary import AxialPositions
 
 
@@ -314,7 +314,8 @@ class PecoAttention:
         ``image_rotary_emb``: the (cos, sin) tables, or a
         ``rotary.AxialPositions`` of the video rows, which are then rotated
         without tables.  A module with a true ``block_operators`` attribute has
-        its projections run by ``linear.linear_act``.
+        its projections run by ``linear.linear_act`` where they are plain
+        linear layers; others (adapted, quantised, with hooks) are called.
         """
         _native.require_cuda(hidden_states)
         n_text = 0 if encoder_hidden_states is None else encoder_hidden_states.shape[1]
@@ -376,12 +377,10 @@ class PecoAttention:
 
 
 def _project(layer, x):
-    """``layer(x)`` through linear_act where the layer is a linear map of this rank alone."""
-    weight = getattr(layer, "weight", None)
-    sharded = getattr(getattr(layer, "tp", None), "world", 1) > 1
-    if weight is None or weight.dim() != 2 or sharded:
+    """``layer(x)``, through linear_act where that computes the same: a linear map of this rank alone, without hooks."""
+    if not is_plain_linear(layer) or getattr(getattr(layer, "tp", None), "world", 1) > 1:
         return layer(x)
-    return linear_act(x, weight, layer.bias)
+    return linear_act(x, layer.weight, layer.bias)
 
 
 def _rms_gain(norm, dims):
