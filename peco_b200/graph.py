@@ -33,7 +33,8 @@ class PecoCallGraph:
     ``processor`` must already hold centroids (one eager call ran, or they were
     preset) and its context must be past the warm-up steps; every replay then
     performs the same work as one eager steady-state call on the new inputs.
-    The context's text lengths are frozen at capture.
+    The context's text lengths are frozen at capture.  ``centroids`` are the
+    (q, k) tensors the graph reads and writes.
     """
 
     def __init__(self, processor, query, key, value):
@@ -51,6 +52,8 @@ class PecoCallGraph:
         processor.q_centroids = processor.q_centroids.float().contiguous().clone()
         processor.k_centroids = processor.k_centroids.float().contiguous().clone()
         processor.update_centroids_in_place = True
+        # the graph's own references: the processor may take other centroids (another capture, a reset)
+        self.centroids = (processor.q_centroids, processor.k_centroids)
         self.graph = torch.cuda.CUDAGraph()
         events, processor.stage_events = processor.stage_events, None
         try:
@@ -59,11 +62,6 @@ class PecoCallGraph:
                 self.output = processor.attention(*self.inputs)
         finally:
             processor.stage_events = events
-
-    @property
-    def centroids(self):
-        """The (q, k) centroid tensors the graph reads and writes."""
-        return self.processor.q_centroids, self.processor.k_centroids
 
     def set_centroids(self, q_centroids, k_centroids):
         """Copy new centroids into the graph's state (e.g. to rerun from a fixed init)."""
@@ -111,6 +109,9 @@ class PecoStepGraph:
             p.q_centroids = p.q_centroids.float().contiguous().clone()
             p.k_centroids = p.k_centroids.float().contiguous().clone()
             p.update_centroids_in_place = True
+        # what the graph reads and writes and did not allocate itself lives as long as the graph, whatever the
+        # processors and the model take afterwards (another capture, a reset, another token grid)
+        self.kept = ([(p.q_centroids, p.k_centroids) for p in processors], getattr(model, "_rope", None))
         self.model = model
         self.frozen = (ctx.step, ctx.text_length, ctx.valid_text_length)
         self.inputs = tuple(t.detach().clone() if torch.is_tensor(t) else t for t in inputs)
