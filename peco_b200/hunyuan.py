@@ -183,7 +183,9 @@ class SDPAProcessor(PecoAttention):
             return norms[0](q), norms[1](k), v
 
         q, k, v = heads_of(video, (attn.to_q, attn.to_k, attn.to_v), (attn.norm_q, attn.norm_k))
-        if rope is not None:
+        if isinstance(rope, AxialPositions):
+            q, k = rope.checked(q.shape[2]).rotate(q, k)
+        elif rope is not None:
             q, k = rotate_pairs(q, *rope), rotate_pairs(k, *rope)
         if n_text:
             layers = (attn.add_q_proj, attn.add_k_proj, attn.add_v_proj) if separate else (attn.to_q, attn.to_k, attn.to_v)
@@ -240,8 +242,9 @@ class Attention(nn.Module):
 
 
 # Block operators (``use_block_operators``): the same block math through
-# linear_act, modulated_norm and table-free rotary positions.  A layer that is
-# more than a plain linear (a wrapper, an adapter, hooks) is called instead.
+# linear_act and modulated_norm (and, on request, rotary positions instead of
+# tables).  A layer that is more than a plain linear (a wrapper, an adapter,
+# hooks) is called instead.
 
 def _linear(layer, x, activation=None):
     """activation(layer(x)); ``activation`` None or "gelu_tanh"."""
@@ -379,7 +382,7 @@ class HunyuanVideoTransformer(nn.Module):
         super().__init__()
         self.cfg = cfg
         self.tp = tp
-        self.block_operators = False
+        self.rotary_positions = False
         d = cfg.hidden
         self.x_embedder = nn.Conv3d(cfg.in_channels, d, kernel_size=cfg.patch, stride=cfg.patch)
         self.context_embedder = nn.Linear(cfg.text_dim, d)
@@ -423,7 +426,7 @@ class HunyuanVideoTransformer(nn.Module):
         temb = self.time_in(_timestep_embedding(timestep).to(img.dtype)) + self.vector_in(pooled_projections)
         key = (grid, img.device)
         rope = self._rope.get(key) if hasattr(self, "_rope") else None
-        if self.block_operators:  # positions instead of tables
+        if self.rotary_positions:  # instead of tables
             rope = AxialPositions(self.cfg.rope_axes, self.cfg.rope_theta, grid=grid)
         elif rope is None:  # built once per grid (host tables copied to the device)
             rope = rope_3d(grid, self.cfg.rope_axes, self.cfg.rope_theta, img.device)
@@ -463,12 +466,18 @@ class Pipe:
         self.transformer = transformer
 
 
-def use_block_operators(transformer, enabled=True):
+def use_block_operators(transformer, enabled=True, positions=False):
     """Run every block's norms, modulation, projections, MLPs, gates and
-    residuals through ``modulated_norm`` and ``linear_act``, and rotate Q and K by
-    grid positions instead of tables.  For CUDA float16 / bfloat16 inference; the
-    attention processors stay as installed (their bfloat16 rule included)."""
-    transformer.block_operators = enabled
+    residuals through ``modulated_norm`` and ``linear_act``.  For CUDA float16 /
+    bfloat16 inference; the attention processors stay as installed (their
+    bfloat16 rule included).
+
+    ``positions``: Q and K turn by grid positions (``rotate``) instead of by
+    tables.  The processor's bfloat16 entry turns by tables inside its pass over
+    Q and K, whereas ``rotate`` is a pass of its own (135 us at 48 heads x 34680
+    rows; a step of 60 such blocks 822.5 ms by tables, 824.4 ms by positions):
+    tables are the faster form where they exist."""
+    transformer.rotary_positions = enabled and positions
     for block in [*transformer.transformer_blocks, *transformer.single_transformer_blocks]:
         block.block_operators = enabled
         block.attn.block_operators = enabled

@@ -313,7 +313,8 @@ class PecoAttention:
 
         ``image_rotary_emb``: the (cos, sin) tables, or a
         ``rotary.AxialPositions`` of the video rows, which are then rotated
-        without tables.  A module with a true ``block_operators`` attribute has
+        without tables (by a pass of its own: where there are tables, the
+        fused pass turns by them at no cost).  A module with a true ``block_operators`` attribute has
         its projections run by ``linear.linear_act`` where they are plain
         linear layers; others (adapted, quantised, with hooks) are called.
         """
@@ -340,8 +341,7 @@ class PecoAttention:
         cos = sin = None
         positions = image_rotary_emb if isinstance(image_rotary_emb, AxialPositions) else None
         if positions is not None:
-            if positions.rows != n_video:
-                raise ValueError(f"rotary positions of {positions.rows} rows for {n_video} video rows")
+            positions.checked(n_video)
         elif image_rotary_emb is not None:
             cos, sin = (t.to(device=hidden_states.device, dtype=torch.float32).reshape(n_video, dims).contiguous()
                         for t in image_rotary_emb)

@@ -186,6 +186,12 @@ class AxialPositions:
         """How many rows have positions."""
         return math.prod(self.grid) if self.grid is not None else self.positions.shape[-2]
 
+    def checked(self, rows: int) -> "AxialPositions":
+        """These positions, which have to be of exactly ``rows`` rows."""
+        if self.rows != rows:
+            raise ValueError(f"rotary positions of {self.rows} rows for {rows} video rows")
+        return self
+
     def rotate(self, q, k=None, **options):
         return rotate(q, k, axes=self.axes, theta=self.theta, grid=self.grid, positions=self.positions,
                       interleaved=self.interleaved, **options)

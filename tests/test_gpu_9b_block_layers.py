@@ -51,3 +51,41 @@ def test_hooks_run_and_change_the_result():
         got = model(*args)
         assert set(seen) == set(layers)
     assert _cosine(got, want) >= 0.9995 > _cosine(plain, want)
+
+
+def test_rotary_tables_stay_unless_positions_are_asked_for():
+    from peco_b200 import _native
+    model, args = _model_and_inputs()
+    blocks = CFG.dual_blocks + CFG.single_blocks
+    count = _native.load().peco_launch_count
+
+    def run():
+        before = count()
+        with torch.no_grad():
+            out = model(*args)
+        return out, count() - before
+
+    use_block_operators(model)
+    tables, launches = run()
+    use_block_operators(model, positions=True)
+    positions, more = run()
+    assert more == launches + blocks  # one pass over Q and K more in every block
+    # the fused pass rounds Q and K once, the two passes twice: one more bf16 rounding of Q and K
+    assert _cosine(tables, positions) >= 0.9995
+    use_block_operators(model, False)
+    assert torch.equal(run()[0], model(*args)) and not model.rotary_positions
+
+
+@pytest.mark.parametrize("positions", [False, True])
+def test_float16_model(positions):
+    # the processor computes a float16 module in plain torch; tolerance as above, float16 rounds finer
+    model, args = _model_and_inputs(torch.float16)
+    with torch.no_grad():
+        want = model(*args)
+        use_block_operators(model, positions=positions)
+        got = model(*args)
+        assert torch.isfinite(got).all() and _cosine(got, want) >= 0.9995
+        with pytest.raises(ValueError, match="rotary positions"):
+            from peco_b200.rotary import AxialPositions
+            short = AxialPositions(CFG.rope_axes, CFG.rope_theta, grid=(2, 8, 7))
+            model.transformer_blocks[0].attn(torch.zeros(1, 128, 256, device="cuda", dtype=torch.float16), None, None, short)
