@@ -62,7 +62,7 @@ def _run(q, k, axes, theta, grid, positions, interleaved, inverse, inplace):
             raise ValueError("inplace would turn q and k twice: they are one tensor")
     if d % 2 or not 2 <= d <= 256:
         raise ValueError("the head dimension must be even and at most 256")
-    sections = _sections(tuple(axes), d)
+    sections = _sections(axes, d)
     a = len(sections)
     if not (theta > 0 and math.isfinite(theta)):
         raise ValueError("theta must be positive")
@@ -71,7 +71,7 @@ def _run(q, k, axes, theta, grid, positions, interleaved, inverse, inplace):
     pos_p = pos_sb = pos_sn = pos_type = 0
     grid_c = None
     if grid is not None:
-        grid_c, turned = _grid(tuple(grid), a)
+        grid_c, turned = _grid(grid, a)
     else:
         if positions.dtype not in _POSITION_TYPES:
             raise TypeError("positions must be int32, int64 or float32")
@@ -127,24 +127,25 @@ def _source(t, d, inplace):
 
 class _Rotate(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, options):
+    def forward(ctx, q, k, positions, options):
         ctx.options = options
+        ctx.save_for_backward(positions)  # a change of them before the backward is an error
         ctx.set_materialize_grads(False)
-        q, k = _run(q, k, **options, inplace=False)
+        q, k = _run(q, k, positions=positions, **options, inplace=False)
         return q if k is None else (q, k)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
-        back = dict(ctx.options, inverse=not ctx.options["inverse"])
+        back = dict(ctx.options, inverse=not ctx.options["inverse"], positions=ctx.saved_tensors[0])
         gq, gk = (*grads, None)[:2]
         if gq is None and gk is None:
-            return None, None, None
+            return (None,) * 4
         if gq is None:
             gk, _ = _run(gk, None, **back, inplace=False)
         else:
             gq, gk = _run(gq, gk, **back, inplace=False)
-        return gq, gk, None
+        return gq, gk, None, None
 
 
 def rotate(q, k=None, *, axes, theta=256.0, grid=None, positions=None, interleaved=True, inverse=False,
@@ -160,12 +161,14 @@ def rotate(q, k=None, *, axes, theta=256.0, grid=None, positions=None, interleav
     ``inverse``: the opposite turn.  ``inplace`` (not under autograd)
     overwrites q and k.  Returns q, or (q, k).
     """
-    options = dict(axes=axes, theta=theta, grid=grid, positions=positions, interleaved=interleaved, inverse=inverse)
+    # fixed here: the backward turns by the same sections and grid
+    options = dict(axes=tuple(axes), theta=theta, grid=None if grid is None else tuple(grid), interleaved=interleaved,
+                   inverse=inverse)
     if torch.is_grad_enabled() and isinstance(q, torch.Tensor) and _native.wants_grad(q, k):
         if inplace:
             raise RuntimeError("rotate(inplace=True) does not record gradients; use torch.no_grad()")
-        return _Rotate.apply(q, k, options)
-    q, k = _run(q, k, **options, inplace=inplace)
+        return _Rotate.apply(q, k, positions, options)
+    q, k = _run(q, k, positions=positions, **options, inplace=inplace)
     return q if k is None else (q, k)
 
 
