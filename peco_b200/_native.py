@@ -12,6 +12,7 @@ import threading
 from pathlib import Path
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent / "libpeco_b200.so"
 _LOCK = threading.Lock()
@@ -163,6 +164,16 @@ def wants_grad(*inputs) -> bool:
         if t is not None and t.requires_grad:
             return True
     return False
+
+
+def refuse_tangents(what: str, *inputs) -> None:
+    """Raise if an input carries a forward-mode tangent: the operators have no
+    forward-mode derivative, and a result without one would be a silent zero."""
+    if getattr(_forward_ad, "_current_level", 0) < 0:  # no dual level is open
+        return
+    for t in inputs:
+        if isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 def address(t: torch.Tensor | None) -> int:

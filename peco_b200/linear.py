@@ -197,6 +197,7 @@ def linear_act(x, weight, bias=None, *, activation=None, gate=None, residual=Non
     (keep odd-width weights in padded rows to avoid that).  ``out`` (not under
     autograd) receives the result and may be ``residual``.
     """
+    _native.refuse_tangents("linear_act", x, weight, bias, gate, residual, x2)
     if torch.is_grad_enabled() and _native.wants_grad(x, weight, bias, gate, residual, x2):
         if out is not None:
             raise RuntimeError("linear_act(out=...) does not record gradients; use torch.no_grad()")
@@ -213,6 +214,7 @@ def linear_act_backward(grad, x, weight, *, preact=None, activation=None, gate=N
     layer has one.  ``needs``: names of the gradients to compute (default: all
     of x, x2, weight, bias, gate that are there).
     """
+    _native.refuse_tangents("linear_act_backward", grad, x, weight, preact, gate, x2)
     k, k2, n, samples = _check(x, weight, None, gate, grad, x2, activation)
     if needs is None:
         want_x, want_x2, want_w, want_b, want_g = True, x2 is not None, True, bool(bias), gate is not None

@@ -192,6 +192,7 @@ def modulated_norm(x, branch=None, *, gate=None, scale=None, shift=None, weight=
     variance) or "rms"; ``post_eps`` defaults to ``eps``.  Absent parts drop out
     of the formulas.
     """
+    _native.refuse_tangents("modulated_norm", x, branch, gate, scale, shift, weight, post_weight)
     if torch.is_grad_enabled() and _native.wants_grad(x, branch, gate, scale, shift, weight, post_weight):
         options = dict(norm=norm, post_norm=post_norm, eps=eps, post_eps=post_eps, residual_scale=residual_scale)
         return _ModulatedNorm.apply(x, branch, gate, scale, shift, weight, post_weight, options)
@@ -206,6 +207,8 @@ def modulated_norm_backward(grad_normed, grad_residual, x, branch=None, *, gate=
     """Gradients of ``modulated_norm`` for ``grad_normed`` = d h and
     ``grad_residual`` = d r (None: zero).  ``needs``: names of the gradients to
     compute (default: those of all inputs that are there)."""
+    _native.refuse_tangents("modulated_norm_backward", grad_normed, grad_residual, x, branch, gate, scale, shift, weight,
+                            post_weight)
     _check(x, branch, gate, scale, shift, weight, post_weight, norm, post_norm, eps, post_eps, residual_scale)
     if grad_normed is None:
         raise ValueError("grad_normed is required")

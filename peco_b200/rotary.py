@@ -161,6 +161,7 @@ def rotate(q, k=None, *, axes, theta=256.0, grid=None, positions=None, interleav
     ``inverse``: the opposite turn.  ``inplace`` (not under autograd)
     overwrites q and k.  Returns q, or (q, k).
     """
+    _native.refuse_tangents("rotate", q, k, positions)
     # fixed here: the backward turns by the same sections and grid
     options = dict(axes=tuple(axes), theta=theta, grid=None if grid is None else tuple(grid), interleaved=interleaved,
                    inverse=inverse)

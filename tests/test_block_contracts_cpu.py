@@ -1,0 +1,33 @@
+"""What the block operators refuse before they look for a device."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+from peco_b200.linear import linear_act, linear_act_backward
+from peco_b200.norms import modulated_norm, modulated_norm_backward
+from peco_b200.rotary import rotate
+
+
+def test_forward_mode_tangents_are_refused():
+    x = torch.zeros(1, 4, 16, dtype=torch.bfloat16)
+    w, v = torch.zeros(16, 16, dtype=torch.bfloat16), torch.zeros(16, dtype=torch.bfloat16)
+    rot = dict(axes=(16,), grid=(4,))
+    calls = [
+        lambda dual: linear_act(dual(x), w), lambda dual: linear_act(x, dual(w)), lambda dual: linear_act(x, w, dual(v)),
+        lambda dual: linear_act(x, w, gate=dual(v)), lambda dual: linear_act(x, w, residual=dual(x)),
+        lambda dual: linear_act_backward(dual(x), x, w), lambda dual: linear_act_backward(x, x, w, preact=dual(x), activation="silu"),
+        lambda dual: modulated_norm(dual(x)), lambda dual: modulated_norm(x, dual(x)), lambda dual: modulated_norm(x, scale=dual(v)),
+        lambda dual: modulated_norm(x, weight=dual(v)), lambda dual: modulated_norm_backward(dual(x), None, x),
+        lambda dual: modulated_norm_backward(x, None, x, shift=dual(v)),
+        lambda dual: rotate(dual(x[None]), **rot), lambda dual: rotate(x[None], dual(x[None]), **rot),
+    ]
+    with forward_ad.dual_level():
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(lambda t: forward_ad.make_dual(t, torch.ones_like(t)))
+            with pytest.raises(RuntimeError, match="CUDA"):  # an open level alone changes nothing
+                call(lambda t: t)
+    for call in calls:
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call(lambda t: t)
