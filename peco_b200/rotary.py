@@ -155,13 +155,15 @@ def rotate(q, k=None, *, axes, theta=256.0, grid=None, positions=None, interleav
     ``axes``: dimensions of each axis's section, in order, e.g. (16, 56, 56);
     dimensions after them are copied.  ``grid``: sizes of a row-major token
     grid that the first prod(grid) rows walk; or ``positions`` [N', axes] /
-    [B, N', axes] (int32, int64 or float32) of the first N' rows.  Later rows
+    [B, N', axes] (int32, int64 or float32; no gradient) of the first N' rows.  Later rows
     (the text) are copied.  ``interleaved``: pairs (2i, 2i+1), else one from
     each half of the rotated dimensions.  Angles are position * theta^(-2j/d).
     ``inverse``: the opposite turn.  ``inplace`` (not under autograd)
     overwrites q and k.  Returns q, or (q, k).
     """
     _native.refuse_tangents("rotate", q, k, positions)
+    if isinstance(positions, torch.Tensor) and positions.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("rotate has no gradient of positions; detach them")
     # fixed here: the backward turns by the same sections and grid
     options = dict(axes=tuple(axes), theta=theta, grid=None if grid is None else tuple(grid), interleaved=interleaved,
                    inverse=inverse)

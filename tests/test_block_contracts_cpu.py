@@ -31,3 +31,14 @@ def test_forward_mode_tangents_are_refused():
     for call in calls:
         with pytest.raises(RuntimeError, match="CUDA"):
             call(lambda t: t)
+
+
+def test_positions_that_want_a_gradient_are_refused():
+    q, pos = torch.zeros(1, 1, 4, 16), torch.zeros(4, 1, requires_grad=True)
+    for x in (q, q.clone().requires_grad_()):
+        with pytest.raises(RuntimeError, match="gradient of positions"):
+            rotate(x, axes=(16,), positions=pos)
+        with pytest.raises(RuntimeError, match="CUDA"):
+            rotate(x, axes=(16,), positions=pos.detach())
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+        rotate(q, axes=(16,), positions=pos)
