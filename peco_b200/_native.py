@@ -166,6 +166,12 @@ def wants_grad(*inputs) -> bool:
     return False
 
 
+def wrote(*outputs) -> None:
+    """Tell autograd that these tensors of the caller's were overwritten: a
+    backward that saved one of them fails instead of using the new values."""
+    torch.autograd.graph.increment_version(outputs)
+
+
 def refuse_tangents(what: str, *inputs) -> None:
     """Raise if an input carries a forward-mode tangent: the operators have no
     forward-mode derivative, and a result without one would be a silent zero."""

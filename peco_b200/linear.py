@@ -115,7 +115,8 @@ def _misaligned(ptrs: int, strides: int) -> bool:
 def _forward(x, weight, bias, gate, residual, x2, activation, out, want_preact):
     k, k2, n, samples = _check(x, weight, bias, gate, residual, x2, activation)
     shape = (*x.shape[:-1], n)
-    if out is None:
+    given = out is not None
+    if not given:
         out = out_rows = x.new_empty(shape)
         out_step = n
     else:
@@ -159,6 +160,8 @@ def _forward(x, weight, bias, gate, residual, x2, activation, out, want_preact):
                      _native.address(preact), samples, per, k, k2, n, ACTIVATIONS[activation],
                      _native.DTYPE_CODE[x.dtype], _native.address(ws), max(need, 0)),
                     (x, weight, bias, gate, residual, x2, out))
+    if given:
+        _native.wrote(out)
     return out, preact
 
 

@@ -101,6 +101,8 @@ def _run(q, k, axes, theta, grid, positions, interleaved, inverse, inplace):
     _native.enqueue(device, "peco_rotary", _native.load().peco_rotary,
                     (*q_args, *k_args, b, n, turned, d, sections, a, theta, grid_c, pos_p, pos_sb, pos_sn, pos_type,
                      1 if interleaved else 0, 1 if inverse else 0, code), (q, k, positions))
+    if inplace:
+        _native.wrote(q_out, *(() if k is None else (k_out,)))
     return q_out, k_out
 
 
