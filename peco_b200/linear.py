@@ -201,7 +201,7 @@ def linear_act(x, weight, bias=None, *, activation=None, gate=None, residual=Non
     autograd) receives the result and may be ``residual``.
     """
     _native.refuse_tangents("linear_act", x, weight, bias, gate, residual, x2)
-    if torch.is_grad_enabled() and _native.wants_grad(x, weight, bias, gate, residual, x2):
+    if torch.is_grad_enabled() and _native.wants_grad(x, weight, bias, gate, residual, x2, out):
         if out is not None:
             raise RuntimeError("linear_act(out=...) does not record gradients; use torch.no_grad()")
         return _LinearAct.apply(x, weight, bias, gate, residual, x2, activation)

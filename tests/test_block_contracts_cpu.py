@@ -42,3 +42,12 @@ def test_positions_that_want_a_gradient_are_refused():
             rotate(x, axes=(16,), positions=pos.detach())
     with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
         rotate(q, axes=(16,), positions=pos)
+
+
+def test_out_that_wants_a_gradient_is_refused():
+    x, w = torch.zeros(4, 16, dtype=torch.bfloat16), torch.zeros(8, 16, dtype=torch.bfloat16)
+    out = torch.zeros(4, 8, dtype=torch.bfloat16, requires_grad=True)
+    with pytest.raises(RuntimeError, match="does not record gradients"):
+        linear_act(x, w, out=out)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+        linear_act(x, w, out=out)
