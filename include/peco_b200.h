@@ -247,7 +247,8 @@ int peco_exchange_wait(const long long* flags, int world, int flag_slot, long lo
  * one for all); either and residual may be null.  preact, if given, [rows, n]
  * contiguous, receives the pre-activation.  activation 0 none, 1 gelu (tanh
  * form), 2 gelu (erf), 3 silu; dtype 0 fp16, 1 bf16.  Sums are fp32, each
- * output is rounded once.  out may be residual.  Operands whose base or row
+ * output is rounded once.  out may be residual (the same rows) and shares no
+ * memory with the operands otherwise.  Operands whose base or row
  * stride is not a multiple of 16 bytes are copied into ``workspace`` first:
  * peco_linear_forward_workspace says how many bytes (0 when all are aligned;
  * -1: sizes out of range). */

@@ -172,6 +172,25 @@ def wrote(*outputs) -> None:
     torch.autograd.graph.increment_version(outputs)
 
 
+def rows_overlap(a, b) -> bool:
+    """Whether two sets of rows (address, rows, step, width; integers of one unit,
+    rows and width positive) have an element in common."""
+    (pa, na, sa, wa), (pb, nb, sb, wb) = a, b
+    sa, sb = sa if na > 1 else wa, sb if nb > 1 else wb
+    if pa >= pb + (nb - 1) * sb + wb or pb >= pa + (na - 1) * sa + wa:
+        return False
+    if sa == sb:  # columns of one buffer
+        apart = (pa - pb) % sa
+        if apart >= wb and sa - apart >= wa:
+            return False
+    if na > nb:
+        (pa, na, sa, wa), (pb, nb, sb, wb) = (pb, nb, sb, wb), (pa, na, sa, wa)
+    # the first row of b that ends behind the start of each row of a
+    start = torch.arange(na, dtype=torch.int64) * sa + (pa - pb)
+    j = ((start - wb).div(sb, rounding_mode="floor") + 1).clamp_(min=0)
+    return bool(((j < nb) & (j * sb < start + wa)).any())
+
+
 def refuse_tangents(what: str, *inputs) -> None:
     """Raise if an input carries a forward-mode tangent: the operators have no
     forward-mode derivative, and a result without one would be a silent zero."""

@@ -107,6 +107,18 @@ def _weight_rows(weight):
     return weight.contiguous(), k
 
 
+def _check_out(out, operands):
+    """Refuse an ``out`` (address in elements, rows, step, width) that shares memory with an operand, which other
+    parts of the product may read after its first results are written; the residual's own rows alone may be it."""
+    for name, t, rows, step, width in operands:
+        if t is None:
+            continue
+        other = (t.data_ptr() // 2, rows, step, width)
+        same_rows = other[0] == out[0] and (step == out[2] or rows == 1)
+        if not (name == "residual" and same_rows) and _native.rows_overlap(out, other):
+            raise ValueError(f"out shares memory with {name}")
+
+
 def _misaligned(ptrs: int, strides: int) -> bool:
     """Whether some operand may not start every row on 16 bytes."""
     return bool(ptrs & 15 or strides & 7)
@@ -150,6 +162,11 @@ def _forward(x, weight, bias, gate, residual, x2, activation, out, want_preact):
     if residual is not None:
         residual, r_step = _rows(residual, n)
         rp = residual.data_ptr()
+    if given:
+        _check_out((out_rows.data_ptr() // 2, rows, out_step, n),
+                   (("x", x, rows, x_step, k), ("x2", x2, rows, x2_step, k2), ("weight", weight, n, w_step, k + k2),
+                    ("bias", bias, 1, n, n), ("gate", gate, samples if g_step else 1, g_step, n),
+                    ("residual", residual, rows, r_step, n)))
     lib = _native.load()
     per, need, ws = rows // samples, 0, None
     if _misaligned(xp | wp | x2p, x_step | w_step | x2_step | (k if k2 else 0)):
@@ -198,7 +215,8 @@ def linear_act(x, weight, bias=None, *, activation=None, gate=None, residual=Non
     for each sample of x [B, ..., K]; residual [..., N].  Row strides are free;
     operands whose rows do not start on 16-byte boundaries are copied first
     (keep odd-width weights in padded rows to avoid that).  ``out`` (not under
-    autograd) receives the result and may be ``residual``.
+    autograd) receives the result; it may be ``residual`` and may share no
+    memory with the operands otherwise.
     """
     _native.refuse_tangents("linear_act", x, weight, bias, gate, residual, x2)
     if torch.is_grad_enabled() and _native.wants_grad(x, weight, bias, gate, residual, x2, out):

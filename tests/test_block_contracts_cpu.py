@@ -1,9 +1,12 @@
 """What the block operators refuse before they look for a device."""
 
+import random
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
+from peco_b200 import _native
 from peco_b200.linear import linear_act, linear_act_backward
 from peco_b200.norms import modulated_norm, modulated_norm_backward
 from peco_b200.rotary import rotate
@@ -51,3 +54,24 @@ def test_out_that_wants_a_gradient_is_refused():
         linear_act(x, w, out=out)
     with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
         linear_act(x, w, out=out)
+
+
+def test_rows_overlap_against_every_element():
+    rng = random.Random(0)
+    seen = [0, 0]
+    for _ in range(4000):
+        sets = []
+        for _ in range(2):
+            width = rng.randint(1, 6)
+            sets.append((rng.randint(0, 60), rng.randint(1, 7), rng.randint(width, 14), width))
+        if rng.random() < 0.5:  # columns of one buffer
+            step = max(sets[0][2], sets[1][2])
+            sets = [(p, n, step, w) for p, n, _, w in sets]
+        a, b = ({p + i * s + j for i in range(n) for j in range(w)} for p, n, s, w in sets)
+        assert _native.rows_overlap(*sets) == bool(a & b) == _native.rows_overlap(*sets[::-1]), sets
+        seen[bool(a & b)] += 1
+    assert min(seen) > 500
+    big = 1 << 40  # rows of a long buffer
+    assert not _native.rows_overlap((big, 1 << 20, 4096, 2048), (big + 2048, 1 << 20, 4096, 2048))
+    assert _native.rows_overlap((big, 1 << 20, 4096, 2048), (big + 2047, 1 << 20, 4096, 2048))
+    assert _native.rows_overlap((big, 1 << 20, 4096, 2049), (big + 2048, 7, 8192, 2048))

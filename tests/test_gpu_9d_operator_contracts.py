@@ -53,3 +53,33 @@ def test_written_tensors_are_known_to_autograd():
         out = torch.empty(4, 8, device=DEV, dtype=torch.bfloat16)
         assert linear_act(x, w, out=out) is out
         rotate(torch.ones(1, 2, 4, 16, device=DEV), axes=(16,), grid=(4,), inplace=True)
+
+
+def test_out_shares_no_memory_with_the_operands():
+    m, k, n = 40, 16, 16
+    x, w = torch.randn(m, k, device=DEV).bfloat16(), torch.randn(n, k, device=DEV).bfloat16()
+    vec = torch.randn(n, device=DEV).bfloat16()
+    wide = torch.randn(m + 1, 3 * n, device=DEV).bfloat16()
+    left, mid, right = (wide[:m, i * n:(i + 1) * n] for i in range(3))
+    below = wide[1:, n:2 * n]
+    flat = torch.randn(2 * m * n, device=DEV).bfloat16()
+    for kw in (dict(x=x, weight=w, out=x), dict(x=left, weight=w, out=left), dict(x=left, weight=w, out=wide[:m, 8:8 + n]),
+               dict(x=left, weight=w, x2=mid, out=mid), dict(x=x[:n], weight=w, out=w), dict(x=x[:1], weight=w, bias=vec, out=vec[None]),
+               dict(x=x[:1], weight=w, gate=vec, out=vec[None]), dict(x=x, weight=w, residual=mid, out=below),
+               dict(x=x, weight=w, residual=flat[:m * n].view(m, n), out=flat[n:(m + 1) * n].view(m, n)),
+               dict(x=x, weight=w, residual=flat[:m * n].view(m, n), out=flat.view(m, 2 * n)[:, :n])):
+        kw = {key: torch.cat((t, t), 1) if key == "weight" and "x2" in kw else t for key, t in kw.items()}
+        before = [t.clone() for t in kw.values()]
+        with pytest.raises(ValueError, match="out shares memory with"):
+            linear_act(**kw)
+        assert all(torch.equal(a, b) for a, b in zip(before, kw.values()))
+    # neighbours in one buffer, and the residual itself
+    ref = linear_act(left, w, residual=right)
+    assert linear_act(left, w, residual=right, out=mid) is mid and torch.equal(mid, ref)
+    assert torch.equal(linear_act(left, w, residual=right, out=right), ref)
+    ref = linear_act(x[:1], w, residual=wide[:1, :n])
+    assert torch.equal(linear_act(x[:1], w, residual=wide[:1, :n], out=wide[0, :n][None]), ref)
+    # an operand that has to be copied is read from its copy
+    square = torch.randn(n, n, device=DEV).bfloat16()
+    ref = linear_act(square.t(), w)
+    assert torch.equal(linear_act(square.t(), w, out=square), ref)
