@@ -58,8 +58,6 @@ def _run(q, k, axes, theta, grid, positions, interleaved, inverse, inplace):
             raise ValueError("q and k must agree in batch, tokens and head dimension")
         if k.dtype is not dtype:
             raise TypeError("q and k must have one dtype")
-        if inplace and k.data_ptr() == q.data_ptr() and q.numel():
-            raise ValueError("inplace would turn q and k twice: they are one tensor")
     if d % 2 or not 2 <= d <= 256:
         raise ValueError("the head dimension must be even and at most 256")
     sections = _sections(axes, d)
@@ -98,12 +96,38 @@ def _run(q, k, axes, theta, grid, positions, interleaved, inverse, inplace):
     k_out, k_args = None, (0, 0, 0, None)
     if k is not None:
         k, k_out, k_args = _source(k, d, inplace)
+        if inplace and _share_memory(q, k):
+            raise ValueError("inplace would turn elements twice: q and k share memory")
     _native.enqueue(device, "peco_rotary", _native.load().peco_rotary,
                     (*q_args, *k_args, b, n, turned, d, sections, a, theta, grid_c, pos_p, pos_sb, pos_sn, pos_type,
                      1 if interleaved else 0, 1 if inverse else 0, code), (q, k, positions))
     if inplace:
         _native.wrote(q_out, *(() if k is None else (k_out,)))
     return q_out, k_out
+
+
+def _share_memory(q, k) -> bool:
+    """Whether q and k [B, H, N, D] (adjacent dimensions, no expanded axes) have an element in common."""
+    if not q.numel() or not k.numel():
+        return False
+    (b, hq, n, d), hk, size = q.shape, k.shape[1], q.element_size()
+    pq, pk, width = q.data_ptr(), k.data_ptr(), d * size
+    (qb, qh, qn), (kb, kh, kn) = ([t.stride(i) * size for i in range(3)] for t in (q, k))
+    if pq >= pk + (b - 1) * kb + (hk - 1) * kh + (n - 1) * kn + width or \
+            pk >= pq + (b - 1) * qb + (hq - 1) * qh + (n - 1) * qn + width:
+        return False
+    if (b == 1 or qb == kb) and (hq == 1 or hk == 1 or qh == kh) and (n == 1 or qn == kn):
+        # parts of one buffer: only the difference of two rows' batches and heads counts
+        qs = (pq, n, qn, width)
+        if hq > 1 and hk > 1 or hq == hk:
+            places = {i * qb + j * qh for i in range(1 - b, b) for j in range(1 - hq, hk)}
+        elif hq == 1:
+            places = {i * qb + j * kh for i in range(1 - b, b) for j in range(hk)}
+        else:
+            places = {i * qb - j * qh for i in range(1 - b, b) for j in range(hq)}
+        return any(_native.rows_overlap((pk + at, n, kn, width), qs) for at in places)
+    return any(_native.rows_overlap((pq + i * qb + j * qh, n, qn, width), (pk + x * kb + y * kh, n, kn, width))
+               for i in range(b) for j in range(hq) for x in range(b) for y in range(hk))
 
 
 def _source(t, d, inplace):
@@ -161,7 +185,7 @@ def rotate(q, k=None, *, axes, theta=256.0, grid=None, positions=None, interleav
     (the text) are copied.  ``interleaved``: pairs (2i, 2i+1), else one from
     each half of the rotated dimensions.  Angles are position * theta^(-2j/d).
     ``inverse``: the opposite turn.  ``inplace`` (not under autograd)
-    overwrites q and k.  Returns q, or (q, k).
+    overwrites q and k, which share no memory then.  Returns q, or (q, k).
     """
     _native.refuse_tangents("rotate", q, k, positions)
     if isinstance(positions, torch.Tensor) and positions.requires_grad and torch.is_grad_enabled():

@@ -9,7 +9,7 @@ import torch.autograd.forward_ad as forward_ad
 from peco_b200 import _native
 from peco_b200.linear import linear_act, linear_act_backward
 from peco_b200.norms import modulated_norm, modulated_norm_backward
-from peco_b200.rotary import rotate
+from peco_b200.rotary import _share_memory, rotate
 
 
 def test_forward_mode_tangents_are_refused():
@@ -75,3 +75,38 @@ def test_rows_overlap_against_every_element():
     assert not _native.rows_overlap((big, 1 << 20, 4096, 2048), (big + 2048, 1 << 20, 4096, 2048))
     assert _native.rows_overlap((big, 1 << 20, 4096, 2048), (big + 2047, 1 << 20, 4096, 2048))
     assert _native.rows_overlap((big, 1 << 20, 4096, 2049), (big + 2048, 7, 8192, 2048))
+
+
+def test_shared_memory_of_queries_and_keys_against_every_element():
+    """Views of one small buffer in the layouts of attention calls, and arbitrary ones."""
+    rng = random.Random(1)
+    buffer = torch.arange(4096, dtype=torch.float32)
+    seen = [0, 0]
+
+    def elements(t):
+        return set(t.reshape(-1).tolist())
+
+    def view(b, h, n, d):
+        order = rng.sample(range(3), 3)     # which of batch, head and token runs innermost
+        strides, step = [0, 0, 0], d + rng.choice((0, 0, 3))
+        for axis in order:
+            strides[axis] = step
+            step *= (b, h, n)[axis] + rng.choice((0, 0, 1))
+        return torch.as_strided(buffer, (b, h, n, d), (*strides, 1), rng.randint(0, 120))
+
+    for _ in range(3000):
+        b, n, d = rng.randint(1, 2), rng.randint(1, 4), 2 * rng.randint(1, 2)
+        if rng.random() < 0.5:              # heads of one projection, [B, N, heads, D] or [B, heads, N, D]
+            heads = 5
+            whole = torch.as_strided(buffer, (b, n, heads, d), (n * heads * d, heads * d, d, 1)).transpose(1, 2) \
+                if rng.random() < 0.5 else torch.as_strided(buffer, (b, heads, n, d), (heads * n * d, n * d, d, 1))
+            cut, end = sorted(rng.sample(range(1, heads + 1), 2))
+            start = rng.randint(0, cut)
+            q, k = whole[:, :cut], whole[:, start if start < end else cut:end]
+        else:
+            q, k = view(b, rng.randint(1, 3), n, d), view(b, rng.randint(1, 3), n, d)
+        common = bool(elements(q) & elements(k))
+        assert _share_memory(q, k) == common == _share_memory(k, q), (q.shape, q.stride(), k.shape, k.stride())
+        seen[common] += 1
+    assert min(seen) > 300
+    assert not _share_memory(buffer[:0].view(1, 0, 4, 2), buffer[:8].view(1, 1, 4, 2))

@@ -83,3 +83,19 @@ def test_out_shares_no_memory_with_the_operands():
     square = torch.randn(n, n, device=DEV).bfloat16()
     ref = linear_act(square.t(), w)
     assert torch.equal(linear_act(square.t(), w, out=square), ref)
+
+
+def test_inplace_queries_and_keys_share_no_memory():
+    opts = dict(axes=(8, 8), grid=(2, 3))
+    qkv = torch.randn(2, 7, 10, 16, device=DEV)                   # token rows of 10 heads
+    heads = qkv.transpose(1, 2)
+    keep = qkv.clone()
+    for q, k in ((heads[:, :4], heads[:, 3:6]), (heads[:, 2:6], heads[:, :3]), (heads, heads[:, 9:]), (heads[:1], heads[:1]),
+                 (heads[:, :1], heads[:, 1:2].as_strided((2, 1, 7, 16), (1120, 160, 80, 1), 80))):
+        with pytest.raises(ValueError, match="share memory"):
+            rotate(q, k, **opts, inplace=True)
+    assert torch.equal(qkv, keep)
+    want_q, want_k = rotate(heads[:, :6], heads[:, 6:8], **opts)  # neighbours in one buffer
+    q, k = rotate(heads[:, :6], heads[:, 6:8], **opts, inplace=True)
+    assert torch.equal(q, want_q) and torch.equal(k, want_k)
+    assert torch.equal(qkv[:, :, 8:], keep[:, :, 8:])
