@@ -238,7 +238,8 @@ int peco_exchange_put(const void* src, const long long* src_offsets, const int* 
 int peco_exchange_wait(const long long* flags, int world, int flag_slot, long long epoch, void* stream);
 
 /* ---- transformer-block operators (no counterpart in the reference, whose
- * blocks are the host framework's) ------------------------------------------ */
+ * blocks are the host framework's) ------------------------------------------
+ * Workspaces start on 16 bytes. */
 
 /* out = residual + gate * act([x | x2] W^T + bias) over samples *
  * rows_per_sample rows.  x [rows, k], x2 [rows, k2] (k2 = 0: absent), weight
@@ -248,8 +249,8 @@ int peco_exchange_wait(const long long* flags, int world, int flag_slot, long lo
  * contiguous, receives the pre-activation.  activation 0 none, 1 gelu (tanh
  * form), 2 gelu (erf), 3 silu; dtype 0 fp16, 1 bf16.  Sums are fp32, each
  * output is rounded once.  out may be residual (the same rows) and shares no
- * memory with the operands otherwise.  Operands whose base or row
- * stride is not a multiple of 16 bytes are copied into ``workspace`` first:
+ * memory with the operands otherwise.  Operands whose base or row stride is
+ * not a multiple of 16 bytes are copied into ``workspace`` first:
  * peco_linear_forward_workspace says how many bytes (0 when all are aligned;
  * -1: sizes out of range). */
 int peco_linear_forward(const void* x, long long x_stride, const void* x2, long long x2_stride, const void* weight,

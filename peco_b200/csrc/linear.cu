@@ -1465,7 +1465,7 @@ extern "C" int peco_linear_forward(const void* x, long long x_stride, const void
     return kErrInvalidValue;
   const long long need =
       peco_linear_forward_workspace(x, x_stride, x2, x2_stride, weight, w_stride, samples, rows_per_sample, k, k2, n);
-  if (need > 0 && (!workspace || workspace_bytes < need)) return kErrWorkspace;
+  if (need > 0 && !usable_workspace(workspace, workspace_bytes, need)) return kErrWorkspace;
   Operand a[2], b[2];
   make_operands(s, x, x_stride, x2, x2_stride, weight, w_stride, a, b);
   GemmArgs g{};
@@ -1522,7 +1522,7 @@ extern "C" int peco_linear_backward(const void* grad, long long grad_stride, con
   if ((activation != kActNone || dgate) && !preact) return kErrInvalidValue;
   const long long need = peco_linear_backward_workspace(grad, grad_stride, x, x_stride, x2, x2_stride, weight, w_stride,
                                                         samples, rows_per_sample, k, k2, n, activation, gate != nullptr);
-  if (need > 0 && (!workspace || workspace_bytes < need)) return kErrWorkspace;
+  if (need > 0 && !usable_workspace(workspace, workspace_bytes, need)) return kErrWorkspace;
   Operand a[2], b[2];
   make_operands(s, x, x_stride, x2, x2_stride, weight, w_stride, a, b);
   const Operand g{grad, grad_stride, static_cast<int>(s.rows()), n};

@@ -984,7 +984,7 @@ extern "C" int peco_gated_norm_backward(
       (dpost_weight && !post_weight))
     return kErrInvalidValue;
   const bool sums = dgate || dscale || dshift || dweight || dpost_weight;
-  if (sums && (!workspace || workspace_bytes < peco_gated_norm_backward_workspace(samples, rows, width)))
+  if (sums && !usable_workspace(workspace, workspace_bytes, peco_gated_norm_backward_workspace(samples, rows, width)))
     return kErrWorkspace;
   NormArgs a{};
   a.x = RowTensor{x, x_batch, x_row};

@@ -47,6 +47,11 @@ __device__ __forceinline__ void load8(const T* p, int vec, int count, float (&v)
 __device__ __forceinline__ void wait_for_prior() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// A caller's workspace: large enough, and on the 16 bytes that vector stores and TMA start on.
+inline bool usable_workspace(const void* workspace, long long bytes, long long need) {
+  return workspace && bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0;
+}
+
 // Launch of a kernel that begins with wait_for_prior().
 template <typename... P, typename... A>
 int launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t stream, A... args) {
