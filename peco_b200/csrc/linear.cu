@@ -1518,7 +1518,7 @@ extern "C" int peco_linear_backward(const void* grad, long long grad_stride, con
   if (!grad || grad_stride < n || gate_stride < 0) return kErrInvalidValue;
   if ((dx || dx2) && (!weight || w_stride < static_cast<long long>(k) + k2)) return kErrInvalidValue;
   if (dweight && (!x || x_stride < k || (k2 > 0 && (!x2 || x2_stride < k2)))) return kErrInvalidValue;
-  if (dx2 && k2 == 0) return kErrInvalidValue;
+  if ((dx2 && k2 == 0) || (dgate && !gate)) return kErrInvalidValue;
   if ((activation != kActNone || dgate) && !preact) return kErrInvalidValue;
   const long long need = peco_linear_backward_workspace(grad, grad_stride, x, x_stride, x2, x2_stride, weight, w_stride,
                                                         samples, rows_per_sample, k, k2, n, activation, gate != nullptr);

@@ -28,3 +28,11 @@ def test_workspaces_start_on_sixteen_bytes(lib):
         assert lib.peco_gated_norm_backward(p, 64, 16, z, 0, 0, p, 64, 16, z, 0, 0, z, 0, p, 0, z, z, p, z, z, p, z, 0, z, z,
                                             1, 4, 16, 1, 0, 1e-6, 1e-6, 1.0, 1, at, 1 << 20, s) == WORKSPACE
     assert lib.peco_launch_count() == launches
+
+
+def test_a_gate_gradient_needs_a_gate(lib):
+    p, z = 1 << 20, 0
+    launches = lib.peco_launch_count()
+    # without one its sums would be read before they are written
+    assert lib.peco_linear_backward(p, 8, p, p, 16, z, 0, p, 16, z, 0, z, z, z, z, p, 1, 2, 16, 0, 8, 1, 1, p, 1 << 20, 0) == 1
+    assert lib.peco_launch_count() == launches
