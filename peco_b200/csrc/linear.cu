@@ -970,8 +970,11 @@ __global__ void __launch_bounds__(256, GATE ? 3 : 4) act_backward_kernel(const _
   wait_for_prior();
   let_next_start();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int sample = blockIdx.y / a.chunks, chunk = blockIdx.y - sample * a.chunks;
-  const int col = blockIdx.x * 256 + lane * 8;
+  // a one-dimensional grid, the column blocks of a chunk side by side: as many samples as there are rows
+  const unsigned col_blocks = (static_cast<unsigned>(a.n) + 255) / 256;
+  const int piece = blockIdx.x / col_blocks, col0 = (blockIdx.x - piece * col_blocks) * 256;
+  const int sample = piece / a.chunks, chunk = piece - sample * a.chunks;
+  const int col = col0 + lane * 8;
   const int count = min(8, a.n - col);
   constexpr bool kValue = ACT != kActNone || GATE;  // the pre-activation is read
   float2 gate[4], sum_dz[4], sum_ga[4];
@@ -1038,7 +1041,7 @@ __global__ void __launch_bounds__(256, GATE ? 3 : 4) act_backward_kernel(const _
     if (GATE) *reinterpret_cast<float2*>(&red[GATE ? 1 : 0][warp][lane * 8 + 2 * i]) = sum_ga[i];
   }
   __syncthreads();
-  const int c = blockIdx.x * 256 + threadIdx.x;
+  const int c = col0 + threadIdx.x;
   if (c < a.n) {
     float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
@@ -1046,7 +1049,7 @@ __global__ void __launch_bounds__(256, GATE ? 3 : 4) act_backward_kernel(const _
       s0 += red[0][w][threadIdx.x];
       if (GATE) s1 += red[GATE ? 1 : 0][w][threadIdx.x];
     }
-    const long long at = static_cast<long long>(blockIdx.y) * a.n + c;
+    const long long at = static_cast<long long>(piece) * a.n + c;
     if (a.part_bias) a.part_bias[at] = s0;
     if (GATE && a.part_gate) a.part_gate[at] = s1;
   }
@@ -1310,9 +1313,8 @@ int backward_chunks(const LinearShape& s, bool gate) {
       chunks = c;
     }
   }
-  const long long shortest = (s.rows_per_sample + 15) / 16, cap = 65535 / s.samples;
+  const long long shortest = (s.rows_per_sample + 15) / 16;
   if (chunks > shortest) chunks = shortest;
-  if (chunks > cap) chunks = cap;
   return chunks < 1 ? 1 : static_cast<int>(chunks);
 }
 
@@ -1369,7 +1371,9 @@ int backward(const LinearShape& s, Operand grad, const void* preact, Operand (&x
     a.chunk_rows = (s.rows_per_sample + p.chunks - 1) / p.chunks;
     a.act = s.act;
     a.vec = s.n % 8 == 0 && aligned16(grad.ptr, grad.stride) && aligned16(a.preact, s.n) && aligned16(gate, gate_stride);
-    const dim3 grid((s.n + 255) / 256, s.samples * p.chunks);
+    const long long blocks = (s.n + 255LL) / 256 * s.samples * p.chunks;
+    if (blocks > 0x7fffffffLL) return kErrUnsupported;
+    const dim3 grid(static_cast<unsigned>(blocks));
     const int st = s.act == kActGeluTanh ? launch_act_backward<T, kActGeluTanh>(a, grid, stream)
                    : s.act == kActGelu   ? launch_act_backward<T, kActGelu>(a, grid, stream)
                    : s.act == kActSilu   ? launch_act_backward<T, kActSilu>(a, grid, stream)
@@ -1514,7 +1518,6 @@ extern "C" int peco_linear_backward(const void* grad, long long grad_stride, con
   if (dtype != 0 && dtype != 1) return kErrUnsupported;
   if (!s.valid()) return kErrInvalidValue;
   if (s.rows() == 0) return kErrInvalidValue;  // the sums over no rows are the caller's zeros
-  if (samples > 65535) return kErrUnsupported;
   if (!grad || grad_stride < n || gate_stride < 0) return kErrInvalidValue;
   if ((dx || dx2) && (!weight || w_stride < static_cast<long long>(k) + k2)) return kErrInvalidValue;
   if (dweight && (!x || x_stride < k || (k2 > 0 && (!x2 || x2_stride < k2)))) return kErrInvalidValue;

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from peco_b200 import _native
-from peco_b200.linear import linear_act
+from peco_b200.linear import linear_act, linear_act_backward
 
 pytestmark = pytest.mark.gpu
 
@@ -60,4 +60,24 @@ def test_sums_shared_out_over_ragged_rows(rows, k, n):
     _within(got, y, slack + 2.0 ** -23 * y.abs(), U[torch.bfloat16])
     for _ in range(10):
         assert torch.equal(linear_act(x, w, b), got)
+    assert _native.device_status(clear=True) == 0
+
+
+@pytest.mark.parametrize("samples,rows", [(65535, 1), (65536, 1), (70001, 2)])
+def test_gradient_of_many_samples(samples, rows):
+    # a gate row for every sample.  Sums of one or two rows (gate) and of all (bias): fp32 in runs, 2^-16 of their terms
+    normal = _normal(samples)
+    k, n = 16, 24
+    x, w, gate = normal(samples, rows, k), normal(n, k, std=0.25), normal(samples, n)
+    z, g = normal(samples, rows, n), normal(samples, rows, n)
+    got = linear_act_backward(g, x, w, preact=z, activation="silu", gate=gate, bias=True)
+    u = U[torch.bfloat16]
+    zd, gd = z.double(), g.double()
+    s = torch.sigmoid(zd)
+    dz, value = gd * gate.double()[:, None] * (s * (1 + zd * (1 - s))), gd * zd * s
+    _within(got.gate, value.sum(1), 2.0 ** -16 * value.abs().sum(1), u)
+    _within(got.bias, dz.sum((0, 1)), 2.0 ** -16 * dz.abs().sum((0, 1)), u)
+    _within(got.x, dz @ w.double(), (u + 2.0 ** -16) * (dz.abs() @ w.double().abs()), u)  # dz is rounded for the products
+    flat, rows_x = dz.flatten(0, 1), x.double().flatten(0, 1)
+    _within(got.weight, flat.t() @ rows_x, (u + (samples * rows) * 2.0 ** -24) * (flat.abs().t() @ rows_x.abs()), u)
     assert _native.device_status(clear=True) == 0
