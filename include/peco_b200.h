@@ -330,6 +330,14 @@ int peco_rotary(const void* q, void* q_out, int q_heads, const long long* q_stri
 
 /* ---- diagnostics --------------------------------------------------------- */
 
+/* How a product of the linear layer, [m, n] results over k_blocks blocks of 64
+ * summands, is cut (no device is touched).  product 0 the forward with its
+ * activation, 1 the gradient of the rows, 2 of the weight.  plan (host) gets
+ * CTAs per tile, columns per accumulator, accumulators per tile, groups that
+ * share a tile's sum, stages of the shared-memory ring, tile rows, tile
+ * columns and the tile rows walked together. */
+int peco_linear_tiles(int m, int n, int k_blocks, int product, int activation, int* plan);
+
 /* Copies the device status word of the current device to *out (synchronising
  * ``stream``) and clears it when ``clear`` != 0. */
 int peco_device_status(unsigned* out, int clear, void* stream);

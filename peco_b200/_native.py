@@ -47,6 +47,7 @@ _SIGNATURES = {
     "peco_linear_forward_workspace": [P, LL] * 3 + [I] * 5,
     "peco_linear_backward": [P, LL, P] + [P, LL] * 4 + [P] * 5 + [I] * 7 + [P, LL, P],
     "peco_linear_backward_workspace": [P, LL] * 4 + [I] * 7,
+    "peco_linear_tiles": [I] * 5 + [P],
     "peco_gated_norm": [P, LL, LL] * 2 + [P, LL] * 3 + [P] * 4 + [I] * 5 + [F] * 3 + [I, P],
     "peco_gated_norm_backward": [P, LL, LL] * 4 + [P, LL] * 2 + [P] * 7 + [I] + [P] * 2 + [I] * 5 + [F] * 3
     + [I, P, LL, P],

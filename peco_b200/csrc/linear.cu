@@ -1225,18 +1225,13 @@ int launch_tiles(const GemmArgs& g, int splits, cudaStream_t stream) {
   return launch_overlapped(kernel, dim3(grid), dim3(kGemmThreads), kGemmSmem, CG * splits, stream, g, splits);
 }
 
-template <typename T, bool AMN, bool BMN, bool EPI>
-int launch_gemm(GemmArgs& g, const Operand* a, const Operand* b, int segments, int dtype, cudaStream_t stream) {
-  int kblocks = 0;
-  for (int s = 0; s < segments; ++s) {
-    g.kblocks[s] = ((AMN ? a[s].rows : a[s].cols) + kTileK - 1) / kTileK;
-    kblocks += g.kblocks[s];
-  }
+// Everything of a product's cut that does not need its operands: g.m, g.n and g.act are set.
+template <bool AMN, bool BMN, bool EPI>
+TileChoice plan_tiles(GemmArgs& g, int kblocks) {
   const TileChoice c = choose_tiles(g.m, g.n, kblocks, AMN, !EPI ? 24.0 : g.act == kActNone ? 72.0 : 88.0);
   g.bn = c.bn;
   g.tiles_m = (g.m + c.cg * kTileM - 1) / (c.cg * kTileM);
   g.tiles_n = (g.n + c.bn * c.halves - 1) / (c.bn * c.halves);
-  if (static_cast<long long>(g.tiles_m) * g.tiles_n > 0x0fffffffLL) return kErrUnsupported;
   // The smaller operand stays in L2 while the larger passes once: A smaller, all
   // m tiles under every column of tiles; B smaller, two m tiles across all
   // columns.  The SMs are at their power limit in long products, so DRAM traffic
@@ -1258,6 +1253,19 @@ int launch_gemm(GemmArgs& g, const Operand* a, const Operand* b, int segments, i
   // a joined copy starts on a whole panel
   g.a_joined = AMN && g.m % 64 == 0;
   g.b_joined = BMN && g.n % 64 == 0 && b_rows % 64 == 0;
+  return c;
+}
+
+template <typename T, bool AMN, bool BMN, bool EPI>
+int launch_gemm(GemmArgs& g, const Operand* a, const Operand* b, int segments, int dtype, cudaStream_t stream) {
+  int kblocks = 0;
+  for (int s = 0; s < segments; ++s) {
+    g.kblocks[s] = ((AMN ? a[s].rows : a[s].cols) + kTileK - 1) / kTileK;
+    kblocks += g.kblocks[s];
+  }
+  const TileChoice c = plan_tiles<AMN, BMN, EPI>(g, kblocks);
+  if (static_cast<long long>(g.tiles_m) * g.tiles_n > 0x0fffffffLL) return kErrUnsupported;
+  const int a_rows = g.m < kTileM ? (g.m + 7) / 8 * 8 : kTileM, b_rows = c.bn / c.cg;
   for (int s = 0; s < segments; ++s)
     if (!operand_map(&g.a[s], a[s], AMN, a_rows, g.a_joined ? g.a_panels : 0, dtype) ||
         !operand_map(&g.b[s], b[s], BMN, b_rows, g.b_joined ? g.b_panels : 0, dtype))
@@ -1533,4 +1541,19 @@ extern "C" int peco_linear_backward(const void* grad, long long grad_stride, con
   Carver ws{static_cast<unsigned char*>(workspace), 0};
   return dtype == 1 ? backward<__nv_bfloat16>(s, g, preact, a, b, gate, gate_stride, dxs, dweight, dbias, dgate, ws, stream)
                     : backward<__half>(s, g, preact, a, b, gate, gate_stride, dxs, dweight, dbias, dgate, ws, stream);
+}
+
+extern "C" int peco_linear_tiles(int m, int n, int k_blocks, int product, int activation, int* plan) {
+  if (m < 1 || n < 1 || k_blocks < 1 || product < 0 || product > 2 || activation < kActNone || activation > kActSilu || !plan)
+    return kErrInvalidValue;
+  GemmArgs g{};
+  g.m = m;
+  g.n = n;
+  g.act = activation;
+  const TileChoice c = product == 0   ? plan_tiles<false, false, true>(g, k_blocks)
+                       : product == 1 ? plan_tiles<false, true, false>(g, k_blocks)
+                                      : plan_tiles<true, true, false>(g, k_blocks);
+  const int values[8] = {c.cg, c.bn, c.halves, c.splits, g.stages, g.tiles_m, g.tiles_n, g.band};
+  for (int i = 0; i < 8; ++i) plan[i] = values[i];
+  return kOk;
 }
