@@ -267,7 +267,8 @@ long long peco_linear_forward_workspace(const void* x, long long x_stride, const
  * activation is not 0 or dgate is asked for.  dx [rows, k], dx2 [rows, k2],
  * dweight [n, k + k2], dbias [n], dgate [samples, n], contiguous; null: not
  * computed.  grad * gate * act' is rounded to the operands' type for the two
- * products; the sums for dbias and dgate are of the unrounded values and do
+ * products (fp16: to its range too, infinite past 65504, zero below 6e-8); the
+ * sums for dbias and dgate are of the unrounded values and do
  * not depend on the launch order.  Needs at least one row. */
 int peco_linear_backward(const void* grad, long long grad_stride, const void* preact, const void* x,
                          long long x_stride, const void* x2, long long x2_stride, const void* weight,

@@ -24,10 +24,11 @@
 // registers of the threads that share it, and every statistic is taken from
 // there in fp32, squares around the mean.  The backward kernel recomputes r
 // from x and the branch, so nothing has to be saved.  Measured at 3072 bf16
-// columns: forward with branch, gate and modulation 34680 rows 133 us (6.4
-// TB/s), backward 7006 rows 57 us (4.5 TB/s, of it 6 us for the second kernel),
-// 34680 rows 238 us (5.4 TB/s); the backward is bound by the latency of a row's
-// reduction at the 12 warps per SM that its registers allow.
+// columns with branch, gate and modulation: forward 34680 rows 133 us (6.4 TB/s;
+// 138 us over two sets of inputs back to back), backward 7006 rows 57 us (4.5
+// TB/s, of it 6 us for the second kernel), 34680 rows 235 us (5.4 TB/s); the
+// backward is bound by the latency of a row's reduction at the 12 warps per SM
+// that its registers allow.
 #include "common.cuh"
 #include "../../include/peco_b200.h"
 #include "internal.h"
@@ -831,7 +832,7 @@ int launch_forward_mode(NormArgs a, cudaStream_t stream) {
     a.stage_bytes = a.width * 2 * (a.branch.p ? 2 : 1);
     while (blocks > 1 && ring_bytes_of(blocks) < 2 * a.stage_bytes) --blocks;
     // three stages: deeper rings read further ahead of the writes and measured
-    // slower (gated rows of 3072: 145 us with three, 161 with four and more)
+    // slower (34680 gated rows of 3072: 138 us with three, 156 with four)
     a.stages = ring_stages(a.stage_bytes, blocks) < 3 ? 2 : 3;
     smem = a.stages * a.stage_bytes;
     static std::atomic<unsigned long long> opened;
@@ -855,12 +856,19 @@ int launch_forward(const NormArgs& a, cudaStream_t stream) {
 }
 
 // Threads per row.  Few warps keep a row's reduction cheap, few columns per
-// thread its registers; measured at 3072 columns (34680 rows): backward 238 us
-// with 6 warps x 2 chunks, 412 with 12 x 1, 234 with 4 x 3 (equal at 7006 rows);
-// forward 145 us with 4 x 3, 161 with 12 x 1, 179 with 8 x 2.  Unaligned rows
-// hold a register per element ahead and take fewer of them: 14769 x 2241 backward
-// 168 us with 12 x 1 (348 with 6 x 2, two elements to a register), forward 68 us
-// with 4 x 3, 90 with 8 x 2; 8000 x 6001 forward 104 us with 16 x 2, 151 with 8 x 3.
+// thread its registers; measured at 34680 x 3072 with branch, gate and modulation:
+// backward 235 us with 6 warps x 2 chunks, 318 with 12 x 1, 407 with 4 x 3 (three
+// blocks of it per SM spill); forward 138 us with 4 x 3, 140 with 12 x 1, 174 with
+// 8 x 2.  Unaligned rows hold a register per element ahead and take fewer of them
+// (fp16 with branch, gate and weight): 14769 x 2241 backward 168 us with 12 x 1
+// (348 with 6 x 2, two elements to a register), forward 68 us with 4 x 3, 90 with
+// 8 x 2; 8000 x 6001 forward 104 us with 16 x 2, 151 with 8 x 3.
+// The widest forms do not fit their registers: the forward above 8192 columns and
+// the gradient above 6144 (unaligned 4096), and of 257 to 512, spill; with a post
+// norm the gradient's other forms do too, by 0.1 to 0.2 KB a thread.  bf16 with
+// branch, gate and modulation, floors in brackets: 8192 x 12288 forward 274 us
+// (125), gradient 990 (188); 8192 x 8192 gradient 256 us (125); 8192 x 16383
+// forward 1314 us (167).
 template <typename T, bool POST>
 int launch_norm(const NormArgs& a, bool backward, cudaStream_t stream) {
   const int w = a.width;
@@ -897,8 +905,10 @@ int launch_any(const NormArgs& a, int dtype, bool backward, cudaStream_t stream)
   return dtype == 1 ? launch_norm<__nv_bfloat16, false>(a, backward, stream) : launch_norm<__half, false>(a, backward, stream);
 }
 
-// Row chunks per sample of the backward kernel, one block each: the resident
-// blocks of launch_backward, but no more than there are rows.
+// Row chunks per sample of the backward kernel, one block each, but no more than
+// there are rows: the resident blocks of launch_norm's aligned forms.  The
+// unaligned forms of 1025 to 3072 columns hold fewer (two blocks per SM to 2048,
+// one to 3072), so that theirs run in more than one round.
 int norm_chunks(int samples, int rows, int width) {
   if (samples < 1) return 1;
   const long long per_sm = width <= 512 ? 12 : width <= 1024 ? 4 : width <= 2048 ? 3 : width <= 3072 ? 2 : 1;

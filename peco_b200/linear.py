@@ -6,7 +6,9 @@ activation, a product with the adaLN gate and a residual sum.  The products run
 on the tcgen05 tensor cores with fp32 sums and each output element is rounded
 once; float16 and bfloat16.  Differentiable: under autograd the pre-activation
 is saved (rounded to the operands' type) when a gradient needs it, and
-``linear_act_backward`` computes the gradients with the same product kernel.
+``linear_act_backward`` computes the gradients with the same product kernel: for
+its products grad * gate * act' is rounded to the operands' type, in float16 to
+that type's range too (as unfused float16 layers do; scale the loss for it).
 
 CUDA tensors only; work is enqueued on the current stream.
 """
