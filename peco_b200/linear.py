@@ -242,6 +242,7 @@ def linear_act_backward(grad, x, weight, *, preact=None, activation=None, gate=N
     if needs is None:
         want_x, want_x2, want_w, want_b, want_g = True, x2 is not None, True, bool(bias), gate is not None
     else:
+        needs = tuple(needs)  # looked through more than once
         want_x, want_x2, want_w, want_b, want_g = (name in needs for name in LinearGrads._fields)
         if len(set(needs) - set(LinearGrads._fields)) or want_x2 and x2 is None or want_b and not bias or \
                 want_g and gate is None:

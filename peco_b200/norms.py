@@ -225,6 +225,7 @@ def modulated_norm_backward(grad_normed, grad_residual, x, branch=None, *, gate=
     if needs is None:
         grads = [None if t is None else x.new_empty(t.shape) for t in inputs]
     else:
+        needs = tuple(needs)  # looked through more than once
         if any(n not in NormGrads._fields or inputs[NormGrads._fields.index(n)] is None for n in needs):
             raise ValueError("needs names a gradient whose input is absent")
         grads = [x.new_empty(t.shape) if n in needs else None for n, t in zip(NormGrads._fields, inputs)]

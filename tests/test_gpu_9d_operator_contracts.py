@@ -3,7 +3,8 @@
 import pytest
 import torch
 
-from peco_b200.linear import linear_act
+from peco_b200.linear import linear_act, linear_act_backward
+from peco_b200.norms import modulated_norm_backward
 from peco_b200.rotary import rotate
 
 pytestmark = pytest.mark.gpu
@@ -99,3 +100,15 @@ def test_inplace_queries_and_keys_share_no_memory():
     q, k = rotate(heads[:, :6], heads[:, 6:8], **opts, inplace=True)
     assert torch.equal(q, want_q) and torch.equal(k, want_k)
     assert torch.equal(qkv[:, :, 8:], keep[:, :, 8:])
+
+
+def test_needs_may_be_any_iterable():
+    x, w, g = (torch.randn(16, 16, device=DEV).bfloat16() for _ in range(3))
+    got = linear_act_backward(g, x, w, bias=True, needs=iter(["weight", "x"]))
+    assert got.x is not None and got.weight is not None and got.bias is None
+    with pytest.raises(ValueError):
+        linear_act_backward(g, x, w, needs=iter(["x", "gain"]))
+    got = modulated_norm_backward(g, None, x, scale=x[0], shift=w[0], needs=iter(["shift", "x"]))
+    assert got.x is not None and got.shift is not None and got.scale is None
+    with pytest.raises(ValueError):
+        modulated_norm_backward(g, None, x, needs=iter(["x", "scale"]))
