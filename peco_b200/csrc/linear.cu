@@ -95,43 +95,41 @@ __device__ __forceinline__ float2 normal_integral_pair(float2 z, float2& bell) {
   return make_float2(z.x > 0.0f ? 1.0f - tail.x : tail.x, z.y > 0.0f ? 1.0f - tail.y : tail.y);
 }
 
-// (act(z), act'(z)) of the forms that take no pairs
-template <int ACT>
-__device__ __forceinline__ float2 activate_slope(float z) {
-  if constexpr (ACT == kActSilu) {
-    const float s = recip_approx(1.0f + exp2_approx(-kLog2e * z));
-    return make_float2(z * s, s * fmaf(z, 1.0f - s, 1.0f));
-  } else {
-    return make_float2(z, 1.0f);
-  }
-}
-
-// (act(z), act'(z)) of a pair; the value only where ``value`` is set
+// (act(z), act'(z)) of a pair; the value only where ``value`` is set.  A saved
+// pre-activation may be infinite where its 16-bit type ended (fp16: past 65504):
+// in products, where a factor vanishes or meets a zero gradient, it is held
+// finite (a NaN comes back through the other factor).
 template <int ACT, bool VALUE>
 __device__ __forceinline__ void activate_slope2(float2 z, float2& value, float2& slope) {
   auto both = [](float x) { return make_float2(x, x); };
+  auto held = [](float x) { return fminf(fmaxf(x, -1e30f), 1e30f); };
+  const float2 f = make_float2(held(z.x), held(z.y));
   if constexpr (ACT == kActGeluTanh) {
     const float2 z2 = fmul2(z, z);
     const float2 w = fmul2(z, ffma2(z2, both(-kLog2e * kGelu3), both(-kLog2e * kGelu1)));
     const float2 e = fadd2(make_float2(exp2_approx(w.x), exp2_approx(w.y)), both(1.0f));
     const float2 s = make_float2(recip_approx(e.x), recip_approx(e.y));
-    // s + z s (1 - s) d(2u)/dz; far out a vanishing factor meets one that
-    // overflows, which is held finite (a NaN comes back through s)
+    // s + z s (1 - s) d(2u)/dz
     float2 d = fmul2(z, ffma2(z2, both(3.0f * kGelu3), both(kGelu1)));
-    d.x = fminf(fmaxf(d.x, -1e30f), 1e30f);
-    d.y = fminf(fmaxf(d.y, -1e30f), 1e30f);
+    d = make_float2(held(d.x), held(d.y));
     const float2 rest = ffma2(make_float2(-s.x, -s.y), d, d);
     slope = ffma2(s, rest, s);
-    if (VALUE) value = fmul2(z, s);
+    if (VALUE) value = fmul2(f, s);
   } else if constexpr (ACT == kActGelu) {
     float2 bell;
     const float2 p = normal_integral_pair(z, bell);
-    slope = ffma2(fmul2(z, both(0.3989422804014327f)), bell, p);
-    if (VALUE) value = fmul2(z, p);
+    slope = ffma2(fmul2(f, both(0.3989422804014327f)), bell, p);
+    if (VALUE) value = fmul2(f, p);
+  } else if constexpr (ACT == kActSilu) {
+    const float2 w = fmul2(z, both(-kLog2e));
+    const float2 e = fadd2(make_float2(exp2_approx(w.x), exp2_approx(w.y)), both(1.0f));
+    const float2 s = make_float2(recip_approx(e.x), recip_approx(e.y));
+    const float2 rest = ffma2(make_float2(-s.x, -s.y), f, f);  // z (1 - s)
+    slope = ffma2(s, rest, s);
+    if (VALUE) value = fmul2(f, s);
   } else {
-    const float2 a = activate_slope<ACT>(z.x), b = activate_slope<ACT>(z.y);
-    value = make_float2(a.x, b.x);
-    slope = make_float2(a.y, b.y);
+    value = z;
+    slope = both(1.0f);
   }
 }
 
@@ -917,7 +915,7 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const __grid_constant__ 
 // ---- gradient of the epilogue --------------------------------------------------------
 // Bound by HBM with the arithmetic close behind: 6750 x 12288 with gelu (tanh form)
 // reads g and z, writes dz: 498 MB in 93 us (5.4 TB/s); for the bias gradient
-// alone 68 us, 77 us in the erf form.
+// alone 68 us, 80 us in the erf form.
 // One block per (256 columns, chunk of one sample's rows): lane l of every
 // warp owns 8 columns, the 8 warps take every eighth row.  Writes dz and the
 // chunk's column sums of dz and of g * act(z); a second kernel adds the

@@ -61,3 +61,27 @@ def test_gelu_gradient_tail(dtype):
         _near(g.weight[:, 0], slope, size, dtype)  # dz, rounded for the product with x = 1
         if gate is not None:
             _near(g.gate, z.double() * cdf, (z.double() * cdf).abs(), dtype)
+
+
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("gated", [False, True])
+def test_gradient_past_the_range_of_the_saved_preactivation(act, gated):
+    # float16 saves a pre-activation of -90000 as -infinity: the slope there is 0 and the value 0, far above it is 1
+    x = torch.tensor([[-300.0], [300.0], [-1.0]], device=DEV, dtype=torch.float16, requires_grad=True)
+    w = torch.tensor([[300.0], [-300.0]], device=DEV, dtype=torch.float16)
+    gate = torch.tensor([0.5, 0.5], device=DEV, dtype=torch.float16, requires_grad=True) if gated else None
+    out = linear_act(x, w, activation=act, gate=gate)
+    down, up = (out[0, 0], out[1, 1]), (out[1, 0], out[0, 1])  # at -90000 and at 90000
+    assert all(v == 0 for v in down) and all(v.isinf() if not gated else v > 44000 for v in up)
+    pick = torch.zeros_like(out)
+    pick[0, 0] = pick[1, 1] = 1.0
+    grads = torch.autograd.grad(out, (x, gate) if gated else (x,), pick, retain_graph=True)
+    assert all((g == 0).all() for g in grads)
+    pick = torch.zeros_like(out)
+    pick[1, 0] = 1.0
+    (gx,) = torch.autograd.grad(out, x, pick)
+    assert torch.equal(gx[:, 0], torch.tensor([0.0, 150.0 if gated else 300.0, 0.0], device=DEV, dtype=torch.float16))
+    # a pre-activation that is no number stays none
+    one = torch.ones(1, 1, device=DEV, dtype=torch.float16)
+    g = linear_act_backward(one, one, one, preact=one * float("nan"), activation=act, gate=one[0], bias=True)
+    assert g.bias.isnan().all() and g.gate.isnan().all() and g.x.isnan().all()
