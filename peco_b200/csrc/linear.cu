@@ -1156,18 +1156,6 @@ bool operand_map(CUtensorMap* map, const Operand& o, bool mn, int tile_rows, int
   return encode_tensor_map(map, type, 2, o.ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// Dynamic shared memory of a kernel, granted once per device.
-cudaError_t grant_smem(const void* kernel, int bytes, std::atomic<unsigned long long>& done) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  const unsigned long long bit = 1ull << (dev & 63);
-  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
-  return e;
-}
-
 // How a product is cut: CTAs per group, columns per accumulator, accumulators
 // per tile, K splits.
 struct TileChoice {

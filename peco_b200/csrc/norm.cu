@@ -773,18 +773,6 @@ int blocks_per_sm(const void* kernel, int threads, std::atomic<int>& known) {
   return n;
 }
 
-// Lets a kernel take ``bytes`` of dynamic shared memory, once per device.
-cudaError_t grant_smem(const void* kernel, int bytes, std::atomic<unsigned long long>& done) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  const unsigned long long bit = 1ull << (dev & 63);
-  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
-  return e;
-}
-
 // Stages of a ring with ``blocks`` blocks per SM: as many as fit beside each
 // block's static arrays and the system's part, two at least.
 constexpr int kRingBudget = 220 * 1024;  // of one block alone

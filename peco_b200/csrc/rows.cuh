@@ -3,6 +3,8 @@
 
 #include "common.cuh"
 
+#include <atomic>
+
 namespace peco {
 
 template <typename T>
@@ -50,6 +52,18 @@ __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.
 // A caller's workspace: large enough, and on the 16 bytes that vector stores and TMA start on.
 inline bool usable_workspace(const void* workspace, long long bytes, long long need) {
   return workspace && bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0;
+}
+
+// Dynamic shared memory of a kernel, granted once per device.
+inline cudaError_t grant_smem(const void* kernel, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 // Launch of a kernel that begins with wait_for_prior().
