@@ -280,6 +280,32 @@ long long peco_linear_backward_workspace(const void* grad, long long grad_stride
                                          int samples, int rows_per_sample, int k, int k2, int n, int activation,
                                          int has_gate);
 
+/* Rows of 16-bit elements in 8-bit integers, one scale a row: scales[m] = max / 127
+ * with max the largest magnitude in [x | x2] of row m, values[m, k] = 127 x[m, k]
+ * / max rounded to the nearest integer (ties to even, as of the exact quotient).
+ * A row of zeros has scale 0, one with an infinity or NaN scale NaN and values 0.
+ * x [rows, k], x2 [rows, k2] (k2 = 0: absent), values [rows, k + k2]: rows
+ * ``*_stride`` elements apart; dtype 0 fp16, 1 bf16. */
+int peco_quantize_rows(const void* x, long long x_stride, const void* x2, long long x2_stride, void* values,
+                       long long v_stride, float* scales, long long rows, int k, int k2, int dtype, void* stream);
+
+/* out = residual + gate * act(row_scales[m] col_scales[n] (X W^T)[m, n] + bias)
+ * with 8-bit signed X and W [n, k + k2] and exact integer sums (k + k2 <=
+ * 131071).  X is ``values`` [rows, k] with row_scales [rows] (k2 = 0), or, with
+ * values null, [x | x2] quantised as by peco_quantize_rows into the workspace.
+ * bias, gate, residual, out, activation and dtype as in peco_linear_forward; out
+ * shares no memory with the operands.  8-bit rows whose base or stride is not
+ * a multiple of 16 bytes are copied into the workspace first;
+ * peco_linear_int8_workspace says how many bytes it needs (-1: sizes out of range). */
+int peco_linear_int8(const void* x, long long x_stride, const void* x2, long long x2_stride, const void* values,
+                     long long v_stride, const float* row_scales, const void* weight, long long w_stride,
+                     const float* col_scales, const void* bias, const void* gate, long long gate_stride,
+                     const void* residual, long long res_stride, void* out, long long out_stride, int samples,
+                     int rows_per_sample, int k, int k2, int n, int activation, int dtype, void* workspace,
+                     long long workspace_bytes, void* stream);
+long long peco_linear_int8_workspace(int from_16_bits, const void* values, long long v_stride, const void* weight,
+                                     long long w_stride, int samples, int rows_per_sample, int k, int k2, int n);
+
 /* Gated residual and norm: with b = post_norm(branch) * post_weight,
  *   residual = residual_scale * x + gate * b
  *   normed = norm(residual) * weight * (1 + scale) + shift

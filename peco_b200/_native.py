@@ -48,6 +48,9 @@ _SIGNATURES = {
     "peco_linear_backward": [P, LL, P] + [P, LL] * 4 + [P] * 5 + [I] * 7 + [P, LL, P],
     "peco_linear_backward_workspace": [P, LL] * 4 + [I] * 7,
     "peco_linear_tiles": [I] * 5 + [P],
+    "peco_quantize_rows": [P, LL] * 3 + [P, LL, I, I, I, P],
+    "peco_linear_int8": [P, LL] * 3 + [P] + [P, LL] + [P, P, P, LL, P, LL, P, LL] + [I] * 7 + [P, LL, P],
+    "peco_linear_int8_workspace": [I] + [P, LL] * 2 + [I] * 5,
     "peco_gated_norm": [P, LL, LL] * 2 + [P, LL] * 3 + [P] * 4 + [I] * 5 + [F] * 3 + [I, P],
     "peco_gated_norm_backward": [P, LL, LL] * 4 + [P, LL] * 2 + [P] * 7 + [I] + [P] * 2 + [I] * 5 + [F] * 3
     + [I, P, LL, P],
@@ -67,6 +70,7 @@ _RESTYPES = {
     "peco_launch_count": ctypes.c_ulonglong,
     "peco_linear_forward_workspace": LL,
     "peco_linear_backward_workspace": LL,
+    "peco_linear_int8_workspace": LL,
     "peco_gated_norm_backward_workspace": LL,
     "peco_attention_workspace_stride": LL,
     "peco_key_block_rows": LL,
