@@ -306,6 +306,35 @@ int peco_linear_int8(const void* x, long long x_stride, const void* x2, long lon
 long long peco_linear_int8_workspace(int from_16_bits, const void* values, long long v_stride, const void* weight,
                                      long long w_stride, int samples, int rows_per_sample, int k, int k2, int n);
 
+/* Spans of keys for attention: rows [batch, queries, 4] gets (first key, key
+ * behind the last, position among the keys, 0) of every query row, tiles [batch,
+ * ceil(queries / 128), 4] bounds over 128 rows; both start on 16 bytes.
+ * Documents (documents > 0): document i of sample b holds rows [q_ends[b *
+ * q_stride + i], q_ends[... + i + 1]) and keys likewise by k_ends; rows outside
+ * see nothing.  Otherwise lengths [batch] (null: all keys).  A document's last
+ * row stands at its last key.  causal: a row sees the keys up to its position and
+ * its document's first prefix[b * prefix_batch + i * prefix_document] keys
+ * (prefix null: prefix_all).  window > 0: keys less than ``window`` away.
+ * Offsets are device memory and are held to the sequence. */
+int peco_key_spans(const int* q_ends, long long q_stride, const int* k_ends, long long k_stride, int documents,
+                   const int* lengths, const int* prefix, long long prefix_batch, int prefix_document, int prefix_all,
+                   int causal, int window, int batch, int queries, int keys, int* rows, int* tiles, void* stream);
+
+/* Attention of q [batch, heads, sq, d] over k, v [batch, kv_heads, sk, d]:
+ * z_ij = cap tanh(scale q_i.k_j / cap) - slopes[h] |pos_i - j| (cap 0 and slopes
+ * null: without), out_i = sum_j softmax(z)_ij v_j over the row's span, lse [batch,
+ * heads, sq] its logarithmic sum (a row without keys: 0 and -inf).  strides (host
+ * memory): batch, head and row strides of q, k, v and out in elements; d is
+ * adjacent, rows, heads and samples start on 16 bytes.  span_rows and span_tiles
+ * from peco_key_spans (null: every key, pos = i + sk - sq), of one sample for
+ * all or, with spans_batched, of each.  heads is a multiple of kv_heads, d of 8 up
+ * to 128; dtype 0 fp16, 1 bf16.  Calls of few rows keep parts in the workspace. */
+int peco_span_attention(const void* q, const void* k, const void* v, const long long* strides, const int* span_rows,
+                        const int* span_tiles, int spans_batched, const float* slopes, float scale, float cap, void* out,
+                        float* lse, int batch, int heads, int kv_heads, int sq, int sk, int d, int dtype, void* workspace,
+                        long long workspace_bytes, void* stream);
+long long peco_span_attention_workspace(int batch, int heads, int kv_heads, int sq, int sk, int d);
+
 /* Gated residual and norm: with b = post_norm(branch) * post_weight,
  *   residual = residual_scale * x + gate * b
  *   normed = norm(residual) * weight * (1 + scale) + shift

@@ -1,0 +1,233 @@
+"""Exact attention under masks of key spans, over libpeco_b200.so.
+
+Each query row sees one interval of keys, which covers the documents of a packed
+sequence, a causal order with a prefix that every row sees, windows, and
+samples of unequal lengths (``key_spans``).  Scores can be capped by a tanh and
+get a bias that depends on the distance:
+
+    z_ij = cap tanh(scale q_i.k_j / cap) - slope_h |pos_i - j|
+    out_i = sum_j softmax_j(z_ij) v_j      over the keys that row i sees
+
+Products run on the tcgen05 tensor cores with fp32 sums, softmax statistics in
+fp32; float16 and bfloat16; keys may be shared by groups of query heads.  A row
+that sees no key is 0.  CUDA tensors only; work is enqueued on
+the current stream.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from dataclasses import dataclass
+from typing import NamedTuple, Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native
+
+_Strides = ctypes.c_longlong * 12
+_GradStrides = ctypes.c_longlong * 24
+_SIXTEEN_BITS = (torch.float16, torch.bfloat16)
+
+
+class AttentionGrads(NamedTuple):
+    """Gradients of ``attention``; None where not asked for."""
+
+    q: Optional[torch.Tensor]
+    k: Optional[torch.Tensor]
+    v: Optional[torch.Tensor]
+
+
+@dataclass(frozen=True)
+class KeySpans:
+    """The keys that each query row sees, as ``key_spans`` lays them out."""
+
+    rows: torch.Tensor   # int32 [B or 1, queries, 4]: first key, key behind the last, the row's position among the keys
+    tiles: torch.Tensor  # int32 [B or 1, tiles of 128 rows, 4]
+    queries: int
+    keys: int
+
+
+def _ends(ends, batch, what):
+    """Document ends as int32 [1 or batch, n + 1] rows."""
+    if not isinstance(ends, torch.Tensor) or ends.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{what} must be an int32 or int64 tensor")
+    if ends.dim() not in (1, 2) or ends.shape[-1] < 2 or ends.dim() == 2 and ends.shape[0] not in (1, batch):
+        raise ValueError(f"{what} must be [n + 1] or one such row for each of the {batch} samples")
+    ends = ends.to(torch.int32).contiguous()
+    return ends, ends.shape[1] if ends.dim() == 2 and ends.shape[0] > 1 else 0
+
+
+def key_spans(batch, queries, keys, *, documents=None, key_documents=None, lengths=None, causal=False, prefix=None,
+              window=None, device=None) -> KeySpans:
+    """Spans of keys for ``queries`` rows and ``keys`` keys of ``batch`` samples (1: the same for all samples of a call).
+
+    ``documents``: ends of a packed sequence's documents, int [n + 1] or
+    [batch, n + 1], ascending from the first row: document i holds rows
+    [documents[i], documents[i + 1]) and, with ``key_documents`` (default: the
+    same), those keys; its rows see its keys only.  Rows outside all documents
+    see nothing.  ``lengths``: int [batch], each sample's number of keys, instead
+    of documents.  The last row of a document (or sample) stands at its last key.
+    ``causal``: a row sees the keys up to its own position, and the first
+    ``prefix`` keys of its document wherever it stands (an int, or an int tensor
+    [n], [batch, 1] or [batch, n]).  ``window``: a row sees the keys less
+    than ``window`` away from its position (not with a prefix).
+
+    Offsets are read on the device and held to the sequence there; nothing is
+    synchronised.  A plan serves every layer that has the same mask.
+    """
+    batch, queries, keys = int(batch), int(queries), int(keys)
+    if batch < 1 or batch > 65535 or queries < 0 or keys < 0:
+        raise ValueError("Expected a batch of 1 to 65535 and nonnegative lengths")
+    if lengths is not None and documents is not None:
+        raise ValueError("lengths and documents exclude each other")
+    if key_documents is not None and documents is None:
+        raise ValueError("key_documents goes with documents")
+    if prefix is not None and not causal:
+        raise ValueError("a prefix goes with a causal order")
+    if window is not None and (int(window) < 1 or prefix is not None):
+        raise ValueError("window must be positive and has no prefix")
+    tensors, n = [], 0
+    q_ends = k_ends = None
+    q_stride = k_stride = 0
+    if documents is not None:
+        q_ends, q_stride = _ends(documents, batch, "documents")
+        k_ends, k_stride = (q_ends, q_stride) if key_documents is None else _ends(key_documents, batch, "key_documents")
+        n = q_ends.shape[-1] - 1
+        if k_ends.shape[-1] != n + 1:
+            raise ValueError("documents and key_documents must have as many documents")
+        tensors += [q_ends, k_ends]
+    elif lengths is not None:
+        if not isinstance(lengths, torch.Tensor) or lengths.dtype not in (torch.int32, torch.int64):
+            raise TypeError("lengths must be an int32 or int64 tensor")
+        if lengths.shape != (batch,):
+            raise ValueError(f"lengths must be [{batch}]")
+        lengths = lengths.to(torch.int32).contiguous()
+        tensors.append(lengths)
+    prefix_rows, prefix_all, prefix_batch, prefix_doc = None, 0, 0, 0
+    if isinstance(prefix, torch.Tensor):
+        if prefix.dtype not in (torch.int32, torch.int64):
+            raise TypeError("prefix must be an int or an int32 or int64 tensor")
+        shape = tuple(prefix.shape)
+        if shape not in ((max(n, 1),), (batch, 1), (batch, max(n, 1))):
+            raise ValueError(f"prefix must be one number, [{max(n, 1)}], [{batch}, 1] or [{batch}, {max(n, 1)}]")
+        prefix_rows = prefix.to(torch.int32).contiguous()
+        prefix_batch, prefix_doc = (shape[1] if len(shape) == 2 else 0), 1 if shape[-1] > 1 else 0
+        tensors.append(prefix_rows)
+    elif prefix is not None:
+        prefix_all = min(max(int(prefix), 0), 2 ** 31 - 1)
+    device = tensors[0].device if device is None and tensors else torch.device("cuda" if device is None else device)
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    if device.type != "cuda" or any(t.device != device for t in tensors):
+        _native.require_cuda(torch.empty(0, device=device), *tensors)
+    rows = torch.empty((batch, queries, 4), dtype=torch.int32, device=device)
+    tiles = torch.empty((batch, -(-queries // 128), 4), dtype=torch.int32, device=device)
+    address = _native.address
+    _native.enqueue(device, "peco_key_spans", _native.load().peco_key_spans,
+                    (address(q_ends), q_stride, address(k_ends), k_stride, n, address(lengths), address(prefix_rows),
+                     prefix_batch, prefix_doc, prefix_all, 1 if causal else 0,
+                     min(int(window), 2 ** 31 - 1) if window is not None else 0, batch, queries, keys, rows.data_ptr(),
+                     tiles.data_ptr()), tensors)
+    return KeySpans(rows, tiles, queries, keys)
+
+
+def _check(q, k, v, spans, scale, softcap, slopes):
+    """Checked (batch, heads, key heads, queries, keys, dims), scale and cap."""
+    if not all(isinstance(t, torch.Tensor) and t.dim() == 4 for t in (q, k, v)):
+        raise ValueError("Expected q [B, H, N, D] and k, v [B, KV, M, D]")
+    if q.dtype not in _SIXTEEN_BITS or k.dtype is not q.dtype or v.dtype is not q.dtype:
+        raise TypeError("attention takes float16 or bfloat16 tensors of one dtype")
+    b, h, n, d = q.shape
+    kv, m = k.shape[1:3]
+    if k.shape != (b, kv, m, d) or v.shape != k.shape:
+        raise ValueError("k and v must be [B, KV, M, D] with the batch and head dimension of q")
+    if kv < 1 or h < 1 or h % kv:
+        raise ValueError("the query heads must be a multiple of the key heads")
+    if d < 8 or d > 128 or d % 8:
+        raise ValueError("the head dimension must be a multiple of 8 up to 128")
+    if max(n, m) > 0x7ffffe00:
+        raise ValueError("too many rows")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError("scale must be positive")
+    cap = 0.0 if softcap is None else float(softcap)
+    if softcap is not None and not (cap > 0 and math.isfinite(cap)):
+        raise ValueError("softcap must be positive")
+    others = [k, v]
+    if slopes is not None:
+        if not isinstance(slopes, torch.Tensor) or slopes.dtype is not torch.float32 or slopes.shape != (h,):
+            raise ValueError(f"slopes must be a float32 tensor [{h}]")
+        if torch.is_grad_enabled() and slopes.requires_grad:
+            raise RuntimeError("attention has no gradient of slopes")
+        others.append(slopes)
+    if spans is not None:
+        if not isinstance(spans, KeySpans):
+            raise TypeError("spans must come from key_spans")
+        if (spans.queries, spans.keys) != (n, m) or spans.rows.shape[0] not in (1, b):
+            raise ValueError(f"spans are for {spans.rows.shape[0]} samples of {spans.queries} rows and {spans.keys} keys, "
+                             f"the call has {b} of {n} and {m}")
+        others += [spans.rows, spans.tiles]
+    _native.require_cuda(q, *others)
+    return (b, h, kv, n, m, d), scale, cap
+
+
+def _readable(t):
+    """``t`` with adjacent dims and every row on 16 bytes: itself, or a copy."""
+    sizes, steps = t.shape, t.stride()
+    if steps[3] == 1 and t.data_ptr() % 16 == 0 and all(
+            n <= 1 or 0 < s < 1 << 38 and s % 8 == 0 for n, s in zip(sizes[:3], steps[:3])):
+        return t
+    return t.contiguous() if not t.is_contiguous() else t.clone()
+
+
+def _mask_args(spans, b):
+    if spans is None:
+        return 0, 0, 0
+    return spans.rows.data_ptr(), spans.tiles.data_ptr(), 1 if spans.rows.shape[0] == b and b > 1 else 0
+
+
+def _forward(q, k, v, spans, scale, softcap, slopes):
+    sizes, scale, cap = _check(q, k, v, spans, scale, softcap, slopes)
+    b, h, kv, n, m, d = sizes
+    out = torch.empty_like(q)
+    lse = torch.empty((b, h, n), dtype=torch.float32, device=q.device)
+    if out.numel() == 0:
+        return out, lse
+    q, k, v = _readable(q), _readable(k), _readable(v)
+    whole = out if _readable(out) is out else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if slopes is not None:
+        slopes = slopes.contiguous()
+    lib = _native.load()
+    need = int(lib.peco_span_attention_workspace(b, h, kv, n, m, d))
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+    strides = _Strides(*(s for t in (q, k, v, whole) for s in t.stride()[:3]))
+    rows, tiles, batched = _mask_args(spans, b)
+    _native.enqueue(q.device, "peco_span_attention", lib.peco_span_attention,
+                    (q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, rows, tiles, batched, _native.address(slopes), scale,
+                     cap, whole.data_ptr(), lse.data_ptr(), b, h, kv, n, m, d, _native.DTYPE_CODE[q.dtype],
+                     _native.address(ws), max(need, 0)),
+                    (q, k, v, slopes, *((spans.rows, spans.tiles) if spans is not None else ())))
+    return out.copy_(whole) if whole is not out else out, lse
+
+
+def attention(q, k, v, *, spans=None, scale=None, softcap=None, slopes=None, return_lse=False):
+    """Attention of q [B, H, N, D] over k, v [B, KV, M, D] (H a multiple of KV: each key head serves H / KV query heads).
+
+    ``spans``: what ``key_spans(B or 1, N, M, ...)`` gives; None: every row sees
+    every key, and the last row stands at the last key.  ``scale`` defaults to
+    D^-0.5.  ``softcap``: scores are softcap * tanh(score / softcap).  ``slopes``
+    float32 [H]: slope * |position - j| is taken from the score of key j.
+    ``return_lse``: also the logarithm of each row's sum of exponentials, float32
+    [B, H, N] (no gradient flows through it), -inf where a row sees nothing.
+
+    D is a multiple of 8 up to 128.  Strides are free where D is adjacent and
+    rows, heads and samples start on 16 bytes; other layouts are copied first.
+    The result has the layout of q.
+    """
+    _native.refuse_tangents("attention", q, k, v, slopes)
+    if torch.is_grad_enabled() and _native.wants_grad(q, k, v):
+        raise RuntimeError("attention records no gradient yet; use torch.no_grad()")
+    out, lse = _forward(q, k, v, spans, scale, softcap, slopes)
+    return (out, lse) if return_lse else out

@@ -130,19 +130,6 @@ __device__ __forceinline__ void activate_slope2(float2 z, float2& value, float2&
   }
 }
 
-// One lane of a converged warp.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t p;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
-  return p != 0;
-}
-
-// Bounded wait of a whole warp: one try by every lane, then as mbar_wait_warp.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t phase, volatile int* abort_flag, unsigned* status) {
-  if (__all_sync(0xffffffffu, mbar_try_wait(bar, phase))) return true;
-  return mbar_wait_warp(bar, phase, abort_flag, status);
-}
-
 // ---- CTA pairs -------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;

@@ -49,6 +49,19 @@ __device__ __forceinline__ void load8(const T* p, int vec, int count, float (&v)
 __device__ __forceinline__ void wait_for_prior() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// Bounded wait of a whole warp: one try by every lane, then as mbar_wait_warp.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t phase, volatile int* abort_flag, unsigned* status) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, phase))) return true;
+  return mbar_wait_warp(bar, phase, abort_flag, status);
+}
+
 // A caller's workspace: large enough, and on the 16 bytes that vector stores and TMA start on.
 inline bool usable_workspace(const void* workspace, long long bytes, long long need) {
   return workspace && bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0;

@@ -1,0 +1,706 @@
+// Attention over key spans on sm_100a tensor cores (see span_attention.cuh for the
+// mathematics): softmax(z) v with its logarithmic sums, for any lengths, shared
+// key heads, capped scores and a bias by distance.
+//
+//  * key_spans_kernel writes every query row's span of keys (documents of a packed
+//    sequence, a causal order with a prefix, a window, lengths) and, for every 128
+//    rows, the bounds that decide which key tiles are walked and which need masks;
+//  * span_attention_kernel walks them; split_attention_kernel joins the parts of
+//    calls with few rows, whose keys are split over CTAs.
+//
+// A CTA takes two tiles of 128 query rows of one head (or one: few rows, or rows
+// of several heads that share their keys side by side).  Per 128 keys and tile:
+//   S = Q K^T        tcgen05.mma, both in shared memory, S in TMEM
+//   P = 2^(z - m)    four warps, a query row a thread; m, the running maximum, is
+//                    raised only when it grows by more than 2^8, and O rescaled
+//   O += P V         tcgen05.mma, P from TMEM (over S, as 16-bit pairs)
+// While one tile's softmax runs, the tensor core works on the other's products.
+// K and V stream through five shared-memory slots by TMA.
+#include "span_attention.cuh"
+#include "../../include/peco_b200.h"
+#include "internal.h"
+
+namespace peco {
+namespace {
+
+// ---- spans ------------------------------------------------------------------------------
+struct SpanArgs {
+  const int* q_ends;        // [batch or 1, documents + 1] first rows of the documents, then the end (null: one document)
+  const int* k_ends;
+  long long q_stride, k_stride;
+  int documents;
+  const int* lengths;       // [batch] keys of each sample (without documents; null: all)
+  const int* prefix;        // [batch or 1, documents or 1] (null: prefix_all)
+  long long prefix_batch;   // elements between samples and between documents
+  int prefix_doc, prefix_all;
+  int causal, window;       // window 0: none
+  int batch, queries, keys;
+  int4* rows;
+  int4* tiles;
+};
+
+__device__ __forceinline__ int clamped(int v, int lo, int hi) { return min(max(v, lo), hi); }
+
+// A block per 128 rows of a sample, a row per thread.
+__global__ void __launch_bounds__(kTile) key_spans_kernel(const SpanArgs a) {
+  __shared__ int4 part[4];
+  wait_for_prior();
+  let_next_start();
+  const int b = blockIdx.y, i = blockIdx.x * kTile + threadIdx.x;
+  int lo = 0, hi = 0, pos = 0;
+  if (i < a.queries) {
+    int q0 = 0, q1 = a.queries, k0 = 0, k1 = a.keys, doc = 0;
+    bool inside = true;
+    if (a.documents > 0) {
+      const int* qe = a.q_ends + b * a.q_stride;
+      const int* ke = a.k_ends + b * a.k_stride;
+      int l = -1, h = a.documents + 1;  // the last entry not behind the row
+      while (h - l > 1) {
+        const int mid = (l + h) >> 1;
+        if (qe[mid] <= i) l = mid;
+        else h = mid;
+      }
+      inside = l >= 0 && l < a.documents;
+      doc = clamped(l, 0, a.documents - 1);
+      q0 = clamped(qe[doc], 0, a.queries);
+      q1 = clamped(qe[doc + 1], q0, a.queries);
+      k0 = clamped(ke[doc], 0, a.keys);
+      k1 = clamped(ke[doc + 1], k0, a.keys);
+      inside = inside && i >= q0 && i < q1;
+    } else if (a.lengths) {
+      k1 = clamped(a.lengths[b], 0, a.keys);
+    }
+    pos = k0 + (i - q0) + (k1 - k0) - (q1 - q0);
+    lo = k0;
+    hi = inside ? k1 : k0;
+    if (a.causal) {
+      const int prefix = a.prefix ? a.prefix[b * a.prefix_batch + doc * a.prefix_doc] : a.prefix_all;
+      hi = min(hi, max(pos + 1, k0 + clamped(prefix, 0, a.keys)));
+    }
+    if (a.window > 0) {
+      lo = max(lo, static_cast<int>(max(static_cast<long long>(pos) - a.window + 1, 0LL)));
+      hi = static_cast<int>(min(static_cast<long long>(hi), static_cast<long long>(pos) + a.window));
+    }
+    if (hi <= lo) lo = hi = 0;
+    a.rows[static_cast<long long>(b) * a.queries + i] = make_int4(lo, hi, pos, 0);
+  }
+  // rows that see nothing count for the masks only; rows past the end not at all
+  const bool real = i < a.queries, sees = hi > lo;
+  int4 t = make_int4(sees ? lo : 0x7fffffff, sees ? hi : 0, !real ? 0 : sees ? lo : 0x7fffffff, !real ? 0x7fffffff : hi);
+  t.x = __reduce_min_sync(0xffffffffu, t.x);
+  t.y = __reduce_max_sync(0xffffffffu, t.y);
+  t.z = __reduce_max_sync(0xffffffffu, t.z);
+  t.w = __reduce_min_sync(0xffffffffu, t.w);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = t;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 4; ++w) {
+      t.x = min(t.x, part[w].x);
+      t.y = max(t.y, part[w].y);
+      t.z = max(t.z, part[w].z);
+      t.w = min(t.w, part[w].w);
+    }
+    a.tiles[static_cast<long long>(b) * gridDim.x + blockIdx.x] = t;
+  }
+}
+
+// ---- forward ----------------------------------------------------------------------------
+constexpr int kSlots = 5;        // of K(t) in slot 2t mod 5, V(t) in slot 2t + 1 mod 5
+constexpr int kThreads = 384;    // two softmax warpgroups, one with the TMA warp and the MMA warp
+// A softmax thread holds a tile's 128 scores: the launch's 168 registers a thread
+// go 208 to 208 to 88 (256 * 208 + 128 * 88 = 384 * 168).
+constexpr uint32_t kTmemCols = 512;  // S of both tiles, then O of both
+
+struct ForwardArgs {
+  ScoreArgs s;
+  HeadRows q, k, v;         // for rows whose result is not finite
+  void* out;
+  long long out_batch, out_head, out_row;
+  float* lse;               // [batch, heads, sq]
+  int packed;               // heads side by side in a tile (1: consecutive rows of one head)
+  int tiles;                // query tiles a CTA takes: 1 or 2
+  int row_blocks;           // CTAs along a head's rows
+  int splits;               // CTAs along the keys
+  float* part;              // [unit][split][tile][128][d] unnormalised, then (max, sum) of each row
+  float2* part_sums;
+};
+
+struct __align__(8) ForwardShared {
+  uint64_t q_full, slot_full[kSlots], slot_empty[kSlots], s_full[2], p_full[2], o_full[2];
+  uint32_t tmem;
+  int abort_flag;
+};
+
+template <int D>
+constexpr int forward_smem() { return 1024 + (2 + kSlots) * kTile * D * 2 + 512; }
+static_assert(sizeof(ForwardShared) <= 512 && forward_smem<128>() <= 227 * 1024, "shared memory of a CTA");
+
+// Which head and query row thread ``r`` of tile ``w`` of a unit holds.
+struct Unit {
+  int b, head0, row0;       // first head, first row
+  __device__ Unit(const ForwardArgs& a, int unit) {
+    const int groups = a.s.heads / a.packed;
+    const int block = a.row_blocks - 1 - unit % a.row_blocks;  // in causal order the later rows see more keys
+    const int rest = unit / a.row_blocks;
+    head0 = rest % groups * a.packed;
+    b = rest / groups;
+    row0 = block * a.tiles * kTile;
+  }
+  __device__ __forceinline__ bool row(const ForwardArgs& a, int w, int r, int& head, int& i) const {
+    if (a.packed > 1) {
+      head = head0 + r / a.s.sq;
+      i = r % a.s.sq;
+      return w == 0 && r < a.packed * a.s.sq;
+    }
+    head = head0;
+    i = row0 + w * kTile + r;
+    return i < a.s.sq;
+  }
+  // keys that a row of the unit sees: [lo, hi)
+  __device__ __forceinline__ int2 keys(const ForwardArgs& a) const {
+    const int4 t0 = tile_span(a.s, b, row0 / kTile);
+    int lo = t0.x, hi = t0.y;
+    if (a.tiles == 2 && row0 + kTile < a.s.sq) {
+      const int4 t1 = tile_span(a.s, b, row0 / kTile + 1);
+      lo = min(lo, t1.x);
+      hi = max(hi, t1.y);
+    }
+    lo = max(lo, 0);
+    hi = min(hi, a.s.sk);
+    return make_int2(min(lo, hi), hi);
+  }
+};
+
+// Key tiles of one split: first key, tiles
+__device__ __forceinline__ int2 split_keys(int2 keys, int split, int splits) {
+  const int all = (keys.y - keys.x + kTile - 1) / kTile;
+  const int per = (all + splits - 1) / splits;
+  const int first = min(all, split * per);
+  return make_int2(keys.x + first * kTile, min(all, first + per) - first);
+}
+
+// One row's result again, by a warp, without the tensor core: a masked key's
+// probability is 0, but 0 times an infinite or NaN value of a key that other rows
+// of the tile do see is NaN.  Here masked keys are left out.  Rare (only rows
+// whose result is not finite, where masks were at work), so it is not fast.
+template <int AB, int D>
+__device__ __noinline__ void masked_row(const ForwardArgs& a, int b, int head, int i, int lo, int hi, int pos, int from,
+                                        int to, float m, float (&acc)[D / 32]) {
+  using T = Element<AB>;
+  const int lane = lane_id(), kv = head / (a.s.heads / a.s.kv_heads), d = a.s.d;
+  const T* q = static_cast<const T*>(a.q.ptr) + b * a.q.batch + head * a.q.head + static_cast<long long>(i) * a.q.row;
+  const T* k = static_cast<const T*>(a.k.ptr) + b * a.k.batch + kv * a.k.head;
+  const T* v = static_cast<const T*>(a.v.ptr) + b * a.v.batch + kv * a.v.head;
+  const float slope = a.s.slopes ? a.s.slopes[head] * kLog2E : 0.0f;
+  const Cap cap(a.s);
+#pragma unroll
+  for (int e = 0; e < D / 32; ++e) acc[e] = 0.0f;
+  lo = max(lo, from);
+  hi = min(hi, to);
+  for (int j0 = lo; j0 < hi; j0 += 32) {
+    const int j = j0 + lane;
+    float p = 0.0f;
+    if (j < hi) {
+      float raw = 0.0f;
+      for (int e = 0; e < d; ++e) raw = fmaf(to_f32<T>(q[e]), to_f32<T>(k[j * a.k.row + e]), raw);
+      float z = a.s.cap > 0.0f ? cap.value(cap.recip(raw)) : raw * a.s.scale * kLog2E;
+      if (a.s.slopes) z = fmaf(-slope, fabsf(static_cast<float>(pos - j)), z);
+      p = exp2_approx(z - m);
+    }
+    const int count = min(32, hi - j0);
+    for (int n = 0; n < count; ++n) {
+      const float w = __shfl_sync(0xffffffffu, p, n);
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e)
+        if (lane + 32 * e < d) acc[e] = fmaf(w, to_f32<T>(v[static_cast<long long>(j0 + n) * a.v.row + lane + 32 * e]), acc[e]);
+    }
+  }
+}
+
+// RICH: capped scores or a bias by distance
+template <int AB, int D, bool RICH>
+__global__ void __launch_bounds__(kThreads, 1)
+    span_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                          const __grid_constant__ CUtensorMap vmap, const __grid_constant__ ForwardArgs a) {
+  using T = Element<AB>;
+  constexpr int kPanels = D / 64, kTileBytes = kPanels * kPanelBytes;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  unsigned char* slots = base + 2 * kTileBytes;
+  ForwardShared& sh = *reinterpret_cast<ForwardShared*>(slots + kSlots * kTileBytes);
+  volatile int* abort_flag = &sh.abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(&sh.q_full, 1);
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&sh.slot_full[i], 1);
+      mbar_init(&sh.slot_empty[i], 1);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&sh.s_full[w], 1);
+      mbar_init(&sh.p_full[w], 4);
+      mbar_init(&sh.o_full[w], 1);
+    }
+    sh.abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 8 && lane == 0) {
+    prefetch_tensormap(&qmap);
+    prefetch_tensormap(&kmap);
+    prefetch_tensormap(&vmap);
+  }
+  if (warp == 9) {
+    tmem_alloc(&sh.tmem, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  wait_for_prior();
+  let_next_start();
+  const uint32_t tmem = sh.tmem;
+  const int split = blockIdx.x % a.splits;
+  const Unit unit(a, blockIdx.x / a.splits);
+  const int2 all_keys = unit.keys(a);
+  const int2 mine = split_keys(all_keys, split, a.splits);
+  const int key0 = mine.x, ntiles = mine.y;
+  const int tiles = a.tiles == 2 && unit.row0 + kTile < a.s.sq ? 2 : 1;
+
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  if (warp == 8) {
+    // ---------------------------------------------------------------- TMA
+    const bool issuer = elect_one();
+    const int kv = unit.head0 / (a.s.heads / a.s.kv_heads);
+    bool ok = true;
+    if (ntiles > 0 && issuer) {
+      const uint32_t q_bytes = a.packed > 1 ? static_cast<uint32_t>(a.packed * a.s.sq) * 128u * kPanels
+                                            : static_cast<uint32_t>(min(a.s.sq, kTile)) * 128u * kPanels;
+      mbar_arrive_expect_tx(&sh.q_full, q_bytes * tiles);
+      for (int w = 0; w < tiles; ++w)
+        load_rows<kPanels>(base + w * kTileBytes, &qmap, unit.row0 + w * kTile, unit.head0, unit.b, &sh.q_full);
+    }
+    __syncwarp();
+    for (int item = 0; item < 2 * ntiles && ok; ++item) {
+      const int s = item % kSlots, use = item / kSlots;
+      if (use > 0) ok = warp_wait(&sh.slot_empty[s], (use - 1) & 1, abort_flag, a.s.status);
+      if (ok && issuer) {
+        mbar_arrive_expect_tx(&sh.slot_full[s], kTileBytes);
+        load_rows<kPanels>(slots + s * kTileBytes, item & 1 ? &vmap : &kmap, key0 + (item >> 1) * kTile, kv, unit.b,
+                           &sh.slot_full[s]);
+      }
+      __syncwarp();
+    }
+    if (!ok) {  // time for the copies in flight to land before the CTA ends
+      const unsigned long long t0 = globaltimer();
+      while (globaltimer() - t0 < 2000000ull) {
+      }
+    }
+  } else if (warp == 9) {
+    // ---------------------------------------------------------------- MMA
+    constexpr uint32_t idesc_qk = instr_desc(kTile, kTile, AB, false, false);
+    constexpr uint32_t idesc_pv = instr_desc(kTile, D, AB, false, true);
+    const bool issuer = elect_one();
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t phase) {
+      if (ok) ok = warp_wait(bar, phase, abort_flag, a.s.status);
+      if (ok) tc_fence_after();
+      return ok;
+    };
+    auto wait_slot = [&](int item) { return wait(&sh.slot_full[item % kSlots], (item / kSlots) & 1); };
+    auto scores = [&](int w, int t) {
+      if (issuer) {
+        const uint32_t q = smem_u32(base + w * kTileBytes), k = smem_u32(slots + 2 * t % kSlots * kTileBytes);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) umma_ss(tmem + w * kTile, desc_dims(q, i), desc_dims(k, i), idesc_qk, i > 0);
+        umma_commit(&sh.s_full[w]);
+      }
+      __syncwarp();
+    };
+    if (ntiles > 0) {
+      wait(&sh.q_full, 0);
+      wait_slot(0);
+      for (int w = 0; w < tiles && ok; ++w) scores(w, 0);
+      if (ok && issuer) umma_commit(&sh.slot_empty[0]);
+      __syncwarp();
+      for (int t = 0; t < ntiles && ok; ++t) {
+        const int item = 2 * t + 1, s = item % kSlots;
+        if (!wait_slot(item)) break;
+        const int seen = all_keys.y - (key0 + t * kTile);  // keys past these are nobody's: their values may be anything
+        if (seen < kTile) clear_rows<kPanels>(slots + s * kTileBytes, seen, kTile, lane);
+        for (int w = 0; w < tiles; ++w) {
+          if (!wait(&sh.p_full[w], t & 1)) break;
+          if (issuer) {
+            const uint32_t v = smem_u32(slots + s * kTileBytes);
+#pragma unroll
+            for (int i = 0; i < kTile / 16; ++i)
+              umma_ts(tmem + 2 * kTile + w * kTile, tmem + w * kTile + i * 8, desc_rows(v, i), idesc_pv, t > 0 || i > 0);
+            if (w == tiles - 1) umma_commit(&sh.slot_empty[s]);
+            if (t == ntiles - 1) umma_commit(&sh.o_full[w]);
+          }
+          __syncwarp();
+          if (t + 1 < ntiles) {
+            if (w == 0 && !wait_slot(2 * t + 2)) break;
+            scores(w, t + 1);
+            if (w == tiles - 1 && issuer) umma_commit(&sh.slot_empty[(2 * t + 2) % kSlots]);
+            __syncwarp();
+          }
+        }
+      }
+    }
+  }
+  } else {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+  if ((warp >> 2) < tiles) {
+    // ------------------------------------------------------- softmax, epilogue
+    const int w = warp >> 2, r = threadIdx.x & (kTile - 1);
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + w * kTile + lanes, o_at = tmem + 2 * kTile + w * kTile + lanes;
+    int head, i;
+    const bool real = unit.row(a, w, r, head, i);
+    const int4 span = real ? span_of(a.s, unit.b, i) : make_int4(0, 0, 0, 0);
+    const int lo = span.x, hi = span.y;
+    const float scale_log2 = a.s.scale * kLog2E;
+    const Cap cap(a.s);
+    const float slope = RICH && a.s.slopes && real ? a.s.slopes[head] * kLog2E : 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true, masked = false;
+    for (int t = 0; t < ntiles; ++t) {
+      ok = warp_wait(&sh.s_full[w], t & 1, abort_flag, a.s.status);
+      if (!ok) break;
+      tc_fence_after();
+      const int j0 = key0 + t * kTile;
+      float s[kTile];
+#pragma unroll
+      for (int c = 0; c < kTile / 32; ++c) {
+        uint32_t raw[32];
+        tmem_ld32_sync(s_at + c * 32, raw);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) s[c * 32 + e] = __uint_as_float(raw[e]);
+      }
+      if constexpr (RICH) {  // to log2 units
+        if (a.s.cap > 0.0f) {
+#pragma unroll
+          for (int e = 0; e < kTile; ++e) s[e] = cap.value(cap.recip(s[e]));
+        } else {
+#pragma unroll
+          for (int e = 0; e < kTile; ++e) s[e] *= scale_log2;
+        }
+        if (a.s.slopes) {
+          const float apart = static_cast<float>(span.z - j0);
+#pragma unroll
+          for (int e = 0; e < kTile; ++e) s[e] = fmaf(-slope, fabsf(apart - static_cast<float>(e)), s[e]);
+        }
+      }
+      // rows past the tensor's end are not looked at
+      if (!__all_sync(0xffffffffu, !real || (lo <= j0 && hi >= j0 + kTile))) {
+        masked = true;
+        const int from = lo - j0, to = hi - j0;
+#pragma unroll
+        for (int e = 0; e < kTile; ++e) s[e] = e >= from && e < to ? s[e] : -INFINITY;
+      }
+      float mx[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mx[e] = fmaxf(s[e], s[e + 8]);
+#pragma unroll
+      for (int e = 16; e < kTile; e += 16)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) mx[c] = fmaxf(mx[c], fmaxf(s[e + c], s[e + 8 + c]));
+#pragma unroll
+      for (int c = 4; c > 0; c >>= 1)
+#pragma unroll
+        for (int e = 0; e < c; ++e) mx[e] = fmaxf(mx[e], mx[e + c]);
+      const float top = RICH ? mx[0] : mx[0] * scale_log2;
+      const bool grow = top > m + 8.0f || (m == -INFINITY && top > -INFINITY);
+      // the products of the tile before are complete: S came after them
+      const bool rescale = grow && m != -INFINITY;
+      if (t > 0 && __any_sync(0xffffffffu, rescale)) {
+        const float f = rescale ? exp2_approx(m - top) : 1.0f;
+        l *= f;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t raw[32], part[16];
+          tmem_ld32_sync(o_at + c * 32, raw);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) part[e] = __float_as_uint(__uint_as_float(raw[h * 16 + e]) * f);
+            tmem_st16(o_at + c * 32 + h * 16, part);
+          }
+        }
+      }
+      if (grow) m = top;
+      const float neg = m == -INFINITY ? 0.0f : -m;
+      const float2 neg2 = make_float2(neg, neg), scale2 = make_float2(scale_log2, scale_log2);
+      float2 sums[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sums[e] = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int c = 0; c < kTile / 32; ++c) {
+        uint32_t packed[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float2 z = make_float2(s[c * 32 + e], s[c * 32 + e + 1]);
+          const float2 x = RICH ? fadd2(z, neg2) : ffma2(z, scale2, neg2);
+          const float2 p = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+          sums[(e >> 1) & 3] = fadd2(sums[(e >> 1) & 3], p);
+          packed[e >> 1] = pack2<T>(p.x, p.y);
+        }
+        tmem_st16(s_at + c * 16, packed);
+      }
+      const float2 sum = fadd2(fadd2(sums[0], sums[1]), fadd2(sums[2], sums[3]));
+      l += sum.x + sum.y;
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.p_full[w]);
+    }
+    if (ok && ntiles > 0) {
+      ok = warp_wait(&sh.o_full[w], 0, abort_flag, a.s.status);
+      tc_fence_after();
+    }
+    if (ok) {
+      const bool whole = a.splits == 1;
+      const float inv = !whole ? 1.0f : l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;  // (a NaN stays)
+      T* out = nullptr;
+      float* part = nullptr;
+      if (real && whole) {
+        out = static_cast<T*>(a.out) + unit.b * a.out_batch + head * a.out_head + static_cast<long long>(i) * a.out_row;
+        a.lse[(static_cast<long long>(unit.b) * a.s.heads + head) * a.s.sq + i] =
+            l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+      } else if (real) {
+        const long long at = (static_cast<long long>(blockIdx.x) * a.tiles + w) * kTile + r;
+        part = a.part + at * a.s.d;
+        a.part_sums[at] = make_float2(m, l);
+      }
+      bool finite = true;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t raw[32];
+        if (ntiles > 0) tmem_ld32_sync(o_at + c * 32, raw);
+        else
+#pragma unroll
+          for (int e = 0; e < 32; ++e) raw[e] = 0u;
+        float2 v[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          // a row without a visible key is 0 whatever its masked values were
+          v[e] = l == 0.0f ? make_float2(0.0f, 0.0f)
+                           : fmul2(make_float2(__uint_as_float(raw[2 * e]), __uint_as_float(raw[2 * e + 1])), make_float2(inv, inv));
+          finite = finite && fabsf(v[e].x) < INFINITY && fabsf(v[e].y) < INFINITY;
+        }
+        if (out) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            if (c * 32 + g * 8 < a.s.d)
+              *reinterpret_cast<uint4*>(out + c * 32 + g * 8) =
+                  make_uint4(pack2<T>(v[4 * g].x, v[4 * g].y), pack2<T>(v[4 * g + 1].x, v[4 * g + 1].y),
+                             pack2<T>(v[4 * g + 2].x, v[4 * g + 2].y), pack2<T>(v[4 * g + 3].x, v[4 * g + 3].y));
+        } else if (part) {
+#pragma unroll
+          for (int g = 0; g < 8; ++g)
+            if (c * 32 + g * 4 < a.s.d)
+              *reinterpret_cast<float4*>(part + c * 32 + g * 4) = make_float4(v[2 * g].x, v[2 * g].y, v[2 * g + 1].x, v[2 * g + 1].y);
+        }
+      }
+      // (with a NaN or infinite sum the row sees such scores itself)
+      uint32_t again = __ballot_sync(0xffffffffu, masked && real && !finite && l > 0.0f && l < INFINITY);
+      while (again) {
+        __syncwarp();  // the row's first result is written
+        const int from = __ffs(again) - 1;
+        again &= again - 1;
+        auto of = [&](int v) { return __shfl_sync(0xffffffffu, v, from); };
+        const int h2 = of(head), i2 = of(i);
+        const float f = __shfl_sync(0xffffffffu, inv, from);
+        float acc[D / 32];
+        masked_row<AB, D>(a, unit.b, h2, i2, of(lo), of(hi), of(span.z), key0, key0 + ntiles * kTile,
+                          __shfl_sync(0xffffffffu, m, from), acc);
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) {
+          const int c = lane + 32 * e;
+          if (c >= a.s.d) continue;
+          if (whole)
+            static_cast<T*>(a.out)[unit.b * a.out_batch + h2 * a.out_head + static_cast<long long>(i2) * a.out_row + c] =
+                from_f32<T>(acc[e] * f);
+          else
+            a.part[((static_cast<long long>(blockIdx.x) * a.tiles + w) * kTile + (r - lane) + from) * a.s.d + c] = acc[e] * f;
+        }
+      }
+    }
+  }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// A row's parts joined: out = sum_p O_p 2^(m_p - M) / sum_p l_p 2^(m_p - M); a warp a row.
+template <int AB>
+__global__ void __launch_bounds__(128) split_attention_kernel(const __grid_constant__ ForwardArgs a) {
+  using T = Element<AB>;
+  wait_for_prior();
+  let_next_start();
+  const int lane = threadIdx.x & 31;
+  const long long at = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);  // (unit, tile, row of the tile)
+  const int r = static_cast<int>(at % kTile), w = static_cast<int>(at / kTile % a.tiles);
+  const int n = static_cast<int>(at / kTile / a.tiles);
+  const Unit unit(a, n);
+  int head, i;
+  if (!unit.row(a, w, r, head, i)) return;
+  const long long first = (static_cast<long long>(n) * a.splits * a.tiles + w) * kTile + r, step = static_cast<long long>(a.tiles) * kTile;
+  float m = -INFINITY;
+  for (int p = lane; p < a.splits; p += 32) m = fmaxf(m, a.part_sums[first + p * step].x);
+  m = warp_max(m);
+  float l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int p = 0; p < a.splits; ++p) {
+    const float2 s = a.part_sums[first + p * step];
+    if (s.y == 0.0f) continue;
+    const float f = exp2_approx(s.x - m);
+    l = fmaf(s.y, f, l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (lane + 32 * e < a.s.d) acc[e] = fmaf(a.part[(first + p * step) * a.s.d + lane + 32 * e], f, acc[e]);
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  T* out = static_cast<T*>(a.out) + unit.b * a.out_batch + head * a.out_head + static_cast<long long>(i) * a.out_row;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (lane + 32 * e < a.s.d) out[lane + 32 * e] = from_f32<T>(acc[e] * inv);
+  if (lane == 0)
+    a.lse[(static_cast<long long>(unit.b) * a.s.heads + head) * a.s.sq + i] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// ---- host ---------------------------------------------------------------------------------
+// How a call is cut.  Two tiles a CTA keep the tensor core busy under the softmax;
+// one where that leaves SMs without work.  Rows of heads that share their keys go
+// side by side into one tile where they fit: the keys are then read once for all of
+// them.  Calls that still leave half of the SMs idle split the keys, four tiles at
+// least to a part.
+struct ForwardCut {
+  int packed, tiles, row_blocks, splits;
+  long long units;
+};
+
+ForwardCut cut_forward(int batch, int heads, int kv_heads, int sq, int sk) {
+  ForwardCut c{1, 1, 1, 1, 0};
+  const int group = heads / kv_heads;
+  for (int n = 2; n <= group; ++n)
+    if (group % n == 0 && static_cast<long long>(n) * sq <= kTile) c.packed = n;
+  const long long pairs = (sq + 2LL * kTile - 1) / (2 * kTile);
+  if (sq > kTile && pairs * batch * heads >= kNumSMs) c.tiles = 2;
+  c.row_blocks = static_cast<int>((sq + static_cast<long long>(c.tiles) * kTile - 1) / (c.tiles * kTile));
+  c.units = static_cast<long long>(batch) * (heads / c.packed) * c.row_blocks;
+  if (c.units * 2 <= kNumSMs) {
+    const long long most = (static_cast<long long>(sk) + 4 * kTile - 1) / (4 * kTile), fill = kNumSMs / c.units;
+    c.splits = static_cast<int>(fill < most ? fill : most);
+    if (c.splits < 1) c.splits = 1;
+  }
+  return c;
+}
+
+bool valid_attention(int batch, int heads, int kv_heads, int sq, int sk, int d) {
+  return batch >= 0 && heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0 && sq >= 0 && sk >= 0 && d >= 8 && d <= 128 &&
+         d % 8 == 0 && sq <= 0x7ffffe00 && sk <= 0x7ffffe00;
+}
+
+long long part_rows(const ForwardCut& c) { return c.splits > 1 ? c.units * c.splits * c.tiles * kTile : 0; }
+
+template <int AB, int D>
+int launch_forward(const ForwardArgs& a, const ForwardCut& c, const CUtensorMap (&maps)[3], cudaStream_t stream) {
+  const bool rich = a.s.cap > 0.0f || a.s.slopes;
+  auto kernel = rich ? span_attention_kernel<AB, D, true> : span_attention_kernel<AB, D, false>;
+  static std::atomic<unsigned long long> granted[2] = {};
+  if (cudaError_t e = grant_smem(reinterpret_cast<const void*>(kernel), forward_smem<D>(), granted[rich])) return static_cast<int>(e);
+  const dim3 grid(static_cast<unsigned>(c.units * c.splits));
+  if (int st = launch_overlapped(kernel, grid, dim3(kThreads), forward_smem<D>(), 0, stream, maps[0], maps[1], maps[2], a)) return st;
+  if (c.splits == 1) return kOk;
+  return launch_overlapped(split_attention_kernel<AB>, dim3(static_cast<unsigned>(c.units * c.tiles * (kTile / 4))), dim3(128), 0,
+                           0, stream, a);
+}
+
+}  // namespace
+}  // namespace peco
+
+using namespace peco;
+
+extern "C" int peco_key_spans(const int* q_ends, long long q_stride, const int* k_ends, long long k_stride, int documents,
+                              const int* lengths, const int* prefix, long long prefix_batch, int prefix_document,
+                              int prefix_all, int causal, int window, int batch, int queries, int keys, int* rows,
+                              int* tiles, void* stream_ptr) {
+  if (batch < 0 || batch > 65535 || queries < 0 || keys < 0 || queries > 0x7ffffe00 || keys > 0x7ffffe00 || documents < 0 ||
+      documents > 0x7ffffff0 || window < 0 || (documents > 0 && (!q_ends || !k_ends || lengths)))
+    return kErrInvalidValue;
+  if (batch == 0 || queries == 0) return kOk;
+  if (!rows || !tiles || (reinterpret_cast<uintptr_t>(rows) & 15) || (reinterpret_cast<uintptr_t>(tiles) & 15)) return kErrInvalidValue;
+  SpanArgs a{q_ends, k_ends, q_stride, k_stride, documents, lengths, prefix, prefix_batch, prefix_document, prefix_all,
+             causal, window, batch, queries, keys, reinterpret_cast<int4*>(rows), reinterpret_cast<int4*>(tiles)};
+  return launch_overlapped(key_spans_kernel, dim3((queries + kTile - 1) / kTile, batch), dim3(kTile), 0, 0,
+                           static_cast<cudaStream_t>(stream_ptr), a);
+}
+
+extern "C" long long peco_span_attention_workspace(int batch, int heads, int kv_heads, int sq, int sk, int d) {
+  if (!valid_attention(batch, heads, kv_heads, sq, sk, d)) return -1;
+  if (batch == 0 || sq == 0) return 0;
+  const ForwardCut c = cut_forward(batch, heads, kv_heads, sq, sk);
+  return part_rows(c) * (4LL * d + 8);
+}
+
+extern "C" int peco_span_attention(const void* q, const void* k, const void* v, const long long* strides,
+                                   const int* span_rows, const int* span_tiles, int spans_batched, const float* slopes,
+                                   float scale, float cap, void* out, float* lse, int batch, int heads, int kv_heads, int sq,
+                                   int sk, int d, int dtype, void* workspace, long long workspace_bytes,
+                                   void* stream_ptr) {
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  if (dtype != 0 && dtype != 1) return kErrUnsupported;
+  if (!valid_attention(batch, heads, kv_heads, sq, sk, d) || !(scale > 0.0f) || !(cap >= 0.0f) || !strides) return kErrInvalidValue;
+  if (batch == 0 || sq == 0) return kOk;
+  if (!q || !out || !lse || (sk > 0 && (!k || !v)) || (span_rows == nullptr) != (span_tiles == nullptr)) return kErrInvalidValue;
+  ForwardArgs a{};
+  a.q = HeadRows{q, strides[0], strides[1], strides[2]};
+  a.k = HeadRows{k, strides[3], strides[4], strides[5]};
+  a.v = HeadRows{v, strides[6], strides[7], strides[8]};
+  const HeadRows o{out, strides[9], strides[10], strides[11]};
+  if (!readable(a.q, batch, heads, sq) || !readable(o, batch, heads, sq) ||
+      (sk > 0 && (!readable(a.k, batch, kv_heads, sk) || !readable(a.v, batch, kv_heads, sk))))
+    return kErrInvalidValue;
+  const ForwardCut c = cut_forward(batch, heads, kv_heads, sq, sk);
+  if (c.units * c.splits > 0x7fffffffLL) return kErrUnsupported;
+  if (c.splits > 1 && !usable_workspace(workspace, workspace_bytes, part_rows(c) * (4LL * d + 8))) return kErrWorkspace;
+  a.s.spans = reinterpret_cast<const int4*>(span_rows);
+  a.s.span_tiles = reinterpret_cast<const int4*>(span_tiles);
+  a.s.spans_batched = spans_batched;
+  a.s.slopes = slopes;
+  a.s.batch = batch;
+  a.s.heads = heads;
+  a.s.kv_heads = kv_heads;
+  a.s.sq = sq;
+  a.s.sk = sk;
+  a.s.d = d;
+  a.s.scale = scale;
+  a.s.cap = cap;
+  a.s.status = device_status_ptr();
+  a.out = out;
+  a.out_batch = o.batch;
+  a.out_head = o.head;
+  a.out_row = o.row;
+  a.lse = lse;
+  a.packed = c.packed;
+  a.tiles = c.tiles;
+  a.row_blocks = c.row_blocks;
+  a.splits = c.splits;
+  a.part = static_cast<float*>(workspace);
+  a.part_sums = reinterpret_cast<float2*>(static_cast<float*>(workspace) + part_rows(c) * d);
+  const HeadRows none{q, 0, 0, 0};  // without keys nothing is loaded
+  CUtensorMap maps[3];
+  const int box_rows = sq < kTile ? sq : kTile, key_rows = sk > 0 ? sk : 1;
+  if (!head_map(&maps[0], a.q, batch, heads, sq, d, box_rows, c.packed, dtype) ||
+      !head_map(&maps[1], sk > 0 ? a.k : none, sk > 0 ? batch : 1, sk > 0 ? kv_heads : 1, key_rows, d, kTile, 1, dtype) ||
+      !head_map(&maps[2], sk > 0 ? a.v : none, sk > 0 ? batch : 1, sk > 0 ? kv_heads : 1, key_rows, d, kTile, 1, dtype))
+    return kErrTensorMap;
+  if (d <= 64) return dtype == 1 ? launch_forward<1, 64>(a, c, maps, stream) : launch_forward<0, 64>(a, c, maps, stream);
+  return dtype == 1 ? launch_forward<1, 128>(a, c, maps, stream) : launch_forward<0, 128>(a, c, maps, stream);
+}
