@@ -10,7 +10,7 @@ get a bias that depends on the distance:
 
 Products run on the tcgen05 tensor cores with fp32 sums, softmax statistics in
 fp32; float16 and bfloat16; keys may be shared by groups of query heads.  A row
-that sees no key is 0.  CUDA tensors only; work is enqueued on
+that sees no key is 0.  Differentiable.  CUDA tensors only; work is enqueued on
 the current stream.
 """
 
@@ -212,6 +212,27 @@ def _forward(q, k, v, spans, scale, softcap, slopes):
     return out.copy_(whole) if whole is not out else out, lse
 
 
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, spans, scale, softcap, slopes):
+        out, lse = _forward(q, k, v, spans, scale, softcap, slopes)
+        ctx.sizes, ctx.scores = (spans.queries, spans.keys) if spans is not None else None, (scale, softcap)
+        mask = (spans.rows, spans.tiles) if spans is not None else (None, None)
+        ctx.save_for_backward(q, k, v, out, lse, slopes, *mask)  # (changing any of them meanwhile is an error)
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, _):
+        q, k, v, out, lse, slopes, rows, tiles = ctx.saved_tensors
+        spans = KeySpans(rows, tiles, *ctx.sizes) if ctx.sizes is not None else None
+        scale, softcap = ctx.scores
+        names = [n for n, need in zip("qkv", ctx.needs_input_grad) if need]
+        g = attention_backward(grad, q, k, v, out, lse, spans=spans, scale=scale, softcap=softcap, slopes=slopes, needs=names)
+        return g.q, g.k, g.v, None, None, None, None
+
+
 def attention(q, k, v, *, spans=None, scale=None, softcap=None, slopes=None, return_lse=False):
     """Attention of q [B, H, N, D] over k, v [B, KV, M, D] (H a multiple of KV: each key head serves H / KV query heads).
 
@@ -224,10 +245,65 @@ def attention(q, k, v, *, spans=None, scale=None, softcap=None, slopes=None, ret
 
     D is a multiple of 8 up to 128.  Strides are free where D is adjacent and
     rows, heads and samples start on 16 bytes; other layouts are copied first.
-    The result has the layout of q.
+    The result has the layout of q.  Keys and values that a row's mask leaves
+    out do not reach its result, whatever they hold.
     """
     _native.refuse_tangents("attention", q, k, v, slopes)
     if torch.is_grad_enabled() and _native.wants_grad(q, k, v):
-        raise RuntimeError("attention records no gradient yet; use torch.no_grad()")
-    out, lse = _forward(q, k, v, spans, scale, softcap, slopes)
+        out, lse = _Attention.apply(q, k, v, spans, scale, softcap, slopes)
+    else:
+        out, lse = _forward(q, k, v, spans, scale, softcap, slopes)
     return (out, lse) if return_lse else out
+
+
+def attention_backward(grad, q, k, v, out, lse, *, spans=None, scale=None, softcap=None, slopes=None, needs=None):
+    """Gradients of ``attention`` for ``grad`` = d out, with the call's results ``out`` and ``lse``.
+
+    ``needs``: names of the gradients to compute (default: q, k and v).  The
+    probabilities and their gradients are rounded to the operands' type for the
+    products (in float16 to that type's range too: scale the loss for it); sums
+    run in a fixed order.  Rows that see no key, and keys that no row sees, get
+    zeros and may hold anything; a NaN in a row or key that is seen reaches
+    the gradients of its tile.
+    """
+    _native.refuse_tangents("attention_backward", grad, q, k, v, out, slopes)
+    sizes, scale, cap = _check(q, k, v, spans, scale, softcap, slopes)
+    b, h, kv, n, m, d = sizes
+    for name, t in (("grad", grad), ("out", out)):
+        if not isinstance(t, torch.Tensor) or t.shape != q.shape:
+            raise ValueError(f"{name} must have the shape of q")
+        if t.dtype is not q.dtype:
+            raise TypeError(f"{name} must have the dtype of q")
+    if not isinstance(lse, torch.Tensor) or lse.dtype is not torch.float32 or lse.shape != (b, h, n):
+        raise ValueError(f"lse must be a float32 tensor {[b, h, n]}")
+    needs = ("q", "k", "v") if needs is None else tuple(needs)
+    if set(needs) - {"q", "k", "v"}:
+        raise ValueError(f"needs must name gradients of q, k and v, got {list(needs)}")
+    _native.require_cuda(q, grad, out, lse)
+    given = {"q": q, "k": k, "v": v}
+    made = {name: torch.empty_like(t) for name, t in given.items() if name in needs}
+    if not made:
+        return AttentionGrads(None, None, None)
+    # results whose layout TMA could not read are made elsewhere and copied
+    whole = {name: t if t.numel() == 0 or _readable(t) is t else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+             for name, t in made.items()}
+    if b and (n or m):
+        grad, q, k, v, out = (t if t.numel() == 0 else _readable(t) for t in (grad, q, k, v, out))
+        lse = lse.contiguous()
+        if slopes is not None:
+            slopes = slopes.contiguous()
+        lib = _native.load()
+        need = int(lib.peco_span_attention_backward_workspace(b, h, n))
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+        to = [whole.get(name) for name in "qkv"]
+        strides = _GradStrides(*(s for t in (grad, q, k, v, out, *to) for s in (t.stride()[:3] if t is not None else (0, 0, 0))))
+        rows, tiles, batched = _mask_args(spans, b)
+        _native.enqueue(q.device, "peco_span_attention_backward", lib.peco_span_attention_backward,
+                        (grad.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), strides,
+                         rows, tiles, batched, _native.address(slopes), scale, cap, *(_native.address(t) for t in to), b, h,
+                         kv, n, m, d, _native.DTYPE_CODE[q.dtype], _native.address(ws), max(need, 0)),
+                        (grad, q, k, v, out, lse, slopes, *((spans.rows, spans.tiles) if spans is not None else ())))
+    for name, t in made.items():
+        if whole[name] is not t:
+            t.copy_(whole[name])
+    return AttentionGrads(*(made.get(name) for name in "qkv"))

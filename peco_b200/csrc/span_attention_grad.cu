@@ -1,0 +1,732 @@
+// Gradient of attention over key spans on sm_100a tensor cores (see
+// span_attention.cuh).  With p_ij = exp(z_ij - lse_i), delta_i = sum_d g_id out_id
+// and s' = dz/d(scale q.k), 1 or 1 - tanh^2:
+//   ds_ij = p_ij (g_i.v_j - delta_i) s'_ij
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij g_i
+//
+// One launch holds two kinds of CTAs.  Those of 128 keys walk the query tiles (of
+// all the heads that share the keys) and keep dk and dv in TMEM; those of 128
+// query rows walk the keys and keep dq.  Scores and g.v are computed in both,
+// seven products instead of five; in exchange no sum crosses a CTA: there are no
+// atomics, no fp32 copy of dq in memory, and results do not depend on the launch.
+#include "span_attention.cuh"
+#include "../../include/peco_b200.h"
+#include "internal.h"
+
+namespace peco {
+namespace {
+
+constexpr int kGradThreads = 384;  // eight softmax warps, then TMA, MMA and statistics warps
+constexpr int kKeySlots = 4;       // of K(t) and V(t) under a query tile
+
+struct GradArgs {
+  ScoreArgs s;
+  HeadRows out, grad;        // of the statistics
+  const float* lse;
+  float2* stats;             // [batch, heads, padded rows]: lse in log2 units (none: infinity) and delta
+  int padded;                // rows, a multiple of 128
+  void *dq, *dk, *dv;
+  long long q_batch, q_head, q_row, k_batch, k_head, k_row, v_batch, v_head, v_row;
+  int key_units, query_units;
+};
+
+// fp16's small probabilities would lose bits below 2^-14: they are held 2^10
+// times larger (at most 2^10), and dv is scaled back.
+template <int AB>
+struct Held {
+  static constexpr float kShift = AB == 1 ? 0.0f : 10.0f, kBack = AB == 1 ? 1.0f : 1.0f / 1024.0f;
+};
+
+// stats of every row; 16 lanes a row
+template <int AB>
+__global__ void __launch_bounds__(256) grad_stats_kernel(const __grid_constant__ GradArgs a) {
+  using T = Element<AB>;
+  wait_for_prior();
+  let_next_start();
+  const long long at = static_cast<long long>(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  const long long heads = at / a.padded;
+  const int i = static_cast<int>(at - heads * a.padded), lane = threadIdx.x & 15;
+  const int b = static_cast<int>(heads / a.s.heads), h = static_cast<int>(heads - static_cast<long long>(b) * a.s.heads);
+  float sum = 0.0f, l = -INFINITY;
+  if (b < a.s.batch && i < a.s.sq) {
+    l = a.lse[heads * a.s.sq + i];
+    if (lane * 8 < a.s.d) {
+      float x[8], y[8];
+      load8(static_cast<const T*>(a.out.ptr) + b * a.out.batch + h * a.out.head + static_cast<long long>(i) * a.out.row + lane * 8, 1, 8, x);
+      load8(static_cast<const T*>(a.grad.ptr) + b * a.grad.batch + h * a.grad.head + static_cast<long long>(i) * a.grad.row + lane * 8, 1, 8, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum = fmaf(x[e], y[e], sum);
+    }
+  }
+#pragma unroll
+  for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0 && b < a.s.batch)
+    a.stats[at] = l == -INFINITY ? make_float2(INFINITY, 0.0f) : make_float2(l * kLog2E - Held<AB>::kShift, sum * Held<AB>::kBack);
+}
+
+// One step of a CTA of keys: a query tile of one head, as the statistics warp lays it out.
+struct Step {
+  float lse[kTile], delta[kTile], pos[kTile];
+  int lo[kTile], hi[kTile];
+  int masked, clear, end, head;
+};
+
+struct __align__(16) GradShared {
+  Step step[2];
+  uint64_t own_full;                                 // the CTA's own two tiles
+  uint64_t rows_full[2], step_full[2], rows_empty[2];  // CTAs of keys: stages of query rows
+  uint64_t slot_full[kKeySlots], slot_empty[kKeySlots];  // CTAs of query rows: K and V
+  uint64_t s_full[2], p_full, dp_full, dp_free, ds_full[2], done;
+  uint32_t tmem;
+  int first, last, abort_flag;
+};
+
+template <int D>
+constexpr int grad_smem() { return 1024 + (2 + kKeySlots) * kTile * D * 2 + 16; }
+static_assert(grad_smem<128>() + sizeof(GradShared) <= 227 * 1024, "shared memory of a CTA");
+
+struct Roles {
+  int warp, lane;
+  bool ok;
+  volatile int* abort_flag;
+  unsigned* status;
+  __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t phase) {
+    if (ok) ok = warp_wait(bar, phase & 1, abort_flag, status);
+    if (ok) tc_fence_after();
+    return ok;
+  }
+  __device__ __forceinline__ void arrive(uint64_t* bar) {
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+  }
+  __device__ __forceinline__ void land() {  // copies in flight land before the CTA ends
+    if (ok) return;
+    const unsigned long long t0 = globaltimer();
+    while (globaltimer() - t0 < 2000000ull) {
+    }
+  }
+};
+
+// A 128 x 16n product from two tiles along the dimensions: X Y^T
+template <int D>
+__device__ __forceinline__ void product_dims(uint32_t to, uint32_t x, uint32_t y, uint32_t idesc) {
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) umma_ss(to, desc_dims(x, i), desc_dims(y, i), idesc, i > 0);
+}
+// to (+)= A Y over Y's rows, A 16-bit pairs in TMEM, each half of 64 over the half of the scores it came from
+__device__ __forceinline__ void product_rows(uint32_t to, uint32_t a, uint32_t y, uint32_t idesc, bool accumulate) {
+#pragma unroll
+  for (int i = 0; i < kTile / 16; ++i) umma_ts(to, a + (i >> 2) * 64 + (i & 3) * 8, desc_rows(y, i), idesc, accumulate || i > 0);
+}
+
+// 64 columns of TMEM as fp32
+__device__ __forceinline__ void load_half(uint32_t at, float (&v)[64]) {
+  uint32_t raw[64];
+  tmem_ld64_sync(at, raw);
+#pragma unroll
+  for (int e = 0; e < 64; ++e) v[e] = __uint_as_float(raw[e]);
+}
+template <typename T>
+__device__ __forceinline__ void store_half(uint32_t at, const float (&v)[64]) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint32_t packed[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) packed[e] = pack2<T>(v[c * 32 + 2 * e], v[c * 32 + 2 * e + 1]);
+    tmem_st16(at + c * 16, packed);
+  }
+  tmem_st_wait();
+}
+
+// A row of an accumulator, scaled, to memory (zeros without one)
+template <typename T, int D>
+__device__ __forceinline__ void store_row(T* out, uint32_t at, float scale, int d, bool any) {
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t raw[32];
+    if (any) tmem_ld32_sync(at + c * 32, raw);
+    else
+#pragma unroll
+      for (int e = 0; e < 32; ++e) raw[e] = 0u;
+    if (out) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        if (c * 32 + g * 8 < d) {
+          uint32_t u[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            u[e] = pack2<T>(__uint_as_float(raw[g * 8 + 2 * e]) * scale, __uint_as_float(raw[g * 8 + 2 * e + 1]) * scale);
+          *reinterpret_cast<uint4*>(out + c * 32 + g * 8) = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+    }
+  }
+}
+
+// The steps of a CTA of keys: heads of the group, query tiles that see one of its keys.
+struct StepWalk {
+  int head, tile;
+  __device__ __forceinline__ bool next(const ScoreArgs& s, int b, int j0, int first, int last, int end_head) {
+    for (;;) {
+      if (++tile >= last) {
+        tile = first - 1;
+        if (++head >= end_head) return false;
+        continue;
+      }
+      if (!s.spans) return true;
+      const int4 t = tile_span(s, b, tile);
+      if (t.x < j0 + kTile && t.y > j0) return true;
+    }
+  }
+};
+
+template <int AB, int D, bool RICH>
+__global__ void __launch_bounds__(kGradThreads, 1)
+    span_attention_grad_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                               const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap gmap,
+                               const __grid_constant__ GradArgs a) {
+  using T = Element<AB>;
+  constexpr int kPanels = D / 64, kTileBytes = kPanels * kPanelBytes;
+  constexpr uint32_t kDims = instr_desc(kTile, kTile, AB, false, false), kRows = instr_desc(kTile, D, AB, false, true);
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  __shared__ GradShared sh;
+  unsigned char* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  unsigned char* ring = base + 2 * kTileBytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Roles me{warp, lane, true, &sh.abort_flag, a.s.status};
+  if (threadIdx.x == 0) {
+    mbar_init(&sh.own_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.rows_full[i], 1);
+      mbar_init(&sh.step_full[i], 1);
+      mbar_init(&sh.rows_empty[i], 1);
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.ds_full[i], 8);
+    }
+    for (int i = 0; i < kKeySlots; ++i) {
+      mbar_init(&sh.slot_full[i], 1);
+      mbar_init(&sh.slot_empty[i], 1);
+    }
+    mbar_init(&sh.p_full, 8);
+    mbar_init(&sh.dp_full, 1);
+    mbar_init(&sh.dp_free, 8);
+    mbar_init(&sh.done, 1);
+    sh.abort_flag = 0;
+    sh.first = 0x7fffffff;
+    sh.last = 0;
+    fence_barrier_init();
+  }
+  if (warp == 8 && lane == 0) {
+    prefetch_tensormap(&qmap);
+    prefetch_tensormap(&kmap);
+    prefetch_tensormap(&vmap);
+    prefetch_tensormap(&gmap);
+  }
+  if (warp == 9) {
+    tmem_alloc(&sh.tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  wait_for_prior();
+  let_next_start();
+  const uint32_t tmem = sh.tmem;
+  const int group = a.s.heads / a.s.kv_heads;
+  const int half = (warp >> 2) & 1;  // of a softmax warp: its 64 columns
+  const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+  const int r = (warp & 3) * 32 + lane;
+  const float scale_log2 = a.s.scale * kLog2E;
+
+  if (static_cast<int>(blockIdx.x) < a.key_units) {
+    // ================================================================ dk and dv of 128 keys
+    const int blocks = (a.s.sk + kTile - 1) / kTile;
+    const int j0 = static_cast<int>(blockIdx.x) % blocks * kTile;
+    const int kv = static_cast<int>(blockIdx.x) / blocks % a.s.kv_heads, b = static_cast<int>(blockIdx.x) / blocks / a.s.kv_heads;
+    const int tiles = row_tiles(a.s);
+    if (a.s.spans) {  // the query tiles between the first and the last that see one of the keys
+      for (int t = threadIdx.x; t < tiles; t += kGradThreads) {
+        const int4 sp = tile_span(a.s, b, t);
+        if (sp.x < j0 + kTile && sp.y > j0) {
+          atomicMin(&sh.first, t);
+          atomicMax(&sh.last, t + 1);
+        }
+      }
+    } else if (threadIdx.x == 0) {
+      sh.first = 0;
+      sh.last = tiles;
+    }
+    __syncthreads();
+    const int first = sh.first, last = sh.last;
+    const bool any = first < last;
+    const uint32_t s_at = tmem, dp_at = tmem + kTile, dv_at = tmem + 2 * kTile, dk_at = tmem + 3 * kTile;
+    StepWalk walk{kv * group, first - 1};
+    if (warp >= 8) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+      if (any && warp == 8) {
+        // ------------------------------------------------------------ TMA
+        const bool issuer = elect_one();
+        if (issuer) {
+          mbar_arrive_expect_tx(&sh.own_full, 2 * kTileBytes);
+          load_rows<kPanels>(base, &kmap, j0, kv, b, &sh.own_full);
+          load_rows<kPanels>(base + kTileBytes, &vmap, j0, kv, b, &sh.own_full);
+        }
+        __syncwarp();
+        for (int n = 0; me.ok && walk.next(a.s, b, j0, first, last, (kv + 1) * group); ++n) {
+          const int st = n & 1;
+          if (n >= 2 && !me.wait(&sh.rows_empty[st], (n >> 1) - 1)) break;
+          if (issuer) {
+            mbar_arrive_expect_tx(&sh.rows_full[st], 2 * kTileBytes);
+            load_rows<kPanels>(ring + st * 2 * kTileBytes, &qmap, walk.tile * kTile, walk.head, b, &sh.rows_full[st]);
+            load_rows<kPanels>(ring + (st * 2 + 1) * kTileBytes, &gmap, walk.tile * kTile, walk.head, b, &sh.rows_full[st]);
+          }
+          __syncwarp();
+        }
+        me.land();
+      } else if (any && warp == 10) {
+        // ------------------------------------------------------------ statistics of each step
+        for (int n = 0;; ++n) {
+          const bool more = walk.next(a.s, b, j0, first, last, (kv + 1) * group);
+          Step& step = sh.step[n & 1];
+          if (n >= 2 && !me.wait(&sh.rows_empty[n & 1], (n >> 1) - 1)) break;
+          if (more) {
+            const int i0 = walk.tile * kTile;
+            const int4 t = tile_span(a.s, b, walk.tile);
+            const bool full = t.z <= j0 && t.w >= min(j0 + kTile, a.s.sk) && i0 + kTile <= a.s.sq;
+            const float2* stats = a.stats + (static_cast<long long>(b) * a.s.heads + walk.head) * a.padded + i0;
+#pragma unroll
+            for (int e = 0; e < kTile; e += 32) {
+              const float2 f = stats[e + lane];
+              step.lse[e + lane] = f.x;
+              step.delta[e + lane] = f.y;
+              if (RICH || !full) {
+                const int4 sp = i0 + e + lane < a.s.sq ? span_of(a.s, b, i0 + e + lane) : make_int4(0, 0, 0, 0);
+                step.lo[e + lane] = sp.x;
+                step.hi[e + lane] = sp.y;
+                step.pos[e + lane] = static_cast<float>(sp.z);
+              }
+            }
+            if (lane == 0) {
+              step.head = walk.head;
+              step.masked = full ? 0 : 1;
+              step.clear = t.z == 0x7fffffff ? 1 : 0;  // some row sees nothing
+            }
+          }
+          if (lane == 0) step.end = more ? 0 : 1;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.step_full[n & 1]);
+          if (!more) break;
+        }
+      } else if (any && warp == 9) {
+        // ------------------------------------------------------------ MMA
+        const bool issuer = elect_one();
+        const uint32_t k = smem_u32(base), v = k + kTileBytes;
+        auto q_of = [&](int n) { return smem_u32(ring + (n & 1) * 2 * kTileBytes); };
+        // the step's tiles are there; false at the end
+        auto ready = [&](int n) {
+          const int st = n & 1;
+          if (!me.wait(&sh.step_full[st], n >> 1) || sh.step[st].end || !me.wait(&sh.rows_full[st], n >> 1)) return false;
+          if (sh.step[st].clear) {  // rows that see nothing may hold anything
+            for (int row = lane; row < kTile; row += 32)
+              if (sh.step[st].lo[row] >= sh.step[st].hi[row])
+                for (int p = 0; p < 2 * kPanels; ++p)
+                  for (int c = 0; c < 8; ++c)
+                    *reinterpret_cast<uint4*>(ring + st * 2 * kTileBytes + p * kPanelBytes + row * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+            fence_async_smem();
+            __syncwarp();
+          }
+          return true;
+        };
+        auto scores = [&](int n) {
+          if (issuer) {
+            product_dims<D>(s_at, k, q_of(n), kDims);
+            umma_commit(&sh.s_full[0]);
+          }
+          __syncwarp();
+        };
+        auto values = [&](int n) {
+          if (issuer) {
+            product_dims<D>(dp_at, v, q_of(n) + kTileBytes, kDims);
+            umma_commit(&sh.dp_full);
+          }
+          __syncwarp();
+        };
+        me.wait(&sh.own_full, 0);
+        bool more = me.ok && ready(0);
+        if (more) {
+          scores(0);
+          values(0);
+        }
+        for (int n = 0; more && me.ok; ++n) {
+          if (!me.wait(&sh.p_full, n)) break;
+          if (issuer) product_rows(dv_at, s_at, q_of(n) + kTileBytes, kRows, n > 0);
+          __syncwarp();
+          more = ready(n + 1);
+          if (more) scores(n + 1);
+          if (!me.wait(&sh.ds_full[0], n)) break;
+          if (issuer) {
+            product_rows(dk_at, dp_at, q_of(n), kRows, n > 0);
+            umma_commit(&sh.rows_empty[n & 1]);
+            if (!more) umma_commit(&sh.done);
+          }
+          __syncwarp();
+          if (more) values(n + 1);
+        }
+      }
+    } else {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+      // -------------------------------------------------------------- probabilities; a key a thread
+      const int j = j0 + r;
+      const Cap cap(a.s);
+      const float at_key = static_cast<float>(j);
+      const uint32_t s_own = s_at + lanes + half * 64, dp_own = dp_at + lanes + half * 64;
+      int n = 0;
+      for (; any; ++n) {
+        const Step& step = sh.step[n & 1];
+        if (!me.wait(&sh.step_full[n & 1], n >> 1) || step.end) break;
+        if (!me.wait(&sh.s_full[0], n)) break;
+        const int c0 = half * 64;
+        float p[64], slopes[RICH ? 64 : 1];
+        load_half(s_own, p);
+        if constexpr (RICH) {
+          const float bias = a.s.slopes ? a.s.slopes[step.head] * kLog2E : 0.0f;
+#pragma unroll
+          for (int e = 0; e < 64; ++e) {
+            slopes[e] = 1.0f;
+            if (a.s.cap > 0.0f) {
+              const float rc = cap.recip(p[e]);
+              slopes[e] = cap.slope(rc);
+              p[e] = cap.value(rc);
+            } else {
+              p[e] *= scale_log2;
+            }
+            if (a.s.slopes) p[e] = fmaf(-bias, fabsf(step.pos[c0 + e] - at_key), p[e]);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 64; e += 4) {
+          const float4 l = *reinterpret_cast<const float4*>(step.lse + c0 + e);
+          if constexpr (RICH) {
+            p[e] -= l.x;
+            p[e + 1] -= l.y;
+            p[e + 2] -= l.z;
+            p[e + 3] -= l.w;
+          } else {
+            const float2 sc = make_float2(scale_log2, scale_log2);
+            const float2 x = ffma2(make_float2(p[e], p[e + 1]), sc, make_float2(-l.x, -l.y));
+            const float2 y = ffma2(make_float2(p[e + 2], p[e + 3]), sc, make_float2(-l.z, -l.w));
+            p[e] = x.x;
+            p[e + 1] = x.y;
+            p[e + 2] = y.x;
+            p[e + 3] = y.y;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 64; ++e) p[e] = exp2_approx(p[e]);
+        const bool masked = step.masked;
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 64; e += 4) {
+            const int4 lo = *reinterpret_cast<const int4*>(step.lo + c0 + e), hi = *reinterpret_cast<const int4*>(step.hi + c0 + e);
+            p[e] = j >= lo.x && j < hi.x ? p[e] : 0.0f;
+            p[e + 1] = j >= lo.y && j < hi.y ? p[e + 1] : 0.0f;
+            p[e + 2] = j >= lo.z && j < hi.z ? p[e + 2] : 0.0f;
+            p[e + 3] = j >= lo.w && j < hi.w ? p[e + 3] : 0.0f;
+          }
+        }
+        store_half<T>(s_own, p);
+        me.arrive(&sh.p_full);
+        if (!me.wait(&sh.dp_full, n)) break;
+        float ds[64];
+        load_half(dp_own, ds);
+#pragma unroll
+        for (int e = 0; e < 64; e += 4) {
+          const float4 l = *reinterpret_cast<const float4*>(step.delta + c0 + e);
+          const float2 back = make_float2(Held<AB>::kBack, Held<AB>::kBack);
+          const float2 x = ffma2(make_float2(ds[e], ds[e + 1]), back, make_float2(-l.x, -l.y));
+          const float2 y = ffma2(make_float2(ds[e + 2], ds[e + 3]), back, make_float2(-l.z, -l.w));
+          ds[e] = p[e] * x.x;
+          ds[e + 1] = p[e + 1] * x.y;
+          ds[e + 2] = p[e + 2] * y.x;
+          ds[e + 3] = p[e + 3] * y.y;
+        }
+        if constexpr (RICH) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e) ds[e] *= slopes[e];
+        }
+        if (masked) {  // a masked pair's g.v may be anything
+#pragma unroll
+          for (int e = 0; e < 64; ++e) ds[e] = p[e] == 0.0f ? 0.0f : ds[e];
+        }
+        store_half<T>(dp_own, ds);
+        me.arrive(&sh.ds_full[0]);
+      }
+      if (any) me.wait(&sh.done, 0);
+      if (me.ok) {  // the first warps store dv, the others dk
+        T* out = nullptr;
+        if (j < a.s.sk) {
+          if (half == 0 && a.dv) out = static_cast<T*>(a.dv) + b * a.v_batch + kv * a.v_head + static_cast<long long>(j) * a.v_row;
+          if (half == 1 && a.dk) out = static_cast<T*>(a.dk) + b * a.k_batch + kv * a.k_head + static_cast<long long>(j) * a.k_row;
+        }
+        store_row<T, D>(out, (half ? dk_at : dv_at) + lanes, half ? a.s.scale : Held<AB>::kBack, a.s.d, any);
+      }
+    }
+  } else {
+    // ================================================================ dq of 128 query rows
+    const int tiles = row_tiles(a.s), unit = static_cast<int>(blockIdx.x) - a.key_units;
+    const int tile = tiles - 1 - unit % tiles, head = unit / tiles % a.s.heads, b = unit / tiles / a.s.heads;
+    const int i0 = tile * kTile, kv = head / group;
+    const int4 seen = tile_span(a.s, b, tile);
+    const int key0 = max(seen.x, 0), key_end = min(seen.y, a.s.sk);
+    const int ntiles = key_end > key0 ? (key_end - key0 + kTile - 1) / kTile : 0;
+    const uint32_t dp_at = tmem + 2 * kTile, dq_at = tmem + 3 * kTile;
+    if (warp >= 8) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+      if (ntiles > 0 && warp == 8) {
+        // ------------------------------------------------------------ TMA
+        const bool issuer = elect_one();
+        if (issuer) {
+          mbar_arrive_expect_tx(&sh.own_full, 2 * kTileBytes);
+          load_rows<kPanels>(base, &qmap, i0, head, b, &sh.own_full);
+          load_rows<kPanels>(base + kTileBytes, &gmap, i0, head, b, &sh.own_full);
+        }
+        __syncwarp();
+        for (int item = 0; item < 2 * ntiles && me.ok; ++item) {
+          const int sl = item % kKeySlots, use = item / kKeySlots;
+          if (use > 0 && !me.wait(&sh.slot_empty[sl], use - 1)) break;
+          if (issuer) {
+            mbar_arrive_expect_tx(&sh.slot_full[sl], kTileBytes);
+            load_rows<kPanels>(ring + sl * kTileBytes, item & 1 ? &vmap : &kmap, key0 + (item >> 1) * kTile, kv, b, &sh.slot_full[sl]);
+          }
+          __syncwarp();
+        }
+        me.land();
+      } else if (ntiles > 0 && warp == 9) {
+        // ------------------------------------------------------------ MMA
+        const bool issuer = elect_one();
+        const uint32_t q = smem_u32(base), g = q + kTileBytes;
+        auto slot_of = [&](int item) { return smem_u32(ring + item % kKeySlots * kTileBytes); };
+        auto wait_slot = [&](int item) { return me.wait(&sh.slot_full[item % kKeySlots], item / kKeySlots); };
+        auto scores = [&](int t) {
+          if (!wait_slot(2 * t)) return;
+          const int left = key_end - (key0 + t * kTile);  // keys past these are nobody's and may hold anything
+          if (left < kTile) clear_rows<kPanels>(ring + 2 * t % kKeySlots * kTileBytes, left, kTile, lane);
+          if (issuer) {
+            product_dims<D>(tmem + (t & 1) * kTile, q, slot_of(2 * t), kDims);
+            umma_commit(&sh.s_full[t & 1]);
+          }
+          __syncwarp();
+        };
+        auto values = [&](int t) {
+          if (!wait_slot(2 * t + 1)) return;
+          if (issuer) {
+            product_dims<D>(dp_at, g, slot_of(2 * t + 1), kDims);
+            umma_commit(&sh.dp_full);
+            umma_commit(&sh.slot_empty[(2 * t + 1) % kKeySlots]);
+          }
+          __syncwarp();
+        };
+        me.wait(&sh.own_full, 0);
+        if (me.ok) scores(0);
+        if (me.ok) values(0);
+        for (int t = 0; t < ntiles && me.ok; ++t) {
+          if (t + 1 < ntiles) {
+            if (t > 0 && !me.wait(&sh.slot_empty[2 * (t - 1) % kKeySlots], (t - 1) / 2)) break;
+            scores(t + 1);
+            if (me.wait(&sh.dp_free, t)) values(t + 1);
+          }
+          if (!me.wait(&sh.ds_full[t & 1], t >> 1)) break;
+          if (issuer) {
+            product_rows(dq_at, tmem + (t & 1) * kTile, slot_of(2 * t), kRows, t > 0);
+            umma_commit(&sh.slot_empty[2 * t % kKeySlots]);
+            if (t == ntiles - 1) umma_commit(&sh.done);
+          }
+          __syncwarp();
+        }
+      }
+    } else {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+      // -------------------------------------------------------------- a query row a thread, 64 of the keys
+      const int i = i0 + r;
+      const bool real = i < a.s.sq;
+      const int4 span = real ? span_of(a.s, b, i) : make_int4(0, 0, 0, 0);
+      const float2 stat = a.stats[(static_cast<long long>(b) * a.s.heads + head) * a.padded + i];
+      const Cap cap(a.s);
+      const float bias = RICH && a.s.slopes ? a.s.slopes[head] * kLog2E : 0.0f;
+      const float2 neg2 = make_float2(-stat.x, -stat.x), scale2 = make_float2(scale_log2, scale_log2);
+      const float2 back = make_float2(Held<AB>::kBack, Held<AB>::kBack), delta2 = make_float2(-stat.y, -stat.y);
+      for (int t = 0; t < ntiles; ++t) {
+        const uint32_t s_own = tmem + (t & 1) * kTile + lanes + half * 64;
+        if (!me.wait(&sh.s_full[t & 1], t >> 1)) break;
+        const int j0 = key0 + t * kTile + half * 64;
+        float p[64], slopes[RICH ? 64 : 1];
+        load_half(s_own, p);
+        if constexpr (RICH) {
+          const float apart = static_cast<float>(span.z - j0);
+#pragma unroll
+          for (int e = 0; e < 64; ++e) {
+            slopes[e] = 1.0f;
+            if (a.s.cap > 0.0f) {
+              const float rc = cap.recip(p[e]);
+              slopes[e] = cap.slope(rc);
+              p[e] = cap.value(rc);
+            } else {
+              p[e] *= scale_log2;
+            }
+            if (a.s.slopes) p[e] = fmaf(-bias, fabsf(apart - static_cast<float>(e)), p[e]);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 64; e += 2) {
+          const float2 z = make_float2(p[e], p[e + 1]);
+          const float2 x = RICH ? fadd2(z, neg2) : ffma2(z, scale2, neg2);
+          p[e] = exp2_approx(x.x);
+          p[e + 1] = exp2_approx(x.y);
+        }
+        const bool masked = !__all_sync(0xffffffffu, !real || (span.x <= j0 && span.y >= j0 + 64));
+        const int from = span.x - j0, to = span.y - j0;
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e) p[e] = e >= from && e < to ? p[e] : 0.0f;
+        }
+        if (!me.wait(&sh.dp_full, t)) break;
+        float ds[64];
+        load_half(dp_at + lanes + half * 64, ds);
+        me.arrive(&sh.dp_free);
+#pragma unroll
+        for (int e = 0; e < 64; e += 2) {
+          const float2 x = fmul2(make_float2(p[e], p[e + 1]), ffma2(make_float2(ds[e], ds[e + 1]), back, delta2));
+          ds[e] = x.x;
+          ds[e + 1] = x.y;
+        }
+        if constexpr (RICH) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e) ds[e] *= slopes[e];
+        }
+        if (masked) {  // a masked pair's g.v may be anything
+#pragma unroll
+          for (int e = 0; e < 64; ++e) ds[e] = e >= from && e < to ? ds[e] : 0.0f;
+        }
+        store_half<T>(s_own, ds);
+        me.arrive(&sh.ds_full[t & 1]);  // two barriers: a fast warp may be through the next step before a slow one is here
+      }
+      if (ntiles > 0) me.wait(&sh.done, 0);
+      if (me.ok && half == 0) {
+        // (a row that sees nothing: its g may hold anything)
+        T* out = real ? static_cast<T*>(a.dq) + b * a.q_batch + head * a.q_head + static_cast<long long>(i) * a.q_row : nullptr;
+        store_row<T, D>(out, dq_at + lanes, a.s.scale, a.s.d, ntiles > 0);
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---- host ---------------------------------------------------------------------------------
+long long padded_rows(int sq) { return round_up(sq, kTile); }
+
+template <int AB, int D>
+int launch_grad(const GradArgs& a, const CUtensorMap (&maps)[4], cudaStream_t stream) {
+  const bool rich = a.s.cap > 0.0f || a.s.slopes;
+  auto kernel = rich ? span_attention_grad_kernel<AB, D, true> : span_attention_grad_kernel<AB, D, false>;
+  static std::atomic<unsigned long long> granted[2] = {};
+  if (cudaError_t e = grant_smem(reinterpret_cast<const void*>(kernel), grad_smem<D>(), granted[rich])) return static_cast<int>(e);
+  if (a.s.sq > 0) {
+    const long long rows = static_cast<long long>(a.s.batch) * a.s.heads * a.padded;
+    if (int st = launch_overlapped(grad_stats_kernel<AB>, dim3(static_cast<unsigned>((rows + 15) / 16)), dim3(256), 0, 0, stream, a)) return st;
+  }
+  return launch_overlapped(kernel, dim3(a.key_units + a.query_units), dim3(kGradThreads), grad_smem<D>(), 0, stream, maps[0],
+                           maps[1], maps[2], maps[3], a);
+}
+
+}  // namespace
+}  // namespace peco
+
+using namespace peco;
+
+extern "C" long long peco_span_attention_backward_workspace(int batch, int heads, int sq) {
+  if (batch < 0 || heads < 1 || sq < 0 || sq > 0x7ffffe00) return -1;
+  return 8LL * batch * heads * padded_rows(sq);
+}
+
+extern "C" int peco_span_attention_backward(const void* grad, const void* q, const void* k, const void* v, const void* out,
+                                            const float* lse, const long long* strides, const int* span_rows,
+                                            const int* span_tiles, int spans_batched, const float* slopes, float scale,
+                                            float cap, void* dq, void* dk, void* dv, int batch, int heads, int kv_heads,
+                                            int sq, int sk, int d, int dtype, void* workspace, long long workspace_bytes,
+                                            void* stream_ptr) {
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  if (dtype != 0 && dtype != 1) return kErrUnsupported;
+  if (batch < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || sq < 0 || sk < 0 || sq > 0x7ffffe00 || sk > 0x7ffffe00 ||
+      d < 8 || d > 128 || d % 8 || !(scale > 0.0f) || !(cap >= 0.0f) || !strides)
+    return kErrInvalidValue;
+  const bool keys = (dk || dv) && batch > 0 && sk > 0, rows = dq && batch > 0 && sq > 0;
+  if (!keys && !rows) return kOk;
+  if ((span_rows == nullptr) != (span_tiles == nullptr)) return kErrInvalidValue;
+  HeadRows t[8];  // grad, q, k, v, out, dq, dk, dv
+  const void* at[8] = {grad, q, k, v, out, dq, dk, dv};
+  for (int i = 0; i < 8; ++i) {
+    const bool of_keys = i == 2 || i == 3 || i == 6 || i == 7;
+    t[i] = HeadRows{at[i], strides[3 * i], strides[3 * i + 1], strides[3 * i + 2]};
+    const int n = of_keys ? sk : sq;
+    if (n == 0 || (i > 4 && !at[i])) continue;
+    if (!readable(t[i], batch, of_keys ? kv_heads : heads, n)) return kErrInvalidValue;
+  }
+  if (sq > 0 && !lse) return kErrInvalidValue;
+  if (sq > 0 && !usable_workspace(workspace, workspace_bytes, peco_span_attention_backward_workspace(batch, heads, sq))) return kErrWorkspace;
+  GradArgs a{};
+  a.s.spans = reinterpret_cast<const int4*>(span_rows);
+  a.s.span_tiles = reinterpret_cast<const int4*>(span_tiles);
+  a.s.spans_batched = spans_batched;
+  a.s.slopes = slopes;
+  a.s.batch = batch;
+  a.s.heads = heads;
+  a.s.kv_heads = kv_heads;
+  a.s.sq = sq;
+  a.s.sk = sk;
+  a.s.d = d;
+  a.s.scale = scale;
+  a.s.cap = cap;
+  a.s.status = device_status_ptr();
+  a.grad = t[0];
+  a.out = t[4];
+  a.lse = lse;
+  a.stats = static_cast<float2*>(workspace);
+  a.padded = static_cast<int>(padded_rows(sq));
+  a.dq = dq;
+  a.dk = dk;
+  a.dv = dv;
+  a.q_batch = t[5].batch;
+  a.q_head = t[5].head;
+  a.q_row = t[5].row;
+  a.k_batch = t[6].batch;
+  a.k_head = t[6].head;
+  a.k_row = t[6].row;
+  a.v_batch = t[7].batch;
+  a.v_head = t[7].head;
+  a.v_row = t[7].row;
+  const long long key_units = keys ? static_cast<long long>(batch) * kv_heads * ((sk + kTile - 1) / kTile) : 0;
+  const long long query_units = rows ? static_cast<long long>(batch) * heads * (a.padded / kTile) : 0;
+  const long long stat_blocks = (static_cast<long long>(batch) * heads * a.padded + 15) / 16;
+  if (key_units + query_units > 0x7fffffffLL || stat_blocks > 0x7fffffffLL) return kErrUnsupported;
+  a.key_units = static_cast<int>(key_units);
+  a.query_units = static_cast<int>(query_units);
+  // an empty side is never loaded: its maps stand on the other's rows
+  CUtensorMap maps[4];
+  const int order[4] = {1, 2, 3, 0};
+  for (int i = 0; i < 4; ++i) {
+    const bool of_keys = i == 1 || i == 2;
+    const bool empty = of_keys ? sk == 0 : sq == 0;
+    const HeadRows& from = !empty ? t[order[i]] : sk == 0 ? t[1] : t[2];
+    const bool as_keys = empty ? sk != 0 : of_keys;
+    // whole tiles: rows past the end read as zeros, as the products over rows need them
+    if (!head_map(&maps[i], from, batch, as_keys ? kv_heads : heads, as_keys ? sk : sq, d, kTile, 1, dtype)) return kErrTensorMap;
+  }
+  if (d <= 64) return dtype == 1 ? launch_grad<1, 64>(a, maps, stream) : launch_grad<0, 64>(a, maps, stream);
+  return dtype == 1 ? launch_grad<1, 128>(a, maps, stream) : launch_grad<0, 128>(a, maps, stream);
+}
