@@ -350,18 +350,6 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t base) {
   return MN ? smem_desc(base, 8192, 1024) : smem_desc(base, 16, 1024);
 }
 
-// Position in the ring: stage and the phase of its barriers.
-struct RingPos {
-  int s;
-  uint32_t phase;
-  __device__ __forceinline__ void step(int stages) {
-    if (++s == stages) {
-      s = 0;
-      phase ^= 1;
-    }
-  }
-};
-
 template <typename T, bool EPI>
 __device__ __forceinline__ const T* gate_row(const GemmArgs& args, long long row) {
   if (!EPI || !args.gate || row >= args.m) return nullptr;

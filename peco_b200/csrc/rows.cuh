@@ -62,6 +62,18 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t phase, volatil
   return mbar_wait_warp(bar, phase, abort_flag, status);
 }
 
+// Position in the ring: stage and the phase of its barriers.
+struct RingPos {
+  int s;
+  uint32_t phase;
+  __device__ __forceinline__ void step(int stages) {
+    if (++s == stages) {
+      s = 0;
+      phase ^= 1;
+    }
+  }
+};
+
 // A caller's workspace: large enough, and on the 16 bytes that vector stores and TMA start on.
 inline bool usable_workspace(const void* workspace, long long bytes, long long need) {
   return workspace && bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0;

@@ -14,8 +14,16 @@
 //   P = 2^(z - m)    four warps, a query row a thread; m, the running maximum, is
 //                    raised only when it grows by more than 2^8, and O rescaled
 //   O += P V         tcgen05.mma, P from TMEM (over S, as 16-bit pairs)
-// While one tile's softmax runs, the tensor core works on the other's products.
-// K and V stream through five shared-memory slots by TMA.
+// While one tile's softmax runs, the tensor core works on the other's products.  A
+// tile's next S overwrites the P that O's product before it reads: products that
+// one thread issues are executed in the order of their issue.  K and V stream
+// through five shared-memory slots by TMA.
+//
+// What it measured (B200, bf16): 24 heads x 7006 rows x 128 dims, every key: 565 us
+// (1.02 PFLOP/s of the visible pairs; 606 us at the power limit after 300 calls in a
+// row); 64 dims 480 us; causal, 24 query heads on 4, 4096 rows 151 us.  Bound by the round trip
+// of a tile: 1500 clocks of softmax and 1000 of products, 1670 a tile with two in
+// flight (without the softmax 375 us, without the products 405).
 #include "span_attention.cuh"
 #include "../../include/peco_b200.h"
 #include "internal.h"
@@ -300,52 +308,52 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------------------------------------------------------- MMA
     constexpr uint32_t idesc_qk = instr_desc(kTile, kTile, AB, false, false);
     constexpr uint32_t idesc_pv = instr_desc(kTile, D, AB, false, true);
+    constexpr uint32_t kSlotStep = kTileBytes >> 4;
     const bool issuer = elect_one();
+    const uint32_t s_at = uniform(tmem), o_at = s_at + 2 * kTile;
+    const uint32_t q = uniform(desc_dims(smem_u32(base))), k = uniform(desc_dims(smem_u32(slots)));
+    const uint32_t v = uniform(desc_rows(smem_u32(slots)));
+    const int last = static_cast<int>(uniform(ntiles)) - 1, both = static_cast<int>(uniform(tiles)) - 1;
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t phase) {
       if (ok) ok = warp_wait(bar, phase, abort_flag, a.s.status);
       if (ok) tc_fence_after();
       return ok;
     };
-    auto wait_slot = [&](int item) { return wait(&sh.slot_full[item % kSlots], (item / kSlots) & 1); };
-    auto scores = [&](int w, int t) {
+    auto scores = [&](int w, int slot) {
       if (issuer) {
-        const uint32_t q = smem_u32(base + w * kTileBytes), k = smem_u32(slots + 2 * t % kSlots * kTileBytes);
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) umma_ss(tmem + w * kTile, desc_dims(q, i), desc_dims(k, i), idesc_qk, i > 0);
+        product_dims<D>(s_at + w * kTile, q + w * kSlotStep, k + slot * kSlotStep, idesc_qk);
         umma_commit(&sh.s_full[w]);
+        if (w == both) umma_commit(&sh.slot_empty[slot]);
       }
       __syncwarp();
     };
-    if (ntiles > 0) {
+    if (last >= 0) {
+      RingPos pos{0, 0};  // of the next slot to wait for
       wait(&sh.q_full, 0);
-      wait_slot(0);
-      for (int w = 0; w < tiles && ok; ++w) scores(w, 0);
-      if (ok && issuer) umma_commit(&sh.slot_empty[0]);
-      __syncwarp();
-      for (int t = 0; t < ntiles && ok; ++t) {
-        const int item = 2 * t + 1, s = item % kSlots;
-        if (!wait_slot(item)) break;
+      if (wait(&sh.slot_full[0], 0)) {
+        scores(0, 0);
+        if (both) scores(1, 0);
+      }
+      pos.step(kSlots);
+      for (int t = 0; t <= last && ok; ++t) {
+        const int vs = pos.s;
+        if (!wait(&sh.slot_full[vs], pos.phase)) break;
+        pos.step(kSlots);
         const int seen = all_keys.y - (key0 + t * kTile);  // keys past these are nobody's: their values may be anything
-        if (seen < kTile) clear_rows<kPanels>(slots + s * kTileBytes, seen, kTile, lane);
-        for (int w = 0; w < tiles; ++w) {
+        if (seen < kTile) clear_rows<kPanels>(slots + vs * kTileBytes, seen, kTile, lane);
+        if (t < last && !wait(&sh.slot_full[pos.s], pos.phase)) break;
+        for (int w = 0; w <= both; ++w) {
           if (!wait(&sh.p_full[w], t & 1)) break;
           if (issuer) {
-            const uint32_t v = smem_u32(slots + s * kTileBytes);
-#pragma unroll
-            for (int i = 0; i < kTile / 16; ++i)
-              umma_ts(tmem + 2 * kTile + w * kTile, tmem + w * kTile + i * 8, desc_rows(v, i), idesc_pv, t > 0 || i > 0);
-            if (w == tiles - 1) umma_commit(&sh.slot_empty[s]);
-            if (t == ntiles - 1) umma_commit(&sh.o_full[w]);
+            product_rows<kTile>(o_at + w * kTile, s_at + w * kTile, v + vs * kSlotStep, idesc_pv, t > 0);
+            if (w == both) umma_commit(&sh.slot_empty[vs]);
+            if (t == last) umma_commit(&sh.o_full[w]);
           }
           __syncwarp();
-          if (t + 1 < ntiles) {
-            if (w == 0 && !wait_slot(2 * t + 2)) break;
-            scores(w, t + 1);
-            if (w == tiles - 1 && issuer) umma_commit(&sh.slot_empty[(2 * t + 2) % kSlots]);
-            __syncwarp();
-          }
+          if (t < last) scores(w, pos.s);
         }
+        if (t < last) pos.step(kSlots);
       }
     }
   }
@@ -371,12 +379,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const int j0 = key0 + t * kTile;
       float s[kTile];
+      {
+        uint32_t raw[kTile];
+        tmem_ld128_sync(s_at, raw);
 #pragma unroll
-      for (int c = 0; c < kTile / 32; ++c) {
-        uint32_t raw[32];
-        tmem_ld32_sync(s_at + c * 32, raw);
-#pragma unroll
-        for (int e = 0; e < 32; ++e) s[c * 32 + e] = __uint_as_float(raw[e]);
+        for (int e = 0; e < kTile; ++e) s[e] = __uint_as_float(raw[e]);
       }
       if constexpr (RICH) {  // to log2 units
         if (a.s.cap > 0.0f) {
@@ -442,11 +449,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 0; e < 32; e += 2) {
           const float2 z = make_float2(s[c * 32 + e], s[c * 32 + e + 1]);
           const float2 x = RICH ? fadd2(z, neg2) : ffma2(z, scale2, neg2);
-          const float2 p = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+          const float2 p = exp2_pair(e >> 1, x);
           sums[(e >> 1) & 3] = fadd2(sums[(e >> 1) & 3], p);
           packed[e >> 1] = pack2<T>(p.x, p.y);
         }
-        tmem_st16(s_at + c * 16, packed);
+        tmem_st16(s_at + (c >> 1) * 64 + (c & 1) * 16, packed);
       }
       const float2 sum = fadd2(fadd2(sums[0], sums[1]), fadd2(sums[2], sums[3]));
       l += sum.x + sum.y;

@@ -63,6 +63,60 @@ struct Cap {
   __device__ __forceinline__ float slope(float r) const { return 4.0f * r * (1.0f - r); }
 };
 
+// 128 columns of a TMEM lane: four loads in flight, one wait.
+__device__ __forceinline__ void tmem_ld128_sync(uint32_t at, uint32_t (&r)[128]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%128];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%129];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, %80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95}, [%130];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, %112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127}, [%131];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
+        "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
+        "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
+        "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
+        "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
+        "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
+        "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
+        "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
+        "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+      : "r"(at), "r"(at + 32), "r"(at + 64), "r"(at + 96)
+      : "memory");
+}
+
+// 2^x of a pair on the fused multiply-add pipe, which has time left where the
+// special-function unit (16 a clock and SM) has not: x = n + f with n its nearest
+// integer, 2^f by a polynomial (own fit on |f| <= 1/2: relative error 2^-23.5, 2^-22.5 as
+// evaluated, as good as the unit's), times 2^n.  x up to 127; below -126.5 it is
+// 0, a NaN stays.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  auto both = [](float v) { return make_float2(v, v); };
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));  // -127
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
+  const float2 t = fadd2(x, both(12582912.0f));         // n in the low bits
+  const float2 n = fadd2(t, both(-12582912.0f));
+  const float2 f = ffma2(n, both(-1.0f), x);
+  float2 p = ffma2(f, both(0.001327398233115673f), both(0.009671970270574093f));
+  p = ffma2(f, p, both(0.05550680309534073f));
+  p = ffma2(f, p, both(0.24022234976291656f));
+  p = ffma2(f, p, both(0.6931470632553101f));
+  p = ffma2(f, p, both(1.0f));
+  return fmul2(p, make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
+                              __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u)));
+}
+// A pair of a run of pairs: of every eight, ``kPolyPairs`` by the polynomial.
+constexpr int kPolyPairs = 1;
+__device__ __forceinline__ float2 exp2_pair(int pair, float2 x) {  // ``pair`` known when compiled
+  return (pair & 7) * kPolyPairs % 8 < kPolyPairs ? exp2_poly(x) : make_float2(exp2_approx(x.x), exp2_approx(x.y));
+}
+
 __device__ __forceinline__ void tile_load_4d(void* dst, const CUtensorMap* map, int x, int row, int head, int batch,
                                              uint64_t* bar) {
   asm volatile(
@@ -91,13 +145,40 @@ __device__ __forceinline__ void clear_rows(unsigned char* tile, int from, int to
   __syncwarp();
 }
 
-// Descriptors of a tile's 16-wide steps along the dimensions (K-major) and along the rows (MN-major).
-__device__ __forceinline__ uint64_t desc_dims(uint32_t tile, int step) {
-  return smem_desc(tile + (step >> 2) * kPanelBytes + (step & 3) * 32, 16, 1024);
+// A tile's descriptor for steps of 16 along the dimensions (K-major) or along the
+// rows (MN-major): the low word, to which a step adds a constant; the high word is
+// the same for all.  The issuing warp runs whole with one elected lane issuing, and
+// takes what it computes from warp-uniform values, so that descriptors stay in
+// uniform registers: moving each there first made issuing a step slower than the
+// tensor core.
+__device__ __forceinline__ uint32_t desc_dims(uint32_t tile) { return ((tile >> 4) & 0x3fffu) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_rows(uint32_t tile) {
+  return ((tile >> 4) & 0x3fffu) | (static_cast<uint32_t>(kPanelBytes >> 4) << 16);
 }
-__device__ __forceinline__ uint64_t desc_rows(uint32_t tile, int step) {
-  return smem_desc(tile + step * 2048, kPanelBytes, 1024);
+__host__ __device__ constexpr uint32_t dims_step(int i) { return (i >> 2) * (kPanelBytes >> 4) + (i & 3) * 2; }
+__host__ __device__ constexpr uint32_t rows_step(int i) { return i * 128; }
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);  // 8 rows 1024 bytes apart, sm_100 form, 128-byte swizzle
+
+__device__ __forceinline__ uint64_t whole_desc(uint32_t low) { return (static_cast<uint64_t>(kDescHigh) << 32) | low; }
+
+// to = X Y^T over D dimensions
+template <int D>
+__device__ __forceinline__ void product_dims(uint32_t to, uint32_t x, uint32_t y, uint32_t idesc) {
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+    umma_ss(to, whole_desc(x + dims_step(i)), whole_desc(y + dims_step(i)), idesc, i > 0);
 }
+// to (+)= A Y over ``ROWS`` rows of a tile, A 16-bit pairs in TMEM, each run of 64 rows
+// 64 columns after the one before
+template <int ROWS>
+__device__ __forceinline__ void product_rows(uint32_t to, uint32_t a, uint32_t y, uint32_t idesc, uint32_t accumulate) {
+#pragma unroll
+  for (int i = 0; i < ROWS / 16; ++i)
+    umma_ts(to, a + (i >> 2) * 64 + (i & 3) * 8, whole_desc(y + rows_step(i)), idesc, i > 0 ? 1u : accumulate);
+}
+
+// A value that all lanes hold, as the compiler can see
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 template <int AB>
 using Element = typename std::conditional<AB == 1, __nv_bfloat16, __half>::type;

@@ -16,8 +16,12 @@
 namespace peco {
 namespace {
 
-constexpr int kGradThreads = 384;  // eight softmax warps, then TMA, MMA and statistics warps
-constexpr int kKeySlots = 4;       // of K(t) and V(t) under a query tile
+constexpr int kGradThreads = 384;  // eight softmax warps, then TMA, MMA, MMA and statistics warps
+// Tiles that stream past a CTA's own two: of Q (under a tile of keys) or K (under a
+// tile of rows), used by its step's first and last product, and of g or V.
+constexpr int kSecond = 2;
+template <bool RICH>
+constexpr int kFirst = RICH ? 2 : 3;  // (capped or biased scores keep the rows' positions there)
 
 struct GradArgs {
   ScoreArgs s;
@@ -65,25 +69,33 @@ __global__ void __launch_bounds__(256) grad_stats_kernel(const __grid_constant__
 }
 
 // One step of a CTA of keys: a query tile of one head, as the statistics warp lays it out.
+template <bool RICH>
 struct Step {
-  float lse[kTile], delta[kTile], pos[kTile];
-  int lo[kTile], hi[kTile];
+  float lse[kTile], delta[kTile];
+  uint32_t range[kTile / 2];  // bytes: first key of the tile that a row sees, and the key behind the last
+  float pos[RICH ? kTile : 4];
   int masked, clear, end, head;
 };
 
+template <bool RICH>
 struct __align__(16) GradShared {
-  Step step[2];
-  uint64_t own_full;                                 // the CTA's own two tiles
-  uint64_t rows_full[2], step_full[2], rows_empty[2];  // CTAs of keys: stages of query rows
-  uint64_t slot_full[kKeySlots], slot_empty[kKeySlots];  // CTAs of query rows: K and V
-  uint64_t s_full[2], p_full, dp_full, dp_free, ds_full[2], done;
+  Step<RICH> step[2];
+  uint64_t own_full;                              // the CTA's own two tiles
+  uint64_t first_full[3], first_empty[3], second_full[2], second_empty[2], step_full[2], step_empty[2];
+  uint64_t s_full[2], p_full, dp_full, dp_free, ds_full[2], dq_done[2], done;
   uint32_t tmem;
   int first, last, abort_flag;
 };
 
-template <int D>
-constexpr int grad_smem() { return 1024 + (2 + kKeySlots) * kTile * D * 2 + 16; }
-static_assert(grad_smem<128>() + sizeof(GradShared) <= 227 * 1024, "shared memory of a CTA");
+template <int D, bool RICH>
+constexpr int tiles_bytes() { return (2 + kFirst<RICH> + kSecond) * kTile * D * 2; }
+template <int D, bool RICH>
+constexpr int grad_smem() {
+  constexpr int need = tiles_bytes<D, RICH>() + static_cast<int>(sizeof(GradShared<RICH>));
+  return need + 1024 < 227 * 1024 ? need + 1024 : 227 * 1024;  // room to start on 1024 bytes
+}
+static_assert(tiles_bytes<128, false>() + sizeof(GradShared<false>) <= 227 * 1024 &&
+                  tiles_bytes<128, true>() + sizeof(GradShared<true>) <= 226 * 1024, "shared memory of a CTA");
 
 struct Roles {
   int warp, lane;
@@ -107,18 +119,6 @@ struct Roles {
     }
   }
 };
-
-// A 128 x 16n product from two tiles along the dimensions: X Y^T
-template <int D>
-__device__ __forceinline__ void product_dims(uint32_t to, uint32_t x, uint32_t y, uint32_t idesc) {
-#pragma unroll
-  for (int i = 0; i < D / 16; ++i) umma_ss(to, desc_dims(x, i), desc_dims(y, i), idesc, i > 0);
-}
-// to (+)= A Y over Y's rows, A 16-bit pairs in TMEM, each half of 64 over the half of the scores it came from
-__device__ __forceinline__ void product_rows(uint32_t to, uint32_t a, uint32_t y, uint32_t idesc, bool accumulate) {
-#pragma unroll
-  for (int i = 0; i < kTile / 16; ++i) umma_ts(to, a + (i >> 2) * 64 + (i & 3) * 8, desc_rows(y, i), idesc, accumulate || i > 0);
-}
 
 // 64 columns of TMEM as fp32
 __device__ __forceinline__ void load_half(uint32_t at, float (&v)[64]) {
@@ -188,24 +188,34 @@ __global__ void __launch_bounds__(kGradThreads, 1)
   using T = Element<AB>;
   constexpr int kPanels = D / 64, kTileBytes = kPanels * kPanelBytes;
   constexpr uint32_t kDims = instr_desc(kTile, kTile, AB, false, false), kRows = instr_desc(kTile, D, AB, false, true);
+  constexpr int kFirsts = kFirst<RICH>;
+  constexpr uint32_t kTileStep = kTileBytes >> 4;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  __shared__ GradShared sh;
   unsigned char* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  unsigned char* ring = base + 2 * kTileBytes;
+  unsigned char* firsts = base + 2 * kTileBytes;
+  unsigned char* seconds = firsts + kFirsts * kTileBytes;
+  GradShared<RICH>& sh = *reinterpret_cast<GradShared<RICH>*>(base + tiles_bytes<D, RICH>());
+  if (base - smem_raw + tiles_bytes<D, RICH>() + static_cast<int>(sizeof(sh)) > grad_smem<D, RICH>()) {
+    record_status(a.s.status, kDevBadIndex);  // (dynamic shared memory starts on 1024 bytes where nothing else is in front)
+    return;
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   Roles me{warp, lane, true, &sh.abort_flag, a.s.status};
+  const bool of_keys = static_cast<int>(blockIdx.x) < a.key_units;
   if (threadIdx.x == 0) {
     mbar_init(&sh.own_full, 1);
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(&sh.first_full[i], 1);
+      mbar_init(&sh.first_empty[i], 1);
+    }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&sh.rows_full[i], 1);
+      mbar_init(&sh.second_full[i], 1);
+      mbar_init(&sh.second_empty[i], 1);
       mbar_init(&sh.step_full[i], 1);
-      mbar_init(&sh.rows_empty[i], 1);
+      mbar_init(&sh.step_empty[i], 1);
+      mbar_init(&sh.dq_done[i], 1);
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.ds_full[i], 8);
-    }
-    for (int i = 0; i < kKeySlots; ++i) {
-      mbar_init(&sh.slot_full[i], 1);
-      mbar_init(&sh.slot_empty[i], 1);
     }
     mbar_init(&sh.p_full, 8);
     mbar_init(&sh.dp_full, 1);
@@ -238,7 +248,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
   const int r = (warp & 3) * 32 + lane;
   const float scale_log2 = a.s.scale * kLog2E;
 
-  if (static_cast<int>(blockIdx.x) < a.key_units) {
+  if (of_keys) {
     // ================================================================ dk and dv of 128 keys
     const int blocks = (a.s.sk + kTile - 1) / kTile;
     const int j0 = static_cast<int>(blockIdx.x) % blocks * kTile;
@@ -272,23 +282,30 @@ __global__ void __launch_bounds__(kGradThreads, 1)
           load_rows<kPanels>(base + kTileBytes, &vmap, j0, kv, b, &sh.own_full);
         }
         __syncwarp();
-        for (int n = 0; me.ok && walk.next(a.s, b, j0, first, last, (kv + 1) * group); ++n) {
-          const int st = n & 1;
-          if (n >= 2 && !me.wait(&sh.rows_empty[st], (n >> 1) - 1)) break;
+        RingPos f{0, 0}, s{0, 0};
+        while (me.ok && walk.next(a.s, b, j0, first, last, (kv + 1) * group)) {
+          if (!me.wait(&sh.first_empty[f.s], f.phase ^ 1)) break;
           if (issuer) {
-            mbar_arrive_expect_tx(&sh.rows_full[st], 2 * kTileBytes);
-            load_rows<kPanels>(ring + st * 2 * kTileBytes, &qmap, walk.tile * kTile, walk.head, b, &sh.rows_full[st]);
-            load_rows<kPanels>(ring + (st * 2 + 1) * kTileBytes, &gmap, walk.tile * kTile, walk.head, b, &sh.rows_full[st]);
+            mbar_arrive_expect_tx(&sh.first_full[f.s], kTileBytes);
+            load_rows<kPanels>(firsts + f.s * kTileBytes, &qmap, walk.tile * kTile, walk.head, b, &sh.first_full[f.s]);
           }
           __syncwarp();
+          if (!me.wait(&sh.second_empty[s.s], s.phase ^ 1)) break;
+          if (issuer) {
+            mbar_arrive_expect_tx(&sh.second_full[s.s], kTileBytes);
+            load_rows<kPanels>(seconds + s.s * kTileBytes, &gmap, walk.tile * kTile, walk.head, b, &sh.second_full[s.s]);
+          }
+          __syncwarp();
+          f.step(kFirsts);
+          s.step(kSecond);
         }
         me.land();
-      } else if (any && warp == 10) {
+      } else if (any && warp == 11) {
         // ------------------------------------------------------------ statistics of each step
         for (int n = 0;; ++n) {
           const bool more = walk.next(a.s, b, j0, first, last, (kv + 1) * group);
-          Step& step = sh.step[n & 1];
-          if (n >= 2 && !me.wait(&sh.rows_empty[n & 1], (n >> 1) - 1)) break;
+          Step<RICH>& step = sh.step[n & 1];
+          if (!me.wait(&sh.step_empty[n & 1], (n >> 1) + 1)) break;
           if (more) {
             const int i0 = walk.tile * kTile;
             const int4 t = tile_span(a.s, b, walk.tile);
@@ -301,9 +318,11 @@ __global__ void __launch_bounds__(kGradThreads, 1)
               step.delta[e + lane] = f.y;
               if (RICH || !full) {
                 const int4 sp = i0 + e + lane < a.s.sq ? span_of(a.s, b, i0 + e + lane) : make_int4(0, 0, 0, 0);
-                step.lo[e + lane] = sp.x;
-                step.hi[e + lane] = sp.y;
-                step.pos[e + lane] = static_cast<float>(sp.z);
+                const int from = min(max(sp.x - j0, 0), kTile), to = min(max(sp.y - j0, 0), kTile);
+                // whether the row sees anything at all is told apart by the order of the two
+                reinterpret_cast<uint16_t*>(step.range)[e + lane] =
+                    static_cast<uint16_t>(sp.y > sp.x ? from | to << 8 : 255 | 0 << 8);
+                if constexpr (RICH) step.pos[e + lane] = static_cast<float>(sp.z);
               }
             }
             if (lane == 0) {
@@ -320,57 +339,71 @@ __global__ void __launch_bounds__(kGradThreads, 1)
       } else if (any && warp == 9) {
         // ------------------------------------------------------------ MMA
         const bool issuer = elect_one();
-        const uint32_t k = smem_u32(base), v = k + kTileBytes;
-        auto q_of = [&](int n) { return smem_u32(ring + (n & 1) * 2 * kTileBytes); };
-        // the step's tiles are there; false at the end
-        auto ready = [&](int n) {
-          const int st = n & 1;
-          if (!me.wait(&sh.step_full[st], n >> 1) || sh.step[st].end || !me.wait(&sh.rows_full[st], n >> 1)) return false;
-          if (sh.step[st].clear) {  // rows that see nothing may hold anything
+        const uint32_t at = uniform(tmem), s_to = at, dp_to = at + kTile, dv_to = at + 2 * kTile, dk_to = at + 3 * kTile;
+        const uint32_t k = uniform(desc_dims(smem_u32(base))), v = k + kTileStep;
+        const uint32_t q_dims = k + 2 * kTileStep, g_dims = q_dims + kFirsts * kTileStep;
+        const uint32_t q_rows = uniform(desc_rows(smem_u32(firsts))), g_rows = q_rows + kFirsts * kTileStep;
+        // the step's rows are there, those that see nothing zeroed (they may hold anything); false at the end
+        auto ready = [&](int n, const RingPos& f, const RingPos& s) {
+          const Step<RICH>& step = sh.step[n & 1];
+          if (!me.wait(&sh.step_full[n & 1], n >> 1) || step.end || !me.wait(&sh.first_full[f.s], f.phase)) return false;
+          if (step.clear) {
+            if (!me.wait(&sh.second_full[s.s], s.phase)) return false;
             for (int row = lane; row < kTile; row += 32)
-              if (sh.step[st].lo[row] >= sh.step[st].hi[row])
-                for (int p = 0; p < 2 * kPanels; ++p)
-                  for (int c = 0; c < 8; ++c)
-                    *reinterpret_cast<uint4*>(ring + st * 2 * kTileBytes + p * kPanelBytes + row * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+              if ((reinterpret_cast<const uint16_t*>(step.range)[row] & 255) == 255)
+                for (int p = 0; p < kPanels; ++p)
+                  for (int c = 0; c < 8; ++c) {
+                    *reinterpret_cast<uint4*>(firsts + f.s * kTileBytes + p * kPanelBytes + row * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(seconds + s.s * kTileBytes + p * kPanelBytes + row * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+                  }
             fence_async_smem();
             __syncwarp();
           }
           return true;
         };
-        auto scores = [&](int n) {
+        RingPos f{0, 0}, s{0, 0};
+        auto scores = [&]() {
           if (issuer) {
-            product_dims<D>(s_at, k, q_of(n), kDims);
+            product_dims<D>(s_to, k, q_dims + f.s * kTileStep, kDims);
             umma_commit(&sh.s_full[0]);
           }
           __syncwarp();
         };
-        auto values = [&](int n) {
+        auto values = [&]() {
+          if (!me.wait(&sh.second_full[s.s], s.phase)) return;
           if (issuer) {
-            product_dims<D>(dp_at, v, q_of(n) + kTileBytes, kDims);
+            product_dims<D>(dp_to, v, g_dims + s.s * kTileStep, kDims);
             umma_commit(&sh.dp_full);
           }
           __syncwarp();
         };
         me.wait(&sh.own_full, 0);
-        bool more = me.ok && ready(0);
+        bool more = me.ok && ready(0, f, s);
         if (more) {
-          scores(0);
-          values(0);
+          scores();
+          values();
         }
         for (int n = 0; more && me.ok; ++n) {
+          const int q_slot = f.s, g_slot = s.s;
           if (!me.wait(&sh.p_full, n)) break;
-          if (issuer) product_rows(dv_at, s_at, q_of(n) + kTileBytes, kRows, n > 0);
+          if (issuer) {
+            product_rows<kTile>(dv_to, s_to, g_rows + g_slot * kTileStep, kRows, n > 0);
+            umma_commit(&sh.second_empty[g_slot]);
+          }
           __syncwarp();
-          more = ready(n + 1);
-          if (more) scores(n + 1);
+          f.step(kFirsts);
+          s.step(kSecond);
+          more = ready(n + 1, f, s);
+          if (more) scores();
           if (!me.wait(&sh.ds_full[0], n)) break;
           if (issuer) {
-            product_rows(dk_at, dp_at, q_of(n), kRows, n > 0);
-            umma_commit(&sh.rows_empty[n & 1]);
+            product_rows<kTile>(dk_to, dp_to, q_rows + q_slot * kTileStep, kRows, n > 0);
+            umma_commit(&sh.first_empty[q_slot]);
+            umma_commit(&sh.step_empty[n & 1]);
             if (!more) umma_commit(&sh.done);
           }
           __syncwarp();
-          if (more) values(n + 1);
+          if (more) values();
         }
       }
     } else {
@@ -382,7 +415,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
       const uint32_t s_own = s_at + lanes + half * 64, dp_own = dp_at + lanes + half * 64;
       int n = 0;
       for (; any; ++n) {
-        const Step& step = sh.step[n & 1];
+        const Step<RICH>& step = sh.step[n & 1];
         if (!me.wait(&sh.step_full[n & 1], n >> 1) || step.end) break;
         if (!me.wait(&sh.s_full[0], n)) break;
         const int c0 = half * 64;
@@ -426,12 +459,10 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         const bool masked = step.masked;
         if (masked) {
 #pragma unroll
-          for (int e = 0; e < 64; e += 4) {
-            const int4 lo = *reinterpret_cast<const int4*>(step.lo + c0 + e), hi = *reinterpret_cast<const int4*>(step.hi + c0 + e);
-            p[e] = j >= lo.x && j < hi.x ? p[e] : 0.0f;
-            p[e + 1] = j >= lo.y && j < hi.y ? p[e + 1] : 0.0f;
-            p[e + 2] = j >= lo.z && j < hi.z ? p[e + 2] : 0.0f;
-            p[e + 3] = j >= lo.w && j < hi.w ? p[e + 3] : 0.0f;
+          for (int e = 0; e < 64; e += 2) {
+            const uint32_t two = step.range[(c0 + e) >> 1];
+            p[e] = r >= static_cast<int>(two & 255u) && r < static_cast<int>(two >> 8 & 255u) ? p[e] : 0.0f;
+            p[e + 1] = r >= static_cast<int>(two >> 16 & 255u) && r < static_cast<int>(two >> 24) ? p[e + 1] : 0.0f;
           }
         }
         store_half<T>(s_own, p);
@@ -491,57 +522,75 @@ __global__ void __launch_bounds__(kGradThreads, 1)
           load_rows<kPanels>(base + kTileBytes, &gmap, i0, head, b, &sh.own_full);
         }
         __syncwarp();
-        for (int item = 0; item < 2 * ntiles && me.ok; ++item) {
-          const int sl = item % kKeySlots, use = item / kKeySlots;
-          if (use > 0 && !me.wait(&sh.slot_empty[sl], use - 1)) break;
+        RingPos f{0, 0}, s{0, 0};
+        for (int t = 0; t < ntiles; ++t) {
+          if (!me.wait(&sh.first_empty[f.s], f.phase ^ 1)) break;
           if (issuer) {
-            mbar_arrive_expect_tx(&sh.slot_full[sl], kTileBytes);
-            load_rows<kPanels>(ring + sl * kTileBytes, item & 1 ? &vmap : &kmap, key0 + (item >> 1) * kTile, kv, b, &sh.slot_full[sl]);
+            mbar_arrive_expect_tx(&sh.first_full[f.s], kTileBytes);
+            load_rows<kPanels>(firsts + f.s * kTileBytes, &kmap, key0 + t * kTile, kv, b, &sh.first_full[f.s]);
           }
           __syncwarp();
+          if (!me.wait(&sh.second_empty[s.s], s.phase ^ 1)) break;
+          if (issuer) {
+            mbar_arrive_expect_tx(&sh.second_full[s.s], kTileBytes);
+            load_rows<kPanels>(seconds + s.s * kTileBytes, &vmap, key0 + t * kTile, kv, b, &sh.second_full[s.s]);
+          }
+          __syncwarp();
+          f.step(kFirsts);
+          s.step(kSecond);
         }
         me.land();
       } else if (ntiles > 0 && warp == 9) {
-        // ------------------------------------------------------------ MMA
+        // ------------------------------------------------------------ MMA: scores
         const bool issuer = elect_one();
-        const uint32_t q = smem_u32(base), g = q + kTileBytes;
-        auto slot_of = [&](int item) { return smem_u32(ring + item % kKeySlots * kTileBytes); };
-        auto wait_slot = [&](int item) { return me.wait(&sh.slot_full[item % kKeySlots], item / kKeySlots); };
-        auto scores = [&](int t) {
-          if (!wait_slot(2 * t)) return;
+        const uint32_t at = uniform(tmem);
+        const uint32_t q = uniform(desc_dims(smem_u32(base))), k = uniform(desc_dims(smem_u32(firsts)));
+        const int last = static_cast<int>(uniform(ntiles)) - 1;
+        RingPos f{0, 0};
+        me.wait(&sh.own_full, 0);
+        for (int t = 0; t <= last && me.ok; ++t) {
+          if (!me.wait(&sh.first_full[f.s], f.phase)) break;
           const int left = key_end - (key0 + t * kTile);  // keys past these are nobody's and may hold anything
-          if (left < kTile) clear_rows<kPanels>(ring + 2 * t % kKeySlots * kTileBytes, left, kTile, lane);
+          if (left < kTile) clear_rows<kPanels>(firsts + f.s * kTileBytes, left, kTile, lane);
+          // dq's product two tiles before has read the buffer
+          if (t > 1 && !me.wait(&sh.dq_done[t & 1], (t >> 1) - 1)) break;
           if (issuer) {
-            product_dims<D>(tmem + (t & 1) * kTile, q, slot_of(2 * t), kDims);
+            product_dims<D>(at + (t & 1) * kTile, q, k + f.s * kTileStep, kDims);
             umma_commit(&sh.s_full[t & 1]);
           }
           __syncwarp();
-        };
-        auto values = [&](int t) {
-          if (!wait_slot(2 * t + 1)) return;
+          f.step(kFirsts);
+        }
+      } else if (ntiles > 0 && warp == 10) {
+        // ------------------------------------------------------------ MMA: g.v and dq
+        const bool issuer = elect_one();
+        const uint32_t at = uniform(tmem), dp_to = at + 2 * kTile, dq_to = at + 3 * kTile;
+        const uint32_t g = uniform(desc_dims(smem_u32(base) + kTileBytes)), v = uniform(desc_dims(smem_u32(seconds)));
+        const uint32_t k_rows = uniform(desc_rows(smem_u32(firsts)));
+        const int last = static_cast<int>(uniform(ntiles)) - 1;
+        RingPos f{0, 0}, s{0, 0};
+        auto values = [&]() {
+          if (!me.wait(&sh.second_full[s.s], s.phase)) return;
           if (issuer) {
-            product_dims<D>(dp_at, g, slot_of(2 * t + 1), kDims);
+            product_dims<D>(dp_to, g, v + s.s * kTileStep, kDims);
             umma_commit(&sh.dp_full);
-            umma_commit(&sh.slot_empty[(2 * t + 1) % kKeySlots]);
+            umma_commit(&sh.second_empty[s.s]);
           }
           __syncwarp();
+          s.step(kSecond);
         };
         me.wait(&sh.own_full, 0);
-        if (me.ok) scores(0);
-        if (me.ok) values(0);
-        for (int t = 0; t < ntiles && me.ok; ++t) {
-          if (t + 1 < ntiles) {
-            if (t > 0 && !me.wait(&sh.slot_empty[2 * (t - 1) % kKeySlots], (t - 1) / 2)) break;
-            scores(t + 1);
-            if (me.wait(&sh.dp_free, t)) values(t + 1);
-          }
-          if (!me.wait(&sh.ds_full[t & 1], t >> 1)) break;
+        if (me.ok) values();
+        for (int t = 0; t <= last && me.ok; ++t) {
+          if (t < last && me.wait(&sh.dp_free, t)) values();
+          if (!me.wait(&sh.first_full[f.s], f.phase) || !me.wait(&sh.ds_full[t & 1], t >> 1)) break;
           if (issuer) {
-            product_rows(dq_at, tmem + (t & 1) * kTile, slot_of(2 * t), kRows, t > 0);
-            umma_commit(&sh.slot_empty[2 * t % kKeySlots]);
-            if (t == ntiles - 1) umma_commit(&sh.done);
+            product_rows<kTile>(dq_to, at + (t & 1) * kTile, k_rows + f.s * kTileStep, kRows, t > 0);
+            umma_commit(&sh.first_empty[f.s]);
+            umma_commit(t == last ? &sh.done : &sh.dq_done[t & 1]);
           }
           __syncwarp();
+          f.step(kFirsts);
         }
       }
     } else {
@@ -634,13 +683,14 @@ template <int AB, int D>
 int launch_grad(const GradArgs& a, const CUtensorMap (&maps)[4], cudaStream_t stream) {
   const bool rich = a.s.cap > 0.0f || a.s.slopes;
   auto kernel = rich ? span_attention_grad_kernel<AB, D, true> : span_attention_grad_kernel<AB, D, false>;
+  const int smem = rich ? grad_smem<D, true>() : grad_smem<D, false>();
   static std::atomic<unsigned long long> granted[2] = {};
-  if (cudaError_t e = grant_smem(reinterpret_cast<const void*>(kernel), grad_smem<D>(), granted[rich])) return static_cast<int>(e);
+  if (cudaError_t e = grant_smem(reinterpret_cast<const void*>(kernel), smem, granted[rich])) return static_cast<int>(e);
   if (a.s.sq > 0) {
     const long long rows = static_cast<long long>(a.s.batch) * a.s.heads * a.padded;
     if (int st = launch_overlapped(grad_stats_kernel<AB>, dim3(static_cast<unsigned>((rows + 15) / 16)), dim3(256), 0, 0, stream, a)) return st;
   }
-  return launch_overlapped(kernel, dim3(a.key_units + a.query_units), dim3(kGradThreads), grad_smem<D>(), 0, stream, maps[0],
+  return launch_overlapped(kernel, dim3(a.key_units + a.query_units), dim3(kGradThreads), smem, 0, stream, maps[0],
                            maps[1], maps[2], maps[3], a);
 }
 
