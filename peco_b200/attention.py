@@ -55,7 +55,9 @@ def _ends(ends, batch, what):
         raise TypeError(f"{what} must be an int32 or int64 tensor")
     if ends.dim() not in (1, 2) or ends.shape[-1] < 2 or ends.dim() == 2 and ends.shape[0] not in (1, batch):
         raise ValueError(f"{what} must be [n + 1] or one such row for each of the {batch} samples")
-    ends = ends.to(torch.int32).contiguous()
+    if ends.dtype is not torch.int32:
+        ends = ends.to(torch.int32)
+    ends = ends.contiguous()
     return ends, ends.shape[1] if ends.dim() == 2 and ends.shape[0] > 1 else 0
 
 
@@ -117,11 +119,17 @@ def key_spans(batch, queries, keys, *, documents=None, key_documents=None, lengt
         tensors.append(prefix_rows)
     elif prefix is not None:
         prefix_all = min(max(int(prefix), 0), 2 ** 31 - 1)
-    device = tensors[0].device if device is None and tensors else torch.device("cuda" if device is None else device)
-    if device.type == "cuda" and device.index is None:
-        device = torch.device("cuda", torch.cuda.current_device())
-    if device.type != "cuda" or any(t.device != device for t in tensors):
-        _native.require_cuda(torch.empty(0, device=device), *tensors)
+    if device is None:
+        device = tensors[0].device if tensors else torch.device("cuda", torch.cuda.current_device())
+    elif not isinstance(device, torch.device) or device.type == "cuda" and device.index is None:
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+    if device.type != "cuda":
+        raise RuntimeError("peco_b200 runs on CUDA devices only; got " + str(device))
+    for t in tensors:
+        if t.device != device:
+            raise ValueError("all tensors must be on the same CUDA device")
     rows = torch.empty((batch, queries, 4), dtype=torch.int32, device=device)
     tiles = torch.empty((batch, -(-queries // 128), 4), dtype=torch.int32, device=device)
     address = _native.address
@@ -135,51 +143,57 @@ def key_spans(batch, queries, keys, *, documents=None, key_documents=None, lengt
 
 def _check(q, k, v, spans, scale, softcap, slopes):
     """Checked (batch, heads, key heads, queries, keys, dims), scale and cap."""
-    if not all(isinstance(t, torch.Tensor) and t.dim() == 4 for t in (q, k, v)):
+    if not (isinstance(q, torch.Tensor) and isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor)
+            and q.dim() == 4 and k.dim() == 4):
         raise ValueError("Expected q [B, H, N, D] and k, v [B, KV, M, D]")
-    if q.dtype not in _SIXTEEN_BITS or k.dtype is not q.dtype or v.dtype is not q.dtype:
+    dtype, device = q.dtype, q.device
+    if dtype not in _SIXTEEN_BITS or k.dtype is not dtype or v.dtype is not dtype:
         raise TypeError("attention takes float16 or bfloat16 tensors of one dtype")
     b, h, n, d = q.shape
-    kv, m = k.shape[1:3]
-    if k.shape != (b, kv, m, d) or v.shape != k.shape:
+    shape = k.shape
+    kv, m = shape[1], shape[2]
+    if shape[0] != b or shape[3] != d or v.shape != shape:
         raise ValueError("k and v must be [B, KV, M, D] with the batch and head dimension of q")
     if kv < 1 or h < 1 or h % kv:
         raise ValueError("the query heads must be a multiple of the key heads")
     if d < 8 or d > 128 or d % 8:
         raise ValueError("the head dimension must be a multiple of 8 up to 128")
-    if max(n, m) > 0x7ffffe00:
+    if n > 0x7ffffe00 or m > 0x7ffffe00:
         raise ValueError("too many rows")
     scale = d ** -0.5 if scale is None else float(scale)
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError("scale must be positive")
-    cap = 0.0 if softcap is None else float(softcap)
-    if softcap is not None and not (cap > 0 and math.isfinite(cap)):
-        raise ValueError("softcap must be positive")
-    others = [k, v]
+    cap = 0.0
+    if softcap is not None:
+        cap = float(softcap)
+        if not (cap > 0 and math.isfinite(cap)):
+            raise ValueError("softcap must be positive")
     if slopes is not None:
         if not isinstance(slopes, torch.Tensor) or slopes.dtype is not torch.float32 or slopes.shape != (h,):
             raise ValueError(f"slopes must be a float32 tensor [{h}]")
-        if torch.is_grad_enabled() and slopes.requires_grad:
+        if slopes.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("attention has no gradient of slopes")
-        others.append(slopes)
     if spans is not None:
         if not isinstance(spans, KeySpans):
             raise TypeError("spans must come from key_spans")
-        if (spans.queries, spans.keys) != (n, m) or spans.rows.shape[0] not in (1, b):
+        if spans.queries != n or spans.keys != m or spans.rows.shape[0] not in (1, b):
             raise ValueError(f"spans are for {spans.rows.shape[0]} samples of {spans.queries} rows and {spans.keys} keys, "
                              f"the call has {b} of {n} and {m}")
-        others += [spans.rows, spans.tiles]
-    _native.require_cuda(q, *others)
+    if device.type != "cuda" or k.device != device or v.device != device or (slopes is not None and slopes.device != device) \
+            or (spans is not None and spans.rows.device != device):
+        _native.require_cuda(q, k, v, *(t for t in (slopes, spans and spans.rows) if t is not None))
     return (b, h, kv, n, m, d), scale, cap
 
 
 def _readable(t):
     """``t`` with adjacent dims and every row on 16 bytes: itself, or a copy."""
-    sizes, steps = t.shape, t.stride()
-    if steps[3] == 1 and t.data_ptr() % 16 == 0 and all(
-            n <= 1 or 0 < s < 1 << 38 and s % 8 == 0 for n, s in zip(sizes[:3], steps[:3])):
-        return t
-    return t.contiguous() if not t.is_contiguous() else t.clone()
+    if t.data_ptr() & 15 == 0:
+        if t.is_contiguous():
+            return t
+        sizes, steps = t.shape, t.stride()
+        if steps[3] == 1 and all(n <= 1 or 0 < s < 1 << 38 and s % 8 == 0 for n, s in zip(sizes[:3], steps[:3])):
+            return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _mask_args(spans, b):
@@ -189,26 +203,27 @@ def _mask_args(spans, b):
 
 
 def _forward(q, k, v, spans, scale, softcap, slopes):
-    sizes, scale, cap = _check(q, k, v, spans, scale, softcap, slopes)
-    b, h, kv, n, m, d = sizes
+    (b, h, kv, n, m, d), scale, cap = _check(q, k, v, spans, scale, softcap, slopes)
+    device = q.device
     out = torch.empty_like(q)
-    lse = torch.empty((b, h, n), dtype=torch.float32, device=q.device)
-    if out.numel() == 0:
+    lse = torch.empty((b, h, n), dtype=torch.float32, device=device)
+    if b == 0 or n == 0:
         return out, lse
-    q, k, v = _readable(q), _readable(k), _readable(v)
-    whole = out if _readable(out) is out else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    q, k, v, whole = _readable(q), _readable(k), _readable(v), out
+    if not out.is_contiguous() and _readable(out) is not out:
+        whole = torch.empty(q.shape, dtype=q.dtype, device=device)
     if slopes is not None:
         slopes = slopes.contiguous()
     lib = _native.load()
     need = int(lib.peco_span_attention_workspace(b, h, kv, n, m, d))
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-    strides = _Strides(*(s for t in (q, k, v, whole) for s in t.stride()[:3]))
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+    strides = _Strides(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *whole.stride()[:3])
     rows, tiles, batched = _mask_args(spans, b)
-    _native.enqueue(q.device, "peco_span_attention", lib.peco_span_attention,
+    inputs = (q, k, v, slopes) if spans is None else (q, k, v, slopes, spans.rows, spans.tiles)
+    _native.enqueue(device, "peco_span_attention", lib.peco_span_attention,
                     (q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, rows, tiles, batched, _native.address(slopes), scale,
                      cap, whole.data_ptr(), lse.data_ptr(), b, h, kv, n, m, d, _native.DTYPE_CODE[q.dtype],
-                     _native.address(ws), max(need, 0)),
-                    (q, k, v, slopes, *((spans.rows, spans.tiles) if spans is not None else ())))
+                     _native.address(ws), max(need, 0)), inputs)
     return out.copy_(whole) if whole is not out else out, lse
 
 

@@ -8,21 +8,26 @@
 //  * span_attention_kernel walks them; split_attention_kernel joins the parts of
 //    calls with few rows, whose keys are split over CTAs.
 //
-// A CTA takes two tiles of 128 query rows of one head (or one: few rows, or rows
-// of several heads that share their keys side by side).  Per 128 keys and tile:
+// A CTA takes a tile of 128 query rows of one head (or rows of several heads that
+// share their keys, side by side); two warpgroups take its even and its odd key
+// tiles, each with its own running maximum, sum and accumulator, joined at the
+// end.  Per tile of 128 keys:
 //   S = Q K^T        tcgen05.mma, both in shared memory, S in TMEM
-//   P = 2^(z - m)    four warps, a query row a thread; m, the running maximum, is
-//                    raised only when it grows by more than 2^8, and O rescaled
+//   P = 2^(z - m)    a query row a thread; m, the running maximum, is raised only
+//                    when it grows by more than 2^8, and O rescaled
 //   O += P V         tcgen05.mma, P from TMEM (over S, as 16-bit pairs)
-// While one tile's softmax runs, the tensor core works on the other's products.  A
+// While one warpgroup's softmax runs, the tensor core works for the other.  A
 // tile's next S overwrites the P that O's product before it reads: products that
 // one thread issues are executed in the order of their issue.  K and V stream
-// through five shared-memory slots by TMA.
+// through six shared-memory slots by TMA.
 //
 // What it measured (B200, bf16): 24 heads x 7006 rows x 128 dims, every key: 565 us
-// (1.02 PFLOP/s of the visible pairs; 606 us at the power limit after 300 calls in a
-// row); 64 dims 480 us; causal, 24 query heads on 4, 4096 rows 151 us.  Bound by the round trip
-// of a tile: 1500 clocks of softmax and 1000 of products, 1670 a tile with two in
+// (1.02 PFLOP/s; about 606 us at the power limit after 300 calls in a row), 64 dims 467
+// us; causal, 24 query heads on 4, 4096 rows 146 us; one row of 24 heads on 4, four
+// samples of up to 16384 keys 32 us.  Two tiles of rows with the same key tile instead,
+// which halves the traffic from L2, took as long on full masks and more on others
+// (causal 150, clips packed in causal order 102 us against 89).  Bound by a tile's
+// round trip: 1500 clocks of softmax and 1000 of products, 1670 a tile with two in
 // flight (without the softmax 375 us, without the products 405).
 #include "span_attention.cuh"
 #include "../../include/peco_b200.h"
@@ -113,11 +118,11 @@ __global__ void __launch_bounds__(kTile) key_spans_kernel(const SpanArgs a) {
 }
 
 // ---- forward ----------------------------------------------------------------------------
-constexpr int kSlots = 5;        // of K(t) in slot 2t mod 5, V(t) in slot 2t + 1 mod 5
+constexpr int kSlots = 6;        // of K(t) in slot 2t mod 6, V(t) in slot 2t + 1 mod 6
 constexpr int kThreads = 384;    // two softmax warpgroups, one with the TMA warp and the MMA warp
 // A softmax thread holds a tile's 128 scores: the launch's 168 registers a thread
 // go 208 to 208 to 88 (256 * 208 + 128 * 88 = 384 * 168).
-constexpr uint32_t kTmemCols = 512;  // S of both tiles, then O of both
+constexpr uint32_t kTmemCols = 512;  // S of both warpgroups, then O of both
 
 struct ForwardArgs {
   ScoreArgs s;
@@ -126,24 +131,24 @@ struct ForwardArgs {
   long long out_batch, out_head, out_row;
   float* lse;               // [batch, heads, sq]
   int packed;               // heads side by side in a tile (1: consecutive rows of one head)
-  int tiles;                // query tiles a CTA takes: 1 or 2
   int row_blocks;           // CTAs along a head's rows
   int splits;               // CTAs along the keys
-  float* part;              // [unit][split][tile][128][d] unnormalised, then (max, sum) of each row
+  float* part;              // [unit][split][128][d] unnormalised, then (max, sum) of each row
   float2* part_sums;
 };
 
 struct __align__(8) ForwardShared {
   uint64_t q_full, slot_full[kSlots], slot_empty[kSlots], s_full[2], p_full[2], o_full[2];
   uint32_t tmem;
-  int abort_flag;
+  int abort_flag, masked;
+  float2 sums[kTile];       // of the odd key tiles' (maximum, sum)
 };
 
 template <int D>
-constexpr int forward_smem() { return 1024 + (2 + kSlots) * kTile * D * 2 + 512; }
-static_assert(sizeof(ForwardShared) <= 512 && forward_smem<128>() <= 227 * 1024, "shared memory of a CTA");
+constexpr int forward_smem() { return 1024 + (1 + kSlots) * kTile * D * 2 + 1536; }
+static_assert(sizeof(ForwardShared) <= 1536 && forward_smem<128>() <= 227 * 1024, "shared memory of a CTA");
 
-// Which head and query row thread ``r`` of tile ``w`` of a unit holds.
+// Which head and query row thread ``r`` of a unit holds.
 struct Unit {
   int b, head0, row0;       // first head, first row
   __device__ Unit(const ForwardArgs& a, int unit) {
@@ -152,29 +157,22 @@ struct Unit {
     const int rest = unit / a.row_blocks;
     head0 = rest % groups * a.packed;
     b = rest / groups;
-    row0 = block * a.tiles * kTile;
+    row0 = block * kTile;
   }
-  __device__ __forceinline__ bool row(const ForwardArgs& a, int w, int r, int& head, int& i) const {
+  __device__ __forceinline__ bool row(const ForwardArgs& a, int r, int& head, int& i) const {
     if (a.packed > 1) {
       head = head0 + r / a.s.sq;
       i = r % a.s.sq;
-      return w == 0 && r < a.packed * a.s.sq;
+      return r < a.packed * a.s.sq;
     }
     head = head0;
-    i = row0 + w * kTile + r;
+    i = row0 + r;
     return i < a.s.sq;
   }
   // keys that a row of the unit sees: [lo, hi)
   __device__ __forceinline__ int2 keys(const ForwardArgs& a) const {
-    const int4 t0 = tile_span(a.s, b, row0 / kTile);
-    int lo = t0.x, hi = t0.y;
-    if (a.tiles == 2 && row0 + kTile < a.s.sq) {
-      const int4 t1 = tile_span(a.s, b, row0 / kTile + 1);
-      lo = min(lo, t1.x);
-      hi = max(hi, t1.y);
-    }
-    lo = max(lo, 0);
-    hi = min(hi, a.s.sk);
+    const int4 t = tile_span(a.s, b, row0 / kTile);
+    const int lo = max(t.x, 0), hi = min(t.y, a.s.sk);
     return make_int2(min(lo, hi), hi);
   }
 };
@@ -234,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kPanels = D / 64, kTileBytes = kPanels * kPanelBytes;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  unsigned char* slots = base + 2 * kTileBytes;
+  unsigned char* slots = base + kTileBytes;
   ForwardShared& sh = *reinterpret_cast<ForwardShared*>(slots + kSlots * kTileBytes);
   volatile int* abort_flag = &sh.abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -250,6 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sh.o_full[w], 1);
     }
     sh.abort_flag = 0;
+    sh.masked = 0;
     fence_barrier_init();
   }
   if (warp == 8 && lane == 0) {
@@ -272,7 +271,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int2 all_keys = unit.keys(a);
   const int2 mine = split_keys(all_keys, split, a.splits);
   const int key0 = mine.x, ntiles = mine.y;
-  const int tiles = a.tiles == 2 && unit.row0 + kTile < a.s.sq ? 2 : 1;
 
   if (warp >= 8) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
@@ -282,11 +280,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int kv = unit.head0 / (a.s.heads / a.s.kv_heads);
     bool ok = true;
     if (ntiles > 0 && issuer) {
-      const uint32_t q_bytes = a.packed > 1 ? static_cast<uint32_t>(a.packed * a.s.sq) * 128u * kPanels
-                                            : static_cast<uint32_t>(min(a.s.sq, kTile)) * 128u * kPanels;
-      mbar_arrive_expect_tx(&sh.q_full, q_bytes * tiles);
-      for (int w = 0; w < tiles; ++w)
-        load_rows<kPanels>(base + w * kTileBytes, &qmap, unit.row0 + w * kTile, unit.head0, unit.b, &sh.q_full);
+      mbar_arrive_expect_tx(&sh.q_full, static_cast<uint32_t>(a.packed * min(a.s.sq, kTile)) * 128u * kPanels);
+      load_rows<kPanels>(base, &qmap, unit.row0, unit.head0, unit.b, &sh.q_full);
     }
     __syncwarp();
     for (int item = 0; item < 2 * ntiles && ok; ++item) {
@@ -313,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_at = uniform(tmem), o_at = s_at + 2 * kTile;
     const uint32_t q = uniform(desc_dims(smem_u32(base))), k = uniform(desc_dims(smem_u32(slots)));
     const uint32_t v = uniform(desc_rows(smem_u32(slots)));
-    const int last = static_cast<int>(uniform(ntiles)) - 1, both = static_cast<int>(uniform(tiles)) - 1;
+    const int last = static_cast<int>(uniform(ntiles)) - 1;
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t phase) {
       if (ok) ok = warp_wait(bar, phase, abort_flag, a.s.status);
@@ -322,50 +317,55 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     auto scores = [&](int w, int slot) {
       if (issuer) {
-        product_dims<D>(s_at + w * kTile, q + w * kSlotStep, k + slot * kSlotStep, idesc_qk);
+        product_dims<D>(s_at + w * kTile, q, k + slot * kSlotStep, idesc_qk);
         umma_commit(&sh.s_full[w]);
-        if (w == both) umma_commit(&sh.slot_empty[slot]);
+        umma_commit(&sh.slot_empty[slot]);
       }
       __syncwarp();
     };
+    // keys past a unit's last are nobody's: their values may be anything
+    auto clear_unseen = [&](int t, int slot) {
+      const int seen = all_keys.y - (key0 + t * kTile);
+      if (seen < kTile) clear_rows<kPanels>(slots + slot * kTileBytes, seen, kTile, lane);
+    };
     if (last >= 0) {
-      RingPos pos{0, 0};  // of the next slot to wait for
+      // K(t) is item 2t of the ring, V(t) item 2t + 1; the scores run two tiles ahead of the values
+      RingPos ks{0, 0}, vs{1, 0};
+      auto two_on = [](RingPos& p) {
+        p.step(kSlots);
+        p.step(kSlots);
+      };
       wait(&sh.q_full, 0);
-      if (wait(&sh.slot_full[0], 0)) {
-        scores(0, 0);
-        if (both) scores(1, 0);
-      }
-      pos.step(kSlots);
-      for (int t = 0; t <= last && ok; ++t) {
-        const int vs = pos.s;
-        if (!wait(&sh.slot_full[vs], pos.phase)) break;
-        pos.step(kSlots);
-        const int seen = all_keys.y - (key0 + t * kTile);  // keys past these are nobody's: their values may be anything
-        if (seen < kTile) clear_rows<kPanels>(slots + vs * kTileBytes, seen, kTile, lane);
-        if (t < last && !wait(&sh.slot_full[pos.s], pos.phase)) break;
-        for (int w = 0; w <= both; ++w) {
-          if (!wait(&sh.p_full[w], t & 1)) break;
-          if (issuer) {
-            product_rows<kTile>(o_at + w * kTile, s_at + w * kTile, v + vs * kSlotStep, idesc_pv, t > 0);
-            if (w == both) umma_commit(&sh.slot_empty[vs]);
-            if (t == last) umma_commit(&sh.o_full[w]);
-          }
-          __syncwarp();
-          if (t < last) scores(w, pos.s);
+      for (int t = 0; t < 2 && t <= last; ++t, two_on(ks))
+        if (wait(&sh.slot_full[ks.s], ks.phase)) scores(t, ks.s);
+      for (int t = 0; t <= last && ok; ++t, two_on(vs)) {
+        const int w = t & 1;
+        if (!wait(&sh.slot_full[vs.s], vs.phase)) break;
+        clear_unseen(t, vs.s);
+        if (!wait(&sh.p_full[w], (t >> 1) & 1)) break;
+        if (issuer) {
+          product_rows<kTile>(o_at + w * kTile, s_at + w * kTile, v + vs.s * kSlotStep, idesc_pv, t > 1);
+          umma_commit(&sh.slot_empty[vs.s]);
+          if (t + 2 > last) umma_commit(&sh.o_full[w]);
         }
-        if (t < last) pos.step(kSlots);
+        __syncwarp();
+        if (t + 2 <= last) {
+          if (!wait(&sh.slot_full[ks.s], ks.phase)) break;
+          scores(w, ks.s);
+          two_on(ks);
+        }
       }
     }
   }
   } else {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-  if ((warp >> 2) < tiles) {
     // ------------------------------------------------------- softmax, epilogue
     const int w = warp >> 2, r = threadIdx.x & (kTile - 1);
+    const int turns = (ntiles + 1 - w) >> 1;  // key tiles of this warpgroup
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + w * kTile + lanes, o_at = tmem + 2 * kTile + w * kTile + lanes;
     int head, i;
-    const bool real = unit.row(a, w, r, head, i);
+    const bool real = unit.row(a, r, head, i);
     const int4 span = real ? span_of(a.s, unit.b, i) : make_int4(0, 0, 0, 0);
     const int lo = span.x, hi = span.y;
     const float scale_log2 = a.s.scale * kLog2E;
@@ -373,11 +373,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float slope = RICH && a.s.slopes && real ? a.s.slopes[head] * kLog2E : 0.0f;
     float m = -INFINITY, l = 0.0f;
     bool ok = true, masked = false;
-    for (int t = 0; t < ntiles; ++t) {
+    for (int t = 0; t < turns; ++t) {
       ok = warp_wait(&sh.s_full[w], t & 1, abort_flag, a.s.status);
       if (!ok) break;
       tc_fence_after();
-      const int j0 = key0 + t * kTile;
+      const int j0 = key0 + (2 * t + w) * kTile;
       float s[kTile];
       {
         uint32_t raw[kTile];
@@ -462,11 +462,40 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.p_full[w]);
     }
-    if (ok && ntiles > 0) {
+    if (ok && turns > 0) {
       ok = warp_wait(&sh.o_full[w], 0, abort_flag, a.s.status);
       tc_fence_after();
     }
-    if (ok) {
+    // the odd key tiles' result through shared memory (the slots, once both accumulators are
+    // complete): columns in fours, [fours][128 rows]
+    float own = 1.0f, other = 0.0f;  // factors of this accumulator and of the odd tiles'
+    const uint32_t exchange = smem_u32(slots) + r * 16;
+    if (w == 1 && turns > 0 && ok) {
+      ok = warp_wait(&sh.o_full[0], 0, abort_flag, a.s.status);
+      if (masked && lane == 0) sh.masked = 1;
+      sh.sums[r] = make_float2(m, l);
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t raw[32];
+        tmem_ld32_sync(o_at + c * 32, raw);
+#pragma unroll
+        for (int g = 0; g < 8; ++g)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(exchange + (c * 8 + g) * kTile * 16), "r"(raw[4 * g]),
+                       "r"(raw[4 * g + 1]), "r"(raw[4 * g + 2]), "r"(raw[4 * g + 3])
+                       : "memory");
+      }
+    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");  // (after an expired wait too)
+    if (w == 0 && ntiles > 1) {
+      masked = masked || sh.masked;
+      const float2 odd = sh.sums[r];
+      const float top = fmaxf(m, odd.x);
+      own = m == -INFINITY ? 0.0f : exp2_approx(m - top);
+      other = odd.x == -INFINITY ? 0.0f : exp2_approx(odd.x - top);
+      l = l * own + odd.y * other;
+      m = top;
+    }
+    if (ok && w == 0 && !*abort_flag) {
       const bool whole = a.splits == 1;
       const float inv = !whole ? 1.0f : l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;  // (a NaN stays)
       T* out = nullptr;
@@ -476,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         a.lse[(static_cast<long long>(unit.b) * a.s.heads + head) * a.s.sq + i] =
             l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
       } else if (real) {
-        const long long at = (static_cast<long long>(blockIdx.x) * a.tiles + w) * kTile + r;
+        const long long at = static_cast<long long>(blockIdx.x) * kTile + r;
         part = a.part + at * a.s.d;
         a.part_sums[at] = make_float2(m, l);
       }
@@ -488,6 +517,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         else
 #pragma unroll
           for (int e = 0; e < 32; ++e) raw[e] = 0u;
+        if (ntiles > 1) {
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            float odd[4];
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(odd[0]), "=f"(odd[1]), "=f"(odd[2]), "=f"(odd[3])
+                         : "r"(exchange + (c * 8 + g) * kTile * 16)
+                         : "memory");
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              raw[4 * g + e] = __float_as_uint(fmaf(odd[e], other, __uint_as_float(raw[4 * g + e]) * own));
+          }
+        }
         float2 v[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -530,11 +572,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             static_cast<T*>(a.out)[unit.b * a.out_batch + h2 * a.out_head + static_cast<long long>(i2) * a.out_row + c] =
                 from_f32<T>(acc[e] * f);
           else
-            a.part[((static_cast<long long>(blockIdx.x) * a.tiles + w) * kTile + (r - lane) + from) * a.s.d + c] = acc[e] * f;
+            a.part[(static_cast<long long>(blockIdx.x) * kTile + (r - lane) + from) * a.s.d + c] = acc[e] * f;
         }
       }
     }
-  }
   }
   __syncwarp();
   tc_fence_before();
@@ -545,63 +586,67 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// A row's parts joined: out = sum_p O_p 2^(m_p - M) / sum_p l_p 2^(m_p - M); a warp a row.
+// A row's parts joined: out = sum_p O_p 2^(m_p - M) / sum_p l_p 2^(m_p - M).  A block
+// a row: its warps take every fourth part, and their sums are added in order.
 template <int AB>
 __global__ void __launch_bounds__(128) split_attention_kernel(const __grid_constant__ ForwardArgs a) {
   using T = Element<AB>;
+  __shared__ float sums[4][kTile + 1];
   wait_for_prior();
   let_next_start();
-  const int lane = threadIdx.x & 31;
-  const long long at = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);  // (unit, tile, row of the tile)
-  const int r = static_cast<int>(at % kTile), w = static_cast<int>(at / kTile % a.tiles);
-  const int n = static_cast<int>(at / kTile / a.tiles);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rows = a.packed > 1 ? a.packed * a.s.sq : min(a.s.sq, kTile);  // of a unit that can be there
+  const int n = static_cast<int>(blockIdx.x) / rows, r = static_cast<int>(blockIdx.x) % rows;
   const Unit unit(a, n);
   int head, i;
-  if (!unit.row(a, w, r, head, i)) return;
-  const long long first = (static_cast<long long>(n) * a.splits * a.tiles + w) * kTile + r, step = static_cast<long long>(a.tiles) * kTile;
+  if (!unit.row(a, r, head, i)) return;
+  const long long first = static_cast<long long>(n) * a.splits * kTile + r;
   float m = -INFINITY;
-  for (int p = lane; p < a.splits; p += 32) m = fmaxf(m, a.part_sums[first + p * step].x);
+  for (int p = lane; p < a.splits; p += 32) m = fmaxf(m, a.part_sums[first + p * static_cast<long long>(kTile)].x);
   m = warp_max(m);
   float l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int p = 0; p < a.splits; ++p) {
-    const float2 s = a.part_sums[first + p * step];
-    if (s.y == 0.0f) continue;
-    const float f = exp2_approx(s.x - m);
+#pragma unroll 4
+  for (int p = warp; p < a.splits; p += 4) {
+    const long long at = first + p * static_cast<long long>(kTile);
+    const float2 s = a.part_sums[at];
+    const float f = s.y == 0.0f ? 0.0f : exp2_approx(s.x - m);
     l = fmaf(s.y, f, l);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (lane + 32 * e < a.s.d) acc[e] = fmaf(a.part[(first + p * step) * a.s.d + lane + 32 * e], f, acc[e]);
+      if (lane + 32 * e < a.s.d) acc[e] = fmaf(a.part[at * a.s.d + lane + 32 * e], f, acc[e]);
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  T* out = static_cast<T*>(a.out) + unit.b * a.out_batch + head * a.out_head + static_cast<long long>(i) * a.out_row;
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (lane + 32 * e < a.s.d) out[lane + 32 * e] = from_f32<T>(acc[e] * inv);
-  if (lane == 0)
+  for (int e = 0; e < 4; ++e) sums[warp][lane + 32 * e] = acc[e];
+  if (lane == 0) sums[warp][kTile] = l;
+  __syncthreads();
+  const int c = threadIdx.x;
+  l = sums[0][kTile] + sums[1][kTile] + sums[2][kTile] + sums[3][kTile];
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if (c < a.s.d)
+    static_cast<T*>(a.out)[unit.b * a.out_batch + head * a.out_head + static_cast<long long>(i) * a.out_row + c] =
+        from_f32<T>((sums[0][c] + sums[1][c] + sums[2][c] + sums[3][c]) * inv);
+  if (c == 0)
     a.lse[(static_cast<long long>(unit.b) * a.s.heads + head) * a.s.sq + i] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 // ---- host ---------------------------------------------------------------------------------
-// How a call is cut.  Two tiles a CTA keep the tensor core busy under the softmax;
-// one where that leaves SMs without work.  Rows of heads that share their keys go
-// side by side into one tile where they fit: the keys are then read once for all of
-// them.  Calls that still leave half of the SMs idle split the keys, four tiles at
-// least to a part.
+// How a call is cut.  Rows of heads that share their keys go side by side into one
+// tile where they fit: the keys are then read once for all of them.  Calls that
+// leave half of the SMs idle split the keys, four tiles at least to a part.
+// (Splitting a last round that leaves many SMs idle gained nothing.)
 struct ForwardCut {
-  int packed, tiles, row_blocks, splits;
+  int packed, row_blocks, splits;
   long long units;
 };
 
 ForwardCut cut_forward(int batch, int heads, int kv_heads, int sq, int sk) {
-  ForwardCut c{1, 1, 1, 1, 0};
+  ForwardCut c{1, 1, 1, 0};
   const int group = heads / kv_heads;
-  for (int n = 2; n <= group; ++n)
-    if (group % n == 0 && static_cast<long long>(n) * sq <= kTile) c.packed = n;
-  const long long pairs = (sq + 2LL * kTile - 1) / (2 * kTile);
-  if (sq > kTile && pairs * batch * heads >= kNumSMs) c.tiles = 2;
-  c.row_blocks = static_cast<int>((sq + static_cast<long long>(c.tiles) * kTile - 1) / (c.tiles * kTile));
+  for (int n = 2; n <= group && static_cast<long long>(n) * sq <= kTile; ++n)
+    if (group % n == 0) c.packed = n;
+  c.row_blocks = (sq + kTile - 1) / kTile;
   c.units = static_cast<long long>(batch) * (heads / c.packed) * c.row_blocks;
-  if (c.units * 2 <= kNumSMs) {
+  if (c.units > 0 && c.units * 2 <= kNumSMs) {
     const long long most = (static_cast<long long>(sk) + 4 * kTile - 1) / (4 * kTile), fill = kNumSMs / c.units;
     c.splits = static_cast<int>(fill < most ? fill : most);
     if (c.splits < 1) c.splits = 1;
@@ -614,7 +659,7 @@ bool valid_attention(int batch, int heads, int kv_heads, int sq, int sk, int d) 
          d % 8 == 0 && sq <= 0x7ffffe00 && sk <= 0x7ffffe00;
 }
 
-long long part_rows(const ForwardCut& c) { return c.splits > 1 ? c.units * c.splits * c.tiles * kTile : 0; }
+long long part_rows(const ForwardCut& c) { return c.splits > 1 ? c.units * c.splits * kTile : 0; }
 
 template <int AB, int D>
 int launch_forward(const ForwardArgs& a, const ForwardCut& c, const CUtensorMap (&maps)[3], cudaStream_t stream) {
@@ -625,7 +670,7 @@ int launch_forward(const ForwardArgs& a, const ForwardCut& c, const CUtensorMap 
   const dim3 grid(static_cast<unsigned>(c.units * c.splits));
   if (int st = launch_overlapped(kernel, grid, dim3(kThreads), forward_smem<D>(), 0, stream, maps[0], maps[1], maps[2], a)) return st;
   if (c.splits == 1) return kOk;
-  return launch_overlapped(split_attention_kernel<AB>, dim3(static_cast<unsigned>(c.units * c.tiles * (kTile / 4))), dim3(128), 0,
+  return launch_overlapped(split_attention_kernel<AB>, dim3(static_cast<unsigned>(c.units * (a.packed > 1 ? a.packed * a.s.sq : a.s.sq < kTile ? a.s.sq : kTile))), dim3(128), 0,
                            0, stream, a);
 }
 
@@ -696,7 +741,6 @@ extern "C" int peco_span_attention(const void* q, const void* k, const void* v, 
   a.out_row = o.row;
   a.lse = lse;
   a.packed = c.packed;
-  a.tiles = c.tiles;
   a.row_blocks = c.row_blocks;
   a.splits = c.splits;
   a.part = static_cast<float*>(workspace);
