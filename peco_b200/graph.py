@@ -110,8 +110,9 @@ class PecoStepGraph:
             p.k_centroids = p.k_centroids.float().contiguous().clone()
             p.update_centroids_in_place = True
         # what the graph reads and writes and did not allocate itself lives as long as the graph, whatever the
-        # processors and the model take afterwards (another capture, a reset, another token grid)
-        self.kept = ([(p.q_centroids, p.k_centroids) for p in processors], getattr(model, "_rope", None))
+        # processors and the model take afterwards (another capture, a reset, another token grid, 16-bit layers again)
+        self.kept = ([(p.q_centroids, p.k_centroids) for p in processors], getattr(model, "_rope", None),
+                     [m.int8 for m in getattr(model, "modules", tuple)() if hasattr(m, "int8")])
         self.model = model
         self.frozen = (ctx.step, ctx.text_length, ctx.valid_text_length)
         self.inputs = tuple(t.detach().clone() if torch.is_tensor(t) else t for t in inputs)

@@ -47,9 +47,11 @@ import torch.distributed as dist
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .attention import attention, key_spans
+from .int8 import int8_weight, linear_int8, quantize_layer
 from .linear import is_plain_linear, linear_act, without_hooks
 from .norms import modulated_norm
-from .processor import InferenceContext, PecoAttention, PecoConfig
+from .processor import InferenceContext, PecoAttention, PecoConfig, _project
 from .rotary import AxialPositions
 
 
@@ -174,12 +176,12 @@ class SDPAProcessor(PecoAttention):
             return super().__call__(attn, hidden_states, encoder_hidden_states, attention_mask, image_rotary_emb)
         return self._torch_call(attn, hidden_states, encoder_hidden_states, image_rotary_emb)
 
-    def _torch_call(self, attn, video, text, rope):
+    def _torch_call(self, attn, video, text, rope, project=lambda layer, x: layer(x)):
         separate = attn.add_q_proj is not None
         n_text = 0 if text is None else text.shape[1]
 
         def heads_of(x, layers, norms):
-            q, k, v = (layer(x).unflatten(-1, (attn.heads, -1)).transpose(1, 2) for layer in layers)
+            q, k, v = (project(layer, x).unflatten(-1, (attn.heads, -1)).transpose(1, 2) for layer in layers)
             return norms[0](q), norms[1](k), v
 
         q, k, v = heads_of(video, (attn.to_q, attn.to_k, attn.to_v), (attn.norm_q, attn.norm_k))
@@ -198,10 +200,34 @@ class SDPAProcessor(PecoAttention):
             return video_out, text
         if attn.to_out is not None:
             for layer in attn.to_out:
-                video_out = layer(video_out)
+                video_out = project(layer, video_out)
         if attn.to_add_out is not None:
-            text_out = attn.to_add_out(text_out)
+            text_out = project(attn.to_add_out, text_out)
         return video_out, text_out
+
+
+class SpanProcessor(SDPAProcessor):
+    """Exact joint attention of one or several prompts on the package's own kernels, differentiable.
+
+    Every sample's rows are two documents, its video and valid text, and its
+    padding; ``context.valid_text_length`` is a number, or an int tensor [B] on
+    the model's device with one for each sample (read there: nothing is
+    synchronised).  For float16 / bfloat16 models on CUDA; training runs
+    through it where the block operators or plain layers do."""
+
+    def attention(self, query, key, value, value_ready=None, key_ready=None):
+        b, _, s, _ = query.shape
+        ends = torch.full((b, 3), s, dtype=torch.int32, device=query.device)
+        ends[:, 0] = 0
+        ends[:, 1] = s - self.context.text_length + self.context.valid_text_length
+        return attention(query, key, value, spans=key_spans(b, s, s, documents=ends))
+
+    def __call__(self, attn, hidden_states, encoder_hidden_states=None, attention_mask=None, image_rotary_emb=None):
+        if not torch.is_grad_enabled() and hidden_states.shape[0] == 1 and hidden_states.dtype == torch.bfloat16:
+            # inference of one prompt: the fused stage between projections and attention
+            return PecoAttention.__call__(self, attn, hidden_states, encoder_hidden_states, attention_mask, image_rotary_emb)
+        project = _project if getattr(attn, "block_operators", False) else (lambda layer, x: layer(x))
+        return self._torch_call(attn, hidden_states, encoder_hidden_states, image_rotary_emb, project)
 
 
 def rotate_pairs(x, cos, sin):
@@ -249,6 +275,9 @@ class Attention(nn.Module):
 def _linear(layer, x, activation=None):
     """activation(layer(x)); ``activation`` None or "gelu_tanh"."""
     if is_plain_linear(layer):
+        w8 = int8_weight(layer)
+        if w8 is not None:
+            return linear_int8(x, w8, layer.bias, activation=activation)
         return linear_act(x, layer.weight, layer.bias, activation=activation)
     y = layer(x)
     return y if activation is None else F.gelu(y, approximate="tanh")
@@ -265,9 +294,12 @@ def _row_operator(layer, x, gate, residual, x2=None):
     if not is_plain_linear(layer):
         return residual + gate[:, None] * layer(x if x2 is None else torch.cat((x, x2), -1))
     tp = getattr(layer, "tp", SINGLE)
+    w8 = int8_weight(layer)
     if tp.world == 1:
+        if w8 is not None:
+            return linear_int8(x, w8, layer.bias, gate=gate, residual=residual, x2=x2)
         return linear_act(x, layer.weight, layer.bias, gate=gate, residual=residual, x2=x2)
-    y = linear_act(x, layer.weight, x2=x2)
+    y = linear_act(x, layer.weight, x2=x2) if w8 is None else linear_int8(x, w8, x2=x2)
     dist.all_reduce(y, group=tp.group)
     return torch.addcmul(residual, gate[:, None], y + layer.bias)
 
@@ -466,7 +498,19 @@ class Pipe:
         self.transformer = transformer
 
 
-def use_block_operators(transformer, enabled=True, positions=False):
+def _block_linears(block):
+    """The layers of a block that its rows pass (not the modulation's, of one row a sample)."""
+    attn = block.attn
+    layers = [attn.to_q, attn.to_k, attn.to_v, attn.add_q_proj, attn.add_k_proj, attn.add_v_proj, attn.to_add_out,
+              *(attn.to_out or ())]
+    if isinstance(block, SingleStreamBlock):
+        layers += [block.proj_mlp, block.proj_out]
+    else:
+        layers += [*block.ff, *block.ff_context]
+    return [layer for layer in layers if layer is not None]
+
+
+def use_block_operators(transformer, enabled=True, positions=False, int8=False):
     """Run every block's norms, modulation, projections, MLPs, gates and
     residuals through ``modulated_norm`` and ``linear_act``.  For CUDA float16 /
     bfloat16 inference; the attention processors stay as installed (their
@@ -476,14 +520,27 @@ def use_block_operators(transformer, enabled=True, positions=False):
     tables.  The processor's bfloat16 entry turns by tables inside its pass over
     Q and K, whereas ``rotate`` is a pass of its own (135 us at 48 heads x 34680
     rows; a step of 60 such blocks 822.5 ms by tables, 824.4 ms by positions):
-    tables are the faster form where they exist."""
+    tables are the faster form where they exist.
+
+    ``int8``: the blocks' linear layers, the modulation's excepted, multiply in
+    8-bit integers (``linear_int8``; weights with a scale for each channel, laid
+    out here beside the 16-bit ones, rows with a scale each).  Inference only;
+    call it again after the weights change."""
     transformer.rotary_positions = enabled and positions
     for block in [*transformer.transformer_blocks, *transformer.single_transformer_blocks]:
         block.block_operators = enabled
         block.attn.block_operators = enabled
+        for layer in _block_linears(block):
+            if enabled and int8:
+                quantize_layer(layer)
+            elif hasattr(layer, "int8"):
+                del layer.int8
 
 
-def use_dense_attention(transformer, context: InferenceContext):
-    """Give every attention layer the exact SDPA processor (the dense baseline)."""
+def use_dense_attention(transformer, context: InferenceContext, spans=False):
+    """Give every attention layer the exact SDPA processor (the dense baseline),
+    or with ``spans`` the package's own exact attention (``SpanProcessor``), which
+    takes several prompts a call and trains."""
+    kind = SpanProcessor if spans else SDPAProcessor
     for block in [*transformer.transformer_blocks, *transformer.single_transformer_blocks]:
-        block.attn.set_processor(SDPAProcessor(context))
+        block.attn.set_processor(kind(context))

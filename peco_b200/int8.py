@@ -20,7 +20,7 @@ from typing import NamedTuple
 import torch
 
 from . import _native
-from .linear import ACTIVATIONS, _gate_rows, _rows, _weight_rows
+from .linear import ACTIVATIONS, _gate_rows, _rows, _weight_rows, is_plain_linear
 
 MAX_FEATURES = 131071  # 128 * 128 * K stays below 2^31
 _SIXTEEN_BITS = (torch.float16, torch.bfloat16)
@@ -174,3 +174,31 @@ def linear_int8(x, weight, bias=None, *, activation=None, gate=None, residual=No
                      ACTIVATIONS[activation], _native.DTYPE_CODE[dtype], _native.address(ws), max(need, 0)),
                     (None if given else x, x2, values, scales, w_values, w_scales, bias, gate, residual))
     return out
+
+
+class LayerInt8(NamedTuple):
+    """A layer's weight in 8-bit integers, and the parameter it was taken from."""
+
+    weight: QuantizedRows
+    source: torch.Tensor
+    version: int
+
+
+@torch.no_grad()
+def quantize_layer(layer) -> bool:
+    """Keep ``layer``'s weight in 8-bit integers beside it (``layer.int8``), where it is a plain linear layer on a CUDA
+    device in 16 bits; whether it is.  The 16-bit weight stays the layer's parameter."""
+    if not is_plain_linear(layer) or layer.weight.dtype not in _SIXTEEN_BITS or not layer.weight.is_cuda:
+        return False
+    layer.int8 = LayerInt8(quantize_rows(layer.weight), layer.weight, layer.weight._version)
+    return True
+
+
+def int8_weight(layer):
+    """The 8-bit weight that ``quantize_layer`` keeps with ``layer``, or None."""
+    kept = getattr(layer, "int8", None)
+    if not isinstance(kept, LayerInt8) or not is_plain_linear(layer):
+        return None
+    if kept.source is not layer.weight or kept.version != layer.weight._version:
+        raise RuntimeError("the layer's weight changed after it was quantised; quantise it again")
+    return kept.weight

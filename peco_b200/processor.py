@@ -30,6 +30,7 @@ import torch
 
 from . import _native
 from .clustering import kmeans_fit_pair, fit_token_clusters
+from .int8 import int8_weight, linear_int8, quantize_rows
 from .linear import is_plain_linear, linear_act
 from .rotary import AxialPositions
 
@@ -316,17 +317,19 @@ class PecoAttention:
         without tables (by a pass of its own: where there are tables, the
         fused pass turns by them at no cost).  A module with a true ``block_operators`` attribute has
         its projections run by ``linear.linear_act`` where they are plain
-        linear layers; others (adapted, quantised, with hooks) are called.
+        linear layers, or by ``int8.linear_int8`` where their weights are kept in
+        8-bit integers too (``int8.quantize_layer``); others (adapted, quantised
+        otherwise, with hooks) are called.
         """
         _native.require_cuda(hidden_states)
         n_text = 0 if encoder_hidden_states is None else encoder_hidden_states.shape[1]
         separate_text = attn.add_q_proj is not None  # dual-stream: text has its own weights
         heads = attn.heads
         project = _project if getattr(attn, "block_operators", False) else (lambda layer, x: layer(x))
-        video_proj = [project(layer, hidden_states) for layer in (attn.to_q, attn.to_k, attn.to_v)]
+        video_proj = _project_all(project, (attn.to_q, attn.to_k, attn.to_v), hidden_states)
         text_layers = (attn.add_q_proj, attn.add_k_proj, attn.add_v_proj) if separate_text else \
             (attn.to_q, attn.to_k, attn.to_v)
-        text_proj = [project(layer, encoder_hidden_states) for layer in text_layers] if n_text else [None] * 3
+        text_proj = _project_all(project, text_layers, encoder_hidden_states) if n_text else [None] * 3
         b, n_video, inner = video_proj[0].shape
         if b != 1:
             raise ValueError("This minimal HunyuanVideo entry supports one prompt per call")
@@ -380,7 +383,18 @@ def _project(layer, x):
     """``layer(x)``, through linear_act where that computes the same: a linear map of this rank alone, without hooks."""
     if not is_plain_linear(layer) or getattr(getattr(layer, "tp", None), "world", 1) > 1:
         return layer(x)
-    return linear_act(x, layer.weight, layer.bias)
+    w8 = int8_weight(layer)
+    return linear_act(x, layer.weight, layer.bias) if w8 is None else linear_int8(x, w8, layer.bias)
+
+
+def _project_all(project, layers, x):
+    """``project(layer, x)`` of layers that read the same rows, which are quantised once where all of them take 8 bits."""
+    if project is _project and all(getattr(getattr(layer, "tp", None), "world", 1) == 1 for layer in layers):
+        weights = [int8_weight(layer) for layer in layers]
+        if all(w is not None for w in weights):
+            rows = quantize_rows(x)
+            return [linear_int8(rows, w, layer.bias, dtype=x.dtype) for w, layer in zip(weights, layers)]
+    return [project(layer, x) for layer in layers]
 
 
 def _rms_gain(norm, dims):
