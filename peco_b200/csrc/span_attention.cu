@@ -118,11 +118,12 @@ __global__ void __launch_bounds__(kTile) key_spans_kernel(const SpanArgs a) {
 }
 
 // ---- forward ----------------------------------------------------------------------------
-constexpr int kSlots = 6;        // of K(t) in slot 2t mod 6, V(t) in slot 2t + 1 mod 6
+constexpr int kSlots = 3;        // tiles of K, and as many of V
+constexpr int kScores = 3;       // S buffers
 constexpr int kThreads = 384;    // two softmax warpgroups, one with the TMA warp and the MMA warp
 // A softmax thread holds a tile's 128 scores: the launch's 168 registers a thread
 // go 208 to 208 to 88 (256 * 208 + 128 * 88 = 384 * 168).
-constexpr uint32_t kTmemCols = 512;  // S of both warpgroups, then O of both
+constexpr uint32_t kTmemCols = 512;  // three tiles' S, then O
 
 struct ForwardArgs {
   ScoreArgs s;
@@ -138,15 +139,15 @@ struct ForwardArgs {
 };
 
 struct __align__(8) ForwardShared {
-  uint64_t q_full, slot_full[kSlots], slot_empty[kSlots], s_full[2], p_full[2], o_full[2];
+  uint64_t q_full, k_full[kSlots], k_empty[kSlots], v_full[kSlots], v_empty[kSlots], s_full[kScores], p_full[kScores], o_done[kScores], o_full, reference[2][4];
   uint32_t tmem;
   int abort_flag, masked;
-  float2 sums[kTile];       // of the odd key tiles' (maximum, sum)
+  float top[kTile];         // the maximum that O's rows stand on
 };
 
 template <int D>
-constexpr int forward_smem() { return 1024 + (1 + kSlots) * kTile * D * 2 + 1536; }
-static_assert(sizeof(ForwardShared) <= 1536 && forward_smem<128>() <= 227 * 1024, "shared memory of a CTA");
+constexpr int forward_smem() { return 1024 + (1 + 2 * kSlots) * kTile * D * 2 + 1024; }
+static_assert(sizeof(ForwardShared) <= 1024 && forward_smem<128>() <= 227 * 1024, "shared memory of a CTA");
 
 // Which head and query row thread ``r`` of a unit holds.
 struct Unit {
@@ -232,20 +233,27 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kPanels = D / 64, kTileBytes = kPanels * kPanelBytes;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  unsigned char* slots = base + kTileBytes;
-  ForwardShared& sh = *reinterpret_cast<ForwardShared*>(slots + kSlots * kTileBytes);
+  unsigned char* k_slots = base + kTileBytes;
+  unsigned char* v_slots = k_slots + kSlots * kTileBytes;
+  ForwardShared& sh = *reinterpret_cast<ForwardShared*>(v_slots + kSlots * kTileBytes);
   volatile int* abort_flag = &sh.abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(&sh.q_full, 1);
     for (int i = 0; i < kSlots; ++i) {
-      mbar_init(&sh.slot_full[i], 1);
-      mbar_init(&sh.slot_empty[i], 1);
+      mbar_init(&sh.k_full[i], 1);
+      mbar_init(&sh.k_empty[i], 1);
+      mbar_init(&sh.v_full[i], 1);
+      mbar_init(&sh.v_empty[i], 1);
     }
+    for (int i = 0; i < kScores; ++i) {
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_full[i], 4);
+      mbar_init(&sh.o_done[i], 1);
+    }
+    mbar_init(&sh.o_full, 1);
     for (int w = 0; w < 2; ++w) {
-      mbar_init(&sh.s_full[w], 1);
-      mbar_init(&sh.p_full[w], 4);
-      mbar_init(&sh.o_full[w], 1);
+      for (int i = 0; i < 4; ++i) mbar_init(&sh.reference[w][i], 1);
     }
     sh.abort_flag = 0;
     sh.masked = 0;
@@ -284,30 +292,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       load_rows<kPanels>(base, &qmap, unit.row0, unit.head0, unit.b, &sh.q_full);
     }
     __syncwarp();
-    for (int item = 0; item < 2 * ntiles && ok; ++item) {
-      const int s = item % kSlots, use = item / kSlots;
-      if (use > 0) ok = warp_wait(&sh.slot_empty[s], (use - 1) & 1, abort_flag, a.s.status);
+    auto load = [&](const CUtensorMap* map, unsigned char* slots, uint64_t* full, uint64_t* empty, RingPos& pos, int t) {
+      if (ok) ok = warp_wait(&empty[pos.s], pos.phase ^ 1, abort_flag, a.s.status);
       if (ok && issuer) {
-        mbar_arrive_expect_tx(&sh.slot_full[s], kTileBytes);
-        load_rows<kPanels>(slots + s * kTileBytes, item & 1 ? &vmap : &kmap, key0 + (item >> 1) * kTile, kv, unit.b,
-                           &sh.slot_full[s]);
+        mbar_arrive_expect_tx(&full[pos.s], kTileBytes);
+        load_rows<kPanels>(slots + pos.s * kTileBytes, map, key0 + t * kTile, kv, unit.b, &full[pos.s]);
       }
       __syncwarp();
+      pos.step(kSlots);
+    };
+    RingPos ks{0, 0}, vs{0, 0};
+    for (int t = 0; t < 2 && t < ntiles; ++t) load(&kmap, k_slots, sh.k_full, sh.k_empty, ks, t);
+    for (int t = 0; t < ntiles && ok; ++t) {
+      if (t + 2 < ntiles) load(&kmap, k_slots, sh.k_full, sh.k_empty, ks, t + 2);
+      load(&vmap, v_slots, sh.v_full, sh.v_empty, vs, t);
     }
     if (!ok) {  // time for the copies in flight to land before the CTA ends
       const unsigned long long t0 = globaltimer();
       while (globaltimer() - t0 < 2000000ull) {
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == 9 || warp == 10) {
     // ---------------------------------------------------------------- MMA
+    // One warp issues the scores, the other the products with V, so that neither's waits hold the other up.
     constexpr uint32_t idesc_qk = instr_desc(kTile, kTile, AB, false, false);
     constexpr uint32_t idesc_pv = instr_desc(kTile, D, AB, false, true);
     constexpr uint32_t kSlotStep = kTileBytes >> 4;
     const bool issuer = elect_one();
-    const uint32_t s_at = uniform(tmem), o_at = s_at + 2 * kTile;
-    const uint32_t q = uniform(desc_dims(smem_u32(base))), k = uniform(desc_dims(smem_u32(slots)));
-    const uint32_t v = uniform(desc_rows(smem_u32(slots)));
+    const uint32_t s_at = uniform(tmem), o_at = s_at + kScores * kTile;
     const int last = static_cast<int>(uniform(ntiles)) - 1;
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t phase) {
@@ -315,45 +327,39 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok) tc_fence_after();
       return ok;
     };
-    auto scores = [&](int w, int slot) {
-      if (issuer) {
-        product_dims<D>(s_at + w * kTile, q, k + slot * kSlotStep, idesc_qk);
-        umma_commit(&sh.s_full[w]);
-        umma_commit(&sh.slot_empty[slot]);
-      }
-      __syncwarp();
-    };
-    // keys past a unit's last are nobody's: their values may be anything
-    auto clear_unseen = [&](int t, int slot) {
-      const int seen = all_keys.y - (key0 + t * kTile);
-      if (seen < kTile) clear_rows<kPanels>(slots + slot * kTileBytes, seen, kTile, lane);
-    };
-    if (last >= 0) {
-      // K(t) is item 2t of the ring, V(t) item 2t + 1; the scores run two tiles ahead of the values
-      RingPos ks{0, 0}, vs{1, 0};
-      auto two_on = [](RingPos& p) {
-        p.step(kSlots);
-        p.step(kSlots);
-      };
-      wait(&sh.q_full, 0);
-      for (int t = 0; t < 2 && t <= last; ++t, two_on(ks))
-        if (wait(&sh.slot_full[ks.s], ks.phase)) scores(t, ks.s);
-      for (int t = 0; t <= last && ok; ++t, two_on(vs)) {
-        const int w = t & 1;
-        if (!wait(&sh.slot_full[vs.s], vs.phase)) break;
-        clear_unseen(t, vs.s);
-        if (!wait(&sh.p_full[w], (t >> 1) & 1)) break;
+    RingPos slot{0, 0}, buffer{0, 0};
+    if (warp == 9) {
+      const uint32_t q = uniform(desc_dims(smem_u32(base))), k = uniform(desc_dims(smem_u32(k_slots)));
+      if (last >= 0) wait(&sh.q_full, 0);
+      for (int t = 0; t <= last && ok; ++t) {
+        if (!wait(&sh.k_full[slot.s], slot.phase)) break;
+        // the buffer's last P has been read
+        if (t >= kScores && !wait(&sh.o_done[buffer.s], buffer.phase ^ 1)) break;
         if (issuer) {
-          product_rows<kTile>(o_at + w * kTile, s_at + w * kTile, v + vs.s * kSlotStep, idesc_pv, t > 1);
-          umma_commit(&sh.slot_empty[vs.s]);
-          if (t + 2 > last) umma_commit(&sh.o_full[w]);
+          product_dims<D>(s_at + buffer.s * kTile, q, k + slot.s * kSlotStep, idesc_qk);
+          umma_commit(&sh.s_full[buffer.s]);
+          umma_commit(&sh.k_empty[slot.s]);
         }
         __syncwarp();
-        if (t + 2 <= last) {
-          if (!wait(&sh.slot_full[ks.s], ks.phase)) break;
-          scores(w, ks.s);
-          two_on(ks);
+        slot.step(kSlots);
+        buffer.step(kScores);
+      }
+    } else {
+      const uint32_t v = uniform(desc_rows(smem_u32(v_slots)));
+      for (int t = 0; t <= last && ok; ++t) {
+        if (!wait(&sh.v_full[slot.s], slot.phase)) break;
+        const int seen = all_keys.y - (key0 + t * kTile);  // keys past a unit's last are nobody's: their values may be anything
+        if (seen < kTile) clear_rows<kPanels>(v_slots + slot.s * kTileBytes, seen, kTile, lane);
+        if (!wait(&sh.p_full[buffer.s], buffer.phase)) break;
+        if (issuer) {
+          product_rows<kTile>(o_at, s_at + buffer.s * kTile, v + slot.s * kSlotStep, idesc_pv, t > 0);
+          umma_commit(&sh.o_done[buffer.s]);
+          umma_commit(&sh.v_empty[slot.s]);
+          if (t == last) umma_commit(&sh.o_full);
         }
+        __syncwarp();
+        slot.step(kSlots);
+        buffer.step(kScores);
       }
     }
   }
@@ -361,9 +367,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ------------------------------------------------------- softmax, epilogue
     const int w = warp >> 2, r = threadIdx.x & (kTile - 1);
-    const int turns = (ntiles + 1 - w) >> 1;  // key tiles of this warpgroup
-    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + w * kTile + lanes, o_at = tmem + 2 * kTile + w * kTile + lanes;
+    const int quarter = warp & 3;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t o_at = tmem + kScores * kTile + lanes;
     int head, i;
     const bool real = unit.row(a, r, head, i);
     const int4 span = real ? span_of(a.s, unit.b, i) : make_int4(0, 0, 0, 0);
@@ -373,11 +379,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float slope = RICH && a.s.slopes && real ? a.s.slopes[head] * kLog2E : 0.0f;
     float m = -INFINITY, l = 0.0f;
     bool ok = true, masked = false;
-    for (int t = 0; t < turns; ++t) {
-      ok = warp_wait(&sh.s_full[w], t & 1, abort_flag, a.s.status);
+    int buffer = w, phase = 0;  // of the tile's S
+    for (int t = w; t < ntiles; t += 2) {
+      ok = warp_wait(&sh.s_full[buffer], phase, abort_flag, a.s.status);
       if (!ok) break;
       tc_fence_after();
-      const int j0 = key0 + (2 * t + w) * kTile;
+      const uint32_t s_at = tmem + buffer * kTile + lanes;
+      const int j0 = key0 + t * kTile;
       float s[kTile];
       {
         uint32_t raw[kTile];
@@ -418,25 +426,43 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int e = 0; e < c; ++e) mx[e] = fmaxf(mx[e], mx[e + c]);
       const float top = RICH ? mx[0] : mx[0] * scale_log2;
-      const bool grow = top > m + 8.0f || (m == -INFINITY && top > -INFINITY);
-      // the products of the tile before are complete: S came after them
-      const bool rescale = grow && m != -INFINITY;
-      if (t > 0 && __any_sync(0xffffffffu, rescale)) {
-        const float f = rescale ? exp2_approx(m - top) : 1.0f;
-        l *= f;
+      // what O stands on so far: the maximum that the tile before left
+      float before = -INFINITY;
+      if (t > 0) {
+        ok = warp_wait(&sh.reference[w ^ 1][quarter], ((t - 1) >> 1) & 1, abort_flag, a.s.status);
+        if (!ok) break;
+        before = sh.top[r];
+      }
+      const bool grow = top > before + 8.0f || (before == -INFINITY && top > -INFINITY);
+      const float now = grow ? top : before;
+      if (__any_sync(0xffffffffu, grow)) {
+        const bool rescale = grow && before != -INFINITY;
+        if (t > 0 && __any_sync(0xffffffffu, rescale)) {  // with the tile before in it
+          // (the phase before is over: S came after it)
+          ok = warp_wait(&sh.o_done[(t - 1) % kScores], (t - 1) / kScores & 1, abort_flag, a.s.status);
+          if (!ok) break;
+          tc_fence_after();
+          const float f = rescale ? exp2_approx(before - top) : 1.0f;
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t raw[32], part[16];
-          tmem_ld32_sync(o_at + c * 32, raw);
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t raw[32], part[16];
+            tmem_ld32_sync(o_at + c * 32, raw);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) part[e] = __float_as_uint(__uint_as_float(raw[h * 16 + e]) * f);
-            tmem_st16(o_at + c * 32 + h * 16, part);
+              for (int e = 0; e < 16; ++e) part[e] = __float_as_uint(__uint_as_float(raw[h * 16 + e]) * f);
+              tmem_st16(o_at + c * 32 + h * 16, part);
+            }
           }
+          tmem_st_wait();
+          tc_fence_before();
         }
       }
-      if (grow) m = top;
+      if (grow || t == 0) sh.top[r] = now;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.reference[w][quarter]);
+      if (now != m) l *= m == -INFINITY ? 0.0f : exp2_approx(m - now);
+      m = now;
       const float neg = m == -INFINITY ? 0.0f : -m;
       const float2 neg2 = make_float2(neg, neg), scale2 = make_float2(scale_log2, scale_log2);
       float2 sums[4];
@@ -449,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 0; e < 32; e += 2) {
           const float2 z = make_float2(s[c * 32 + e], s[c * 32 + e + 1]);
           const float2 x = RICH ? fadd2(z, neg2) : ffma2(z, scale2, neg2);
-          const float2 p = exp2_pair(e >> 1, x);
+          const float2 p = make_float2(exp2_approx(x.x), exp2_approx(x.y));
           sums[(e >> 1) & 3] = fadd2(sums[(e >> 1) & 3], p);
           packed[e >> 1] = pack2<T>(p.x, p.y);
         }
@@ -460,76 +486,54 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.p_full[w]);
-    }
-    if (ok && turns > 0) {
-      ok = warp_wait(&sh.o_full[w], 0, abort_flag, a.s.status);
-      tc_fence_after();
-    }
-    // the odd key tiles' result through shared memory (the slots, once both accumulators are
-    // complete): columns in fours, [fours][128 rows]
-    float own = 1.0f, other = 0.0f;  // factors of this accumulator and of the odd tiles'
-    const uint32_t exchange = smem_u32(slots) + r * 16;
-    if (w == 1 && turns > 0 && ok) {
-      ok = warp_wait(&sh.o_full[0], 0, abort_flag, a.s.status);
-      if (masked && lane == 0) sh.masked = 1;
-      sh.sums[r] = make_float2(m, l);
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t raw[32];
-        tmem_ld32_sync(o_at + c * 32, raw);
-#pragma unroll
-        for (int g = 0; g < 8; ++g)
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(exchange + (c * 8 + g) * kTile * 16), "r"(raw[4 * g]),
-                       "r"(raw[4 * g + 1]), "r"(raw[4 * g + 2]), "r"(raw[4 * g + 3])
-                       : "memory");
+      if (lane == 0) mbar_arrive(&sh.p_full[buffer]);
+      buffer += 2;
+      if (buffer >= kScores) {
+        buffer -= kScores;
+        phase ^= 1;
       }
     }
-    asm volatile("bar.sync 1, 256;" ::: "memory");  // (after an expired wait too)
-    if (w == 0 && ntiles > 1) {
-      masked = masked || sh.masked;
-      const float2 odd = sh.sums[r];
-      const float top = fmaxf(m, odd.x);
-      own = m == -INFINITY ? 0.0f : exp2_approx(m - top);
-      other = odd.x == -INFINITY ? 0.0f : exp2_approx(odd.x - top);
-      l = l * own + odd.y * other;
-      m = top;
+    if (ok && ntiles > 0) {
+      ok = warp_wait(&sh.o_full, 0, abort_flag, a.s.status);
+      tc_fence_after();
     }
-    if (ok && w == 0 && !*abort_flag) {
+    float2* sums = reinterpret_cast<float2*>(base);  // (maximum, sum) of each warpgroup, where Q was
+    sums[w * kTile + r] = make_float2(m, l);
+    if (masked && lane == 0) sh.masked = 1;
+    asm volatile("bar.sync 1, 256;" ::: "memory");  // (after an expired wait too)
+    if (ok && !*abort_flag) {
+      const float2 other = sums[(w ^ 1) * kTile + r];
+      const float last = ntiles > 0 ? sh.top[r] : -INFINITY;  // what O stands on
+      masked = sh.masked;
+      // the two in a fixed order
+      const float own = m == -INFINITY ? 0.0f : l * exp2_approx(m - last);
+      const float its = other.x == -INFINITY ? 0.0f : other.y * exp2_approx(other.x - last);
+      l = w == 0 ? own + its : its + own;
+      m = last;
       const bool whole = a.splits == 1;
       const float inv = !whole ? 1.0f : l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;  // (a NaN stays)
+      // each warpgroup stores half of the columns
+      constexpr int kHalf = D / 2;
       T* out = nullptr;
       float* part = nullptr;
       if (real && whole) {
         out = static_cast<T*>(a.out) + unit.b * a.out_batch + head * a.out_head + static_cast<long long>(i) * a.out_row;
-        a.lse[(static_cast<long long>(unit.b) * a.s.heads + head) * a.s.sq + i] =
-            l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+        if (w == 0)
+          a.lse[(static_cast<long long>(unit.b) * a.s.heads + head) * a.s.sq + i] =
+              l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
       } else if (real) {
         const long long at = static_cast<long long>(blockIdx.x) * kTile + r;
         part = a.part + at * a.s.d;
-        a.part_sums[at] = make_float2(m, l);
+        if (w == 0) a.part_sums[at] = make_float2(m, l);
       }
       bool finite = true;
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
+      for (int c = w * kHalf; c < (w + 1) * kHalf; c += 32) {
         uint32_t raw[32];
-        if (ntiles > 0) tmem_ld32_sync(o_at + c * 32, raw);
+        if (ntiles > 0) tmem_ld32_sync(o_at + c, raw);
         else
 #pragma unroll
           for (int e = 0; e < 32; ++e) raw[e] = 0u;
-        if (ntiles > 1) {
-#pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            float odd[4];
-            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                         : "=f"(odd[0]), "=f"(odd[1]), "=f"(odd[2]), "=f"(odd[3])
-                         : "r"(exchange + (c * 8 + g) * kTile * 16)
-                         : "memory");
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              raw[4 * g + e] = __float_as_uint(fmaf(odd[e], other, __uint_as_float(raw[4 * g + e]) * own));
-          }
-        }
         float2 v[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -541,15 +545,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (out) {
 #pragma unroll
           for (int g = 0; g < 4; ++g)
-            if (c * 32 + g * 8 < a.s.d)
-              *reinterpret_cast<uint4*>(out + c * 32 + g * 8) =
+            if (c + g * 8 < a.s.d)
+              *reinterpret_cast<uint4*>(out + c + g * 8) =
                   make_uint4(pack2<T>(v[4 * g].x, v[4 * g].y), pack2<T>(v[4 * g + 1].x, v[4 * g + 1].y),
                              pack2<T>(v[4 * g + 2].x, v[4 * g + 2].y), pack2<T>(v[4 * g + 3].x, v[4 * g + 3].y));
         } else if (part) {
 #pragma unroll
           for (int g = 0; g < 8; ++g)
-            if (c * 32 + g * 4 < a.s.d)
-              *reinterpret_cast<float4*>(part + c * 32 + g * 4) = make_float4(v[2 * g].x, v[2 * g].y, v[2 * g + 1].x, v[2 * g + 1].y);
+            if (c + g * 4 < a.s.d)
+              *reinterpret_cast<float4*>(part + c + g * 4) = make_float4(v[2 * g].x, v[2 * g].y, v[2 * g + 1].x, v[2 * g + 1].y);
         }
       }
       // (with a NaN or infinite sum the row sees such scores itself)
@@ -567,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int e = 0; e < D / 32; ++e) {
           const int c = lane + 32 * e;
-          if (c >= a.s.d) continue;
+          if (c >= a.s.d || c / kHalf != w) continue;
           if (whole)
             static_cast<T*>(a.out)[unit.b * a.out_batch + h2 * a.out_head + static_cast<long long>(i2) * a.out_row + c] =
                 from_f32<T>(acc[e] * f);
