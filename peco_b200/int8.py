@@ -80,12 +80,15 @@ def quantize_rows(x, x2=None) -> QuantizedRows:
 
 
 def _quantized(rows, what):
-    if not isinstance(rows, tuple) or len(rows) != 2 or not all(isinstance(t, torch.Tensor) for t in rows):
+    if not isinstance(rows, tuple) or len(rows) != 2:
         raise TypeError(f"{what} must be QuantizedRows(values, scales)")
     values, scales = rows
+    if not isinstance(values, torch.Tensor) or not isinstance(scales, torch.Tensor):
+        raise TypeError(f"{what} must be QuantizedRows(values, scales)")
     if values.dtype is not torch.int8 or scales.dtype is not torch.float32:
         raise TypeError(f"{what} must have int8 values and float32 scales")
-    if values.dim() < 1 or values.shape[-1] < 1 or scales.shape != values.shape[:-1]:
+    shape = values.shape
+    if not shape or shape[-1] < 1 or scales.shape != shape[:-1]:
         raise ValueError(f"{what} must have values [..., K] and scales [...] of one leading shape")
     return values, scales
 
@@ -121,33 +124,45 @@ def linear_int8(x, weight, bias=None, *, activation=None, gate=None, residual=No
         first, lead, dtype = x, x.shape[:-1], x.dtype
     operands = (None if given else x, x2, values, scales, w_values, w_scales, bias, gate, residual)
     _no_gradient("linear_int8", *operands)
-    if ACTIVATIONS.get(activation) is None:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"activation must be one of {sorted(a for a in ACTIVATIONS if a)} or None, got {activation!r}")
-    for t in (bias, gate, residual):
-        if t is not None and t.dtype is not dtype:
-            raise TypeError("bias, gate and residual must have the result's dtype")
     if w_values.dim() != 2 or w_values.shape[1] != k + k2 or w_values.shape[0] < 1:
         raise ValueError(f"weight values must be [N, {k + k2}] for these inputs, got {list(w_values.shape)}")
     n = w_values.shape[0]
-    if bias is not None and bias.shape != (n,):
-        raise ValueError(f"bias must be [{n}]")
     samples = 1
-    if gate is not None and gate.shape != (n,):
-        samples = lead[0] if len(lead) >= 2 else 1
-        if tuple(gate.shape) not in ((samples, n), (samples, 1, n)):
-            raise ValueError(f"gate must be [{n}] or one row for each of the {samples} samples, got {list(gate.shape)}")
-    if residual is not None and residual.shape != (*lead, n):
-        raise ValueError(f"residual must have the output's shape {[*lead, n]}")
-    device = _native.require_cuda(first, *(t for t in operands if t is not None))
+    if bias is not None:
+        if bias.dtype is not dtype:
+            raise TypeError("bias must have the result's dtype")
+        if bias.shape != (n,):
+            raise ValueError(f"bias must be [{n}]")
+    if gate is not None:
+        if gate.dtype is not dtype:
+            raise TypeError("gate must have the result's dtype")
+        if gate.shape != (n,):
+            samples = lead[0] if len(lead) >= 2 else 1
+            if tuple(gate.shape) not in ((samples, n), (samples, 1, n)):
+                raise ValueError(f"gate must be [{n}] or one row for each of the {samples} samples, got {list(gate.shape)}")
+    if residual is not None:
+        if residual.dtype is not dtype:
+            raise TypeError("residual must have the result's dtype")
+        if residual.shape != (*lead, n):
+            raise ValueError(f"residual must have the output's shape {[*lead, n]}")
+    device = first.device
+    if device.type != "cuda":
+        _native.require_cuda(first)
+    for t in operands:
+        if t is not None and t.device != device:
+            _native.require_cuda(first, t)
     out = torch.empty((*lead, n), dtype=dtype, device=device)
     rows = out.numel() // n
     if rows == 0:
         return out
-    xp = x2p = vp = x_step = x2_step = v_step = gp = g_step = rp = r_step = 0
+    xp = x2p = vp = x_step = x2_step = v_step = bp = gp = g_step = rp = r_step = sp = 0
     if given:
         values, v_step = _rows(values, k)
         scales = scales.contiguous()
-        vp = values.data_ptr()
+        vp, sp = values.data_ptr(), scales.data_ptr()
     else:
         x, x_step = _rows(x, k)
         xp = x.data_ptr()
@@ -158,6 +173,7 @@ def linear_int8(x, weight, bias=None, *, activation=None, gate=None, residual=No
     w_scales = w_scales.contiguous()
     if bias is not None:
         bias = bias.contiguous()
+        bp = bias.data_ptr()
     if gate is not None:
         gate, g_step = _gate_rows(gate, n, samples)
         gp = gate.data_ptr()
@@ -165,15 +181,22 @@ def linear_int8(x, weight, bias=None, *, activation=None, gate=None, residual=No
         residual, r_step = _rows(residual, n)
         rp = residual.data_ptr()
     lib = _native.load()
-    sizes = (samples, rows // samples, k, k2, n)
-    need = int(lib.peco_linear_int8_workspace(0 if given else 1, vp, v_step, w_values.data_ptr(), w_step, *sizes))
-    ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+    wp, per, need, ws = w_values.data_ptr(), rows // samples, 0, 0
+    # (quantised rows and weights on 16 bytes need no workspace)
+    if not given or _off_16_bytes(vp | wp, v_step | w_step):
+        need = int(lib.peco_linear_int8_workspace(0 if given else 1, vp, v_step, wp, w_step, samples, per, k, k2, n))
+        space = torch.empty(need, dtype=torch.uint8, device=device)
+        ws = space.data_ptr()
     _native.enqueue(device, "peco_linear_int8", lib.peco_linear_int8,
-                    (xp, x_step, x2p, x2_step, vp, v_step, _native.address(scales), w_values.data_ptr(), w_step,
-                     w_scales.data_ptr(), _native.address(bias), gp, g_step, rp, r_step, out.data_ptr(), n, *sizes,
-                     ACTIVATIONS[activation], _native.DTYPE_CODE[dtype], _native.address(ws), max(need, 0)),
+                    (xp, x_step, x2p, x2_step, vp, v_step, sp, wp, w_step, w_scales.data_ptr(), bp, gp, g_step, rp, r_step,
+                     out.data_ptr(), n, samples, per, k, k2, n, act, _native.DTYPE_CODE[dtype], ws, need),
                     (None if given else x, x2, values, scales, w_values, w_scales, bias, gate, residual))
     return out
+
+
+def _off_16_bytes(pointers: int, strides: int) -> bool:
+    """Whether some rows of bytes may not start on 16 bytes."""
+    return bool((pointers | strides) & 15)
 
 
 class LayerInt8(NamedTuple):
