@@ -64,7 +64,8 @@ def _check(got, ref, slack):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("rows,k", [(1, 1), (3, 7), (5, 64), (300, 1000), (9, 1024), (9, 1032), (17, 2048), (33, 2056),
-                                    (33, 4096), (6, 4104), (5, 8192), (3, 8200), (2, 16384), (2, 16392), (4, 1001)])
+                                    (33, 4096), (6, 4104), (5, 8192), (3, 8200), (2, 16384), (2, 16392), (4, 1001),
+                                    (2501, 2047), (7, 2049), (5, 4095), (3, 4097), (5000, 1024), (2700, 3000)])
 def test_integers_are_those_of_the_exact_quotient(rows, k, dtype):
     g = torch.Generator(device=DEV).manual_seed(rows * k)
     x = _normal(g, rows, k, std=0.3, dtype=dtype)
