@@ -49,15 +49,18 @@ class KeySpans:
     keys: int
 
 
+def _int32(t):
+    """Counts as contiguous int32; larger ones held to its range."""
+    return t.contiguous() if t.dtype is torch.int32 else t.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+
+
 def _ends(ends, batch, what):
     """Document ends as int32 [1 or batch, n + 1] rows."""
     if not isinstance(ends, torch.Tensor) or ends.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{what} must be an int32 or int64 tensor")
     if ends.dim() not in (1, 2) or ends.shape[-1] < 2 or ends.dim() == 2 and ends.shape[0] not in (1, batch):
         raise ValueError(f"{what} must be [n + 1] or one such row for each of the {batch} samples")
-    if ends.dtype is not torch.int32:
-        ends = ends.to(torch.int32)
-    ends = ends.contiguous()
+    ends = _int32(ends)
     return ends, ends.shape[1] if ends.dim() == 2 and ends.shape[0] > 1 else 0
 
 
@@ -105,7 +108,7 @@ def key_spans(batch, queries, keys, *, documents=None, key_documents=None, lengt
             raise TypeError("lengths must be an int32 or int64 tensor")
         if lengths.shape != (batch,):
             raise ValueError(f"lengths must be [{batch}]")
-        lengths = lengths.to(torch.int32).contiguous()
+        lengths = _int32(lengths)
         tensors.append(lengths)
     prefix_rows, prefix_all, prefix_batch, prefix_doc = None, 0, 0, 0
     if isinstance(prefix, torch.Tensor):
@@ -114,7 +117,7 @@ def key_spans(batch, queries, keys, *, documents=None, key_documents=None, lengt
         shape = tuple(prefix.shape)
         if shape not in ((max(n, 1),), (batch, 1), (batch, max(n, 1))):
             raise ValueError(f"prefix must be one number, [{max(n, 1)}], [{batch}, 1] or [{batch}, {max(n, 1)}]")
-        prefix_rows = prefix.to(torch.int32).contiguous()
+        prefix_rows = _int32(prefix)
         prefix_batch, prefix_doc = (shape[1] if len(shape) == 2 else 0), 1 if shape[-1] > 1 else 0
         tensors.append(prefix_rows)
     elif prefix is not None:
@@ -146,7 +149,7 @@ def _check(q, k, v, spans, scale, softcap, slopes):
     if not (isinstance(q, torch.Tensor) and isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor)
             and q.dim() == 4 and k.dim() == 4):
         raise ValueError("Expected q [B, H, N, D] and k, v [B, KV, M, D]")
-    dtype, device = q.dtype, q.device
+    dtype = q.dtype
     if dtype not in _SIXTEEN_BITS or k.dtype is not dtype or v.dtype is not dtype:
         raise TypeError("attention takes float16 or bfloat16 tensors of one dtype")
     b, h, n, d = q.shape
@@ -179,21 +182,38 @@ def _check(q, k, v, spans, scale, softcap, slopes):
         if spans.queries != n or spans.keys != m or spans.rows.shape[0] not in (1, b):
             raise ValueError(f"spans are for {spans.rows.shape[0]} samples of {spans.queries} rows and {spans.keys} keys, "
                              f"the call has {b} of {n} and {m}")
-    if device.type != "cuda" or k.device != device or v.device != device or (slopes is not None and slopes.device != device) \
-            or (spans is not None and spans.rows.device != device):
-        _native.require_cuda(q, k, v, *(t for t in (slopes, spans and spans.rows) if t is not None))
+        samples = spans.rows.shape[0]
+        if spans.rows.shape != (samples, n, 4) or spans.tiles.shape != (samples, -(-n // 128), 4) or \
+                spans.rows.dtype is not torch.int32 or spans.tiles.dtype is not torch.int32 or \
+                not spans.rows.is_contiguous() or not spans.tiles.is_contiguous():
+            raise ValueError("spans must be as key_spans lays them out")
     return (b, h, kv, n, m, d), scale, cap
 
 
+def _on_one_device(q, *others):
+    """The inputs' CUDA device."""
+    device = q.device
+    if device.type != "cuda":
+        _native.require_cuda(q)
+    for t in others:
+        if t is not None and t.device != device:
+            _native.require_cuda(q, t)
+    return device
+
+
+def _in_place(t) -> bool:
+    """Whether the kernels can read and write ``t`` as it lies: dims adjacent, every row, head and sample on 16 bytes."""
+    if t.data_ptr() & 15:
+        return False
+    if t.is_contiguous():
+        return True
+    steps = t.stride()
+    return steps[3] == 1 and all(n <= 1 or 0 < s < 1 << 38 and s % 8 == 0 for n, s in zip(t.shape[:3], steps[:3]))
+
+
 def _readable(t):
-    """``t`` with adjacent dims and every row on 16 bytes: itself, or a copy."""
-    if t.data_ptr() & 15 == 0:
-        if t.is_contiguous():
-            return t
-        sizes, steps = t.shape, t.stride()
-        if steps[3] == 1 and all(n <= 1 or 0 < s < 1 << 38 and s % 8 == 0 for n, s in zip(sizes[:3], steps[:3])):
-            return t
-    return t.clone(memory_format=torch.contiguous_format)
+    """``t``, or a copy of a layout that the kernels can read."""
+    return t if _in_place(t) else t.clone(memory_format=torch.contiguous_format)
 
 
 def _mask_args(spans, b):
@@ -204,13 +224,14 @@ def _mask_args(spans, b):
 
 def _forward(q, k, v, spans, scale, softcap, slopes):
     (b, h, kv, n, m, d), scale, cap = _check(q, k, v, spans, scale, softcap, slopes)
-    device = q.device
+    mask = (None, None) if spans is None else (spans.rows, spans.tiles)
+    device = _on_one_device(q, k, v, slopes, *mask)
     out = torch.empty_like(q)
     lse = torch.empty((b, h, n), dtype=torch.float32, device=device)
     if b == 0 or n == 0:
         return out, lse
     q, k, v, whole = _readable(q), _readable(k), _readable(v), out
-    if not out.is_contiguous() and _readable(out) is not out:
+    if not _in_place(out):
         whole = torch.empty(q.shape, dtype=q.dtype, device=device)
     if slopes is not None:
         slopes = slopes.contiguous()
@@ -219,11 +240,10 @@ def _forward(q, k, v, spans, scale, softcap, slopes):
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
     strides = _Strides(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *whole.stride()[:3])
     rows, tiles, batched = _mask_args(spans, b)
-    inputs = (q, k, v, slopes) if spans is None else (q, k, v, slopes, spans.rows, spans.tiles)
     _native.enqueue(device, "peco_span_attention", lib.peco_span_attention,
                     (q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, rows, tiles, batched, _native.address(slopes), scale,
                      cap, whole.data_ptr(), lse.data_ptr(), b, h, kv, n, m, d, _native.DTYPE_CODE[q.dtype],
-                     _native.address(ws), max(need, 0)), inputs)
+                     _native.address(ws), max(need, 0)), (q, k, v, slopes, *mask))
     return out.copy_(whole) if whole is not out else out, lse
 
 
@@ -294,13 +314,14 @@ def attention_backward(grad, q, k, v, out, lse, *, spans=None, scale=None, softc
     needs = ("q", "k", "v") if needs is None else tuple(needs)
     if set(needs) - {"q", "k", "v"}:
         raise ValueError(f"needs must name gradients of q, k and v, got {list(needs)}")
-    _native.require_cuda(q, grad, out, lse)
+    mask = (None, None) if spans is None else (spans.rows, spans.tiles)
+    device = _on_one_device(q, k, v, grad, out, lse, slopes, *mask)
     given = {"q": q, "k": k, "v": v}
     made = {name: torch.empty_like(t) for name, t in given.items() if name in needs}
     if not made:
         return AttentionGrads(None, None, None)
     # results whose layout TMA could not read are made elsewhere and copied
-    whole = {name: t if t.numel() == 0 or _readable(t) is t else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    whole = {name: t if t.numel() == 0 or _in_place(t) else torch.empty(t.shape, dtype=t.dtype, device=device)
              for name, t in made.items()}
     if b and (n or m):
         grad, q, k, v, out = (t if t.numel() == 0 else _readable(t) for t in (grad, q, k, v, out))
@@ -309,15 +330,15 @@ def attention_backward(grad, q, k, v, out, lse, *, spans=None, scale=None, softc
             slopes = slopes.contiguous()
         lib = _native.load()
         need = int(lib.peco_span_attention_backward_workspace(b, h, n))
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
         to = [whole.get(name) for name in "qkv"]
         strides = _GradStrides(*(s for t in (grad, q, k, v, out, *to) for s in (t.stride()[:3] if t is not None else (0, 0, 0))))
         rows, tiles, batched = _mask_args(spans, b)
-        _native.enqueue(q.device, "peco_span_attention_backward", lib.peco_span_attention_backward,
+        _native.enqueue(device, "peco_span_attention_backward", lib.peco_span_attention_backward,
                         (grad.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), strides,
                          rows, tiles, batched, _native.address(slopes), scale, cap, *(_native.address(t) for t in to), b, h,
                          kv, n, m, d, _native.DTYPE_CODE[q.dtype], _native.address(ws), max(need, 0)),
-                        (grad, q, k, v, out, lse, slopes, *((spans.rows, spans.tiles) if spans is not None else ())))
+                        (grad, q, k, v, out, lse, slopes, *mask))
     for name, t in made.items():
         if whole[name] is not t:
             t.copy_(whole[name])

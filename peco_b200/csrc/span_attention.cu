@@ -10,25 +10,25 @@
 //
 // A CTA takes a tile of 128 query rows of one head (or rows of several heads that
 // share their keys, side by side); two warpgroups take its even and its odd key
-// tiles, each with its own running maximum, sum and accumulator, joined at the
-// end.  Per tile of 128 keys:
-//   S = Q K^T        tcgen05.mma, both in shared memory, S in TMEM
-//   P = 2^(z - m)    a query row a thread; m, the running maximum, is raised only
-//                    when it grows by more than 2^8, and O rescaled
+// tiles.  Per tile of 128 keys:
+//   S = Q K^T        tcgen05.mma, both in shared memory, into one of three buffers in TMEM
+//   P = 2^(z - m)    a query row a thread; m, the row's running maximum, goes from
+//                    tile to tile through shared memory and is raised only when it
+//                    grows by more than 2^8, O rescaled then
 //   O += P V         tcgen05.mma, P from TMEM (over S, as 16-bit pairs)
-// While one warpgroup's softmax runs, the tensor core works for the other.  A
-// tile's next S overwrites the P that O's product before it reads: products that
-// one thread issues are executed in the order of their issue.  K and V stream
-// through six shared-memory slots by TMA.
+// Scores run two tiles ahead of the softmax, issued by a warp of their own; a
+// second one issues the products with V.  K and V stream through three
+// shared-memory slots each by TMA.  Whatever is written over is waited for.
 //
-// What it measured (B200, bf16): 24 heads x 7006 rows x 128 dims, every key: 565 us
-// (1.02 PFLOP/s; about 606 us at the power limit after 300 calls in a row), 64 dims 467
-// us; causal, 24 query heads on 4, 4096 rows 146 us; one row of 24 heads on 4, four
-// samples of up to 16384 keys 32 us.  Two tiles of rows with the same key tile instead,
-// which halves the traffic from L2, took as long on full masks and more on others
-// (causal 150, clips packed in causal order 102 us against 89).  Bound by a tile's
-// round trip: 1500 clocks of softmax and 1000 of products, 1670 a tile with two in
-// flight (without the softmax 375 us, without the products 405).
+// What it measured (B200, bf16): 24 heads x 7006 rows x 128 dims, every key: 490 us
+// (1.18 PFLOP/s; 535 us at the power limit after 300 calls in a row), 64 dims 423 us;
+// causal, 24 query heads on 4, 4096 rows 123 us; one row of 24 heads on 4, four samples of
+// up to 16384 keys 34 us.  Tensor core and special-function unit are both 62% busy:
+// the two warps of a scheduler do not hide all of each other's maxima, TMEM loads
+// and hand-offs.  Before, with a maximum, sum and accumulator for each warpgroup
+// 563 us, and with one warp that issued all products 536 us; two tiles of rows a
+// CTA in place of two of keys, which halves the traffic from L2, took as long on full
+// masks and more on others (clips packed in causal order 102 us against 89).
 #include "span_attention.cuh"
 #include "../../include/peco_b200.h"
 #include "internal.h"
@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kTile) key_spans_kernel(const SpanArgs a) {
     hi = inside ? k1 : k0;
     if (a.causal) {
       const int prefix = a.prefix ? a.prefix[b * a.prefix_batch + doc * a.prefix_doc] : a.prefix_all;
-      hi = min(hi, max(pos + 1, k0 + clamped(prefix, 0, a.keys)));
+      hi = min(hi, max(pos + 1, k0 + clamped(prefix, 0, a.keys - k0)));
     }
     if (a.window > 0) {
       lo = max(lo, static_cast<int>(max(static_cast<long long>(pos) - a.window + 1, 0LL)));
@@ -506,8 +506,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float last = ntiles > 0 ? sh.top[r] : -INFINITY;  // what O stands on
       masked = sh.masked;
       // the two in a fixed order
-      const float own = m == -INFINITY ? 0.0f : l * exp2_approx(m - last);
-      const float its = other.x == -INFINITY ? 0.0f : other.y * exp2_approx(other.x - last);
+      const float own = m == -INFINITY ? l : l * exp2_approx(m - last);  // without a maximum: 0, or NaN of NaN scores
+      const float its = other.x == -INFINITY ? other.y : other.y * exp2_approx(other.x - last);
       l = w == 0 ? own + its : its + own;
       m = last;
       const bool whole = a.splits == 1;

@@ -91,32 +91,6 @@ __device__ __forceinline__ void tmem_ld128_sync(uint32_t at, uint32_t (&r)[128])
       : "memory");
 }
 
-// 2^x of a pair on the fused multiply-add pipe, which has time left where the
-// special-function unit (16 a clock and SM) has not: x = n + f with n its nearest
-// integer, 2^f by a polynomial (own fit on |f| <= 1/2: relative error 2^-23.5, 2^-22.5 as
-// evaluated, as good as the unit's), times 2^n.  x up to 127; below -126.5 it is
-// 0, a NaN stays.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-  auto both = [](float v) { return make_float2(v, v); };
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));  // -127
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
-  const float2 t = fadd2(x, both(12582912.0f));         // n in the low bits
-  const float2 n = fadd2(t, both(-12582912.0f));
-  const float2 f = ffma2(n, both(-1.0f), x);
-  float2 p = ffma2(f, both(0.001327398233115673f), both(0.009671970270574093f));
-  p = ffma2(f, p, both(0.05550680309534073f));
-  p = ffma2(f, p, both(0.24022234976291656f));
-  p = ffma2(f, p, both(0.6931470632553101f));
-  p = ffma2(f, p, both(1.0f));
-  return fmul2(p, make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
-                              __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u)));
-}
-// A pair of a run of pairs: of every eight, ``kPolyPairs`` by the polynomial.
-constexpr int kPolyPairs = 1;
-__device__ __forceinline__ float2 exp2_pair(int pair, float2 x) {  // ``pair`` known when compiled
-  return (pair & 7) * kPolyPairs % 8 < kPolyPairs ? exp2_poly(x) : make_float2(exp2_approx(x.x), exp2_approx(x.y));
-}
-
 __device__ __forceinline__ void tile_load_4d(void* dst, const CUtensorMap* map, int x, int row, int head, int batch,
                                              uint64_t* bar) {
   asm volatile(

@@ -9,6 +9,13 @@
 // query rows walk the keys and keep dq.  Scores and g.v are computed in both,
 // seven products instead of five; in exchange no sum crosses a CTA: there are no
 // atomics, no fp32 copy of dq in memory, and results do not depend on the launch.
+//
+// What it measured (B200, bf16): 24 heads x 7006 rows x 128 dims, every key: 1615 us (0.90
+// PFLOP/s of five products, 1.25 of the seven; 1.8 ms at the power limit after 300
+// calls in a row), of it the CTAs of keys 990, those of rows 660; tensor pipe 65%. In the
+// CTAs of keys every product waits for the one whose operand it overwrites, and so
+// for the softmax between; issuing S right behind dv's product (1640 us), or the two
+// chains by a warp each (1680 us), was slower, although both wait less.
 #include "span_attention.cuh"
 #include "../../include/peco_b200.h"
 #include "internal.h"
@@ -47,13 +54,13 @@ __global__ void __launch_bounds__(256) grad_stats_kernel(const __grid_constant__
   using T = Element<AB>;
   wait_for_prior();
   let_next_start();
-  const long long at = static_cast<long long>(blockIdx.x) * 16 + (threadIdx.x >> 4);
-  const long long heads = at / a.padded;
-  const int i = static_cast<int>(at - heads * a.padded), lane = threadIdx.x & 15;
-  const int b = static_cast<int>(heads / a.s.heads), h = static_cast<int>(heads - static_cast<long long>(b) * a.s.heads);
+  const unsigned blocks = static_cast<unsigned>(a.padded) >> 4, heads = blockIdx.x / blocks;  // of a head; head of all samples
+  const int i = static_cast<int>((blockIdx.x - heads * blocks) * 16 + (threadIdx.x >> 4)), lane = threadIdx.x & 15;
+  const int b = static_cast<int>(heads / a.s.heads), h = static_cast<int>(heads % a.s.heads);
+  const long long at = static_cast<long long>(heads) * a.padded + i;
   float sum = 0.0f, l = -INFINITY;
-  if (b < a.s.batch && i < a.s.sq) {
-    l = a.lse[heads * a.s.sq + i];
+  if (i < a.s.sq) {
+    l = a.lse[static_cast<long long>(heads) * a.s.sq + i];
     if (lane * 8 < a.s.d) {
       float x[8], y[8];
       load8(static_cast<const T*>(a.out.ptr) + b * a.out.batch + h * a.out.head + static_cast<long long>(i) * a.out.row + lane * 8, 1, 8, x);
@@ -64,7 +71,7 @@ __global__ void __launch_bounds__(256) grad_stats_kernel(const __grid_constant__
   }
 #pragma unroll
   for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0 && b < a.s.batch)
+  if (lane == 0)
     a.stats[at] = l == -INFINITY ? make_float2(INFINITY, 0.0f) : make_float2(l * kLog2E - Held<AB>::kShift, sum * Held<AB>::kBack);
 }
 
@@ -82,7 +89,7 @@ struct __align__(16) GradShared {
   Step<RICH> step[2];
   uint64_t own_full;                              // the CTA's own two tiles
   uint64_t first_full[3], first_empty[3], second_full[2], second_empty[2], step_full[2], step_empty[2];
-  uint64_t s_full[2], p_full, dp_full, dp_free, ds_full[2], dq_done[2], done;
+  uint64_t s_full[2], p_full, dp_full, dp_free, ds_full[2], dq_done[2], p_read, ds_read, done;
   uint32_t tmem;
   int first, last, abort_flag;
 };
@@ -220,6 +227,8 @@ __global__ void __launch_bounds__(kGradThreads, 1)
     mbar_init(&sh.p_full, 8);
     mbar_init(&sh.dp_full, 1);
     mbar_init(&sh.dp_free, 8);
+    mbar_init(&sh.p_read, 1);
+    mbar_init(&sh.ds_read, 1);
     mbar_init(&sh.done, 1);
     sh.abort_flag = 0;
     sh.first = 0x7fffffff;
@@ -322,7 +331,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
                 // whether the row sees anything at all is told apart by the order of the two
                 reinterpret_cast<uint16_t*>(step.range)[e + lane] =
                     static_cast<uint16_t>(sp.y > sp.x ? from | to << 8 : 255 | 0 << 8);
-                if constexpr (RICH) step.pos[e + lane] = static_cast<float>(sp.z);
+                if constexpr (RICH) step.pos[e + lane] = static_cast<float>(sp.z - j0);  // from the tile's first key
               }
             }
             if (lane == 0) {
@@ -389,20 +398,23 @@ __global__ void __launch_bounds__(kGradThreads, 1)
           if (issuer) {
             product_rows<kTile>(dv_to, s_to, g_rows + g_slot * kTileStep, kRows, n > 0);
             umma_commit(&sh.second_empty[g_slot]);
+            umma_commit(&sh.p_read);
           }
           __syncwarp();
           f.step(kFirsts);
           s.step(kSecond);
           more = ready(n + 1, f, s);
+          if (more && !me.wait(&sh.p_read, n)) break;  // S goes where the probabilities were
           if (more) scores();
           if (!me.wait(&sh.ds_full[0], n)) break;
           if (issuer) {
             product_rows<kTile>(dk_to, dp_to, q_rows + q_slot * kTileStep, kRows, n > 0);
             umma_commit(&sh.first_empty[q_slot]);
             umma_commit(&sh.step_empty[n & 1]);
-            if (!more) umma_commit(&sh.done);
+            umma_commit(more ? &sh.ds_read : &sh.done);
           }
           __syncwarp();
+          if (more && !me.wait(&sh.ds_read, n)) break;  // g.v goes where ds was
           if (more) values();
         }
       }
@@ -411,7 +423,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
       // -------------------------------------------------------------- probabilities; a key a thread
       const int j = j0 + r;
       const Cap cap(a.s);
-      const float at_key = static_cast<float>(j);
+      const float at_key = static_cast<float>(r);
       const uint32_t s_own = s_at + lanes + half * 64, dp_own = dp_at + lanes + half * 64;
       int n = 0;
       for (; any; ++n) {
@@ -688,7 +700,7 @@ int launch_grad(const GradArgs& a, const CUtensorMap (&maps)[4], cudaStream_t st
   if (cudaError_t e = grant_smem(reinterpret_cast<const void*>(kernel), smem, granted[rich])) return static_cast<int>(e);
   if (a.s.sq > 0) {
     const long long rows = static_cast<long long>(a.s.batch) * a.s.heads * a.padded;
-    if (int st = launch_overlapped(grad_stats_kernel<AB>, dim3(static_cast<unsigned>((rows + 15) / 16)), dim3(256), 0, 0, stream, a)) return st;
+    if (int st = launch_overlapped(grad_stats_kernel<AB>, dim3(static_cast<unsigned>(rows / 16)), dim3(256), 0, 0, stream, a)) return st;
   }
   return launch_overlapped(kernel, dim3(a.key_units + a.query_units), dim3(kGradThreads), smem, 0, stream, maps[0],
                            maps[1], maps[2], maps[3], a);
@@ -762,7 +774,7 @@ extern "C" int peco_span_attention_backward(const void* grad, const void* q, con
   a.v_row = t[7].row;
   const long long key_units = keys ? static_cast<long long>(batch) * kv_heads * ((sk + kTile - 1) / kTile) : 0;
   const long long query_units = rows ? static_cast<long long>(batch) * heads * (a.padded / kTile) : 0;
-  const long long stat_blocks = (static_cast<long long>(batch) * heads * a.padded + 15) / 16;
+  const long long stat_blocks = static_cast<long long>(batch) * heads * a.padded / 16;
   if (key_units + query_units > 0x7fffffffLL || stat_blocks > 0x7fffffffLL) return kErrUnsupported;
   a.key_units = static_cast<int>(key_units);
   a.query_units = static_cast<int>(query_units);

@@ -530,11 +530,12 @@ def use_block_operators(transformer, enabled=True, positions=False, int8=False):
     for block in [*transformer.transformer_blocks, *transformer.single_transformer_blocks]:
         block.block_operators = enabled
         block.attn.block_operators = enabled
-        for layer in _block_linears(block):
-            if enabled and int8:
-                quantize_layer(layer)
-            elif hasattr(layer, "int8"):
+        for layer in block.modules():
+            if "int8" in vars(layer):
                 del layer.int8
+        if enabled and int8:
+            for layer in _block_linears(block):
+                quantize_layer(layer)
 
 
 def use_dense_attention(transformer, context: InferenceContext, spans=False):

@@ -154,6 +154,37 @@ def test_masked_keys_and_values_may_hold_anything(bad):
     assert _native.device_status(clear=True) == 0
 
 
+def test_what_a_row_sees_reaches_it():
+    """NaN in a query row, or in a key that a row sees, makes that row NaN and no other; also in parts of split keys."""
+    for h, kv, n, m in ((2, 2, 300, 500), (4, 1, 2, 5000), (2, 2, 3, 60), (2, 1, 130, 129)):
+        spans, seen, pos = plan(1, n, m, causal=True, window=200)
+        q, k, v = inputs(23, 1, h, kv, n, m, 64)
+        clean = attention(q, k, v, spans=spans, return_lse=True)
+        for args in ({}, dict(softcap=9.0)):
+            bad_q, bad_k = q.clone(), k.clone()
+            bad_q[:, 0, n // 2, 3] = float("nan")
+            out, lse = attention(bad_q, k, v, spans=spans, return_lse=True, **args)
+            row = torch.zeros(1, h, n, dtype=torch.bool, device=DEV)
+            row[:, 0, n // 2] = seen[0, n // 2].any()
+            assert torch.equal(lse.isnan(), row) and torch.equal(out.isnan().all(-1), row) and torch.equal(out.isnan().any(-1), row)
+            bad_k[:, :, m - 20, 5] = float("nan")
+            out, lse = attention(q, bad_k, v, spans=spans, return_lse=True, **args)
+            row = seen[:, None, :, m - 20].expand(1, h, n)
+            assert row.any() and torch.equal(lse.isnan(), row) and torch.equal(out.isnan().all(-1), row)
+            if not args:
+                assert torch.equal(out[~row], clean[0][~row]) and torch.equal(lse[~row], clean[1][~row])
+
+
+def test_wide_offsets():
+    ends = torch.tensor([0, 70, 2 ** 40], device=DEV)  # the last document ends with the sequence
+    spans = key_spans(1, 100, 100, documents=ends, causal=True, prefix=torch.tensor([2 ** 33, 5], device=DEV))
+    same = key_spans(1, 100, 100, documents=torch.tensor([0, 70, 100], dtype=torch.int32, device=DEV), causal=True,
+                     prefix=torch.tensor([100, 5], device=DEV))
+    assert torch.equal(spans.rows, same.rows) and torch.equal(spans.tiles, same.tiles)
+    lengths = key_spans(2, 3, 50, lengths=torch.tensor([2 ** 35, -2 ** 40], device=DEV))
+    assert lengths.rows[0, :, 1].tolist() == [50] * 3 and lengths.rows[1, :, 1].tolist() == [0] * 3
+
+
 def test_scores_at_the_ends_of_their_range():
     q, k, v = inputs(2, 1, 2, 2, 140, 200, 64, std=8.0)  # scores of some hundreds
     spans, seen, pos = plan(1, 140, 200, causal=True)
