@@ -16,6 +16,8 @@
 // CTAs of keys every product waits for the one whose operand it overwrites, and so
 // for the softmax between; issuing S right behind dv's product (1640 us), or the two
 // chains by a warp each (1680 us), was slower, although both wait less.
+// Under two documents 1600 us: a warp reads each step's statistics and spans while the
+// place for them is still in use (read after it was free: 1890 us).
 #include "span_attention.cuh"
 #include "../../include/peco_b200.h"
 #include "internal.h"
@@ -313,31 +315,43 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         // ------------------------------------------------------------ statistics of each step
         for (int n = 0;; ++n) {
           const bool more = walk.next(a.s, b, j0, first, last, (kv + 1) * group);
-          Step<RICH>& step = sh.step[n & 1];
-          if (!me.wait(&sh.step_empty[n & 1], (n >> 1) + 1)) break;
+          // read before the place is free, so that only the stores follow the step before
+          constexpr int kEach = kTile / 32;
+          float2 stat[kEach];
+          int4 span[kEach];
+          bool full = true, blind = false;
           if (more) {
             const int i0 = walk.tile * kTile;
             const int4 t = tile_span(a.s, b, walk.tile);
-            const bool full = t.z <= j0 && t.w >= min(j0 + kTile, a.s.sk) && i0 + kTile <= a.s.sq;
+            full = t.z <= j0 && t.w >= min(j0 + kTile, a.s.sk) && i0 + kTile <= a.s.sq;
+            blind = t.z == 0x7fffffff;  // some row sees nothing
             const float2* stats = a.stats + (static_cast<long long>(b) * a.s.heads + walk.head) * a.padded + i0;
 #pragma unroll
-            for (int e = 0; e < kTile; e += 32) {
-              const float2 f = stats[e + lane];
-              step.lse[e + lane] = f.x;
-              step.delta[e + lane] = f.y;
+            for (int e = 0; e < kEach; ++e) {
+              const int i = i0 + e * 32 + lane;
+              stat[e] = stats[e * 32 + lane];
+              span[e] = (RICH || !full) && i < a.s.sq ? span_of(a.s, b, i) : make_int4(0, 0, 0, 0);
+            }
+          }
+          Step<RICH>& step = sh.step[n & 1];
+          if (!me.wait(&sh.step_empty[n & 1], (n >> 1) + 1)) break;
+          if (more) {
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+              const int i = e * 32 + lane;
+              step.lse[i] = stat[e].x;
+              step.delta[i] = stat[e].y;
               if (RICH || !full) {
-                const int4 sp = i0 + e + lane < a.s.sq ? span_of(a.s, b, i0 + e + lane) : make_int4(0, 0, 0, 0);
-                const int from = min(max(sp.x - j0, 0), kTile), to = min(max(sp.y - j0, 0), kTile);
-                // whether the row sees anything at all is told apart by the order of the two
-                reinterpret_cast<uint16_t*>(step.range)[e + lane] =
-                    static_cast<uint16_t>(sp.y > sp.x ? from | to << 8 : 255 | 0 << 8);
-                if constexpr (RICH) step.pos[e + lane] = static_cast<float>(sp.z - j0);  // from the tile's first key
+                const int from = min(max(span[e].x - j0, 0), kTile), to = min(max(span[e].y - j0, 0), kTile);
+                // a row that sees nothing at all is told apart by the order of the two
+                reinterpret_cast<uint16_t*>(step.range)[i] = static_cast<uint16_t>(span[e].y > span[e].x ? from | to << 8 : 255);
+                if constexpr (RICH) step.pos[i] = static_cast<float>(span[e].z - j0);  // from the tile's first key
               }
             }
             if (lane == 0) {
               step.head = walk.head;
               step.masked = full ? 0 : 1;
-              step.clear = t.z == 0x7fffffff ? 1 : 0;  // some row sees nothing
+              step.clear = blind ? 1 : 0;
             }
           }
           if (lane == 0) step.end = more ? 0 : 1;
