@@ -336,7 +336,8 @@ int peco_span_attention(const void* q, const void* k, const void* v, const long 
 long long peco_span_attention_workspace(int batch, int heads, int kv_heads, int sq, int sk, int d);
 
 /* Gradients of peco_span_attention for ``grad`` = d out, with its result ``out``
- * and ``lse`` (null outputs: not computed).  strides (host memory): batch, head
+ * and ``lse`` (null outputs: not computed); ``spans`` of the workspace: whether
+ * there are any.  strides (host memory): batch, head
  * and row strides of grad, q, k, v, out, dq, dk and dv.  Sums run in a fixed
  * order; the probabilities and their gradients are rounded to the operands'
  * type for the products. */
@@ -345,7 +346,8 @@ int peco_span_attention_backward(const void* grad, const void* q, const void* k,
                                  int spans_batched, const float* slopes, float scale, float cap, void* dq, void* dk,
                                  void* dv, int batch, int heads, int kv_heads, int sq, int sk, int d, int dtype,
                                  void* workspace, long long workspace_bytes, void* stream);
-long long peco_span_attention_backward_workspace(int batch, int heads, int sq);
+long long peco_span_attention_backward_workspace(int batch, int heads, int kv_heads, int sq, int sk, int d,
+                                                 int spans);
 
 /* Gated residual and norm: with b = post_norm(branch) * post_weight,
  *   residual = residual_scale * x + gate * b

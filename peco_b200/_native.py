@@ -55,7 +55,7 @@ _SIGNATURES = {
     "peco_span_attention": [P] * 6 + [I, P, F, F, P, P] + [I] * 7 + [P, LL, P],
     "peco_span_attention_workspace": [I] * 6,
     "peco_span_attention_backward": [P] * 9 + [I, P, F, F, P, P, P] + [I] * 7 + [P, LL, P],
-    "peco_span_attention_backward_workspace": [I] * 3,
+    "peco_span_attention_backward_workspace": [I] * 7,
     "peco_gated_norm": [P, LL, LL] * 2 + [P, LL] * 3 + [P] * 4 + [I] * 5 + [F] * 3 + [I, P],
     "peco_gated_norm_backward": [P, LL, LL] * 4 + [P, LL] * 2 + [P] * 7 + [I] + [P] * 2 + [I] * 5 + [F] * 3
     + [I, P, LL, P],

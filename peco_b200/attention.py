@@ -329,7 +329,7 @@ def attention_backward(grad, q, k, v, out, lse, *, spans=None, scale=None, softc
         if slopes is not None:
             slopes = slopes.contiguous()
         lib = _native.load()
-        need = int(lib.peco_span_attention_backward_workspace(b, h, n))
+        need = int(lib.peco_span_attention_backward_workspace(b, h, kv, n, m, d, 0 if spans is None else 1))
         ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
         to = [whole.get(name) for name in "qkv"]
         strides = _GradStrides(*(s for t in (grad, q, k, v, out, *to) for s in (t.stride()[:3] if t is not None else (0, 0, 0))))

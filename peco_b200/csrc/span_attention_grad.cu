@@ -41,6 +41,8 @@ struct GradArgs {
   void *dq, *dk, *dv;
   long long q_batch, q_head, q_row, k_batch, k_head, k_row, v_batch, v_head, v_row;
   int key_units, query_units;
+  int parts;                 // CTAs that share a tile of keys, each some of the heads on them
+  float* part;               // with several: dv, then dk, [parts, batch, key heads, keys, dims] each
 };
 
 // fp16's small probabilities would lose bits below 2^-14: they are held 2^10
@@ -172,6 +174,27 @@ __device__ __forceinline__ void store_row(T* out, uint32_t at, float scale, int 
   }
 }
 
+// The same in fp32, for the sum over the parts
+template <int D>
+__device__ __forceinline__ void store_part(float* out, uint32_t at, float scale, int d, bool any) {
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t raw[32];
+    if (any) tmem_ld32_sync(at + c * 32, raw);
+    else
+#pragma unroll
+      for (int e = 0; e < 32; ++e) raw[e] = 0u;
+    if (out) {
+#pragma unroll
+      for (int g = 0; g < 8; ++g)
+        if (c * 32 + g * 4 < d)
+          *reinterpret_cast<float4*>(out + c * 32 + g * 4) =
+              make_float4(__uint_as_float(raw[g * 4]) * scale, __uint_as_float(raw[g * 4 + 1]) * scale,
+                          __uint_as_float(raw[g * 4 + 2]) * scale, __uint_as_float(raw[g * 4 + 3]) * scale);
+    }
+  }
+}
+
 // The steps of a CTA of keys: heads of the group, query tiles that see one of its keys.
 struct StepWalk {
   int head, tile;
@@ -262,8 +285,9 @@ __global__ void __launch_bounds__(kGradThreads, 1)
   if (of_keys) {
     // ================================================================ dk and dv of 128 keys
     const int blocks = (a.s.sk + kTile - 1) / kTile;
-    const int j0 = static_cast<int>(blockIdx.x) % blocks * kTile;
-    const int kv = static_cast<int>(blockIdx.x) / blocks % a.s.kv_heads, b = static_cast<int>(blockIdx.x) / blocks / a.s.kv_heads;
+    const int j0 = static_cast<int>(blockIdx.x) % blocks * kTile, unit = static_cast<int>(blockIdx.x) / blocks;
+    const int part = unit % a.parts, kv = unit / a.parts % a.s.kv_heads, b = unit / a.parts / a.s.kv_heads;
+    const int head0 = kv * group + part * group / a.parts, head_end = kv * group + (part + 1) * group / a.parts;
     const int tiles = row_tiles(a.s);
     if (a.s.spans) {  // the query tiles between the first and the last that see one of the keys
       for (int t = threadIdx.x; t < tiles; t += kGradThreads) {
@@ -281,7 +305,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
     const int first = sh.first, last = sh.last;
     const bool any = first < last;
     const uint32_t s_at = tmem, dp_at = tmem + kTile, dv_at = tmem + 2 * kTile, dk_at = tmem + 3 * kTile;
-    StepWalk walk{kv * group, first - 1};
+    StepWalk walk{head0, first - 1};
     if (warp >= 8) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
       if (any && warp == 8) {
@@ -294,7 +318,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         }
         __syncwarp();
         RingPos f{0, 0}, s{0, 0};
-        while (me.ok && walk.next(a.s, b, j0, first, last, (kv + 1) * group)) {
+        while (me.ok && walk.next(a.s, b, j0, first, last, head_end)) {
           if (!me.wait(&sh.first_empty[f.s], f.phase ^ 1)) break;
           if (issuer) {
             mbar_arrive_expect_tx(&sh.first_full[f.s], kTileBytes);
@@ -314,7 +338,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
       } else if (any && warp == 11) {
         // ------------------------------------------------------------ statistics of each step
         for (int n = 0;; ++n) {
-          const bool more = walk.next(a.s, b, j0, first, last, (kv + 1) * group);
+          const bool more = walk.next(a.s, b, j0, first, last, head_end);
           // read before the place is free, so that only the stores follow the step before
           constexpr int kEach = kTile / 32;
           float2 stat[kEach];
@@ -520,12 +544,20 @@ __global__ void __launch_bounds__(kGradThreads, 1)
       }
       if (any) me.wait(&sh.done, 0);
       if (me.ok) {  // the first warps store dv, the others dk
-        T* out = nullptr;
-        if (j < a.s.sk) {
-          if (half == 0 && a.dv) out = static_cast<T*>(a.dv) + b * a.v_batch + kv * a.v_head + static_cast<long long>(j) * a.v_row;
-          if (half == 1 && a.dk) out = static_cast<T*>(a.dk) + b * a.k_batch + kv * a.k_head + static_cast<long long>(j) * a.k_row;
+        const uint32_t at = (half ? dk_at : dv_at) + lanes;
+        const float back = half ? a.s.scale : Held<AB>::kBack;
+        const bool wanted = j < a.s.sk && (half ? a.dk : a.dv);
+        if (a.parts > 1) {
+          const long long rows = static_cast<long long>(a.s.batch) * a.s.kv_heads * a.s.sk;
+          const long long row = (static_cast<long long>(b) * a.s.kv_heads + kv) * a.s.sk + j;
+          store_part<D>(wanted ? a.part + ((half * a.parts + part) * rows + row) * a.s.d : nullptr, at, back, a.s.d, any);
+        } else {
+          T* out = nullptr;
+          if (wanted)
+            out = half ? static_cast<T*>(a.dk) + b * a.k_batch + kv * a.k_head + static_cast<long long>(j) * a.k_row
+                       : static_cast<T*>(a.dv) + b * a.v_batch + kv * a.v_head + static_cast<long long>(j) * a.v_row;
+          store_row<T, D>(out, at, back, a.s.d, any);
         }
-        store_row<T, D>(out, (half ? dk_at : dv_at) + lanes, half ? a.s.scale : Held<AB>::kBack, a.s.d, any);
       }
     }
   } else {
@@ -702,8 +734,51 @@ __global__ void __launch_bounds__(kGradThreads, 1)
   }
 }
 
+// dv and dk from their parts, added in order; 8 dims a thread
+template <int AB>
+__global__ void __launch_bounds__(256) join_grad_kernel(const __grid_constant__ GradArgs a) {
+  using T = Element<AB>;
+  wait_for_prior();
+  let_next_start();
+  const int eights = a.s.d >> 3;
+  const long long rows = static_cast<long long>(a.s.batch) * a.s.kv_heads * a.s.sk;
+  const long long n = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x, row = n / eights;
+  const bool of_k = blockIdx.y == 1;
+  if (row >= rows || !(of_k ? a.dk : a.dv)) return;
+  const float4* from = reinterpret_cast<const float4*>(a.part + of_k * a.parts * rows * a.s.d) + 2 * n;
+  const long long step = rows * a.s.d >> 2;
+  float4 x = from[0], y = from[1];
+#pragma unroll 4
+  for (int p = 1; p < a.parts; ++p) {
+    const float4 u = from[p * step], v = from[p * step + 1];
+    x = make_float4(x.x + u.x, x.y + u.y, x.z + u.z, x.w + u.w);
+    y = make_float4(y.x + v.x, y.y + v.y, y.z + v.z, y.w + v.w);
+  }
+  const long long heads = row / a.s.sk, b = heads / a.s.kv_heads, h = heads % a.s.kv_heads, j = row % a.s.sk;
+  T* out = (of_k ? static_cast<T*>(a.dk) + b * a.k_batch + h * a.k_head + j * a.k_row
+                 : static_cast<T*>(a.dv) + b * a.v_batch + h * a.v_head + j * a.v_row) + n % eights * 8;
+  *reinterpret_cast<uint4*>(out) = make_uint4(pack2<T>(x.x, x.y), pack2<T>(x.z, x.w), pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
+}
+
 // ---- host ---------------------------------------------------------------------------------
 long long padded_rows(int sq) { return round_up(sq, kTile); }
+
+// CTAs that share a tile of keys, each some of the query heads on them.  Their sums
+// pass through memory (about 15 us for 148 tiles of 128 dims), so only where a CTA a
+// tile would leave SMs idle.  Measured (us, one CTA a tile and several): 24 heads on
+// one, 2048 rows 712 and 184; 8 on 2, 2000 rows, 64 dims 114 and 60; 12 on 2, 256
+// rows 30 and 18.  Up to 148 tiles under spans (in causal order the first tile's CTA is
+// the last to end): 24 on 4, 4096 rows 455 and 351, but 8 on 4, 4 x 1024 rows 56 and 72;
+// without spans 564 and 581.
+int key_parts(int batch, int heads, int kv_heads, int sq, int sk, bool spans) {
+  const long long units = static_cast<long long>(batch) * kv_heads * ((sk + kTile - 1) / kTile), group = heads / kv_heads;
+  const long long steps = group * (padded_rows(sq) / kTile);  // of a CTA, at most
+  if (units == 0 || steps < (2 * units <= kNumSMs ? 6 : spans ? 64 : steps + 1)) return 1;
+  const long long parts = (kNumSMs + units - 1) / units;
+  return static_cast<int>(parts < group ? parts : group);
+}
+
+long long stats_bytes(int batch, int heads, int sq) { return 8LL * batch * heads * padded_rows(sq); }
 
 template <int AB, int D>
 int launch_grad(const GradArgs& a, const CUtensorMap (&maps)[4], cudaStream_t stream) {
@@ -716,8 +791,12 @@ int launch_grad(const GradArgs& a, const CUtensorMap (&maps)[4], cudaStream_t st
     const long long rows = static_cast<long long>(a.s.batch) * a.s.heads * a.padded;
     if (int st = launch_overlapped(grad_stats_kernel<AB>, dim3(static_cast<unsigned>(rows / 16)), dim3(256), 0, 0, stream, a)) return st;
   }
-  return launch_overlapped(kernel, dim3(a.key_units + a.query_units), dim3(kGradThreads), smem, 0, stream, maps[0],
-                           maps[1], maps[2], maps[3], a);
+  if (int st = launch_overlapped(kernel, dim3(a.key_units + a.query_units), dim3(kGradThreads), smem, 0, stream, maps[0],
+                                 maps[1], maps[2], maps[3], a))
+    return st;
+  if (a.key_units == 0 || a.parts == 1) return kOk;
+  const long long eights = static_cast<long long>(a.s.batch) * a.s.kv_heads * a.s.sk * (a.s.d / 8);
+  return launch_overlapped(join_grad_kernel<AB>, dim3(static_cast<unsigned>((eights + 255) / 256), 2), dim3(256), 0, 0, stream, a);
 }
 
 }  // namespace
@@ -725,9 +804,12 @@ int launch_grad(const GradArgs& a, const CUtensorMap (&maps)[4], cudaStream_t st
 
 using namespace peco;
 
-extern "C" long long peco_span_attention_backward_workspace(int batch, int heads, int sq) {
-  if (batch < 0 || heads < 1 || sq < 0 || sq > 0x7ffffe00) return -1;
-  return 8LL * batch * heads * padded_rows(sq);
+extern "C" long long peco_span_attention_backward_workspace(int batch, int heads, int kv_heads, int sq, int sk, int d, int spans) {
+  if (batch < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || sq < 0 || sk < 0 || sq > 0x7ffffe00 || sk > 0x7ffffe00 ||
+      d < 8 || d > 128 || d % 8)
+    return -1;
+  const long long parts = key_parts(batch, heads, kv_heads, sq, sk, spans != 0);
+  return stats_bytes(batch, heads, sq) + (parts > 1 ? 8 * parts * batch * kv_heads * sk * d : 0);
 }
 
 extern "C" int peco_span_attention_backward(const void* grad, const void* q, const void* k, const void* v, const void* out,
@@ -754,7 +836,8 @@ extern "C" int peco_span_attention_backward(const void* grad, const void* q, con
     if (!readable(t[i], batch, of_keys ? kv_heads : heads, n)) return kErrInvalidValue;
   }
   if (sq > 0 && !lse) return kErrInvalidValue;
-  if (sq > 0 && !usable_workspace(workspace, workspace_bytes, peco_span_attention_backward_workspace(batch, heads, sq))) return kErrWorkspace;
+  if (sq > 0 && !usable_workspace(workspace, workspace_bytes, peco_span_attention_backward_workspace(batch, heads, kv_heads, sq, sk, d, span_rows ? 1 : 0)))
+    return kErrWorkspace;
   GradArgs a{};
   a.s.spans = reinterpret_cast<const int4*>(span_rows);
   a.s.span_tiles = reinterpret_cast<const int4*>(span_tiles);
@@ -774,6 +857,8 @@ extern "C" int peco_span_attention_backward(const void* grad, const void* q, con
   a.lse = lse;
   a.stats = static_cast<float2*>(workspace);
   a.padded = static_cast<int>(padded_rows(sq));
+  a.parts = key_parts(batch, heads, kv_heads, sq, sk, span_rows != nullptr);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + stats_bytes(batch, heads, sq));
   a.dq = dq;
   a.dk = dk;
   a.dv = dv;
@@ -786,7 +871,7 @@ extern "C" int peco_span_attention_backward(const void* grad, const void* q, con
   a.v_batch = t[7].batch;
   a.v_head = t[7].head;
   a.v_row = t[7].row;
-  const long long key_units = keys ? static_cast<long long>(batch) * kv_heads * ((sk + kTile - 1) / kTile) : 0;
+  const long long key_units = keys ? static_cast<long long>(batch) * kv_heads * ((sk + kTile - 1) / kTile) * a.parts : 0;
   const long long query_units = rows ? static_cast<long long>(batch) * heads * (a.padded / kTile) : 0;
   const long long stat_blocks = static_cast<long long>(batch) * heads * a.padded / 16;
   if (key_units + query_units > 0x7fffffffLL || stat_blocks > 0x7fffffffLL) return kErrUnsupported;

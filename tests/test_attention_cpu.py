@@ -136,7 +136,7 @@ def test_entries_check_their_arguments():
                 dict(heads=5), dict(d=4), dict(st=strides(8, s15=4)), dict(st=strides(8, s22=0))):
         assert backward(**bad) == 1, bad
     assert backward(dtype=2) == 20001
-    need = lib.peco_span_attention_backward_workspace(2, 4, 6)
+    need = lib.peco_span_attention_backward_workspace(2, 4, 2, 6, 9, 64, 0)
     assert need == 8 * 2 * 4 * 128
     for bad in (dict(ws=0), dict(n=need - 1), dict(ws=at + 8)):
         assert backward(**bad) == 20005

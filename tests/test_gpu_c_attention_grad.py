@@ -99,6 +99,29 @@ def test_masks(mask, form):
             check(got, formula(q, k, v, g, out, seen, pos, **args))
 
 
+# heads on shared keys whose sums several CTAs share: unequal shares, one head each, a share for every two; causal over more tiles
+@pytest.mark.parametrize("size", [(1, 13, 1, 300, 5100, 24), (2, 10, 2, 259, 130, 128), (1, 12, 2, 390, 4600, 64),
+                                  (1, 36, 3, 700, 4000, 16)])
+def test_shared_keys_in_parts(size):
+    b, h, kv, n, m, d = size
+    spans, seen, pos = plan(b, n, m, causal=True) if m == 4000 else (
+        None, torch.ones(b, n, m, dtype=torch.bool, device=DEV), (torch.arange(n, device=DEV) + m - n).expand(b, n))
+    bits = 1 if spans is not None else 0
+    lib = _native.load()
+    assert lib.peco_span_attention_backward_workspace(b, h, kv, n, m, d, bits) > 8 * b * h * ((n + 127) // 128 * 128)
+    q, k, v = inputs(n, *size, dtype=torch.float16)
+    g = inputs(1, *size, dtype=torch.float16)[0]
+    out, lse = attention(q, k, v, spans=spans, return_lse=True)
+    got = attention_backward(g, q, k, v, out, lse, spans=spans)
+    check(got, formula(q, k, v, g, out, seen, pos))
+    for name in "kv":
+        alone = attention_backward(g, q, k, v, out, lse, spans=spans, needs=[name])
+        assert torch.equal(getattr(alone, name), getattr(got, name))
+    inner = torch.zeros(b, m, kv, d, device=DEV, dtype=torch.float16).transpose(1, 2)  # another layout of k's gradient
+    again = attention_backward(g, q, inner.copy_(k), v, out, lse, spans=spans)
+    assert again.k.stride() == inner.stride() and all(torch.equal(x, y) for x, y in zip(again, got))
+
+
 def test_differences_of_the_loss():
     """The gradient along a direction against the loss's difference quotient in 64 bits (central, step 2^-13: the
     quotient is off by about 2^-26 of third derivatives), to the gradient's rounding."""
