@@ -394,18 +394,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 0; e < kTile; ++e) s[e] = __uint_as_float(raw[e]);
       }
       if constexpr (RICH) {  // to log2 units
-        if (a.s.cap > 0.0f) {
-#pragma unroll
-          for (int e = 0; e < kTile; ++e) s[e] = cap.value(cap.recip(s[e]));
-        } else {
-#pragma unroll
-          for (int e = 0; e < kTile; ++e) s[e] *= scale_log2;
-        }
-        if (a.s.slopes) {
-          const float apart = static_cast<float>(span.z - j0);
-#pragma unroll
-          for (int e = 0; e < kTile; ++e) s[e] = fmaf(-slope, fabsf(apart - static_cast<float>(e)), s[e]);
-        }
+        scaled_scores(a.s, cap, s, nullptr);
+        if (a.s.slopes) less_distance(slope, static_cast<float>(span.z - j0), s);
       }
       // rows past the tensor's end are not looked at
       if (!__all_sync(0xffffffffu, !real || (lo <= j0 && hi >= j0 + kTile))) {

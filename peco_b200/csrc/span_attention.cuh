@@ -59,9 +59,54 @@ struct Cap {
     return y;
   }
   __device__ __forceinline__ float value(float r) const { return fmaf(-2.0f * a, r, a); }
-  // d capped / d raw, without the scale: 1 - tanh^2 = 4 r (1 - r)
-  __device__ __forceinline__ float slope(float r) const { return 4.0f * r * (1.0f - r); }
+  // two scores at a time
+  __device__ __forceinline__ float2 recip(float2 raw) const {
+    const float2 x = fmul2(raw, make_float2(b, b));
+    const float2 y = fadd2(make_float2(exp2_approx(x.x), exp2_approx(x.y)), make_float2(1.0f, 1.0f));
+    float2 r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(y.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(y.y));
+    return r;
+  }
+  __device__ __forceinline__ float2 value(float2 r) const { return ffma2(r, make_float2(-2.0f * a, -2.0f * a), make_float2(a, a)); }
+  // d capped / d raw, without the scale: 1 - tanh^2 = 4 r - 4 r r (r rounded to 2^-24: off by a few 2^-24 in absolute terms)
+  static __device__ __forceinline__ float2 slope(float2 r) {
+    const float2 f = fmul2(r, make_float2(4.0f, 4.0f));
+    return ffma2(f, make_float2(-r.x, -r.y), f);
+  }
 };
+
+// N scores in log2 units, capped or scaled; the slopes of capped ones
+template <int N>
+__device__ __forceinline__ void scaled_scores(const ScoreArgs& s, const Cap& cap, float (&z)[N], float* slopes) {
+  if (s.cap > 0.0f) {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const float2 r = cap.recip(make_float2(z[e], z[e + 1])), v = cap.value(r);
+      if (slopes) {
+        const float2 d = Cap::slope(r);
+        slopes[e] = d.x;
+        slopes[e + 1] = d.y;
+      }
+      z[e] = v.x;
+      z[e + 1] = v.y;
+    }
+  } else {
+    const float f = s.scale * kLog2E;
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const float2 v = fmul2(make_float2(z[e], z[e + 1]), make_float2(f, f));
+      z[e] = v.x;
+      z[e + 1] = v.y;
+    }
+  }
+}
+// less slope |apart - e|, for the keys side by side from a tile's first
+template <int N>
+__device__ __forceinline__ void less_distance(float slope, float apart, float (&z)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) z[e] = fmaf(-slope, fabsf(apart - static_cast<float>(e)), z[e]);
+}
 
 // 128 columns of a TMEM lane: four loads in flight, one wait.
 __device__ __forceinline__ void tmem_ld128_sync(uint32_t at, uint32_t (&r)[128]) {

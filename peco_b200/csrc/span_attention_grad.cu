@@ -16,6 +16,9 @@
 // CTAs of keys every product waits for the one whose operand it overwrites, and so
 // for the softmax between; issuing S right behind dv's product (1640 us), or the two
 // chains by a warp each (1680 us), was slower, although both wait less.
+// Capped scores 2780 us (two more special functions a pair: 1580 us of that unit in all),
+// a bias by distance 2100 us; their slopes go into p before g.v is read (after it, which
+// held three rows of registers at once: 4090 and 2790 us).
 // Under two documents 1600 us: a warp reads each step's statistics and spans while the
 // place for them is still in use (read after it was free: 1890 us).
 #include "span_attention.cuh"
@@ -472,28 +475,31 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         float p[64], slopes[RICH ? 64 : 1];
         load_half(s_own, p);
         if constexpr (RICH) {
-          const float bias = a.s.slopes ? a.s.slopes[step.head] * kLog2E : 0.0f;
+          scaled_scores(a.s, cap, p, slopes);
+          if (a.s.slopes) {
+            const float bias = a.s.slopes[step.head] * kLog2E;
 #pragma unroll
-          for (int e = 0; e < 64; ++e) {
-            slopes[e] = 1.0f;
-            if (a.s.cap > 0.0f) {
-              const float rc = cap.recip(p[e]);
-              slopes[e] = cap.slope(rc);
-              p[e] = cap.value(rc);
-            } else {
-              p[e] *= scale_log2;
+            for (int e = 0; e < 64; e += 4) {
+              const float4 pos = *reinterpret_cast<const float4*>(step.pos + c0 + e);
+              const float2 x = fadd2(make_float2(pos.x, pos.y), make_float2(-at_key, -at_key));
+              const float2 y = fadd2(make_float2(pos.z, pos.w), make_float2(-at_key, -at_key));
+              p[e] = fmaf(-bias, fabsf(x.x), p[e]);
+              p[e + 1] = fmaf(-bias, fabsf(x.y), p[e + 1]);
+              p[e + 2] = fmaf(-bias, fabsf(y.x), p[e + 2]);
+              p[e + 3] = fmaf(-bias, fabsf(y.y), p[e + 3]);
             }
-            if (a.s.slopes) p[e] = fmaf(-bias, fabsf(step.pos[c0 + e] - at_key), p[e]);
           }
         }
 #pragma unroll
         for (int e = 0; e < 64; e += 4) {
           const float4 l = *reinterpret_cast<const float4*>(step.lse + c0 + e);
           if constexpr (RICH) {
-            p[e] -= l.x;
-            p[e + 1] -= l.y;
-            p[e + 2] -= l.z;
-            p[e + 3] -= l.w;
+            const float2 x = fadd2(make_float2(p[e], p[e + 1]), make_float2(-l.x, -l.y));
+            const float2 y = fadd2(make_float2(p[e + 2], p[e + 3]), make_float2(-l.z, -l.w));
+            p[e] = x.x;
+            p[e + 1] = x.y;
+            p[e + 2] = y.x;
+            p[e + 3] = y.y;
           } else {
             const float2 sc = make_float2(scale_log2, scale_log2);
             const float2 x = ffma2(make_float2(p[e], p[e + 1]), sc, make_float2(-l.x, -l.y));
@@ -517,6 +523,16 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         }
         store_half<T>(s_own, p);
         me.arrive(&sh.p_full);
+        if constexpr (RICH) {
+          if (a.s.cap > 0.0f) {
+#pragma unroll
+            for (int e = 0; e < 64; e += 2) {
+              const float2 x = fmul2(make_float2(p[e], p[e + 1]), make_float2(slopes[e], slopes[e + 1]));
+              p[e] = x.x;
+              p[e + 1] = x.y;
+            }
+          }
+        }
         if (!me.wait(&sh.dp_full, n)) break;
         float ds[64];
         load_half(dp_own, ds);
@@ -530,10 +546,6 @@ __global__ void __launch_bounds__(kGradThreads, 1)
           ds[e + 1] = p[e + 1] * x.y;
           ds[e + 2] = p[e + 2] * y.x;
           ds[e + 3] = p[e + 3] * y.y;
-        }
-        if constexpr (RICH) {
-#pragma unroll
-          for (int e = 0; e < 64; ++e) ds[e] *= slopes[e];
         }
         if (masked) {  // a masked pair's g.v may be anything
 #pragma unroll
@@ -669,19 +681,8 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         float p[64], slopes[RICH ? 64 : 1];
         load_half(s_own, p);
         if constexpr (RICH) {
-          const float apart = static_cast<float>(span.z - j0);
-#pragma unroll
-          for (int e = 0; e < 64; ++e) {
-            slopes[e] = 1.0f;
-            if (a.s.cap > 0.0f) {
-              const float rc = cap.recip(p[e]);
-              slopes[e] = cap.slope(rc);
-              p[e] = cap.value(rc);
-            } else {
-              p[e] *= scale_log2;
-            }
-            if (a.s.slopes) p[e] = fmaf(-bias, fabsf(apart - static_cast<float>(e)), p[e]);
-          }
+          scaled_scores(a.s, cap, p, slopes);
+          if (a.s.slopes) less_distance(bias, static_cast<float>(span.z - j0), p);
         }
 #pragma unroll
         for (int e = 0; e < 64; e += 2) {
@@ -696,6 +697,16 @@ __global__ void __launch_bounds__(kGradThreads, 1)
 #pragma unroll
           for (int e = 0; e < 64; ++e) p[e] = e >= from && e < to ? p[e] : 0.0f;
         }
+        if constexpr (RICH) {
+          if (a.s.cap > 0.0f) {
+#pragma unroll
+            for (int e = 0; e < 64; e += 2) {
+              const float2 x = fmul2(make_float2(p[e], p[e + 1]), make_float2(slopes[e], slopes[e + 1]));
+              p[e] = x.x;
+              p[e + 1] = x.y;
+            }
+          }
+        }
         if (!me.wait(&sh.dp_full, t)) break;
         float ds[64];
         load_half(dp_at + lanes + half * 64, ds);
@@ -705,10 +716,6 @@ __global__ void __launch_bounds__(kGradThreads, 1)
           const float2 x = fmul2(make_float2(p[e], p[e + 1]), ffma2(make_float2(ds[e], ds[e + 1]), back, delta2));
           ds[e] = x.x;
           ds[e + 1] = x.y;
-        }
-        if constexpr (RICH) {
-#pragma unroll
-          for (int e = 0; e < 64; ++e) ds[e] *= slopes[e];
         }
         if (masked) {  // a masked pair's g.v may be anything
 #pragma unroll
