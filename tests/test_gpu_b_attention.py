@@ -119,6 +119,22 @@ def test_masks(mask, form):
             check(q, k, v, out, lse, seen, pos, **args)
 
 
+# few rows over caches of very unequal lengths, an empty one among them: their keys are shared out over the CTAs
+@pytest.mark.parametrize("form", [(6, 1, 8, 2, 64), (9, 3, 16, 8, 128), (37, 1, 2, 2, 40), (1, 200, 8, 1, 128)])
+def test_unequal_caches(form):
+    b, n, h, kv, d = form
+    lengths = [(7000, 0, 129, 1, 2500, 640)[i % 6] + i for i in range(b)]
+    spans, seen, pos = plan(b, n, 7100, lengths=lengths, causal=True)
+    q, k, v = inputs(b, b, h, kv, n, 7100, d)
+    slopes = torch.rand(h, device=DEV) * 0.01
+    for args in ({}, dict(softcap=5.0, slopes=slopes)):
+        out, lse = attention(q, k, v, spans=spans, return_lse=True, **args)
+        check(q, k, v, out, lse, seen, pos, **args)
+    none = plan(b, n, 7100, lengths=[0] * b)[0]
+    out, lse = attention(q, k, v, spans=none, return_lse=True)
+    assert (out == 0).all() and (lse == -torch.inf).all()
+
+
 def test_one_plan_for_all_samples():
     spans, seen, pos = plan(1, 200, 200, causal=True)
     q, k, v = inputs(0, 3, 2, 2, 200, 200, 64)
