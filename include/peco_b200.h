@@ -307,8 +307,9 @@ long long peco_linear_int8_workspace(int from_16_bits, const void* values, long 
                                      long long w_stride, int samples, int rows_per_sample, int k, int k2, int n);
 
 /* Spans of keys for attention: rows [batch, queries, 4] gets (first key, key
- * behind the last, position among the keys, 0) of every query row, tiles [batch,
- * ceil(queries / 128), 4] bounds over 128 rows; both start on 16 bytes.
+ * behind the last, position among the keys, n) of every query row, tiles [batch,
+ * ceil(queries / 128), 4] bounds over 128 rows; both start on 16 bytes.  n of the
+ * first rows: the tiles of 128 rows, those that see most keys first.
  * Documents (documents > 0): document i of sample b holds rows [q_ends[b *
  * q_stride + i], q_ends[... + i + 1]) and keys likewise by k_ends; rows outside
  * see nothing.  Otherwise lengths [batch] (null: all keys).  A document's last

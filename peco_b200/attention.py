@@ -43,7 +43,8 @@ class AttentionGrads(NamedTuple):
 class KeySpans:
     """The keys that each query row sees, as ``key_spans`` lays them out."""
 
-    rows: torch.Tensor   # int32 [B or 1, queries, 4]: first key, key behind the last, the row's position among the keys
+    rows: torch.Tensor   # int32 [B or 1, queries, 4]: first key, key behind the last, the row's position among the keys;
+                         # of the first rows also the tiles of 128 rows, those that see most keys first
     tiles: torch.Tensor  # int32 [B or 1, tiles of 128 rows, 4]
     queries: int
     keys: int

@@ -22,7 +22,7 @@
 //
 // What it measured (B200, bf16): 24 heads x 7006 rows x 128 dims, every key: 490 us
 // (1.18 PFLOP/s; 535 us at the power limit after 300 calls in a row), 64 dims 423 us;
-// causal, 24 query heads on 4, 4096 rows 123 us; one row of 24 heads on 4, four samples of
+// causal, 24 query heads on 4, 4096 rows 120 us; one row of 24 heads on 4, four samples of
 // up to 16384 keys 34 us.  Tensor core and special-function unit are both 62% busy:
 // the two warps of a scheduler do not hide all of each other's maxima, TMEM loads
 // and hand-offs.  Before, with a maximum, sum and accumulator for each warpgroup
@@ -54,48 +54,80 @@ struct SpanArgs {
 
 __device__ __forceinline__ int clamped(int v, int lo, int hi) { return min(max(v, lo), hi); }
 
-// A block per 128 rows of a sample, a row per thread.
+// (first key, key behind the last, position) of a row
+__device__ int3 row_span(const SpanArgs& a, int b, int i) {
+  int lo = 0, hi = 0, pos = 0;
+  int q0 = 0, q1 = a.queries, k0 = 0, k1 = a.keys, doc = 0;
+  bool inside = true;
+  if (a.documents > 0) {
+    const int* qe = a.q_ends + b * a.q_stride;
+    const int* ke = a.k_ends + b * a.k_stride;
+    int l = -1, h = a.documents + 1;  // the last entry not behind the row
+    while (h - l > 1) {
+      const int mid = (l + h) >> 1;
+      if (qe[mid] <= i) l = mid;
+      else h = mid;
+    }
+    inside = l >= 0 && l < a.documents;
+    doc = clamped(l, 0, a.documents - 1);
+    q0 = clamped(qe[doc], 0, a.queries);
+    q1 = clamped(qe[doc + 1], q0, a.queries);
+    k0 = clamped(ke[doc], 0, a.keys);
+    k1 = clamped(ke[doc + 1], k0, a.keys);
+    inside = inside && i >= q0 && i < q1;
+  } else if (a.lengths) {
+    k1 = clamped(a.lengths[b], 0, a.keys);
+  }
+  pos = k0 + (i - q0) + (k1 - k0) - (q1 - q0);
+  lo = k0;
+  hi = inside ? k1 : k0;
+  if (a.causal) {
+    const int prefix = a.prefix ? a.prefix[b * a.prefix_batch + doc * a.prefix_doc] : a.prefix_all;
+    hi = min(hi, max(pos + 1, k0 + clamped(prefix, 0, a.keys - k0)));
+  }
+  if (a.window > 0) {
+    lo = max(lo, static_cast<int>(max(static_cast<long long>(pos) - a.window + 1, 0LL)));
+    hi = static_cast<int>(min(static_cast<long long>(hi), static_cast<long long>(pos) + a.window));
+  }
+  if (hi <= lo) lo = hi = 0;
+  return make_int3(lo, hi, pos);
+}
+
+// A block per 128 rows of a sample, a row per thread.  Each also ranks its tile by
+// the keys that its first and last row see, for the attention's CTAs to take the
+// longest tiles first (among more than kRanked tiles: the later ones).
+constexpr int kRanked = 1024;
 __global__ void __launch_bounds__(kTile) key_spans_kernel(const SpanArgs a) {
   __shared__ int4 part[4];
+  __shared__ int sizes[kRanked];
+  __shared__ int ahead;
   wait_for_prior();
   let_next_start();
-  const int b = blockIdx.y, i = blockIdx.x * kTile + threadIdx.x;
-  int lo = 0, hi = 0, pos = 0;
+  const int b = blockIdx.y, i = blockIdx.x * kTile + threadIdx.x, tiles = gridDim.x, mine = blockIdx.x;
+  if (threadIdx.x == 0) ahead = 0;
+  int lo = 0, hi = 0;
   if (i < a.queries) {
-    int q0 = 0, q1 = a.queries, k0 = 0, k1 = a.keys, doc = 0;
-    bool inside = true;
-    if (a.documents > 0) {
-      const int* qe = a.q_ends + b * a.q_stride;
-      const int* ke = a.k_ends + b * a.k_stride;
-      int l = -1, h = a.documents + 1;  // the last entry not behind the row
-      while (h - l > 1) {
-        const int mid = (l + h) >> 1;
-        if (qe[mid] <= i) l = mid;
-        else h = mid;
-      }
-      inside = l >= 0 && l < a.documents;
-      doc = clamped(l, 0, a.documents - 1);
-      q0 = clamped(qe[doc], 0, a.queries);
-      q1 = clamped(qe[doc + 1], q0, a.queries);
-      k0 = clamped(ke[doc], 0, a.keys);
-      k1 = clamped(ke[doc + 1], k0, a.keys);
-      inside = inside && i >= q0 && i < q1;
-    } else if (a.lengths) {
-      k1 = clamped(a.lengths[b], 0, a.keys);
+    const int3 s = row_span(a, b, i);
+    lo = s.x;
+    hi = s.y;
+    int* row = reinterpret_cast<int*>(a.rows + static_cast<long long>(b) * a.queries + i);
+    *reinterpret_cast<int2*>(row) = make_int2(lo, hi);
+    row[2] = s.z;
+    if (i >= tiles) row[3] = 0;  // (the others' by rank below)
+  }
+  if (tiles <= kRanked) {
+    for (int t = threadIdx.x; t < tiles; t += kTile) {
+      const int3 u = row_span(a, b, t * kTile), v = row_span(a, b, min(t * kTile + kTile, a.queries) - 1);
+      const int from = min(u.y > u.x ? u.x : 0x7fffffff, v.y > v.x ? v.x : 0x7fffffff), to = max(u.y, v.y);
+      sizes[t] = to > from ? (to - from + kTile - 1) / kTile : 0;
     }
-    pos = k0 + (i - q0) + (k1 - k0) - (q1 - q0);
-    lo = k0;
-    hi = inside ? k1 : k0;
-    if (a.causal) {
-      const int prefix = a.prefix ? a.prefix[b * a.prefix_batch + doc * a.prefix_doc] : a.prefix_all;
-      hi = min(hi, max(pos + 1, k0 + clamped(prefix, 0, a.keys - k0)));
-    }
-    if (a.window > 0) {
-      lo = max(lo, static_cast<int>(max(static_cast<long long>(pos) - a.window + 1, 0LL)));
-      hi = static_cast<int>(min(static_cast<long long>(hi), static_cast<long long>(pos) + a.window));
-    }
-    if (hi <= lo) lo = hi = 0;
-    a.rows[static_cast<long long>(b) * a.queries + i] = make_int4(lo, hi, pos, 0);
+    __syncthreads();
+    int count = 0;
+    for (int t = threadIdx.x; t < tiles; t += kTile) count += sizes[t] > sizes[mine] || (sizes[t] == sizes[mine] && t > mine);
+    count = __reduce_add_sync(0xffffffffu, count);
+    if ((threadIdx.x & 31) == 0) atomicAdd(&ahead, count);
+  } else if (threadIdx.x == 0) {
+    ahead = tiles - 1 - mine;
   }
   // rows that see nothing count for the masks only; rows past the end not at all
   const bool real = i < a.queries, sees = hi > lo;
@@ -113,7 +145,8 @@ __global__ void __launch_bounds__(kTile) key_spans_kernel(const SpanArgs a) {
       t.z = max(t.z, part[w].z);
       t.w = min(t.w, part[w].w);
     }
-    a.tiles[static_cast<long long>(b) * gridDim.x + blockIdx.x] = t;
+    a.tiles[static_cast<long long>(b) * tiles + mine] = t;
+    a.rows[static_cast<long long>(b) * a.queries + ahead].w = mine;
   }
 }
 
@@ -133,6 +166,7 @@ struct ForwardArgs {
   float* lse;               // [batch, heads, sq]
   int packed;               // heads side by side in a tile (1: consecutive rows of one head)
   int row_blocks;           // CTAs along a head's rows
+  int together;             // heads whose tiles are taken in turn
   int splits;               // CTAs along the keys
   float* part;              // [unit][split][128][d] unnormalised, then (max, sum) of each row
   float2* part_sums;
@@ -153,12 +187,12 @@ static_assert(sizeof(ForwardShared) <= 1024 && forward_smem<128>() <= 227 * 1024
 struct Unit {
   int b, head0, row0;       // first head, first row
   __device__ Unit(const ForwardArgs& a, int unit) {
-    const int groups = a.s.heads / a.packed;
-    const int block = a.row_blocks - 1 - unit % a.row_blocks;  // in causal order the later rows see more keys
-    const int rest = unit / a.row_blocks;
-    head0 = rest % groups * a.packed;
-    b = rest / groups;
-    row0 = block * kTile;
+    const int groups = a.s.heads / a.packed, sample = groups * a.row_blocks;
+    b = unit / sample;
+    const int n = unit - b * sample, first = n / (a.together * a.row_blocks) * a.together;
+    const int heads = min(a.together, groups - first), m = n - first * a.row_blocks;
+    head0 = (first + m % heads) * a.packed;
+    row0 = ranked_tile(a.s, b, m / heads, a.row_blocks) * kTile;
   }
   __device__ __forceinline__ bool row(const ForwardArgs& a, int r, int& head, int& i) const {
     if (a.packed > 1) {
@@ -736,6 +770,7 @@ extern "C" int peco_span_attention(const void* q, const void* k, const void* v, 
   a.lse = lse;
   a.packed = c.packed;
   a.row_blocks = c.row_blocks;
+  a.together = heads_together(a.s, c.row_blocks, heads / c.packed);
   a.splits = c.splits;
   a.part = static_cast<float*>(workspace);
   a.part_sums = reinterpret_cast<float2*>(static_cast<float*>(workspace) + part_rows(c) * d);

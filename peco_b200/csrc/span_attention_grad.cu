@@ -44,6 +44,7 @@ struct GradArgs {
   void *dq, *dk, *dv;
   long long q_batch, q_head, q_row, k_batch, k_head, k_row, v_batch, v_head, v_row;
   int key_units, query_units;
+  int together;              // heads whose query tiles are taken in turn
   int parts;                 // CTAs that share a tile of keys, each some of the heads on them
   float* part;               // with several: dv, then dk, [parts, batch, key heads, keys, dims] each
 };
@@ -575,7 +576,9 @@ __global__ void __launch_bounds__(kGradThreads, 1)
   } else {
     // ================================================================ dq of 128 query rows
     const int tiles = row_tiles(a.s), unit = static_cast<int>(blockIdx.x) - a.key_units;
-    const int tile = tiles - 1 - unit % tiles, head = unit / tiles % a.s.heads, b = unit / tiles / a.s.heads;
+    const int sample = a.s.heads * tiles, b = unit / sample, n = unit - b * sample;
+    const int first = n / (a.together * tiles) * a.together, heads = min(a.together, a.s.heads - first), m = n - first * tiles;
+    const int head = first + m % heads, tile = ranked_tile(a.s, b, m / heads, tiles);
     const int i0 = tile * kTile, kv = head / group;
     const int4 seen = tile_span(a.s, b, tile);
     const int key0 = max(seen.x, 0), key_end = min(seen.y, a.s.sk);
@@ -864,6 +867,7 @@ extern "C" int peco_span_attention_backward(const void* grad, const void* q, con
   a.lse = lse;
   a.stats = static_cast<float2*>(workspace);
   a.padded = static_cast<int>(padded_rows(sq));
+  a.together = sq > 0 ? heads_together(a.s, a.padded / kTile, heads) : 1;
   a.parts = key_parts(batch, heads, kv_heads, sq, sk, span_rows != nullptr);
   a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + stats_bytes(batch, heads, sq));
   a.dq = dq;

@@ -135,6 +135,21 @@ def test_unequal_caches(form):
     assert (out == 0).all() and (lse == -torch.inf).all()
 
 
+@pytest.mark.parametrize("mask", [(1, 520, 520, dict(documents=[0, 100, 300, 500], causal=True)), (3, 1500, 700, dict(lengths=[700, 0, 9])),
+                                  (2, 1000, 1000, dict(window=40, causal=True)), (1, 140000, 140000, dict(causal=True)), (1, 1, 5, {})])
+def test_every_tile_has_its_turn(mask):
+    """The plan names each tile of rows once, and no tile before one that sees more keys (of up to 1024 tiles)."""
+    b, n, m, words = mask
+    words = {k: torch.tensor(v, dtype=torch.int32, device=DEV) if isinstance(v, list) else v for k, v in words.items()}
+    spans = key_spans(b, n, m, device=DEV, **words)
+    tiles = -(-n // 128)
+    turn = spans.rows[:, :tiles, 3].long()
+    assert (turn.sort(1).values == torch.arange(tiles, device=DEV)).all() and (spans.rows[:, tiles:, 3] == 0).all()
+    sizes = ((spans.tiles[..., 1].long() - spans.tiles[..., 0]).clamp(min=0) + 127) // 128
+    if tiles <= 1024:
+        assert (sizes.gather(1, turn).diff(dim=1) <= 0).all()
+
+
 def test_one_plan_for_all_samples():
     spans, seen, pos = plan(1, 200, 200, causal=True)
     q, k, v = inputs(0, 3, 2, 2, 200, 200, 64)
