@@ -22,8 +22,8 @@
 //
 // What it measured (B200, bf16): 24 heads x 7006 rows x 128 dims, every key: 490 us
 // (1.18 PFLOP/s; 535 us at the power limit after 300 calls in a row), 64 dims 423 us;
-// causal, 24 query heads on 4, 4096 rows 120 us; one row of 24 heads on 4, four samples of
-// up to 16384 keys 34 us.  Tensor core and special-function unit are both 62% busy:
+// causal, 24 query heads on 4, 4096 rows 116 us; one row of 24 heads on 4, four samples of
+// up to 16384 keys 32 us.  Tensor core and special-function unit are both 62% busy:
 // the two warps of a scheduler do not hide all of each other's maxima, TMEM loads
 // and hand-offs.  Before, with a maximum, sum and accumulator for each warpgroup
 // 563 us, and with one warp that issued all products 536 us; two tiles of rows a
@@ -165,9 +165,9 @@ struct ForwardArgs {
   long long out_batch, out_head, out_row;
   float* lse;               // [batch, heads, sq]
   int packed;               // heads side by side in a tile (1: consecutive rows of one head)
-  int row_blocks;           // CTAs along a head's rows
-  int together;             // heads whose tiles are taken in turn
-  int splits;               // CTAs along the keys
+  Turns turns;              // of heads (packed ones as one) and their tiles
+  Divisor splits;           // CTAs along the keys
+  Divisor rows;             // query rows
   float* part;              // [unit][split][128][d] unnormalised, then (max, sum) of each row
   float2* part_sums;
 };
@@ -187,17 +187,16 @@ static_assert(sizeof(ForwardShared) <= 1024 && forward_smem<128>() <= 227 * 1024
 struct Unit {
   int b, head0, row0;       // first head, first row
   __device__ Unit(const ForwardArgs& a, int unit) {
-    const int groups = a.s.heads / a.packed, sample = groups * a.row_blocks;
-    b = unit / sample;
-    const int n = unit - b * sample, first = n / (a.together * a.row_blocks) * a.together;
-    const int heads = min(a.together, groups - first), m = n - first * a.row_blocks;
-    head0 = (first + m % heads) * a.packed;
-    row0 = ranked_tile(a.s, b, m / heads, a.row_blocks) * kTile;
+    int rank;
+    a.turns.at(unit, b, head0, rank);
+    head0 *= a.packed;
+    row0 = ranked_tile(a.s, b, rank, a.turns.tiles) * kTile;
   }
   __device__ __forceinline__ bool row(const ForwardArgs& a, int r, int& head, int& i) const {
     if (a.packed > 1) {
-      head = head0 + r / a.s.sq;
-      i = r % a.s.sq;
+      const int n = a.rows(r);
+      head = head0 + n;
+      i = r - n * a.s.sq;
       return r < a.packed * a.s.sq;
     }
     head = head0;
@@ -213,9 +212,9 @@ struct Unit {
 };
 
 // Key tiles of one split: first key, tiles
-__device__ __forceinline__ int2 split_keys(int2 keys, int split, int splits) {
+__device__ __forceinline__ int2 split_keys(int2 keys, int split, const Divisor& splits) {
   const int all = (keys.y - keys.x + kTile - 1) / kTile;
-  const int per = (all + splits - 1) / splits;
+  const int per = splits(all + splits.by - 1);
   const int first = min(all, split * per);
   return make_int2(keys.x + first * kTile, min(all, first + per) - first);
 }
@@ -228,7 +227,7 @@ template <int AB, int D>
 __device__ __noinline__ void masked_row(const ForwardArgs& a, int b, int head, int i, int lo, int hi, int pos, int from,
                                         int to, float m, float (&acc)[D / 32]) {
   using T = Element<AB>;
-  const int lane = lane_id(), kv = head / (a.s.heads / a.s.kv_heads), d = a.s.d;
+  const int lane = lane_id(), kv = a.s.group(head), d = a.s.d;
   const T* q = static_cast<const T*>(a.q.ptr) + b * a.q.batch + head * a.q.head + static_cast<long long>(i) * a.q.row;
   const T* k = static_cast<const T*>(a.k.ptr) + b * a.k.batch + kv * a.k.head;
   const T* v = static_cast<const T*>(a.v.ptr) + b * a.v.batch + kv * a.v.head;
@@ -308,8 +307,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   wait_for_prior();
   let_next_start();
   const uint32_t tmem = sh.tmem;
-  const int split = blockIdx.x % a.splits;
-  const Unit unit(a, blockIdx.x / a.splits);
+  const int at = a.splits(blockIdx.x), split = static_cast<int>(blockIdx.x) - at * a.splits.by;
+  const Unit unit(a, at);
   const int2 all_keys = unit.keys(a);
   const int2 mine = split_keys(all_keys, split, a.splits);
   const int key0 = mine.x, ntiles = mine.y;
@@ -319,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 8) {
     // ---------------------------------------------------------------- TMA
     const bool issuer = elect_one();
-    const int kv = unit.head0 / (a.s.heads / a.s.kv_heads);
+    const int kv = a.s.group(unit.head0);
     bool ok = true;
     if (ntiles > 0 && issuer) {
       mbar_arrive_expect_tx(&sh.q_full, static_cast<uint32_t>(a.packed * min(a.s.sq, kTile)) * 128u * kPanels);
@@ -534,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float its = other.x == -INFINITY ? other.y : other.y * exp2_approx(other.x - last);
       l = w == 0 ? own + its : its + own;
       m = last;
-      const bool whole = a.splits == 1;
+      const bool whole = a.splits.by == 1;
       const float inv = !whole ? 1.0f : l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;  // (a NaN stays)
       // each warpgroup stores half of the columns
       constexpr int kHalf = D / 2;
@@ -550,6 +549,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         part = a.part + at * a.s.d;
         if (w == 0) a.part_sums[at] = make_float2(m, l);
       }
+      // (in K's first tile, whose products are over)
+      const RowsOut<kHalf> rows_out{k_slots + warp * (32 * kHalf * 2), lane};
       bool finite = true;
 #pragma unroll
       for (int c = w * kHalf; c < (w + 1) * kHalf; c += 32) {
@@ -566,13 +567,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                            : fmul2(make_float2(__uint_as_float(raw[2 * e]), __uint_as_float(raw[2 * e + 1])), make_float2(inv, inv));
           finite = finite && fabsf(v[e].x) < INFINITY && fabsf(v[e].y) < INFINITY;
         }
-        if (out) {
+        if (whole) {
 #pragma unroll
           for (int g = 0; g < 4; ++g)
-            if (c + g * 8 < a.s.d)
-              *reinterpret_cast<uint4*>(out + c + g * 8) =
-                  make_uint4(pack2<T>(v[4 * g].x, v[4 * g].y), pack2<T>(v[4 * g + 1].x, v[4 * g + 1].y),
-                             pack2<T>(v[4 * g + 2].x, v[4 * g + 2].y), pack2<T>(v[4 * g + 3].x, v[4 * g + 3].y));
+            rows_out.put((c - w * kHalf) / 8 + g,
+                         make_uint4(pack2<T>(v[4 * g].x, v[4 * g].y), pack2<T>(v[4 * g + 1].x, v[4 * g + 1].y),
+                                    pack2<T>(v[4 * g + 2].x, v[4 * g + 2].y), pack2<T>(v[4 * g + 3].x, v[4 * g + 3].y)));
         } else if (part) {
 #pragma unroll
           for (int g = 0; g < 8; ++g)
@@ -580,6 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               *reinterpret_cast<float4*>(part + c + g * 4) = make_float4(v[2 * g].x, v[2 * g].y, v[2 * g + 1].x, v[2 * g + 1].y);
         }
       }
+      if (whole) rows_out.store(out ? out + w * kHalf : nullptr, a.s.d - w * kHalf);
       // (with a NaN or infinite sum the row sees such scores itself)
       uint32_t again = __ballot_sync(0xffffffffu, masked && real && !finite && l > 0.0f && l < INFINITY);
       while (again) {
@@ -615,45 +616,70 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // A row's parts joined: out = sum_p O_p 2^(m_p - M) / sum_p l_p 2^(m_p - M).  A block
-// a row: its warps take every fourth part, and their sums are added in order.
-template <int AB>
-__global__ void __launch_bounds__(128) split_attention_kernel(const __grid_constant__ ForwardArgs a) {
+// a row; each of its warps takes every WARPS-th part, all asked for at once, and their
+// sums are added in order.  Latency bounds it: 16 warps for more than 16 parts (74 parts of
+// 8 rows, launched cold: 4 warps in turn 13.8 us,
+// this 6.1 us), else 4.
+template <int AB, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) split_attention_kernel(const __grid_constant__ ForwardArgs a) {
   using T = Element<AB>;
-  __shared__ float sums[4][kTile + 1];
+  constexpr int kParts = WARPS == 4 ? 16 : kNumSMs, kEach = (kParts + WARPS - 1) / WARPS, kHeld = (kParts + 31) / 32;
+  __shared__ float4 sums[WARPS][kTile / 4];
   wait_for_prior();
   let_next_start();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rows = a.packed > 1 ? a.packed * a.s.sq : min(a.s.sq, kTile);  // of a unit that can be there
-  const int n = static_cast<int>(blockIdx.x) / rows, r = static_cast<int>(blockIdx.x) % rows;
+  const int n = static_cast<int>(blockIdx.x) / rows, r = static_cast<int>(blockIdx.x) - n * rows;
   const Unit unit(a, n);
   int head, i;
   if (!unit.row(a, r, head, i)) return;
-  const long long first = static_cast<long long>(n) * a.splits * kTile + r;
-  float m = -INFINITY;
-  for (int p = lane; p < a.splits; p += 32) m = fmaxf(m, a.part_sums[first + p * static_cast<long long>(kTile)].x);
-  m = warp_max(m);
-  float l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (int p = warp; p < a.splits; p += 4) {
-    const long long at = first + p * static_cast<long long>(kTile);
-    const float2 s = a.part_sums[at];
-    const float f = s.y == 0.0f ? 0.0f : exp2_approx(s.x - m);
-    l = fmaf(s.y, f, l);
+  const int parts = a.splits.by, c = lane * 4;
+  const long long first = static_cast<long long>(n) * parts * kTile + r;
+  float2 of[kHeld];  // (maximum, sum) of parts lane, lane + 32, ...
+  float4 v[kEach];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (lane + 32 * e < a.s.d) acc[e] = fmaf(a.part[at * a.s.d + lane + 32 * e], f, acc[e]);
+  for (int k = 0; k < kHeld; ++k) {
+    const int p = lane + 32 * k;
+    of[k] = p < parts ? a.part_sums[first + p * static_cast<long long>(kTile)] : make_float2(-INFINITY, 0.0f);
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) sums[warp][lane + 32 * e] = acc[e];
-  if (lane == 0) sums[warp][kTile] = l;
+  for (int k = 0; k < kEach; ++k) {
+    const int p = warp + WARPS * k;
+    v[k] = p < parts && c < a.s.d ? *reinterpret_cast<const float4*>(a.part + (first + p * static_cast<long long>(kTile)) * a.s.d + c)
+                                  : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+  float m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) m = fmaxf(m, of[k].x);
+  m = warp_max(m);
+  float f[kHeld];
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) {
+    f[k] = of[k].y == 0.0f ? 0.0f : exp2_approx(of[k].x - m);
+    l = fmaf(of[k].y, f[k], l);
+  }
+  l = warp_sum(l);
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int p = warp + WARPS * k;
+    float w = f[0];
+#pragma unroll
+    for (int h = 1; h < kHeld; ++h) w = p >> 5 == h ? f[h] : w;
+    w = __shfl_sync(0xffffffffu, w, p & 31);
+    acc = make_float4(fmaf(v[k].x, w, acc.x), fmaf(v[k].y, w, acc.y), fmaf(v[k].z, w, acc.z), fmaf(v[k].w, w, acc.w));
+  }
+  sums[warp][lane] = acc;
   __syncthreads();
-  const int c = threadIdx.x;
-  l = sums[0][kTile] + sums[1][kTile] + sums[2][kTile] + sums[3][kTile];
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  if (c < a.s.d)
-    static_cast<T*>(a.out)[unit.b * a.out_batch + head * a.out_head + static_cast<long long>(i) * a.out_row + c] =
-        from_f32<T>((sums[0][c] + sums[1][c] + sums[2][c] + sums[3][c]) * inv);
-  if (c == 0)
+  const int col = threadIdx.x;
+  if (col < a.s.d) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    float o = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) o += reinterpret_cast<const float*>(sums[w])[col];
+    static_cast<T*>(a.out)[unit.b * a.out_batch + head * a.out_head + static_cast<long long>(i) * a.out_row + col] = from_f32<T>(o * inv);
+  }
+  if (col == 0)
     a.lse[(static_cast<long long>(unit.b) * a.s.heads + head) * a.s.sq + i] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
@@ -698,8 +724,10 @@ int launch_forward(const ForwardArgs& a, const ForwardCut& c, const CUtensorMap 
   const dim3 grid(static_cast<unsigned>(c.units * c.splits));
   if (int st = launch_overlapped(kernel, grid, dim3(kThreads), forward_smem<D>(), 0, stream, maps[0], maps[1], maps[2], a)) return st;
   if (c.splits == 1) return kOk;
-  return launch_overlapped(split_attention_kernel<AB>, dim3(static_cast<unsigned>(c.units * (a.packed > 1 ? a.packed * a.s.sq : a.s.sq < kTile ? a.s.sq : kTile))), dim3(128), 0,
-                           0, stream, a);
+  const int rows = a.packed > 1 ? a.packed * a.s.sq : a.s.sq < kTile ? a.s.sq : kTile;
+  const dim3 joins(static_cast<unsigned>(c.units * rows));
+  return c.splits > 16 ? launch_overlapped(split_attention_kernel<AB, 16>, joins, dim3(512), 0, 0, stream, a)
+                       : launch_overlapped(split_attention_kernel<AB, 4>, joins, dim3(128), 0, 0, stream, a);
 }
 
 }  // namespace
@@ -769,9 +797,10 @@ extern "C" int peco_span_attention(const void* q, const void* k, const void* v, 
   a.out_row = o.row;
   a.lse = lse;
   a.packed = c.packed;
-  a.row_blocks = c.row_blocks;
-  a.together = heads_together(a.s, c.row_blocks, heads / c.packed);
-  a.splits = c.splits;
+  a.turns = turns(a.s, c.row_blocks, heads / c.packed);
+  a.splits = divisor(c.splits);
+  a.rows = divisor(sq);
+  a.s.group = divisor(heads / kv_heads);
   a.part = static_cast<float*>(workspace);
   a.part_sums = reinterpret_cast<float2*>(static_cast<float*>(workspace) + part_rows(c) * d);
   const HeadRows none{q, 0, 0, 0};  // without keys nothing is loaded

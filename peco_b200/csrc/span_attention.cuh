@@ -25,12 +25,44 @@ struct HeadRows {
   long long batch, head, row;
 };
 
+// n / by for 0 <= n < 2^31, without the divide's latency (a CTA's place takes seven of
+// them in a row before its first load, 1200 clocks; 592 CTAs of one key tile 24.0 us
+// and 22.4).  mul = ceil(2^s / by) with s = 31 +
+// ceil(log2 by): mul by - 2^s < by <= 2^(s - 31), so n mul / 2^s is off by less than 1 / by.
+struct Divisor {
+  unsigned mul;
+  int by, shift;
+  __device__ __forceinline__ int operator()(int n) const {
+    return static_cast<int>(static_cast<unsigned long long>(n) * mul >> shift);
+  }
+};
+inline Divisor divisor(int by) {
+  int log = 0;
+  while ((1LL << log) < by) ++log;
+  const unsigned long long whole = 1ull << (31 + log);
+  return Divisor{static_cast<unsigned>((whole + by - 1) / by), by, 31 + log};
+}
+
+// Units (heads by tiles of rows, of every sample) in the order in which CTAs take them
+struct Turns {
+  Divisor sample, chunk, heads, rest;  // units of a sample and of the heads in turn; heads in turn, and of the last ones
+  int tiles, all;                      // tiles of rows, heads
+  __device__ __forceinline__ void at(int unit, int& b, int& head, int& rank) const {
+    b = sample(unit);
+    const int n = unit - b * sample.by, first = chunk(n) * heads.by, m = n - first * tiles;
+    const Divisor& of = all - first < heads.by ? rest : heads;
+    rank = of(m);
+    head = first + m - rank * of.by;
+  }
+};
+
 struct ScoreArgs {
-  const int4* spans;        // [batch or 1, sq]: lo, hi, pos, 0 (null: every row sees every key, pos = i + sk - sq)
+  const int4* spans;        // [batch or 1, sq]: lo, hi, pos, ranked tile (null: every row sees every key, pos = i + sk - sq)
   const int4* span_tiles;   // [batch or 1, ceil(sq / 128)]: least lo, largest hi, largest lo, least hi of the rows
   int spans_batched;
   const float* slopes;      // [heads] or null
   int batch, heads, kv_heads, sq, sk, d;
+  Divisor group;            // heads on a key head
   float scale;              // > 0
   float cap;                // 0: none
   unsigned* status;
@@ -57,10 +89,10 @@ __device__ __forceinline__ int ranked_tile(const ScoreArgs& a, int b, int n, int
 // of every head; no more heads than fill the SMs twice, for their keys to stay in L2.
 // With the longest first, 8 heads of 9999 rows in four documents 162 -> 125 us, in
 // causal order with 64 dims 98 -> 76 us (a window of 1000 on 16000 rows 448 -> 458 us).
-inline int heads_together(const ScoreArgs& a, int tiles, int heads) {
-  if (!a.spans) return 1;
-  const int fill = (2 * kNumSMs + tiles - 1) / tiles;
-  return fill < heads ? fill : heads;
+inline Turns turns(const ScoreArgs& a, int tiles, int heads) {
+  const int fill = a.spans ? (2 * kNumSMs + tiles - 1) / tiles : 1, together = fill < heads ? fill : heads;
+  return Turns{divisor(heads * tiles), divisor(together * tiles), divisor(together),
+               divisor(heads % together ? heads % together : together), tiles, heads};
 }
 
 // cap tanh(s / cap) in log2 units: with A = cap log2(e) and e = 2^(2 log2(e) s
@@ -123,6 +155,33 @@ __device__ __forceinline__ void less_distance(float slope, float apart, float (&
 #pragma unroll
   for (int e = 0; e < N; ++e) z[e] = fmaf(-slope, fabsf(apart - static_cast<float>(e)), z[e]);
 }
+
+// 16-bit rows that the lanes of a warp hold, on their way to memory through shared
+// memory, so that a store writes whole rows: 16 bytes of 32 rows each take the
+// store unit eight times as long (24 heads x 16000 rows under a window of 1000: 449
+// and 436 us).  ``at``: 32 rows of COLS, the warp's own.
+template <int COLS>
+struct RowsOut {
+  static constexpr int kChunks = COLS / 8, kTurn = 32 / kChunks;  // 16-byte chunks of a row, rows a store writes
+  unsigned char* at;
+  int lane;
+  __device__ __forceinline__ uint4* place(int row, int chunk) const {  // turned, so that eight lanes meet all banks
+    return reinterpret_cast<uint4*>(at) + row * kChunks + (chunk ^ (kChunks >= 8 ? row & 7 : row >> 1 & 3));
+  }
+  __device__ __forceinline__ void put(int chunk, uint4 v) const { *place(lane, chunk) = v; }
+  // every lane's row to its ``out`` (null: nowhere), the first ``cols`` columns
+  template <typename T>
+  __device__ __forceinline__ void store(T* out, int cols) const {
+    __syncwarp();
+    const int chunk = lane % kChunks;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const int row = i * kTurn + lane / kChunks;
+      T* to = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(out), row));
+      if (to && chunk * 8 < cols) *reinterpret_cast<uint4*>(to + chunk * 8) = *place(row, chunk);
+    }
+  }
+};
 
 // 128 columns of a TMEM lane: four loads in flight, one wait.
 __device__ __forceinline__ void tmem_ld128_sync(uint32_t at, uint32_t (&r)[128]) {

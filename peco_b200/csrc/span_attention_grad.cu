@@ -44,7 +44,8 @@ struct GradArgs {
   void *dq, *dk, *dv;
   long long q_batch, q_head, q_row, k_batch, k_head, k_row, v_batch, v_head, v_row;
   int key_units, query_units;
-  int together;              // heads whose query tiles are taken in turn
+  Turns turns;               // of heads and their query tiles
+  Divisor blocks, by_parts, kv;  // tiles of keys, parts, key heads
   int parts;                 // CTAs that share a tile of keys, each some of the heads on them
   float* part;               // with several: dv, then dk, [parts, batch, key heads, keys, dims] each
 };
@@ -154,9 +155,9 @@ __device__ __forceinline__ void store_half(uint32_t at, const float (&v)[64]) {
   tmem_st_wait();
 }
 
-// A row of an accumulator, scaled, to memory (zeros without one)
+// Rows of an accumulator, scaled, to memory (zeros without one) by way of ``stage``
 template <typename T, int D>
-__device__ __forceinline__ void store_row(T* out, uint32_t at, float scale, int d, bool any) {
+__device__ __forceinline__ void store_row(T* out, uint32_t at, float scale, int d, bool any, const RowsOut<D>& stage) {
 #pragma unroll
   for (int c = 0; c < D / 32; ++c) {
     uint32_t raw[32];
@@ -164,18 +165,16 @@ __device__ __forceinline__ void store_row(T* out, uint32_t at, float scale, int 
     else
 #pragma unroll
       for (int e = 0; e < 32; ++e) raw[e] = 0u;
-    if (out) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        if (c * 32 + g * 8 < d) {
-          uint32_t u[4];
+    for (int g = 0; g < 4; ++g) {
+      uint32_t u[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            u[e] = pack2<T>(__uint_as_float(raw[g * 8 + 2 * e]) * scale, __uint_as_float(raw[g * 8 + 2 * e + 1]) * scale);
-          *reinterpret_cast<uint4*>(out + c * 32 + g * 8) = make_uint4(u[0], u[1], u[2], u[3]);
-        }
+      for (int e = 0; e < 4; ++e)
+        u[e] = pack2<T>(__uint_as_float(raw[g * 8 + 2 * e]) * scale, __uint_as_float(raw[g * 8 + 2 * e + 1]) * scale);
+      stage.put(c * 4 + g, make_uint4(u[0], u[1], u[2], u[3]));
     }
   }
+  stage.store(out, d);
 }
 
 // The same in fp32, for the sum over the parts
@@ -280,18 +279,18 @@ __global__ void __launch_bounds__(kGradThreads, 1)
   wait_for_prior();
   let_next_start();
   const uint32_t tmem = sh.tmem;
-  const int group = a.s.heads / a.s.kv_heads;
+  const int group = a.s.group.by;
   const int half = (warp >> 2) & 1;  // of a softmax warp: its 64 columns
   const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
   const int r = (warp & 3) * 32 + lane;
   const float scale_log2 = a.s.scale * kLog2E;
+  const RowsOut<D> stage{base + warp * (32 * D * 2), lane};  // of a softmax warp, where the CTA's own tiles are read no more
 
   if (of_keys) {
     // ================================================================ dk and dv of 128 keys
-    const int blocks = (a.s.sk + kTile - 1) / kTile;
-    const int j0 = static_cast<int>(blockIdx.x) % blocks * kTile, unit = static_cast<int>(blockIdx.x) / blocks;
-    const int part = unit % a.parts, kv = unit / a.parts % a.s.kv_heads, b = unit / a.parts / a.s.kv_heads;
-    const int head0 = kv * group + part * group / a.parts, head_end = kv * group + (part + 1) * group / a.parts;
+    const int unit = a.blocks(blockIdx.x), j0 = (static_cast<int>(blockIdx.x) - unit * a.blocks.by) * kTile;
+    const int heads = a.by_parts(unit), part = unit - heads * a.parts, b = a.kv(heads), kv = heads - b * a.s.kv_heads;
+    const int head0 = kv * group + a.by_parts(part * group), head_end = kv * group + a.by_parts((part + 1) * group);
     const int tiles = row_tiles(a.s);
     if (a.s.spans) {  // the query tiles between the first and the last that see one of the keys
       for (int t = threadIdx.x; t < tiles; t += kGradThreads) {
@@ -569,17 +568,16 @@ __global__ void __launch_bounds__(kGradThreads, 1)
           if (wanted)
             out = half ? static_cast<T*>(a.dk) + b * a.k_batch + kv * a.k_head + static_cast<long long>(j) * a.k_row
                        : static_cast<T*>(a.dv) + b * a.v_batch + kv * a.v_head + static_cast<long long>(j) * a.v_row;
-          store_row<T, D>(out, at, back, a.s.d, any);
+          store_row<T, D>(out, at, back, a.s.d, any, stage);
         }
       }
     }
   } else {
     // ================================================================ dq of 128 query rows
     const int tiles = row_tiles(a.s), unit = static_cast<int>(blockIdx.x) - a.key_units;
-    const int sample = a.s.heads * tiles, b = unit / sample, n = unit - b * sample;
-    const int first = n / (a.together * tiles) * a.together, heads = min(a.together, a.s.heads - first), m = n - first * tiles;
-    const int head = first + m % heads, tile = ranked_tile(a.s, b, m / heads, tiles);
-    const int i0 = tile * kTile, kv = head / group;
+    int b, head, rank;
+    a.turns.at(unit, b, head, rank);
+    const int tile = ranked_tile(a.s, b, rank, tiles), i0 = tile * kTile, kv = a.s.group(head);
     const int4 seen = tile_span(a.s, b, tile);
     const int key0 = max(seen.x, 0), key_end = min(seen.y, a.s.sk);
     const int ntiles = key_end > key0 ? (key_end - key0 + kTile - 1) / kTile : 0;
@@ -731,7 +729,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
       if (me.ok && half == 0) {
         // (a row that sees nothing: its g may hold anything)
         T* out = real ? static_cast<T*>(a.dq) + b * a.q_batch + head * a.q_head + static_cast<long long>(i) * a.q_row : nullptr;
-        store_row<T, D>(out, dq_at + lanes, a.s.scale, a.s.d, ntiles > 0);
+        store_row<T, D>(out, dq_at + lanes, a.s.scale, a.s.d, ntiles > 0, stage);
       }
     }
   }
@@ -867,7 +865,6 @@ extern "C" int peco_span_attention_backward(const void* grad, const void* q, con
   a.lse = lse;
   a.stats = static_cast<float2*>(workspace);
   a.padded = static_cast<int>(padded_rows(sq));
-  a.together = sq > 0 ? heads_together(a.s, a.padded / kTile, heads) : 1;
   a.parts = key_parts(batch, heads, kv_heads, sq, sk, span_rows != nullptr);
   a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + stats_bytes(batch, heads, sq));
   a.dq = dq;
@@ -886,6 +883,11 @@ extern "C" int peco_span_attention_backward(const void* grad, const void* q, con
   const long long query_units = rows ? static_cast<long long>(batch) * heads * (a.padded / kTile) : 0;
   const long long stat_blocks = static_cast<long long>(batch) * heads * a.padded / 16;
   if (key_units + query_units > 0x7fffffffLL || stat_blocks > 0x7fffffffLL) return kErrUnsupported;
+  if (query_units > 0) a.turns = turns(a.s, a.padded / kTile, heads);
+  if (key_units > 0) a.blocks = divisor((sk + kTile - 1) / kTile);
+  a.by_parts = divisor(a.parts);
+  a.kv = divisor(kv_heads);
+  a.s.group = divisor(heads / kv_heads);
   a.key_units = static_cast<int>(key_units);
   a.query_units = static_cast<int>(query_units);
   // an empty side is never loaded: its maps stand on the other's rows
