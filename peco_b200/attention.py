@@ -16,8 +16,9 @@ the current stream.
 
 from __future__ import annotations
 
-import ctypes
+import functools
 import math
+import struct
 from dataclasses import dataclass
 from typing import NamedTuple, Optional
 
@@ -26,8 +27,8 @@ from torch.autograd.function import once_differentiable
 
 from . import _native
 
-_Strides = ctypes.c_longlong * 12
-_GradStrides = ctypes.c_longlong * 24
+_strides = struct.Struct("=12q").pack  # (quicker to make than an array of ctypes)
+_grad_strides = struct.Struct("=24q").pack
 _SIXTEEN_BITS = (torch.float16, torch.bfloat16)
 
 
@@ -223,6 +224,11 @@ def _mask_args(spans, b):
     return spans.rows.data_ptr(), spans.tiles.data_ptr(), 1 if spans.rows.shape[0] == b and b > 1 else 0
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(*sizes) -> int:
+    return int(_native.load().peco_span_attention_workspace(*sizes))
+
+
 def _forward(q, k, v, spans, scale, softcap, slopes):
     (b, h, kv, n, m, d), scale, cap = _check(q, k, v, spans, scale, softcap, slopes)
     mask = (None, None) if spans is None else (spans.rows, spans.tiles)
@@ -237,9 +243,9 @@ def _forward(q, k, v, spans, scale, softcap, slopes):
     if slopes is not None:
         slopes = slopes.contiguous()
     lib = _native.load()
-    need = int(lib.peco_span_attention_workspace(b, h, kv, n, m, d))
+    need = _workspace_bytes(b, h, kv, n, m, d)
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
-    strides = _Strides(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *whole.stride()[:3])
+    strides = _strides(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *whole.stride()[:3])
     rows, tiles, batched = _mask_args(spans, b)
     _native.enqueue(device, "peco_span_attention", lib.peco_span_attention,
                     (q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, rows, tiles, batched, _native.address(slopes), scale,
@@ -333,7 +339,7 @@ def attention_backward(grad, q, k, v, out, lse, *, spans=None, scale=None, softc
         need = int(lib.peco_span_attention_backward_workspace(b, h, kv, n, m, d, 0 if spans is None else 1))
         ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
         to = [whole.get(name) for name in "qkv"]
-        strides = _GradStrides(*(s for t in (grad, q, k, v, out, *to) for s in (t.stride()[:3] if t is not None else (0, 0, 0))))
+        strides = _grad_strides(*(s for t in (grad, q, k, v, out, *to) for s in (t.stride()[:3] if t is not None else (0, 0, 0))))
         rows, tiles, batched = _mask_args(spans, b)
         _native.enqueue(device, "peco_span_attention_backward", lib.peco_span_attention_backward,
                         (grad.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), strides,
