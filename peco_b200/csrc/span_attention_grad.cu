@@ -88,10 +88,13 @@ __global__ void __launch_bounds__(256) grad_stats_kernel(const __grid_constant__
 template <bool RICH>
 struct Step {
   float lse[kTile], delta[kTile];
-  uint32_t range[kTile / 2];  // bytes: first key of the tile that a row sees, and the key behind the last
+  uint32_t range[kTile / 2];  // 16 bits a row: first key of the tile that it sees (0 to 127), kOneKey, the key behind the last << 8
   float pos[RICH ? kTile : 4];
-  int masked, clear, end, head;
+  int masked, clear, end, head;  // masked: 1, or 2 with rows of one key
 };
+// A row that sees one key has p = 1 whatever its score, so its ds are 0: the difference
+// of g.v and delta, sums of different orders, would be what is left of their rounding.
+constexpr uint32_t kOneKey = 0x80, kBlind = 0xff;  // a row that sees nothing: kOneKey, from 127 to 0
 
 template <bool RICH>
 struct __align__(16) GradShared {
@@ -346,11 +349,12 @@ __global__ void __launch_bounds__(kGradThreads, 1)
           constexpr int kEach = kTile / 32;
           float2 stat[kEach];
           int4 span[kEach];
-          bool full = true, blind = false;
+          bool full = true, blind = false, ones = false;
           if (more) {
             const int i0 = walk.tile * kTile;
             const int4 t = tile_span(a.s, b, walk.tile);
-            full = t.z <= j0 && t.w >= min(j0 + kTile, a.s.sk) && i0 + kTile <= a.s.sq;
+            // (a row that sees the last key alone would pass for one that sees the whole tile)
+            full = t.z <= j0 && t.w >= min(j0 + kTile, a.s.sk) && t.z < a.s.sk - 1 && i0 + kTile <= a.s.sq;
             blind = t.z == 0x7fffffff;  // some row sees nothing
             const float2* stats = a.stats + (static_cast<long long>(b) * a.s.heads + walk.head) * a.padded + i0;
 #pragma unroll
@@ -358,7 +362,9 @@ __global__ void __launch_bounds__(kGradThreads, 1)
               const int i = i0 + e * 32 + lane;
               stat[e] = stats[e * 32 + lane];
               span[e] = (RICH || !full) && i < a.s.sq ? span_of(a.s, b, i) : make_int4(0, 0, 0, 0);
+              ones = ones || span[e].y - span[e].x == 1;
             }
+            ones = __any_sync(0xffffffffu, ones);
           }
           Step<RICH>& step = sh.step[n & 1];
           if (!me.wait(&sh.step_empty[n & 1], (n >> 1) + 1)) break;
@@ -370,14 +376,14 @@ __global__ void __launch_bounds__(kGradThreads, 1)
               step.delta[i] = stat[e].y;
               if (RICH || !full) {
                 const int from = min(max(span[e].x - j0, 0), kTile), to = min(max(span[e].y - j0, 0), kTile);
-                // a row that sees nothing at all is told apart by the order of the two
-                reinterpret_cast<uint16_t*>(step.range)[i] = static_cast<uint16_t>(span[e].y > span[e].x ? from | to << 8 : 255);
+                const uint32_t seen = (from < to ? from | to << 8 : 0) | (span[e].y - span[e].x == 1 ? kOneKey : 0);
+                reinterpret_cast<uint16_t*>(step.range)[i] = static_cast<uint16_t>(span[e].y > span[e].x ? seen : kBlind);
                 if constexpr (RICH) step.pos[i] = static_cast<float>(span[e].z - j0);  // from the tile's first key
               }
             }
             if (lane == 0) {
               step.head = walk.head;
-              step.masked = full ? 0 : 1;
+              step.masked = full ? 0 : ones ? 2 : 1;
               step.clear = blind ? 1 : 0;
             }
           }
@@ -400,7 +406,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
           if (step.clear) {
             if (!me.wait(&sh.second_full[s.s], s.phase)) return false;
             for (int row = lane; row < kTile; row += 32)
-              if ((reinterpret_cast<const uint16_t*>(step.range)[row] & 255) == 255)
+              if (reinterpret_cast<const uint16_t*>(step.range)[row] == kBlind)
                 for (int p = 0; p < kPanels; ++p)
                   for (int c = 0; c < 8; ++c) {
                     *reinterpret_cast<uint4*>(firsts + f.s * kTileBytes + p * kPanelBytes + row * 128 + c * 16) = make_uint4(0, 0, 0, 0);
@@ -512,13 +518,13 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         }
 #pragma unroll
         for (int e = 0; e < 64; ++e) p[e] = exp2_approx(p[e]);
-        const bool masked = step.masked;
+        const int masked = step.masked;
         if (masked) {
 #pragma unroll
           for (int e = 0; e < 64; e += 2) {
             const uint32_t two = step.range[(c0 + e) >> 1];
-            p[e] = r >= static_cast<int>(two & 255u) && r < static_cast<int>(two >> 8 & 255u) ? p[e] : 0.0f;
-            p[e + 1] = r >= static_cast<int>(two >> 16 & 255u) && r < static_cast<int>(two >> 24) ? p[e + 1] : 0.0f;
+            p[e] = r >= static_cast<int>(two & 127u) && r < static_cast<int>(two >> 8 & 255u) ? p[e] : 0.0f;
+            p[e + 1] = r >= static_cast<int>(two >> 16 & 127u) && r < static_cast<int>(two >> 24) ? p[e + 1] : 0.0f;
           }
         }
         store_half<T>(s_own, p);
@@ -550,6 +556,14 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         if (masked) {  // a masked pair's g.v may be anything
 #pragma unroll
           for (int e = 0; e < 64; ++e) ds[e] = p[e] == 0.0f ? 0.0f : ds[e];
+          if (masked > 1) {  // (a NaN stays)
+#pragma unroll
+            for (int e = 0; e < 64; e += 2) {
+              const uint32_t two = step.range[(c0 + e) >> 1];
+              if (two & kOneKey) ds[e] *= 0.0f;
+              if (two & kOneKey << 16) ds[e + 1] *= 0.0f;
+            }
+          }
         }
         store_half<T>(dp_own, ds);
         me.arrive(&sh.ds_full[0]);
@@ -673,6 +687,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
       const float2 stat = a.stats[(static_cast<long long>(b) * a.s.heads + head) * a.padded + i];
       const Cap cap(a.s);
       const float bias = RICH && a.s.slopes ? a.s.slopes[head] * kLog2E : 0.0f;
+      const bool one = span.y - span.x == 1, ones = __any_sync(0xffffffffu, one);
       const float2 neg2 = make_float2(-stat.x, -stat.x), scale2 = make_float2(scale_log2, scale_log2);
       const float2 back = make_float2(Held<AB>::kBack, Held<AB>::kBack), delta2 = make_float2(-stat.y, -stat.y);
       for (int t = 0; t < ntiles; ++t) {
@@ -721,6 +736,15 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         if (masked) {  // a masked pair's g.v may be anything
 #pragma unroll
           for (int e = 0; e < 64; ++e) ds[e] = e >= from && e < to ? ds[e] : 0.0f;
+          if (ones) {  // (rows of one key are never whole)
+            const float2 keep = one ? make_float2(0.0f, 0.0f) : make_float2(1.0f, 1.0f);
+#pragma unroll
+            for (int e = 0; e < 64; e += 2) {
+              const float2 x = fmul2(make_float2(ds[e], ds[e + 1]), keep);
+              ds[e] = x.x;
+              ds[e + 1] = x.y;
+            }
+          }
         }
         store_half<T>(s_own, ds);
         me.arrive(&sh.ds_full[t & 1]);  // two barriers: a fast warp may be through the next step before a slow one is here
