@@ -531,6 +531,10 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         me.arrive(&sh.p_full);
         if constexpr (RICH) {
           if (a.s.cap > 0.0f) {
+            if (masked) {  // a score of NaN has a slope of NaN: 0 in its place, for the 0 of a masked pair (a seen one's p is NaN)
+#pragma unroll
+              for (int e = 0; e < 64; ++e) slopes[e] = fmaxf(slopes[e], 0.0f);
+            }
 #pragma unroll
             for (int e = 0; e < 64; e += 2) {
               const float2 x = fmul2(make_float2(p[e], p[e + 1]), make_float2(slopes[e], slopes[e + 1]));
