@@ -201,6 +201,37 @@ __device__ __forceinline__ void store_part(float* out, uint32_t at, float scale,
   }
 }
 
+// Zeros in the rows of a tile of keys that no row of a tile of query rows sees (they may
+// hold anything, and 0 times that would reach dq), by one warp; visible to the tensor
+// core.  ``spans``: four query rows' a lane; j0: the tile's first key.
+template <int PANELS>
+__device__ __forceinline__ void clear_unseen(unsigned char* tile, const int4 (&spans)[kTile / 32], int j0, int lane) {
+  uint32_t seen[kTile / 32] = {};  // a bit a key
+  bool whole = false;              // a row that sees all
+#pragma unroll
+  for (int i = 0; i < kTile / 32; ++i) {
+    const int from = max(spans[i].x - j0, 0), to = min(spans[i].y - j0, kTile);
+    whole = whole || to - from == kTile;
+#pragma unroll
+    for (int w = 0; w < kTile / 32; ++w) {
+      const int lo = max(from - 32 * w, 0), hi = min(to - 32 * w, 32);
+      if (lo < hi) seen[w] |= 0xffffffffu >> (32 - (hi - lo)) << lo;
+    }
+  }
+  if (__any_sync(0xffffffffu, whole)) return;
+#pragma unroll
+  for (int w = 0; w < kTile / 32; ++w) {
+    const bool blind = !(__reduce_or_sync(0xffffffffu, seen[w]) >> lane & 1u);
+    if (blind)
+#pragma unroll
+      for (int p = 0; p < PANELS; ++p)
+        for (int c = 0; c < 8; ++c)
+          *reinterpret_cast<uint4*>(tile + p * kPanelBytes + (32 * w + lane) * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_async_smem();
+  __syncwarp();
+}
+
 // The steps of a CTA of keys: heads of the group, query tiles that see one of its keys.
 struct StepWalk {
   int head, tile;
@@ -635,10 +666,17 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         const uint32_t at = uniform(tmem);
         const uint32_t q = uniform(desc_dims(smem_u32(base))), k = uniform(desc_dims(smem_u32(firsts)));
         const int last = static_cast<int>(uniform(ntiles)) - 1;
+        // spans that share a key or meet (the largest first key is not behind the least last) leave none out between them
+        const bool gaps = seen.z > seen.w;
+        int4 spans[kTile / 32];
+#pragma unroll
+        for (int i = 0; i < kTile / 32; ++i)
+          spans[i] = gaps && i0 + i * 32 + lane < a.s.sq ? span_of(a.s, b, i0 + i * 32 + lane) : make_int4(0, 0, 0, 0);
         RingPos f{0, 0};
         me.wait(&sh.own_full, 0);
         for (int t = 0; t <= last && me.ok; ++t) {
           if (!me.wait(&sh.first_full[f.s], f.phase)) break;
+          if (gaps) clear_unseen<kPanels>(firsts + f.s * kTileBytes, spans, key0 + t * kTile, lane);
           const int left = key_end - (key0 + t * kTile);  // keys past these are nobody's and may hold anything
           if (left < kTile) clear_rows<kPanels>(firsts + f.s * kTileBytes, left, kTile, lane);
           // dq's product two tiles before has read the buffer

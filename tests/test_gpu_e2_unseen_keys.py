@@ -45,3 +45,24 @@ def test_behind_the_last_key(bad, args):
                                (2, 2, 140, 500, dict(documents=[0, 60, 80], key_documents=[0, 250, 400]))):
         for d, dtype in ((64, torch.bfloat16), (128, torch.float16)):
             unseen_keys(bad, h, kv, n, m, words, d, dtype, args)
+
+
+# documents with keys and no rows, and more keys than rows under a window: what nobody sees lies between keys that are seen
+GAPS = [
+    (60, 300, dict(documents=[0, 30, 30, 60], key_documents=[0, 100, 200, 300])),
+    (60, 300, dict(documents=[0, 30, 60], key_documents=[0, 150, 300], window=4)),
+    (60, 2000, dict(documents=[0, 30, 60], key_documents=[0, 900, 2000], window=20, causal=True)),
+    (300, 1500, dict(documents=[0, 100, 100, 250, 290], key_documents=[0, 130, 700, 1000, 1200])),
+    (300, 400, dict(documents=[0, 128, 128, 300], key_documents=[0, 127, 129, 300])),
+    (40, 400, dict(documents=list(range(0, 41)), key_documents=list(range(0, 401, 10)), window=2)),
+    (200, 700, dict(documents=[0, 90, 90, 200], key_documents=[0, 200, 201, 700], causal=True, prefix=30)),
+]
+
+
+@pytest.mark.parametrize("args", SCORES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("gap", GAPS)
+def test_between_the_spans_of_a_tile(gap, bad, args):
+    n, m, words = gap
+    for h, kv, d, dtype in ((2, 2, 128, torch.bfloat16), (4, 1, 40, torch.float16)):
+        unseen_keys(bad, h, kv, n, m, words, d, dtype, args)
