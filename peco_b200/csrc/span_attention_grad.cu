@@ -37,7 +37,7 @@ constexpr int kFirst = RICH ? 2 : 3;  // (capped or biased scores keep the rows'
 
 struct GradArgs {
   ScoreArgs s;
-  HeadRows out, grad;        // of the statistics
+  HeadRows out, grad, q, k, v;  // of the statistics
   const float* lse;
   float2* stats;             // [batch, heads, padded rows]: lse in log2 units (none: infinity) and delta
   int padded;                // rows, a multiple of 128
@@ -57,20 +57,95 @@ struct Held {
   static constexpr float kShift = AB == 1 ? 0.0f : 10.0f, kBack = AB == 1 ? 1.0f : 1.0f / 1024.0f;
 };
 
-// stats of every row; 16 lanes a row
+// Rows of up to this many keys take delta from their probabilities.  The rounding of
+// ``out`` is one error in every ds of a row, and the fewer the keys, the more of ds it
+// is: relative error of dq over 2 keys 0.0038 (bf16) with it and 0.0023 without, 4
+// keys 0.0030, 8 keys 0.0027, 128 keys 0.0024.  The statistics of 24 heads x 16000 rows
+// of 7 keys each take 232 us with it (39 without), of 24 x 4096 rows in causal order 15 (12).
+constexpr int kFewKeys = 8;
+
+// sum_j p_j (g.v_j) over a row's ``count`` keys from ``lo`` on, 16 lanes a row with 8 dims
+// each, two keys at a time.  By whole warps.
 template <int AB>
-__global__ void __launch_bounds__(256) grad_stats_kernel(const __grid_constant__ GradArgs a) {
+__device__ __noinline__ float few_keys_delta(const GradArgs& a, int b, int h, int i, int lo, int pos, int count, float lse,
+                                             int lane) {
+  using T = Element<AB>;
+  const int most = __reduce_max_sync(0xffffffffu, count), kv = a.s.group(h), at = lane >> 3 & 1;
+  const float slope = a.s.slopes ? a.s.slopes[h] * kLog2E : 0.0f;
+  const Cap cap(a.s);
+  float q[8] = {}, g[8] = {}, delta = 0.0f;
+  if (lane * 8 >= a.s.d) count = 0;  // (of what this lane reads)
+  const int reads = count;
+  count = __shfl_sync(0xffffffffu, count, threadIdx.x & 16);
+  if (reads > 0) {
+    load8(static_cast<const T*>(a.grad.ptr) + b * a.grad.batch + h * a.grad.head + static_cast<long long>(i) * a.grad.row + lane * 8, 1, 8, g);
+    load8(static_cast<const T*>(a.q.ptr) + b * a.q.batch + h * a.q.head + static_cast<long long>(i) * a.q.row + lane * 8, 1, 8, q);
+  }
+  const T* k = static_cast<const T*>(a.k.ptr) + b * a.k.batch + kv * a.k.head + lo * a.k.row + lane * 8;
+  const T* v = static_cast<const T*>(a.v.ptr) + b * a.v.batch + kv * a.v.head + lo * a.v.row + lane * 8;
+  for (int n = 0; n < most; n += 2) {
+    float score[2] = {}, gv[2] = {};
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (n + u < reads) {
+        float x[8];
+        load8(k, 1, 8, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) score[u] = fmaf(q[e], x[e], score[u]);
+        load8(v, 1, 8, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) gv[u] = fmaf(g[e], x[e], gv[u]);
+      }
+      k += a.k.row;
+      v += a.v.row;
+    }
+    // sums over the lanes: half of them take one key, and of those half the score
+    const bool second = lane & 8, value = lane & 4;
+    float s = second ? score[1] : score[0], y = second ? gv[1] : gv[0];
+    s += __shfl_xor_sync(0xffffffffu, second ? score[0] : score[1], 8);
+    y += __shfl_xor_sync(0xffffffffu, second ? gv[0] : gv[1], 8);
+    float sum = value ? y : s;
+    sum += __shfl_xor_sync(0xffffffffu, value ? s : y, 4);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    const float other = __shfl_xor_sync(0xffffffffu, sum, 4);
+    s = value ? other : sum;
+    y = value ? sum : other;
+    float z = a.s.cap > 0.0f ? cap.value(cap.recip(s)) : s * a.s.scale * kLog2E;
+    if (a.s.slopes) z = fmaf(-slope, fabsf(static_cast<float>(pos - lo - n - at)), z);
+    if (n + at < count) delta = fmaf(exp2_approx(z - lse), y, delta);
+  }
+  return delta + __shfl_xor_sync(0xffffffffu, delta, 8);
+}
+
+// stats of every row; 16 lanes a row.  FEW: some row may see few keys.
+template <int AB, bool FEW>
+__global__ void __launch_bounds__(256, 8) grad_stats_kernel(const __grid_constant__ GradArgs a) {
   using T = Element<AB>;
   wait_for_prior();
   let_next_start();
-  const unsigned blocks = static_cast<unsigned>(a.padded) >> 4, heads = blockIdx.x / blocks;  // of a head; head of all samples
-  const int i = static_cast<int>((blockIdx.x - heads * blocks) * 16 + (threadIdx.x >> 4)), lane = threadIdx.x & 15;
+  // the first rows of all heads first: in causal order they are those of few keys, which take longer
+  const unsigned all = static_cast<unsigned>(a.s.batch) * static_cast<unsigned>(a.s.heads), rows = blockIdx.x / all;
+  const unsigned heads = blockIdx.x - rows * all;  // head of all samples
+  const int i = static_cast<int>(rows * 16 + (threadIdx.x >> 4)), lane = threadIdx.x & 15;
   const int b = static_cast<int>(heads / a.s.heads), h = static_cast<int>(heads % a.s.heads);
   const long long at = static_cast<long long>(heads) * a.padded + i;
-  float sum = 0.0f, l = -INFINITY;
-  if (i < a.s.sq) {
-    l = a.lse[static_cast<long long>(heads) * a.s.sq + i];
-    if (lane * 8 < a.s.d) {
+  bool few = false;
+  float l = -INFINITY, sum = 0.0f;
+  if (i < a.s.sq) l = a.lse[static_cast<long long>(heads) * a.s.sq + i];
+  if constexpr (FEW) {
+    // a row of the tile sees at least the keys from the largest first to the least last
+    const int4 bounds = tile_span(a.s, b, static_cast<int>(rows / (kTile / 16)));
+    if (bounds.w <= kFewKeys || bounds.z >= bounds.w - kFewKeys) {
+      int4 span = make_int4(0, 0, 0, 0);
+      if (i < a.s.sq) span = span_of(a.s, b, i);
+      few = span.x >= 0 && span.y <= a.s.sk && span.y - span.x <= kFewKeys && span.y > span.x;
+      if (__any_sync(0xffffffffu, few)) sum = few_keys_delta<AB>(a, b, h, i, span.x, span.z, few ? span.y - span.x : 0, l * kLog2E, lane);
+    }
+  }
+  if (!few) {
+    sum = 0.0f;
+    if (i < a.s.sq && lane * 8 < a.s.d) {
       float x[8], y[8];
       load8(static_cast<const T*>(a.out.ptr) + b * a.out.batch + h * a.out.head + static_cast<long long>(i) * a.out.row + lane * 8, 1, 8, x);
       load8(static_cast<const T*>(a.grad.ptr) + b * a.grad.batch + h * a.grad.head + static_cast<long long>(i) * a.grad.row + lane * 8, 1, 8, y);
@@ -78,8 +153,10 @@ __global__ void __launch_bounds__(256) grad_stats_kernel(const __grid_constant__
       for (int e = 0; e < 8; ++e) sum = fmaf(x[e], y[e], sum);
     }
   }
+  float all16 = sum;
 #pragma unroll
-  for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  for (int o = 8; o; o >>= 1) all16 += __shfl_xor_sync(0xffffffffu, all16, o);
+  if (!few) sum = all16;
   if (lane == 0)
     a.stats[at] = l == -INFINITY ? make_float2(INFINITY, 0.0f) : make_float2(l * kLog2E - Held<AB>::kShift, sum * Held<AB>::kBack);
 }
@@ -863,7 +940,8 @@ int launch_grad(const GradArgs& a, const CUtensorMap (&maps)[4], cudaStream_t st
   if (cudaError_t e = grant_smem(reinterpret_cast<const void*>(kernel), smem, granted[rich])) return static_cast<int>(e);
   if (a.s.sq > 0) {
     const long long rows = static_cast<long long>(a.s.batch) * a.s.heads * a.padded;
-    if (int st = launch_overlapped(grad_stats_kernel<AB>, dim3(static_cast<unsigned>(rows / 16)), dim3(256), 0, 0, stream, a)) return st;
+    auto stats = a.s.spans || a.s.sk <= kFewKeys ? grad_stats_kernel<AB, true> : grad_stats_kernel<AB, false>;
+    if (int st = launch_overlapped(stats, dim3(static_cast<unsigned>(rows / 16)), dim3(256), 0, 0, stream, a)) return st;
   }
   if (int st = launch_overlapped(kernel, dim3(a.key_units + a.query_units), dim3(kGradThreads), smem, 0, stream, maps[0],
                                  maps[1], maps[2], maps[3], a))
@@ -927,6 +1005,9 @@ extern "C" int peco_span_attention_backward(const void* grad, const void* q, con
   a.s.cap = cap;
   a.s.status = device_status_ptr();
   a.grad = t[0];
+  a.q = t[1];
+  a.k = t[2];
+  a.v = t[3];
   a.out = t[4];
   a.lse = lse;
   a.stats = static_cast<float2*>(workspace);
