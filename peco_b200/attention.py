@@ -176,8 +176,6 @@ def _check(q, k, v, spans, scale, softcap, slopes):
     if slopes is not None:
         if not isinstance(slopes, torch.Tensor) or slopes.dtype is not torch.float32 or slopes.shape != (h,):
             raise ValueError(f"slopes must be a float32 tensor [{h}]")
-        if slopes.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("attention has no gradient of slopes")
     if spans is not None:
         if not isinstance(spans, KeySpans):
             raise TypeError("spans must come from key_spans")
@@ -190,6 +188,12 @@ def _check(q, k, v, spans, scale, softcap, slopes):
                 not spans.rows.is_contiguous() or not spans.tiles.is_contiguous():
             raise ValueError("spans must be as key_spans lays them out")
     return (b, h, kv, n, m, d), scale, cap
+
+
+def _refuse_slopes_gradient(slopes):
+    """Where grad mode is still the caller's: a Function's forward runs without."""
+    if isinstance(slopes, torch.Tensor) and slopes.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("attention has no gradient of slopes")
 
 
 def _on_one_device(q, *others):
@@ -281,7 +285,8 @@ def attention(q, k, v, *, spans=None, scale=None, softcap=None, slopes=None, ret
     ``spans``: what ``key_spans(B or 1, N, M, ...)`` gives; None: every row sees
     every key, and the last row stands at the last key.  ``scale`` defaults to
     D^-0.5.  ``softcap``: scores are softcap * tanh(score / softcap).  ``slopes``
-    float32 [H]: slope * |position - j| is taken from the score of key j.
+    float32 [H]: slope * |position - j| is taken from the score of key j (no
+    gradient of slopes: such a call is refused).
     ``return_lse``: also the logarithm of each row's sum of exponentials, float32
     [B, H, N] (no gradient flows through it), -inf where a row sees nothing.
 
@@ -291,6 +296,7 @@ def attention(q, k, v, *, spans=None, scale=None, softcap=None, slopes=None, ret
     out do not reach its result, whatever they hold.
     """
     _native.refuse_tangents("attention", q, k, v, slopes)
+    _refuse_slopes_gradient(slopes)
     if torch.is_grad_enabled() and _native.wants_grad(q, k, v):
         out, lse = _Attention.apply(q, k, v, spans, scale, softcap, slopes)
     else:
@@ -309,6 +315,7 @@ def attention_backward(grad, q, k, v, out, lse, *, spans=None, scale=None, softc
     the gradients of its tile.
     """
     _native.refuse_tangents("attention_backward", grad, q, k, v, out, slopes)
+    _refuse_slopes_gradient(slopes)
     sizes, scale, cap = _check(q, k, v, spans, scale, softcap, slopes)
     b, h, kv, n, m, d = sizes
     for name, t in (("grad", grad), ("out", out)):
