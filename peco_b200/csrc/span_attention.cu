@@ -243,7 +243,7 @@ __device__ __noinline__ void masked_row(const ForwardArgs& a, int b, int head, i
     if (j < hi) {
       float raw = 0.0f;
       for (int e = 0; e < d; ++e) raw = fmaf(to_f32<T>(q[e]), to_f32<T>(k[j * a.k.row + e]), raw);
-      float z = a.s.cap > 0.0f ? cap.value(cap.recip(raw)) : raw * a.s.scale * kLog2E;
+      float z = a.s.cap > 0.0f ? cap.value(raw, cap.recip(raw)) : raw * a.s.scale * kLog2E;
       if (a.s.slopes) z = fmaf(-slope, fabsf(static_cast<float>(pos - j)), z);
       p = exp2_approx(z - m);
     }
@@ -257,8 +257,8 @@ __device__ __noinline__ void masked_row(const ForwardArgs& a, int b, int head, i
   }
 }
 
-// RICH: capped scores or a bias by distance
-template <int AB, int D, bool RICH>
+// RICH: capped scores or a bias by distance; WIDE: a cap above kWideCap
+template <int AB, int D, bool RICH, bool WIDE>
 __global__ void __launch_bounds__(kThreads, 1)
     span_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                           const __grid_constant__ CUtensorMap vmap, const __grid_constant__ ForwardArgs a) {
@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 0; e < kTile; ++e) s[e] = __uint_as_float(raw[e]);
       }
       if constexpr (RICH) {  // to log2 units
-        scaled_scores(a.s, cap, s, nullptr);
+        scaled_scores<WIDE>(a.s, cap, s, nullptr);
         if (a.s.slopes) less_distance(slope, static_cast<float>(span.z - j0), s);
       }
       // rows past the tensor's end are not looked at
@@ -717,10 +717,11 @@ long long part_rows(const ForwardCut& c) { return c.splits > 1 ? c.units * c.spl
 
 template <int AB, int D>
 int launch_forward(const ForwardArgs& a, const ForwardCut& c, const CUtensorMap (&maps)[3], cudaStream_t stream) {
-  const bool rich = a.s.cap > 0.0f || a.s.slopes;
-  auto kernel = rich ? span_attention_kernel<AB, D, true> : span_attention_kernel<AB, D, false>;
-  static std::atomic<unsigned long long> granted[2] = {};
-  if (cudaError_t e = grant_smem(reinterpret_cast<const void*>(kernel), forward_smem<D>(), granted[rich])) return static_cast<int>(e);
+  const int form = score_form(a.s);
+  auto kernel = form == 2 ? span_attention_kernel<AB, D, true, true>
+                : form == 1 ? span_attention_kernel<AB, D, true, false> : span_attention_kernel<AB, D, false, false>;
+  static std::atomic<unsigned long long> granted[3] = {};
+  if (cudaError_t e = grant_smem(reinterpret_cast<const void*>(kernel), forward_smem<D>(), granted[form])) return static_cast<int>(e);
   const dim3 grid(static_cast<unsigned>(c.units * c.splits));
   if (int st = launch_overlapped(kernel, grid, dim3(kThreads), forward_smem<D>(), 0, stream, maps[0], maps[1], maps[2], a)) return st;
   if (c.splits == 1) return kOk;

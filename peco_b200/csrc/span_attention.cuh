@@ -97,16 +97,27 @@ inline Turns turns(const ScoreArgs& a, int tiles, int heads) {
 
 // cap tanh(s / cap) in log2 units: with A = cap log2(e) and e = 2^(2 log2(e) s
 // scale / cap), A tanh = A - 2A / (1 + e); infinite e gives A, e = 0 gives -A.
-// Within a few 2^-23 of A in absolute terms.
+// Within a few 2^-23 of A in absolute terms: for caps up to kWideCap 2e-5, a
+// probability's rounding to fp16 being 2^-12 of it.  Under larger caps that is all
+// that small scores are, so those below a quarter of the cap take the series x (1 -
+// x^2/3 + 2 x^4/15 - 17 x^6/315 + 62 x^8/2835), off by 2^-26 of the value (24 heads x 7006
+// rows of 128 dims: forward 1009 us without it and 1144 with it, gradient 2667 and
+// 3092), in kernels of their own (a branch on the cap cost the others 4%).
+constexpr float kWideCap = 64.0f;
 struct Cap {
-  float a, b;
-  __device__ explicit Cap(const ScoreArgs& s) : a(s.cap * kLog2E), b(2.0f * kLog2E * s.scale / s.cap) {}
+  float a, b, x, unit;
+  bool wide;
+  __device__ explicit Cap(const ScoreArgs& s)
+      : a(s.cap * kLog2E), b(2.0f * kLog2E * s.scale / s.cap), x(s.scale / s.cap), unit(s.scale * kLog2E), wide(s.cap > kWideCap) {}
   __device__ __forceinline__ float recip(float raw) const {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.0f + exp2_approx(raw * b)));
     return y;
   }
-  __device__ __forceinline__ float value(float r) const { return fmaf(-2.0f * a, r, a); }
+  __device__ __forceinline__ float value(float raw, float r) const {
+    const float2 twice = make_float2(raw, raw), both = make_float2(r, r);
+    return wide ? value<true>(twice, both).x : value<false>(twice, both).x;
+  }
   // two scores at a time
   __device__ __forceinline__ float2 recip(float2 raw) const {
     const float2 x = fmul2(raw, make_float2(b, b));
@@ -116,7 +127,18 @@ struct Cap {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(y.y));
     return r;
   }
-  __device__ __forceinline__ float2 value(float2 r) const { return ffma2(r, make_float2(-2.0f * a, -2.0f * a), make_float2(a, a)); }
+  template <bool WIDE>
+  __device__ __forceinline__ float2 value(float2 raw, float2 r) const {
+    const float2 whole = ffma2(r, make_float2(-2.0f * a, -2.0f * a), make_float2(a, a));
+    if constexpr (!WIDE) return whole;
+    auto both = [](float v) { return make_float2(v, v); };
+    const float2 y = fmul2(raw, both(x)), t = fmul2(y, y), s = fmul2(raw, both(unit));
+    float2 p = ffma2(t, both(62.0f / 2835.0f), both(-17.0f / 315.0f));
+    p = ffma2(t, p, both(2.0f / 15.0f));
+    p = ffma2(t, p, both(-1.0f / 3.0f));
+    p = ffma2(fmul2(t, p), s, s);
+    return make_float2(t.x < 0.0625f ? p.x : whole.x, t.y < 0.0625f ? p.y : whole.y);
+  }
   // d capped / d raw, without the scale: 1 - tanh^2 = 4 r - 4 r r (r rounded to 2^-24: off by a few 2^-24 in absolute terms)
   static __device__ __forceinline__ float2 slope(float2 r) {
     const float2 f = fmul2(r, make_float2(4.0f, 4.0f));
@@ -124,13 +146,13 @@ struct Cap {
   }
 };
 
-// N scores in log2 units, capped or scaled; the slopes of capped ones
-template <int N>
+// N scores in log2 units, capped (WIDE: by a cap above kWideCap) or scaled; the slopes of capped ones
+template <bool WIDE, int N>
 __device__ __forceinline__ void scaled_scores(const ScoreArgs& s, const Cap& cap, float (&z)[N], float* slopes) {
-  if (s.cap > 0.0f) {
+  if (WIDE || s.cap > 0.0f) {
 #pragma unroll
     for (int e = 0; e < N; e += 2) {
-      const float2 r = cap.recip(make_float2(z[e], z[e + 1])), v = cap.value(r);
+      const float2 raw = make_float2(z[e], z[e + 1]), r = cap.recip(raw), v = cap.value<WIDE>(raw, r);
       if (slopes) {
         const float2 d = Cap::slope(r);
         slopes[e] = d.x;
@@ -278,6 +300,8 @@ template <int AB>
 using Element = typename std::conditional<AB == 1, __nv_bfloat16, __half>::type;
 
 // ---- host ----
+// 0: scores as they are, 1: capped or with a bias by distance, 2: under a wide cap
+inline int score_form(const ScoreArgs& s) { return s.cap > kWideCap ? 2 : s.cap > 0.0f || s.slopes ? 1 : 0; }
 inline long long round_up(long long v, long long a) { return (v + a - 1) / a * a; }
 
 // Whether TMA can read it in place: every row, head and sample on 16 bytes.

@@ -111,7 +111,7 @@ __device__ __noinline__ float few_keys_delta(const GradArgs& a, int b, int h, in
     const float other = __shfl_xor_sync(0xffffffffu, sum, 4);
     s = value ? other : sum;
     y = value ? sum : other;
-    float z = a.s.cap > 0.0f ? cap.value(cap.recip(s)) : s * a.s.scale * kLog2E;
+    float z = a.s.cap > 0.0f ? cap.value(s, cap.recip(s)) : s * a.s.scale * kLog2E;
     if (a.s.slopes) z = fmaf(-slope, fabsf(static_cast<float>(pos - lo - n - at)), z);
     if (n + at < count) delta = fmaf(exp2_approx(z - lse), y, delta);
   }
@@ -326,7 +326,7 @@ struct StepWalk {
   }
 };
 
-template <int AB, int D, bool RICH>
+template <int AB, int D, bool RICH, bool WIDE>
 __global__ void __launch_bounds__(kGradThreads, 1)
     span_attention_grad_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                                const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap gmap,
@@ -589,7 +589,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         float p[64], slopes[RICH ? 64 : 1];
         load_half(s_own, p);
         if constexpr (RICH) {
-          scaled_scores(a.s, cap, p, slopes);
+          scaled_scores<WIDE>(a.s, cap, p, slopes);
           if (a.s.slopes) {
             const float bias = a.s.slopes[step.head] * kLog2E;
 #pragma unroll
@@ -816,7 +816,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         float p[64], slopes[RICH ? 64 : 1];
         load_half(s_own, p);
         if constexpr (RICH) {
-          scaled_scores(a.s, cap, p, slopes);
+          scaled_scores<WIDE>(a.s, cap, p, slopes);
           if (a.s.slopes) less_distance(bias, static_cast<float>(span.z - j0), p);
         }
 #pragma unroll
@@ -933,11 +933,12 @@ long long stats_bytes(int batch, int heads, int sq) { return 8LL * batch * heads
 
 template <int AB, int D>
 int launch_grad(const GradArgs& a, const CUtensorMap (&maps)[4], cudaStream_t stream) {
-  const bool rich = a.s.cap > 0.0f || a.s.slopes;
-  auto kernel = rich ? span_attention_grad_kernel<AB, D, true> : span_attention_grad_kernel<AB, D, false>;
-  const int smem = rich ? grad_smem<D, true>() : grad_smem<D, false>();
-  static std::atomic<unsigned long long> granted[2] = {};
-  if (cudaError_t e = grant_smem(reinterpret_cast<const void*>(kernel), smem, granted[rich])) return static_cast<int>(e);
+  const int form = score_form(a.s);
+  auto kernel = form == 2 ? span_attention_grad_kernel<AB, D, true, true>
+                : form == 1 ? span_attention_grad_kernel<AB, D, true, false> : span_attention_grad_kernel<AB, D, false, false>;
+  const int smem = form ? grad_smem<D, true>() : grad_smem<D, false>();
+  static std::atomic<unsigned long long> granted[3] = {};
+  if (cudaError_t e = grant_smem(reinterpret_cast<const void*>(kernel), smem, granted[form])) return static_cast<int>(e);
   if (a.s.sq > 0) {
     const long long rows = static_cast<long long>(a.s.batch) * a.s.heads * a.padded;
     auto stats = a.s.spans || a.s.sk <= kFewKeys ? grad_stats_kernel<AB, true> : grad_stats_kernel<AB, false>;
