@@ -329,7 +329,8 @@ int peco_key_spans(const int* q_ends, long long q_stride, const int* k_ends, lon
  * adjacent, rows, heads and samples start on 16 bytes.  span_rows and span_tiles
  * from peco_key_spans (null: every key, pos = i + sk - sq), of one sample for
  * all or, with spans_batched, of each.  heads is a multiple of kv_heads, d of 8 up
- * to 128; dtype 0 fp16, 1 bf16.  Calls of few rows keep parts in the workspace. */
+ * to 128; scale and cap from 1e-30 to 1e30, scale / cap at most 1e30; dtype 0 fp16,
+ * 1 bf16.  Calls of few rows keep parts in the workspace. */
 int peco_span_attention(const void* q, const void* k, const void* v, const long long* strides, const int* span_rows,
                         const int* span_tiles, int spans_batched, const float* slopes, float scale, float cap, void* out,
                         float* lse, int batch, int heads, int kv_heads, int sq, int sk, int d, int dtype, void* workspace,

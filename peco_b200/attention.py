@@ -17,7 +17,6 @@ the current stream.
 from __future__ import annotations
 
 import functools
-import math
 import struct
 from dataclasses import dataclass
 from typing import NamedTuple, Optional
@@ -30,6 +29,7 @@ from . import _native
 _strides = struct.Struct("=12q").pack  # (quicker to make than an array of ctypes)
 _grad_strides = struct.Struct("=24q").pack
 _SIXTEEN_BITS = (torch.float16, torch.bfloat16)
+_LEAST, _MOST = 1e-30, 1e30  # scale and cap reach the kernels in fp32, their quotient too
 
 
 class AttentionGrads(NamedTuple):
@@ -166,13 +166,13 @@ def _check(q, k, v, spans, scale, softcap, slopes):
     if n > 0x7ffffe00 or m > 0x7ffffe00:
         raise ValueError("too many rows")
     scale = d ** -0.5 if scale is None else float(scale)
-    if not (scale > 0 and math.isfinite(scale)):
-        raise ValueError("scale must be positive")
+    if not (_LEAST <= scale <= _MOST):
+        raise ValueError("scale must be positive, from 1e-30 to 1e30")
     cap = 0.0
     if softcap is not None:
         cap = float(softcap)
-        if not (cap > 0 and math.isfinite(cap)):
-            raise ValueError("softcap must be positive")
+        if not (_LEAST <= cap <= _MOST and scale / cap <= _MOST):
+            raise ValueError("softcap must be positive, from 1e-30 to 1e30 (scale / softcap at most 1e30)")
     if slopes is not None:
         if not isinstance(slopes, torch.Tensor) or slopes.dtype is not torch.float32 or slopes.shape != (h,):
             raise ValueError(f"slopes must be a float32 tensor [{h}]")
@@ -284,7 +284,8 @@ def attention(q, k, v, *, spans=None, scale=None, softcap=None, slopes=None, ret
 
     ``spans``: what ``key_spans(B or 1, N, M, ...)`` gives; None: every row sees
     every key, and the last row stands at the last key.  ``scale`` defaults to
-    D^-0.5.  ``softcap``: scores are softcap * tanh(score / softcap).  ``slopes``
+    D^-0.5.  ``softcap``: scores are softcap * tanh(score / softcap); it, ``scale`` and
+    scale / softcap stay inside fp32 (1e-30 to 1e30).  ``slopes``
     float32 [H]: slope * |position - j| is taken from the score of key j (no
     gradient of slopes: such a call is refused).
     ``return_lse``: also the logarithm of each row's sum of exponentials, float32

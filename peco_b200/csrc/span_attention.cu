@@ -765,7 +765,7 @@ extern "C" int peco_span_attention(const void* q, const void* k, const void* v, 
                                    void* stream_ptr) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
   if (dtype != 0 && dtype != 1) return kErrUnsupported;
-  if (!valid_attention(batch, heads, kv_heads, sq, sk, d) || !(scale > 0.0f) || !(cap >= 0.0f) || !strides) return kErrInvalidValue;
+  if (!valid_attention(batch, heads, kv_heads, sq, sk, d) || !valid_scores(scale, cap) || !strides) return kErrInvalidValue;
   if (batch == 0 || sq == 0) return kOk;
   if (!q || !out || !lse || (sk > 0 && (!k || !v)) || (span_rows == nullptr) != (span_tiles == nullptr)) return kErrInvalidValue;
   ForwardArgs a{};

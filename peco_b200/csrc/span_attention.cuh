@@ -300,6 +300,11 @@ template <int AB>
 using Element = typename std::conditional<AB == 1, __nv_bfloat16, __half>::type;
 
 // ---- host ----
+// Scale, cap (0: none) and their quotient stay well inside fp32.
+inline bool valid_scores(float scale, float cap) {
+  auto fits = [](float v) { return v >= 0.99e-30f && v <= 1.01e30f; };
+  return fits(scale) && (cap == 0.0f || (fits(cap) && scale / cap <= 1.01e30f));
+}
 // 0: scores as they are, 1: capped or with a bias by distance, 2: under a wide cap
 inline int score_form(const ScoreArgs& s) { return s.cap > kWideCap ? 2 : s.cap > 0.0f || s.slopes ? 1 : 0; }
 inline long long round_up(long long v, long long a) { return (v + a - 1) / a * a; }

@@ -974,7 +974,7 @@ extern "C" int peco_span_attention_backward(const void* grad, const void* q, con
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
   if (dtype != 0 && dtype != 1) return kErrUnsupported;
   if (batch < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || sq < 0 || sk < 0 || sq > 0x7ffffe00 || sk > 0x7ffffe00 ||
-      d < 8 || d > 128 || d % 8 || !(scale > 0.0f) || !(cap >= 0.0f) || !strides)
+      d < 8 || d > 128 || d % 8 || !valid_scores(scale, cap) || !strides)
     return kErrInvalidValue;
   const bool keys = (dk || dv) && batch > 0 && sk > 0, rows = dq && batch > 0 && sq > 0;
   if (!keys && !rows) return kOk;

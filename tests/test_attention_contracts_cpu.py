@@ -1,8 +1,11 @@
 """What attention refuses whatever else its call asks for."""
 
+import ctypes
+
 import pytest
 import torch
 
+from peco_b200 import _native
 from peco_b200.attention import attention, attention_backward
 
 Q = torch.zeros(2, 4, 6, 64, dtype=torch.bfloat16)
@@ -23,3 +26,24 @@ def test_a_gradient_of_slopes_is_refused(wants):
         attention(q, k, v, slopes=slopes)
     with pytest.raises(RuntimeError, match="CUDA"):
         attention(q, k, v, slopes=slopes.detach())
+
+
+@pytest.mark.parametrize("args", [dict(softcap=1e-50), dict(softcap=1e-31), dict(softcap=1e31), dict(softcap=1e300), dict(scale=1e-46),
+                                  dict(scale=1e39), dict(scale=1e300), dict(scale=1e25, softcap=1e-10)])
+def test_scales_and_caps_past_fp32_are_refused(args):
+    """They would reach the kernels as 0 (a cap of 0 is none), as infinity, or make their quotient infinite."""
+    with pytest.raises(ValueError, match="scale|softcap"):
+        attention(Q, K, K, **args)
+    with pytest.raises(ValueError, match="scale|softcap"):
+        attention_backward(Q, Q, K, K, Q, LSE, **args)
+
+
+@pytest.mark.parametrize("scale,cap", [(float("inf"), 0.0), (1e31, 0.0), (1e-31, 0.0), (1.0, float("inf")), (1.0, 1e31), (1.0, 1e-31),
+                                       (1.0, float("nan")), (1e20, 1e-20)])
+def test_entries_refuse_scales_and_caps_out_of_range(scale, cap):
+    lib = _native.load()
+    at = 0x10000  # never read: every call is refused
+    strides = (ctypes.c_longlong * 24)(*[4 * 6 * 64, 6 * 64, 64] * 8)
+    assert lib.peco_span_attention(at, at, at, strides, 0, 0, 0, 0, scale, cap, at, at, 2, 4, 2, 6, 9, 64, 1, 0, 0, 0) == 1
+    assert lib.peco_span_attention_backward(at, at, at, at, at, at, strides, 0, 0, 0, 0, scale, cap, at, at, at, 2, 4, 2, 6, 9, 64, 1,
+                                            at, 1 << 20, 0) == 1
