@@ -15,6 +15,7 @@ CUDA tensors only; work is enqueued on the current stream.
 
 from __future__ import annotations
 
+import weakref
 from typing import NamedTuple
 
 import torch
@@ -200,20 +201,38 @@ def _off_16_bytes(pointers: int, strides: int) -> bool:
 
 
 class LayerInt8(NamedTuple):
-    """A layer's weight in 8-bit integers, and the parameter it was taken from."""
+    """A layer's weight in 8-bit integers, the parameter it was taken from, its storage, and its address and version then."""
 
     weight: QuantizedRows
     source: torch.Tensor
-    version: int
+    place: object  # weak reference to the parameter's storage (whose address may be another's later); None: stale
+    state: tuple
+
+    def fresh(self) -> bool:
+        return self.place is not None and self.place() is self.source.untyped_storage() and \
+            self.state == _state(self.source)
+
+    def __reduce__(self):  # a copied or stored layer's weight lies elsewhere and counts its versions anew
+        return _layer_int8, (self.weight, self.source, self.fresh())
+
+
+def _state(weight):
+    return weight.data_ptr(), None if weight.is_inference() else weight._version  # (tensors of inference mode have none)
+
+
+def _layer_int8(weight, source, fresh=True):
+    return LayerInt8(weight, source, weakref.ref(source.untyped_storage()) if fresh else None, _state(source))
 
 
 @torch.no_grad()
 def quantize_layer(layer) -> bool:
     """Keep ``layer``'s weight in 8-bit integers beside it (``layer.int8``), where it is a plain linear layer on a CUDA
-    device in 16 bits; whether it is.  The 16-bit weight stays the layer's parameter."""
+    device in 16 bits; whether it is.  The 16-bit weight stays the layer's parameter.  A layer whose weight is changed,
+    replaced or moved afterwards raises until it is quantised again.  Values written in place through ``weight.data`` (as
+    some ways of merging adapters do) leave no trace: quantise again after them."""
     if not is_plain_linear(layer) or layer.weight.dtype not in _SIXTEEN_BITS or not layer.weight.is_cuda:
         return False
-    layer.int8 = LayerInt8(quantize_rows(layer.weight), layer.weight, layer.weight._version)
+    layer.int8 = _layer_int8(quantize_rows(layer.weight), layer.weight)
     return True
 
 
@@ -222,6 +241,6 @@ def int8_weight(layer):
     kept = getattr(layer, "int8", None)
     if not isinstance(kept, LayerInt8) or not is_plain_linear(layer):
         return None
-    if kept.source is not layer.weight or kept.version != layer.weight._version:
-        raise RuntimeError("the layer's weight changed after it was quantised; quantise it again")
+    if kept.source is not layer.weight or not kept.fresh():
+        raise RuntimeError("the layer's weight changed or moved after it was quantised; quantise it again")
     return kept.weight
