@@ -26,6 +26,8 @@ from __future__ import annotations
 
 import torch
 
+from .int8 import int8_weight
+
 
 class PecoCallGraph:
     """Capture ``processor.attention(query, key, value)`` and replay it.
@@ -94,7 +96,9 @@ class PecoStepGraph:
     eagerly); every processor's centroids become fixed tensors that each
     replay reads as the k-means init and overwrites, so replays chain like
     eager steps.  ``inputs`` are the forward's positional arguments (CUDA
-    tensors); a replay copies new values into the captured ones.
+    tensors); a replay copies new values into the captured ones.  Layers in
+    8-bit integers are replayed as captured: a call after their weights changed
+    raises.
     """
 
     def __init__(self, model, *inputs):
@@ -111,8 +115,8 @@ class PecoStepGraph:
             p.update_centroids_in_place = True
         # what the graph reads and writes and did not allocate itself lives as long as the graph, whatever the
         # processors and the model take afterwards (another capture, a reset, another token grid, 16-bit layers again)
-        self.kept = ([(p.q_centroids, p.k_centroids) for p in processors], getattr(model, "_rope", None),
-                     [m.int8 for m in getattr(model, "modules", tuple)() if hasattr(m, "int8")])
+        self.kept = ([(p.q_centroids, p.k_centroids) for p in processors], getattr(model, "_rope", None))
+        self.int8 = [(m, m.int8) for m in getattr(model, "modules", tuple)() if int8_weight(m) is not None]
         self.model = model
         self.frozen = (ctx.step, ctx.text_length, ctx.valid_text_length)
         self.inputs = tuple(t.detach().clone() if torch.is_tensor(t) else t for t in inputs)
@@ -129,6 +133,9 @@ class PecoStepGraph:
                 _register_context_hook(model, ctx)
 
     def __call__(self, *inputs):
+        for layer, kept in self.int8:
+            if layer.weight is not kept.source or not kept.fresh():
+                raise RuntimeError("a layer's weight changed after the capture, which replays over its 8-bit form; capture again")
         for dst, src in zip(self.inputs, inputs):
             if torch.is_tensor(dst) and src.data_ptr() != dst.data_ptr():
                 dst.copy_(src)
