@@ -48,7 +48,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .attention import attention, key_spans
-from .int8 import int8_weight, linear_int8, quantize_layer
+from .int8 import LayerInt8, int8_weight, linear_int8, quantize_layer
 from .linear import is_plain_linear, linear_act, without_hooks
 from .norms import modulated_norm
 from .processor import InferenceContext, PecoAttention, PecoConfig, _project
@@ -531,7 +531,7 @@ def use_block_operators(transformer, enabled=True, positions=False, int8=False):
         block.block_operators = enabled
         block.attn.block_operators = enabled
         for layer in block.modules():
-            if "int8" in vars(layer):
+            if isinstance(vars(layer).get("int8"), LayerInt8):
                 del layer.int8
         if enabled and int8:
             for layer in _block_linears(block):

@@ -230,7 +230,8 @@ def quantize_layer(layer) -> bool:
     device in 16 bits; whether it is.  The 16-bit weight stays the layer's parameter.  A layer whose weight is changed,
     replaced or moved afterwards raises until it is quantised again.  Values written in place through ``weight.data`` (as
     some ways of merging adapters do) leave no trace: quantise again after them."""
-    if not is_plain_linear(layer) or layer.weight.dtype not in _SIXTEEN_BITS or not layer.weight.is_cuda:
+    if not is_plain_linear(layer) or layer.weight.dtype not in _SIXTEEN_BITS or not layer.weight.is_cuda or \
+            not isinstance(getattr(layer, "int8", None), (LayerInt8, type(None))):  # (an attribute of somebody else's)
         return False
     layer.int8 = _layer_int8(quantize_rows(layer.weight), layer.weight)
     return True

@@ -71,3 +71,16 @@ def test_a_graph_outlives_the_8_bit_form(no_capture):
     graph = PecoStepGraph(model, torch.zeros(3))
     del model.layer.int8  # 16 bits again: the weights are the same
     assert (graph(torch.zeros(3)) == 1).all()
+
+
+def test_an_attribute_of_that_name_stays():
+    """use_block_operators drops what it keeps with layers, not what others keep there under the same name."""
+    model = build_transformer(HunyuanConfig(hidden=32, heads=2, head_dim=16, dual_blocks=1, single_blocks=1, text_dim=8, pooled_dim=8),
+                              device="cpu", dtype=torch.bfloat16)
+    block = model.transformer_blocks[0]
+    block.attn.to_q.int8 = block.ff[0].int8 = True
+    keep(block.attn.to_k)
+    for args in ({}, dict(enabled=False), dict(int8=True)):
+        use_block_operators(model, **args)
+        assert block.attn.to_q.int8 is True and block.ff[0].int8 is True
+        assert "int8" not in vars(block.attn.to_k)
