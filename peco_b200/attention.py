@@ -291,6 +291,9 @@ def attention(q, k, v, *, spans=None, scale=None, softcap=None, slopes=None, ret
     ``return_lse``: also the logarithm of each row's sum of exponentials, float32
     [B, H, N] (no gradient flows through it), -inf where a row sees nothing.
 
+    Scores are fp32 with its rounding, 2^-23 of their size, which is the relative
+    error of a probability.  Past 2^26 (uncapped) a row may be infinite or NaN.
+
     D is a multiple of 8 up to 128.  Strides are free where D is adjacent and
     rows, heads and samples start on 16 bytes; other layouts are copied first.
     The result has the layout of q.  Keys and values that a row's mask leaves
@@ -311,7 +314,8 @@ def attention_backward(grad, q, k, v, out, lse, *, spans=None, scale=None, softc
     ``needs``: names of the gradients to compute (default: q, k and v).  The
     probabilities and their gradients are rounded to the operands' type for the
     products (in float16 to that type's range too: scale the loss for it); sums
-    run in a fixed order.  Rows that see no key, and keys that no row sees, get
+    run in a fixed order.  Probabilities come from ``lse``, whose rounding is 2^-23 of
+    its size: scores past some 2^16 leave little of them.  Rows that see no key, and keys that no row sees, get
     zeros and may hold anything; a NaN in a row or key that is seen reaches
     the gradients of its tile.
     """
