@@ -185,7 +185,8 @@ def _check(q, k, v, spans, scale, softcap, slopes):
         samples = spans.rows.shape[0]
         if spans.rows.shape != (samples, n, 4) or spans.tiles.shape != (samples, -(-n // 128), 4) or \
                 spans.rows.dtype is not torch.int32 or spans.tiles.dtype is not torch.int32 or \
-                not spans.rows.is_contiguous() or not spans.tiles.is_contiguous():
+                not spans.rows.is_contiguous() or not spans.tiles.is_contiguous() or \
+                (spans.rows.data_ptr() | spans.tiles.data_ptr()) & 15:
             raise ValueError("spans must be as key_spans lays them out")
     return (b, h, kv, n, m, d), scale, cap
 

@@ -767,7 +767,7 @@ extern "C" int peco_span_attention(const void* q, const void* k, const void* v, 
   if (dtype != 0 && dtype != 1) return kErrUnsupported;
   if (!valid_attention(batch, heads, kv_heads, sq, sk, d) || !valid_scores(scale, cap) || !strides) return kErrInvalidValue;
   if (batch == 0 || sq == 0) return kOk;
-  if (!q || !out || !lse || (sk > 0 && (!k || !v)) || (span_rows == nullptr) != (span_tiles == nullptr)) return kErrInvalidValue;
+  if (!q || !out || !lse || (sk > 0 && (!k || !v)) || !valid_plan(span_rows, span_tiles)) return kErrInvalidValue;
   ForwardArgs a{};
   a.q = HeadRows{q, strides[0], strides[1], strides[2]};
   a.k = HeadRows{k, strides[3], strides[4], strides[5]};

@@ -309,6 +309,11 @@ inline bool valid_scores(float scale, float cap) {
 inline int score_form(const ScoreArgs& s) { return s.cap > kWideCap ? 2 : s.cap > 0.0f || s.slopes ? 1 : 0; }
 inline long long round_up(long long v, long long a) { return (v + a - 1) / a * a; }
 
+// Rows and tiles of a plan, both or neither; read 16 bytes at a time.
+inline bool valid_plan(const int* rows, const int* tiles) {
+  return (rows == nullptr) == (tiles == nullptr) && ((reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(tiles)) & 15) == 0;
+}
+
 // Whether TMA can read it in place: every row, head and sample on 16 bytes.
 inline bool readable(const HeadRows& t, int batch, int heads, int rows) {
   auto fits = [](long long stride, int n) { return n <= 1 || (stride > 0 && (stride & 7) == 0 && stride < (1LL << 38)); };

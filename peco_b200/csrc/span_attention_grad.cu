@@ -978,7 +978,7 @@ extern "C" int peco_span_attention_backward(const void* grad, const void* q, con
     return kErrInvalidValue;
   const bool keys = (dk || dv) && batch > 0 && sk > 0, rows = dq && batch > 0 && sq > 0;
   if (!keys && !rows) return kOk;
-  if ((span_rows == nullptr) != (span_tiles == nullptr)) return kErrInvalidValue;
+  if (!valid_plan(span_rows, span_tiles)) return kErrInvalidValue;
   HeadRows t[8];  // grad, q, k, v, out, dq, dk, dv
   const void* at[8] = {grad, q, k, v, out, dq, dk, dv};
   for (int i = 0; i < 8; ++i) {

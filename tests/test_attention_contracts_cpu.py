@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from peco_b200 import _native
-from peco_b200.attention import attention, attention_backward
+from peco_b200.attention import KeySpans, attention, attention_backward
 
 Q = torch.zeros(2, 4, 6, 64, dtype=torch.bfloat16)
 K = torch.zeros(2, 2, 9, 64, dtype=torch.bfloat16)
@@ -47,3 +47,29 @@ def test_entries_refuse_scales_and_caps_out_of_range(scale, cap):
     assert lib.peco_span_attention(at, at, at, strides, 0, 0, 0, 0, scale, cap, at, at, 2, 4, 2, 6, 9, 64, 1, 0, 0, 0) == 1
     assert lib.peco_span_attention_backward(at, at, at, at, at, at, strides, 0, 0, 0, 0, scale, cap, at, at, at, 2, 4, 2, 6, 9, 64, 1,
                                             at, 1 << 20, 0) == 1
+
+
+def off_16_bytes(t):
+    return torch.cat((t.new_zeros(1), t.flatten()))[1:].view(t.shape)
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_plans_off_16_bytes_are_refused(which):
+    """The kernels read them 16 bytes at a time: a misaligned address would be a fault."""
+    rows, tiles = torch.zeros(2, 6, 4, dtype=torch.int32), torch.zeros(2, 1, 4, dtype=torch.int32)
+    rows, tiles = (off_16_bytes(t) if i == which else t for i, t in enumerate((rows, tiles)))
+    spans = KeySpans(rows, tiles, 6, 9)
+    with pytest.raises(ValueError, match="spans"):
+        attention(Q, K, K, spans=spans)
+    with pytest.raises(ValueError, match="spans"):
+        attention_backward(Q, Q, K, K, Q, LSE, spans=spans)
+
+
+@pytest.mark.parametrize("rows,tiles", [(4, 0), (8, 0), (0, 4), (0, 12)])
+def test_entries_refuse_plans_off_16_bytes(rows, tiles):
+    lib = _native.load()
+    at = 0x10000  # never read: every call is refused
+    strides = (ctypes.c_longlong * 24)(*[4 * 6 * 64, 6 * 64, 64] * 8)
+    assert lib.peco_span_attention(at, at, at, strides, at + rows, at + tiles, 1, 0, 1.0, 0.0, at, at, 2, 4, 2, 6, 9, 64, 1, 0, 0, 0) == 1
+    assert lib.peco_span_attention_backward(at, at, at, at, at, at, strides, at + rows, at + tiles, 1, 0, 1.0, 0.0, at, at, at, 2, 4, 2,
+                                            6, 9, 64, 1, at, 1 << 20, 0) == 1
