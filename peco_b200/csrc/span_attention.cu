@@ -236,7 +236,7 @@ __device__ __noinline__ void masked_row(const ForwardArgs& a, int b, int head, i
 #pragma unroll
   for (int e = 0; e < D / 32; ++e) acc[e] = 0.0f;
   lo = max(lo, from);
-  hi = min(hi, to);
+  hi = min(hi, min(to, a.s.sk));  // (``to`` is a whole tile's end)
   for (int j0 = lo; j0 < hi; j0 += 32) {
     const int j = j0 + lane;
     float p = 0.0f;
