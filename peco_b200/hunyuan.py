@@ -223,8 +223,10 @@ class SpanProcessor(SDPAProcessor):
         return attention(query, key, value, spans=key_spans(b, s, s, documents=ends))
 
     def __call__(self, attn, hidden_states, encoder_hidden_states=None, attention_mask=None, image_rotary_emb=None):
-        if not torch.is_grad_enabled() and hidden_states.shape[0] == 1 and hidden_states.dtype == torch.bfloat16:
-            # inference of one prompt: the fused stage between projections and attention
+        width = getattr(attn.to_q, "out_features", None)
+        if not torch.is_grad_enabled() and hidden_states.shape[0] == 1 and hidden_states.dtype == torch.bfloat16 and \
+                (width is None or width // attn.heads in (64, 128)):
+            # inference of one prompt: the fused stage between projections and attention, for the dims it takes
             return PecoAttention.__call__(self, attn, hidden_states, encoder_hidden_states, attention_mask, image_rotary_emb)
         project = _project if getattr(attn, "block_operators", False) else (lambda layer, x: layer(x))
         return self._torch_call(attn, hidden_states, encoder_hidden_states, image_rotary_emb, project)
