@@ -182,7 +182,7 @@ class SDPAProcessor(PecoAttention):
 
         def heads_of(x, layers, norms):
             q, k, v = (project(layer, x).unflatten(-1, (attn.heads, -1)).transpose(1, 2) for layer in layers)
-            return norms[0](q), norms[1](k), v
+            return *(x if norm is None else norm(x) for norm, x in zip(norms, (q, k))), v
 
         q, k, v = heads_of(video, (attn.to_q, attn.to_k, attn.to_v), (attn.norm_q, attn.norm_k))
         if isinstance(rope, AxialPositions):
@@ -198,10 +198,10 @@ class SDPAProcessor(PecoAttention):
         video_out, text_out = rows[:, : video.shape[1]], rows[:, video.shape[1]:]
         if not n_text:
             return video_out, text
-        if attn.to_out is not None:
+        if getattr(attn, "to_out", None) is not None:
             for layer in attn.to_out:
                 video_out = project(layer, video_out)
-        if attn.to_add_out is not None:
+        if getattr(attn, "to_add_out", None) is not None:
             text_out = project(attn.to_add_out, text_out)
         return video_out, text_out
 

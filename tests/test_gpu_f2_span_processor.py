@@ -6,6 +6,7 @@ Paths differ in where they round (2^-9 a step): cosine >= 0.9995 against each ot
 import pytest
 import torch
 import torch.nn as nn
+import torch.nn as nn
 
 from peco_b200 import _native
 from peco_b200.hunyuan import HunyuanConfig, build_transformer, use_block_operators, use_dense_attention
@@ -38,3 +39,35 @@ def test_head_dimensions(axes, operators):
         one, two = model(*prompts(cfg, 1)), model(*prompts(cfg, 2))
     assert one.isfinite().all() and close(one, two[:1]) and close(one, two[1:])
     assert _native.device_status(clear=True) == 0
+
+
+def test_modules_without_norms():
+    cfg = HunyuanConfig(hidden=128, heads=2, head_dim=64, dual_blocks=1, single_blocks=1, text_dim=64, pooled_dim=32,
+                        rope_axes=(16, 24, 24))
+    model = build_transformer(cfg, device="cuda", dtype=torch.bfloat16)
+    for block in [*model.transformer_blocks, *model.single_transformer_blocks]:
+        for name in ("norm_q", "norm_k", "norm_added_q", "norm_added_k"):
+            setattr(block.attn, name, None)
+    use_dense_attention(model, InferenceContext(step=0, text_length=16, valid_text_length=12), spans=True)
+    with torch.no_grad():
+        one, two = model(*prompts(cfg, 1)), model(*prompts(cfg, 2))
+    assert one.isfinite().all() and close(one, two[:1]) and close(one, two[1:])
+
+
+@pytest.mark.parametrize("batch", [1, 2])
+def test_modules_without_output_layers(batch):
+    """As single-stream modules of other libraries: no such attributes at all."""
+    class Single(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.heads = 2
+            self.to_q, self.to_k, self.to_v = (nn.Linear(128, 128) for _ in range(3))
+            self.norm_q = self.norm_k = self.add_q_proj = None
+
+    from peco_b200.hunyuan import SpanProcessor
+    module = Single().to("cuda", torch.bfloat16)
+    call = SpanProcessor(InferenceContext(step=0, text_length=16, valid_text_length=12))
+    x, text = (torch.randn(1, n, 128, device="cuda").bfloat16().repeat(batch, 1, 1) for n in (40, 16))
+    with torch.no_grad():
+        video, words = call(module, x, text)
+    assert video.shape == x.shape and words.shape == text.shape and video.isfinite().all()
