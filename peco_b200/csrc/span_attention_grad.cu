@@ -743,12 +743,27 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         const uint32_t at = uniform(tmem);
         const uint32_t q = uniform(desc_dims(smem_u32(base))), k = uniform(desc_dims(smem_u32(firsts)));
         const int last = static_cast<int>(uniform(ntiles)) - 1;
-        // spans that share a key or meet (the largest first key is not behind the least last) leave none out between them
-        const bool gaps = seen.z > seen.w;
+        // Spans that share a key or meet leave none out between them: all of them (the
+        // largest first key is not behind the least last), or every row's and the next one's
+        // (packed documents, windows: 15 keys a row, 24 heads x 16000 rows 584 and 554 us).
+        bool gaps = seen.z > seen.w;
         int4 spans[kTile / 32];
+        if (gaps) {
 #pragma unroll
-        for (int i = 0; i < kTile / 32; ++i)
-          spans[i] = gaps && i0 + i * 32 + lane < a.s.sq ? span_of(a.s, b, i0 + i * 32 + lane) : make_int4(0, 0, 0, 0);
+          for (int i = 0; i < kTile / 32; ++i)
+            spans[i] = i0 + i * 32 + lane < a.s.sq ? span_of(a.s, b, i0 + i * 32 + lane) : make_int4(0, 0, 0, 0);
+          bool meet = true;
+#pragma unroll
+          for (int i = 0; i < kTile / 32; ++i) {
+            const int after = min(i + 1, kTile / 32 - 1);  // (the tile's last row has no next)
+            const int lo = __shfl_sync(0xffffffffu, lane == 0 ? spans[after].x : spans[i].x, lane + 1);
+            const int hi = __shfl_sync(0xffffffffu, lane == 0 ? spans[after].y : spans[i].y, lane + 1);
+            const int row = i * 32 + lane + 1;
+            if (row < kTile && i0 + row < a.s.sq)
+              meet = meet && spans[i].x < spans[i].y && lo < hi && lo <= spans[i].y && spans[i].x <= hi;
+          }
+          gaps = !__all_sync(0xffffffffu, meet);
+        }
         RingPos f{0, 0};
         me.wait(&sh.own_full, 0);
         for (int t = 0; t <= last && me.ok; ++t) {
