@@ -327,7 +327,7 @@ int peco_key_spans(const int* q_ends, long long q_stride, const int* k_ends, lon
  * heads, sq] its logarithmic sum (a row without keys: 0 and -inf).  strides (host
  * memory): batch, head and row strides of q, k, v and out in elements; d is
  * adjacent, rows, heads and samples start on 16 bytes.  span_rows and span_tiles
- * from peco_key_spans (null: every key, pos = i + sk - sq), of one sample for
+ * from peco_key_spans, on 16 bytes (null: every key, pos = i + sk - sq), of one sample for
  * all or, with spans_batched, of each.  heads is a multiple of kv_heads, d of 8 up
  * to 128; scale and cap from 1e-30 to 1e30, scale / cap at most 1e30; dtype 0 fp16,
  * 1 bf16.  Calls of few rows keep parts in the workspace. */
@@ -342,7 +342,8 @@ long long peco_span_attention_workspace(int batch, int heads, int kv_heads, int 
  * there are any.  strides (host memory): batch, head
  * and row strides of grad, q, k, v, out, dq, dk and dv.  Sums run in a fixed
  * order; the probabilities and their gradients are rounded to the operands'
- * type for the products. */
+ * type for the products.  A row of one key has no gradient of its score; keys
+ * that no row sees, and rows that see none, get zeros whatever they hold. */
 int peco_span_attention_backward(const void* grad, const void* q, const void* k, const void* v, const void* out,
                                  const float* lse, const long long* strides, const int* span_rows, const int* span_tiles,
                                  int spans_batched, const float* slopes, float scale, float cap, void* dq, void* dk,

@@ -315,7 +315,9 @@ def attention_backward(grad, q, k, v, out, lse, *, spans=None, scale=None, softc
     ``needs``: names of the gradients to compute (default: q, k and v).  The
     probabilities and their gradients are rounded to the operands' type for the
     products (in float16 to that type's range too: scale the loss for it); sums
-    run in a fixed order.  Probabilities come from ``lse``, whose rounding is 2^-23 of
+    run in a fixed order.  A row that sees one key has no gradient of its score (q's and
+    k's are exact zeros); rows of up to eight keys take grad.out from their probabilities,
+    others from ``out`` as it is rounded.  Probabilities come from ``lse``, whose rounding is 2^-23 of
     its size: scores past some 2^16 leave little of them.  Rows that see no key, and keys that no row sees, get
     zeros and may hold anything; a NaN in a row or key that is seen reaches
     the gradients of its tile.

@@ -46,7 +46,7 @@ __device__ __forceinline__ RowScale row_scale_of(uint32_t top) {
 // round(127 x / max) of a pair, ties to even, each as the low byte of a word.
 // x inv is within 2^-23 of 127 x / max, relatively.  Where that quotient is not half
 // an odd number it is 2^-19 away from it (relatively: x and max have at most 11
-// significant bits), so rounding to 20 bits, 2^-21 at most, keeps it on its side
+// significant bits), so rounding to 20 bits, 2^-20 at most, keeps it on its side
 // and puts the quotients that are half an odd number exactly there: the integers
 // are those of the exact quotient.  Adding 1.5 * 2^23 rounds to even.
 __device__ __forceinline__ uint2 round_pair(float2 x, float2 inv) {

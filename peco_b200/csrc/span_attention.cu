@@ -25,7 +25,9 @@
 // causal, 24 query heads on 4, 4096 rows 116 us; one row of 24 heads on 4, four samples of
 // up to 16384 keys 32 us.  Tensor core and special-function unit are both 62% busy:
 // the two warps of a scheduler do not hide all of each other's maxima, TMEM loads
-// and hand-offs.  Before, with a maximum, sum and accumulator for each warpgroup
+// and hand-offs, and the 128 scores of a thread leave some registers in local memory
+// (16 loads and 7 stores a warp and tile, 3% of its instructions).  Capped 1010 us, under
+// a cap above 64 1150 us, by distance 830 us.  Before, with a maximum, sum and accumulator for each warpgroup
 // 563 us, and with one warp that issued all products 536 us; two tiles of rows a
 // CTA in place of two of keys, which halves the traffic from L2, took as long on full
 // masks and more on others (clips packed in causal order 102 us against 89).
@@ -153,7 +155,7 @@ __global__ void __launch_bounds__(kTile) key_spans_kernel(const SpanArgs a) {
 // ---- forward ----------------------------------------------------------------------------
 constexpr int kSlots = 3;        // tiles of K, and as many of V
 constexpr int kScores = 3;       // S buffers
-constexpr int kThreads = 384;    // two softmax warpgroups, one with the TMA warp and the MMA warp
+constexpr int kThreads = 384;    // two softmax warpgroups, one with the TMA warp and the two MMA warps
 // A softmax thread holds a tile's 128 scores: the launch's 168 registers a thread
 // go 208 to 208 to 88 (256 * 208 + 128 * 88 = 384 * 168).
 constexpr uint32_t kTmemCols = 512;  // three tiles' S, then O

@@ -3,6 +3,7 @@
 // and s' = dz/d(scale q.k), 1 or 1 - tanh^2:
 //   ds_ij = p_ij (g_i.v_j - delta_i) s'_ij
 //   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij g_i
+// A row that sees one key has ds 0; rows of few keys take delta_i = sum_j p_ij (g_i.v_j).
 //
 // One launch holds two kinds of CTAs.  Those of 128 keys walk the query tiles (of
 // all the heads that share the keys) and keep dk and dv in TMEM; those of 128
@@ -10,16 +11,16 @@
 // seven products instead of five; in exchange no sum crosses a CTA: there are no
 // atomics, no fp32 copy of dq in memory, and results do not depend on the launch.
 //
-// What it measured (B200, bf16): 24 heads x 7006 rows x 128 dims, every key: 1615 us (0.90
-// PFLOP/s of five products, 1.25 of the seven; 1.8 ms at the power limit after 300
-// calls in a row), of it the CTAs of keys 990, those of rows 660; tensor pipe 65%. In the
+// What it measured (B200, bf16): 24 heads x 7006 rows x 128 dims, every key: 1580 us (0.92
+// PFLOP/s of five products, 1.28 of the seven; 1.8 ms at the power limit after 300
+// calls in a row), the CTAs of keys alone 950, those of rows 655; tensor pipe 64%. In the
 // CTAs of keys every product waits for the one whose operand it overwrites, and so
 // for the softmax between; issuing S right behind dv's product (1640 us), or the two
 // chains by a warp each (1680 us), was slower, although both wait less.
-// Capped scores 2780 us (two more special functions a pair: 1580 us of that unit in all),
-// a bias by distance 2100 us; their slopes go into p before g.v is read (after it, which
+// Capped scores 2660 us (two more special functions a pair: 1580 us of that unit in all),
+// under a cap above 64 2960 us, a bias by distance 2120 us; their slopes go into p before g.v is read (after it, which
 // held three rows of registers at once: 4090 and 2790 us).
-// Under two documents 1600 us: a warp reads each step's statistics and spans while the
+// Under two documents 1570 us: a warp reads each step's statistics and spans while the
 // place for them is still in use (read after it was free: 1890 us).
 #include "span_attention.cuh"
 #include "../../include/peco_b200.h"
