@@ -286,9 +286,9 @@ def attention(q, k, v, *, spans=None, scale=None, softcap=None, slopes=None, ret
     ``spans``: what ``key_spans(B or 1, N, M, ...)`` gives; None: every row sees
     every key, and the last row stands at the last key.  ``scale`` defaults to
     D^-0.5.  ``softcap``: scores are softcap * tanh(score / softcap); it, ``scale`` and
-    scale / softcap stay inside fp32 (1e-30 to 1e30).  ``slopes``
-    float32 [H]: slope * |position - j| is taken from the score of key j (no
-    gradient of slopes: such a call is refused).
+    scale / softcap stay inside fp32 (1e-30 to 1e30).  ``slopes`` float32 [H]:
+    slope * |position - j| is taken from the score of key j (no gradient of
+    slopes: such a call is refused).
     ``return_lse``: also the logarithm of each row's sum of exponentials, float32
     [B, H, N] (no gradient flows through it), -inf where a row sees nothing.
 
@@ -315,10 +315,11 @@ def attention_backward(grad, q, k, v, out, lse, *, spans=None, scale=None, softc
     ``needs``: names of the gradients to compute (default: q, k and v).  The
     probabilities and their gradients are rounded to the operands' type for the
     products (in float16 to that type's range too: scale the loss for it); sums
-    run in a fixed order.  A row that sees one key has no gradient of its score (q's and
-    k's are exact zeros); rows of up to eight keys take grad.out from their probabilities,
-    others from ``out`` as it is rounded.  Probabilities come from ``lse``, whose rounding is 2^-23 of
-    its size: scores past some 2^16 leave little of them.  Rows that see no key, and keys that no row sees, get
+    run in a fixed order.  A row that sees one key has no gradient of its score
+    (q's and k's are exact zeros); rows of up to eight keys take grad.out from
+    their probabilities, others from ``out`` as it is rounded.  Probabilities
+    come from ``lse``, whose rounding is 2^-23 of its size: scores past some 2^16
+    leave little of them.  Rows that see no key, and keys that no row sees, get
     zeros and may hold anything; a NaN in a row or key that is seen reaches
     the gradients of its tile.
     """
